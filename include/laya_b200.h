@@ -35,6 +35,7 @@ extern "C" {
 #define LAYA_DTYPE_F32 0
 #define LAYA_DTYPE_F16 1
 #define LAYA_DTYPE_BF16 2
+#define LAYA_DTYPE_MX8 3         /* E4M3 values with a power-of-two scale per 32 (laya_op_mx8_*) */
 
 #define LAYA_PRECISION_BF16 0  /* 16-bit GEMM/attention operands: bfloat16 (fp32 accumulate) */
 #define LAYA_PRECISION_F16 1   /* 16-bit operands: float16, as the reference (runtime.py:157-158) */
@@ -283,6 +284,71 @@ int laya_op_norm(int precision, float* residual, const float* partials, int spli
 #define LAYA_STATIC_SCRATCH_FLOATS (4 * 1024 * 1024)
 int laya_op_gemm_residual_static(int precision, const void* x, const void* w, int M, int N, int K, int splits,
                                  float* residual, const float* bias, int* err, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * 8-bit linear layers (no counterpart in the reference): matrices in MX8, the norm that writes
+ * them and the product that reads and writes them.
+ *
+ * An MX8 matrix [rows][cols] is two device buffers, both 16-byte aligned:
+ *   values  E4M3, [rows][ld] bytes, ld a multiple of 16 of at least cols; columns from cols to the
+ *           next multiple of 16 are written as zeros and never read into a result
+ *   scales  E8M0 bytes (2^(byte - 127), 255 is NaN), laya_mx8_scale_bytes(rows, cols) of them: tiles
+ *           of 128 rows x 4 blocks of 32 columns, 512 bytes each, tile (row / 128, block / 4)
+ *           row-major; in a tile, (row, block) is byte (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4
+ * A block of 32 consecutive values of a row has the scale 2^e with e = floor(log2 a) - 8, plus one
+ * where a / 2^floor(log2 a) > 1.75, a the block's largest magnitude (e at least -127): the
+ * smallest power of two under which no value passes 448.  Values are rounded to nearest even.  A
+ * block that holds an infinity or a NaN reads back as NaN.  Scales of blocks past the last column
+ * are written as 0 up to the tile's end; those of rows past the last are not written.
+ *
+ * dtype: LAYA_DTYPE_F32, _F16 or _BF16.  Row strides (ld*) count elements; rows are contiguous and
+ * may have any alignment their type allows (16-byte aligned rows run faster).  rows may be 0
+ * (nothing is done).  Buffers belong to the current device, and so must `stream`
+ * (LAYA_ERR_INVALID otherwise).  The calls allocate nothing and wait for nothing.
+ * ------------------------------------------------------------------------------------------ */
+#define LAYA_ACT_NONE 0
+#define LAYA_ACT_RELU 1
+#define LAYA_ACT_GELU 2  /* exact (erf) */
+#define LAYA_ACT_SILU 3
+
+/* Bytes of the scales of an MX8 matrix; -1 for a bad shape (rows >= 0, cols >= 1). */
+int64_t laya_mx8_scale_bytes(int rows, int cols);
+
+/* x [rows][cols] -> MX8. */
+int laya_op_mx8_quantize(int dtype, const void* x, int64_t ldx, int rows, int cols, void* values, int64_t ldv,
+                         void* scales, void* stream);
+
+/* MX8 -> out [rows][cols], value times scale rounded once to dtype (exact in F32 and BF16 unless it
+ * leaves their range). */
+int laya_op_mx8_dequantize(const void* values, int64_t ldv, const void* scales, int rows, int cols, int dtype, void* out,
+                           int64_t ldo, void* stream);
+
+/* h = x + residual; sum_out = h rounded to residual_dtype; y = h / sqrt(mean(h^2) + eps) * weight
+ * (from the unrounded h, in fp32), written as MX8.  residual and sum_out may be NULL, and sum_out
+ * may be the residual itself.  weight: fp32 [cols], 16-byte aligned. */
+int laya_op_rms_norm_mx8(int dtype, const void* x, int64_t ldx, int residual_dtype, const void* residual, int64_t ldr,
+                         void* sum_out, int64_t lds, const float* weight, float eps, int rows, int cols, void* values,
+                         int64_t ldv, void* scales, void* stream);
+
+/* Arguments of laya_op_mx8_linear. */
+typedef struct laya_mx8_linear {
+  int32_t rows, features, cols;  /* x [rows][cols], w and gate [features][cols] */
+  int32_t activation;            /* LAYA_ACT_* */
+  const void* x; const void* x_scales; int64_t ldx;
+  const void* w; const void* w_scales; int64_t ldw;
+  const void* gate; const void* gate_scales; int64_t ldg;  /* NULL: not gated */
+  const float* bias;             /* fp32 [features], 16-byte aligned, or NULL */
+  const float* gate_bias;        /* fp32 [features], 16-byte aligned, or NULL */
+  const void* residual; int64_t ldr;  /* [rows][features] of residual_dtype, or NULL; may be out itself */
+  void* out; void* out_scales; int64_t ldo;  /* [rows][features] of out_dtype; out_scales: MX8 only */
+  int32_t residual_dtype;
+  int32_t out_dtype;             /* LAYA_DTYPE_F32, _F16, _BF16 or _MX8 */
+} laya_mx8_linear;
+
+/* out = act(x w^T + bias) + residual, or, gated, act(x gate^T + gate_bias) * (x w^T + bias) +
+ * residual.  Sums in fp32, rounded once to out_dtype.  err (zero on entry, or NULL) receives a
+ * device error: a pipeline wait that ran out. */
+int laya_op_mx8_linear(const laya_mx8_linear* args, int* err, void* stream);
 
 #ifdef __cplusplus
 }

@@ -35,6 +35,7 @@
 #include <vector>
 
 #include "../../include/laya_b200.h"
+#include "host.cuh"
 #include "gemm.cuh"
 #include "rowops.cuh"
 #include "tc_attention.cuh"
@@ -45,54 +46,10 @@ using namespace laya;
 
 namespace {
 
-// ---------------------------------------------------------------------------------------------
-// Errors
-// ---------------------------------------------------------------------------------------------
-thread_local std::string g_create_error;
-
-struct Failure {
-  int code;
-  std::string msg;
-};
-
-[[noreturn]] void fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  throw Failure{code, buf};
-}
-
-#define CK(call)                                                                                    \
-  do {                                                                                              \
-    cudaError_t e_ = (call);                                                                        \
-    if (e_ != cudaSuccess) fail(LAYA_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(e_));     \
-  } while (0)
-
 // Residual GEMMs of classes up to this many rows may split K across CTAs (their partial sums are
 // added, in split order, by the LayerNorm that follows), so small batches fill the SMs.
 constexpr int kSplitRowsMax = 2048;
 constexpr int kMaxSplits = 8;
-
-// ---------------------------------------------------------------------------------------------
-// Driver entry point for tensor-map encoding (no link-time dependency on libcuda).
-// ---------------------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
-    if (!p || q != cudaDriverEntryPointSuccess) fail(LAYA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-    fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
-  return fn;
-}
 
 // 2-D K-major operand [rows][cols] of 16-bit elements, box {64, box_rows}, 128-byte swizzle.
 CUtensorMap make_map(const void* ptr, int64_t rows, int64_t cols, int box_rows, bool bf16) {
@@ -128,25 +85,6 @@ CUtensorMap make_map_f32(const float* ptr, int64_t rows, int64_t cols, int64_t l
   return m;
 }
 
-int sm_count(int device) {
-  static std::map<int, int> cache;
-  auto it = cache.find(device);
-  if (it != cache.end()) return it->second;
-  int n = 0;
-  CK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
-  cache[device] = n;
-  return n;
-}
-
-// Process-wide launch options (laya_set_launch_options): programmatic dependent launch on every
-// kernel (on by default), and the wait limit every pipelined kernel's bounded waits use
-// (0: the kernels' default of 2 s).  Passes captured into CUDA graphs keep the options in effect
-// at capture.
-std::atomic<bool> g_pdl{true};
-std::atomic<unsigned long long> g_wait_ns{0};
-bool pdl_enabled() { return g_pdl.load(std::memory_order_relaxed); }
-unsigned long long wait_ns() { return g_wait_ns.load(std::memory_order_relaxed); }
-
 // Warps (= rows) per block of the row kernels: 8, or fewer when that leaves SMs idle, so that a
 // small class's rows spread over the whole GPU (one row per warp either way).
 int row_warps(int rows) {
@@ -156,21 +94,6 @@ int row_warps(int rows) {
   int w = kRowWarps;
   while (w > 1 && rows < w * sms) w /= 2;
   return w;
-}
-
-template <typename... KArgs, typename... Args>
-void launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  CK(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -1,0 +1,203 @@
+// Entry points of the MX8 operators (see include/laya_b200.h): checks of arguments and launches.
+#include <algorithm>
+#include <exception>
+
+#include "host.cuh"
+#include "mx8.cuh"
+#include "mx8_linear.cuh"
+
+using namespace laya;
+
+namespace {
+
+#define MX_API_BEGIN try {
+#define MX_API_END                                     \
+  }                                                    \
+  catch (const Failure& f) {                           \
+    g_create_error = f.msg;                            \
+    return f.code;                                     \
+  }                                                    \
+  catch (const std::exception& x) {                    \
+    g_create_error = x.what();                         \
+    return LAYA_ERR_CUDA;                              \
+  }                                                    \
+  return LAYA_OK;
+
+size_t dtype_size(int dtype) {
+  switch (dtype) {
+    case LAYA_DTYPE_F32: return 4;
+    case LAYA_DTYPE_F16:
+    case LAYA_DTYPE_BF16: return 2;
+    default: fail(LAYA_ERR_INVALID, "dtype %d is not F32, F16 or BF16", dtype);
+  }
+}
+
+// Calls f with a null pointer of the element type that `dtype` names.
+template <typename F>
+void with_type(int dtype, F f) {
+  switch (dtype) {
+    case LAYA_DTYPE_F32: return f((float*)nullptr);
+    case LAYA_DTYPE_F16: return f((__half*)nullptr);
+    case LAYA_DTYPE_BF16: return f((__nv_bfloat16*)nullptr);
+    default: fail(LAYA_ERR_INVALID, "dtype %d is not F32, F16 or BF16", dtype);
+  }
+}
+
+void check_shape(int rows, int cols) {
+  if (rows < 0 || cols < 1) fail(LAYA_ERR_INVALID, "bad shape %d x %d: rows may be 0, columns may not", rows, cols);
+}
+
+void check_rows(const char* what, const void* p, int64_t ld, int cols, int dtype) {
+  if (!p) fail(LAYA_ERR_INVALID, "%s is null", what);
+  if (ld < cols) fail(LAYA_ERR_INVALID, "%s: row stride %lld is less than %d columns", what, (long long)ld, cols);
+  if (reinterpret_cast<uintptr_t>(p) % dtype_size(dtype)) fail(LAYA_ERR_INVALID, "%s is not aligned to its elements", what);
+}
+
+void check_mx8(const char* what, const void* q, int64_t ld, const void* scales, int cols) {
+  if (!q || !scales) fail(LAYA_ERR_INVALID, "%s: null values or scales", what);
+  if (ld % 16 || ld < cols) fail(LAYA_ERR_INVALID, "%s: row stride %lld is not a multiple of 16 of at least %d", what, (long long)ld, cols);
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(scales)) & 15)
+    fail(LAYA_ERR_INVALID, "%s: values and scales must be 16-byte aligned", what);
+}
+
+void check_vector(const char* what, const float* p) {
+  if (p && (reinterpret_cast<uintptr_t>(p) & 15)) fail(LAYA_ERR_INVALID, "%s must be 16-byte aligned", what);
+}
+
+// The current device, checked to be `stream`'s.
+int current_device(cudaStream_t stream) {
+  int dev = 0;
+  CK(cudaGetDevice(&dev));
+  if (stream) {
+    int of = -1;
+    CK(cudaStreamGetDevice(stream, &of));
+    if (of != dev) fail(LAYA_ERR_INVALID, "stream belongs to device %d, the current device is %d", of, dev);
+  }
+  return dev;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t laya_mx8_scale_bytes(int rows, int cols) {
+  if (rows < 0 || cols < 1) return -1;
+  return ((int64_t)rows + kMxTileRows - 1) / kMxTileRows * (((int64_t)cols + kMxTileCols - 1) / kMxTileCols) * kMxTileBytes;
+}
+
+int laya_op_mx8_quantize(int dtype, const void* x, int64_t ldx, int rows, int cols, void* q, int64_t ldq, void* scales,
+                         void* stream) {
+  MX_API_BEGIN
+  check_shape(rows, cols);
+  dtype_size(dtype);
+  if (!rows) return LAYA_OK;
+  check_rows("x", x, ldx, cols, dtype);
+  check_mx8("out", q, ldq, scales, cols);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count(current_device(st));
+  const int64_t groups = (int64_t)rows * mx_col_tiles(cols);
+  const int grid = (int)std::min<int64_t>((groups + 15) / 16, 8LL * sms);
+  with_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    launch_k(mx8_quantize_kernel<T>, dim3(grid), dim3(kMxThreads), 0, st, static_cast<const T*>(x), ldx, rows, cols,
+             static_cast<uint8_t*>(q), ldq, static_cast<uint8_t*>(scales));
+  });
+  MX_API_END
+}
+
+int laya_op_mx8_dequantize(const void* q, int64_t ldq, const void* scales, int rows, int cols, int dtype, void* out,
+                           int64_t ldo, void* stream) {
+  MX_API_BEGIN
+  check_shape(rows, cols);
+  dtype_size(dtype);
+  if (!rows) return LAYA_OK;
+  check_mx8("x", q, ldq, scales, cols);
+  check_rows("out", out, ldo, cols, dtype);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count(current_device(st));
+  const int64_t pieces = (int64_t)rows * ((cols + 7) / 8);
+  const int grid = (int)std::min<int64_t>((pieces + kMxThreads - 1) / kMxThreads, 8LL * sms);
+  with_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    launch_k(mx8_dequantize_kernel<T>, dim3(grid), dim3(kMxThreads), 0, st, static_cast<const uint8_t*>(q), ldq,
+             static_cast<const uint8_t*>(scales), rows, cols, static_cast<T*>(out), ldo);
+  });
+  MX_API_END
+}
+
+int laya_op_rms_norm_mx8(int dtype, const void* x, int64_t ldx, int residual_dtype, const void* residual, int64_t ldr,
+                         void* sum_out, int64_t lds, const float* weight, float eps, int rows, int cols, void* q,
+                         int64_t ldq, void* scales, void* stream) {
+  MX_API_BEGIN
+  check_shape(rows, cols);
+  dtype_size(dtype);
+  dtype_size(residual_dtype);
+  if (!(eps >= 0.f)) fail(LAYA_ERR_INVALID, "eps must be at least 0");
+  if (!rows) return LAYA_OK;
+  check_rows("x", x, ldx, cols, dtype);
+  if (residual) check_rows("residual", residual, ldr, cols, residual_dtype);
+  if (sum_out) check_rows("sum_out", sum_out, lds, cols, residual_dtype);
+  if (!weight) fail(LAYA_ERR_INVALID, "weight is null");
+  check_vector("weight", weight);
+  check_mx8("out", q, ldq, scales, cols);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count(current_device(st));
+  RmsNormArgs a{};
+  a.x = x; a.ldx = ldx; a.residual = residual; a.ldr = ldr; a.sum_out = sum_out; a.lds = lds;
+  a.weight = weight; a.eps = eps; a.rows = rows; a.cols = cols;
+  a.q = static_cast<uint8_t*>(q); a.ldq = ldq; a.scales = static_cast<uint8_t*>(scales);
+  const int grid = std::min(rows, 8 * sms);
+  with_type(dtype, [&](auto* t) {
+    with_type(residual_dtype, [&](auto* r) {
+      launch_k(rms_norm_mx8_kernel<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(r)>>, dim3(grid),
+               dim3(kMxThreads), 0, st, a);
+    });
+  });
+  MX_API_END
+}
+
+int laya_op_mx8_linear(const laya_mx8_linear* p, int* err, void* stream) {
+  MX_API_BEGIN
+  if (!p) fail(LAYA_ERR_INVALID, "null argument");
+  const int M = p->rows, N = p->features, K = p->cols;
+  check_shape(M, N);
+  if (K < 1) fail(LAYA_ERR_INVALID, "bad depth %d", K);
+  if (p->activation < LAYA_ACT_NONE || p->activation > LAYA_ACT_SILU) fail(LAYA_ERR_INVALID, "unknown activation %d", p->activation);
+  if (p->out_dtype != LAYA_DTYPE_MX8) dtype_size(p->out_dtype);
+  if (p->residual) dtype_size(p->residual_dtype);
+  const bool gated = p->gate != nullptr;
+  if (p->gate_bias && !gated) fail(LAYA_ERR_INVALID, "gate_bias without a gate");
+  if (!M) return LAYA_OK;
+  check_mx8("x", p->x, p->ldx, p->x_scales, K);
+  check_mx8("w", p->w, p->ldw, p->w_scales, K);
+  if (gated) check_mx8("gate", p->gate, p->ldg, p->gate_scales, K);
+  check_vector("bias", p->bias);
+  check_vector("gate_bias", p->gate_bias);
+  if (p->residual) check_rows("residual", p->residual, p->ldr, N, p->residual_dtype);
+  if (p->out_dtype == LAYA_DTYPE_MX8) check_mx8("out", p->out, p->ldo, p->out_scales, N);
+  else check_rows("out", p->out, p->ldo, N, p->out_dtype);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  current_device(st);
+  auto vec4 = [](const void* q, int64_t ld, size_t size) {
+    return (reinterpret_cast<uintptr_t>(q) % (4 * size)) == 0 && ld % 4 == 0;
+  };
+  MxLinearArgs a{};
+  a.M = M; a.N = N; a.K = K;
+  a.x = {static_cast<const uint8_t*>(p->x), p->ldx, static_cast<const uint8_t*>(p->x_scales)};
+  a.w = {static_cast<const uint8_t*>(p->w), p->ldw, static_cast<const uint8_t*>(p->w_scales)};
+  a.gate = {static_cast<const uint8_t*>(p->gate), p->ldg, static_cast<const uint8_t*>(p->gate_scales)};
+  a.bias = p->bias; a.gate_bias = p->gate_bias; a.act = p->activation;
+  a.residual = p->residual; a.ldr = p->ldr; a.residual_type = p->residual_dtype;
+  if (p->residual) a.residual_vec = vec4(p->residual, p->ldr, dtype_size(p->residual_dtype));
+  a.out = p->out; a.ldo = p->ldo; a.out_type = p->out_dtype; a.out_scales = static_cast<uint8_t*>(p->out_scales);
+  if (p->out_dtype != LAYA_DTYPE_MX8) a.out_vec = vec4(p->out, p->ldo, dtype_size(p->out_dtype));
+  a.err = err;
+  a.wait_ns = wait_ns();
+  const dim3 grid((N + kMxSimpleTile - 1) / kMxSimpleTile, (M + kMxSimpleTile - 1) / kMxSimpleTile);
+  if (grid.y > 65535) fail(LAYA_ERR_INVALID, "too many rows: %d", M);
+  if (gated) launch_k(mx8_linear_simple_kernel<true>, grid, dim3(256), 0, st, a);
+  else launch_k(mx8_linear_simple_kernel<false>, grid, dim3(256), 0, st, a);
+  MX_API_END
+}
+
+}  // extern "C"

@@ -10,7 +10,8 @@ LIB_NAME = "liblaya_b200.so"
 LIB_PATH = Path(__file__).with_name(LIB_NAME)
 
 OK, ERR_INVALID, ERR_CUDA, ERR_DEVICE, ERR_STATE, ERR_NO_DEVICE = range(6)
-DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_MX8 = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 PRECISION_BF16, PRECISION_F16 = 0, 1
 
 # Every symbol declared in include/laya_b200.h.
@@ -21,6 +22,7 @@ EXPORTS = (
     "laya_profile_read", "laya_read_tensor", "laya_cached_shapes", "laya_pool_bytes", "laya_destroy",
     "laya_last_error", "laya_set_launch_options", "laya_op_gemm", "laya_op_gemm_ln", "laya_interleave_geglu", "laya_op_attention", "laya_op_attention_gathered",
     "laya_attention_tiles", "laya_op_embed_norm", "laya_op_head_tail", "laya_op_norm", "laya_op_gemm_residual_static",
+    "laya_mx8_scale_bytes", "laya_op_mx8_quantize", "laya_op_mx8_dequantize", "laya_op_rms_norm_mx8", "laya_op_mx8_linear",
 )
 STATIC_SCRATCH_FLOATS = 4 * 1024 * 1024
 
@@ -37,6 +39,17 @@ class Metrics(ct.Structure):
     _fields_ = [("gpu_ms", ct.c_float), ("rows", ct.c_int32), ("batch", ct.c_int32), ("options", ct.c_int32),
                 ("cache_miss", ct.c_int32), ("graph_capture", ct.c_int32), ("graph_replay", ct.c_int32),
                 ("kernel_launches", ct.c_int32), ("owned_gpu_bytes", ct.c_uint64)]
+
+
+class Mx8Linear(ct.Structure):
+    _fields_ = [("rows", ct.c_int32), ("features", ct.c_int32), ("cols", ct.c_int32), ("activation", ct.c_int32),
+                ("x", ct.c_void_p), ("x_scales", ct.c_void_p), ("ldx", ct.c_int64),
+                ("w", ct.c_void_p), ("w_scales", ct.c_void_p), ("ldw", ct.c_int64),
+                ("gate", ct.c_void_p), ("gate_scales", ct.c_void_p), ("ldg", ct.c_int64),
+                ("bias", ct.c_void_p), ("gate_bias", ct.c_void_p),
+                ("residual", ct.c_void_p), ("ldr", ct.c_int64),
+                ("out", ct.c_void_p), ("out_scales", ct.c_void_p), ("ldo", ct.c_int64),
+                ("residual_dtype", ct.c_int32), ("out_dtype", ct.c_int32)]
 
 
 _lib = None
@@ -85,6 +98,14 @@ def load():
         "laya_op_norm": (i, [i, p, p, i, p, p, ct.c_float, p, i, i, p]),
         "laya_op_head_tail": (i, [i, p, p, p, i, i, i, p, p, p, p, p, p, i, p, p, p, p, p, p]),
         "laya_op_gemm_residual_static": (i, [i, p, p, i, i, i, i, p, p, p, p]),
+    }
+    q = ct.c_int64
+    sig |= {
+        "laya_mx8_scale_bytes": (q, [i, i]),
+        "laya_op_mx8_quantize": (i, [i, p, q, i, i, p, q, p, p]),
+        "laya_op_mx8_dequantize": (i, [p, q, p, i, i, i, p, q, p]),
+        "laya_op_rms_norm_mx8": (i, [i, p, q, i, p, q, p, q, p, ct.c_float, i, i, p, q, p, p]),
+        "laya_op_mx8_linear": (i, [ct.POINTER(Mx8Linear), p, p]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

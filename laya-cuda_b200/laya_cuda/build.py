@@ -12,10 +12,10 @@ PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE.parent / "csrc"
 INCLUDE = PACKAGE.parents[1] / "include"
 TARGET = PACKAGE / "liblaya_b200.so"
-SOURCES = [CSRC / "laya_b200.cu"]
+SOURCES = [CSRC / "laya_b200.cu", CSRC / "mx8.cu"]
 DEPENDS = SOURCES + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "laya_b200.h"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-         "-Xcompiler", "-fPIC", "-shared", "-cudart", "static"]
+         "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "--threads", "2"]
 
 
 def nvcc():

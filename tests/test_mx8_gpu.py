@@ -1,0 +1,498 @@
+"""The MX8 operators on the GPU against their definitions in 64 bits.
+
+Quantising and reading back are exact operations and are compared bit for bit.  The norm and the
+product compute in fp32; their tolerances are bounds on that arithmetic (see `norm_slack` and
+`product_slack`) plus the one rounding of the output.
+"""
+import ctypes as ct
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from laya_cuda import _lib, mx8  # noqa: E402
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+# Half a unit in the last place of a rounded output, relative.
+HALF_ULP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TINY = {"f32": 2.0 ** -149, "f16": 2.0 ** -25, "bf16": 2.0 ** -133}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("CUDA device required")
+
+
+# -------------------------------------------------------------------------------- the format in 64 bits
+
+def e4m3_table():
+    out = np.empty(256)
+    for b in range(256):
+        sign, power, fraction = -1.0 if b & 128 else 1.0, (b >> 3) & 15, b & 7
+        v = (1 + fraction / 8) * 2.0 ** (power - 7) if power else fraction / 8 * 2.0 ** -6
+        out[b] = math.nan if (b & 127) == 127 else sign * v
+    return out
+
+
+TABLE = e4m3_table()
+
+
+def scale_index(rows, cols):
+    """Byte index of each (row, block)."""
+    r, b = np.arange(rows)[:, None], np.arange(-(-cols // 32))[None, :]
+    return (r // 128 * -(-cols // 128) + b // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + b % 4
+
+
+def decode(m):
+    """A Matrix in float64, [rows][cols], and its scale exponents [rows][blocks] (255: NaN)."""
+    q = m.values.cpu().numpy()[:, : m.cols]
+    byte = m.scales.cpu().numpy()[scale_index(m.rows, m.cols)].astype(np.int64)
+    scale = np.where(byte == 255, math.nan, np.ldexp(1.0, byte - 127))
+    return TABLE[q] * np.repeat(scale, 32, axis=1)[:, : m.cols], byte
+
+
+def blocks(v):
+    rows, cols = v.shape
+    out = np.zeros((rows, -(-cols // 32) * 32))
+    out[:, :cols] = v
+    return out.reshape(rows, -1, 32)
+
+
+def define(v):
+    """The definition: E4M3 codes and scale bytes of float64 values."""
+    b = blocks(v)
+    bad = ~np.isfinite(b).all(-1)
+    a = np.abs(np.where(np.isfinite(b), b, 0)).max(-1)
+    mantissa, power = np.frexp(a)
+    e = np.where(a > 0, power - 9 + (mantissa > 0.875), -127)
+    e = np.maximum(e, -127)
+    x = np.where(bad[..., None], 0, b) / np.ldexp(1.0, e)[..., None]
+    # Nearest E4M3 magnitude, ties to the even code (codes 0..126 ascend).
+    mags = TABLE[:127]
+    hi = np.clip(np.searchsorted(mags, np.abs(x)), 0, 126)
+    lo = np.maximum(hi - 1, 0)
+    dl, dh = np.abs(x) - mags[lo], mags[hi] - np.abs(x)
+    code = np.where((dl < dh) | ((dl == dh) & (lo % 2 == 0)), lo, hi)
+    code = np.where(np.signbit(x), code + 128, code)
+    code = np.where(bad[..., None], 127, code)
+    return code.reshape(v.shape[0], -1)[:, : v.shape[1]].astype(np.uint8), np.where(bad, 255, e + 127)
+
+
+def matrix(v):
+    """A Matrix that holds float64/float32 values `v` (numpy), and what it stands for."""
+    rows, cols = v.shape
+    code, byte = define(v.astype(np.float64))
+    room = (cols + 15) // 16 * 16
+    q = np.zeros((rows, room), np.uint8)
+    q[:, :cols] = code
+    s = np.full(mx8.scale_bytes(rows, cols), 255, np.uint8)  # unwritten rows may hold anything
+    idx = scale_index(rows, -(-cols // 128) * 128)
+    s[idx] = 0
+    s[scale_index(rows, cols)] = byte
+    m = mx8.Matrix(torch.from_numpy(q).cuda(), torch.from_numpy(s).cuda(), rows, cols)
+    return m, decode(m)[0]
+
+
+def fresh(rows, cols):
+    m = mx8.Matrix.empty(torch.empty(0, device="cuda"), rows, cols)
+    m.values.fill_(0xA5)
+    m.scales.fill_(0xA5)
+    return m
+
+
+def strided(rows, cols, dtype, pad=0, offset=0, fill=None):
+    """[rows][cols] view with row stride cols + pad, starting `offset` elements into its buffer."""
+    store = torch.full((rows * (cols + pad) + offset + 8,), 7.0, dtype=dtype, device="cuda")
+    view = store[offset: offset + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+    if fill is not None:
+        view.copy_(torch.from_numpy(fill))
+    return view, store
+
+
+def untouched(view, store, pad, offset):
+    """Every element of the buffer outside the view still holds 7."""
+    rest = store.clone()
+    rows, cols = view.shape
+    rest[offset: offset + rows * (cols + pad)].view(rows, cols + pad)[:, :cols] = 7.0
+    return bool((rest == 7.0).all())
+
+
+def activations(rng, rows, cols):
+    return (rng.normal(0, 1, (rows, cols)) * np.exp(0.8 * rng.normal(0, 1, cols))).astype(np.float32)
+
+
+SHAPES = [(1, 1), (1, 31), (3, 32), (5, 33), (1, 768), (129, 100), (257, 128), (33, 1000), (1, 5000), (300, 264)]
+
+
+# -------------------------------------------------------------------------------- quantize, dequantize
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("pad,offset", [(0, 0), (3, 1), (8, 8)])
+def test_quantize_is_the_definition_bit_for_bit(dtype, rows, cols, pad, offset):
+    rng = np.random.default_rng(rows * 1000 + cols)
+    v = activations(rng, rows, cols) * np.ldexp(1.0, rng.integers(-12, 5, (rows, 1))).astype(np.float32)
+    v[rng.random((rows, cols)) < 0.05] = 0
+    if cols >= 64:
+        v[0, :32] = 0  # a block of zeros
+    x, _ = strided(rows, cols, TYPES[dtype], pad, offset, v)
+    out = fresh(rows, cols)
+    mx8.quantize(x, out)
+    code, byte = define(x.double().cpu().numpy())
+    got = out.values.cpu().numpy()
+    np.testing.assert_array_equal(got[:, :cols], code)
+    assert not got[:, cols:].any()
+    np.testing.assert_array_equal(out.scales.cpu().numpy()[scale_index(rows, cols)], byte)
+    whole = out.scales.cpu().numpy()[scale_index(rows, -(-cols // 128) * 128)]
+    assert not whole[:, -(-cols // 32):].any()
+
+
+def test_quantize_at_the_edges_of_the_range():
+    """Largest magnitudes around 1.75 x 2^p, ties, subnormals, the extremes of fp32 and signed zeros."""
+    up = np.nextafter(np.float32(1.75), np.float32(2))
+    rows = [[1.75], [up], [np.float32(2.0 ** -126)], [np.float32(1e-45)], [np.float32(3.4028235e38)], [-0.0],
+            [448.0, 17.0, 18.0, 19.0, 2.0 ** -10, 3 * 2.0 ** -10], [np.float32(1.75 * 2.0 ** -119)], [np.float32(2.0 ** -119)]]
+    v = np.zeros((len(rows), 32), np.float32)
+    for i, r in enumerate(rows):
+        v[i, :len(r)] = r
+    out = fresh(*v.shape)
+    mx8.quantize(torch.from_numpy(v).cuda(), out)
+    code, byte = define(v.astype(np.float64))
+    np.testing.assert_array_equal(out.values.cpu().numpy(), code)
+    np.testing.assert_array_equal(out.scales.cpu().numpy()[scale_index(*v.shape)], byte)
+    assert byte[0, 0] == 119 and byte[1, 0] == 120
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_non_finite_blocks_read_back_as_nan_and_no_other(bad):
+    v = np.ones((4, 96), np.float32)
+    v[2, 40] = bad
+    out, back = fresh(4, 96), torch.empty(4, 96, device="cuda")
+    mx8.quantize(torch.from_numpy(v).cuda(), out)
+    mx8.dequantize(out, back)
+    want = v.copy()
+    want[2, 32:64] = math.nan
+    np.testing.assert_array_equal(back.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("pad,offset", [(0, 0), (3, 1)])
+def test_dequantize_is_exact(dtype, rows, cols, pad, offset):
+    rng = np.random.default_rng(rows * 1000 + cols + 1)
+    m, v = matrix(activations(rng, rows, cols))
+    out, store = strided(rows, cols, TYPES[dtype], pad, offset)
+    mx8.dequantize(m, out)
+    want = torch.from_numpy(v).to(TYPES[dtype])
+    assert torch.equal(out.cpu(), want)
+    assert untouched(out, store, pad, offset)
+
+
+def test_dequantize_every_code_and_scale():
+    """Each E4M3 code under each scale byte (fp32 output; overflow to infinity as the rounding gives)."""
+    q = torch.arange(256, dtype=torch.uint8).repeat(256, 1)
+    m = mx8.Matrix(q.cuda(), torch.zeros(mx8.scale_bytes(256, 256), dtype=torch.uint8, device="cuda"), 256, 256)
+    byte = np.repeat(np.arange(256, dtype=np.uint8)[:, None], 8, axis=1)
+    s = m.scales.cpu().numpy()
+    s[scale_index(256, 256)] = byte
+    m.scales.copy_(torch.from_numpy(s))
+    out = torch.empty(256, 256, device="cuda")
+    mx8.dequantize(m, out)
+    with np.errstate(over="ignore"):
+        want = decode(m)[0].astype(np.float32)
+    np.testing.assert_array_equal(out.cpu().numpy(), want)
+
+
+# -------------------------------------------------------------------------------- rms_norm
+
+def norm_slack(cols):
+    """Relative error of y: the sum of squares is a tree over at most cols / 32 + 32 serial additions
+    and products, halved by the root; then four roundings."""
+    return (cols / 32 + 32) * 2.0 ** -24 / 2 + 5 * 2.0 ** -24
+
+
+def check_mx8(out, y, slack):
+    """`out` holds y (float64) to within `slack` (absolute, per element) and E4M3's rounding."""
+    got, byte = decode(out)
+    a = np.abs(blocks(y)).max(-1)
+    da = blocks(np.broadcast_to(slack, y.shape)).max(-1)
+    lo, hi = define(np.maximum(a - da, 0).reshape(-1, 1))[1], define((a + da).reshape(-1, 1))[1]
+    assert ((byte >= lo.reshape(byte.shape)) & (byte <= hi.reshape(byte.shape))).all()
+    scale = np.repeat(np.ldexp(1.0, byte - 127), 32, axis=1)[:, : y.shape[1]]
+    power = np.floor(np.log2(np.maximum(np.abs(y) / scale, 2.0 ** -6)))
+    # Half a step: 2^(power - 4), one binade up where the slack may cross it.
+    half = scale * np.ldexp(1.0, power.astype(np.int64) - 4)
+    off = np.abs(got - y)
+    tol = half * (1 + 1e-12) + 2 * slack
+    assert (off <= tol).all(), float((off / tol).max())
+    q = out.values.cpu().numpy()
+    assert not q[:, out.cols: (out.cols + 15) // 16 * 16].any()
+
+
+NORM_SHAPES = [(1, 1), (2, 31), (7, 33), (1, 768), (130, 256), (33, 1000), (3, 2048), (2, 4100), (5, 8192), (1, 16384), (2, 40000)]
+
+
+@pytest.mark.parametrize("dtype,rdtype", [("bf16", "f32"), ("f16", "f16"), ("f32", "f32"), ("bf16", "bf16"), ("f32", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("rows,cols", NORM_SHAPES)
+@pytest.mark.parametrize("pad,offset", [(0, 0), (5, 1)])
+def test_rms_norm(dtype, rdtype, rows, cols, pad, offset):
+    rng = np.random.default_rng(rows * 31 + cols)
+    x, _ = strided(rows, cols, TYPES[dtype], pad, offset, activations(rng, rows, cols))
+    r, _ = strided(rows, cols, TYPES[rdtype], pad, offset, rng.normal(0, 1, (rows, cols)).astype(np.float32))
+    w = torch.from_numpy((1 + 0.2 * rng.normal(0, 1, cols)).astype(np.float32)).cuda()
+    total, store = strided(rows, cols, TYPES[rdtype], pad, offset)
+    out = fresh(rows, cols)
+    mx8.rms_norm(x, w, out, residual=r, sum_out=total, eps=1e-5)
+    h = x.double().cpu().numpy() + r.double().cpu().numpy()
+    y = h / np.sqrt((h * h).mean(1, keepdims=True) + 1e-5) * w.double().cpu().numpy()
+    off = np.abs(total.double().cpu().numpy() - h)
+    assert (off <= (HALF_ULP[rdtype] + 2.0 ** -23) * np.abs(h) + TINY[rdtype]).all()
+    assert untouched(total, store, pad, offset)
+    # h itself is rounded to fp32 once before it is squared and scaled.
+    check_mx8(out, y, norm_slack(cols) * np.abs(y))
+
+
+def test_rms_norm_without_residual_and_in_place():
+    rng = np.random.default_rng(5)
+    rows, cols = 9, 520
+    v = activations(rng, rows, cols)
+    x, w = torch.from_numpy(v).cuda(), torch.ones(cols, device="cuda")
+    out = fresh(rows, cols)
+    mx8.rms_norm(x, w, out)
+    h = v.astype(np.float64)
+    check_mx8(out, h / np.sqrt((h * h).mean(1, keepdims=True) + 1e-6), norm_slack(cols) * np.abs(h) * 2)
+    r = torch.from_numpy(rng.normal(0, 1, (rows, cols)).astype(np.float32)).cuda()
+    keep, one, two = r.clone(), fresh(rows, cols), torch.empty_like(r)
+    mx8.rms_norm(x, w, one, residual=r, sum_out=two)
+    mx8.rms_norm(x, w, out, residual=r, sum_out=r)
+    assert torch.equal(r, two) and torch.equal(out.values, one.values) and not torch.equal(r, keep)
+
+
+def test_rms_norm_of_zero_rows_is_zero_and_non_finite_rows_are_nan():
+    x = torch.ones(5, 300, device="cuda")
+    x[1] = 0
+    x[3, 7] = math.inf
+    x[4, 299] = math.nan
+    out, back = fresh(5, 300), torch.empty(5, 300, device="cuda")
+    mx8.rms_norm(x, torch.ones(300, device="cuda"), out, eps=0.0)
+    mx8.dequantize(out, back)
+    got = back.cpu()
+    assert torch.equal(got[0], torch.ones(300)) and torch.equal(got[2], torch.ones(300))
+    assert torch.isnan(got[4]).all()
+    # 0 * rsqrt(0) is NaN without eps; with eps it is 0.
+    assert torch.isnan(got[1]).all()
+    mx8.rms_norm(x, torch.ones(300, device="cuda"), out)
+    mx8.dequantize(out, back)
+    assert not back[1].any()
+    # inf / inf is NaN; the finite values of that row are over infinity, 0, outside the NaN's block.
+    assert torch.isnan(back[3, :32]).all() and not back[3, 32:].any()
+
+
+# -------------------------------------------------------------------------------- linear
+
+def act64(v, name):
+    if name == "relu":
+        return np.maximum(v, 0)
+    if name == "gelu":
+        return 0.5 * v * (1 + torch.erf(torch.from_numpy(v / math.sqrt(2))).numpy())
+    if name == "silu":
+        return v / (1 + np.exp(-v))
+    return v
+
+
+def product_slack(x, w):
+    """Error of the fp32 sums: K / 32 accumulation steps, each off by at most 2^-22 (a unit in the last place of
+    a truncated fp32 sum and of its aligned terms) of the largest partial sum, which for these inputs stays
+    under four times the root of the sum of the squared products."""
+    k = x.shape[1]
+    return (k / 32 + 1) * 2.0 ** -20 * np.sqrt((x * x) @ (w * w).T)
+
+
+def reference(x, w, gate, bias, gate_bias, act, residual):
+    """The result in float64 and its slack before the output's rounding."""
+    u, du = x @ w.T, product_slack(x, w)
+    if bias is not None:
+        u, du = u + bias, du + 2.0 ** -23 * np.abs(u + bias)
+    if gate is not None:
+        g, dg = x @ gate.T, product_slack(x, gate)
+        if gate_bias is not None:
+            g, dg = g + gate_bias, dg + 2.0 ** -23 * np.abs(g + gate_bias)
+        a = act64(g, act)
+        # Activations have slopes up to 1.13 and are themselves within 1e-6 (absolute, or relative where larger).
+        da = 1.13 * dg + 1e-6 * (1 + np.abs(a))
+        y, dy = a * u, np.abs(u) * da + np.abs(a) * du + da * du
+    else:
+        y = act64(u, act)
+        dy = 1.13 * du + (0 if act == "none" else 1e-6 * (1 + np.abs(y)))
+    if residual is not None:
+        y, dy = y + residual, dy + 2.0 ** -23 * np.abs(y + residual)
+    return y, dy + 2.0 ** -22 * np.abs(y)
+
+
+def run_linear(rows, cols, n, out_type, act="none", gated=False, bias=False, residual=None, seed=0, pad=0, offset=0):
+    rng = np.random.default_rng(seed + rows * 7 + cols * 3 + n)
+    x, xd = matrix(activations(rng, rows, cols))
+    w, wd = matrix((rng.normal(0, 1, (n, cols)) / math.sqrt(cols)).astype(np.float32))
+    g, gd = matrix((rng.normal(0, 1, (n, cols)) / math.sqrt(cols)).astype(np.float32)) if gated else (None, None)
+    vec = lambda on: torch.from_numpy((0.1 * rng.normal(0, 1, n)).astype(np.float32)).cuda() if on else None  # noqa: E731
+    b, gb = vec(bias), vec(bias and gated)
+    r = None
+    if residual:
+        r, _ = strided(rows, n, TYPES[residual], pad, offset, rng.normal(0, 1, (rows, n)).astype(np.float32))
+    to64 = lambda t: None if t is None else t.double().cpu().numpy()  # noqa: E731
+    y, dy = reference(xd, wd, gd, to64(b), to64(gb), act, to64(r))
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    if out_type == "mx8":
+        out, store = fresh(rows, n), None
+    else:
+        out, store = strided(rows, n, TYPES[out_type], pad, offset)
+    mx8.linear(x, w, out, bias=b, gate=g, gate_bias=gb, activation=act, residual=r, err=err)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    if out_type == "mx8":
+        check_mx8(out, y, dy)
+    else:
+        off = np.abs(out.double().cpu().numpy() - y)
+        tol = dy + HALF_ULP[out_type] * (np.abs(y) + dy) + TINY[out_type]
+        assert (off <= tol).all(), float((off / tol).max())
+        assert untouched(out, store, pad, offset)
+
+
+LINEAR_SHAPES = [(1, 1, 1), (1, 32, 8), (1, 768, 768), (2, 33, 31), (7, 128, 129), (16, 1000, 257), (17, 160, 64), (31, 31, 300),
+                 (33, 512, 200), (64, 2048, 384), (65, 256, 130), (100, 777, 513), (128, 128, 128), (129, 96, 257),
+                 (200, 1024, 640), (257, 4096, 96), (300, 260, 1000), (513, 640, 300)]
+
+
+@pytest.mark.parametrize("rows,cols,n", LINEAR_SHAPES)
+@pytest.mark.parametrize("out_type", ["bf16", "f32", "mx8"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_linear_shapes(rows, cols, n, out_type, gated):
+    run_linear(rows, cols, n, out_type, act="silu" if gated else "none", gated=gated)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("out_type,residual", [("f16", None), ("bf16", "f32"), ("f32", "bf16"), ("mx8", "f16")])
+def test_linear_epilogues(rows, act, gated, out_type, residual):
+    run_linear(rows, 320, 264, out_type, act=act, gated=gated, bias=True, residual=residual, seed=1)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("pad,offset", [(1, 1), (4, 0), (3, 2), (8, 8)])
+@pytest.mark.parametrize("out_type", ["f16", "f32"])
+def test_linear_strides_and_alignment(rows, pad, offset, out_type):
+    run_linear(rows, 200, 133, out_type, bias=True, residual="bf16", seed=2, pad=pad, offset=offset)
+
+
+@pytest.mark.parametrize("rows", [3, 260])
+def test_linear_adds_into_the_residual_in_place(rows):
+    rng = np.random.default_rng(8)
+    x, _ = matrix(activations(rng, rows, 192))
+    w, _ = matrix(rng.normal(0, 0.1, (256, 192)).astype(np.float32))
+    r = torch.from_numpy(rng.normal(0, 1, (rows, 256)).astype(np.float32)).cuda()
+    want = torch.empty_like(r)
+    mx8.linear(x, w, want, residual=r)
+    mx8.linear(x, w, r, residual=r)
+    assert torch.equal(r, want)
+
+
+@pytest.mark.parametrize("rows", [5, 150, 400])
+def test_linear_keeps_non_finite_values_to_their_rows(rows):
+    """A NaN block of x makes its row NaN, one of w its column; nothing else changes.  The scales of rows past
+    the last hold NaN bytes (see `matrix`) and reach no result."""
+    rng = np.random.default_rng(9)
+    xv, wv = activations(rng, rows, 256), rng.normal(0, 0.1, (300, 256)).astype(np.float32)
+    plain = torch.empty(rows, 300, device="cuda")
+    mx8.linear(matrix(xv)[0], matrix(wv)[0], plain)
+    assert torch.isfinite(plain).all()
+    xv[2, 70], wv[291, 3] = math.inf, math.nan
+    out = torch.empty(rows, 300, device="cuda")
+    mx8.linear(matrix(xv)[0], matrix(wv)[0], out)
+    want = plain.clone()
+    want[2], want[:, 291] = math.nan, math.nan
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(out), torch.nan_to_num(want))
+
+
+@pytest.mark.parametrize("rows,cols,n", [(4, 2048, 512), (90, 1024, 512), (700, 512, 768)])
+def test_linear_gives_the_same_bits_each_time_and_a_row_does_not_depend_on_the_others(rows, cols, n):
+    rng = np.random.default_rng(10)
+    xv = activations(rng, rows, cols)
+    w, _ = matrix(rng.normal(0, 0.1, (n, cols)).astype(np.float32))
+    x, _ = matrix(xv)
+    one, two, other = (torch.empty(rows, n, device="cuda") for _ in range(3))
+    mx8.linear(x, w, one)
+    xv[1:] *= -3
+    mx8.linear(matrix(xv)[0], w, other)
+    mx8.linear(x, w, two)
+    assert torch.equal(one, two) and torch.equal(one[0], other[0])
+
+
+def test_one_layer_on_another_stream():
+    """norm -> gated product in MX8 -> product onto the residual, on a side stream."""
+    rng = np.random.default_rng(11)
+    rows, d, f = 70, 256, 352
+    x = torch.from_numpy(activations(rng, rows, d)).cuda().bfloat16()
+    r = torch.from_numpy(rng.normal(0, 1, (rows, d)).astype(np.float32)).cuda()
+    weight = torch.ones(d, device="cuda")
+    (up, _), (gate, _), (down, downd) = (matrix(rng.normal(0, 0.08, s).astype(np.float32)) for s in ((f, d), (f, d), (d, f)))
+    n8, a8, y = fresh(rows, d), fresh(rows, f), torch.empty(rows, d, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    s = side.cuda_stream
+    mx8.rms_norm(x, weight, n8, residual=r, sum_out=r, stream=s)
+    mx8.linear(n8, up, a8, gate=gate, activation="silu", stream=s)
+    mx8.linear(a8, down, y, residual=r, stream=s)
+    side.synchronize()
+    a = decode(a8)[0]
+    want, slack = reference(a, downd, None, None, None, "none", r.double().cpu().numpy())
+    assert (np.abs(y.double().cpu().numpy() - want) <= slack + 2.0 ** -23 * np.abs(want)).all()
+
+
+def test_no_rows_is_no_work():
+    w, _ = matrix(np.ones((8, 32), np.float32))
+    x = mx8.Matrix.empty(w.values, 0, 32)
+    mx8.linear(x, w, torch.empty(0, 8, device="cuda"))
+    mx8.quantize(torch.empty(0, 32, device="cuda"), x)
+    mx8.dequantize(x, torch.empty(0, 32, device="cuda"))
+    mx8.rms_norm(torch.empty(0, 32, device="cuda"), torch.ones(32, device="cuda"), x)
+    torch.cuda.synchronize()
+
+
+def test_refusals():
+    w, _ = matrix(np.ones((8, 32), np.float32))
+    x, _ = matrix(np.ones((3, 32), np.float32))
+    other, _ = matrix(np.ones((3, 64), np.float32))
+    good = torch.empty(3, 8, device="cuda")
+    for bad in (lambda: mx8.linear(other, w, good),
+                lambda: mx8.linear(x, w, torch.empty(3, 9, device="cuda")),
+                lambda: mx8.linear(x, w, good.double()),
+                lambda: mx8.linear(x, w, torch.empty(8, 3, device="cuda").T),
+                lambda: mx8.linear(x, w, good, activation="tanh"),
+                lambda: mx8.linear(x, w, good, gate=other),
+                lambda: mx8.linear(x, w, good, gate_bias=torch.zeros(8, device="cuda")),
+                lambda: mx8.linear(x, w, good, bias=torch.zeros(8, device="cuda").half()),
+                lambda: mx8.linear(x, w, good, bias=torch.zeros(9, device="cuda")[1:]),
+                lambda: mx8.linear(x, w, good, residual=torch.zeros(1, 8, device="cuda").expand(3, 8)),
+                lambda: mx8.linear(x, w, good.cpu()),
+                lambda: mx8.quantize(torch.ones(3, 31, device="cuda"), x),
+                lambda: mx8.quantize(torch.ones(3, 32, device="cuda", dtype=torch.int32), x),
+                lambda: mx8.rms_norm(torch.ones(3, 32, device="cuda"), torch.ones(31, device="cuda"), x),
+                lambda: mx8.rms_norm(torch.ones(3, 32, device="cuda"), torch.ones(32, device="cuda"), x, eps=-1.0),
+                lambda: mx8.rms_norm(torch.ones(3, 32, device="cuda"), torch.ones(32, device="cuda"), x,
+                                     residual=torch.ones(3, 32, device="cuda"),
+                                     sum_out=torch.ones(3, 32, device="cuda").half()),
+                lambda: mx8.Matrix(x.values[:, 1:], x.scales, 3, 31),
+                lambda: mx8.Matrix(x.values, x.scales[:511], 3, 32),
+                lambda: mx8.Matrix.empty(good, 3, 0)):
+        with pytest.raises(ValueError):
+            bad()
+    # A matrix whose rows are not 16-byte aligned is refused when it is used.
+    shifted = torch.zeros(3 * 48 + 1, dtype=torch.uint8, device="cuda")[1:].view(3, 48)
+    with pytest.raises(ValueError, match="aligned"):
+        mx8.linear(mx8.Matrix(shifted, x.scales, 3, 32), w, good)
