@@ -4,7 +4,7 @@
 
 #include "host.cuh"
 #include "mx8.cuh"
-#include "mx8_linear.cuh"
+#include "mx8_gemm.cuh"
 
 using namespace laya;
 
@@ -74,6 +74,112 @@ int current_device(cudaStream_t stream) {
     if (of != dev) fail(LAYA_ERR_INVALID, "stream belongs to device %d, the current device is %d", of, dev);
   }
   return dev;
+}
+
+// E4M3 values [rows][cols], row stride ld bytes; box {128 columns, box_rows}, 128-byte swizzle.
+CUtensorMap value_map(const MxOperand& m, int rows, int cols, int box_rows) {
+  CUtensorMap map;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)m.ld};
+  cuuint32_t box[2] = {kMxBK, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(m.q), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) fail(LAYA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return map;
+}
+
+// Scale tiles [row tiles][column tiles][512 bytes]; box {512 bytes, 1, box_tiles}.  Row tiles past the last read as zeros
+// (scale 2^-127).
+CUtensorMap scale_map(const MxOperand& m, int rows, int cols, int box_tiles) {
+  CUtensorMap map;
+  const cuuint64_t col_tiles = mx_col_tiles(cols), row_tiles = ((cuuint64_t)rows + kMxTileRows - 1) / kMxTileRows;
+  cuuint64_t dims[3] = {kMxTileBytes / 4, col_tiles, row_tiles};
+  cuuint64_t strides[2] = {kMxTileBytes, col_tiles * kMxTileBytes};
+  cuuint32_t box[3] = {kMxTileBytes / 4, 1, (cuuint32_t)box_tiles};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, const_cast<uint8_t*>(m.scales), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) fail(LAYA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return map;
+}
+
+MxMaps linear_maps(const MxLinearArgs& a, int x_box, int w_box, int w_tiles) {
+  MxMaps m{};
+  m.x = value_map(a.x, a.M, a.K, x_box);
+  m.xs = scale_map(a.x, a.M, a.K, 1);
+  m.w = value_map(a.w, a.N, a.K, w_box);
+  m.ws = scale_map(a.w, a.N, a.K, w_tiles);
+  if (a.gate.q) {
+    m.g = value_map(a.gate, a.N, a.K, w_box);
+    m.gs = scale_map(a.gate, a.N, a.K, w_tiles);
+  }
+  return m;
+}
+
+// Raises the kernel's dynamic shared memory limit once per device (`done`: one bit per device).
+template <typename K>
+void allow_smem(K kern, int bytes, int dev, std::atomic<uint64_t>& done) {
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
+template <typename K>
+void launch_cluster(K kern, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, const MxMaps& m, const MxLinearArgs& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster.x;
+  attr[0].val.clusterDim.y = cluster.y;
+  attr[0].val.clusterDim.z = cluster.z;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  CK(cudaLaunchKernelEx(&cfg, kern, m, a));
+}
+
+template <int BN, bool kGated>
+void launch_pair(const MxLinearArgs& a, int dev, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  using Cfg = MxPairCfg<BN>;
+  auto kern = mx8_linear_pair_kernel<BN, kGated>;
+  allow_smem(kern, Cfg::kSmemBytes, dev, done);
+  const MxMaps m = linear_maps(a, 128, BN / 2, kGated ? 1 : Cfg::kWeightTiles);
+  const int out_cols = kGated ? BN / 2 : BN;
+  const int64_t tiles = (((int64_t)a.M + 255) / 256) * ((a.N + out_cols - 1) / out_cols);
+  if (tiles > INT32_MAX / 2) fail(LAYA_ERR_INVALID, "result of %d x %d is too large", a.M, a.N);
+  const int pairs = (int)std::min<int64_t>(tiles, sm_count(dev) / 2);
+  launch_cluster(kern, dim3(2 * pairs), kMxThreadsPair, Cfg::kSmemBytes, dim3(2, 1, 1), st, m, a);
+}
+
+template <int BN, bool kGated>
+void launch_few(const MxLinearArgs& a, int dev, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  using Cfg = MxFewCfg<BN, kGated>;
+  auto kern = mx8_linear_few_kernel<BN, kGated>;
+  allow_smem(kern, Cfg::kSmemBytes, dev, done);
+  const MxMaps m = linear_maps(a, BN, 128, 1);
+  const int tiles = (a.N + 127) / 128, row_tiles = (a.M + BN - 1) / BN, k_tiles = mx_col_tiles(a.K);
+  int split = 1;
+  while (split < kMxMaxSplit && 2 * split <= k_tiles && (int64_t)tiles * row_tiles * split < sm_count(dev)) split *= 2;
+  launch_cluster(kern, dim3(tiles, row_tiles, split), kMxThreadsFew, Cfg::kSmemBytes, dim3(1, 1, split), st, m, a);
+}
+
+template <bool kGated>
+void launch_linear(const MxLinearArgs& a, int dev, cudaStream_t st) {
+  if (a.M <= 16) return launch_few<16, kGated>(a, dev, st);
+  if (a.M <= 32) return launch_few<32, kGated>(a, dev, st);
+  if (a.M <= 128) return launch_few<64, kGated>(a, dev, st);
+  launch_pair<256, kGated>(a, dev, st);
 }
 
 }  // namespace
@@ -177,7 +283,7 @@ int laya_op_mx8_linear(const laya_mx8_linear* p, int* err, void* stream) {
   if (p->out_dtype == LAYA_DTYPE_MX8) check_mx8("out", p->out, p->ldo, p->out_scales, N);
   else check_rows("out", p->out, p->ldo, N, p->out_dtype);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  current_device(st);
+  const int dev = current_device(st);
   auto vec4 = [](const void* q, int64_t ld, size_t size) {
     return (reinterpret_cast<uintptr_t>(q) % (4 * size)) == 0 && ld % 4 == 0;
   };
@@ -193,10 +299,8 @@ int laya_op_mx8_linear(const laya_mx8_linear* p, int* err, void* stream) {
   if (p->out_dtype != LAYA_DTYPE_MX8) a.out_vec = vec4(p->out, p->ldo, dtype_size(p->out_dtype));
   a.err = err;
   a.wait_ns = wait_ns();
-  const dim3 grid((N + kMxSimpleTile - 1) / kMxSimpleTile, (M + kMxSimpleTile - 1) / kMxSimpleTile);
-  if (grid.y > 65535) fail(LAYA_ERR_INVALID, "too many rows: %d", M);
-  if (gated) launch_k(mx8_linear_simple_kernel<true>, grid, dim3(256), 0, st, a);
-  else launch_k(mx8_linear_simple_kernel<false>, grid, dim3(256), 0, st, a);
+  if (gated) launch_linear<true>(a, dev, st);
+  else launch_linear<false>(a, dev, st);
   MX_API_END
 }
 

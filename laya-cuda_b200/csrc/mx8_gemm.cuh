@@ -1,0 +1,511 @@
+// tcgen05 products of MX8 matrices (tcgen05.mma kind::mxf8f6f4 with block scales in tensor memory)
+// with the layer's epilogue (mx8_linear.cuh).
+//
+// Operands are K-major E4M3 tiles of 128 columns (128-byte swizzle, four MMAs of K = 32 each), read by
+// TMA; the scale tiles of mx8.cuh travel beside them (512 bytes per 128 rows) and are copied into
+// tensor memory by tcgen05.cp (32 lanes x 16 bytes, repeated for the four lane quarters), where an
+// MMA takes byte k of each 32-bit column for its k-th block of 32.  No copy is multicast.
+#pragma once
+#include "mx8_linear.cuh"
+
+namespace laya {
+
+constexpr int kMxBK = 128;                 // columns of K per stage, one scale tile
+constexpr int kMxOperandBytes = 128 * kMxBK;
+
+struct MxMaps {
+  CUtensorMap x, xs, w, ws, g, gs;  // values {128 columns, rows}, scales {512 bytes, 1, tiles}; g, gs: gated only
+};
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y,
+                                                 int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// Instruction descriptor of kind::mxf8f6f4: E4M3 operands, both K-major, E8M0 scales; `k` selects
+// the byte of the scale columns.
+__host__ __device__ constexpr uint32_t mx_idesc(int M, int N, int k) {
+  return ((uint32_t)k << 4) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24) | ((uint32_t)k << 29);
+}
+
+// Shared-memory descriptor of a scale tile: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t mx_scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFF) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+
+template <bool kPair>
+__device__ __forceinline__ void mx_copy_scales(uint32_t taddr, uint32_t saddr) {
+  const uint64_t d = mx_scale_desc(saddr);
+  if (kPair) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+template <bool kPair>
+__device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
+                                       uint32_t b_scales, uint32_t accumulate) {
+  if (kPair)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(a_scales), "r"(b_scales)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(a_scales), "r"(b_scales)
+        : "memory");
+}
+
+// A warp's 32 x 32 fp32 staging block (rows of 128 bytes, 16-byte pieces swizzled by row): lanes
+// write the tile row that tensor memory gives them and read four columns of rows 4k + lane / 8.
+__device__ __forceinline__ void mx_stage_put(uint8_t* buf, int lane, const uint32_t (&v)[32]) {
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+        make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  __syncwarp();
+}
+__device__ __forceinline__ void mx_stage_get(const uint8_t* buf, int lane, float (&v)[8][4]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int r = 4 * k + (lane >> 3);
+    const float4 t = *reinterpret_cast<const float4*>(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+    v[k][0] = t.x; v[k][1] = t.y; v[k][2] = t.z; v[k][3] = t.w;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Many rows: CTA pairs (cta_group::2), 256 x BN output tiles, persistent.  Each CTA holds its
+// 128 rows of X, half of the tile's rows of W (gated: rank 0 the rows of G and rank 1 those of W, the
+// tile's output being 256 x BN / 2), its X scales and all of the tile's weight scales.
+//
+// Warps: 0 TMA producer, 1 tensor-memory allocator and (in the leader) MMA issuer, 2..9 epilogue (two
+// per lane quarter, each with half of the columns).  Tensor memory: two accumulators, so that the
+// epilogue of a tile overlaps the next tile's MMAs, and two sets of scale columns.  With BN = 256
+// the accumulators take 2 x 256 of the 512 columns and would leave none for the scales, so they
+// share 32 columns, [224, 256): the epilogue reads those first and the next tile's MMAs wait for
+// that (barrier `shared`) instead of for half of the tile's columns.
+//
+// Barriers as in gemm_pair_kernel: full[s] in the leader (both CTAs' copies), empty[s] and
+// tfull[a] in both (committed by the leader), tempty[a] and shared in the leader.
+// ---------------------------------------------------------------------------------------------
+constexpr int kMxThreadsPair = 320;
+constexpr int kMxEpiWarps = 8;
+constexpr int kMxEpiBytes = kMxEpiWarps * 4096;
+
+template <int BN>
+struct MxPairCfg {
+  static constexpr int kStageB = BN / 2 * kMxBK;
+  static constexpr int kWeightTiles = (BN + 127) / 128;  // scale tiles of the weight rows
+  static constexpr int kStageScales = (1 + kWeightTiles) * kMxTileBytes;
+  static constexpr int kStageBytes = kMxOperandBytes + kStageB + kStageScales;
+  static constexpr int kStages = (196 * 1024 - 1024) / kStageBytes;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kMxEpiBytes + 1024 /*align*/ + 512 /*barriers*/;
+  static constexpr uint32_t kAcc1 = BN == 256 ? 224 : BN;  // column of the second accumulator
+  static constexpr bool kShared = kAcc1 < BN;
+  static constexpr uint32_t kScales = 480;                  // two sets of 16 columns
+  static_assert(kAcc1 + BN <= kScales, "accumulators and scale columns overlap");
+};
+
+template <int BN, bool kGated>
+__global__ void __launch_bounds__(kMxThreadsPair, 1)
+    mx8_linear_pair_kernel(const __grid_constant__ MxMaps maps, const __grid_constant__ MxLinearArgs args) {
+  using Cfg = MxPairCfg<BN>;
+  static_assert(!kGated || BN == 256, "gated tiles pair 128 rows of G with 128 of W");
+  constexpr int S = Cfg::kStages;
+  constexpr int kOutCols = kGated ? BN / 2 : BN;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + S * kMxOperandBytes;
+  uint8_t* epi = sB + S * Cfg::kStageB;
+  uint8_t* sS = epi + kMxEpiBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sS + S * Cfg::kStageScales);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + S;
+  uint64_t* tfull = bars + 2 * S;
+  uint64_t* tempty = bars + 2 * S + 2;
+  uint64_t* shared = bars + 2 * S + 4;
+  uint64_t* drain = bars + 2 * S + 5;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 6);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* issued_blocks = abort_flag + 1;  // [2]: k-blocks whose copies each CTA of the pair issued
+  const unsigned long long wait_ns = wait_limit(args.wait_ns);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  const int m_blocks = (args.M + 255) / 256;
+  const int n_blocks = (args.N + kOutCols - 1) / kOutCols;
+  const int k_blocks = (args.K + kMxBK - 1) / kMxBK;
+  const int tiles = m_blocks * n_blocks;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], 2 * kMxEpiWarps); }
+    mbar_init(shared, kMxEpiWarps);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    issued_blocks[0] = issued_blocks[1] = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&maps.x); tma_prefetch_desc(&maps.xs);
+    tma_prefetch_desc(&maps.w); tma_prefetch_desc(&maps.ws);
+    if (kGated) { tma_prefetch_desc(&maps.g); tma_prefetch_desc(&maps.gs); }
+  }
+  if (warp == 1) { tmem_alloc_pair(tmem_slot, 512); tmem_relinquish_pair(); }
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers initialised before any cross-CTA arrival
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0; uint32_t phase = 0;
+      uint32_t issued = 0, last_par = 0;
+      int count = 0;
+      bool ok = true;
+      const CUtensorMap* wmap = kGated && leader ? &maps.g : &maps.w;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        const int mb = t / n_blocks, nb = t - mb * n_blocks;
+        const int arow = mb * 256 + (int)rank * 128;
+        const int brow = kGated ? nb * 128 : nb * BN + (int)rank * (BN / 2);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, args.err, kErrGemmProducerWait, abort_flag, wait_ns)) { ok = false; break; }
+          const uint32_t bar = cluster_addr(smem_u32(&full[stage]), 0);
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::kStageBytes);
+          uint8_t* sc = sS + stage * Cfg::kStageScales;
+          tma_load_2d_pair(sA + stage * kMxOperandBytes, &maps.x, bar, kb * kMxBK, arow);
+          tma_load_2d_pair(sB + stage * Cfg::kStageB, wmap, bar, kb * kMxBK, brow);
+          tma_load_3d_pair(sc, &maps.xs, bar, 0, kb, arow / 128);
+          if (kGated) {
+            tma_load_3d_pair(sc + kMxTileBytes, &maps.gs, bar, 0, kb, nb);
+            tma_load_3d_pair(sc + 2 * kMxTileBytes, &maps.ws, bar, 0, kb, nb);
+          } else {
+            tma_load_3d_pair(sc + kMxTileBytes, &maps.ws, bar, 0, kb, nb * Cfg::kWeightTiles);
+          }
+          ++count;
+          issued |= 1u << stage;
+          last_par = (last_par & ~(1u << stage)) | (phase << stage);
+          if (++stage == S) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (leader) {
+        // Both CTAs' copies complete on the leader's full barriers: wait for them by time only, on
+        // every path, so that nothing is still landing when the pair exits.
+        for (int s = 0; s < S; ++s)
+          if (issued & (1u << s)) mbar_drain(&full[s], (last_par >> s) & 1);
+      }
+      issued_blocks[rank] = count;
+      const uint32_t there = cluster_addr(smem_u32(const_cast<int*>(issued_blocks + rank)), rank ^ 1);
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(count) : "memory");
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      int stage = 0; uint32_t phase = 0;
+      int set = 0;
+      bool ok = true;
+      int i = 0;  // this pair's tile
+      int done_stage = 0; uint32_t done_phase = 0;  // the k-block two before the current one
+      int blocks = 0;
+      for (int t = pair; t < tiles && ok; t += pairs, ++i) {
+        const int acc = i & 1;
+        if (!mbar_wait(&tempty[acc], ((i >> 1) & 1) ^ 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+        if (Cfg::kShared && i > 0 && !mbar_wait(shared, (i - 1) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d = tmem + (acc ? Cfg::kAcc1 : 0);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&full[stage], phase, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+          // The scale columns of this set were last read by the MMAs two k-blocks ago.
+          if (blocks >= 2) {
+            if (!mbar_wait(&empty[done_stage], done_phase, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+            if (++done_stage == S) { done_stage = 0; done_phase ^= 1; }
+          }
+          ++blocks;
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + stage * kMxOperandBytes);
+          const uint32_t b0 = smem_u32(sB + stage * Cfg::kStageB);
+          const uint32_t s0 = smem_u32(sS + stage * Cfg::kStageScales);
+          const uint32_t ts = tmem + Cfg::kScales + set * 16;
+          mx_copy_scales<true>(ts, s0);
+#pragma unroll
+          for (int j = 0; j < Cfg::kWeightTiles; ++j) mx_copy_scales<true>(ts + 4 + 4 * j, s0 + (1 + j) * kMxTileBytes);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mx_mma<true>(d, smem_desc_sw128(a0 + k * 32), smem_desc_sw128(b0 + k * 32), mx_idesc(256, BN, k), ts, ts + 4,
+                         (kb > 0 || k > 0) ? 1u : 0u);
+          const uint32_t e = smem_u32(&empty[stage]);
+          tc_commit_pair(cluster_addr(e, 0));
+          tc_commit_pair(cluster_addr(e, 1));
+          set ^= 1;
+          if (++stage == S) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        const uint32_t f = smem_u32(&tfull[acc]);
+        tc_commit_pair(cluster_addr(f, 0));
+        tc_commit_pair(cluster_addr(f, 1));
+      }
+      tc_commit_pair(cluster_addr(smem_u32(drain), 0));
+      mbar_drain(drain, 0);
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* buf = epi + (warp - 2) * 4096;
+    const uint32_t bar_shared = cluster_addr(smem_u32(shared), 0);
+    constexpr int kChunks = kOutCols / 64;  // 32-column chunks of this warp
+    int i = 0;
+    for (int t = pair; t < tiles; t += pairs, ++i) {
+      const int acc = i & 1;
+      const int mb = t / n_blocks, nb = t - mb * n_blocks;
+      const int row0 = mb * 256 + (int)rank * 128 + quarter * 32;
+      if (!mbar_wait(&tfull[acc], (i >> 1) & 1, args.err, kErrGemmEpilogueWait, abort_flag, wait_ns)) break;
+      tc_fence_after();
+      const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (acc ? Cfg::kAcc1 : 0);
+#pragma unroll 1
+      for (int j = 0; j < kChunks; ++j) {
+        // Outwards in: the shared columns are the second half's last of accumulator 0 and the first half's first of accumulator 1.
+        const int c = half ? 2 * kChunks - 1 - j : j;
+        float v[8][4], g[8][4];
+        if (kGated) {
+          uint32_t r[32], u[32];
+          tmem_ld32_async(tbase + c * 32, r);
+          tmem_ld32_async(tbase + 128 + c * 32, u);
+          tmem_wait_ld(r);
+          tmem_wait_ld(u);
+          mx_stage_put(buf, lane, r);
+          mx_stage_get(buf, lane, g);
+          mx_stage_put(buf, lane, u);
+          mx_stage_get(buf, lane, v);
+        } else {
+          uint32_t r[32];
+          tmem_ld32_async(tbase + c * 32, r);
+          tmem_wait_ld(r);
+          mx_stage_put(buf, lane, r);
+          mx_stage_get(buf, lane, v);
+        }
+        if (j == 0 && Cfg::kShared && half != acc) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(bar_shared);
+        }
+        if (j == kChunks - 1) {
+          // The accumulator has been read; the stores that follow need no ordering with the next MMAs.
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(cluster_addr(smem_u32(&tempty[acc]), 0));
+        }
+        mx_finish<kGated, 8>(args, row0 + (lane >> 3), 4, nb * kOutCols + c * 32 + 4 * (lane & 7), v, g);
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();  // both CTAs done with tensor memory and with the peer's barriers
+  tc_fence_after();
+  if (issued_blocks[0] != issued_blocks[1]) {
+    // One CTA gave up on a wait before the other.  Copies that the peer issued for stages the
+    // leader never armed still land on the leader's barriers: arm those and wait (by time only).
+    if (leader && threadIdx.x == 0)
+      for (int b = issued_blocks[0]; b < issued_blocks[1]; ++b) {
+        mbar_arrive_expect_tx(&full[b % S], Cfg::kStageBytes);
+        mbar_drain(&full[b % S], (b / S) & 1);
+      }
+    __syncwarp();
+    cluster_sync();
+  }
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Few rows: the weights are the 128-row operand and the tokens the BN-column one, so a tile is 128
+// features x BN rows of X and reads each weight byte once.  The K tiles are split over the CTAs of a
+// cluster (as many as keep the SMs busy); each CTA leaves its partial sums in shared memory, and
+// every CTA adds and finishes its share of the rows from all of them in rank order, so the result
+// does not depend on timing.
+//
+// Warps: 0..3 read tensor memory and finish rows, 4 TMA producer, 5 tensor-memory allocator and MMA
+// issuer.
+// ---------------------------------------------------------------------------------------------
+constexpr int kMxThreadsFew = 192;
+constexpr int kMxMaxSplit = 8;
+
+template <int BN, bool kGated>
+struct MxFewCfg {
+  static constexpr int kWeights = kGated ? 2 : 1;
+  static constexpr int kStageB = BN * kMxBK;
+  static constexpr int kStageScales = (kWeights + 1) * kMxTileBytes;
+  static constexpr int kStageBytes = kWeights * kMxOperandBytes + kStageB + kStageScales;
+  static constexpr int kStages = (kGated ? 200 * 1024 : 104 * 1024) / kStageBytes;
+  static constexpr int kPartialBytes = kWeights * BN * 128 * 4;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 1024 /*align*/ + 256 /*barriers*/;
+  static constexpr int kScales = kWeights * BN;  // first scale column, two sets of 12
+  static constexpr int kTmemCols = kScales + 24 <= 64 ? 64 : kScales + 24 <= 128 ? 128 : 256;
+  static_assert(kPartialBytes <= kStages * kStageBytes, "partial sums reuse the stages");
+};
+
+template <int BN, bool kGated>
+__global__ void __launch_bounds__(kMxThreadsFew)
+    mx8_linear_few_kernel(const __grid_constant__ MxMaps maps, const __grid_constant__ MxLinearArgs args) {
+  using Cfg = MxFewCfg<BN, kGated>;
+  constexpr int S = Cfg::kStages;
+  constexpr int W = Cfg::kWeights;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + S * W * kMxOperandBytes;
+  uint8_t* sS = sB + S * Cfg::kStageB;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sS + S * Cfg::kStageScales);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + S;
+  uint64_t* tfull = bars + 2 * S;
+  uint64_t* drain = bars + 2 * S + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* partial = reinterpret_cast<float*>(smem);  // [W][BN][128], over the stages once they are consumed
+  const unsigned long long wait_ns = wait_limit(args.wait_ns);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = (int)gridDim.z, rank = (int)cluster_rank();
+  const int f0 = blockIdx.x * 128, t0 = blockIdx.y * BN;
+  const int k_tiles = (args.K + kMxBK - 1) / kMxBK;
+  const int kb0 = (int)((int64_t)k_tiles * rank / split), kb1 = (int)((int64_t)k_tiles * (rank + 1) / split);
+  const int k_blocks = kb1 - kb0;  // at least 1: split <= k_tiles
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(tfull, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 4 && lane == 0) {
+    tma_prefetch_desc(&maps.x); tma_prefetch_desc(&maps.xs);
+    tma_prefetch_desc(&maps.w); tma_prefetch_desc(&maps.ws);
+    if (kGated) { tma_prefetch_desc(&maps.g); tma_prefetch_desc(&maps.gs); }
+  }
+  if (warp == 5) { tmem_alloc(tmem_slot, Cfg::kTmemCols); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  if (warp == 4) {
+    if (lane == 0) {
+      uint32_t issued = 0, last_par = 0;
+      for (int b = 0; b < k_blocks; ++b) {
+        const int stage = b % S; const uint32_t phase = (b / S) & 1;
+        if (!mbar_wait(&empty[stage], phase ^ 1, args.err, kErrGemmProducerWait, abort_flag, wait_ns)) break;
+        mbar_arrive_expect_tx(&full[stage], Cfg::kStageBytes);
+        const int kb = kb0 + b;
+        uint8_t* sc = sS + stage * Cfg::kStageScales;
+        tma_load_2d(sA + stage * W * kMxOperandBytes, &maps.w, &full[stage], kb * kMxBK, f0);
+        tma_load_3d(sc, &maps.ws, &full[stage], 0, kb, f0 / 128);
+        if (kGated) {
+          tma_load_2d(sA + (stage * W + 1) * kMxOperandBytes, &maps.g, &full[stage], kb * kMxBK, f0);
+          tma_load_3d(sc + kMxTileBytes, &maps.gs, &full[stage], 0, kb, f0 / 128);
+        }
+        tma_load_2d(sB + stage * Cfg::kStageB, &maps.x, &full[stage], kb * kMxBK, t0);
+        tma_load_3d(sc + W * kMxTileBytes, &maps.xs, &full[stage], 0, kb, t0 / 128);
+        issued |= 1u << stage;
+        last_par = (last_par & ~(1u << stage)) | (phase << stage);
+      }
+      for (int s = 0; s < S; ++s)
+        if (issued & (1u << s)) mbar_drain(&full[s], (last_par >> s) & 1);
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int b = 0; b < k_blocks; ++b) {
+        const int stage = b % S;
+        if (!mbar_wait(&full[stage], (b / S) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+        // The scale columns of this set were last read by the MMAs two k-blocks ago.
+        if (b >= 2 && !mbar_wait(&empty[(b - 2) % S], ((b - 2) / S) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t a0 = smem_u32(sA + stage * W * kMxOperandBytes);
+        const uint32_t b0 = smem_u32(sB + stage * Cfg::kStageB);
+        const uint32_t s0 = smem_u32(sS + stage * Cfg::kStageScales);
+        const uint32_t ts = tmem + Cfg::kScales + (b & 1) * 12;
+#pragma unroll
+        for (int j = 0; j <= W; ++j) mx_copy_scales<false>(ts + 4 * j, s0 + j * kMxTileBytes);
+        // Tokens t0 .. t0 + BN - 1 are the lanes from column (t0 % 128) / 32 of their scale tile on.
+        const uint32_t xs = ts + 4 * W + (t0 % 128) / 32;
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mx_mma<false>(tmem + j * BN, smem_desc_sw128(a0 + j * kMxOperandBytes + k * 32), smem_desc_sw128(b0 + k * 32),
+                          mx_idesc(128, BN, k), ts + 4 * j, xs, (b > 0 || k > 0) ? 1u : 0u);
+        tc_commit(&empty[stage]);
+      }
+      if (ok) tc_commit(tfull);
+      tc_commit(drain);
+      mbar_drain(drain, 0);
+    }
+  } else {
+    // This CTA's sums: lane = feature, columns = rows of X.
+    if (mbar_wait(tfull, 0, args.err, kErrGemmEpilogueWait, abort_flag, wait_ns)) {
+      tc_fence_after();
+      const uint32_t tbase = tmem + ((uint32_t)(warp * 32) << 16);
+#pragma unroll
+      for (int c = 0; c < W * BN / 16; ++c) {
+        uint32_t r[16];
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(tbase + c * 16)
+            : "memory");
+#pragma unroll
+        for (int i = 0; i < 16; ++i) partial[(c * 16 + i) * 128 + warp * 32 + lane] = __uint_as_float(r[i]);
+      }
+      tc_fence_before();
+    }
+  }
+  __syncwarp();
+  cluster_sync();  // every CTA's sums are in its shared memory
+  if (warp < 4) {
+    const uint32_t mine = smem_u32(partial);
+    for (int t = rank * 4 + warp; t < BN && t0 + t < args.M; t += 4 * split) {  // one row of X per warp
+      float v[1][4] = {}, g[1][4] = {};
+      for (int r = 0; r < split; ++r) {
+        const uint32_t there = cluster_addr(mine, r) + (t * 128 + lane * 4) * 4;
+        float4 s;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(s.x), "=f"(s.y), "=f"(s.z), "=f"(s.w) : "r"(there));
+        v[0][0] += s.x; v[0][1] += s.y; v[0][2] += s.z; v[0][3] += s.w;
+        if (kGated) {
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(s.x), "=f"(s.y), "=f"(s.z), "=f"(s.w)
+                       : "r"(there + BN * 128 * 4));
+          g[0][0] += s.x; g[0][1] += s.y; g[0][2] += s.z; g[0][3] += s.w;
+        }
+      }
+      mx_finish<kGated, 1>(args, t0 + t, 1, f0 + 4 * lane, v, g);
+    }
+  }
+  __syncwarp();
+  cluster_sync();  // no CTA leaves while its sums are read
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc(tmem, Cfg::kTmemCols);
+}
+
+}  // namespace laya

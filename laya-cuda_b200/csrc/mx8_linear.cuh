@@ -1,4 +1,4 @@
-// Product of MX8 matrices with the layer's epilogue:
+// The MX8 linear layer's arguments and epilogue (the products are in mx8_gemm.cuh):
 //
 //   y = act(X W^T + bias) + residual                        or, gated,
 //   y = act(X G^T + gate_bias) * (X W^T + bias) + residual
@@ -36,15 +36,10 @@ struct MxLinearArgs {
   unsigned long long wait_ns;
 };
 
-__device__ __forceinline__ float mx_activate(float v, int act) {
-  switch (act) {
-    case MX_ACT_RELU: return fmaxf(v, 0.f);
-    case MX_ACT_GELU: return gelu_erf(v);
-    // v / (1 + exp(-v)): exp overflows to infinity for v far below zero, and the quotient to -0.
-    case MX_ACT_SILU: return v * rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * v));
-    default: return v;
-  }
-}
+// v / (1 + exp(-v)): the exponential overflows to infinity for v far below zero, the quotient to -0.
+__device__ __forceinline__ float mx_silu(float v) { return v * rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * v)); }
+// max(v, 0) that keeps a NaN.
+__device__ __forceinline__ float mx_relu(float v) { return v < 0.f ? 0.f : v; }
 
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, int n, bool vec, float* v) {
@@ -75,116 +70,96 @@ __device__ __forceinline__ void store4(T* p, int n, bool vec, const float* v) {
   }
 }
 
-// The epilogue of four accumulators of one row, columns col .. col + 3 (col a multiple of 4).
-// Eight neighbouring threads hold 32 consecutive columns of one row from a multiple of 32 on, and the warp calls
-// this together (an MX8 block's scale is found by shuffles).  Rows and columns outside the
-// result are computed as zeros and not written.  The result is rounded once, here.
-template <bool kGated>
-__device__ __forceinline__ void mx_finish4(const MxLinearArgs& a, int row, int col, const float* acc, const float* gate) {
-  const bool live = row < a.M;
-  const int n = live ? max(0, min(4, a.N - col)) : 0;
-  float v[4], t[4];
+// Epilogue of R rows by four columns per thread: thread's rows row0, row0 + step, ..., columns
+// col .. col + 3 (col a multiple of 4).  Eight neighbouring threads hold 32 consecutive columns
+// of a row from a multiple of 32 on, and the warp calls this together (an MX8 block's scale is
+// found by shuffles).  acc: the products with W, gate: those with G.  Rows and columns outside
+// the result are not read or written.  Everything is fp32 and rounded once, to the output's type.
+template <bool kGated, int R>
+__device__ __forceinline__ void mx_finish(const MxLinearArgs& a, int row0, int step, int col, float (&acc)[R][4],
+                                          float (&gate)[R][4]) {
+  const int n = max(0, min(4, a.N - col));
+  float res[R][4];
+  if (a.residual) {
+    auto read = [&](auto* p) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = acc[i];
+      for (int k = 0; k < R; ++k) {
+        const int row = row0 + k * step;
+        load4(p + (size_t)row * a.ldr + col, row < a.M ? n : 0, a.residual_vec, res[k]);
+      }
+    };
+    if (a.residual_type == MX_BF16) read(static_cast<const __nv_bfloat16*>(a.residual));
+    else if (a.residual_type == MX_F16) read(static_cast<const __half*>(a.residual));
+    else read(static_cast<const float*>(a.residual));
+  }
   if (a.bias) {
+    float t[4];
     load4(a.bias + col, n, true, t);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += t[i];
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[k][i] += t[i];
   }
-  if (kGated) {
-    float g[4];
+  if (kGated && a.gate_bias) {
+    float t[4];
+    load4(a.gate_bias + col, n, true, t);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) g[i] = gate[i];
-    if (a.gate_bias) {
-      load4(a.gate_bias + col, n, true, t);
+    for (int k = 0; k < R; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] += t[i];
+      for (int i = 0; i < 4; ++i) gate[k][i] += t[i];
+  }
+  float(&on)[R][4] = kGated ? gate : acc;
+  auto apply = [&](auto f) {
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const float2 y = f(make_float2(on[k][i], on[k][i + 1]));
+        on[k][i] = y.x;
+        on[k][i + 1] = y.y;
+      }
+  };
+  if (a.act == MX_ACT_GELU) apply([](float2 v) { return gelu_erf2(v); });
+  else if (a.act == MX_ACT_SILU) apply([](float2 v) { return make_float2(mx_silu(v.x), mx_silu(v.y)); });
+  else if (a.act == MX_ACT_RELU) apply([](float2 v) { return make_float2(mx_relu(v.x), mx_relu(v.y)); });
+#pragma unroll
+  for (int k = 0; k < R; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (kGated) acc[k][i] *= gate[k][i];
+      if (a.residual) acc[k][i] += res[k][i];
     }
+  auto write = [&](auto* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= mx_activate(g[i], a.act);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = mx_activate(v[i], a.act);
-  }
-  if (a.residual) {
-    const size_t at = (size_t)row * a.ldr + col;
-    if (a.residual_type == MX_BF16) load4(static_cast<const __nv_bfloat16*>(a.residual) + at, n, a.residual_vec, t);
-    else if (a.residual_type == MX_F16) load4(static_cast<const __half*>(a.residual) + at, n, a.residual_vec, t);
-    else load4(static_cast<const float*>(a.residual) + at, n, a.residual_vec, t);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += t[i];
-  }
-  const size_t at = (size_t)row * a.ldo + col;
-  if (a.out_type == MX_MX8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? v[i] : 0.f;
-    uint32_t m = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-    const uint32_t byte = mx_scale_byte(m);
-    if (live && col < ((a.N + 15) & ~15)) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + at) = mx_pack4(v, byte);
+    for (int k = 0; k < R; ++k) {
+      const int row = row0 + k * step;
+      if (row < a.M) store4(p + (size_t)row * a.ldo + col, n, a.out_vec, acc[k]);
+    }
+  };
+  if (a.out_type == MX_BF16) write(static_cast<__nv_bfloat16*>(a.out));
+  else if (a.out_type == MX_F16) write(static_cast<__half*>(a.out));
+  else if (a.out_type == MX_F32) write(static_cast<float*>(a.out));
+  else {
     const int col_tiles = mx_col_tiles(a.N), col_tile = col / kMxTileCols;
-    if (live && (threadIdx.x & 7) == 0 && col_tile < col_tiles)
-      a.out_scales[mx_scale_tile(row, col_tile, col_tiles) + mx_scale_row(row) + ((col / kMxBlock) & 3)] = (uint8_t)byte;
-  } else if (a.out_type == MX_BF16) {
-    store4(static_cast<__nv_bfloat16*>(a.out) + at, n, a.out_vec, v);
-  } else if (a.out_type == MX_F16) {
-    store4(static_cast<__half*>(a.out) + at, n, a.out_vec, v);
-  } else {
-    store4(static_cast<float*>(a.out) + at, n, a.out_vec, v);
-  }
-}
-
-// ---------------------------------------------------------------------------------------------
-// Product on the fp32 pipe: 64 x 64 tiles, one block of 32 columns of K at a time through shared
-// memory, 4 x 4 sums per thread.
-// ---------------------------------------------------------------------------------------------
-constexpr int kMxSimpleTile = 64;
-
-__device__ __forceinline__ void mx_stage(const MxOperand& m, int row0, int rows, int k, int K, float (*s)[kMxSimpleTile + 4]) {
-  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8, row = row0 + r;
-  float v[8];
+    const bool in_values = col < ((a.N + 15) & ~15), in_scales = (threadIdx.x & 7) == 0 && col_tile < col_tiles;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  if (row < rows && k + c < K) {
-    const uint2 q = *reinterpret_cast<const uint2*>(m.q + (size_t)row * m.ld + k + c);
-    const float f = mx_scale(m.scales[mx_scale_tile(row, k / kMxTileCols, mx_col_tiles(K)) + mx_scale_row(row) + ((k / kMxBlock) & 3)]);
-    mx_unpack4(q.x, v);
-    mx_unpack4(q.y, v + 4);
+    for (int k = 0; k < R; ++k) {
+      const int row = row0 + k * step;
+      float v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + c + i < K ? v[i] * f : 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[c + i][r] = v[i];
-}
-
-template <bool kGated>
-__global__ void __launch_bounds__(256) mx8_linear_simple_kernel(const MxLinearArgs a) {
-  pdl_wait();
-  __shared__ float sx[kMxBlock][kMxSimpleTile + 4], sw[kMxBlock][kMxSimpleTile + 4], sg[kGated ? kMxBlock : 1][kMxSimpleTile + 4];
-  const int m0 = blockIdx.y * kMxSimpleTile, n0 = blockIdx.x * kMxSimpleTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {}, gate[4][4] = {};
-  for (int k = 0; k < a.K; k += kMxBlock) {
-    mx_stage(a.x, m0, a.M, k, a.K, sx);
-    mx_stage(a.w, n0, a.N, k, a.K, sw);
-    if (kGated) mx_stage(a.gate, n0, a.N, k, a.K, sg);
-    __syncthreads();
-#pragma unroll 8
-    for (int i = 0; i < kMxBlock; ++i) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          acc[r][c] = fmaf(sx[i][ty * 4 + r], sw[i][tx * 4 + c], acc[r][c]);
-          if (kGated) gate[r][c] = fmaf(sx[i][ty * 4 + r], sg[i][tx * 4 + c], gate[r][c]);
-        }
+      for (int i = 0; i < 4; ++i) v[i] = i < n ? acc[k][i] : 0.f;
+      uint32_t m = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+      const uint32_t byte = mx_scale_byte(m);
+      if (row < a.M) {
+        if (in_values) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)row * a.ldo + col) = mx_pack4(v, byte);
+        if (in_scales)
+          a.out_scales[mx_scale_tile(row, col_tile, col_tiles) + mx_scale_row(row) + ((col / kMxBlock) & 3)] = (uint8_t)byte;
+      }
     }
-    __syncthreads();
   }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) mx_finish4<kGated>(a, m0 + ty * 4 + r, n0 + tx * 4, acc[r], gate[r]);
 }
 
 }  // namespace laya
