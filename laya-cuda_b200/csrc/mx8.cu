@@ -64,11 +64,13 @@ void check_vector(const char* what, const float* p) {
   if (p && (reinterpret_cast<uintptr_t>(p) & 15)) fail(LAYA_ERR_INVALID, "%s must be 16-byte aligned", what);
 }
 
-// The current device, checked to be `stream`'s.
+// The current device, checked to be `stream`'s.  A stream under capture cannot be asked.
 int current_device(cudaStream_t stream) {
   int dev = 0;
   CK(cudaGetDevice(&dev));
-  if (stream) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (stream) CK(cudaStreamIsCapturing(stream, &capture));
+  if (stream && capture == cudaStreamCaptureStatusNone) {
     int of = -1;
     CK(cudaStreamGetDevice(stream, &of));
     if (of != dev) fail(LAYA_ERR_INVALID, "stream belongs to device %d, the current device is %d", of, dev);
@@ -296,7 +298,7 @@ int laya_op_mx8_linear(const laya_mx8_linear* p, int* err, void* stream) {
   a.residual = p->residual; a.ldr = p->ldr; a.residual_type = p->residual_dtype;
   if (p->residual) a.residual_vec = vec4(p->residual, p->ldr, dtype_size(p->residual_dtype));
   a.out = p->out; a.ldo = p->ldo; a.out_type = p->out_dtype; a.out_scales = static_cast<uint8_t*>(p->out_scales);
-  if (p->out_dtype != LAYA_DTYPE_MX8) a.out_vec = vec4(p->out, p->ldo, dtype_size(p->out_dtype));
+  a.out_vec = p->out_dtype == LAYA_DTYPE_MX8 || vec4(p->out, p->ldo, dtype_size(p->out_dtype));
   a.err = err;
   a.wait_ns = wait_ns();
   if (gated) launch_linear<true>(a, dev, st);

@@ -13,6 +13,44 @@ namespace laya {
 constexpr int kMxBK = 128;                 // columns of K per stage, one scale tile
 constexpr int kMxOperandBytes = 128 * kMxBK;
 
+// One thread of a converged warp.  Instructions that take uniform registers (tcgen05.*, TMA) are
+// issued under this predicate, which the compiler knows to leave one thread: under a test of the
+// lane's number it serialises each of them over the active lanes (measured in the pair kernel: 575
+// cycles to issue a k-block's 3 scale copies, 4 MMAs and 2 commits, and 1,000 cycles a k-block
+// in all against 512 of MMA time).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t leader;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+  return leader != 0;
+}
+
+// mbar_wait for a converged warp, with the same answer in every lane.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code, volatile int* abort,
+                                          unsigned long long limit_ns) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const unsigned long long start = global_ns();
+  for (;;) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const bool given_up = *abort != 0, late = global_ns() - start > limit_ns;
+    if (__any_sync(0xffffffffu, given_up || late)) {
+      if (late && !given_up) {
+        *abort = 1;
+        if (err) atomicCAS(err, 0, code);
+      }
+      __syncwarp();
+      return false;
+    }
+  }
+}
+
+// tc_commit_pair onto the barrier at the same offset in both CTAs of the pair.
+__device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
 struct MxMaps {
   CUtensorMap x, xs, w, ws, g, gs;  // values {128 columns, rows}, scales {512 bytes, 1, tiles}; g, gs: gated only
 };
@@ -45,8 +83,7 @@ __device__ __forceinline__ uint64_t mx_scale_desc(uint32_t saddr) {
 }
 
 template <bool kPair>
-__device__ __forceinline__ void mx_copy_scales(uint32_t taddr, uint32_t saddr) {
-  const uint64_t d = mx_scale_desc(saddr);
+__device__ __forceinline__ void mx_copy_scales(uint32_t taddr, uint64_t d) {
   if (kPair) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
   else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
@@ -145,7 +182,7 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
   volatile int* issued_blocks = abort_flag + 1;  // [2]: k-blocks whose copies each CTA of the pair issued
   const unsigned long long wait_ns = wait_limit(args.wait_ns);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -177,18 +214,18 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
   pdl_wait();
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0; uint32_t phase = 0;
-      uint32_t issued = 0, last_par = 0;
-      int count = 0;
-      bool ok = true;
-      const CUtensorMap* wmap = kGated && leader ? &maps.g : &maps.w;
-      for (int t = pair; t < tiles && ok; t += pairs) {
-        const int mb = t / n_blocks, nb = t - mb * n_blocks;
-        const int arow = mb * 256 + (int)rank * 128;
-        const int brow = kGated ? nb * 128 : nb * BN + (int)rank * (BN / 2);
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, args.err, kErrGemmProducerWait, abort_flag, wait_ns)) { ok = false; break; }
+    int stage = 0; uint32_t phase = 0;
+    uint32_t issued = 0, last_par = 0;
+    int count = 0;
+    bool ok = true;
+    const CUtensorMap* wmap = kGated && leader ? &maps.g : &maps.w;
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      const int mb = t / n_blocks, nb = t - mb * n_blocks;
+      const int arow = mb * 256 + (int)rank * 128;
+      const int brow = kGated ? nb * 128 : nb * BN + (int)rank * (BN / 2);
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        if (!warp_wait(&empty[stage], phase ^ 1, args.err, kErrGemmProducerWait, abort_flag, wait_ns)) { ok = false; break; }
+        if (elect_one()) {
           const uint32_t bar = cluster_addr(smem_u32(&full[stage]), 0);
           if (leader) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::kStageBytes);
           uint8_t* sc = sS + stage * Cfg::kStageScales;
@@ -201,12 +238,14 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
           } else {
             tma_load_3d_pair(sc + kMxTileBytes, &maps.ws, bar, 0, kb, nb * Cfg::kWeightTiles);
           }
-          ++count;
-          issued |= 1u << stage;
-          last_par = (last_par & ~(1u << stage)) | (phase << stage);
-          if (++stage == S) { stage = 0; phase ^= 1; }
         }
+        ++count;
+        issued |= 1u << stage;
+        last_par = (last_par & ~(1u << stage)) | (phase << stage);
+        if (++stage == S) { stage = 0; phase ^= 1; }
       }
+    }
+    if (lane == 0) {
       if (leader) {
         // Both CTAs' copies complete on the leader's full barriers: wait for them by time only, on
         // every path, so that nothing is still landing when the pair exits.
@@ -218,7 +257,9 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
       asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(count) : "memory");
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
+      const uint64_t adesc = smem_desc_sw128(smem_u32(sA)), bdesc = smem_desc_sw128(smem_u32(sB));
+      const uint64_t sdesc = mx_scale_desc(smem_u32(sS));
       int stage = 0; uint32_t phase = 0;
       int set = 0;
       bool ok = true;
@@ -227,43 +268,42 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
       int blocks = 0;
       for (int t = pair; t < tiles && ok; t += pairs, ++i) {
         const int acc = i & 1;
-        if (!mbar_wait(&tempty[acc], ((i >> 1) & 1) ^ 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
-        if (Cfg::kShared && i > 0 && !mbar_wait(shared, (i - 1) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+        if (!warp_wait(&tempty[acc], ((i >> 1) & 1) ^ 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+        if (Cfg::kShared && i > 0 && !warp_wait(shared, (i - 1) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d = tmem + (acc ? Cfg::kAcc1 : 0);
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait(&full[stage], phase, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+          if (!warp_wait(&full[stage], phase, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
           // The scale columns of this set were last read by the MMAs two k-blocks ago.
           if (blocks >= 2) {
-            if (!mbar_wait(&empty[done_stage], done_phase, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+            if (!warp_wait(&empty[done_stage], done_phase, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
             if (++done_stage == S) { done_stage = 0; done_phase ^= 1; }
           }
           ++blocks;
           tc_fence_after();
-          const uint32_t a0 = smem_u32(sA + stage * kMxOperandBytes);
-          const uint32_t b0 = smem_u32(sB + stage * Cfg::kStageB);
-          const uint32_t s0 = smem_u32(sS + stage * Cfg::kStageScales);
-          const uint32_t ts = tmem + Cfg::kScales + set * 16;
-          mx_copy_scales<true>(ts, s0);
+          if (elect_one()) {
+            const uint64_t a = adesc + (uint64_t)(stage * (kMxOperandBytes >> 4));
+            const uint64_t b = bdesc + (uint64_t)(stage * (Cfg::kStageB >> 4));
+            const uint64_t sc = sdesc + (uint64_t)(stage * (Cfg::kStageScales >> 4));
+            const uint32_t ts = tmem + Cfg::kScales + set * 16;
+            mx_copy_scales<true>(ts, sc);
 #pragma unroll
-          for (int j = 0; j < Cfg::kWeightTiles; ++j) mx_copy_scales<true>(ts + 4 + 4 * j, s0 + (1 + j) * kMxTileBytes);
+            for (int j = 0; j < Cfg::kWeightTiles; ++j) mx_copy_scales<true>(ts + 4 + 4 * j, sc + (1 + j) * (kMxTileBytes >> 4));
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mx_mma<true>(d, smem_desc_sw128(a0 + k * 32), smem_desc_sw128(b0 + k * 32), mx_idesc(256, BN, k), ts, ts + 4,
-                         (kb > 0 || k > 0) ? 1u : 0u);
-          const uint32_t e = smem_u32(&empty[stage]);
-          tc_commit_pair(cluster_addr(e, 0));
-          tc_commit_pair(cluster_addr(e, 1));
+            for (int k = 0; k < 4; ++k)
+              mx_mma<true>(d, a + 2 * k, b + 2 * k, mx_idesc(256, BN, k), ts, ts + 4, (kb > 0 || k > 0) ? 1u : 0u);
+            tc_commit_both(&empty[stage]);
+            if (kb == k_blocks - 1) tc_commit_both(&tfull[acc]);
+          }
+          __syncwarp();
           set ^= 1;
           if (++stage == S) { stage = 0; phase ^= 1; }
         }
-        if (!ok) break;
-        const uint32_t f = smem_u32(&tfull[acc]);
-        tc_commit_pair(cluster_addr(f, 0));
-        tc_commit_pair(cluster_addr(f, 1));
       }
-      tc_commit_pair(cluster_addr(smem_u32(drain), 0));
-      mbar_drain(drain, 0);
+      if (elect_one()) {
+        tc_commit_pair(cluster_addr(smem_u32(drain), 0));
+        mbar_drain(drain, 0);
+      }
     }
   } else {
     const int quarter = warp & 3, half = (warp - 2) >> 2;
@@ -275,31 +315,39 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
       const int acc = i & 1;
       const int mb = t / n_blocks, nb = t - mb * n_blocks;
       const int row0 = mb * 256 + (int)rank * 128 + quarter * 32;
-      if (!mbar_wait(&tfull[acc], (i >> 1) & 1, args.err, kErrGemmEpilogueWait, abort_flag, wait_ns)) break;
+      // Outwards in: the shared columns are the second half's last of accumulator 0 and the first
+      // half's first of accumulator 1.
+      auto chunk = [&](int j) { return half ? 2 * kChunks - 1 - j : j; };
+      auto fetch = [&](int j, MxInputs<8>& in) {
+        const int c0 = nb * kOutCols + chunk(j) * 32;
+        mx_fetch<kGated, 8>(args, row0 + (lane >> 3), 4, c0 + 4 * (lane & 7), row0 + 32 <= args.M && c0 + 32 <= args.N, in);
+      };
+      // The first chunk's inputs are loaded while the tile's MMAs run; the other chunks' residual is
+      // brought into L2 then and loaded one chunk ahead of its use.
+      MxInputs<8> in;
+      fetch(0, in);
+      if (args.residual && row0 + lane < args.M) {
+        const int size = args.residual_type == MX_F32 ? 4 : 2;
+        const char* r = static_cast<const char*>(args.residual) + (size_t)(row0 + lane) * args.ldr * size;
+#pragma unroll
+        for (int j = 1; j < kChunks; ++j) {
+          const int c0 = nb * kOutCols + chunk(j) * 32;
+          if (c0 < args.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(r + (size_t)c0 * size));
+        }
+      }
+      if (!warp_wait(&tfull[acc], (i >> 1) & 1, args.err, kErrGemmEpilogueWait, abort_flag, wait_ns)) break;
       tc_fence_after();
       const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (acc ? Cfg::kAcc1 : 0);
 #pragma unroll 1
       for (int j = 0; j < kChunks; ++j) {
-        // Outwards in: the shared columns are the second half's last of accumulator 0 and the first half's first of accumulator 1.
-        const int c = half ? 2 * kChunks - 1 - j : j;
-        float v[8][4], g[8][4];
-        if (kGated) {
-          uint32_t r[32], u[32];
-          tmem_ld32_async(tbase + c * 32, r);
+        const int c = chunk(j);
+        uint32_t r[32], u[kGated ? 32 : 1];
+        tmem_ld32_async(tbase + c * 32, r);
+        if constexpr (kGated) {
           tmem_ld32_async(tbase + 128 + c * 32, u);
-          tmem_wait_ld(r);
           tmem_wait_ld(u);
-          mx_stage_put(buf, lane, r);
-          mx_stage_get(buf, lane, g);
-          mx_stage_put(buf, lane, u);
-          mx_stage_get(buf, lane, v);
-        } else {
-          uint32_t r[32];
-          tmem_ld32_async(tbase + c * 32, r);
-          tmem_wait_ld(r);
-          mx_stage_put(buf, lane, r);
-          mx_stage_get(buf, lane, v);
         }
+        tmem_wait_ld(r);
         if (j == 0 && Cfg::kShared && half != acc) {
           tc_fence_before();
           __syncwarp();
@@ -311,7 +359,15 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster_relaxed(cluster_addr(smem_u32(&tempty[acc]), 0));
         }
-        mx_finish<kGated, 8>(args, row0 + (lane >> 3), 4, nb * kOutCols + c * 32 + 4 * (lane & 7), v, g);
+        float v[8][4], g[8][4];
+        mx_stage_put(buf, lane, r);
+        mx_stage_get(buf, lane, kGated ? g : v);
+        if constexpr (kGated) {
+          mx_stage_put(buf, lane, u);
+          mx_stage_get(buf, lane, v);
+        }
+        mx_finish<kGated, 8>(args, row0 + (lane >> 3), 4, nb * kOutCols + c * 32 + 4 * (lane & 7), v, g, in);
+        if (j + 1 < kChunks) fetch(j + 1, in);
       }
     }
   }
@@ -356,8 +412,11 @@ struct MxFewCfg {
   static constexpr int kStages = (kGated ? 200 * 1024 : 104 * 1024) / kStageBytes;
   static constexpr int kPartialBytes = kWeights * BN * 128 * 4;
   static constexpr int kSmemBytes = kStages * kStageBytes + 1024 /*align*/ + 256 /*barriers*/;
-  static constexpr int kScales = kWeights * BN;  // first scale column, two sets of 12
-  static constexpr int kTmemCols = kScales + 24 <= 64 ? 64 : kScales + 24 <= 128 ? 128 : 256;
+  static constexpr int kScaleCols = 4 * (kWeights + 1);
+  static constexpr int kScales = kWeights * BN;  // first scale column, a set per stage
+  static constexpr int kUsedCols = kScales + kStages * kScaleCols;
+  static constexpr int kTmemCols = kUsedCols <= 64 ? 64 : kUsedCols <= 128 ? 128 : 256;
+  static_assert(kUsedCols <= 256, "two CTAs share an SM's tensor memory");
   static_assert(kPartialBytes <= kStages * kStageBytes, "partial sums reuse the stages");
 };
 
@@ -382,7 +441,7 @@ __global__ void __launch_bounds__(kMxThreadsFew)
   float* partial = reinterpret_cast<float*>(smem);  // [W][BN][128], over the stages once they are consumed
   const unsigned long long wait_ns = wait_limit(args.wait_ns);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int split = (int)gridDim.z, rank = (int)cluster_rank();
   const int f0 = blockIdx.x * 128, t0 = blockIdx.y * BN;
   const int k_tiles = (args.K + kMxBK - 1) / kMxBK;
@@ -409,11 +468,11 @@ __global__ void __launch_bounds__(kMxThreadsFew)
   pdl_wait();
 
   if (warp == 4) {
-    if (lane == 0) {
-      uint32_t issued = 0, last_par = 0;
-      for (int b = 0; b < k_blocks; ++b) {
-        const int stage = b % S; const uint32_t phase = (b / S) & 1;
-        if (!mbar_wait(&empty[stage], phase ^ 1, args.err, kErrGemmProducerWait, abort_flag, wait_ns)) break;
+    uint32_t issued = 0, last_par = 0;
+    for (int b = 0; b < k_blocks; ++b) {
+      const int stage = b % S; const uint32_t phase = (b / S) & 1;
+      if (!warp_wait(&empty[stage], phase ^ 1, args.err, kErrGemmProducerWait, abort_flag, wait_ns)) break;
+      if (elect_one()) {
         mbar_arrive_expect_tx(&full[stage], Cfg::kStageBytes);
         const int kb = kb0 + b;
         uint8_t* sc = sS + stage * Cfg::kStageScales;
@@ -425,44 +484,48 @@ __global__ void __launch_bounds__(kMxThreadsFew)
         }
         tma_load_2d(sB + stage * Cfg::kStageB, &maps.x, &full[stage], kb * kMxBK, t0);
         tma_load_3d(sc + W * kMxTileBytes, &maps.xs, &full[stage], 0, kb, t0 / 128);
-        issued |= 1u << stage;
-        last_par = (last_par & ~(1u << stage)) | (phase << stage);
       }
+      issued |= 1u << stage;
+      last_par = (last_par & ~(1u << stage)) | (phase << stage);
+    }
+    if (lane == 0)
       for (int s = 0; s < S; ++s)
         if (issued & (1u << s)) mbar_drain(&full[s], (last_par >> s) & 1);
-    }
   } else if (warp == 5) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int b = 0; b < k_blocks; ++b) {
-        const int stage = b % S;
-        if (!mbar_wait(&full[stage], (b / S) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
-        // The scale columns of this set were last read by the MMAs two k-blocks ago.
-        if (b >= 2 && !mbar_wait(&empty[(b - 2) % S], ((b - 2) / S) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t a0 = smem_u32(sA + stage * W * kMxOperandBytes);
-        const uint32_t b0 = smem_u32(sB + stage * Cfg::kStageB);
-        const uint32_t s0 = smem_u32(sS + stage * Cfg::kStageScales);
-        const uint32_t ts = tmem + Cfg::kScales + (b & 1) * 12;
+    const uint64_t adesc = smem_desc_sw128(smem_u32(sA)), bdesc = smem_desc_sw128(smem_u32(sB));
+    const uint64_t sdesc = mx_scale_desc(smem_u32(sS));
+    for (int b = 0; b < k_blocks; ++b) {
+      const int stage = b % S;
+      if (!warp_wait(&full[stage], (b / S) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t a = adesc + (uint64_t)(stage * W * (kMxOperandBytes >> 4));
+        const uint64_t x = bdesc + (uint64_t)(stage * (Cfg::kStageB >> 4));
+        const uint64_t sc = sdesc + (uint64_t)(stage * (Cfg::kStageScales >> 4));
+        // The stage's own scale columns: its last MMAs were done before it was filled again.
+        const uint32_t ts = tmem + Cfg::kScales + stage * Cfg::kScaleCols;
 #pragma unroll
-        for (int j = 0; j <= W; ++j) mx_copy_scales<false>(ts + 4 * j, s0 + j * kMxTileBytes);
+        for (int j = 0; j <= W; ++j) mx_copy_scales<false>(ts + 4 * j, sc + j * (kMxTileBytes >> 4));
         // Tokens t0 .. t0 + BN - 1 are the lanes from column (t0 % 128) / 32 of their scale tile on.
         const uint32_t xs = ts + 4 * W + (t0 % 128) / 32;
 #pragma unroll
         for (int j = 0; j < W; ++j)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mx_mma<false>(tmem + j * BN, smem_desc_sw128(a0 + j * kMxOperandBytes + k * 32), smem_desc_sw128(b0 + k * 32),
-                          mx_idesc(128, BN, k), ts + 4 * j, xs, (b > 0 || k > 0) ? 1u : 0u);
+            mx_mma<false>(tmem + j * BN, a + j * (kMxOperandBytes >> 4) + 2 * k, x + 2 * k, mx_idesc(128, BN, k), ts + 4 * j, xs,
+                          (b > 0 || k > 0) ? 1u : 0u);
         tc_commit(&empty[stage]);
+        if (b == k_blocks - 1) tc_commit(tfull);
       }
-      if (ok) tc_commit(tfull);
+      __syncwarp();
+    }
+    if (elect_one()) {
       tc_commit(drain);
       mbar_drain(drain, 0);
     }
   } else {
     // This CTA's sums: lane = feature, columns = rows of X.
-    if (mbar_wait(tfull, 0, args.err, kErrGemmEpilogueWait, abort_flag, wait_ns)) {
+    if (warp_wait(tfull, 0, args.err, kErrGemmEpilogueWait, abort_flag, wait_ns)) {
       tc_fence_after();
       const uint32_t tbase = tmem + ((uint32_t)(warp * 32) << 16);
 #pragma unroll
@@ -487,6 +550,8 @@ __global__ void __launch_bounds__(kMxThreadsFew)
     const uint32_t mine = smem_u32(partial);
     for (int t = rank * 4 + warp; t < BN && t0 + t < args.M; t += 4 * split) {  // one row of X per warp
       float v[1][4] = {}, g[1][4] = {};
+      MxInputs<1> in;
+      mx_fetch<kGated, 1>(args, t0 + t, 1, f0 + 4 * lane, f0 + 128 <= args.N, in);
       for (int r = 0; r < split; ++r) {
         const uint32_t there = cluster_addr(mine, r) + (t * 128 + lane * 4) * 4;
         float4 s;
@@ -499,7 +564,7 @@ __global__ void __launch_bounds__(kMxThreadsFew)
           g[0][0] += s.x; g[0][1] += s.y; g[0][2] += s.z; g[0][3] += s.w;
         }
       }
-      mx_finish<kGated, 1>(args, t0 + t, 1, f0 + 4 * lane, v, g);
+      mx_finish<kGated, 1>(args, t0 + t, 1, f0 + 4 * lane, v, g, in);
     }
   }
   __syncwarp();

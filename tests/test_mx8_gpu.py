@@ -454,6 +454,34 @@ def test_one_layer_on_another_stream():
     assert (np.abs(y.double().cpu().numpy() - want) <= slack + 2.0 ** -23 * np.abs(want)).all()
 
 
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_captured_in_a_graph(rows):
+    """The calls can be captured and replayed on new inputs, and give the bits of plain calls."""
+    rng = np.random.default_rng(12)
+    d, f = 192, 256
+    (up, _), (down, _) = (matrix(rng.normal(0, 0.1, s).astype(np.float32)) for s in ((f, d), (d, f)))
+    x, r = (torch.from_numpy(activations(rng, rows, d)).cuda() for _ in range(2))
+    weight = torch.ones(d, device="cuda")
+    n8, a8 = fresh(rows, d), fresh(rows, f)
+    y, back = torch.empty(rows, d, device="cuda"), torch.empty(rows, f, device="cuda")
+
+    def layer(s):
+        mx8.rms_norm(x, weight, n8, residual=r, stream=s)
+        mx8.linear(n8, up, a8, activation="gelu", stream=s)
+        mx8.dequantize(a8, back, stream=s)
+        mx8.quantize(back, a8, stream=s)
+        mx8.linear(a8, down, y, residual=r, stream=s)
+
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        layer(side.cuda_stream)
+    x.mul_(0.5)
+    graph.replay()
+    got = y.clone()
+    layer(torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(got, y) and torch.isfinite(y).all()
+
+
 def test_no_rows_is_no_work():
     w, _ = matrix(np.ones((8, 32), np.float32))
     x = mx8.Matrix.empty(w.values, 0, 32)
