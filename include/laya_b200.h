@@ -314,21 +314,36 @@ int laya_op_gemm_residual_static(int precision, const void* x, const void* w, in
 /* Bytes of the scales of an MX8 matrix; -1 for a bad shape (rows >= 0, cols >= 1). */
 int64_t laya_mx8_scale_bytes(int rows, int cols);
 
-/* x [rows][cols] -> MX8. */
-int laya_op_mx8_quantize(int dtype, const void* x, int64_t ldx, int rows, int cols, void* values, int64_t ldv,
-                         void* scales, void* stream);
+/* Arguments of laya_op_mx8_quantize and laya_op_mx8_dequantize: an MX8 matrix and a matrix of dtype. */
+typedef struct laya_mx8_convert {
+  int32_t rows, cols;
+  int32_t dtype;
+  void* values; void* scales; int64_t ldv;
+  void* data; int64_t ld;        /* [rows][cols] of dtype */
+} laya_mx8_convert;
 
-/* MX8 -> out [rows][cols], value times scale rounded once to dtype (exact in F32 and BF16 unless it
- * leaves their range). */
-int laya_op_mx8_dequantize(const void* values, int64_t ldv, const void* scales, int rows, int cols, int dtype, void* out,
-                           int64_t ldo, void* stream);
+/* data -> MX8. */
+int laya_op_mx8_quantize(const laya_mx8_convert* args, void* stream);
+
+/* MX8 -> data, value times scale rounded once to dtype (exact in F32 and BF16 unless it leaves
+ * their range). */
+int laya_op_mx8_dequantize(const laya_mx8_convert* args, void* stream);
+
+/* Arguments of laya_op_rms_norm_mx8. */
+typedef struct laya_rms_norm_mx8 {
+  int32_t rows, cols;
+  int32_t dtype, residual_dtype;
+  const void* x; int64_t ldx;          /* [rows][cols] of dtype */
+  const void* residual; int64_t ldr;   /* [rows][cols] of residual_dtype, or NULL */
+  void* sum_out; int64_t lds;          /* [rows][cols] of residual_dtype, or NULL; may be residual itself */
+  const float* weight;                 /* fp32 [cols], 16-byte aligned */
+  void* values; void* scales; int64_t ldv;
+  float eps;
+} laya_rms_norm_mx8;
 
 /* h = x + residual; sum_out = h rounded to residual_dtype; y = h / sqrt(mean(h^2) + eps) * weight
- * (from the unrounded h, in fp32), written as MX8.  residual and sum_out may be NULL, and sum_out
- * may be the residual itself.  weight: fp32 [cols], 16-byte aligned. */
-int laya_op_rms_norm_mx8(int dtype, const void* x, int64_t ldx, int residual_dtype, const void* residual, int64_t ldr,
-                         void* sum_out, int64_t lds, const float* weight, float eps, int rows, int cols, void* values,
-                         int64_t ldv, void* scales, void* stream);
+ * (from the unrounded h, in fp32), written as MX8. */
+int laya_op_rms_norm_mx8(const laya_rms_norm_mx8* args, void* stream);
 
 /* Arguments of laya_op_mx8_linear. */
 typedef struct laya_mx8_linear {

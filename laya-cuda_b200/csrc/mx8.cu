@@ -184,6 +184,48 @@ void launch_linear(const MxLinearArgs& a, int dev, cudaStream_t st) {
   launch_pair<256, kGated>(a, dev, st);
 }
 
+// Blocks for `pieces` pieces, `per_block` of them per block and pass and `unroll` passes at once: all
+// that are of use, at most 8 per SM.
+int pieces_grid(int64_t pieces, int per_block, int unroll, int sms) {
+  const int64_t per = (int64_t)per_block * unroll;
+  return (int)std::min<int64_t>((pieces + per - 1) / per, 8LL * sms);
+}
+constexpr int kConvertUnroll = 2;
+
+template <typename T, typename R, int CH, bool kVec>
+void launch_norm_rows(RmsNormArgs a, int sms, cudaStream_t st) {
+  auto kern = rms_norm_mx8_kernel<T, R, CH, kVec>;
+  const int need = (a.cols + 32 * kMxPiece * CH - 1) / (32 * kMxPiece * CH);
+  int log = 0;
+  while ((1 << log) < need) ++log;
+  a.warps = 1 << log;
+  const int warps = std::max(a.warps, 8), per_block = warps / a.warps;
+  int64_t blocks = ((int64_t)a.rows + per_block - 1) / per_block;
+  if (blocks > sms) {
+    static std::atomic<int> resident[8];  // by log, 0: not asked yet
+    int n = resident[log].load(std::memory_order_relaxed);
+    if (!n) {
+      CK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, warps * 32, 0));
+      n = std::max(n, 1);
+      resident[log].store(n, std::memory_order_relaxed);
+    }
+    blocks = std::min<int64_t>(blocks, (int64_t)n * sms);
+  }
+  launch_k(kern, dim3((int)blocks), dim3(warps * 32), 0, st, a);
+}
+
+template <typename T, typename R>
+void launch_norm(const RmsNormArgs& a, int sms, cudaStream_t st) {
+  const bool vec = rows_vectored(static_cast<const T*>(a.x), a.ldx, a.cols) &&
+                   (!a.residual || rows_vectored(static_cast<const R*>(a.residual), a.ldr, a.cols)) &&
+                   (!a.sum_out || rows_vectored(static_cast<const R*>(a.sum_out), a.lds, a.cols));
+  constexpr int kCols = 16 * 32 * kMxPiece;  // 16 warps of one piece per thread
+  if (vec && a.cols <= kCols) launch_norm_rows<T, R, 1, true>(a, sms, st);
+  else if (vec && a.cols <= 2 * kCols) launch_norm_rows<T, R, 2, true>(a, sms, st);
+  else if (a.cols <= kCols) launch_norm_rows<T, R, 1, false>(a, sms, st);
+  else launch_k(rms_norm_mx8_long_kernel<T, R>, dim3(std::min(a.rows, 8 * sms)), dim3(kMxThreads), 0, st, a);
+}
+
 }  // namespace
 
 extern "C" {
@@ -193,72 +235,87 @@ int64_t laya_mx8_scale_bytes(int rows, int cols) {
   return ((int64_t)rows + kMxTileRows - 1) / kMxTileRows * (((int64_t)cols + kMxTileCols - 1) / kMxTileCols) * kMxTileBytes;
 }
 
-int laya_op_mx8_quantize(int dtype, const void* x, int64_t ldx, int rows, int cols, void* q, int64_t ldq, void* scales,
-                         void* stream) {
+int laya_op_mx8_quantize(const laya_mx8_convert* p, void* stream) {
   MX_API_BEGIN
+  if (!p) fail(LAYA_ERR_INVALID, "null argument");
+  const int rows = p->rows, cols = p->cols;
   check_shape(rows, cols);
-  dtype_size(dtype);
+  dtype_size(p->dtype);
   if (!rows) return LAYA_OK;
-  check_rows("x", x, ldx, cols, dtype);
-  check_mx8("out", q, ldq, scales, cols);
+  check_rows("x", p->data, p->ld, cols, p->dtype);
+  check_mx8("out", p->values, p->ldv, p->scales, cols);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sms = sm_count(current_device(st));
   const int64_t groups = (int64_t)rows * mx_col_tiles(cols);
-  const int grid = (int)std::min<int64_t>((groups + 15) / 16, 8LL * sms);
-  with_type(dtype, [&](auto* t) {
+  if (groups > INT32_MAX) fail(LAYA_ERR_INVALID, "%d x %d values are too many for one call", rows, cols);
+  with_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    launch_k(mx8_quantize_kernel<T>, dim3(grid), dim3(kMxThreads), 0, st, static_cast<const T*>(x), ldx, rows, cols,
-             static_cast<uint8_t*>(q), ldq, static_cast<uint8_t*>(scales));
+    const T* x = static_cast<const T*>(p->data);
+    auto go = [&](auto kern, int unroll) {
+      launch_k(kern, dim3(pieces_grid(groups, kMxThreads / 8, unroll, sms)), dim3(kMxThreads), 0, st, x, p->ld, rows, cols,
+               FastDiv((uint32_t)mx_col_tiles(cols)),
+               static_cast<uint8_t*>(p->values), p->ldv, static_cast<uint8_t*>(p->scales));
+    };
+    if (!rows_vectored(x, p->ld, cols)) go(mx8_quantize_kernel<T, false, 1>, 1);
+    else if (groups < 8LL * 32 * sms) go(mx8_quantize_kernel<T, true, 1>, 1);
+    else go(mx8_quantize_kernel<T, true, kConvertUnroll>, kConvertUnroll);
   });
   MX_API_END
 }
 
-int laya_op_mx8_dequantize(const void* q, int64_t ldq, const void* scales, int rows, int cols, int dtype, void* out,
-                           int64_t ldo, void* stream) {
+int laya_op_mx8_dequantize(const laya_mx8_convert* p, void* stream) {
   MX_API_BEGIN
+  if (!p) fail(LAYA_ERR_INVALID, "null argument");
+  const int rows = p->rows, cols = p->cols;
   check_shape(rows, cols);
-  dtype_size(dtype);
+  dtype_size(p->dtype);
   if (!rows) return LAYA_OK;
-  check_mx8("x", q, ldq, scales, cols);
-  check_rows("out", out, ldo, cols, dtype);
+  check_mx8("x", p->values, p->ldv, p->scales, cols);
+  check_rows("out", p->data, p->ld, cols, p->dtype);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sms = sm_count(current_device(st));
-  const int64_t pieces = (int64_t)rows * ((cols + 7) / 8);
-  const int grid = (int)std::min<int64_t>((pieces + kMxThreads - 1) / kMxThreads, 8LL * sms);
-  with_type(dtype, [&](auto* t) {
+  const uint32_t per_row = ((uint32_t)cols + kMxPiece - 1) / kMxPiece;
+  const int64_t pieces = (int64_t)rows * per_row;
+  if (pieces > INT32_MAX) fail(LAYA_ERR_INVALID, "%d x %d values are too many for one call", rows, cols);
+  with_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    launch_k(mx8_dequantize_kernel<T>, dim3(grid), dim3(kMxThreads), 0, st, static_cast<const uint8_t*>(q), ldq,
-             static_cast<const uint8_t*>(scales), rows, cols, static_cast<T*>(out), ldo);
+    T* out = static_cast<T*>(p->data);
+    auto go = [&](auto kern, int unroll) {
+      launch_k(kern, dim3(pieces_grid(pieces, kMxThreads, unroll, sms)), dim3(kMxThreads), 0, st,
+               static_cast<const uint8_t*>(p->values), p->ldv, static_cast<const uint8_t*>(p->scales), rows, cols, FastDiv(per_row), out,
+               p->ld);
+    };
+    if (!rows_vectored(out, p->ld, cols)) go(mx8_dequantize_kernel<T, false, 1>, 1);
+    else if (pieces < 8LL * kMxThreads * sms) go(mx8_dequantize_kernel<T, true, 1>, 1);
+    else go(mx8_dequantize_kernel<T, true, kConvertUnroll>, kConvertUnroll);
   });
   MX_API_END
 }
 
-int laya_op_rms_norm_mx8(int dtype, const void* x, int64_t ldx, int residual_dtype, const void* residual, int64_t ldr,
-                         void* sum_out, int64_t lds, const float* weight, float eps, int rows, int cols, void* q,
-                         int64_t ldq, void* scales, void* stream) {
+int laya_op_rms_norm_mx8(const laya_rms_norm_mx8* p, void* stream) {
   MX_API_BEGIN
+  if (!p) fail(LAYA_ERR_INVALID, "null argument");
+  const int rows = p->rows, cols = p->cols;
   check_shape(rows, cols);
-  dtype_size(dtype);
-  dtype_size(residual_dtype);
-  if (!(eps >= 0.f)) fail(LAYA_ERR_INVALID, "eps must be at least 0");
+  dtype_size(p->dtype);
+  dtype_size(p->residual_dtype);
+  if (!(p->eps >= 0.f)) fail(LAYA_ERR_INVALID, "eps must be at least 0");
   if (!rows) return LAYA_OK;
-  check_rows("x", x, ldx, cols, dtype);
-  if (residual) check_rows("residual", residual, ldr, cols, residual_dtype);
-  if (sum_out) check_rows("sum_out", sum_out, lds, cols, residual_dtype);
-  if (!weight) fail(LAYA_ERR_INVALID, "weight is null");
-  check_vector("weight", weight);
-  check_mx8("out", q, ldq, scales, cols);
+  check_rows("x", p->x, p->ldx, cols, p->dtype);
+  if (p->residual) check_rows("residual", p->residual, p->ldr, cols, p->residual_dtype);
+  if (p->sum_out) check_rows("sum_out", p->sum_out, p->lds, cols, p->residual_dtype);
+  if (!p->weight) fail(LAYA_ERR_INVALID, "weight is null");
+  check_vector("weight", p->weight);
+  check_mx8("out", p->values, p->ldv, p->scales, cols);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sms = sm_count(current_device(st));
   RmsNormArgs a{};
-  a.x = x; a.ldx = ldx; a.residual = residual; a.ldr = ldr; a.sum_out = sum_out; a.lds = lds;
-  a.weight = weight; a.eps = eps; a.rows = rows; a.cols = cols;
-  a.q = static_cast<uint8_t*>(q); a.ldq = ldq; a.scales = static_cast<uint8_t*>(scales);
-  const int grid = std::min(rows, 8 * sms);
-  with_type(dtype, [&](auto* t) {
-    with_type(residual_dtype, [&](auto* r) {
-      launch_k(rms_norm_mx8_kernel<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(r)>>, dim3(grid),
-               dim3(kMxThreads), 0, st, a);
+  a.x = p->x; a.ldx = p->ldx; a.residual = p->residual; a.ldr = p->ldr; a.sum_out = p->sum_out; a.lds = p->lds;
+  a.weight = p->weight; a.eps = p->eps; a.rows = rows; a.cols = cols;
+  a.q = static_cast<uint8_t*>(p->values); a.ldq = p->ldv; a.scales = static_cast<uint8_t*>(p->scales);
+  with_type(p->dtype, [&](auto* t) {
+    with_type(p->residual_dtype, [&](auto* r) {
+      launch_norm<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(r)>>(a, sms, st);
     });
   });
   MX_API_END

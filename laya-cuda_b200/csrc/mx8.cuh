@@ -41,8 +41,10 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax) {
   const int e = (int)(amax >> 23) - 8 + ((amax & 0x7FFFFFu) > 0x600000u ? 1 : 0);
   return (uint32_t)max(e, 0);
 }
-// 2^-e of a finite scale byte (bytes are at most 247, so this is a normal fp32).
-__device__ __forceinline__ float mx_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+// 2^-e of a scale byte (finite ones are at most 247, so this is a normal fp32); NaN for 255.
+__device__ __forceinline__ float mx_inverse(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0x7FC00000u : (254u - byte) << 23);
+}
 // 2^e of a scale byte: 2^-127 is a subnormal fp32, 255 a NaN.
 __device__ __forceinline__ float mx_scale(uint32_t byte) {
   return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
@@ -50,14 +52,22 @@ __device__ __forceinline__ float mx_scale(uint32_t byte) {
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// Four values over their block's scale, rounded to nearest even E4M3 (v[0] in the low byte).
-__device__ __forceinline__ uint32_t mx_pack4(const float* v, uint32_t byte) {
-  if (byte == 255u) return 0x7F7F7F7Fu;
-  const float inv = mx_inverse(byte);
+// Four values times their block's inverse scale, rounded to nearest even E4M3 (v[0] in the low byte;
+// a NaN becomes 0x7F).
+__device__ __forceinline__ uint32_t mx_pack4(const float* v, float inverse) {
+  const float2 f = make_float2(inverse, inverse);
+  const float2 a = mul2(make_float2(v[0], v[1]), f), b = mul2(make_float2(v[2], v[3]), f);
   uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v[1] * inv), "f"(v[0] * inv));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(v[3] * inv), "f"(v[2] * inv));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(a.y), "f"(a.x));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(b.y), "f"(b.x));
   return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+// max(a, |b|, |c|) that keeps a NaN.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+  return d;
 }
 
 // Four E4M3 values as fp32 (exact: every E4M3 value is an fp16 value).
@@ -73,129 +83,260 @@ __device__ __forceinline__ float to_f32(float x) { return x; }
 template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 
 // ---------------------------------------------------------------------------------------------
-// Eight consecutive elements of a row, `n` of them valid (the others read as zeros).  `vec`: the
-// pointer is aligned for whole-vector access and all eight elements are valid.
+// A piece: sixteen consecutive columns of a row, half a block, held by one thread.  Eight columns a
+// thread made the conversions instruction-bound (155 instructions per thread for 8 columns, 52 us
+// for 16384 x 4096 bf16 to MX8); sixteen share the addresses and shuffles.
+//
+// kVec: rows of whole 32-byte vectors (`rows_vectored`), read and written as such; a thread's bf16
+// piece is one of them.  (Two 16-byte stores per thread instead fill half sectors: 48 us against
+// 35 us for 16384 x 4096 back to bf16.)  Otherwise rows of any length and alignment: a piece is read
+// as the aligned 16-byte granules that hold it, shifted into place, and written element by element,
+// through shared memory so that neighbouring lanes write neighbouring elements.
 // ---------------------------------------------------------------------------------------------
+constexpr int kMxPiece = 16;
+
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
-  if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+struct Raw {
+  uint32_t w[4 * sizeof(T)];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* p, bool live) {
+  Raw<T> r;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2_f32(w[i], (T*)nullptr);
-        v[2 * i] = f.x; v[2 * i + 1] = f.y;
-      }
+  for (int i = 0; i < (int)sizeof(r.w) / 32; ++i) {
+    uint32_t* w = r.w + 8 * i;
+    if (live) {
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(reinterpret_cast<const char*>(p) + 32 * i));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = 0;
     }
+  }
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw<T>& r, float (&v)[kMxPiece]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < kMxPiece; ++i) v[i] = __uint_as_float(r.w[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
+    for (int i = 0; i < kMxPiece / 2; ++i) {
+      const float2 f = unpack2_f32(r.w[i], (T*)nullptr);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
-  if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      *reinterpret_cast<uint4*>(p) =
-          make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-    }
+__device__ __forceinline__ Raw<T> pack(const float (&v)[kMxPiece]) {
+  Raw<T> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < kMxPiece; ++i) r.w[i] = __float_as_uint(v[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = from_f32<T>(v[i]);
+    for (int i = 0; i < kMxPiece / 2; ++i) r.w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+  }
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, bool live, const float (&v)[kMxPiece]) {
+  const Raw<T> r = pack<T>(v);
+  if (!live) return;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(r.w) / 32; ++i) {
+    const uint32_t* w = r.w + 8 * i;
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<char*>(p) + 32 * i),
+                 "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
   }
 }
 
-// Whether rows at `p` with a stride of `ld` elements can be read eight elements at a time.
+// The first n of sixteen elements at p, zeros for the others.  Only granules that hold an element
+// asked for are read.
 template <typename T>
-__host__ __device__ inline bool rows_aligned(const T* p, int64_t ld) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0;
+__device__ __forceinline__ void load_any(const T* p, int n, float (&v)[kMxPiece]) {
+  n = max(0, min(n, kMxPiece));
+  constexpr int kGranules = (int)sizeof(T) + 1;
+  const uint32_t shift = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15;
+  const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - shift);
+  const int end = n ? (int)shift + n * (int)sizeof(T) : 0;
+  uint32_t w[4 * kGranules];
+#pragma unroll
+  for (int i = 0; i < kGranules; ++i) {
+    uint4 g = make_uint4(0, 0, 0, 0);
+    if (16 * i < end) g = base[i];
+    w[4 * i] = g.x; w[4 * i + 1] = g.y; w[4 * i + 2] = g.z; w[4 * i + 3] = g.w;
+  }
+#pragma unroll
+  for (int i = 0; i + 2 < 4 * kGranules; ++i) w[i] = shift & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i + 1 < 4 * kGranules - 2; ++i) w[i] = shift & 4 ? w[i + 1] : w[i];
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)(4 * sizeof(T)); ++i)
+    r.w[i] = sizeof(T) == 2 && (shift & 2) ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+  unpack(r, v);
+#pragma unroll
+  for (int i = 0; i < kMxPiece; ++i) v[i] = i < n ? v[i] : 0.f;
 }
 
-// Writes eight values of columns col .. col + 7 (a multiple of 8) as MX8.  Four neighbouring
-// threads hold a block and 16 a scale tile's 128 columns; all 32 threads of the warp call this
-// together, with zeros in columns past the last.
-__device__ __forceinline__ void mx_store8(const float (&v)[8], int row, int col, int cols, int col_tiles, bool live,
-                                          uint8_t* q, int64_t ldq, uint8_t* scales) {
-  uint32_t a = 0;
+// The first n of each lane's sixteen elements to its p; the warp calls this together.  `stage`: 512
+// elements of shared memory of the warp's own, 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void store_any(T* stage, T* p, int n, const float (&v)[kMxPiece]) {
+  const int lane = threadIdx.x & 31;
+  const Raw<T> r = pack<T>(v);
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = max(a, abs_bits(v[i]));
+  for (int i = 0; i < (int)sizeof(T); ++i)
+    reinterpret_cast<uint4*>(stage + lane * kMxPiece)[i] = make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < kMxPiece; ++j) {
+    const int from = 2 * j + (lane >> 4), at = lane & 15;
+    T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), from));
+    const int many = __shfl_sync(0xffffffffu, n, from);
+    if (at < many) to[at] = stage[32 * j + lane];
+  }
+}
+
+template <typename T>
+inline bool rows_vectored(const T* p, int64_t ld, int cols) {
+  return reinterpret_cast<uintptr_t>(p) % 32 == 0 && ld * (int64_t)sizeof(T) % 32 == 0 && cols % kMxPiece == 0;
+}
+
+// Division by a number that the kernel gets: n / d for n below 2^31 as a high product, a sum and a shift
+// (Granlund and Montgomery, "Division by invariant integers using multiplication").
+struct FastDiv {
+  uint32_t d, m, s;
+  explicit FastDiv(uint32_t divisor) : d(divisor), m(0), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
+// Writes a piece as MX8.  Two neighbouring threads hold a block and eight a scale tile's 128 columns;
+// all 32 threads of the warp call this together, with zeros in columns past the last.
+__device__ __forceinline__ void mx_store_piece(const float (&v)[kMxPiece], int row, int col, int cols, int col_tiles, bool live,
+                                               uint8_t* q, int64_t ldq, uint8_t* scales) {
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMxPiece; i += 2) most = max_abs3(most, v[i], v[i + 1]);
+  uint32_t a = __float_as_uint(most);
   a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
-  a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
   const uint32_t byte = mx_scale_byte(a);
   const int lane = threadIdx.x & 31;
-  uint32_t word = byte << (8 * ((lane >> 2) & 3));
+  uint32_t word = byte << (4 * (lane & 6));
+  word |= __shfl_xor_sync(0xffffffffu, word, 2);
   word |= __shfl_xor_sync(0xffffffffu, word, 4);
-  word |= __shfl_xor_sync(0xffffffffu, word, 8);
-  if (!live) return;
-  if (col < ((cols + 15) & ~15))
-    *reinterpret_cast<uint2*>(q + (size_t)row * ldq + col) = make_uint2(mx_pack4(v, byte), mx_pack4(v + 4, byte));
-  if ((lane & 15) == 0 && col / kMxTileCols < col_tiles)
+  if (!live || col >= col_tiles * kMxTileCols) return;
+  if (col < cols) {
+    const float inverse = mx_inverse(byte);
+    *reinterpret_cast<uint4*>(q + (size_t)row * ldq + col) =
+        make_uint4(mx_pack4(v, inverse), mx_pack4(v + 4, inverse), mx_pack4(v + 8, inverse), mx_pack4(v + 12, inverse));
+  }
+  if ((lane & 7) == 0)
     *reinterpret_cast<uint32_t*>(scales + mx_scale_tile(row, col / kMxTileCols, col_tiles) + mx_scale_row(row)) = word;
 }
 
 // ---------------------------------------------------------------------------------------------
-// x [rows][cols] -> MX8.  16 threads take 128 columns of a row.
+// x [rows][cols] -> MX8.  Eight threads take 128 columns of a row (a group), and each U of them at
+// once.
 // ---------------------------------------------------------------------------------------------
 constexpr int kMxThreads = 256;
 
-template <typename T>
-__global__ void __launch_bounds__(kMxThreads) mx8_quantize_kernel(const T* x, int64_t ldx, int rows, int cols, uint8_t* q,
-                                                                  int64_t ldq, uint8_t* scales) {
+template <typename T, bool kVec, int U>
+__global__ void __launch_bounds__(kMxThreads) mx8_quantize_kernel(const T* x, int64_t ldx, int rows, int cols, FastDiv col_tiles,
+                                                                  uint8_t* q, int64_t ldq, uint8_t* scales) {
   pdl_wait();
-  const int col_tiles = mx_col_tiles(cols);
-  const int64_t groups = (int64_t)rows * col_tiles;
-  const bool aligned = rows_aligned(x, ldx);
-  const int64_t step = (int64_t)gridDim.x * (kMxThreads / 16);
+  const uint32_t groups = (uint32_t)rows * col_tiles.d;  // below 2^31
+  const uint32_t step = gridDim.x * (kMxThreads / 8);
   // The loop bound is the warp's first group, so that its 32 threads stay together.
-  for (int64_t g0 = (int64_t)blockIdx.x * (kMxThreads / 16) + (threadIdx.x >> 5) * 2; g0 < groups; g0 += step) {
-    const int64_t g = g0 + ((threadIdx.x >> 4) & 1);
-    const bool live = g < groups;
-    const int row = live ? (int)(g / col_tiles) : 0;
-    const int col = live ? (int)(g - (int64_t)row * col_tiles) * kMxTileCols + (threadIdx.x & 15) * 8 : 0;
-    const int n = live ? min(8, cols - col) : 0;
-    float v[8];
-    load8(x + (size_t)row * ldx + col, n, aligned && n == 8, v);
-    mx_store8(v, row, col, cols, col_tiles, live, q, ldq, scales);
+  for (uint32_t g0 = blockIdx.x * (kMxThreads / 8) + (threadIdx.x >> 5) * 4; g0 < groups; g0 += step * U) {
+    int row[U], col[U];
+    bool live[U];
+    Raw<T> raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t g = g0 + u * step + ((threadIdx.x >> 3) & 3);
+      live[u] = g < groups;
+      row[u] = live[u] ? (int)col_tiles.div(g) : 0;
+      col[u] = live[u] ? (int)(g - (uint32_t)row[u] * col_tiles.d) * kMxTileCols + (threadIdx.x & 7) * kMxPiece : 0;
+      if (kVec) raw[u] = load_raw(x + (size_t)row[u] * ldx + col[u], live[u] && col[u] < cols);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[kMxPiece];
+      if (kVec) unpack(raw[u], v);
+      else load_any(x + (size_t)row[u] * ldx + col[u], live[u] ? cols - col[u] : 0, v);
+      mx_store_piece(v, row[u], col[u], cols, (int)col_tiles.d, live[u], q, ldq, scales);
+    }
   }
 }
 
-// MX8 -> out [rows][cols].  A thread takes 8 columns.
-template <typename T>
+// MX8 -> out [rows][cols], U pieces per thread at once.
+template <typename T, bool kVec, int U>
 __global__ void __launch_bounds__(kMxThreads) mx8_dequantize_kernel(const uint8_t* q, int64_t ldq, const uint8_t* scales,
-                                                                    int rows, int cols, T* out, int64_t ldo) {
+                                                                    int rows, int cols, FastDiv per_row, T* out, int64_t ldo) {
   pdl_wait();
   const int col_tiles = mx_col_tiles(cols);
-  const int per_row = (cols + 7) / 8;
-  const int64_t pieces = (int64_t)rows * per_row;
-  const bool aligned = rows_aligned(out, ldo);
-  for (int64_t i = (int64_t)blockIdx.x * kMxThreads + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * kMxThreads) {
-    const int row = (int)(i / per_row), col = (int)(i - (int64_t)row * per_row) * 8;
-    const uint2 w = *reinterpret_cast<const uint2*>(q + (size_t)row * ldq + col);
-    const float s = mx_scale(scales[mx_scale_tile(row, col / kMxTileCols, col_tiles) + mx_scale_row(row) +
-                                    ((col / kMxBlock) & 3)]);
-    float v[8];
-    mx_unpack4(w.x, v);
-    mx_unpack4(w.y, v + 4);
+  const uint32_t pieces = (uint32_t)rows * per_row.d;  // below 2^31
+  const uint32_t step = gridDim.x * kMxThreads;
+  __shared__ __align__(16) T stage[kVec ? 1 : kMxThreads / 32][kVec ? 8 : 32 * kMxPiece];
+  // The loop bound is the warp's first piece, so that its 32 threads stay together.
+  for (uint32_t w0 = blockIdx.x * kMxThreads + (threadIdx.x & ~31u); w0 < pieces; w0 += step * U) {
+    const uint32_t i0 = w0 + (threadIdx.x & 31);
+    int row[U], col[U];
+    uint4 w[U];
+    uint32_t byte[U];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= s;
-    const int n = min(8, cols - col);
-    store8(out + (size_t)row * ldo + col, n, aligned && n == 8, v);
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = min(i0 + u * step, pieces - 1);  // past the end: the last piece again, not stored
+      row[u] = (int)per_row.div(i);
+      col[u] = (int)(i - (uint32_t)row[u] * per_row.d) * kMxPiece;
+      w[u] = *reinterpret_cast<const uint4*>(q + (size_t)row[u] * ldq + col[u]);
+      byte[u] = scales[mx_scale_tile(row[u], col[u] / kMxTileCols, col_tiles) + mx_scale_row(row[u]) + ((col[u] / kMxBlock) & 3)];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float s = mx_scale(byte[u]);
+      const float2 s2 = make_float2(s, s);
+      float v[kMxPiece];
+      mx_unpack4(w[u].x, v);
+      mx_unpack4(w[u].y, v + 4);
+      mx_unpack4(w[u].z, v + 8);
+      mx_unpack4(w[u].w, v + 12);
+#pragma unroll
+      for (int k = 0; k < kMxPiece; k += 2) {
+        const float2 t = mul2(make_float2(v[k], v[k + 1]), s2);
+        v[k] = t.x;
+        v[k + 1] = t.y;
+      }
+      const bool live = i0 + u * step < pieces;
+      T* p = out + (size_t)row[u] * ldo + col[u];
+      if constexpr (kVec) store_vec(p, live, v);
+      else store_any(stage[threadIdx.x >> 5], p, live ? cols - col[u] : 0, v);
+    }
   }
 }
 
 // ---------------------------------------------------------------------------------------------
 // h = x + residual; sum_out = h; y = h * rsqrt(mean(h^2) + eps) * weight, written as MX8.  The row
-// is summed and squared in fp32 and y is formed from the unrounded h.  One block takes one row
-// at a time.
+// is summed and squared in fp32 and y is formed from the unrounded h.
+//
+// HBM-bound: x and the residual are read once and h, the values and the scales written once.  `warps`
+// warps hold a row in registers, CH pieces per thread, and a block of at least 256 threads
+// walks over rows with the weight in registers too; the next row's loads are issued before this
+// row's sum of squares is exchanged, so that a block always has a row in flight.
 // ---------------------------------------------------------------------------------------------
 struct RmsNormArgs {
   const void* x; int64_t ldx;
@@ -206,53 +347,148 @@ struct RmsNormArgs {
   int rows, cols;
   uint8_t* q; int64_t ldq;
   uint8_t* scales;
+  int warps;                          // per row, a power of two
 };
 
+__device__ __forceinline__ float warp_total(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T, typename R, int CH, bool kVec>
+__global__ void __launch_bounds__(512) rms_norm_mx8_kernel(const RmsNormArgs a) {
+  pdl_wait();
+  __shared__ float part[2][16];
+  __shared__ __align__(16) R stage[kVec ? 1 : 16][kVec ? 8 : 32 * kMxPiece];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_block = (int)(blockDim.x >> 5) / a.warps;  // rows of a block
+  const int sub = warp / a.warps, within = warp - sub * a.warps;
+  const int col_tiles = mx_col_tiles(a.cols);
+  const T* x = static_cast<const T*>(a.x);
+  const R* r = static_cast<const R*>(a.residual);
+  R* sum = static_cast<R*>(a.sum_out);
+  int col[CH];
+  float w[CH][kMxPiece];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    col[c] = ((c * a.warps + within) * 32 + lane) * kMxPiece;
+    load_any(a.weight + col[c], a.cols - col[c], w[c]);
+  }
+  Raw<T> rx[kVec ? CH : 1];
+  Raw<R> rr[kVec ? CH : 1];
+  auto fetch = [&](int row) {
+    if constexpr (kVec) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const bool in = row < a.rows && col[c] < a.cols;
+        rx[c] = load_raw(x + (size_t)row * a.ldx + col[c], in);
+        rr[c] = load_raw(r + (size_t)row * a.ldr + col[c], in && r);
+      }
+    }
+  };
+  const int step = gridDim.x * per_block;
+  int turn = 0;
+  int row = blockIdx.x * per_block + sub;
+  fetch(row);
+  for (int row0 = blockIdx.x * per_block; row0 < a.rows; row0 += step, row += step, turn ^= 1) {
+    const bool live = row < a.rows;
+    float h[CH][kMxPiece];
+    float2 sq2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float t[kMxPiece];
+      if constexpr (kVec) {
+        unpack(rx[c], h[c]);
+        unpack(rr[c], t);
+      } else {
+        const int n = live ? a.cols - col[c] : 0;
+        load_any(x + (size_t)row * a.ldx + col[c], n, h[c]);
+        load_any(r + (size_t)row * a.ldr + col[c], r ? n : 0, t);
+      }
+#pragma unroll
+      for (int i = 0; i < kMxPiece; i += 2) {
+        const float2 f = add2(make_float2(h[c][i], h[c][i + 1]), make_float2(t[i], t[i + 1]));
+        sq2 = fma2(f, f, sq2);
+        h[c][i] = f.x;
+        h[c][i + 1] = f.y;
+      }
+    }
+    fetch(row + step);
+    if (sum) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        R* p = sum + (size_t)row * a.lds + col[c];
+        if constexpr (kVec) store_vec(p, live && col[c] < a.cols, h[c]);
+        else store_any(stage[warp], p, live ? a.cols - col[c] : 0, h[c]);
+      }
+    }
+    float sq = warp_total(sq2.x + sq2.y);
+    if (a.warps > 1) {
+      // Two sets of sums, taken in turn: a warp may be one row ahead of the others here.
+      if (lane == 0) part[turn][warp] = sq;
+      __syncthreads();
+      sq = warp_total(lane < a.warps ? part[turn][sub * a.warps + lane] : 0.f);
+    }
+    const float inv = rsqrtf(sq / (float)a.cols + a.eps);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if (col[c] - lane * kMxPiece >= a.cols) break;  // the whole warp is past the row
+#pragma unroll
+      for (int i = 0; i < kMxPiece; i += 2) {
+        const float2 f = mul2(mul2(make_float2(h[c][i], h[c][i + 1]), make_float2(inv, inv)), make_float2(w[c][i], w[c][i + 1]));
+        // A NaN stays out of the columns past the last.
+        h[c][i] = col[c] + (kVec ? 0 : i) < a.cols ? f.x : 0.f;
+        h[c][i + 1] = col[c] + (kVec ? 0 : i + 1) < a.cols ? f.y : 0.f;
+      }
+      mx_store_piece(h[c], row, col[c], a.cols, col_tiles, live, a.q, a.ldq, a.scales);
+    }
+  }
+}
+
+// Rows too long for the registers of 16 warps: one block takes one row at a time and reads it twice.
 template <typename T, typename R>
-__global__ void __launch_bounds__(kMxThreads) rms_norm_mx8_kernel(const RmsNormArgs a) {
+__global__ void __launch_bounds__(kMxThreads) rms_norm_mx8_long_kernel(const RmsNormArgs a) {
   pdl_wait();
   __shared__ float part[kMxThreads / 32];
+  __shared__ __align__(16) R stage[kMxThreads / 32][32 * kMxPiece];
   const int col_tiles = mx_col_tiles(a.cols);
-  const int span = col_tiles * kMxTileCols;
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + (size_t)row * a.ldx;
     const R* r = a.residual ? static_cast<const R*>(a.residual) + (size_t)row * a.ldr : nullptr;
     R* s = a.sum_out ? static_cast<R*>(a.sum_out) + (size_t)row * a.lds : nullptr;
-    const bool ax = rows_aligned(x, a.ldx), ar = rows_aligned(r, a.ldr), as = rows_aligned(s, a.lds);
-    float sq = 0.f;
-    auto load = [&](int col, float (&h)[8]) {
-      const int n = max(0, min(8, a.cols - col));
-      float t[8];
-      load8(x + col, n, ax && n == 8, h);
+    auto load = [&](int col, float (&h)[kMxPiece]) {
+      const int n = a.cols - col;
+      load_any(x + col, n, h);
       if (r) {
-        load8(r + col, n, ar && n == 8, t);
+        float t[kMxPiece];
+        load_any(r + col, n, t);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] += t[i];
+        for (int i = 0; i < kMxPiece; ++i) h[i] += t[i];
       }
-      return n;
     };
-    for (int col = threadIdx.x * 8; col < a.cols; col += kMxThreads * 8) {
-      float h[8];
+    float sq = 0.f;
+    for (int col = threadIdx.x * kMxPiece; col < a.cols; col += kMxThreads * kMxPiece) {
+      float h[kMxPiece];
       load(col, h);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sq += h[i] * h[i];
+      for (int i = 0; i < kMxPiece; ++i) sq = fmaf(h[i], h[i], sq);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+    sq = warp_total(sq);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sq;
     __syncthreads();
     sq = 0.f;
 #pragma unroll
     for (int w = 0; w < kMxThreads / 32; ++w) sq += part[w];
     const float inv = rsqrtf(sq / (float)a.cols + a.eps);
-    for (int col0 = (threadIdx.x & ~31) * 8; col0 < span; col0 += kMxThreads * 8) {  // whole warps
-      const int col = col0 + (threadIdx.x & 31) * 8;
-      float h[8];
-      const int n = load(col, h);
-      if (s) store8(s + col, n, as && n == 8, h);
+    for (int col0 = (threadIdx.x & ~31) * kMxPiece; col0 < a.cols; col0 += kMxThreads * kMxPiece) {  // whole warps
+      const int col = col0 + (threadIdx.x & 31) * kMxPiece, n = a.cols - col;
+      float h[kMxPiece];
+      load(col, h);
+      if (s) store_any(stage[threadIdx.x >> 5], s + col, n, h);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = i < n ? h[i] * inv * a.weight[col + i] : 0.f;
-      mx_store8(h, row, col, a.cols, col_tiles, true, a.q, a.ldq, a.scales);
+      for (int i = 0; i < kMxPiece; ++i) h[i] = i < n ? h[i] * inv * a.weight[col + i] : 0.f;
+      mx_store_piece(h, row, col, a.cols, col_tiles, true, a.q, a.ldq, a.scales);
     }
     __syncthreads();
   }

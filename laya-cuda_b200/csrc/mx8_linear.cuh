@@ -207,13 +207,13 @@ __device__ __forceinline__ void mx_finish(const MxLinearArgs& a, int row0, int s
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[k][i] = i < n ? acc[k][i] : 0.f;
       }
-      uint32_t m = max(max(abs_bits(acc[k][0]), abs_bits(acc[k][1])), max(abs_bits(acc[k][2]), abs_bits(acc[k][3])));
+      uint32_t m = __float_as_uint(max_abs3(max_abs3(0.f, acc[k][0], acc[k][1]), acc[k][2], acc[k][3]));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
       const uint32_t byte = mx_scale_byte(m);
       if (row < a.M) {
-        if (in_values) *reinterpret_cast<uint32_t*>(q + (size_t)(k * step) * a.ldo) = mx_pack4(acc[k], byte);
+        if (in_values) *reinterpret_cast<uint32_t*>(q + (size_t)(k * step) * a.ldo) = mx_pack4(acc[k], mx_inverse(byte));
         if (in_scales)
           a.out_scales[mx_scale_tile(row, col_tile, col_tiles) + mx_scale_row(row) + ((col / kMxBlock) & 3)] = (uint8_t)byte;
       }

@@ -41,6 +41,19 @@ class Metrics(ct.Structure):
                 ("kernel_launches", ct.c_int32), ("owned_gpu_bytes", ct.c_uint64)]
 
 
+class Mx8Convert(ct.Structure):
+    _fields_ = [("rows", ct.c_int32), ("cols", ct.c_int32), ("dtype", ct.c_int32),
+                ("values", ct.c_void_p), ("scales", ct.c_void_p), ("ldv", ct.c_int64),
+                ("data", ct.c_void_p), ("ld", ct.c_int64)]
+
+
+class RmsNormMx8(ct.Structure):
+    _fields_ = [("rows", ct.c_int32), ("cols", ct.c_int32), ("dtype", ct.c_int32), ("residual_dtype", ct.c_int32),
+                ("x", ct.c_void_p), ("ldx", ct.c_int64), ("residual", ct.c_void_p), ("ldr", ct.c_int64),
+                ("sum_out", ct.c_void_p), ("lds", ct.c_int64), ("weight", ct.c_void_p),
+                ("values", ct.c_void_p), ("scales", ct.c_void_p), ("ldv", ct.c_int64), ("eps", ct.c_float)]
+
+
 class Mx8Linear(ct.Structure):
     _fields_ = [("rows", ct.c_int32), ("features", ct.c_int32), ("cols", ct.c_int32), ("activation", ct.c_int32),
                 ("x", ct.c_void_p), ("x_scales", ct.c_void_p), ("ldx", ct.c_int64),
@@ -99,13 +112,13 @@ def load():
         "laya_op_head_tail": (i, [i, p, p, p, i, i, i, p, p, p, p, p, p, i, p, p, p, p, p, p]),
         "laya_op_gemm_residual_static": (i, [i, p, p, i, i, i, i, p, p, p, p]),
     }
-    q = ct.c_int64
+    # The argument structures are passed by address or as their packed bytes (see mx8.py).
     sig |= {
-        "laya_mx8_scale_bytes": (q, [i, i]),
-        "laya_op_mx8_quantize": (i, [i, p, q, i, i, p, q, p, p]),
-        "laya_op_mx8_dequantize": (i, [p, q, p, i, i, i, p, q, p]),
-        "laya_op_rms_norm_mx8": (i, [i, p, q, i, p, q, p, q, p, ct.c_float, i, i, p, q, p, p]),
-        "laya_op_mx8_linear": (i, [ct.POINTER(Mx8Linear), p, p]),
+        "laya_mx8_scale_bytes": (ct.c_int64, [i, i]),
+        "laya_op_mx8_quantize": (i, [p, p]),
+        "laya_op_mx8_dequantize": (i, [p, p]),
+        "laya_op_rms_norm_mx8": (i, [p, p]),
+        "laya_op_mx8_linear": (i, [p, p, p]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

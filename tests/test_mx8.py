@@ -27,34 +27,42 @@ def test_scale_bytes_refuses_bad_shapes(lib, rows, cols):
 P = 0x10000  # stands for an aligned device pointer: every call below is refused before it is used
 
 
-@pytest.mark.parametrize("args,word", [
-    ((3, P, 32, 4, 32, P, 32, P, None), "dtype"),
-    ((0, P, 32, -1, 32, P, 32, P, None), "shape"),
-    ((0, P, 32, 4, 0, P, 32, P, None), "shape"),
-    ((0, None, 32, 4, 32, P, 32, P, None), "null"),
-    ((0, P, 31, 4, 32, P, 32, P, None), "stride"),
-    ((0, P + 2, 32, 4, 32, P, 32, P, None), "aligned"),
-    ((0, P, 32, 4, 32, P, 40, P, None), "16"),
-    ((0, P, 48, 4, 48, P, 32, P, None), "at least"),
-    ((0, P, 32, 4, 32, P + 8, 32, P, None), "16-byte"),
-    ((0, P, 32, 4, 32, P, 32, P + 1, None), "16-byte"),
-    ((0, P, 32, 4, 32, P, 32, None, None), "null"),
+def convert(**other):
+    fields = dict(rows=4, cols=32, dtype=0, values=P, scales=P, ldv=32, data=P, ld=32)
+    return _lib.Mx8Convert(**{**fields, **other})
+
+
+@pytest.mark.parametrize("name", ["laya_op_mx8_quantize", "laya_op_mx8_dequantize"])
+@pytest.mark.parametrize("other,word", [
+    (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(rows=-1), "shape"), (dict(cols=0), "shape"),
+    (dict(data=None), "null"), (dict(ld=31), "stride"), (dict(data=P + 2), "aligned"), (dict(ldv=40), "16"),
+    (dict(cols=48, ld=48), "at least"), (dict(values=P + 8), "16-byte"), (dict(scales=P + 1), "16-byte"),
+    (dict(scales=None), "null"), (dict(values=None), "null"),
 ])
-def test_quantize_refuses(lib, args, word):
+def test_conversions_refuse(lib, name, other, word):
     with pytest.raises(ValueError, match=word):
-        _lib.check(lib.laya_op_mx8_quantize(*args))
+        _lib.check(getattr(lib, name)(ct.byref(convert(**other)), None))
+    with pytest.raises(ValueError, match="null"):
+        _lib.check(getattr(lib, name)(None, None))
 
 
-def test_dequantize_and_norm_refuse(lib):
-    for args in ((None, 32, P, 4, 32, 0, P, 32, None), (P, 32, P, 4, 32, 3, P, 32, None), (P, 32, P, 4, 32, 0, P, 16, None)):
-        with pytest.raises(ValueError):
-            _lib.check(lib.laya_op_mx8_dequantize(*args))
-    good = [0, P, 32, 0, P, 32, P, 32, P, 1e-6, 4, 32, P, 32, P, None]
-    for at, bad in ((0, 3), (1, None), (3, 9), (5, 8), (7, 8), (8, None), (8, P + 4), (9, -1.0), (9, float("nan")), (10, -2), (13, 24)):
-        args = list(good)
-        args[at] = bad
-        with pytest.raises(ValueError):
-            _lib.check(lib.laya_op_rms_norm_mx8(*args))
+def norm(**other):
+    fields = dict(rows=4, cols=32, dtype=0, residual_dtype=0, x=P, ldx=32, residual=P, ldr=32, sum_out=P, lds=32, weight=P,
+                  values=P, scales=P, ldv=32, eps=1e-6)
+    return _lib.RmsNormMx8(**{**fields, **other})
+
+
+@pytest.mark.parametrize("other,word", [
+    (dict(dtype=3), "dtype"), (dict(residual_dtype=9), "dtype"), (dict(x=None), "null"), (dict(ldx=31), "stride"),
+    (dict(ldr=8), "stride"), (dict(lds=8), "stride"), (dict(residual=P + 2), "aligned"), (dict(weight=None), "null"),
+    (dict(weight=P + 4), "16-byte"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(rows=-2), "shape"),
+    (dict(ldv=24), "16"), (dict(values=None), "null"),
+])
+def test_norm_refuses(lib, other, word):
+    with pytest.raises(ValueError, match=word):
+        _lib.check(lib.laya_op_rms_norm_mx8(ct.byref(norm(**other)), None))
+    with pytest.raises(ValueError, match="null"):
+        _lib.check(lib.laya_op_rms_norm_mx8(None, None))
 
 
 def linear(**other):
@@ -79,10 +87,18 @@ def test_linear_refuses(lib, other, word):
 
 
 def test_no_rows_needs_no_buffers_and_no_device(lib):
-    assert lib.laya_op_mx8_quantize(0, None, 32, 0, 32, None, 32, None, None) == 0
-    assert lib.laya_op_mx8_dequantize(None, 32, None, 0, 32, 0, None, 32, None) == 0
-    assert lib.laya_op_rms_norm_mx8(0, None, 32, 0, None, 0, None, 0, None, 1e-6, 0, 32, None, 32, None, None) == 0
+    for name in ("laya_op_mx8_quantize", "laya_op_mx8_dequantize"):
+        assert getattr(lib, name)(ct.byref(convert(rows=0, values=None, scales=None, data=None)), None) == 0
+    assert lib.laya_op_rms_norm_mx8(ct.byref(norm(rows=0, x=None, weight=None, values=None)), None) == 0
     assert lib.laya_op_mx8_linear(ct.byref(linear(rows=0, x=None, w=None, out=None)), None, None) == 0
+
+
+@pytest.mark.parametrize("cls", [_lib.Mx8Convert, _lib.RmsNormMx8, _lib.Mx8Linear])
+def test_packed_arguments_are_the_structure(cls):
+    values = [k + 1 if kind is not ct.c_float else 0.5 for k, (_, kind) in enumerate(cls._fields_)]
+    packed = mx8._packer(cls)(*values)
+    filled = cls.from_buffer_copy(packed)
+    assert [getattr(filled, name) for name, _ in cls._fields_] == values
 
 
 def test_tensors_on_the_host_are_refused():
