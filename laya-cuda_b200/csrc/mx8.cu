@@ -1,5 +1,6 @@
 // Entry points of the MX8 operators (see include/laya_b200.h): checks of arguments and launches.
 #include <algorithm>
+#include <cmath>
 #include <exception>
 
 #include "host.cuh"
@@ -163,6 +164,19 @@ void launch_pair(const MxLinearArgs& a, int dev, cudaStream_t st) {
   launch_cluster(kern, dim3(2 * pairs), kMxThreadsPair, Cfg::kSmemBytes, dim3(2, 1, 1), st, m, a);
 }
 
+// Launch shape of the few-row kernel: 128-feature tiles by BN-row tiles, K split over at most 4 CTAs and no
+// more than there are SMs for.  (One row, 4096 x 4096, 32 tiles: unsplit 8.2 us, 2 CTAs 6.2, 4 CTAs 5.5, 8 CTAs
+// 6.6; 16 x 2048 x 2048, 16 tiles: 5.9, 5.2, 4.8, 7.1.)
+struct FewGrid {
+  int tiles, row_tiles, split;
+};
+FewGrid few_grid(const MxLinearArgs& a, int bn, int sms) {
+  FewGrid g{(a.N + 127) / 128, (a.M + bn - 1) / bn, 1};
+  const int k_tiles = mx_col_tiles(a.K);
+  while (g.split < kMxMaxSplit && g.split < k_tiles && (int64_t)g.tiles * g.row_tiles * (g.split + 1) <= sms) ++g.split;
+  return g;
+}
+
 template <int BN, bool kGated>
 void launch_few(const MxLinearArgs& a, int dev, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
@@ -170,17 +184,37 @@ void launch_few(const MxLinearArgs& a, int dev, cudaStream_t st) {
   auto kern = mx8_linear_few_kernel<BN, kGated>;
   allow_smem(kern, Cfg::kSmemBytes, dev, done);
   const MxMaps m = linear_maps(a, BN, 128, 1);
-  const int tiles = (a.N + 127) / 128, row_tiles = (a.M + BN - 1) / BN, k_tiles = mx_col_tiles(a.K);
-  int split = 1;
-  while (split < kMxMaxSplit && 2 * split <= k_tiles && (int64_t)tiles * row_tiles * split < sm_count(dev)) split *= 2;
-  launch_cluster(kern, dim3(tiles, row_tiles, split), kMxThreadsFew, Cfg::kSmemBytes, dim3(1, 1, split), st, m, a);
+  const FewGrid g = few_grid(a, BN, sm_count(dev));
+  launch_cluster(kern, dim3(g.tiles, g.row_tiles, g.split), kMxThreadsFew, Cfg::kSmemBytes, dim3(1, 1, g.split), st, m, a);
 }
 
+// Which kernel, and which tile.
+//
+// The few-row kernel where its 128 x BN tiles fit the SMs at once (BN 64 past 32 rows) and K is split or
+// short, or a third of the SMs stay free: 128 x 4096 x 4096 takes 7.9 us against the pair kernels' 11.1 (256 x 128
+// tiles) and 15.4 (256 x 256), 511 x 776 x 2304 7.8 against 8.8 and 12.6, 700 x 4096 x 1000 (88 tiles) 9.7 against
+// 11.7; but 256 x 4096 x 4096 (128 tiles) 12.4 against 11.2.  A gated pair tile has only 128 output columns,
+// and the few-row kernel wins wherever it fits (256 x 2048 x 2 x 4096: 12.9 against 13.9).
+//
+// Otherwise CTA pairs: the tile for which this estimate is the shorter.  A wave of tiles takes
+// the longer of its MMAs' and its epilogue's time, and the last epilogue shows (microseconds, fitted to
+// 256..1024 x 4096 x 4096: 512 rows 12.0 against 16.0 us, 1024 rows 19.2 against 17.4).
 template <bool kGated>
 void launch_linear(const MxLinearArgs& a, int dev, cudaStream_t st) {
   if (a.M <= 16) return launch_few<16, kGated>(a, dev, st);
   if (a.M <= 32) return launch_few<32, kGated>(a, dev, st);
-  if (a.M <= 128) return launch_few<64, kGated>(a, dev, st);
+  const int sms = sm_count(dev), k_tiles = mx_col_tiles(a.K);
+  const FewGrid few = few_grid(a, 64, sms);
+  const int64_t few_tiles = (int64_t)few.tiles * few.row_tiles;
+  if (few_tiles <= sms && (kGated || few.split > 1 || k_tiles <= 16 || 3 * few_tiles <= 2 * sms))
+    return launch_few<64, kGated>(a, dev, st);
+  if constexpr (!kGated) {
+    auto estimate = [&](int bn, double per_k_tile, double epilogue) {
+      const double tiles = (double)((a.M + 255) / 256) * ((a.N + bn - 1) / bn);
+      return std::ceil(tiles / (sms / 2)) * std::max(k_tiles * per_k_tile, epilogue) + epilogue;
+    };
+    if (estimate(128, 0.21, 1.3) < estimate(256, 0.29, 2.6)) return launch_pair<128, false>(a, dev, st);
+  }
   launch_pair<256, kGated>(a, dev, st);
 }
 

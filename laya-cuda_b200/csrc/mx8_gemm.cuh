@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
       auto chunk = [&](int j) { return half ? 2 * kChunks - 1 - j : j; };
       auto fetch = [&](int j, MxInputs<8>& in) {
         const int c0 = nb * kOutCols + chunk(j) * 32;
-        mx_fetch<kGated, 8>(args, row0 + (lane >> 3), 4, c0 + 4 * (lane & 7), row0 + 32 <= args.M && c0 + 32 <= args.N, in);
+        mx_fetch<kGated, 8>(args, row0 + (lane >> 3), 4, args.M, c0 + 4 * (lane & 7), row0 + 32 <= args.M && c0 + 32 <= args.N, in);
       };
       // The first chunk's inputs are loaded while the tile's MMAs run; the other chunks' residual is
       // brought into L2 then and loaded one chunk ahead of its use.
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
           mx_stage_put(buf, lane, u);
           mx_stage_get(buf, lane, v);
         }
-        mx_finish<kGated, 8>(args, row0 + (lane >> 3), 4, nb * kOutCols + c * 32 + 4 * (lane & 7), v, g, in);
+        mx_finish<kGated, 8>(args, row0 + (lane >> 3), 4, args.M, nb * kOutCols + c * 32 + 4 * (lane & 7), v, g, in);
         if (j + 1 < kChunks) fetch(j + 1, in);
       }
     }
@@ -397,11 +397,16 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
 // every CTA adds and finishes its share of the rows from all of them in rank order, so the result
 // does not depend on timing.
 //
-// Warps: 0..3 read tensor memory and finish rows, 4 TMA producer, 5 tensor-memory allocator and MMA
-// issuer.
+// One thread issues a k-block (wait, 2 scale copies, 4 MMAs, commit) in about 320 cycles whatever BN is, longer
+// than its MMAs take, so two warps issue, each into an accumulator of its own: not gated, k-blocks in
+// turn (the accumulators are added when they are read); gated, one the products with W and one
+// those with G.  Likewise two warps load: k-blocks in turn, or W and its scales / G and X.
+//
+// Warps: 0..3 read tensor memory, 4 and 7 TMA producers, 5 and 6 MMA issuers (5 allocates tensor
+// memory); all eight finish rows.
 // ---------------------------------------------------------------------------------------------
-constexpr int kMxThreadsFew = 192;
-constexpr int kMxMaxSplit = 8;
+constexpr int kMxThreadsFew = 256;
+constexpr int kMxMaxSplit = 4;
 
 template <int BN, bool kGated>
 struct MxFewCfg {
@@ -409,11 +414,16 @@ struct MxFewCfg {
   static constexpr int kStageB = BN * kMxBK;
   static constexpr int kStageScales = (kWeights + 1) * kMxTileBytes;
   static constexpr int kStageBytes = kWeights * kMxOperandBytes + kStageB + kStageScales;
-  static constexpr int kStages = (kGated ? 200 * 1024 : 104 * 1024) / kStageBytes;
+  // Not gated: shared memory for two CTAs per SM, so that the next kernel's CTAs set up while this one's
+  // finish (64 x 4096 x 4096: 6.8 us, with twice the stages 8.2), and an even number of stages, so that a
+  // stage always belongs to the same producer and issuer.  Gated stages are larger, and two of them too few
+  // (64 x 4096 x 2 x 4096: 12.9 us, with four 11.4).
+  static constexpr int kStages = kGated ? 200 * 1024 / kStageBytes : 111 * 1024 / kStageBytes & ~1;
   static constexpr int kPartialBytes = kWeights * BN * 128 * 4;
   static constexpr int kSmemBytes = kStages * kStageBytes + 1024 /*align*/ + 256 /*barriers*/;
-  static constexpr int kScaleCols = 4 * (kWeights + 1);
-  static constexpr int kScales = kWeights * BN;  // first scale column, a set per stage
+  // Tensor memory: two accumulators, then each stage's scale columns (weights' 4 and X's 4, for each issuer of the stage).
+  static constexpr int kScales = 2 * BN;
+  static constexpr int kScaleCols = 8 * kWeights;
   static constexpr int kUsedCols = kScales + kStages * kScaleCols;
   static constexpr int kTmemCols = kUsedCols <= 64 ? 64 : kUsedCols <= 128 ? 128 : 256;
   static_assert(kUsedCols <= 256, "two CTAs share an SM's tensor memory");
@@ -421,7 +431,7 @@ struct MxFewCfg {
 };
 
 template <int BN, bool kGated>
-__global__ void __launch_bounds__(kMxThreadsFew)
+__global__ void __launch_bounds__(kMxThreadsFew, kGated ? 1 : 2)
     mx8_linear_few_kernel(const __grid_constant__ MxMaps maps, const __grid_constant__ MxLinearArgs args) {
   using Cfg = MxFewCfg<BN, kGated>;
   constexpr int S = Cfg::kStages;
@@ -435,8 +445,8 @@ __global__ void __launch_bounds__(kMxThreadsFew)
   uint64_t* full = bars;
   uint64_t* empty = bars + S;
   uint64_t* tfull = bars + 2 * S;
-  uint64_t* drain = bars + 2 * S + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 2);
+  uint64_t* drain = bars + 2 * S + 1;  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 3);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* partial = reinterpret_cast<float*>(smem);  // [W][BN][128], over the stages once they are consumed
   const unsigned long long wait_ns = wait_limit(args.wait_ns);
@@ -447,17 +457,19 @@ __global__ void __launch_bounds__(kMxThreadsFew)
   const int k_tiles = (args.K + kMxBK - 1) / kMxBK;
   const int kb0 = (int)((int64_t)k_tiles * rank / split), kb1 = (int)((int64_t)k_tiles * (rank + 1) / split);
   const int k_blocks = kb1 - kb0;  // at least 1: split <= k_tiles
+  const int issuers = kGated || k_blocks > 1 ? 2 : 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    mbar_init(tfull, 1);
-    mbar_init(drain, 1);
+    for (int s = 0; s < S; ++s) { mbar_init(&full[s], W); mbar_init(&empty[s], W); }
+    mbar_init(tfull, issuers);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 4 && lane == 0) {
+  if (warp == 4 && lane == 0) { tma_prefetch_desc(&maps.w); tma_prefetch_desc(&maps.ws); }
+  if (warp == 7 && lane == 0) {
     tma_prefetch_desc(&maps.x); tma_prefetch_desc(&maps.xs);
-    tma_prefetch_desc(&maps.w); tma_prefetch_desc(&maps.ws);
     if (kGated) { tma_prefetch_desc(&maps.g); tma_prefetch_desc(&maps.gs); }
   }
   if (warp == 5) { tmem_alloc(tmem_slot, Cfg::kTmemCols); tmem_relinquish(); }
@@ -467,23 +479,28 @@ __global__ void __launch_bounds__(kMxThreadsFew)
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
 
-  if (warp == 4) {
+  if (warp == 4 || warp == 7) {
+    const int who = warp == 4 ? 0 : 1;
     uint32_t issued = 0, last_par = 0;
-    for (int b = 0; b < k_blocks; ++b) {
+    for (int b = kGated ? 0 : who; b < k_blocks; b += kGated ? 1 : 2) {
       const int stage = b % S; const uint32_t phase = (b / S) & 1;
       if (!warp_wait(&empty[stage], phase ^ 1, args.err, kErrGemmProducerWait, abort_flag, wait_ns)) break;
       if (elect_one()) {
-        mbar_arrive_expect_tx(&full[stage], Cfg::kStageBytes);
         const int kb = kb0 + b;
+        uint8_t* a = sA + stage * W * kMxOperandBytes;
         uint8_t* sc = sS + stage * Cfg::kStageScales;
-        tma_load_2d(sA + stage * W * kMxOperandBytes, &maps.w, &full[stage], kb * kMxBK, f0);
-        tma_load_3d(sc, &maps.ws, &full[stage], 0, kb, f0 / 128);
-        if (kGated) {
-          tma_load_2d(sA + (stage * W + 1) * kMxOperandBytes, &maps.g, &full[stage], kb * kMxBK, f0);
+        if (!kGated || who == 0) {
+          mbar_arrive_expect_tx(&full[stage], kGated ? kMxOperandBytes + 2 * kMxTileBytes : Cfg::kStageBytes);
+          tma_load_2d(a, &maps.w, &full[stage], kb * kMxBK, f0);
+          tma_load_3d(sc, &maps.ws, &full[stage], 0, kb, f0 / 128);
+          tma_load_3d(sc + W * kMxTileBytes, &maps.xs, &full[stage], 0, kb, t0 / 128);
+        }
+        if (kGated && who == 1) {
+          mbar_arrive_expect_tx(&full[stage], kMxOperandBytes + kMxTileBytes + Cfg::kStageB);
+          tma_load_2d(a + kMxOperandBytes, &maps.g, &full[stage], kb * kMxBK, f0);
           tma_load_3d(sc + kMxTileBytes, &maps.gs, &full[stage], 0, kb, f0 / 128);
         }
-        tma_load_2d(sB + stage * Cfg::kStageB, &maps.x, &full[stage], kb * kMxBK, t0);
-        tma_load_3d(sc + W * kMxTileBytes, &maps.xs, &full[stage], 0, kb, t0 / 128);
+        if (!kGated || who == 1) tma_load_2d(sB + stage * Cfg::kStageB, &maps.x, &full[stage], kb * kMxBK, t0);
       }
       issued |= 1u << stage;
       last_par = (last_par & ~(1u << stage)) | (phase << stage);
@@ -491,10 +508,14 @@ __global__ void __launch_bounds__(kMxThreadsFew)
     if (lane == 0)
       for (int s = 0; s < S; ++s)
         if (issued & (1u << s)) mbar_drain(&full[s], (last_par >> s) & 1);
-  } else if (warp == 5) {
-    const uint64_t adesc = smem_desc_sw128(smem_u32(sA)), bdesc = smem_desc_sw128(smem_u32(sB));
+  } else if (warp == 5 || warp == 6) {
+    const int who = warp - 5;
+    const uint64_t adesc = smem_desc_sw128(smem_u32(sA) + (kGated ? who * kMxOperandBytes : 0));
+    const uint64_t bdesc = smem_desc_sw128(smem_u32(sB));
     const uint64_t sdesc = mx_scale_desc(smem_u32(sS));
-    for (int b = 0; b < k_blocks; ++b) {
+    const uint32_t d = tmem + who * BN;
+    const int first = kGated ? 0 : who, step = kGated ? 1 : 2;
+    for (int b = first; b < k_blocks; b += step) {
       const int stage = b % S;
       if (!warp_wait(&full[stage], (b / S) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) break;
       tc_fence_after();
@@ -503,25 +524,22 @@ __global__ void __launch_bounds__(kMxThreadsFew)
         const uint64_t x = bdesc + (uint64_t)(stage * (Cfg::kStageB >> 4));
         const uint64_t sc = sdesc + (uint64_t)(stage * (Cfg::kStageScales >> 4));
         // The stage's own scale columns: its last MMAs were done before it was filled again.
-        const uint32_t ts = tmem + Cfg::kScales + stage * Cfg::kScaleCols;
-#pragma unroll
-        for (int j = 0; j <= W; ++j) mx_copy_scales<false>(ts + 4 * j, sc + j * (kMxTileBytes >> 4));
+        const uint32_t ts = tmem + Cfg::kScales + stage * Cfg::kScaleCols + (kGated ? 8 * who : 0);
+        mx_copy_scales<false>(ts, sc + (kGated ? who * (kMxTileBytes >> 4) : 0));
+        mx_copy_scales<false>(ts + 4, sc + W * (kMxTileBytes >> 4));
         // Tokens t0 .. t0 + BN - 1 are the lanes from column (t0 % 128) / 32 of their scale tile on.
-        const uint32_t xs = ts + 4 * W + (t0 % 128) / 32;
+        const uint32_t xs = ts + 4 + (t0 % 128) / 32;
 #pragma unroll
-        for (int j = 0; j < W; ++j)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mx_mma<false>(tmem + j * BN, a + j * (kMxOperandBytes >> 4) + 2 * k, x + 2 * k, mx_idesc(128, BN, k), ts + 4 * j, xs,
-                          (b > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < 4; ++k)
+          mx_mma<false>(d, a + 2 * k, x + 2 * k, mx_idesc(128, BN, k), ts, xs, (b > first || k > 0) ? 1u : 0u);
         tc_commit(&empty[stage]);
-        if (b == k_blocks - 1) tc_commit(tfull);
+        if (b + step >= k_blocks) tc_commit(tfull);
       }
       __syncwarp();
     }
     if (elect_one()) {
-      tc_commit(drain);
-      mbar_drain(drain, 0);
+      tc_commit(&drain[who]);
+      mbar_drain(&drain[who], 0);
     }
   } else {
     // This CTA's sums: lane = feature, columns = rows of X.
@@ -529,43 +547,62 @@ __global__ void __launch_bounds__(kMxThreadsFew)
       tc_fence_after();
       const uint32_t tbase = tmem + ((uint32_t)(warp * 32) << 16);
 #pragma unroll
-      for (int c = 0; c < W * BN / 16; ++c) {
-        uint32_t r[16];
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-            "tcgen05.wait::ld.sync.aligned;"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-            : "r"(tbase + c * 16)
-            : "memory");
+      for (int c = 0; c < BN / 16; ++c) {
+        float v[16], u[16];
+        tmem_ld16x2(tbase + c * 16, tbase + (issuers > 1 ? BN : 0) + c * 16, v, u);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) partial[(c * 16 + i) * 128 + warp * 32 + lane] = __uint_as_float(r[i]);
+        for (int i = 0; i < 16; ++i) {
+          float* p = partial + (c * 16 + i) * 128 + warp * 32 + lane;
+          if (kGated) {
+            p[0] = v[i];
+            p[BN * 128] = u[i];
+          } else {
+            p[0] = issuers > 1 ? v[i] + u[i] : v[i];
+          }
+        }
       }
       tc_fence_before();
     }
   }
   __syncwarp();
   cluster_sync();  // every CTA's sums are in its shared memory
-  if (warp < 4) {
-    const uint32_t mine = smem_u32(partial);
-    for (int t = rank * 4 + warp; t < BN && t0 + t < args.M; t += 4 * split) {  // one row of X per warp
-      float v[1][4] = {}, g[1][4] = {};
-      MxInputs<1> in;
-      mx_fetch<kGated, 1>(args, t0 + t, 1, f0 + 4 * lane, f0 + 128 <= args.N, in);
-      for (int r = 0; r < split; ++r) {
-        const uint32_t there = cluster_addr(mine, r) + (t * 128 + lane * 4) * 4;
-        float4 s;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(s.x), "=f"(s.y), "=f"(s.z), "=f"(s.w) : "r"(there));
-        v[0][0] += s.x; v[0][1] += s.y; v[0][2] += s.z; v[0][3] += s.w;
-        if (kGated) {
+  // Rows of X are dealt to the cluster's warps; a warp finishes R at a time, with all its loads from
+  // the other CTAs in flight together.
+  constexpr int R = kGated ? 1 : 2;
+  const uint32_t mine = smem_u32(partial) + lane * 16;
+  const int col = f0 + 4 * lane;
+  const int step = 8 * split, rows = min(BN, args.M - t0);
+  for (int t = rank * 8 + warp; t < rows; t += R * step) {
+    MxInputs<R> in;
+    mx_fetch<kGated, R>(args, t0 + t, step, t0 + rows, col, f0 + 128 <= args.N && t + (R - 1) * step < rows, in);
+    float4 s[R][kMxMaxSplit], u[kGated ? R : 1][kMxMaxSplit];
+#pragma unroll
+    for (int r = 0; r < kMxMaxSplit; ++r) {
+      if (r >= split) break;
+      const uint32_t there = cluster_addr(mine, r);
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const uint32_t at = there + min(t + k * step, BN - 1) * 512;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(s[k][r].x), "=f"(s[k][r].y), "=f"(s[k][r].z), "=f"(s[k][r].w) : "r"(at));
+        if constexpr (kGated)
           asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(s.x), "=f"(s.y), "=f"(s.z), "=f"(s.w)
-                       : "r"(there + BN * 128 * 4));
-          g[0][0] += s.x; g[0][1] += s.y; g[0][2] += s.z; g[0][3] += s.w;
+                       : "=f"(u[k][r].x), "=f"(u[k][r].y), "=f"(u[k][r].z), "=f"(u[k][r].w) : "r"(at + BN * 512));
+      }
+    }
+    float v[R][4] = {}, g[R][4] = {};
+#pragma unroll
+    for (int r = 0; r < kMxMaxSplit; ++r) {
+      if (r >= split) break;
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        v[k][0] += s[k][r].x; v[k][1] += s[k][r].y; v[k][2] += s[k][r].z; v[k][3] += s[k][r].w;
+        if constexpr (kGated) {
+          g[k][0] += u[k][r].x; g[k][1] += u[k][r].y; g[k][2] += u[k][r].z; g[k][3] += u[k][r].w;
         }
       }
-      mx_finish<kGated, 1>(args, t0 + t, 1, f0 + 4 * lane, v, g, in);
     }
+    mx_finish<kGated, R>(args, t0 + t, step, t0 + rows, col, v, g, in);
   }
   __syncwarp();
   cluster_sync();  // no CTA leaves while its sums are read

@@ -73,7 +73,8 @@ __device__ __forceinline__ void store4(T* p, int n, bool vec, const float* v) {
 // Epilogue of R rows by four columns per thread: the thread's rows row0, row0 + step, ..., columns
 // col .. col + 3 (col a multiple of 4).  Eight neighbouring threads hold 32 consecutive columns
 // of a row from a multiple of 32 on, and the warp calls these functions together (an MX8 block's scale is
-// found by shuffles).  Rows and columns outside the result are not read or written.
+// found by shuffles).  Rows from `end` on (at most M) and columns outside the result are not read or
+// written.
 //
 // MxInputs is what the epilogue reads beside the products.  It is fetched apart from its use, so
 // that a caller can have the next chunk's loads in flight: with the loads inside mx_finish, each behind
@@ -88,7 +89,7 @@ struct MxInputs {
 };
 
 template <bool kGated, int R>
-__device__ __forceinline__ void mx_fetch(const MxLinearArgs& a, int row0, int step, int col, bool whole, MxInputs<R>& in) {
+__device__ __forceinline__ void mx_fetch(const MxLinearArgs& a, int row0, int step, int end, int col, bool whole, MxInputs<R>& in) {
   const int n = max(0, min(4, a.N - col));
   in.whole = whole && a.out_vec && (!a.residual || a.residual_vec);
   if (a.bias) load4(a.bias + col, n, true, in.bias);
@@ -113,7 +114,7 @@ __device__ __forceinline__ void mx_fetch(const MxLinearArgs& a, int row0, int st
       for (int k = 0; k < R; ++k) {
         const int row = row0 + k * step;
         float t[4];
-        load4(p + (size_t)row * a.ldr + col, row < a.M ? n : 0, a.residual_vec, t);
+        load4(p + (size_t)row * a.ldr + col, row < end ? n : 0, a.residual_vec, t);
         in.res[k] = make_uint4(__float_as_uint(t[0]), __float_as_uint(t[1]), __float_as_uint(t[2]), __float_as_uint(t[3]));
       }
     };
@@ -126,8 +127,8 @@ __device__ __forceinline__ void mx_fetch(const MxLinearArgs& a, int row0, int st
 // acc: the products with W, gate: those with G.  Everything is fp32 and rounded once, to the
 // output's type.
 template <bool kGated, int R>
-__device__ __forceinline__ void mx_finish(const MxLinearArgs& a, int row0, int step, int col, float (&acc)[R][4],
-                                          float (&gate)[R][4], const MxInputs<R>& in) {
+__device__ __forceinline__ void mx_finish(const MxLinearArgs& a, int row0, int step, int end, int col,
+                                          float (&acc)[R][4], float (&gate)[R][4], const MxInputs<R>& in) {
   const int n = max(0, min(4, a.N - col));
   if (a.bias) {
 #pragma unroll
@@ -190,7 +191,7 @@ __device__ __forceinline__ void mx_finish(const MxLinearArgs& a, int row0, int s
       } else {
 #pragma unroll
         for (int k = 0; k < R; ++k)
-          if (row0 + k * step < a.M) store4(p + (size_t)(k * step) * a.ldo, n, a.out_vec, acc[k]);
+          if (row0 + k * step < end) store4(p + (size_t)(k * step) * a.ldo, n, a.out_vec, acc[k]);
       }
     };
     if (a.out_type == MX_BF16) write(static_cast<__nv_bfloat16*>(a.out));
@@ -212,7 +213,7 @@ __device__ __forceinline__ void mx_finish(const MxLinearArgs& a, int row0, int s
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
       const uint32_t byte = mx_scale_byte(m);
-      if (row < a.M) {
+      if (row < end) {
         if (in_values) *reinterpret_cast<uint32_t*>(q + (size_t)(k * step) * a.ldo) = mx_pack4(acc[k], mx_inverse(byte));
         if (in_scales)
           a.out_scales[mx_scale_tile(row, col_tile, col_tiles) + mx_scale_row(row) + ((col / kMxBlock) & 3)] = (uint8_t)byte;
