@@ -1,0 +1,674 @@
+// laya_cuda._mx8: the Python calls of the MX8 operators as a CPython extension.
+//
+// A single token's call spends its time on the host: through ctypes a linear layer's arguments took 4-6 us to
+// check and convert beside the 2.5 us of the kernel's launch, and the device waited.  Here the checks read the
+// tensors' attributes directly.  Tensors are anything with torch's `data_ptr`, `shape`, `stride`, `is_contiguous`,
+// `nbytes`, `dtype` and `get_device`; torch is not linked or imported.  The library's functions come by
+// address from laya_cuda._lib (`bind`), which loads it on the first call.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+#include <structmember.h>
+
+#include <cstddef>
+#include <cstring>
+
+#include "../../include/laya_b200.h"
+
+namespace {
+
+using ConvertFn = int (*)(const laya_mx8_convert*, void*);
+using NormFn = int (*)(const laya_rms_norm_mx8*, void*);
+using LinearFn = int (*)(const laya_mx8_linear*, int*, void*);
+using ErrorFn = const char* (*)(laya_engine*);
+
+struct Library {
+  ConvertFn quantize, dequantize;
+  NormFn rms_norm;
+  LinearFn linear;
+  ErrorFn last_error;
+} g_lib = {};
+PyObject* g_loader = nullptr;  // called before the first operator: it calls bind()
+
+enum Name { DATA_PTR, SHAPE, STRIDE, IS_CONTIGUOUS, NBYTES, DTYPE, GET_DEVICE, ELEMENT_SIZE, NUMEL, NAMES };
+PyObject* g_names[NAMES];
+constexpr const char* kNames[NAMES] = {"data_ptr", "shape", "stride", "is_contiguous", "nbytes", "dtype", "get_device",
+                                       "element_size", "numel"};
+
+// An attribute, or the result of a method without arguments, as an integer; -1 with an exception set on failure.
+long long integer(PyObject* value) {
+  if (!value) return -1;
+  const long long n = PyLong_AsLongLong(value);
+  Py_DECREF(value);
+  return n;
+}
+long long attribute(PyObject* o, Name name) { return integer(PyObject_GetAttr(o, g_names[name])); }
+long long method(PyObject* o, Name name) { return integer(PyObject_CallMethodNoArgs(o, g_names[name])); }
+bool failed(long long n) { return n == -1 && PyErr_Occurred(); }
+
+// Whether a tensor is contiguous; -1 on failure.
+int contiguous(PyObject* o) {
+  PyObject* r = PyObject_CallMethodNoArgs(o, g_names[IS_CONTIGUOUS]);
+  if (!r) return -1;
+  const int yes = PyObject_IsTrue(r);
+  Py_DECREF(r);
+  return yes;
+}
+
+// The row stride of a two-dimensional tensor, with the stride of its columns; false on failure.
+bool strides(PyObject* o, long long* row, long long* col) {
+  PyObject* r = PyObject_CallMethodNoArgs(o, g_names[STRIDE]);
+  if (!r) return false;
+  const bool ok = PyArg_ParseTuple(r, "LL", row, col);
+  Py_DECREF(r);
+  return ok;
+}
+
+// The shape of a tensor of `n` dimensions; 1 if it has another number of them, -1 on failure.
+int shape_of(PyObject* o, Py_ssize_t n, long long* dims) {
+  PyObject* s = PyObject_GetAttr(o, g_names[SHAPE]);
+  if (!s) return -1;
+  int status = 0;
+  if (!PyTuple_Check(s) || PyTuple_GET_SIZE(s) != n) {
+    status = 1;
+  } else {
+    for (Py_ssize_t i = 0; i < n && !status; ++i) {
+      dims[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(s, i));
+      if (failed(dims[i])) status = -1;
+    }
+  }
+  Py_DECREF(s);
+  return status;
+}
+
+// Raises ValueError, with a tensor's shape where the format asks for one (%S).
+void refuse_shape(const char* format, const char* what, long long rows, long long cols, PyObject* t) {
+  PyObject* s = PyObject_GetAttr(t, g_names[SHAPE]);
+  if (!s) return;
+  PyObject* shape = PySequence_Tuple(s);
+  Py_DECREF(s);
+  if (!shape) return;
+  PyErr_Format(PyExc_ValueError, format, what, rows, cols, shape);
+  Py_DECREF(shape);
+}
+
+// LAYA_DTYPE_* of a dtype object, kInt32 for int32, -1 for others, -2 on failure.  Dtypes are singletons: each is looked
+// at once by its name and then known by its address (the reference is kept).
+constexpr int kInt32 = 100;
+int dtype_code(PyObject* tensor) {
+  static struct {
+    PyObject* dtype;
+    int code;
+  } known[32];
+  static int count = 0;
+  PyObject* d = PyObject_GetAttr(tensor, g_names[DTYPE]);
+  if (!d) return -2;
+  for (int i = 0; i < count; ++i)
+    if (known[i].dtype == d) {
+      Py_DECREF(d);
+      return known[i].code;
+    }
+  PyObject* s = PyObject_Str(d);
+  const char* text = s ? PyUnicode_AsUTF8(s) : nullptr;
+  int code = -1;
+  if (!text) code = -2;
+  else if (!strcmp(text, "torch.float32")) code = LAYA_DTYPE_F32;
+  else if (!strcmp(text, "torch.float16")) code = LAYA_DTYPE_F16;
+  else if (!strcmp(text, "torch.bfloat16")) code = LAYA_DTYPE_BF16;
+  else if (!strcmp(text, "torch.int32")) code = kInt32;
+  Py_XDECREF(s);
+  if (code != -2 && count < 32) known[count++] = {d, code};  // keeps the reference
+  else Py_DECREF(d);
+  return code;
+}
+
+long long scale_bytes(long long rows, long long cols) { return (rows + 127) / 128 * ((cols + 127) / 128) * 512; }
+
+// ---------------------------------------------------------------------------------------------
+// Arguments: positional or by name, `required` of them at least; the others keep what `out` holds.
+// ---------------------------------------------------------------------------------------------
+template <size_t N>
+struct Signature {
+  const char* function;
+  const char* names[N];
+  PyObject* keys[N];  // the names interned, as call sites hold them
+};
+
+template <size_t N>
+bool parse(Signature<N>& sig, size_t required, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames, PyObject* (&out)[N]) {
+  if (nargs > (Py_ssize_t)N) {
+    PyErr_Format(PyExc_TypeError, "%s() takes at most %zu arguments (%zd given)", sig.function, N, nargs);
+    return false;
+  }
+  for (Py_ssize_t i = 0; i < nargs; ++i) out[i] = args[i];
+  const Py_ssize_t nkw = kwnames ? PyTuple_GET_SIZE(kwnames) : 0;
+  for (size_t i = 0; nkw && i < N; ++i)
+    if (!sig.keys[i] && !(sig.keys[i] = PyUnicode_InternFromString(sig.names[i]))) return false;
+  for (Py_ssize_t k = 0; k < nkw; ++k) {
+    PyObject* key = PyTuple_GET_ITEM(kwnames, k);
+    size_t at = 0;
+    while (at < N && key != sig.keys[at]) ++at;
+    if (at == N)
+      for (at = 0; at < N && PyUnicode_CompareWithASCIIString(key, sig.names[at]) != 0;) ++at;
+    if (at == N) {
+      PyErr_Format(PyExc_TypeError, "%s() got an unexpected keyword argument '%U'", sig.function, key);
+      return false;
+    }
+    if ((Py_ssize_t)at < nargs) {
+      PyErr_Format(PyExc_TypeError, "%s() got multiple values for argument '%s'", sig.function, sig.names[at]);
+      return false;
+    }
+    out[at] = args[nargs + k];
+  }
+  for (size_t i = 0; i < required; ++i)
+    if (!out[i]) {
+      PyErr_Format(PyExc_TypeError, "%s() missing required argument '%s'", sig.function, sig.names[i]);
+      return false;
+    }
+  return true;
+}
+
+bool to_int(PyObject* o, const char* what, int* out) {
+  const long long n = PyLong_AsLongLong(o);
+  if (failed(n)) return false;
+  if (n < -2147483647 || n > 2147483647) {
+    PyErr_Format(PyExc_ValueError, "%s = %lld is out of range", what, n);
+    return false;
+  }
+  *out = (int)n;
+  return true;
+}
+
+bool to_stream(PyObject* o, void** out) {
+  *out = nullptr;
+  if (!o) return true;
+  const unsigned long long n = PyLong_AsUnsignedLongLong(o);
+  if (n == (unsigned long long)-1 && PyErr_Occurred()) return false;
+  *out = reinterpret_cast<void*>(n);
+  return true;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Matrix
+// ---------------------------------------------------------------------------------------------
+struct Matrix {
+  PyObject_HEAD
+  PyObject* values;
+  PyObject* scales;
+  int rows, cols, device;
+  long long ld;
+  unsigned long long values_ptr, scales_ptr;
+};
+
+PyTypeObject MatrixType = {PyVarObject_HEAD_INIT(nullptr, 0)};
+
+// Fills `m` (without references) from its arguments.
+bool matrix_check(Matrix* m, PyObject* values, PyObject* scales, int rows, int cols) {
+  if (rows < 0 || cols < 1) {
+    PyErr_Format(PyExc_ValueError, "bad shape %d x %d: rows may be 0, columns may not", rows, cols);
+    return false;
+  }
+  const long long room = ((long long)cols + 15) / 16 * 16, need = scale_bytes(rows, cols);
+  int whole = contiguous(values);
+  if (whole < 0) return false;
+  const long long bytes = attribute(values, NBYTES);
+  if (failed(bytes)) return false;
+  m->ld = room;
+  if (!whole || bytes != rows * room) {
+    // Rows further apart than they need to be, of one-byte elements.
+    long long dims[2], row = 0, col = 0;
+    const int status = shape_of(values, 2, dims);
+    if (status < 0) return false;
+    const long long size = method(values, ELEMENT_SIZE);
+    if (failed(size)) return false;
+    if (!status && !strides(values, &row, &col)) return false;
+    if (status || dims[0] != rows || col != 1 || size != 1 || dims[1] < room) {
+      refuse_shape("%s of a %lld x %lld matrix must be bytes in as many contiguous rows, with room for a multiple of 16, got %S", "values",
+                   rows, cols, values);
+      return false;
+    }
+    if (rows > 1) m->ld = row;  // the stride of a single row says nothing
+  }
+  whole = contiguous(scales);
+  if (whole < 0) return false;
+  const long long held = attribute(scales, NBYTES);
+  if (failed(held)) return false;
+  if (!whole || held < need) {
+    PyErr_Format(PyExc_ValueError, "scales of a %d x %d matrix need %lld contiguous bytes", rows, cols, need);
+    return false;
+  }
+  const long long device = method(values, GET_DEVICE);
+  if (failed(device) && PyErr_Occurred()) return false;
+  const long long other = method(scales, GET_DEVICE);
+  if (failed(other) && PyErr_Occurred()) return false;
+  if (device < 0 || other != device) {
+    PyErr_SetString(PyExc_ValueError, "values and scales must be on the same CUDA device");
+    return false;
+  }
+  const long long v = method(values, DATA_PTR);
+  if (failed(v)) return false;
+  const long long s = method(scales, DATA_PTR);
+  if (failed(s)) return false;
+  m->rows = rows;
+  m->cols = cols;
+  m->device = (int)device;
+  m->values_ptr = (unsigned long long)v;
+  m->scales_ptr = (unsigned long long)s;
+  return true;
+}
+
+PyObject* matrix_make(PyTypeObject* type, PyObject* (&given)[4]) {
+  int rows, cols;
+  if (!to_int(given[2], "rows", &rows) || !to_int(given[3], "cols", &cols)) return nullptr;
+  Matrix filled;
+  if (!matrix_check(&filled, given[0], given[1], rows, cols)) return nullptr;
+  Matrix* m = reinterpret_cast<Matrix*>(type->tp_alloc(type, 0));
+  if (!m) return nullptr;
+  Py_INCREF(given[0]);
+  Py_INCREF(given[1]);
+  m->values = given[0];
+  m->scales = given[1];
+  m->rows = filled.rows; m->cols = filled.cols; m->device = filled.device; m->ld = filled.ld;
+  m->values_ptr = filled.values_ptr; m->scales_ptr = filled.scales_ptr;
+  return reinterpret_cast<PyObject*>(m);
+}
+
+Signature<4> g_matrix_args = {"Matrix", {"values", "scales", "rows", "cols"}, {}};
+
+PyObject* matrix_call(PyObject* type, PyObject* const* args, size_t nargsf, PyObject* kwnames) {
+  PyObject* given[4] = {};
+  if (!parse(g_matrix_args, 4, args, PyVectorcall_NARGS(nargsf), kwnames, given)) return nullptr;
+  return matrix_make(reinterpret_cast<PyTypeObject*>(type), given);
+}
+
+void matrix_dealloc(PyObject* self) {
+  Matrix* m = reinterpret_cast<Matrix*>(self);
+  Py_XDECREF(m->values);
+  Py_XDECREF(m->scales);
+  Py_TYPE(self)->tp_free(self);
+}
+
+PyObject* matrix_empty(PyObject* type, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  static Signature<3> sig = {"empty", {"like", "rows", "cols"}, {}};
+  PyObject* given[3] = {};
+  int rows, cols;
+  if (!parse(sig, 3, args, nargs, kwnames, given) || !to_int(given[1], "rows", &rows) || !to_int(given[2], "cols", &cols))
+    return nullptr;
+  if (rows < 0 || cols < 1) {
+    PyErr_Format(PyExc_ValueError, "bad shape %d x %d: rows may be 0, columns may not", rows, cols);
+    return nullptr;
+  }
+  // like.new_zeros(n).byte(): a uint8 tensor of n elements beside `like`.
+  auto bytes = [&](long long n) -> PyObject* {
+    PyObject* wide = PyObject_CallMethod(given[0], "new_zeros", "L", n);
+    if (!wide) return nullptr;
+    PyObject* narrow = PyObject_CallMethod(wide, "byte", nullptr);
+    Py_DECREF(wide);
+    return narrow;
+  };
+  const long long room = ((long long)cols + 15) / 16 * 16;
+  PyObject* flat = bytes(rows * room);
+  PyObject* values = flat ? PyObject_CallMethod(flat, "view", "LL", (long long)rows, room) : nullptr;
+  PyObject* scales = values ? bytes(scale_bytes(rows, cols)) : nullptr;
+  PyObject* made = nullptr;
+  if (scales) {
+    PyObject* parts[4] = {values, scales, given[1], given[2]};
+    made = matrix_make(reinterpret_cast<PyTypeObject*>(type), parts);
+  }
+  Py_XDECREF(flat);
+  Py_XDECREF(values);
+  Py_XDECREF(scales);
+  return made;
+}
+
+PyMemberDef matrix_members[] = {
+    {"values", T_OBJECT_EX, offsetof(Matrix, values), READONLY, nullptr},
+    {"scales", T_OBJECT_EX, offsetof(Matrix, scales), READONLY, nullptr},
+    {"rows", T_INT, offsetof(Matrix, rows), READONLY, nullptr},
+    {"cols", T_INT, offsetof(Matrix, cols), READONLY, nullptr},
+    {"ld", T_LONGLONG, offsetof(Matrix, ld), READONLY, "bytes from one row of values to the next"},
+    {"device", T_INT, offsetof(Matrix, device), READONLY, "index of the CUDA device"},
+    {nullptr, 0, 0, 0, nullptr}};
+
+PyMethodDef matrix_methods[] = {
+    {"empty", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(matrix_empty)), METH_FASTCALL | METH_KEYWORDS | METH_CLASS,
+     "empty(like, rows, cols)\n--\n\nBuffers for a matrix on the device of the torch tensor `like` (uint8, cleared)."},
+    {nullptr, nullptr, 0, nullptr}};
+
+// ---------------------------------------------------------------------------------------------
+// Tensors beside a matrix
+// ---------------------------------------------------------------------------------------------
+struct Rows {
+  void* ptr;
+  long long ld;
+  int dtype;
+};
+
+// A [rows][cols] tensor of 16- or 32-bit floats with contiguous rows, on `device`.
+bool take_rows(const char* name, PyObject* t, int rows, int cols, int device, Rows* out) {
+  long long dims[2];
+  const int status = shape_of(t, 2, dims);
+  if (status < 0) return false;
+  if (status || dims[0] != rows || dims[1] != cols) {
+    refuse_shape("%s must be [%lld][%lld], got %S", name, rows, cols, t);
+    return false;
+  }
+  out->ld = cols;
+  const int whole = contiguous(t);
+  if (whole < 0) return false;
+  if (!whole) {
+    long long row, col;
+    if (!strides(t, &row, &col)) return false;
+    if (cols > 1 && col != 1) {
+      PyErr_Format(PyExc_ValueError, "%s: the values of a row must be contiguous", name);
+      return false;
+    }
+    if (rows > 1) out->ld = row;
+  }
+  out->dtype = dtype_code(t);
+  if (out->dtype == -2) return false;
+  if (out->dtype < 0 || out->dtype == kInt32) {
+    PyErr_Format(PyExc_ValueError, "%s is not float32, float16 or bfloat16", name);
+    return false;
+  }
+  const long long on = method(t, GET_DEVICE);
+  if (failed(on) && PyErr_Occurred()) return false;
+  if (on != device) {
+    PyErr_Format(PyExc_ValueError, "%s is not on CUDA device %d, where the matrix is", name, device);
+    return false;
+  }
+  const long long p = method(t, DATA_PTR);
+  if (failed(p)) return false;
+  out->ptr = reinterpret_cast<void*>(p);
+  return true;
+}
+
+// `n` contiguous float32 values on `device`; null where `t` is absent or None.
+bool take_vector(const char* name, PyObject* t, int n, int device, const float** out) {
+  *out = nullptr;
+  if (!t || t == Py_None) return true;
+  long long dims[1];
+  const int status = shape_of(t, 1, dims);
+  if (status < 0) return false;
+  const int code = dtype_code(t);
+  if (code == -2) return false;
+  const int whole = contiguous(t);
+  if (whole < 0) return false;
+  const long long on = method(t, GET_DEVICE);
+  if (failed(on) && PyErr_Occurred()) return false;
+  if (status || dims[0] != n || code != LAYA_DTYPE_F32 || !whole || on != device) {
+    PyErr_Format(PyExc_ValueError, "%s must be %d contiguous float32 values on CUDA device %d", name, n, device);
+    return false;
+  }
+  const long long p = method(t, DATA_PTR);
+  if (failed(p)) return false;
+  *out = reinterpret_cast<const float*>(p);
+  return true;
+}
+
+Matrix* take_matrix(const char* name, PyObject* o) {
+  if (Py_TYPE(o) != &MatrixType) {
+    PyErr_Format(PyExc_TypeError, "%s must be a Matrix, not %s", name, Py_TYPE(o)->tp_name);
+    return nullptr;
+  }
+  return reinterpret_cast<Matrix*>(o);
+}
+
+bool ready() {
+  if (g_lib.linear) return true;
+  if (!g_loader) {
+    PyErr_SetString(PyExc_RuntimeError, "laya_cuda._mx8 is used through laya_cuda.mx8");
+    return false;
+  }
+  PyObject* r = PyObject_CallNoArgs(g_loader);
+  Py_XDECREF(r);
+  if (r && !g_lib.linear) PyErr_SetString(PyExc_RuntimeError, "the library was not bound");
+  return r && g_lib.linear;
+}
+
+// ValueError for refused arguments, RuntimeError for the rest, with the library's message.
+PyObject* finish(int status) {
+  if (status == LAYA_OK) Py_RETURN_NONE;
+  const char* text = g_lib.last_error(nullptr);
+  PyErr_SetString(status == LAYA_ERR_INVALID ? PyExc_ValueError : PyExc_RuntimeError, text ? text : "");
+  return nullptr;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Operators
+// ---------------------------------------------------------------------------------------------
+PyObject* convert(const char* tensor, Matrix* m, PyObject* t, PyObject* stream, ConvertFn Library::*call) {
+  Rows data;
+  void* st;
+  if (!take_rows(tensor, t, m->rows, m->cols, m->device, &data) || !to_stream(stream, &st) || !ready()) return nullptr;
+  laya_mx8_convert a{};
+  a.rows = m->rows; a.cols = m->cols; a.dtype = data.dtype;
+  a.values = reinterpret_cast<void*>(m->values_ptr); a.scales = reinterpret_cast<void*>(m->scales_ptr); a.ldv = m->ld;
+  a.data = data.ptr; a.ld = data.ld;
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = (g_lib.*call)(&a, st);
+  Py_END_ALLOW_THREADS
+  return finish(status);
+}
+
+Signature<3> g_quantize_args = {"quantize", {"x", "out", "stream"}, {}};
+Signature<3> g_dequantize_args = {"dequantize", {"x", "out", "stream"}, {}};
+
+PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  PyObject* g[3] = {};
+  if (!parse(g_quantize_args, 2, args, nargs, kwnames, g)) return nullptr;
+  Matrix* m = take_matrix("out", g[1]);
+  return m ? convert("x", m, g[0], g[2], &Library::quantize) : nullptr;
+}
+
+PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  PyObject* g[3] = {};
+  if (!parse(g_dequantize_args, 2, args, nargs, kwnames, g)) return nullptr;
+  Matrix* m = take_matrix("x", g[0]);
+  return m ? convert("out", m, g[1], g[2], &Library::dequantize) : nullptr;
+}
+
+PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  static Signature<7> sig = {"rms_norm", {"x", "weight", "out", "residual", "sum_out", "eps", "stream"}, {}};
+  PyObject* g[7] = {};
+  if (!parse(sig, 3, args, nargs, kwnames, g)) return nullptr;
+  Matrix* m = take_matrix("out", g[2]);
+  if (!m) return nullptr;
+  laya_rms_norm_mx8 a{};
+  Rows x, r = {}, s = {};
+  void* st;
+  if (!take_rows("x", g[0], m->rows, m->cols, m->device, &x)) return nullptr;
+  a.residual_dtype = x.dtype;
+  const bool residual = g[3] && g[3] != Py_None, sum = g[4] && g[4] != Py_None;
+  if (residual) {
+    if (!take_rows("residual", g[3], m->rows, m->cols, m->device, &r)) return nullptr;
+    a.residual_dtype = r.dtype;
+  }
+  if (sum) {
+    if (!take_rows("sum_out", g[4], m->rows, m->cols, m->device, &s)) return nullptr;
+    if (residual && s.dtype != r.dtype) {
+      PyErr_SetString(PyExc_ValueError, "sum_out must have the residual's type");
+      return nullptr;
+    }
+    a.residual_dtype = s.dtype;
+  }
+  if (g[1] == Py_None) {
+    PyErr_SetString(PyExc_ValueError, "weight must be a tensor");
+    return nullptr;
+  }
+  if (!take_vector("weight", g[1], m->cols, m->device, &a.weight)) return nullptr;
+  a.eps = 1e-6f;
+  if (g[5]) {
+    const double eps = PyFloat_AsDouble(g[5]);
+    if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+    a.eps = (float)eps;
+  }
+  if (!to_stream(g[6], &st) || !ready()) return nullptr;
+  a.rows = m->rows; a.cols = m->cols; a.dtype = x.dtype;
+  a.x = x.ptr; a.ldx = x.ld; a.residual = r.ptr; a.ldr = r.ld; a.sum_out = s.ptr; a.lds = s.ld;
+  a.values = reinterpret_cast<void*>(m->values_ptr); a.scales = reinterpret_cast<void*>(m->scales_ptr); a.ldv = m->ld;
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_lib.rms_norm(&a, st);
+  Py_END_ALLOW_THREADS
+  return finish(status);
+}
+
+// LAYA_ACT_* of a name; -1 with an exception set for others.
+int activation(PyObject* o) {
+  if (!o) return LAYA_ACT_NONE;
+  if (PyUnicode_Check(o)) {
+    static constexpr const char* kActs[] = {"none", "relu", "gelu", "silu"};
+    for (int i = 0; i < 4; ++i)
+      if (PyUnicode_CompareWithASCIIString(o, kActs[i]) == 0) return i;
+  }
+  PyErr_Format(PyExc_ValueError, "activation %R is not one of none, relu, gelu, silu", o);
+  return -1;
+}
+
+PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  static Signature<10> sig = {"linear", {"x", "w", "out", "bias", "gate", "gate_bias", "activation", "residual", "err", "stream"}, {}};
+  PyObject* g[10] = {};
+  if (!parse(sig, 3, args, nargs, kwnames, g)) return nullptr;
+  Matrix *x = take_matrix("x", g[0]), *w = x ? take_matrix("w", g[1]) : nullptr;
+  if (!w) return nullptr;
+  const int rows = x->rows, cols = x->cols, n = w->rows, device = x->device;
+  if (w->cols != cols || w->device != device) {
+    PyErr_Format(PyExc_ValueError, "w is %d x %d on device %d, x has %d columns on device %d", n, w->cols, w->device, cols, device);
+    return nullptr;
+  }
+  laya_mx8_linear a{};
+  a.rows = rows; a.features = n; a.cols = cols;
+  a.activation = activation(g[6]);
+  if (a.activation < 0) return nullptr;
+  a.x = reinterpret_cast<void*>(x->values_ptr); a.x_scales = reinterpret_cast<void*>(x->scales_ptr); a.ldx = x->ld;
+  a.w = reinterpret_cast<void*>(w->values_ptr); a.w_scales = reinterpret_cast<void*>(w->scales_ptr); a.ldw = w->ld;
+  if (g[4] && g[4] != Py_None) {
+    Matrix* gate = take_matrix("gate", g[4]);
+    if (!gate) return nullptr;
+    if (gate->rows != n || gate->cols != cols || gate->device != device) {
+      PyErr_Format(PyExc_ValueError, "gate is %d x %d, w %d x %d", gate->rows, gate->cols, n, cols);
+      return nullptr;
+    }
+    a.gate = reinterpret_cast<void*>(gate->values_ptr); a.gate_scales = reinterpret_cast<void*>(gate->scales_ptr); a.ldg = gate->ld;
+  }
+  if (!take_vector("bias", g[3], n, device, &a.bias) || !take_vector("gate_bias", g[5], n, device, &a.gate_bias)) return nullptr;
+  Rows t;
+  if (g[7] && g[7] != Py_None) {
+    if (!take_rows("residual", g[7], rows, n, device, &t)) return nullptr;
+    a.residual = t.ptr; a.ldr = t.ld; a.residual_dtype = t.dtype;
+  }
+  if (Py_TYPE(g[2]) == &MatrixType) {
+    Matrix* out = reinterpret_cast<Matrix*>(g[2]);
+    if (out->rows != rows || out->cols != n || out->device != device) {
+      PyErr_Format(PyExc_ValueError, "out is %d x %d, the result %d x %d", out->rows, out->cols, rows, n);
+      return nullptr;
+    }
+    a.out = reinterpret_cast<void*>(out->values_ptr); a.out_scales = reinterpret_cast<void*>(out->scales_ptr); a.ldo = out->ld;
+    a.out_dtype = LAYA_DTYPE_MX8;
+  } else {
+    if (!take_rows("out", g[2], rows, n, device, &t)) return nullptr;
+    a.out = t.ptr; a.ldo = t.ld; a.out_dtype = t.dtype;
+  }
+  int* err = nullptr;
+  if (g[8] && g[8] != Py_None) {
+    const int code = dtype_code(g[8]);
+    if (code == -2) return nullptr;
+    const long long on = method(g[8], GET_DEVICE);
+    if (failed(on) && PyErr_Occurred()) return nullptr;
+    const long long count = method(g[8], NUMEL);
+    if (failed(count)) return nullptr;
+    if (code != kInt32 || on != device || count < 1) {
+      PyErr_Format(PyExc_ValueError, "err must be int32 on CUDA device %d", device);
+      return nullptr;
+    }
+    const long long p = method(g[8], DATA_PTR);
+    if (failed(p)) return nullptr;
+    err = reinterpret_cast<int*>(p);
+  }
+  void* st;
+  if (!to_stream(g[9], &st) || !ready()) return nullptr;
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_lib.linear(&a, err, st);
+  Py_END_ALLOW_THREADS
+  return finish(status);
+}
+
+PyObject* py_scale_bytes(PyObject*, PyObject* args) {
+  int rows, cols;
+  if (!PyArg_ParseTuple(args, "ii", &rows, &cols)) return nullptr;
+  if (rows < 0 || cols < 1) {
+    PyErr_Format(PyExc_ValueError, "bad shape %d x %d: rows may be 0, columns may not", rows, cols);
+    return nullptr;
+  }
+  return PyLong_FromLongLong(scale_bytes(rows, cols));
+}
+
+PyObject* set_loader(PyObject*, PyObject* loader) {
+  Py_INCREF(loader);
+  Py_XSETREF(g_loader, loader);
+  Py_RETURN_NONE;
+}
+
+PyObject* bind(PyObject*, PyObject* args) {
+  unsigned long long q, d, n, l, e;
+  if (!PyArg_ParseTuple(args, "KKKKK", &q, &d, &n, &l, &e)) return nullptr;
+  g_lib = {reinterpret_cast<ConvertFn>(q), reinterpret_cast<ConvertFn>(d), reinterpret_cast<NormFn>(n),
+           reinterpret_cast<LinearFn>(l), reinterpret_cast<ErrorFn>(e)};
+  Py_RETURN_NONE;
+}
+
+#define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL | METH_KEYWORDS
+PyMethodDef methods[] = {
+    {"quantize", FAST(quantize), "quantize(x, out, stream=0)\n--\n\nx [rows][cols] in 16 or 32 bits -> the Matrix `out`."},
+    {"dequantize", FAST(dequantize), "dequantize(x, out, stream=0)\n--\n\nThe Matrix `x` -> out [rows][cols] in 16 or 32 bits."},
+    {"rms_norm", FAST(rms_norm),
+     "rms_norm(x, weight, out, residual=None, sum_out=None, eps=1e-6, stream=0)\n--\n\n"
+     "h = x + residual; sum_out = h; out = h / sqrt(mean(h^2) + eps) * weight, in MX8.\n\n"
+     "`residual` and `sum_out` are optional, of one type, and may be the same tensor."},
+    {"linear", FAST(linear),
+     "linear(x, w, out, bias=None, gate=None, gate_bias=None, activation='none', residual=None, err=None, stream=0)\n--\n\n"
+     "out = act(x w^T + bias) + residual, or, with a `gate` matrix,\n"
+     "out = act(x gate^T + gate_bias) * (x w^T + bias) + residual.\n\n"
+     "x: Matrix [rows][cols]; w, gate: Matrix [features][cols]; out: a Matrix or a tensor\n"
+     "[rows][features].  bias, gate_bias: float32 [features].  residual: [rows][features] in 16 or 32\n"
+     "bits, added before the one rounding; it may be `out` itself.  activation: 'none', 'relu', 'gelu' (erf)\n"
+     "or 'silu'.  err: an int32 tensor, zero on entry, that receives a device error."},
+    {"scale_bytes", py_scale_bytes, METH_VARARGS,
+     "scale_bytes(rows, cols)\n--\n\nBytes of the scales of an MX8 matrix (tiles of 128 rows x 128 columns, 512 bytes each)."},
+    {"set_loader", set_loader, METH_O, "set_loader(f)\n--\n\nf() is called before the first operator and calls bind()."},
+    {"bind", bind, METH_VARARGS, "bind(quantize, dequantize, rms_norm, linear, last_error)\n--\n\nAddresses of the library's functions."},
+    {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mx8", nullptr, -1, methods};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__mx8() {
+  for (int i = 0; i < NAMES; ++i)
+    if (!(g_names[i] = PyUnicode_InternFromString(kNames[i]))) return nullptr;
+  MatrixType.tp_name = "laya_cuda.mx8.Matrix";
+  MatrixType.tp_basicsize = sizeof(Matrix);
+  MatrixType.tp_flags = Py_TPFLAGS_DEFAULT;
+  MatrixType.tp_doc =
+      "Matrix(values, scales, rows, cols)\n--\n\n"
+      "An MX8 matrix [rows][cols]: `values`, bytes in `rows` rows of cols rounded up to a multiple of\n"
+      "16, and `scales`, `scale_bytes(rows, cols)` bytes.  Both are contiguous, of any type of that many\n"
+      "bytes; two-dimensional values of one-byte elements may have a larger row stride.  Holds\n"
+      "references to both buffers.";
+  MatrixType.tp_dealloc = matrix_dealloc;
+  MatrixType.tp_vectorcall = matrix_call;
+  MatrixType.tp_members = matrix_members;
+  MatrixType.tp_methods = matrix_methods;
+  if (PyType_Ready(&MatrixType) < 0) return nullptr;
+  PyObject* m = PyModule_Create(&module);
+  if (!m) return nullptr;
+  Py_INCREF(&MatrixType);
+  if (PyModule_AddObject(m, "Matrix", reinterpret_cast<PyObject*>(&MatrixType)) < 0) {
+    Py_DECREF(&MatrixType);
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

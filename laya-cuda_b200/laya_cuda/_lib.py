@@ -112,7 +112,6 @@ def load():
         "laya_op_head_tail": (i, [i, p, p, p, i, i, i, p, p, p, p, p, p, i, p, p, p, p, p, p]),
         "laya_op_gemm_residual_static": (i, [i, p, p, i, i, i, i, p, p, p, p]),
     }
-    # The argument structures are passed by address or as their packed bytes (see mx8.py).
     sig |= {
         "laya_mx8_scale_bytes": (ct.c_int64, [i, i]),
         "laya_op_mx8_quantize": (i, [p, p]),

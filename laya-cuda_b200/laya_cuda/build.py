@@ -1,4 +1,4 @@
-"""Builds liblaya_b200.so in-tree with nvcc for sm_100a (B200).
+"""Builds liblaya_b200.so in-tree with nvcc for sm_100a (B200), and the Python extension _mx8.so.
 
     python -m laya_cuda.build            # from laya-cuda_b200/
 """
@@ -6,6 +6,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -14,6 +15,8 @@ INCLUDE = PACKAGE.parents[1] / "include"
 TARGET = PACKAGE / "liblaya_b200.so"
 SOURCES = [CSRC / "laya_b200.cu", CSRC / "mx8.cu"]
 DEPENDS = SOURCES + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "laya_b200.h"]
+EXTENSION = PACKAGE / "_mx8.so"
+EXTENSION_SOURCE = CSRC / "mx8_python.cpp"
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
          "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "--threads", "2"]
 
@@ -25,22 +28,28 @@ def nvcc():
     return found
 
 
-def up_to_date():
-    if not TARGET.exists():
+def up_to_date(target, depends):
+    if not target.exists():
         return False
-    built = TARGET.stat().st_mtime
-    return all(p.stat().st_mtime <= built for p in DEPENDS)
+    built = target.stat().st_mtime
+    return all(p.stat().st_mtime <= built for p in depends)
 
 
-def build(force=False, verbose=False):
-    if not force and up_to_date():
-        return TARGET
-    tmp = TARGET.with_suffix(".so.tmp")
-    cmd = [nvcc(), *FLAGS, "-I", str(INCLUDE), "-o", str(tmp), *map(str, SOURCES)]
+def run(target, cmd, verbose):
+    tmp = target.with_suffix(".so.tmp")
+    cmd = [*cmd[:1], "-o", str(tmp), *cmd[1:]]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
-    os.replace(tmp, TARGET)
+    os.replace(tmp, target)
+
+
+def build(force=False, verbose=False):
+    if force or not up_to_date(TARGET, DEPENDS):
+        run(TARGET, [nvcc(), *FLAGS, "-I", str(INCLUDE), *map(str, SOURCES)], verbose)
+    if force or not up_to_date(EXTENSION, [EXTENSION_SOURCE, INCLUDE / "laya_b200.h"]):
+        run(EXTENSION, [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+                        "-I", sysconfig.get_paths()["include"], str(EXTENSION_SOURCE)], verbose)
     return TARGET
 
 

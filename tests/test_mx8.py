@@ -1,6 +1,7 @@
 """The MX8 operators' host side (no GPU): buffer sizes, and arguments refused before any CUDA call."""
 import ctypes as ct
 
+import numpy as np
 import pytest
 
 from laya_cuda import _lib, mx8
@@ -93,12 +94,124 @@ def test_no_rows_needs_no_buffers_and_no_device(lib):
     assert lib.laya_op_mx8_linear(ct.byref(linear(rows=0, x=None, w=None, out=None)), None, None) == 0
 
 
-@pytest.mark.parametrize("cls", [_lib.Mx8Convert, _lib.RmsNormMx8, _lib.Mx8Linear])
-def test_packed_arguments_are_the_structure(cls):
-    values = [k + 1 if kind is not ct.c_float else 0.5 for k, (_, kind) in enumerate(cls._fields_)]
-    packed = mx8._packer(cls)(*values)
-    filled = cls.from_buffer_copy(packed)
-    assert [getattr(filled, name) for name, _ in cls._fields_] == values
+class Fake:
+    """Stands for a contiguous CUDA tensor; counts nothing and holds nothing."""
+
+    def __init__(self, shape, dtype="torch.float32", size=4, device=0, stride=None, ptr=P):
+        self.shape, self.dtype, self.size, self.device, self.ptr = tuple(shape), DTYPES[dtype], size, device, ptr
+        self.strides = stride or tuple(int(np.prod(shape[k + 1:])) for k in range(len(shape)))
+        self.nbytes = int(np.prod(shape)) * size
+
+    def stride(self):
+        return self.strides
+
+    def is_contiguous(self):
+        return self.strides == tuple(int(np.prod(self.shape[k + 1:])) for k in range(len(self.shape)))
+
+    def element_size(self):
+        return self.size
+
+    def numel(self):
+        return int(np.prod(self.shape))
+
+    def get_device(self):
+        return self.device
+
+    def data_ptr(self):
+        return self.ptr
+
+
+class Dtype:
+    def __init__(self, name):
+        self.name = name
+
+    def __str__(self):
+        return self.name
+
+
+DTYPES = {n: Dtype(n) for n in ("torch.float32", "torch.float16", "torch.bfloat16", "torch.uint8", "torch.int32", "torch.float64")}
+
+
+def u8(*shape, **other):
+    return Fake(shape, "torch.uint8", 1, **other)
+
+
+def matrix(rows, cols, device=0):
+    return mx8.Matrix(u8(rows, (cols + 15) // 16 * 16, device=device), u8(mx8.scale_bytes(rows, cols), device=device), rows, cols)
+
+
+def test_matrix_reads_its_buffers():
+    m = mx8.Matrix(u8(5, 64, stride=(80, 1), ptr=0x2000), u8(512, ptr=0x4000), rows=5, cols=50)
+    assert (m.rows, m.cols, m.ld, m.device) == (5, 50, 80, 0)
+    assert mx8.Matrix(u8(320), u8(600), 5, 50).ld == 64            # flat bytes
+    assert mx8.Matrix(u8(1, 112, stride=(7, 1)), u8(512), 1, 100).ld == 112  # a single row's stride says nothing
+
+
+@pytest.mark.parametrize("values,scales,rows,cols,word", [
+    (u8(5, 48), u8(512), 5, 50, "bytes"), (u8(4, 64), u8(512), 5, 50, "bytes"), (u8(5, 64, 1, stride=(128, 2, 1)), u8(512), 5, 50, "bytes"),
+    (u8(5, 64, stride=(64, 2)), u8(512), 5, 50, "bytes"), (Fake((5, 128), size=4, stride=(256, 1)), u8(512), 5, 50, "bytes"),
+    (u8(5, 64), u8(511), 5, 50, "scales"), (u8(5, 64), u8(1024, stride=(2,)), 5, 50, "scales"), (u8(5, 64), u8(512, device=1), 5, 50, "CUDA"),
+    (u8(5, 64, device=-1), u8(512, device=-1), 5, 50, "CUDA"), (u8(5, 64), u8(512), -1, 50, "shape"), (u8(5, 64), u8(512), 5, 0, "shape"),
+    (u8(5, 64), u8(512), 2 ** 40, 50, "range"),
+])
+def test_matrix_refuses(values, scales, rows, cols, word):
+    with pytest.raises(ValueError, match=word):
+        mx8.Matrix(values, scales, rows, cols)
+
+
+@pytest.mark.parametrize("call,word", [
+    (lambda: mx8.quantize(Fake((4, 31)), matrix(4, 32)), r"x must be \[4\]\[32\], got \(4, 31\)"),
+    (lambda: mx8.quantize(Fake((128,)), matrix(4, 32)), "must be"),
+    (lambda: mx8.quantize(Fake((4, 32), "torch.float64", 8), matrix(4, 32)), "float32"),
+    (lambda: mx8.quantize(Fake((4, 32), "torch.int32"), matrix(4, 32)), "float32"),
+    (lambda: mx8.quantize(Fake((4, 32), device=1), matrix(4, 32)), "device"),
+    (lambda: mx8.dequantize(matrix(4, 32), Fake((4, 32), stride=(1, 4))), "contiguous"),
+    (lambda: mx8.dequantize(matrix(4, 32), Fake((4, 32), stride=(16, 1))), "stride"),
+    (lambda: mx8.dequantize(matrix(4, 32), Fake((4, 32), ptr=P + 2)), "aligned"),
+    (lambda: mx8.rms_norm(Fake((4, 32)), Fake((31,)), matrix(4, 32)), "weight"),
+    (lambda: mx8.rms_norm(Fake((4, 32)), None, matrix(4, 32)), "weight"),
+    (lambda: mx8.rms_norm(Fake((4, 32)), Fake((32,)), matrix(4, 32), eps=-1), "eps"),
+    (lambda: mx8.rms_norm(Fake((4, 32)), Fake((32,)), matrix(4, 32), residual=Fake((4, 32)),
+                          sum_out=Fake((4, 32), "torch.float16", 2)), "type"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 64), Fake((4, 8))), "columns"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32, device=1), Fake((4, 8))), "device"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32), matrix(4, 9)), "result"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32), Fake((4, 8)), activation="tanh"), "tanh"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32), Fake((4, 8)), activation=3), "activation"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32), Fake((4, 8)), gate=matrix(9, 32)), "gate"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32), Fake((4, 8)), gate_bias=Fake((8,))), "gate"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32), Fake((4, 8)), bias=Fake((8,), "torch.float16", 2)), "bias"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32), Fake((4, 8)), residual=Fake((4, 8), stride=(0, 1))), "stride"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32), Fake((4, 8)), err=Fake((1,))), "err"),
+])
+def test_calls_refuse(call, word):
+    with pytest.raises(ValueError, match=word):
+        call()
+
+
+@pytest.mark.parametrize("call,word", [
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32)), "out"),
+    (lambda: mx8.linear(matrix(4, 32), Fake((8, 32)), Fake((4, 8))), "Matrix"),
+    (lambda: mx8.linear(matrix(4, 32), matrix(8, 32), Fake((4, 8)), gate=Fake((8, 32))), "Matrix"),
+    (lambda: mx8.quantize(Fake((4, 32)), matrix(4, 32), speed=1), "speed"),
+    (lambda: mx8.quantize(Fake((4, 32)), matrix(4, 32), out=matrix(4, 32)), "multiple"),
+    (lambda: mx8.quantize(Fake((4, 32)), matrix(4, 32), 0, 0), "at most"),
+    (lambda: mx8.quantize(Fake((4, 32)), matrix(4, 32), stream="s"), "int"),
+    (lambda: mx8.Matrix(u8(5, 64), u8(512), 5), "cols"),
+])
+def test_calls_refuse_other_types(call, word):
+    with pytest.raises(TypeError, match=word):
+        call()
+
+
+def test_a_failing_tensor_attribute_is_passed_on():
+    class Broken(Fake):
+        def data_ptr(self):
+            raise OSError("gone")
+    with pytest.raises(OSError, match="gone"):
+        mx8.quantize(Broken((4, 32)), matrix(4, 32))
+    with pytest.raises(AttributeError):
+        mx8.quantize(object(), matrix(4, 32))
 
 
 def test_tensors_on_the_host_are_refused():
