@@ -387,9 +387,16 @@ int laya_op_mx8_linear(const laya_mx8_linear* p, int* err, void* stream) {
   a.gate = {static_cast<const uint8_t*>(p->gate), p->ldg, static_cast<const uint8_t*>(p->gate_scales)};
   a.bias = p->bias; a.gate_bias = p->gate_bias; a.act = p->activation;
   a.residual = p->residual; a.ldr = p->ldr; a.residual_type = p->residual_dtype;
-  if (p->residual) a.residual_vec = vec4(p->residual, p->ldr, dtype_size(p->residual_dtype));
+  auto wide = [](const void* q, int64_t ld, size_t size) {
+    return reinterpret_cast<uintptr_t>(q) % 32 == 0 && ld * (int64_t)size % 32 == 0;
+  };
+  if (p->residual) {
+    a.residual_vec = vec4(p->residual, p->ldr, dtype_size(p->residual_dtype));
+    a.residual_wide = wide(p->residual, p->ldr, dtype_size(p->residual_dtype));
+  }
   a.out = p->out; a.ldo = p->ldo; a.out_type = p->out_dtype; a.out_scales = static_cast<uint8_t*>(p->out_scales);
   a.out_vec = p->out_dtype == LAYA_DTYPE_MX8 || vec4(p->out, p->ldo, dtype_size(p->out_dtype));
+  a.out_wide = wide(p->out, p->ldo, p->out_dtype == LAYA_DTYPE_MX8 ? 1 : dtype_size(p->out_dtype));
   a.err = err;
   a.wait_ns = wait_ns();
   if (gated) launch_linear<true>(a, dev, st);

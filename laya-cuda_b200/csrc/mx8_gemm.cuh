@@ -105,25 +105,6 @@ __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a_desc, uint64_t b_d
         : "memory");
 }
 
-// A warp's 32 x 32 fp32 staging block (rows of 128 bytes, 16-byte pieces swizzled by row): lanes
-// write the tile row that tensor memory gives them and read four columns of rows 4k + lane / 8.
-__device__ __forceinline__ void mx_stage_put(uint8_t* buf, int lane, const uint32_t (&v)[32]) {
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-        make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  __syncwarp();
-}
-__device__ __forceinline__ void mx_stage_get(const uint8_t* buf, int lane, float (&v)[8][4]) {
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int r = 4 * k + (lane >> 3);
-    const float4 t = *reinterpret_cast<const float4*>(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-    v[k][0] = t.x; v[k][1] = t.y; v[k][2] = t.z; v[k][3] = t.w;
-  }
-}
-
 // ---------------------------------------------------------------------------------------------
 // Many rows: CTA pairs (cta_group::2), 256 x BN output tiles, persistent.  Each CTA holds its
 // 128 rows of X, half of the tile's rows of W (gated: rank 0 the rows of G and rank 1 those of W, the
@@ -310,6 +291,18 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
     uint8_t* buf = epi + (warp - 2) * 4096;
     const uint32_t bar_shared = cluster_addr(smem_u32(shared), 0);
     constexpr int kChunks = kOutCols / 64;  // 32-column chunks of this warp
+    auto prefetch = [&](int t) {
+      if (!args.residual_wide) return;
+      const int mb = t / n_blocks, nb = t - mb * n_blocks;
+      const int row = mb * 256 + (int)rank * 128 + quarter * 32 + lane, c0 = nb * kOutCols + half * kChunks * 32;
+      const int size = args.residual_type == MX_F32 ? 4 : 2;
+      const int bytes = min(kChunks * 32, args.N - c0) * size & ~15;
+      if (row < args.M && bytes > 0)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
+                         static_cast<const char*>(args.residual) + ((size_t)row * args.ldr + c0) * size),
+                     "r"(bytes));
+    };
+    if (pair < tiles) prefetch(pair);
     int i = 0;
     for (int t = pair; t < tiles; t += pairs, ++i) {
       const int acc = i & 1;
@@ -318,26 +311,17 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
       // Outwards in: the shared columns are the second half's last of accumulator 0 and the first
       // half's first of accumulator 1.
       auto chunk = [&](int j) { return half ? 2 * kChunks - 1 - j : j; };
-      auto fetch = [&](int j, MxInputs<8>& in) {
-        const int c0 = nb * kOutCols + chunk(j) * 32;
-        mx_fetch<kGated, 8>(args, row0 + (lane >> 3), 4, args.M, c0 + 4 * (lane & 7), row0 + 32 <= args.M && c0 + 32 <= args.N, in);
-      };
-      // The first chunk's inputs are loaded while the tile's MMAs run; the other chunks' residual is
-      // brought into L2 then and loaded one chunk ahead of its use.
-      MxInputs<8> in;
+      const int row = row0 + lane;
+      auto fetch = [&](int j, MxResidualRow& in) { mx_fetch_row(args, row, nb * kOutCols + chunk(j) * 32, in); };
+      // The first chunk's residual is loaded while the tile's MMAs run, the others' one chunk ahead of their
+      // use, from L2: a tile's rows are brought there a tile ahead.
+      MxResidualRow in;
       fetch(0, in);
-      if (args.residual && row0 + lane < args.M) {
-        const int size = args.residual_type == MX_F32 ? 4 : 2;
-        const char* r = static_cast<const char*>(args.residual) + (size_t)(row0 + lane) * args.ldr * size;
-#pragma unroll
-        for (int j = 1; j < kChunks; ++j) {
-          const int c0 = nb * kOutCols + chunk(j) * 32;
-          if (c0 < args.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(r + (size_t)c0 * size));
-        }
-      }
+      if (t + pairs < tiles) prefetch(t + pairs);
       if (!warp_wait(&tfull[acc], (i >> 1) & 1, args.err, kErrGemmEpilogueWait, abort_flag, wait_ns)) break;
       tc_fence_after();
       const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (acc ? Cfg::kAcc1 : 0);
+      uint32_t scales = 0;  // MX8: this row's scale bytes of the warp's chunks
 #pragma unroll 1
       for (int j = 0; j < kChunks; ++j) {
         const int c = chunk(j);
@@ -359,15 +343,24 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster_relaxed(cluster_addr(smem_u32(&tempty[acc]), 0));
         }
-        float v[8][4], g[8][4];
-        mx_stage_put(buf, lane, r);
-        mx_stage_get(buf, lane, kGated ? g : v);
-        if constexpr (kGated) {
-          mx_stage_put(buf, lane, u);
-          mx_stage_get(buf, lane, v);
+        float v[32], g[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          v[k] = __uint_as_float(kGated ? u[kGated ? k : 0] : r[k]);
+          if (kGated) g[k] = __uint_as_float(r[k]);
         }
-        mx_finish<kGated, 8>(args, row0 + (lane >> 3), 4, args.M, nb * kOutCols + c * 32 + 4 * (lane & 7), v, g, in);
+        const uint32_t byte = mx_finish_row<kGated>(args, row, nb * kOutCols + c * 32, v, g, in, buf);
+        scales |= byte << (8 * (c & 3));
         if (j + 1 < kChunks) fetch(j + 1, in);
+      }
+      if (args.out_type == MX_MX8 && row < args.M) {
+        // Four chunks are a scale tile's four blocks, two its first or last two.
+        const int col = nb * kOutCols + half * kChunks * 32, col_tiles = mx_col_tiles(args.N), tile = col / kMxTileCols;
+        uint8_t* p = args.out_scales + mx_scale_tile(row, tile, col_tiles) + mx_scale_row(row);
+        if (tile < col_tiles) {
+          if (kChunks == 4) *reinterpret_cast<uint32_t*>(p) = scales;
+          else reinterpret_cast<uint16_t*>(p)[(col / 64) & 1] = (uint16_t)(scales >> (col & 64 ? 16 : 0));
+        }
       }
     }
   }

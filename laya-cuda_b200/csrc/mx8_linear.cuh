@@ -31,7 +31,8 @@ struct MxLinearArgs {
   int64_t ldo;
   int out_type;
   uint8_t* out_scales;        // MX8 output
-  int residual_vec, out_vec;  // four columns at a time may be read / written as one vector
+  int residual_vec, out_vec;    // four columns at a time may be read / written as one vector
+  int residual_wide, out_wide;  // and 32 bytes at a time, from columns that are multiples of 32 on
   int* err;
   unsigned long long wait_ns;
 };
@@ -70,16 +71,15 @@ __device__ __forceinline__ void store4(T* p, int n, bool vec, const float* v) {
   }
 }
 
-// Epilogue of R rows by four columns per thread: the thread's rows row0, row0 + step, ..., columns
+// ---------------------------------------------------------------------------------------------
+// Epilogue of R rows by four columns per thread (few rows): the thread's rows row0, row0 + step, ..., columns
 // col .. col + 3 (col a multiple of 4).  Eight neighbouring threads hold 32 consecutive columns
 // of a row from a multiple of 32 on, and the warp calls these functions together (an MX8 block's scale is
 // found by shuffles).  Rows from `end` on (at most M) and columns outside the result are not read or
 // written.
 //
 // MxInputs is what the epilogue reads beside the products.  It is fetched apart from its use, so
-// that a caller can have the next chunk's loads in flight: with the loads inside mx_finish, each behind
-// its bounds test, the residual's latency was paid eight times a chunk (16384 x 4096 x 4096 + bf16
-// residual: 300 us against 200 us without the residual).  `whole`: every element of the warp's chunk is
+// that a caller can have other loads in flight with these.  `whole`: every element of the warp's chunk is
 // inside the result and may be accessed four columns at a time (the same in all lanes).
 template <int R>
 struct MxInputs {
@@ -220,6 +220,183 @@ __device__ __forceinline__ void mx_finish(const MxLinearArgs& a, int row0, int s
       }
     }
   }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Epilogue of 32 columns of one row per thread (many rows): the lane's accumulator row as tensor memory
+// gives it, columns c0 .. c0 + 31, c0 a multiple of 32.  An MX8 block is one thread's, and 32-byte accesses
+// fill whole sectors without a transpose.  (With four columns of eight rows per thread, through shared
+// memory, a 256 x 256 tile's epilogue took 8.1 us to MX8 and 5.7 us with a GELU; see DESIGN's
+// table for what it takes now.)
+// ---------------------------------------------------------------------------------------------
+
+// 32 residual values of a row: 16-bit pairs in the first 16 words (`packed`), or fp32.
+struct MxResidualRow {
+  uint32_t w[32];
+  bool packed;  // the same in all lanes
+};
+
+// Fetched apart from its use, so that the loads are in flight while the accumulator is waited for.
+__device__ __forceinline__ void mx_fetch_row(const MxLinearArgs& a, int row, int c0, MxResidualRow& in) {
+  if (!a.residual) return;
+  const bool live = row < a.M;
+  const bool whole = c0 + 32 <= a.N && a.residual_wide;
+  in.packed = whole && a.residual_type != MX_F32;
+  const size_t at = (size_t)row * a.ldr + c0;
+  if (in.packed) {
+    const uint16_t* p = static_cast<const uint16_t*>(a.residual) + at;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const Raw<__half> r = load_raw(reinterpret_cast<const __half*>(p) + 16 * i, live);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) in.w[8 * i + k] = r.w[k];
+    }
+  } else if (whole) {
+    const float* p = static_cast<const float*>(a.residual) + at;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const Raw<float> r = load_raw(p + 16 * i, live);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) in.w[16 * i + k] = r.w[k];
+    }
+  } else {
+    auto read = [&](auto* p) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float t[16];
+        load_any(p + at + 16 * i, live ? a.N - c0 - 16 * i : 0, t);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) in.w[16 * i + k] = __float_as_uint(t[k]);
+      }
+    };
+    if (a.residual_type == MX_BF16) read(static_cast<const __nv_bfloat16*>(a.residual));
+    else if (a.residual_type == MX_F16) read(static_cast<const __half*>(a.residual));
+    else read(static_cast<const float*>(a.residual));
+  }
+}
+
+// Adds `bias` (the same 32 values for all lanes) to v.
+__device__ __forceinline__ void mx_add_bias(const float* bias, int c0, int N, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float t[4];
+    load4(bias + c0 + 4 * j, max(0, min(4, N - c0 - 4 * j)), true, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[4 * j + i] += t[i];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void mx_store_row(T* p, const float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float t[kMxPiece];
+#pragma unroll
+    for (int k = 0; k < kMxPiece; ++k) t[k] = v[16 * i + k];
+    store_vec(p + 16 * i, true, t);
+  }
+}
+
+// v: the products with W, g: those with G.  Everything is fp32 and rounded once, to the output's
+// type.  Returns the block's scale byte (MX8; the caller writes it with its neighbours').  `stage`: the warp's 4 KB.
+template <bool kGated>
+__device__ __forceinline__ uint32_t mx_finish_row(const MxLinearArgs& a, int row, int c0, float (&v)[32], float (&g)[32],
+                                                  const MxResidualRow& in, uint8_t* stage) {
+  if (a.bias) mx_add_bias(a.bias, c0, a.N, v);
+  if (kGated && a.gate_bias) mx_add_bias(a.gate_bias, c0, a.N, g);
+  float(&on)[32] = kGated ? g : v;
+  auto apply = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float2 y = f(make_float2(on[i], on[i + 1]));
+      on[i] = y.x;
+      on[i + 1] = y.y;
+    }
+  };
+  if (a.act == MX_ACT_GELU) apply([](float2 x) { return gelu_erf2(x); });
+  else if (a.act == MX_ACT_SILU) apply([](float2 x) { return make_float2(mx_silu(x.x), mx_silu(x.y)); });
+  else if (a.act == MX_ACT_RELU) apply([](float2 x) { return make_float2(mx_relu(x.x), mx_relu(x.y)); });
+  if (kGated) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float2 y = mul2(make_float2(v[i], v[i + 1]), make_float2(g[i], g[i + 1]));
+      v[i] = y.x;
+      v[i + 1] = y.y;
+    }
+  }
+  if (a.residual) {
+    auto add = [&](auto* type) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 r = unpack2_f32(in.w[i], type);
+        v[2 * i] += r.x;
+        v[2 * i + 1] += r.y;
+      }
+    };
+    if (in.packed && a.residual_type == MX_BF16) add((__nv_bfloat16*)nullptr);
+    else if (in.packed) add((__half*)nullptr);
+    else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(in.w[i]);
+    }
+  }
+  const bool live = row < a.M;
+  const size_t at = (size_t)row * a.ldo + c0;
+  if (a.out_type == MX_MX8) {
+    if (c0 + 32 > a.N) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = c0 + i < a.N ? v[i] : 0.f;
+    }
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) most = max_abs3(most, v[i], v[i + 1]);
+    const uint32_t byte = mx_scale_byte(__float_as_uint(most));
+    const float inverse = mx_inverse(byte);
+    uint32_t q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = mx_pack4(v + 4 * i, inverse);
+    uint8_t* p = static_cast<uint8_t*>(a.out) + at;
+    if (a.out_wide && c0 + 16 < a.N) {
+      if (live)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]),
+                     "r"(q[4]), "r"(q[5]), "r"(q[6]), "r"(q[7])
+                     : "memory");
+    } else {
+      if (live && c0 < a.N) reinterpret_cast<uint4*>(p)[0] = make_uint4(q[0], q[1], q[2], q[3]);
+      if (live && c0 + 16 < a.N) reinterpret_cast<uint4*>(p)[1] = make_uint4(q[4], q[5], q[6], q[7]);
+    }
+    return byte;
+  }
+  if (a.out_wide && a.out_type != MX_F32 && c0 + 32 <= a.N) {
+    if (live) {
+      if (a.out_type == MX_BF16) mx_store_row(static_cast<__nv_bfloat16*>(a.out) + at, v);
+      else mx_store_row(static_cast<__half*>(a.out) + at, v);
+    }
+    return 0;
+  }
+  // fp32 rows (a thread's 128 bytes in four stores 16384 x 64 x 4096 + fp32: 131 us, whole lines 98) and rows
+  // that are not made of aligned 32-byte vectors: through shared memory (16-byte pieces swizzled by
+  // row), so that eight lanes write 32 neighbouring columns of a row.
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  __syncwarp();
+  const int col = c0 + 4 * (lane & 7), n = max(0, min(4, a.N - col));
+  auto write = [&](auto* p) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int r = 4 * k + (lane >> 3), to = row - lane + r;
+      const float4 t = *reinterpret_cast<const float4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+      const float f[4] = {t.x, t.y, t.z, t.w};
+      if (to < a.M) store4(p + (size_t)to * a.ldo + col, n, a.out_vec, f);
+    }
+  };
+  if (a.out_type == MX_BF16) write(static_cast<__nv_bfloat16*>(a.out));
+  else if (a.out_type == MX_F16) write(static_cast<__half*>(a.out));
+  else write(static_cast<float*>(a.out));
+  return 0;
 }
 
 }  // namespace laya
