@@ -150,11 +150,11 @@ void launch_cluster(K kern, dim3 grid, int threads, int smem, dim3 cluster, cuda
   CK(cudaLaunchKernelEx(&cfg, kern, m, a));
 }
 
-template <int BN, bool kGated>
-void launch_pair(const MxLinearArgs& a, int dev, cudaStream_t st) {
+template <int BN, bool kGated, int kRes>
+void launch_pair_res(const MxLinearArgs& a, int dev, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   using Cfg = MxPairCfg<BN>;
-  auto kern = mx8_linear_pair_kernel<BN, kGated>;
+  auto kern = mx8_linear_pair_kernel<BN, kGated, kRes>;
   allow_smem(kern, Cfg::kSmemBytes, dev, done);
   const MxMaps m = linear_maps(a, 128, BN / 2, kGated ? 1 : Cfg::kWeightTiles);
   const int out_cols = kGated ? BN / 2 : BN;
@@ -162,6 +162,14 @@ void launch_pair(const MxLinearArgs& a, int dev, cudaStream_t st) {
   if (tiles > INT32_MAX / 2) fail(LAYA_ERR_INVALID, "result of %d x %d is too large", a.M, a.N);
   const int pairs = (int)std::min<int64_t>(tiles, sm_count(dev) / 2);
   launch_cluster(kern, dim3(2 * pairs), kMxThreadsPair, Cfg::kSmemBytes, dim3(2, 1, 1), st, m, a);
+}
+
+template <int BN, bool kGated>
+void launch_pair(const MxLinearArgs& a, int dev, cudaStream_t st) {
+  if (!a.residual) launch_pair_res<BN, kGated, MX_RES_NONE>(a, dev, st);
+  else if (!a.residual_wide || a.N % 32) launch_pair_res<BN, kGated, MX_RES_ANY>(a, dev, st);
+  else if (a.residual_type == LAYA_DTYPE_F32) launch_pair_res<BN, kGated, MX_RES_FULL>(a, dev, st);
+  else launch_pair_res<BN, kGated, MX_RES_HALF>(a, dev, st);
 }
 
 // Launch shape of the few-row kernel: 128-feature tiles by BN-row tiles, K split over at most 4 CTAs and no
@@ -190,30 +198,31 @@ void launch_few(const MxLinearArgs& a, int dev, cudaStream_t st) {
 
 // Which kernel, and which tile.
 //
-// The few-row kernel where its 128 x BN tiles fit the SMs at once (BN 64 past 32 rows) and K is split or
-// short, or a third of the SMs stay free: 128 x 4096 x 4096 takes 7.9 us against the pair kernels' 11.1 (256 x 128
-// tiles) and 15.4 (256 x 256), 511 x 776 x 2304 7.8 against 8.8 and 12.6, 700 x 4096 x 1000 (88 tiles) 9.7 against
-// 11.7; but 256 x 4096 x 4096 (128 tiles) 12.4 against 11.2.  A gated pair tile has only 128 output columns,
-// and the few-row kernel wins wherever it fits (256 x 2048 x 2 x 4096: 12.9 against 13.9).
+// The few-row kernel up to 64 rows; up to 128 where its 128 x 64 tiles fit the SMs at once (128 x 4096 x 4096: 7.7
+// us against 9.7 for 256 x 128 pair tiles; 700 x 4096 x 1000 9.6 against 10.5, but 512 x 1024 x 2304 6.5 against
+// 6.2 and 192 x 2048 x 2048 7.8 against 7.1); and with an exponential to compute for each result, wherever
+// they fit, since a pair tile's epilogue is longer and on fewer SMs (511 x 776 x 2304 with a GELU 7.8 against 9.5;
+// gated, where a pair tile has only 128 output columns, 256 x 2048 x 2 x 4096 12.9 against 13.9).
 //
-// Otherwise CTA pairs: the tile for which this estimate is the shorter.  A wave of tiles takes
-// the longer of its MMAs' and its epilogue's time, and the last epilogue shows (microseconds, fitted to
-// 256..1024 x 4096 x 4096: 512 rows 12.0 against 16.0 us, 1024 rows 19.2 against 17.4).
+// Otherwise CTA pairs: the tile for which this estimate is the shorter.  A wave of tiles takes the longer of
+// its MMAs' and its epilogue's time (microseconds, fitted to 256 .. 3000 rows with 768 .. 4096 columns and
+// to 16384 x 64 x 4096: 512 x 4096 x 4096 10.8 with 256 x 128 tiles against 15.6, 1024 rows 17.3 against 17.0,
+// 16384 x 1024 x 4096 63.8 against 58.5).
 template <bool kGated>
 void launch_linear(const MxLinearArgs& a, int dev, cudaStream_t st) {
   if (a.M <= 16) return launch_few<16, kGated>(a, dev, st);
   if (a.M <= 32) return launch_few<32, kGated>(a, dev, st);
   const int sms = sm_count(dev), k_tiles = mx_col_tiles(a.K);
   const FewGrid few = few_grid(a, 64, sms);
-  const int64_t few_tiles = (int64_t)few.tiles * few.row_tiles;
-  if (few_tiles <= sms && (kGated || few.split > 1 || k_tiles <= 16 || 3 * few_tiles <= 2 * sms))
+  const bool fits = (int64_t)few.tiles * few.row_tiles <= sms;
+  if (a.M <= 64 || (fits && (kGated || a.M <= 128 || a.act == MX_ACT_GELU || a.act == MX_ACT_SILU)))
     return launch_few<64, kGated>(a, dev, st);
   if constexpr (!kGated) {
-    auto estimate = [&](int bn, double per_k_tile, double epilogue) {
+    auto estimate = [&](int bn, double per_k_tile, double epilogue, double once) {
       const double tiles = (double)((a.M + 255) / 256) * ((a.N + bn - 1) / bn);
-      return std::ceil(tiles / (sms / 2)) * std::max(k_tiles * per_k_tile, epilogue) + epilogue;
+      return once + std::ceil(tiles / (sms / 2)) * std::max(k_tiles * per_k_tile, epilogue);
     };
-    if (estimate(128, 0.21, 1.3) < estimate(256, 0.29, 2.6)) return launch_pair<128, false>(a, dev, st);
+    if (estimate(128, 0.17, 1.25, 4.8) < estimate(256, 0.28, 2.45, 5.8)) return launch_pair<128, false>(a, dev, st);
   }
   launch_pair<256, kGated>(a, dev, st);
 }

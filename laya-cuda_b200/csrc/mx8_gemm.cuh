@@ -112,7 +112,7 @@ __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a_desc, uint64_t b_d
 //
 // Warps: 0 TMA producer, 1 tensor-memory allocator and (in the leader) MMA issuer, 2..9 epilogue (two
 // per lane quarter, each with half of the columns).  Tensor memory: two accumulators, so that the
-// epilogue of a tile overlaps the next tile's MMAs, and two sets of scale columns.  With BN = 256
+// epilogue of a tile overlaps the next tile's MMAs, and scale columns.  With BN = 256
 // the accumulators take 2 x 256 of the 512 columns and would leave none for the scales, so they
 // share 32 columns, [224, 256): the epilogue reads those first and the next tile's MMAs wait for
 // that (barrier `shared`) instead of for half of the tile's columns.
@@ -134,11 +134,17 @@ struct MxPairCfg {
   static constexpr int kSmemBytes = kStages * kStageBytes + kMxEpiBytes + 1024 /*align*/ + 512 /*barriers*/;
   static constexpr uint32_t kAcc1 = BN == 256 ? 224 : BN;  // column of the second accumulator
   static constexpr bool kShared = kAcc1 < BN;
-  static constexpr uint32_t kScales = 480;                  // two sets of 16 columns
+  // Scale columns: a set per stage where there is room, so that a stage's are free when it is filled
+  // again; else two, and a set is waited for.
+  static constexpr int kSetCols = 4 + 4 * kWeightTiles;
+  static constexpr bool kSetPerStage = kAcc1 + BN + kStages * kSetCols <= 512;
+  static constexpr int kSets = kSetPerStage ? kStages : 2;
+  static constexpr uint32_t kScales = 512 - kSets * ((kSetCols + 7) & ~7);
+  static constexpr int kSetStride = (kSetCols + 7) & ~7;
   static_assert(kAcc1 + BN <= kScales, "accumulators and scale columns overlap");
 };
 
-template <int BN, bool kGated>
+template <int BN, bool kGated, int kRes>
 __global__ void __launch_bounds__(kMxThreadsPair, 1)
     mx8_linear_pair_kernel(const __grid_constant__ MxMaps maps, const __grid_constant__ MxLinearArgs args) {
   using Cfg = MxPairCfg<BN>;
@@ -249,27 +255,36 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
       int blocks = 0;
       for (int t = pair; t < tiles && ok; t += pairs, ++i) {
         const int acc = i & 1;
-        if (!warp_wait(&tempty[acc], ((i >> 1) & 1) ^ 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
-        if (Cfg::kShared && i > 0 && !warp_wait(shared, (i - 1) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
-        tc_fence_after();
         const uint32_t d = tmem + (acc ? Cfg::kAcc1 : 0);
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!warp_wait(&full[stage], phase, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
           // The scale columns of this set were last read by the MMAs two k-blocks ago.
-          if (blocks >= 2) {
+          if (!Cfg::kSetPerStage && blocks >= 2) {
             if (!warp_wait(&empty[done_stage], done_phase, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
             if (++done_stage == S) { done_stage = 0; done_phase ^= 1; }
           }
           ++blocks;
           tc_fence_after();
-          if (elect_one()) {
-            const uint64_t a = adesc + (uint64_t)(stage * (kMxOperandBytes >> 4));
-            const uint64_t b = bdesc + (uint64_t)(stage * (Cfg::kStageB >> 4));
+          const uint32_t ts = tmem + Cfg::kScales + (Cfg::kSetPerStage ? stage : set) * Cfg::kSetStride;
+          auto copy_scales = [&] {
             const uint64_t sc = sdesc + (uint64_t)(stage * (Cfg::kStageScales >> 4));
-            const uint32_t ts = tmem + Cfg::kScales + set * 16;
             mx_copy_scales<true>(ts, sc);
 #pragma unroll
             for (int j = 0; j < Cfg::kWeightTiles; ++j) mx_copy_scales<true>(ts + 4 + 4 * j, sc + (1 + j) * (kMxTileBytes >> 4));
+          };
+          if (kb == 0) {
+            // The accumulator is waited for last: its columns are free about 500 cycles after the previous tile's
+            // MMAs (commit, epilogue's first read, arrival), and all else is ready then.
+            if (elect_one()) copy_scales();
+            __syncwarp();
+            if (!warp_wait(&tempty[acc], ((i >> 1) & 1) ^ 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+            if (Cfg::kShared && i > 0 && !warp_wait(shared, (i - 1) & 1, args.err, kErrGemmMmaWait, abort_flag, wait_ns)) { ok = false; break; }
+            tc_fence_after();
+          }
+          if (elect_one()) {
+            if (kb > 0) copy_scales();
+            const uint64_t a = adesc + (uint64_t)(stage * (kMxOperandBytes >> 4));
+            const uint64_t b = bdesc + (uint64_t)(stage * (Cfg::kStageB >> 4));
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               mx_mma<true>(d, a + 2 * k, b + 2 * k, mx_idesc(256, BN, k), ts, ts + 4, (kb > 0 || k > 0) ? 1u : 0u);
@@ -291,77 +306,96 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
     uint8_t* buf = epi + (warp - 2) * 4096;
     const uint32_t bar_shared = cluster_addr(smem_u32(shared), 0);
     constexpr int kChunks = kOutCols / 64;  // 32-column chunks of this warp
-    auto prefetch = [&](int t) {
-      if (!args.residual_wide) return;
-      const int mb = t / n_blocks, nb = t - mb * n_blocks;
-      const int row = mb * 256 + (int)rank * 128 + quarter * 32 + lane, c0 = nb * kOutCols + half * kChunks * 32;
-      const int size = args.residual_type == MX_F32 ? 4 : 2;
-      const int bytes = min(kChunks * 32, args.N - c0) * size & ~15;
-      if (row < args.M && bytes > 0)
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
-                         static_cast<const char*>(args.residual) + ((size_t)row * args.ldr + c0) * size),
-                     "r"(bytes));
+    // The shared columns are the second half's last of accumulator 0 and the first half's first of
+    // accumulator 1: outwards in, so that they are read first.
+    auto chunk = [&](int j) { return half ? 2 * kChunks - 1 - j : j; };
+    struct Tile {
+      int row, col;  // this lane's row, the tile's first column
     };
-    if (pair < tiles) prefetch(pair);
+    auto tile_at = [&](int t) {
+      const int mb = t / n_blocks, nb = t - mb * n_blocks;
+      return Tile{mb * 256 + (int)rank * 128 + quarter * 32 + lane, nb * kOutCols};
+    };
+    // The residual is loaded kDepth chunks ahead of its use, over tiles' ends too, and brought into L2 a tile
+    // ahead.  (One chunk ahead, a chunk waits 1,000 to 1,700 cycles for it.)
+    constexpr int kDepth = kRes == MX_RES_HALF || (kRes == MX_RES_FULL && !kGated) ? 2 : 1;
+    MxResidualRow<kRes> in[kDepth];
+    auto prefetch = [&](const Tile& t) {
+      if constexpr (kRes == MX_RES_HALF || kRes == MX_RES_FULL) {
+        constexpr int kSize = kRes == MX_RES_FULL ? 4 : 2;
+        const int c0 = t.col + half * kChunks * 32;
+        const char* p = static_cast<const char*>(args.residual) + ((size_t)t.row * args.ldr + c0) * kSize;
+        if (t.row < args.M) {
+#pragma unroll
+          for (int j = 0; j < kChunks * kSize / 2; ++j)  // 64 bytes each
+            if (c0 + j * (64 / kSize) < args.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + 64 * j));
+        }
+      }
+    };
     int i = 0;
+    Tile now = tile_at(pair);
+    if (pair < tiles) {
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) mx_fetch_row<kRes>(args, now.row, now.col + chunk(d) * 32, in[d]);
+      prefetch(now);
+    }
     for (int t = pair; t < tiles; t += pairs, ++i) {
       const int acc = i & 1;
-      const int mb = t / n_blocks, nb = t - mb * n_blocks;
-      const int row0 = mb * 256 + (int)rank * 128 + quarter * 32;
-      // Outwards in: the shared columns are the second half's last of accumulator 0 and the first
-      // half's first of accumulator 1.
-      auto chunk = [&](int j) { return half ? 2 * kChunks - 1 - j : j; };
-      const int row = row0 + lane;
-      auto fetch = [&](int j, MxResidualRow& in) { mx_fetch_row(args, row, nb * kOutCols + chunk(j) * 32, in); };
-      // The first chunk's residual is loaded while the tile's MMAs run, the others' one chunk ahead of their
-      // use, from L2: a tile's rows are brought there a tile ahead.
-      MxResidualRow in;
-      fetch(0, in);
-      if (t + pairs < tiles) prefetch(t + pairs);
+      const bool more = t + pairs < tiles;
+      const Tile next = more ? tile_at(t + pairs) : now;
+      if (more) prefetch(next);
       if (!warp_wait(&tfull[acc], (i >> 1) & 1, args.err, kErrGemmEpilogueWait, abort_flag, wait_ns)) break;
       tc_fence_after();
       const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (acc ? Cfg::kAcc1 : 0);
       uint32_t scales = 0;  // MX8: this row's scale bytes of the warp's chunks
 #pragma unroll 1
-      for (int j = 0; j < kChunks; ++j) {
-        const int c = chunk(j);
-        uint32_t r[32], u[kGated ? 32 : 1];
-        tmem_ld32_async(tbase + c * 32, r);
-        if constexpr (kGated) {
-          tmem_ld32_async(tbase + 128 + c * 32, u);
-          tmem_wait_ld(u);
-        }
-        tmem_wait_ld(r);
-        if (j == 0 && Cfg::kShared && half != acc) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(bar_shared);
-        }
-        if (j == kChunks - 1) {
-          // The accumulator has been read; the stores that follow need no ordering with the next MMAs.
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(cluster_addr(smem_u32(&tempty[acc]), 0));
-        }
-        float v[32], g[32];
+      for (int j0 = 0; j0 < kChunks; j0 += kDepth) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          v[k] = __uint_as_float(kGated ? u[kGated ? k : 0] : r[k]);
-          if (kGated) g[k] = __uint_as_float(r[k]);
+        for (int d = 0; d < kDepth; ++d) {
+          const int j = j0 + d, c = chunk(j);
+          uint32_t r[32], u[kGated ? 32 : 1];
+          tmem_ld32_async(tbase + c * 32, r);
+          if constexpr (kGated) {
+            tmem_ld32_async(tbase + 128 + c * 32, u);
+            tmem_wait_ld(u);
+          }
+          tmem_wait_ld(r);
+          if (j == 0 && Cfg::kShared && half != acc) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(bar_shared);
+          }
+          if (j == kChunks - 1) {
+            // The accumulator has been read; the stores that follow need no ordering with the next MMAs.
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(cluster_addr(smem_u32(&tempty[acc]), 0));
+          }
+          float v[32], g[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            v[k] = __uint_as_float(kGated ? u[kGated ? k : 0] : r[k]);
+            if (kGated) g[k] = __uint_as_float(r[k]);
+          }
+          const uint32_t byte = mx_finish_row<kGated, kRes>(args, now.row, now.col + c * 32, v, g, in[d], buf);
+          scales |= byte << (8 * (c & 3));
+          const bool here = j + kDepth < kChunks;
+          if (kRes != MX_RES_NONE && (here || more)) {
+            const Tile& at = here ? now : next;
+            mx_fetch_row<kRes>(args, at.row, at.col + chunk(here ? j + kDepth : j + kDepth - kChunks) * 32, in[d]);
+          }
         }
-        const uint32_t byte = mx_finish_row<kGated>(args, row, nb * kOutCols + c * 32, v, g, in, buf);
-        scales |= byte << (8 * (c & 3));
-        if (j + 1 < kChunks) fetch(j + 1, in);
       }
-      if (args.out_type == MX_MX8 && row < args.M) {
+      if (args.out_type == MX_MX8 && now.row < args.M) {
         // Four chunks are a scale tile's four blocks, two its first or last two.
-        const int col = nb * kOutCols + half * kChunks * 32, col_tiles = mx_col_tiles(args.N), tile = col / kMxTileCols;
-        uint8_t* p = args.out_scales + mx_scale_tile(row, tile, col_tiles) + mx_scale_row(row);
+        const int col = now.col + half * kChunks * 32, col_tiles = mx_col_tiles(args.N), tile = col / kMxTileCols;
+        uint8_t* p = args.out_scales + mx_scale_tile(now.row, tile, col_tiles) + mx_scale_row(now.row);
         if (tile < col_tiles) {
           if (kChunks == 4) *reinterpret_cast<uint32_t*>(p) = scales;
           else reinterpret_cast<uint16_t*>(p)[(col / 64) & 1] = (uint16_t)(scales >> (col & 64 ? 16 : 0));
         }
       }
+      now = next;
     }
   }
 

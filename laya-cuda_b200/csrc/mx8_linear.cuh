@@ -230,41 +230,44 @@ __device__ __forceinline__ void mx_finish(const MxLinearArgs& a, int row0, int s
 // table for what it takes now.)
 // ---------------------------------------------------------------------------------------------
 
-// 32 residual values of a row: 16-bit pairs in the first 16 words (`packed`), or fp32.
-struct MxResidualRow {
-  uint32_t w[32];
-  bool packed;  // the same in all lanes
+// How a kernel reads the residual.  The common forms are kernels of their own: a load behind a test (of
+// the type, the alignment, the row) is waited for where the paths join again, and not where it is used
+// (16384 x 64 x 4096 + bf16: 2,200 cycles a tile before the accumulator was even looked at).
+enum MxResidual : int {
+  MX_RES_NONE = 0,
+  MX_RES_HALF = 1,  // 16-bit rows of whole aligned 32-byte vectors, N a multiple of 32
+  MX_RES_FULL = 2,  // 32-bit rows, the same
+  MX_RES_ANY = 3
 };
 
-// Fetched apart from its use, so that the loads are in flight while the accumulator is waited for.
-__device__ __forceinline__ void mx_fetch_row(const MxLinearArgs& a, int row, int c0, MxResidualRow& in) {
-  if (!a.residual) return;
-  const bool live = row < a.M;
-  const bool whole = c0 + 32 <= a.N && a.residual_wide;
-  in.packed = whole && a.residual_type != MX_F32;
-  const size_t at = (size_t)row * a.ldr + c0;
-  if (in.packed) {
-    const uint16_t* p = static_cast<const uint16_t*>(a.residual) + at;
+// 32 residual values of a row: 16-bit pairs (MX_RES_HALF) or fp32.  Fetched apart from their use, so that the
+// loads are in flight while the accumulator is waited for.
+template <int kRes>
+struct MxResidualRow {
+  uint32_t w[kRes == MX_RES_NONE ? 1 : kRes == MX_RES_HALF ? 16 : 32];
+};
+
+template <int kRes>
+__device__ __forceinline__ void mx_fetch_row(const MxLinearArgs& a, int row, int c0, MxResidualRow<kRes>& in) {
+  if constexpr (kRes == MX_RES_HALF || kRes == MX_RES_FULL) {
+    // Lanes and chunks outside the result read its last row or chunk again.
+    const size_t at = (size_t)min(row, a.M - 1) * a.ldr + min(c0, a.N - 32);
+    constexpr int kSize = kRes == MX_RES_HALF ? 2 : 4;
+    const char* p = static_cast<const char*>(a.residual) + at * kSize;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const Raw<__half> r = load_raw(reinterpret_cast<const __half*>(p) + 16 * i, live);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) in.w[8 * i + k] = r.w[k];
+    for (int i = 0; i < kSize; ++i) {
+      uint32_t* w = in.w + 8 * i;
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(p + 32 * i));
     }
-  } else if (whole) {
-    const float* p = static_cast<const float*>(a.residual) + at;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const Raw<float> r = load_raw(p + 16 * i, live);
-#pragma unroll
-      for (int k = 0; k < 16; ++k) in.w[16 * i + k] = r.w[k];
-    }
-  } else {
+  } else if constexpr (kRes == MX_RES_ANY) {
+    const size_t at = (size_t)row * a.ldr + c0;
     auto read = [&](auto* p) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float t[16];
-        load_any(p + at + 16 * i, live ? a.N - c0 - 16 * i : 0, t);
+        load_any(p + at + 16 * i, row < a.M ? a.N - c0 - 16 * i : 0, t);
 #pragma unroll
         for (int k = 0; k < 16; ++k) in.w[16 * i + k] = __float_as_uint(t[k]);
       }
@@ -299,9 +302,9 @@ __device__ __forceinline__ void mx_store_row(T* p, const float (&v)[32]) {
 
 // v: the products with W, g: those with G.  Everything is fp32 and rounded once, to the output's
 // type.  Returns the block's scale byte (MX8; the caller writes it with its neighbours').  `stage`: the warp's 4 KB.
-template <bool kGated>
+template <bool kGated, int kRes>
 __device__ __forceinline__ uint32_t mx_finish_row(const MxLinearArgs& a, int row, int c0, float (&v)[32], float (&g)[32],
-                                                  const MxResidualRow& in, uint8_t* stage) {
+                                                  const MxResidualRow<kRes>& in, uint8_t* stage) {
   if (a.bias) mx_add_bias(a.bias, c0, a.N, v);
   if (kGated && a.gate_bias) mx_add_bias(a.gate_bias, c0, a.N, g);
   float(&on)[32] = kGated ? g : v;
@@ -324,21 +327,20 @@ __device__ __forceinline__ uint32_t mx_finish_row(const MxLinearArgs& a, int row
       v[i + 1] = y.y;
     }
   }
-  if (a.residual) {
+  if constexpr (kRes == MX_RES_HALF) {
     auto add = [&](auto* type) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float2 r = unpack2_f32(in.w[i], type);
-        v[2 * i] += r.x;
-        v[2 * i + 1] += r.y;
+        const float2 r = add2(make_float2(v[2 * i], v[2 * i + 1]), unpack2_f32(in.w[i], type));
+        v[2 * i] = r.x;
+        v[2 * i + 1] = r.y;
       }
     };
-    if (in.packed && a.residual_type == MX_BF16) add((__nv_bfloat16*)nullptr);
-    else if (in.packed) add((__half*)nullptr);
-    else {
+    if (a.residual_type == MX_BF16) add((__nv_bfloat16*)nullptr);
+    else add((__half*)nullptr);
+  } else if constexpr (kRes != MX_RES_NONE) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(in.w[i]);
-    }
+    for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(in.w[i]);
   }
   const bool live = row < a.M;
   const size_t at = (size_t)row * a.ldo + c0;
