@@ -43,6 +43,16 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
   }
 }
 
+// The two halves of cluster_sync: arrive (releasing what this thread wrote), and wait for all to have.
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // tc_commit_pair onto the barrier at the same offset in both CTAs of the pair.
 __device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
   asm volatile(
@@ -591,48 +601,85 @@ __global__ void __launch_bounds__(kMxThreadsFew, kGated ? 1 : 2)
       tc_fence_before();
     }
   }
-  __syncwarp();
-  cluster_sync();  // every CTA's sums are in its shared memory
-  // Rows of X are dealt to the cluster's warps; a warp finishes R at a time, with all its loads from
-  // the other CTAs in flight together.
-  constexpr int R = kGated ? 1 : 2;
-  const uint32_t mine = smem_u32(partial) + lane * 16;
-  const int col = f0 + 4 * lane;
-  const int step = 8 * split, rows = min(BN, args.M - t0);
-  for (int t = rank * 8 + warp; t < rows; t += R * step) {
+  // Rows of X are dealt to the cluster's warps, which finish R at a time.  The loads of a turn are in flight
+  // together, and the first turn's inputs are loaded between the arrival at the barrier that follows the
+  // sums and the wait for it.
+  const int rows = min(BN, args.M - t0), step = 8 * split, col = f0 + 4 * lane;
+  int t = rank * 8 + warp;
+  auto whole = [&](int r) { return f0 + 128 <= args.N && t + (r - 1) * step < rows; };
+  cluster_arrive();  // this CTA's sums are in its shared memory
+  if (split == 1) {
+    constexpr int R = kGated ? 4 : 8;
     MxInputs<R> in;
-    mx_fetch<kGated, R>(args, t0 + t, step, t0 + rows, col, f0 + 128 <= args.N && t + (R - 1) * step < rows, in);
-    float4 s[R][kMxMaxSplit], u[kGated ? R : 1][kMxMaxSplit];
-#pragma unroll
-    for (int r = 0; r < kMxMaxSplit; ++r) {
-      if (r >= split) break;
-      const uint32_t there = cluster_addr(mine, r);
+    mx_fetch<kGated, R>(args, t0 + t, step, t0 + rows, col, whole(R), in);
+    cluster_wait();
+    for (; t < rows; t += R * step) {
+      float v[R][4], g[R][4];
 #pragma unroll
       for (int k = 0; k < R; ++k) {
-        const uint32_t at = there + min(t + k * step, BN - 1) * 512;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(s[k][r].x), "=f"(s[k][r].y), "=f"(s[k][r].z), "=f"(s[k][r].w) : "r"(at));
-        if constexpr (kGated)
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(u[k][r].x), "=f"(u[k][r].y), "=f"(u[k][r].z), "=f"(u[k][r].w) : "r"(at + BN * 512));
-      }
-    }
-    float v[R][4] = {}, g[R][4] = {};
-#pragma unroll
-    for (int r = 0; r < kMxMaxSplit; ++r) {
-      if (r >= split) break;
-#pragma unroll
-      for (int k = 0; k < R; ++k) {
-        v[k][0] += s[k][r].x; v[k][1] += s[k][r].y; v[k][2] += s[k][r].z; v[k][3] += s[k][r].w;
+        const float* p = partial + min(t + k * step, BN - 1) * 128 + 4 * lane;
+        const float4 s = *reinterpret_cast<const float4*>(p);
+        v[k][0] = s.x; v[k][1] = s.y; v[k][2] = s.z; v[k][3] = s.w;
         if constexpr (kGated) {
-          g[k][0] += u[k][r].x; g[k][1] += u[k][r].y; g[k][2] += u[k][r].z; g[k][3] += u[k][r].w;
+          const float4 u = *reinterpret_cast<const float4*>(p + BN * 128);
+          g[k][0] = u.x; g[k][1] = u.y; g[k][2] = u.z; g[k][3] = u.w;
         }
       }
+      mx_finish<kGated, R>(args, t0 + t, step, t0 + rows, col, v, g, in);
+      if (t + R * step < rows) {
+        t += R * step;
+        mx_fetch<kGated, R>(args, t0 + t, step, t0 + rows, col, whole(R), in);
+        t -= R * step;
+      }
     }
-    mx_finish<kGated, R>(args, t0 + t, step, t0 + rows, col, v, g, in);
+  } else {
+    constexpr int R = kGated ? 1 : 2;
+    MxInputs<R> in;
+    mx_fetch<kGated, R>(args, t0 + t, step, t0 + rows, col, whole(R), in);
+    cluster_wait();
+    const uint32_t mine = smem_u32(partial) + lane * 16;
+    bool read = t >= rows;
+    if (read) cluster_arrive();
+    for (; t < rows; t += R * step) {
+      float4 s[R][kMxMaxSplit], u[kGated ? R : 1][kMxMaxSplit];
+#pragma unroll
+      for (int r = 0; r < kMxMaxSplit; ++r) {
+        if (r >= split) break;
+        const uint32_t there = cluster_addr(mine, r);
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const uint32_t at = there + min(t + k * step, BN - 1) * 512;
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(s[k][r].x), "=f"(s[k][r].y), "=f"(s[k][r].z), "=f"(s[k][r].w) : "r"(at));
+          if constexpr (kGated)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(u[k][r].x), "=f"(u[k][r].y), "=f"(u[k][r].z), "=f"(u[k][r].w) : "r"(at + BN * 512));
+        }
+      }
+      float v[R][4] = {}, g[R][4] = {};
+#pragma unroll
+      for (int r = 0; r < kMxMaxSplit; ++r) {
+        if (r >= split) break;
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          v[k][0] += s[k][r].x; v[k][1] += s[k][r].y; v[k][2] += s[k][r].z; v[k][3] += s[k][r].w;
+          if constexpr (kGated) {
+            g[k][0] += u[k][r].x; g[k][1] += u[k][r].y; g[k][2] += u[k][r].z; g[k][3] += u[k][r].w;
+          }
+        }
+      }
+      const bool last = t + R * step >= rows;
+      if (last) cluster_arrive();  // this warp has read the other CTAs' sums
+      mx_finish<kGated, R>(args, t0 + t, step, t0 + rows, col, v, g, in);
+      if (!last) {
+        t += R * step;
+        mx_fetch<kGated, R>(args, t0 + t, step, t0 + rows, col, whole(R), in);
+        t -= R * step;
+      }
+    }
+    cluster_wait();  // no CTA leaves while its sums are read
   }
-  __syncwarp();
-  cluster_sync();  // no CTA leaves while its sums are read
+  __syncthreads();
   tc_fence_after();
   if (warp == 5) tmem_dealloc(tmem, Cfg::kTmemCols);
 }
