@@ -287,10 +287,10 @@ int laya_op_mx8_quantize(const laya_mx8_convert* p, void* stream) {
   if (!rows) return LAYA_OK;
   check_rows("x", p->data, p->ld, cols, p->dtype);
   check_mx8("out", p->values, p->ldv, p->scales, cols);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int sms = sm_count(current_device(st));
   const int64_t groups = (int64_t)rows * mx_col_tiles(cols);
   if (groups > INT32_MAX) fail(LAYA_ERR_INVALID, "%d x %d values are too many for one call", rows, cols);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count(current_device(st));
   with_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const T* x = static_cast<const T*>(p->data);
@@ -315,11 +315,11 @@ int laya_op_mx8_dequantize(const laya_mx8_convert* p, void* stream) {
   if (!rows) return LAYA_OK;
   check_mx8("x", p->values, p->ldv, p->scales, cols);
   check_rows("out", p->data, p->ld, cols, p->dtype);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int sms = sm_count(current_device(st));
   const uint32_t per_row = ((uint32_t)cols + kMxPiece - 1) / kMxPiece;
   const int64_t pieces = (int64_t)rows * per_row;
   if (pieces > INT32_MAX) fail(LAYA_ERR_INVALID, "%d x %d values are too many for one call", rows, cols);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count(current_device(st));
   with_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     T* out = static_cast<T*>(p->data);

@@ -39,6 +39,7 @@ def convert(**other):
     (dict(data=None), "null"), (dict(ld=31), "stride"), (dict(data=P + 2), "aligned"), (dict(ldv=40), "16"),
     (dict(cols=48, ld=48), "at least"), (dict(values=P + 8), "16-byte"), (dict(scales=P + 1), "16-byte"),
     (dict(scales=None), "null"), (dict(values=None), "null"),
+    (dict(rows=2 ** 31 - 1, cols=4096, ld=4096, ldv=4096), "too many"),
 ])
 def test_conversions_refuse(lib, name, other, word):
     with pytest.raises(ValueError, match=word):

@@ -482,6 +482,58 @@ def test_captured_in_a_graph(rows):
     assert torch.equal(got, y) and torch.isfinite(y).all()
 
 
+def test_offsets_past_32_bits():
+    """Rows 2^31 bytes and more apart: values, tensors and results."""
+    rng = np.random.default_rng(13)
+    rows, cols, n, apart = 3, 96, 64, 2 ** 30 + 64
+    v, w = activations(rng, rows, cols), matrix(rng.normal(0, 0.1, (n, cols)).astype(np.float32))[0]
+    near = torch.from_numpy(v).cuda().bfloat16()
+    store = torch.empty((rows - 1) * apart + cols, dtype=torch.bfloat16, device="cuda")
+    far = store.as_strided((rows, cols), (apart, 1))
+    far.copy_(near)
+    byte = torch.zeros((rows - 1) * (2 ** 31 + 64) + 96, dtype=torch.uint8, device="cuda")
+    far8 = mx8.Matrix(byte.as_strided((rows, cols), (2 ** 31 + 64, 1)), torch.zeros(512, dtype=torch.uint8, device="cuda"), rows, cols)
+    near8 = fresh(rows, cols)
+    weight = torch.ones(cols, device="cuda")
+    for to8, x in ((far8, far), (near8, near)):
+        mx8.rms_norm(x, weight, to8, residual=x, sum_out=x)
+        mx8.quantize(x, to8)
+    assert torch.equal(far, near) and torch.equal(far8.values, near8.values)
+    got, want = store.as_strided((rows, n), (apart, 1)), torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+    mx8.dequantize(far8, far)
+    mx8.dequantize(near8, near)
+    assert torch.equal(far, near)
+    mx8.linear(far8, w, got, residual=far[:, :n].clone())
+    mx8.linear(near8, w, want, residual=near[:, :n].clone())
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows,cols,n,gated", [(3, 65536, 256, False), (40, 65536, 300, True), (300, 65536, 520, False), (700, 65536, 512, True)])
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable(rows, cols, n, gated):
+    """Valid calls, deep enough that the epilogue waits for many microseconds, whose waits are limited to a nanosecond: the
+    kernel unwinds and sets `err`; the next call, with the default limit, gives the bits of a call before it."""
+    lib = _lib.load()
+    generator = torch.Generator(device="cuda").manual_seed(14)
+    x, w = fresh(rows, cols), fresh(n, cols)
+    for m in (x, w):
+        mx8.quantize(torch.randn(m.rows, cols, generator=generator, device="cuda"), m)
+    gate = w if gated else None
+    want, got = torch.empty(rows, n, device="cuda"), torch.empty(rows, n, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    mx8.linear(x, w, want, gate=gate, activation="silu", err=err)
+    assert int(err.item()) == 0
+    try:
+        assert lib.laya_set_launch_options(1, 1) == 0
+        mx8.linear(x, w, got, gate=gate, activation="silu", err=err)
+        torch.cuda.synchronize()
+    finally:
+        assert lib.laya_set_launch_options(1, 0) == 0
+    assert 1 <= int(err.item()) <= 3
+    err.zero_()
+    mx8.linear(x, w, got, gate=gate, activation="silu", err=err)
+    assert int(err.item()) == 0 and torch.equal(got, want)
+
+
 def test_no_rows_is_no_work():
     w, _ = matrix(np.ones((8, 32), np.float32))
     x = mx8.Matrix.empty(w.values, 0, 32)
@@ -524,3 +576,28 @@ def test_refusals():
     shifted = torch.zeros(3 * 48 + 1, dtype=torch.uint8, device="cuda")[1:].view(3, 48)
     with pytest.raises(ValueError, match="aligned"):
         mx8.linear(mx8.Matrix(shifted, x.scales, 3, 32), w, good)
+
+
+def test_the_feed_forward_example(capsys):
+    """The example runs, and its block is the operators one after the other, bit for bit."""
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parents[1] / "examples" / "mx8_feed_forward.py"
+    spec = importlib.util.spec_from_file_location("mx8_feed_forward", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    seen = dict(example.main(384, 1000))
+    assert set(seen) == {1, 512, 16384} and all(math.isfinite(off) for off in seen.values())
+    assert capsys.readouterr().out.count("tokens") == 3
+
+    rng = np.random.default_rng(15)
+    tokens, d, f = 33, 256, 160
+    weight, gate, up, down = (torch.from_numpy(rng.normal(0, 0.1, s).astype(np.float32)).cuda() for s in ((d,), (f, d), (f, d), (d, f)))
+    x, r = (torch.from_numpy(activations(rng, tokens, d)).cuda() for _ in range(2))
+    block = example.FeedForward(weight, gate, up, down)
+    got = block(x, r.clone(), block.buffers(tokens, x))
+    total, n8, a8, want = torch.empty_like(r), fresh(tokens, d), fresh(tokens, f), torch.empty_like(r)
+    mx8.rms_norm(x, weight, n8, residual=r, sum_out=total)
+    mx8.linear(n8, block.up, a8, gate=block.gate, activation="silu")
+    mx8.linear(a8, block.down, want, residual=total)
+    assert torch.equal(got, want)
