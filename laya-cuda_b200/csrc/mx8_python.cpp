@@ -1,15 +1,18 @@
 // laya_cuda._mx8: the Python calls of the MX8 operators as a CPython extension.
 //
 // A single token's call spends its time on the host: through ctypes a linear layer's arguments took 4-6 us to
-// check and convert beside the 2.5 us of the kernel's launch, and the device waited.  Here the checks read the
-// tensors' attributes directly.  Tensors are anything with torch's `data_ptr`, `shape`, `stride`, `is_contiguous`,
-// `nbytes`, `dtype` and `get_device`; torch is not linked or imported.  The library's functions come by
-// address from laya_cuda._lib (`bind`), which loads it on the first call.
+// check and convert beside the 2.1 us of the kernel's launch, and the device waited.  Here a tensor is looked
+// at through the DLPack C exchange interface of its type (one call, no Python objects), or, where its type has
+// none, through the attributes of torch's tensors: `data_ptr`, `shape`, `stride`, `dtype`, `element_size` and
+// `get_device`.  torch is not linked or imported.  The library's functions come by address from
+// laya_cuda._lib (`bind`), which loads it on the first call.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <structmember.h>
 
 #include <cstddef>
+#include <cstdint>
+#include <cstdio>
 #include <cstring>
 
 #include "../../include/laya_b200.h"
@@ -29,96 +32,182 @@ struct Library {
 } g_lib = {};
 PyObject* g_loader = nullptr;  // called before the first operator: it calls bind()
 
-enum Name { DATA_PTR, SHAPE, STRIDE, IS_CONTIGUOUS, NBYTES, DTYPE, GET_DEVICE, ELEMENT_SIZE, NUMEL, NAMES };
-PyObject* g_names[NAMES];
-constexpr const char* kNames[NAMES] = {"data_ptr", "shape", "stride", "is_contiguous", "nbytes", "dtype", "get_device",
-                                       "element_size", "numel"};
+// ---------------------------------------------------------------------------------------------
+// Tensors
+// ---------------------------------------------------------------------------------------------
 
-// An attribute, or the result of a method without arguments, as an integer; -1 with an exception set on failure.
-long long integer(PyObject* value) {
+// The parts of the DLPack standard (version 1) that are used: a borrowed view of a tensor, and the table of functions
+// that a tensor type offers in the capsule `__dlpack_c_exchange_api__`.
+struct DLTensor {
+  void* data;
+  int32_t device_type, device_id;
+  int32_t ndim;
+  uint8_t code, bits;
+  uint16_t lanes;
+  int64_t* shape;
+  int64_t* strides;  // elements; null: contiguous
+  uint64_t byte_offset;
+};
+struct DLExchange {
+  uint32_t major, minor;
+  void* previous;
+  void *allocate, *managed_from_object, *managed_to_object;
+  int (*tensor_from_object)(void* object, DLTensor* out);  // no reference is kept, nothing is synchronised; may be null
+  void* current_stream;
+};
+enum { kDLCuda = 2, kDLCudaManaged = 13, kDLInt = 0, kDLFloat = 2, kDLBfloat = 4 };
+
+constexpr int kInt32 = 100;  // a dtype beside LAYA_DTYPE_*
+constexpr int kMostDims = 8;
+
+struct View {
+  void* data;
+  int ndim;
+  int64_t shape[kMostDims], strides[kMostDims];
+  int device;  // index of the CUDA device, -1: not on one
+  int dtype;   // LAYA_DTYPE_*, kInt32, or -1 for others
+  int64_t item, numel;
+  bool contiguous;
+};
+
+enum Name { DATA_PTR, SHAPE, STRIDE, DTYPE, GET_DEVICE, ELEMENT_SIZE, EXCHANGE, NAMES };
+PyObject* g_names[NAMES];
+constexpr const char* kNames[NAMES] = {"data_ptr", "shape", "stride", "dtype", "get_device", "element_size",
+                                       "__dlpack_c_exchange_api__"};
+
+bool failed(long long n) { return n == -1 && PyErr_Occurred(); }
+
+// The result of a method without arguments as an integer; -1 with an exception set on failure.
+long long method(PyObject* o, Name name) {
+  PyObject* value = PyObject_CallMethodNoArgs(o, g_names[name]);
   if (!value) return -1;
   const long long n = PyLong_AsLongLong(value);
   Py_DECREF(value);
   return n;
 }
-long long attribute(PyObject* o, Name name) { return integer(PyObject_GetAttr(o, g_names[name])); }
-long long method(PyObject* o, Name name) { return integer(PyObject_CallMethodNoArgs(o, g_names[name])); }
-bool failed(long long n) { return n == -1 && PyErr_Occurred(); }
 
-// Whether a tensor is contiguous; -1 on failure.
-int contiguous(PyObject* o) {
-  PyObject* r = PyObject_CallMethodNoArgs(o, g_names[IS_CONTIGUOUS]);
-  if (!r) return -1;
-  const int yes = PyObject_IsTrue(r);
-  Py_DECREF(r);
-  return yes;
-}
-
-// The row stride of a two-dimensional tensor, with the stride of its columns; false on failure.
-bool strides(PyObject* o, long long* row, long long* col) {
-  PyObject* r = PyObject_CallMethodNoArgs(o, g_names[STRIDE]);
-  if (!r) return false;
-  const bool ok = PyArg_ParseTuple(r, "LL", row, col);
-  Py_DECREF(r);
-  return ok;
-}
-
-// The shape of a tensor of `n` dimensions; 1 if it has another number of them, -1 on failure.
-int shape_of(PyObject* o, Py_ssize_t n, long long* dims) {
-  PyObject* s = PyObject_GetAttr(o, g_names[SHAPE]);
-  if (!s) return -1;
-  int status = 0;
-  if (!PyTuple_Check(s) || PyTuple_GET_SIZE(s) != n) {
-    status = 1;
+// A tuple of integers (taken over) into out; their number, -1 on failure.
+int integers(PyObject* tuple, int64_t* out) {
+  if (!tuple) return -1;
+  int n = -1;
+  PyObject* items = PySequence_Fast(tuple, "a tensor's shape and stride are sequences");
+  Py_DECREF(tuple);
+  if (!items) return -1;
+  if (PySequence_Fast_GET_SIZE(items) > kMostDims) {
+    PyErr_Format(PyExc_ValueError, "a tensor of %zd dimensions", PySequence_Fast_GET_SIZE(items));
   } else {
-    for (Py_ssize_t i = 0; i < n && !status; ++i) {
-      dims[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(s, i));
-      if (failed(dims[i])) status = -1;
+    n = (int)PySequence_Fast_GET_SIZE(items);
+    for (int i = 0; i < n; ++i) {
+      out[i] = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(items, i));
+      if (failed(out[i])) {
+        n = -1;
+        break;
+      }
     }
   }
-  Py_DECREF(s);
-  return status;
+  Py_DECREF(items);
+  return n;
 }
 
-// Raises ValueError, with a tensor's shape where the format asks for one (%S).
-void refuse_shape(const char* format, const char* what, long long rows, long long cols, PyObject* t) {
-  PyObject* s = PyObject_GetAttr(t, g_names[SHAPE]);
-  if (!s) return;
-  PyObject* shape = PySequence_Tuple(s);
-  Py_DECREF(s);
-  if (!shape) return;
-  PyErr_Format(PyExc_ValueError, format, what, rows, cols, shape);
-  Py_DECREF(shape);
+void settle(View* v) {
+  v->numel = 1;
+  v->contiguous = true;
+  for (int i = v->ndim - 1; i >= 0; --i) {
+    if (v->shape[i] != 1 && v->strides[i] != v->numel) v->contiguous = false;
+    v->numel *= v->shape[i];
+  }
+  if (!v->numel) v->contiguous = true;
 }
 
-// LAYA_DTYPE_* of a dtype object, kInt32 for int32, -1 for others, -2 on failure.  Dtypes are singletons: each is looked
-// at once by its name and then known by its address (the reference is kept).
-constexpr int kInt32 = 100;
-int dtype_code(PyObject* tensor) {
+// The exchange function of a tensor's type; null where it has none.  Types are looked at once (and kept).
+decltype(DLExchange::tensor_from_object) exchange_of(PyTypeObject* type) {
   static struct {
-    PyObject* dtype;
-    int code;
-  } known[32];
+    PyTypeObject* type;
+    decltype(DLExchange::tensor_from_object) function;
+  } known[16];
   static int count = 0;
-  PyObject* d = PyObject_GetAttr(tensor, g_names[DTYPE]);
-  if (!d) return -2;
   for (int i = 0; i < count; ++i)
-    if (known[i].dtype == d) {
-      Py_DECREF(d);
-      return known[i].code;
-    }
-  PyObject* s = PyObject_Str(d);
+    if (known[i].type == type) return known[i].function;
+  decltype(DLExchange::tensor_from_object) function = nullptr;
+  PyObject* capsule = PyObject_GetAttr(reinterpret_cast<PyObject*>(type), g_names[EXCHANGE]);
+  if (capsule && PyCapsule_IsValid(capsule, "dlpack_exchange_api")) {
+    const DLExchange* api = static_cast<const DLExchange*>(PyCapsule_GetPointer(capsule, "dlpack_exchange_api"));
+    if (api->major == 1) function = api->tensor_from_object;
+  }
+  Py_XDECREF(capsule);
+  PyErr_Clear();
+  if (count < 16) {
+    Py_INCREF(type);
+    known[count++] = {type, function};
+  }
+  return function;
+}
+
+// A tensor's attributes; false with an exception set where one is missing or fails.
+bool view_attributes(PyObject* o, View* v) {
+  v->ndim = integers(PyObject_GetAttr(o, g_names[SHAPE]), v->shape);
+  if (v->ndim < 0) return false;
+  const int n = integers(PyObject_CallMethodNoArgs(o, g_names[STRIDE]), v->strides);
+  if (n < 0) return false;
+  if (n != v->ndim) {
+    PyErr_SetString(PyExc_ValueError, "a tensor's shape and stride differ in length");
+    return false;
+  }
+  v->item = method(o, ELEMENT_SIZE);
+  if (failed(v->item)) return false;
+  const long long device = method(o, GET_DEVICE);
+  if (failed(device)) return false;
+  v->device = device < 0 ? -1 : (int)device;
+  const long long data = method(o, DATA_PTR);
+  if (failed(data)) return false;
+  v->data = reinterpret_cast<void*>(data);
+  PyObject* d = PyObject_GetAttr(o, g_names[DTYPE]);
+  PyObject* s = d ? PyObject_Str(d) : nullptr;
+  Py_XDECREF(d);
   const char* text = s ? PyUnicode_AsUTF8(s) : nullptr;
-  int code = -1;
-  if (!text) code = -2;
-  else if (!strcmp(text, "torch.float32")) code = LAYA_DTYPE_F32;
-  else if (!strcmp(text, "torch.float16")) code = LAYA_DTYPE_F16;
-  else if (!strcmp(text, "torch.bfloat16")) code = LAYA_DTYPE_BF16;
-  else if (!strcmp(text, "torch.int32")) code = kInt32;
+  if (text)
+    v->dtype = !strcmp(text, "torch.float32") ? LAYA_DTYPE_F32 : !strcmp(text, "torch.float16") ? LAYA_DTYPE_F16
+               : !strcmp(text, "torch.bfloat16") ? LAYA_DTYPE_BF16 : !strcmp(text, "torch.int32") ? kInt32 : -1;
   Py_XDECREF(s);
-  if (code != -2 && count < 32) known[count++] = {d, code};  // keeps the reference
-  else Py_DECREF(d);
-  return code;
+  if (!text) return false;
+  settle(v);
+  return true;
+}
+
+bool view(PyObject* o, View* v) {
+  const auto exchange = exchange_of(Py_TYPE(o));
+  DLTensor t;
+  if (!exchange) return view_attributes(o, v);
+  // Refused by the type (a tensor that requires a gradient, say): its attributes tell the same.
+  if (exchange(o, &t) != 0 || t.ndim > kMostDims || t.lanes != 1 || t.bits % 8) {
+    PyErr_Clear();
+    return view_attributes(o, v);
+  }
+  v->data = static_cast<char*>(t.data) + t.byte_offset;
+  v->ndim = t.ndim;
+  int64_t next = 1;
+  for (int i = t.ndim - 1; i >= 0; --i) {
+    v->shape[i] = t.shape[i];
+    v->strides[i] = t.strides ? t.strides[i] : next;
+    next *= t.shape[i];
+  }
+  v->device = t.device_type == kDLCuda || t.device_type == kDLCudaManaged ? t.device_id : -1;
+  v->dtype = t.code == kDLFloat && t.bits == 32 ? LAYA_DTYPE_F32 : t.code == kDLFloat && t.bits == 16 ? LAYA_DTYPE_F16
+             : t.code == kDLBfloat && t.bits == 16 ? LAYA_DTYPE_BF16 : t.code == kDLInt && t.bits == 32 ? kInt32 : -1;
+  v->item = t.bits / 8;
+  settle(v);
+  return true;
+}
+
+// Raises ValueError with a tensor's shape at the end.
+void refuse_shape(const char* what, const View& v, const char* format, long long rows, long long cols) {
+  char shape[128] = "(", wanted[160];
+  size_t at = 1;
+  for (int i = 0; i < v.ndim && at < 100; ++i)
+    at += (size_t)snprintf(shape + at, sizeof shape - at, i ? ", %lld" : "%lld", (long long)v.shape[i]);
+  snprintf(shape + at, sizeof shape - at, v.ndim == 1 ? ",)" : ")");
+  snprintf(wanted, sizeof wanted, format, rows, cols);
+  PyErr_Format(PyExc_ValueError, "%s %s, got %s", what, wanted, shape);
 }
 
 long long scale_bytes(long long rows, long long cols) { return (rows + 127) / 128 * ((cols + 127) / 128) * 512; }
@@ -208,51 +297,30 @@ bool matrix_check(Matrix* m, PyObject* values, PyObject* scales, int rows, int c
     return false;
   }
   const long long room = ((long long)cols + 15) / 16 * 16, need = scale_bytes(rows, cols);
-  int whole = contiguous(values);
-  if (whole < 0) return false;
-  const long long bytes = attribute(values, NBYTES);
-  if (failed(bytes)) return false;
+  View v, s;
+  if (!view(values, &v) || !view(scales, &s)) return false;
   m->ld = room;
-  if (!whole || bytes != rows * room) {
+  if (!v.contiguous || v.numel * v.item != rows * room) {
     // Rows further apart than they need to be, of one-byte elements.
-    long long dims[2], row = 0, col = 0;
-    const int status = shape_of(values, 2, dims);
-    if (status < 0) return false;
-    const long long size = method(values, ELEMENT_SIZE);
-    if (failed(size)) return false;
-    if (!status && !strides(values, &row, &col)) return false;
-    if (status || dims[0] != rows || col != 1 || size != 1 || dims[1] < room) {
-      refuse_shape("%s of a %lld x %lld matrix must be bytes in as many contiguous rows, with room for a multiple of 16, got %S", "values",
-                   rows, cols, values);
+    if (v.ndim != 2 || v.shape[0] != rows || v.shape[1] < room || v.strides[1] != 1 || v.item != 1) {
+      refuse_shape("values", v, "of a %lld x %lld matrix must be bytes in as many contiguous rows, with room for a multiple of 16", rows, cols);
       return false;
     }
-    if (rows > 1) m->ld = row;  // the stride of a single row says nothing
+    if (rows > 1) m->ld = v.strides[0];  // the stride of a single row says nothing
   }
-  whole = contiguous(scales);
-  if (whole < 0) return false;
-  const long long held = attribute(scales, NBYTES);
-  if (failed(held)) return false;
-  if (!whole || held < need) {
+  if (!s.contiguous || s.numel * s.item < need) {
     PyErr_Format(PyExc_ValueError, "scales of a %d x %d matrix need %lld contiguous bytes", rows, cols, need);
     return false;
   }
-  const long long device = method(values, GET_DEVICE);
-  if (failed(device) && PyErr_Occurred()) return false;
-  const long long other = method(scales, GET_DEVICE);
-  if (failed(other) && PyErr_Occurred()) return false;
-  if (device < 0 || other != device) {
+  if (v.device < 0 || s.device != v.device) {
     PyErr_SetString(PyExc_ValueError, "values and scales must be on the same CUDA device");
     return false;
   }
-  const long long v = method(values, DATA_PTR);
-  if (failed(v)) return false;
-  const long long s = method(scales, DATA_PTR);
-  if (failed(s)) return false;
   m->rows = rows;
   m->cols = cols;
-  m->device = (int)device;
-  m->values_ptr = (unsigned long long)v;
-  m->scales_ptr = (unsigned long long)s;
+  m->device = v.device;
+  m->values_ptr = reinterpret_cast<unsigned long long>(v.data);
+  m->scales_ptr = reinterpret_cast<unsigned long long>(s.data);
   return true;
 }
 
@@ -345,40 +413,27 @@ struct Rows {
 
 // A [rows][cols] tensor of 16- or 32-bit floats with contiguous rows, on `device`.
 bool take_rows(const char* name, PyObject* t, int rows, int cols, int device, Rows* out) {
-  long long dims[2];
-  const int status = shape_of(t, 2, dims);
-  if (status < 0) return false;
-  if (status || dims[0] != rows || dims[1] != cols) {
-    refuse_shape("%s must be [%lld][%lld], got %S", name, rows, cols, t);
+  View v;
+  if (!view(t, &v)) return false;
+  if (v.ndim != 2 || v.shape[0] != rows || v.shape[1] != cols) {
+    refuse_shape(name, v, "must be [%lld][%lld]", rows, cols);
     return false;
   }
-  out->ld = cols;
-  const int whole = contiguous(t);
-  if (whole < 0) return false;
-  if (!whole) {
-    long long row, col;
-    if (!strides(t, &row, &col)) return false;
-    if (cols > 1 && col != 1) {
-      PyErr_Format(PyExc_ValueError, "%s: the values of a row must be contiguous", name);
-      return false;
-    }
-    if (rows > 1) out->ld = row;
+  if (cols > 1 && v.strides[1] != 1 && !v.contiguous) {
+    PyErr_Format(PyExc_ValueError, "%s: the values of a row must be contiguous", name);
+    return false;
   }
-  out->dtype = dtype_code(t);
-  if (out->dtype == -2) return false;
-  if (out->dtype < 0 || out->dtype == kInt32) {
+  if (v.dtype < 0 || v.dtype == kInt32) {
     PyErr_Format(PyExc_ValueError, "%s is not float32, float16 or bfloat16", name);
     return false;
   }
-  const long long on = method(t, GET_DEVICE);
-  if (failed(on) && PyErr_Occurred()) return false;
-  if (on != device) {
+  if (v.device != device) {
     PyErr_Format(PyExc_ValueError, "%s is not on CUDA device %d, where the matrix is", name, device);
     return false;
   }
-  const long long p = method(t, DATA_PTR);
-  if (failed(p)) return false;
-  out->ptr = reinterpret_cast<void*>(p);
+  out->ptr = v.data;
+  out->ld = rows > 1 && !v.contiguous ? v.strides[0] : cols;
+  out->dtype = v.dtype;
   return true;
 }
 
@@ -386,22 +441,13 @@ bool take_rows(const char* name, PyObject* t, int rows, int cols, int device, Ro
 bool take_vector(const char* name, PyObject* t, int n, int device, const float** out) {
   *out = nullptr;
   if (!t || t == Py_None) return true;
-  long long dims[1];
-  const int status = shape_of(t, 1, dims);
-  if (status < 0) return false;
-  const int code = dtype_code(t);
-  if (code == -2) return false;
-  const int whole = contiguous(t);
-  if (whole < 0) return false;
-  const long long on = method(t, GET_DEVICE);
-  if (failed(on) && PyErr_Occurred()) return false;
-  if (status || dims[0] != n || code != LAYA_DTYPE_F32 || !whole || on != device) {
+  View v;
+  if (!view(t, &v)) return false;
+  if (v.ndim != 1 || v.shape[0] != n || v.dtype != LAYA_DTYPE_F32 || !v.contiguous || v.device != device) {
     PyErr_Format(PyExc_ValueError, "%s must be %d contiguous float32 values on CUDA device %d", name, n, device);
     return false;
   }
-  const long long p = method(t, DATA_PTR);
-  if (failed(p)) return false;
-  *out = reinterpret_cast<const float*>(p);
+  *out = static_cast<const float*>(v.data);
   return true;
 }
 
@@ -572,19 +618,13 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* k
   }
   int* err = nullptr;
   if (g[8] && g[8] != Py_None) {
-    const int code = dtype_code(g[8]);
-    if (code == -2) return nullptr;
-    const long long on = method(g[8], GET_DEVICE);
-    if (failed(on) && PyErr_Occurred()) return nullptr;
-    const long long count = method(g[8], NUMEL);
-    if (failed(count)) return nullptr;
-    if (code != kInt32 || on != device || count < 1) {
+    View v;
+    if (!view(g[8], &v)) return nullptr;
+    if (v.dtype != kInt32 || v.device != device || v.numel < 1) {
       PyErr_Format(PyExc_ValueError, "err must be int32 on CUDA device %d", device);
       return nullptr;
     }
-    const long long p = method(g[8], DATA_PTR);
-    if (failed(p)) return nullptr;
-    err = reinterpret_cast<int*>(p);
+    err = static_cast<int*>(v.data);
   }
   void* st;
   if (!to_stream(g[9], &st) || !ready()) return nullptr;
