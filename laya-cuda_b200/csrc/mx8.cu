@@ -172,16 +172,25 @@ void launch_pair(const MxLinearArgs& a, int dev, cudaStream_t st) {
   else launch_pair_res<BN, kGated, MX_RES_HALF>(a, dev, st);
 }
 
-// Launch shape of the few-row kernel: 128-feature tiles by BN-row tiles, K split over at most 4 CTAs and no
-// more than there are SMs for.  (One row, 4096 x 4096, 32 tiles: unsplit 8.2 us, 2 CTAs 6.2, 4 CTAs 5.5, 8 CTAs
-// 6.6; 16 x 2048 x 2048, 16 tiles: 5.9, 5.2, 4.8, 7.1.)
+// Launch shape of the few-row kernel: 128-feature tiles by BN-row tiles, and K split over the 1 to 4 CTAs for
+// which this estimate is the shortest: a k-tile takes a CTA 0.17 us (gated 0.27), and a cluster's exchange up to 1.1
+// us, in proportion to the CTAs in flight; clusters that would fill more than 7/8 of the SMs do not all fit
+// at once.  Measured, unsplit / 2 / 4 CTAs: 1 x 4096 x 4096 9.1 / 6.3 / 5.4 us, 16 x 2048 x 2048 5.9 / 4.9 / 4.3, 300 x
+// 768 x 768 4.6 / 5.1 / 5.0, 1024 x 8192 x 128 12.1 / 9.0 / 6.9, 1024 x 1024 x 1024 (128 tiles) 4.9 / 6.9 / 12.6.
 struct FewGrid {
   int tiles, row_tiles, split;
 };
 FewGrid few_grid(const MxLinearArgs& a, int bn, int sms) {
   FewGrid g{(a.N + 127) / 128, (a.M + bn - 1) / bn, 1};
   const int k_tiles = mx_col_tiles(a.K);
-  while (g.split < kMxMaxSplit && g.split < k_tiles && (int64_t)g.tiles * g.row_tiles * (g.split + 1) <= sms) ++g.split;
+  const double per_k_tile = a.gate.q ? 0.27 : 0.17;
+  double best = k_tiles * per_k_tile;
+  for (int split = 2; split <= std::min(kMxMaxSplit, k_tiles); ++split) {
+    const double ctas = (double)g.tiles * g.row_tiles * split;
+    if (8 * ctas > 7 * sms) break;
+    const double t = (k_tiles + split - 1) / split * per_k_tile + 1.1 * ctas / 128;
+    if (t < best) { best = t; g.split = split; }
+  }
   return g;
 }
 
@@ -198,11 +207,12 @@ void launch_few(const MxLinearArgs& a, int dev, cudaStream_t st) {
 
 // Which kernel, and which tile.
 //
-// The few-row kernel up to 64 rows; up to 128 where its 128 x 64 tiles fit the SMs at once (128 x 4096 x 4096: 7.7
-// us against 9.7 for 256 x 128 pair tiles; 700 x 4096 x 1000 9.6 against 10.5, but 512 x 1024 x 2304 6.5 against
-// 6.2 and 192 x 2048 x 2048 7.8 against 7.1); and with an exponential to compute for each result, wherever
-// they fit, since a pair tile's epilogue is longer and on fewer SMs (511 x 776 x 2304 with a GELU 7.8 against 9.5;
-// gated, where a pair tile has only 128 output columns, 256 x 2048 x 2 x 4096 12.9 against 13.9).
+// The few-row kernel up to 64 rows, and beyond wherever its 128 x 64 tiles fit the SMs at once, unless they
+// nearly fill them and K is long (the tiles' operands then come from L2 too slowly): 128 x 4096 x 4096 takes
+// 7.8 us against 10.0 for the pair kernel's 256 x 128 tiles, 1024 x 1024 x 1024 4.9 against 5.8, 511 x 776 x 2304 with a
+// GELU 6.9 against 9.5, 192 x 4096 x 4096 (96 tiles) 9.3 against 9.9, but 256 x 4096 x 4096 (128) 11.1 against
+// 9.7.  A gated pair tile has only 128 output columns, and the few-row kernel wins wherever it fits (256 x 2048 x
+// 2 x 4096: 12.9 against 13.9).
 //
 // Otherwise CTA pairs: the tile for which this estimate is the shorter.  A wave of tiles takes the longer of
 // its MMAs' and its epilogue's time (microseconds, fitted to 256 .. 3000 rows with 768 .. 4096 columns and
@@ -215,8 +225,8 @@ void launch_linear(const MxLinearArgs& a, int dev, cudaStream_t st) {
   const int sms = sm_count(dev), k_tiles = mx_col_tiles(a.K);
   const FewGrid few = few_grid(a, 64, sms);
   const bool fits = (int64_t)few.tiles * few.row_tiles <= sms;
-  if (a.M <= 64 || (fits && (kGated || a.M <= 128 || a.act == MX_ACT_GELU || a.act == MX_ACT_SILU)))
-    return launch_few<64, kGated>(a, dev, st);
+  const bool slow = !kGated && few.split == 1 && 4LL * few.tiles * few.row_tiles > 3 * sms && k_tiles > 16;
+  if (a.M <= 64 || (fits && !slow)) return launch_few<64, kGated>(a, dev, st);
   if constexpr (!kGated) {
     auto estimate = [&](int bn, double per_k_tile, double epilogue, double once) {
       const double tiles = (double)((a.M + 255) / 256) * ((a.N + bn - 1) / bn);
