@@ -250,7 +250,8 @@ __device__ __forceinline__ void mx_store_piece(const float (&v)[kMxPiece], int r
 
 // ---------------------------------------------------------------------------------------------
 // x [rows][cols] -> MX8.  Eight threads take 128 columns of a row (a group), and each U of them at
-// once.
+// once.  HBM-bound: x is read and the values and scales written once, 16384 x 4096 bf16 in 32.8 us and 9216 x
+// 4096 fp32 in 30.3 (6.2 TB/s, 95% of a copy's rate); a small call is its launch (768 values: 1.2 us).
 // ---------------------------------------------------------------------------------------------
 constexpr int kMxThreads = 256;
 
@@ -283,7 +284,8 @@ __global__ void __launch_bounds__(kMxThreads) mx8_quantize_kernel(const T* x, in
   }
 }
 
-// MX8 -> out [rows][cols], U pieces per thread at once.
+// MX8 -> out [rows][cols], U pieces per thread at once.  HBM-bound, two thirds of it writes: 16384 x 4096 to
+// bf16 in 34.9 us (5.8 TB/s), to fp32 in 61.8 (5.5).
 template <typename T, bool kVec, int U>
 __global__ void __launch_bounds__(kMxThreads) mx8_dequantize_kernel(const uint8_t* q, int64_t ldq, const uint8_t* scales,
                                                                     int rows, int cols, FastDiv per_row, T* out, int64_t ldo) {
@@ -336,7 +338,9 @@ __global__ void __launch_bounds__(kMxThreads) mx8_dequantize_kernel(const uint8_
 // HBM-bound: x and the residual are read once and h, the values and the scales written once.  `warps`
 // warps hold a row in registers, CH pieces per thread, and a block of at least 256 threads
 // walks over rows with the weight in registers too; the next row's loads are issued before this
-// row's sum of squares is exchanged, so that a block always has a row in flight.
+// row's sum of squares is exchanged, so that a block always has a row in flight.  16384 x 4096 bf16 with the
+// residual in 73-75 us (6.3-6.5 TB/s, 97-99% of a copy's rate; reading the row twice and eight columns per
+// thread took 168); 16384 x 768 bf16 onto fp32 23.6 us (5.9 TB/s); 4096 values 2.3 us.
 // ---------------------------------------------------------------------------------------------
 struct RmsNormArgs {
   const void* x; int64_t ldx;
@@ -446,7 +450,8 @@ __global__ void __launch_bounds__(512) rms_norm_mx8_kernel(const RmsNormArgs a) 
   }
 }
 
-// Rows too long for the registers of 16 warps: one block takes one row at a time and reads it twice.
+// Rows too long for the registers of 16 warps: one block takes one row at a time and reads it twice
+// (1024 x 40000 bf16 with the residual: 159 us, against 80 for 4096 x 16384 in registers).
 template <typename T, typename R>
 __global__ void __launch_bounds__(kMxThreads) rms_norm_mx8_long_kernel(const RmsNormArgs a) {
   pdl_wait();
