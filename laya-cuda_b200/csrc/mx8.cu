@@ -166,10 +166,12 @@ void launch_pair_res(const MxLinearArgs& a, int dev, cudaStream_t st) {
 
 template <int BN, bool kGated>
 void launch_pair(const MxLinearArgs& a, int dev, cudaStream_t st) {
+  const bool wide = a.residual_wide && a.N % 32 == 0, full = a.residual_type == LAYA_DTYPE_F32;
   if (!a.residual) launch_pair_res<BN, kGated, MX_RES_NONE>(a, dev, st);
-  else if (!a.residual_wide || a.N % 32) launch_pair_res<BN, kGated, MX_RES_ANY>(a, dev, st);
-  else if (a.residual_type == LAYA_DTYPE_F32) launch_pair_res<BN, kGated, MX_RES_FULL>(a, dev, st);
-  else launch_pair_res<BN, kGated, MX_RES_HALF>(a, dev, st);
+  else if (wide && full) launch_pair_res<BN, kGated, MX_RES_FULL>(a, dev, st);
+  else if (wide) launch_pair_res<BN, kGated, MX_RES_HALF>(a, dev, st);
+  else if (full) launch_pair_res<BN, kGated, MX_RES_ANY_FULL>(a, dev, st);
+  else launch_pair_res<BN, kGated, MX_RES_ANY_HALF>(a, dev, st);
 }
 
 // Launch shape of the few-row kernel: 128-feature tiles by BN-row tiles, and K split over the 1 to 4 CTAs for
@@ -245,14 +247,15 @@ int pieces_grid(int64_t pieces, int per_block, int unroll, int sms) {
 }
 constexpr int kConvertUnroll = 2;
 
-template <typename T, typename R, int CH, bool kVec>
+template <typename T, typename R, int CH, bool kVec, bool kShort>
 void launch_norm_rows(RmsNormArgs a, int sms, cudaStream_t st) {
-  auto kern = rms_norm_mx8_kernel<T, R, CH, kVec>;
+  auto kern = rms_norm_mx8_kernel<T, R, CH, kVec, kShort>;
   const int need = (a.cols + 32 * kMxPiece * CH - 1) / (32 * kMxPiece * CH);
   int log = 0;
   while ((1 << log) < need) ++log;
   a.warps = 1 << log;
-  const int warps = std::max(a.warps, 8), per_block = warps / a.warps;
+  a.lanes = a.cols > 8 * kMxPiece ? 16 : 8;
+  const int warps = std::max(a.warps, 8), per_block = warps / a.warps * (kShort ? 32 / a.lanes : 1);
   int64_t blocks = ((int64_t)a.rows + per_block - 1) / per_block;
   if (blocks > sms) {
     static std::atomic<int> resident[8];  // by log, 0: not asked yet
@@ -273,9 +276,13 @@ void launch_norm(const RmsNormArgs& a, int sms, cudaStream_t st) {
                    (!a.residual || rows_vectored(static_cast<const R*>(a.residual), a.ldr, a.cols)) &&
                    (!a.sum_out || rows_vectored(static_cast<const R*>(a.sum_out), a.lds, a.cols));
   constexpr int kCols = 16 * 32 * kMxPiece;  // 16 warps of one piece per thread
-  if (vec && a.cols <= kCols) launch_norm_rows<T, R, 1, true>(a, sms, st);
-  else if (vec && a.cols <= 2 * kCols) launch_norm_rows<T, R, 2, true>(a, sms, st);
-  else if (a.cols <= kCols) launch_norm_rows<T, R, 1, false>(a, sms, st);
+  const bool few_cols = a.cols <= 16 * kMxPiece;
+  if (vec && few_cols) launch_norm_rows<T, R, 1, true, true>(a, sms, st);
+  else if (vec && a.cols <= kCols) launch_norm_rows<T, R, 1, true, false>(a, sms, st);
+  else if (vec && a.cols <= 2 * kCols) launch_norm_rows<T, R, 2, true, false>(a, sms, st);
+  else if (few_cols) launch_norm_rows<T, R, 1, false, true>(a, sms, st);
+  else if (a.cols <= kCols) launch_norm_rows<T, R, 1, false, false>(a, sms, st);
+  else if (a.cols <= 2 * kCols) launch_norm_rows<T, R, 2, false, false>(a, sms, st);
   else launch_k(rms_norm_mx8_long_kernel<T, R>, dim3(std::min(a.rows, 8 * sms)), dim3(kMxThreads), 0, st, a);
 }
 

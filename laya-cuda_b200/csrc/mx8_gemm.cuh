@@ -337,8 +337,8 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
     constexpr int kDepth = kRes == MX_RES_HALF || (kRes == MX_RES_FULL && !kGated) ? 2 : 1;
     MxResidualRow<kRes> in[kDepth];
     auto prefetch = [&](const Tile& t) {
-      if constexpr (kRes == MX_RES_HALF || kRes == MX_RES_FULL) {
-        constexpr int kSize = kRes == MX_RES_FULL ? 4 : 2;
+      if constexpr (kRes != MX_RES_NONE) {
+        constexpr int kSize = mx_res_size(kRes);
         const int c0 = t.col + half * kChunks * 32;
         const char* p = static_cast<const char*>(args.residual) + ((size_t)t.row * args.ldr + c0) * kSize;
         if (t.row < args.M) {

@@ -238,11 +238,15 @@ enum MxResidual : int {
   MX_RES_NONE = 0,
   MX_RES_HALF = 1,  // 16-bit rows of whole aligned 32-byte vectors, N a multiple of 32
   MX_RES_FULL = 2,  // 32-bit rows, the same
-  MX_RES_ANY = 3
+  MX_RES_ANY_HALF = 3,  // 16-bit rows of any alignment and length
+  MX_RES_ANY_FULL = 4   // 32-bit rows, the same
 };
+__host__ __device__ constexpr int mx_res_size(int res) { return res == MX_RES_HALF || res == MX_RES_ANY_HALF ? 2 : 4; }
 
 // 32 residual values of a row: 16-bit pairs (MX_RES_HALF) or fp32.  Fetched apart from their use, so that the
-// loads are in flight while the accumulator is waited for.
+// loads are in flight while the accumulator is waited for.  (For rows of any alignment, 32 loads of one row's
+// neighbouring elements each, turned through shared memory, took 50 us where these shifted granules take 36:
+// 16384 x 768 x 767 bf16.)
 template <int kRes>
 struct MxResidualRow {
   uint32_t w[kRes == MX_RES_NONE ? 1 : kRes == MX_RES_HALF ? 16 : 32];
@@ -252,8 +256,8 @@ template <int kRes>
 __device__ __forceinline__ void mx_fetch_row(const MxLinearArgs& a, int row, int c0, MxResidualRow<kRes>& in) {
   if constexpr (kRes == MX_RES_HALF || kRes == MX_RES_FULL) {
     // Lanes and chunks outside the result read its last row or chunk again.
+    constexpr int kSize = mx_res_size(kRes);
     const size_t at = (size_t)min(row, a.M - 1) * a.ldr + min(c0, a.N - 32);
-    constexpr int kSize = kRes == MX_RES_HALF ? 2 : 4;
     const char* p = static_cast<const char*>(a.residual) + at * kSize;
 #pragma unroll
     for (int i = 0; i < kSize; ++i) {
@@ -262,7 +266,7 @@ __device__ __forceinline__ void mx_fetch_row(const MxLinearArgs& a, int row, int
                    : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                    : "l"(p + 32 * i));
     }
-  } else if constexpr (kRes == MX_RES_ANY) {
+  } else if constexpr (kRes != MX_RES_NONE) {
     const size_t at = (size_t)row * a.ldr + c0;
     auto read = [&](auto* p) {
 #pragma unroll
@@ -273,10 +277,16 @@ __device__ __forceinline__ void mx_fetch_row(const MxLinearArgs& a, int row, int
         for (int k = 0; k < 16; ++k) in.w[16 * i + k] = __float_as_uint(t[k]);
       }
     };
-    if (a.residual_type == MX_BF16) read(static_cast<const __nv_bfloat16*>(a.residual));
-    else if (a.residual_type == MX_F16) read(static_cast<const __half*>(a.residual));
-    else read(static_cast<const float*>(a.residual));
+    if (kRes == MX_RES_ANY_FULL) read(static_cast<const float*>(a.residual));
+    else if (a.residual_type == MX_BF16) read(static_cast<const __nv_bfloat16*>(a.residual));
+    else read(static_cast<const __half*>(a.residual));
   }
+}
+
+// Where element (row r, column c) of a warp's 32 x 32 fp32 block lies in its 4 KB of shared memory: rows of 128
+// bytes, 16-byte pieces swizzled by row, so that neither a row per lane nor a column per lane meets in a bank.
+__device__ __forceinline__ float* mx_stage_at(uint8_t* stage, int r, int c) {
+  return reinterpret_cast<float*>(stage + r * 128 + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4);
 }
 
 // Adds `bias` (the same 32 values for all lanes) to v.
@@ -377,23 +387,31 @@ __device__ __forceinline__ uint32_t mx_finish_row(const MxLinearArgs& a, int row
     }
     return 0;
   }
-  // fp32 rows (a thread's 128 bytes in four stores 16384 x 64 x 4096 + fp32: 131 us, whole lines 98) and rows
-  // that are not made of aligned 32-byte vectors: through shared memory (16-byte pieces swizzled by
-  // row), so that eight lanes write 32 neighbouring columns of a row.
-  const int lane = threadIdx.x & 31;
+  // fp32 rows (a thread's 128 bytes in four stores, 16384 x 64 x 4096 + fp32: 131 us, this way 117) and rows
+  // that are not made of aligned 32-byte vectors: through shared memory, so that eight lanes write 32
+  // neighbouring columns of a row, or, where four columns are no vector, the warp writes one row after the other.
+  const int lane = threadIdx.x & 31, row0 = row - lane;
   __syncwarp();
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    *reinterpret_cast<float4*>(mx_stage_at(stage, lane, 4 * j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   __syncwarp();
-  const int col = c0 + 4 * (lane & 7), n = max(0, min(4, a.N - col));
   auto write = [&](auto* p) {
+    using T = std::remove_pointer_t<decltype(p)>;
+    if (a.out_vec) {
+      const int col = c0 + 4 * (lane & 7), n = max(0, min(4, a.N - col));
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int r = 4 * k + (lane >> 3), to = row - lane + r;
-      const float4 t = *reinterpret_cast<const float4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-      const float f[4] = {t.x, t.y, t.z, t.w};
-      if (to < a.M) store4(p + (size_t)to * a.ldo + col, n, a.out_vec, f);
+      for (int k = 0; k < 8; ++k) {
+        const int r = 4 * k + (lane >> 3);
+        const float4 t = *reinterpret_cast<const float4*>(mx_stage_at(stage, r, 4 * (lane & 7)));
+        const float f[4] = {t.x, t.y, t.z, t.w};
+        if (row0 + r < a.M) store4(p + (size_t)(row0 + r) * a.ldo + col, n, true, f);
+      }
+    } else if (c0 + lane < a.N) {
+      T* to = p + (size_t)row0 * a.ldo + c0 + lane;
+      const int rows = min(32, a.M - row0);
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r, to += a.ldo) *to = from_f32<T>(*mx_stage_at(stage, r, lane));
     }
   };
   if (a.out_type == MX_BF16) write(static_cast<__nv_bfloat16*>(a.out));

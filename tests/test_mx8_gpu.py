@@ -233,7 +233,7 @@ def check_mx8(out, y, slack):
     assert not q[:, out.cols: (out.cols + 15) // 16 * 16].any()
 
 
-NORM_SHAPES = [(1, 1), (2, 31), (7, 33), (1, 768), (130, 256), (33, 1000), (3, 2048), (2, 4100), (5, 8192), (1, 16384), (2, 40000)]
+NORM_SHAPES = [(1, 1), (2, 31), (7, 33), (1, 768), (130, 256), (300, 100), (77, 128), (50, 250), (3, 12001), (33, 1000), (3, 2048), (2, 4100), (5, 8192), (1, 16384), (2, 40000)]
 
 
 @pytest.mark.parametrize("dtype,rdtype", [("bf16", "f32"), ("f16", "f16"), ("f32", "f32"), ("bf16", "bf16"), ("f32", "bf16"), ("f16", "f32")])
