@@ -176,8 +176,8 @@ void launch_pair(const MxLinearArgs& a, int dev, cudaStream_t st) {
 
 // Launch shape of the few-row kernel: 128-feature tiles by BN-row tiles, and K split over the 1 to 4 CTAs for
 // which this estimate is the shortest: a k-tile takes a CTA 0.17 us (gated 0.27), and a cluster's exchange up to 1.1
-// us, in proportion to the CTAs in flight; clusters that would fill more than 7/8 of the SMs do not all fit
-// at once.  Measured, unsplit / 2 / 4 CTAs: 1 x 4096 x 4096 9.1 / 6.3 / 5.4 us, 16 x 2048 x 2048 5.9 / 4.9 / 4.3, 300 x
+// us, in proportion to the CTAs in flight; clusters of more than two that would fill more than 7/8 of the SMs do
+// not all fit at once.  Measured, unsplit / 2 / 4 CTAs: 1 x 4096 x 4096 9.1 / 6.3 / 5.4 us, 16 x 2048 x 2048 5.9 / 4.9 / 4.3, 300 x
 // 768 x 768 4.6 / 5.1 / 5.0, 1024 x 8192 x 128 12.1 / 9.0 / 6.9, 1024 x 1024 x 1024 (128 tiles) 4.9 / 6.9 / 12.6.
 struct FewGrid {
   int tiles, row_tiles, split;
@@ -189,7 +189,7 @@ FewGrid few_grid(const MxLinearArgs& a, int bn, int sms) {
   double best = k_tiles * per_k_tile;
   for (int split = 2; split <= std::min(kMxMaxSplit, k_tiles); ++split) {
     const double ctas = (double)g.tiles * g.row_tiles * split;
-    if (8 * ctas > 7 * sms) break;
+    if (split == 2 ? ctas > sms : 8 * ctas > 7 * sms) break;
     const double t = (k_tiles + split - 1) / split * per_k_tile + 1.1 * ctas / 128;
     if (t < best) { best = t; g.split = split; }
   }
@@ -213,8 +213,8 @@ void launch_few(const MxLinearArgs& a, int dev, cudaStream_t st) {
 // nearly fill them and K is long (the tiles' operands then come from L2 too slowly): 128 x 4096 x 4096 takes
 // 7.8 us against 10.0 for the pair kernel's 256 x 128 tiles, 1024 x 1024 x 1024 4.9 against 5.8, 511 x 776 x 2304 with a
 // GELU 6.9 against 9.5, 192 x 4096 x 4096 (96 tiles) 9.3 against 9.9, but 256 x 4096 x 4096 (128) 11.1 against
-// 9.7.  A gated pair tile has only 128 output columns, and the few-row kernel wins wherever it fits (256 x 2048 x
-// 2 x 4096: 12.9 against 13.9).
+// 9.7.  Gated, only where K is split: 128 x 4096 x 2 x 4096 14.3 against 16.4, unsplit 256 x 2048 x 2 x 4096
+// 11.5 against 10.8.
 //
 // Otherwise CTA pairs: the tile for which this estimate is the shorter.  A wave of tiles takes the longer of
 // its MMAs' and its epilogue's time (microseconds, fitted to 256 .. 3000 rows with 768 .. 4096 columns and
@@ -227,7 +227,7 @@ void launch_linear(const MxLinearArgs& a, int dev, cudaStream_t st) {
   const int sms = sm_count(dev), k_tiles = mx_col_tiles(a.K);
   const FewGrid few = few_grid(a, 64, sms);
   const bool fits = (int64_t)few.tiles * few.row_tiles <= sms;
-  const bool slow = !kGated && few.split == 1 && 4LL * few.tiles * few.row_tiles > 3 * sms && k_tiles > 16;
+  const bool slow = few.split == 1 && (kGated || (4LL * few.tiles * few.row_tiles > 3 * sms && k_tiles > 16));
   if (a.M <= 64 || (fits && !slow)) return launch_few<64, kGated>(a, dev, st);
   if constexpr (!kGated) {
     auto estimate = [&](int bn, double per_k_tile, double epilogue, double once) {

@@ -289,14 +289,22 @@ __device__ __forceinline__ float* mx_stage_at(uint8_t* stage, int r, int c) {
   return reinterpret_cast<float*>(stage + r * 128 + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4);
 }
 
-// Adds `bias` (the same 32 values for all lanes) to v.
+// Adds `bias` (the same 32 values for all lanes) to v: a whole chunk's loads in flight together.
 __device__ __forceinline__ void mx_add_bias(const float* bias, int c0, int N, float (&v)[32]) {
+  if (c0 + 32 <= N) {
+    float4 t[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float t[4];
-    load4(bias + c0 + 4 * j, max(0, min(4, N - c0 - 4 * j)), true, t);
+    for (int j = 0; j < 8; ++j) t[j] = reinterpret_cast<const float4*>(bias + c0)[j];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[4 * j + i] += t[i];
+    for (int j = 0; j < 8; ++j) {
+      v[4 * j] += t[j].x; v[4 * j + 1] += t[j].y; v[4 * j + 2] += t[j].z; v[4 * j + 3] += t[j].w;
+    }
+  } else {
+    // The lane's own column's value, handed round.
+    const int lane = threadIdx.x & 31;
+    const float mine = bias[min(c0 + lane, N - 1)];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, mine, i);
   }
 }
 
