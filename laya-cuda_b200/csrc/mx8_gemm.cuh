@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
     };
     // The residual is loaded kDepth chunks ahead of its use, over tiles' ends too, and brought into L2 a tile
     // ahead.  (One chunk ahead, a chunk waits 1,000 to 1,700 cycles for it.)
-    constexpr int kDepth = kRes == MX_RES_HALF || (kRes == MX_RES_FULL && !kGated) ? 2 : 1;
+    constexpr int kDepth =
+        kRes == MX_RES_HALF || (!kGated && (kRes == MX_RES_FULL || kRes == MX_RES_ANY_HALF)) ? 2 : 1;
     MxResidualRow<kRes> in[kDepth];
     auto prefetch = [&](const Tile& t) {
       if constexpr (kRes != MX_RES_NONE) {

@@ -243,13 +243,13 @@ enum MxResidual : int {
 };
 __host__ __device__ constexpr int mx_res_size(int res) { return res == MX_RES_HALF || res == MX_RES_ANY_HALF ? 2 : 4; }
 
-// 32 residual values of a row: 16-bit pairs (MX_RES_HALF) or fp32.  Fetched apart from their use, so that the
-// loads are in flight while the accumulator is waited for.  (For rows of any alignment, 32 loads of one row's
-// neighbouring elements each, turned through shared memory, took 50 us where these shifted granules take 36:
-// 16384 x 768 x 767 bf16.)
+// 32 residual values of a row as loaded: whole vectors, or, for rows of any alignment, the aligned 16-byte granules that
+// hold them, `shift` bytes into the first.  Fetched apart from their use, so that the loads are in flight while
+// the accumulator is waited for.
 template <int kRes>
 struct MxResidualRow {
-  uint32_t w[kRes == MX_RES_NONE ? 1 : kRes == MX_RES_HALF ? 16 : 32];
+  uint32_t w[kRes == MX_RES_NONE ? 1 : kRes == MX_RES_HALF ? 16 : kRes == MX_RES_FULL ? 32 : kRes == MX_RES_ANY_HALF ? 20 : 36];
+  uint32_t shift;
 };
 
 template <int kRes>
@@ -267,19 +267,19 @@ __device__ __forceinline__ void mx_fetch_row(const MxLinearArgs& a, int row, int
                    : "l"(p + 32 * i));
     }
   } else if constexpr (kRes != MX_RES_NONE) {
-    const size_t at = (size_t)row * a.ldr + c0;
-    auto read = [&](auto* p) {
+    // Only granules with an element of the result are read: past the row's last one, that one again.
+    constexpr int kSize = mx_res_size(kRes);
+    const char* first = static_cast<const char*>(a.residual) + (size_t)min(row, a.M - 1) * a.ldr * kSize;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(first) + (size_t)min(c0, a.N - 1) * kSize;
+    const uintptr_t last = (reinterpret_cast<uintptr_t>(first) + (size_t)(a.N - 1) * kSize) & ~(uintptr_t)15;
+    in.shift = (uint32_t)at & 15;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float t[16];
-        load_any(p + at + 16 * i, row < a.M ? a.N - c0 - 16 * i : 0, t);
-#pragma unroll
-        for (int k = 0; k < 16; ++k) in.w[16 * i + k] = __float_as_uint(t[k]);
-      }
-    };
-    if (kRes == MX_RES_ANY_FULL) read(static_cast<const float*>(a.residual));
-    else if (a.residual_type == MX_BF16) read(static_cast<const __nv_bfloat16*>(a.residual));
-    else read(static_cast<const __half*>(a.residual));
+    for (int i = 0; i < 2 * kSize + 1; ++i) {
+      uintptr_t p = (at & ~(uintptr_t)15) + 16 * i;
+      p = p < last ? p : last;
+      uint32_t* w = in.w + 4 * i;
+      asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+    }
   }
 }
 
@@ -357,9 +357,35 @@ __device__ __forceinline__ uint32_t mx_finish_row(const MxLinearArgs& a, int row
     };
     if (a.residual_type == MX_BF16) add((__nv_bfloat16*)nullptr);
     else add((__half*)nullptr);
-  } else if constexpr (kRes != MX_RES_NONE) {
+  } else if constexpr (kRes == MX_RES_FULL) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(in.w[i]);
+  } else if constexpr (kRes != MX_RES_NONE) {
+    constexpr int kWords = 8 * mx_res_size(kRes);
+    uint32_t w[kWords + 4];
+#pragma unroll
+    for (int i = 0; i < kWords + 4; ++i) w[i] = in.w[i];
+#pragma unroll
+    for (int i = 0; i < kWords + 2; ++i) w[i] = in.shift & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < kWords + 1; ++i) w[i] = in.shift & 4 ? w[i + 1] : w[i];
+    if constexpr (kRes == MX_RES_ANY_FULL) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = in.shift & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+      auto add = [&](auto* type) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 r = unpack2_f32(w[i], type);
+          v[2 * i] += r.x;
+          v[2 * i + 1] += r.y;
+        }
+      };
+      if (a.residual_type == MX_BF16) add((__nv_bfloat16*)nullptr);
+      else add((__half*)nullptr);
+    }
   }
   const bool live = row < a.M;
   const size_t at = (size_t)row * a.ldo + c0;

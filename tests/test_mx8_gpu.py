@@ -389,19 +389,92 @@ def test_linear_strides_and_alignment(rows, pad, offset, out_type):
     run_linear(rows, 200, 133, out_type, bias=True, residual="bf16", seed=2, pad=pad, offset=offset)
 
 
-@pytest.mark.parametrize("rows", [3, 260])
-def test_linear_adds_into_the_residual_in_place(rows):
+def decode_gpu(m):
+    """decode() on the GPU, for the larger cases: float64 values."""
+    q = torch.from_numpy(TABLE).cuda()[m.values[:, : m.cols].long()]
+    byte = m.scales[torch.from_numpy(scale_index(m.rows, m.cols)).cuda()].double()
+    return q * torch.exp2(byte - 127).repeat_interleave(32, dim=1)[:, : m.cols]
+
+
+LARGE = [  # rows, cols, features: 256 x 128 tiles; 256 x 256 tiles; gated tiles
+    (2500, 160, 500, False), (2560, 128, 512, False), (2309, 70, 600, False),
+    (1024, 4096, 4096, False), (1030, 4100, 4130, False), (4096, 1024, 3584, False),
+    (1500, 300, 700, True), (2100, 640, 1056, True)]
+
+
+@pytest.mark.parametrize("rows,cols,n,gated", LARGE)
+@pytest.mark.parametrize("out_type,act,bias,residual,pad,offset", [
+    ("bf16", "none", False, None, 0, 0), ("f16", "silu", True, "bf16", 0, 0), ("f32", "none", True, "f32", 0, 0),
+    ("mx8", "relu", False, "f16", 0, 0), ("mx8", "gelu", True, None, 0, 0), ("bf16", "none", False, "f16", 3, 1),
+    ("f32", "gelu", False, "f32", 1, 1), ("f16", "none", False, "f32", 32, 16)])
+def test_linear_large(rows, cols, n, gated, out_type, act, bias, residual, pad, offset):
+    """Results too large for the few-row kernel, over its tile forms, against float64 on the GPU; the operands'
+    float64 values are read back from what `quantize` wrote."""
+    g = torch.Generator(device="cuda").manual_seed(rows + cols + n)
+    rand = lambda *shape: torch.randn(*shape, generator=g, device="cuda")  # noqa: E731
+    x, w, gate = fresh(rows, cols), fresh(n, cols), fresh(n, cols) if gated else None
+    mx8.quantize(rand(rows, cols) * torch.exp(0.8 * rand(cols)), x)
+    for m in (w, gate) if gated else (w,):
+        mx8.quantize(rand(n, cols) / math.sqrt(cols), m)
+    b, gb = 0.1 * rand(n) if bias else None, 0.1 * rand(n) if bias and gated else None
+    r = None
+    if residual:
+        r, _ = strided(rows, n, TYPES[residual], pad, offset)
+        r.copy_(rand(rows, n))
+    xd, to64 = decode_gpu(x), lambda t: None if t is None else t.double()
+
+    def product(m, add):
+        md = decode_gpu(m)
+        v, d = xd @ md.T, (cols / 32 + 1) * 2.0 ** -20 * ((xd * xd) @ (md * md).T).sqrt()
+        return (v, d) if add is None else (v + add, d + 2.0 ** -23 * (v + add).abs())
+
+    def apply(v):
+        f = {"relu": lambda t: t.clamp(min=0), "gelu": lambda t: 0.5 * t * torch.erfc(-t / math.sqrt(2)),
+             "silu": lambda t: t * torch.sigmoid(t)}
+        return f[act](v) if act in f else v
+
+    # The slack of `reference`, on the GPU.
+    u, du = product(w, to64(b))
+    if gated:
+        p, dp = product(gate, to64(gb))
+        a = apply(p)
+        da = 1.13 * dp + 1e-6 * (1 + a.abs())
+        y, dy = a * u, u.abs() * da + a.abs() * du + da * du
+    else:
+        y = apply(u)
+        dy = 1.13 * du + (0 if act == "none" else 1e-6 * (1 + y.abs()))
+    if r is not None:
+        y, dy = y + r.double(), dy + 2.0 ** -23 * (y + r.double()).abs()
+    dy = dy + 2.0 ** -22 * y.abs()
+
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, store = (fresh(rows, n), None) if out_type == "mx8" else strided(rows, n, TYPES[out_type], pad, offset)
+    mx8.linear(x, w, out, bias=b, gate=gate, gate_bias=gb, activation=act, residual=r, err=err)
+    assert int(err.item()) == 0
+    if out_type == "mx8":
+        check_mx8(out, y.cpu().numpy(), dy.cpu().numpy())
+    else:
+        off, tol = (out.double() - y).abs(), dy + HALF_ULP[out_type] * (y.abs() + dy) + TINY[out_type]
+        assert bool((off <= tol).all()), float((off / tol).max())
+        assert untouched(out, store, pad, offset)
+    if r is not None and out_type == residual:
+        mx8.linear(x, w, r, bias=b, gate=gate, gate_bias=gb, activation=act, residual=r)
+        assert torch.equal(r, out)
+
+
+@pytest.mark.parametrize("rows,n", [(3, 256), (260, 255), (2600, 512), (2600, 511), (6000, 129)])
+def test_linear_adds_into_the_residual_in_place(rows, n):
     rng = np.random.default_rng(8)
     x, _ = matrix(activations(rng, rows, 192))
-    w, _ = matrix(rng.normal(0, 0.1, (256, 192)).astype(np.float32))
-    r = torch.from_numpy(rng.normal(0, 1, (rows, 256)).astype(np.float32)).cuda()
+    w, _ = matrix(rng.normal(0, 0.1, (n, 192)).astype(np.float32))
+    r = torch.from_numpy(rng.normal(0, 1, (rows, n)).astype(np.float32)).cuda()
     want = torch.empty_like(r)
     mx8.linear(x, w, want, residual=r)
     mx8.linear(x, w, r, residual=r)
     assert torch.equal(r, want)
 
 
-@pytest.mark.parametrize("rows", [5, 150, 400])
+@pytest.mark.parametrize("rows", [5, 150, 400, 3400])
 def test_linear_keeps_non_finite_values_to_their_rows(rows):
     """A NaN block of x makes its row NaN, one of w its column; nothing else changes.  The scales of rows past
     the last hold NaN bytes (see `matrix`) and reach no result."""
@@ -419,7 +492,7 @@ def test_linear_keeps_non_finite_values_to_their_rows(rows):
     assert torch.equal(torch.nan_to_num(out), torch.nan_to_num(want))
 
 
-@pytest.mark.parametrize("rows,cols,n", [(4, 2048, 512), (90, 1024, 512), (700, 512, 768)])
+@pytest.mark.parametrize("rows,cols,n", [(4, 2048, 512), (90, 1024, 512), (700, 512, 768), (2600, 512, 768)])
 def test_linear_gives_the_same_bits_each_time_and_a_row_does_not_depend_on_the_others(rows, cols, n):
     rng = np.random.default_rng(10)
     xv = activations(rng, rows, cols)
@@ -454,7 +527,7 @@ def test_one_layer_on_another_stream():
     assert (np.abs(y.double().cpu().numpy() - want) <= slack + 2.0 ** -23 * np.abs(want)).all()
 
 
-@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("rows", [1, 40, 300, 10000])
 def test_captured_in_a_graph(rows):
     """The calls can be captured and replayed on new inputs, and give the bits of plain calls."""
     rng = np.random.default_rng(12)
@@ -508,7 +581,7 @@ def test_offsets_past_32_bits():
     assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("rows,cols,n,gated", [(3, 65536, 256, False), (40, 65536, 300, True), (300, 65536, 520, False), (700, 65536, 512, True)])
+@pytest.mark.parametrize("rows,cols,n,gated", [(3, 65536, 256, False), (40, 65536, 300, True), (300, 65536, 520, False), (3000, 32768, 520, False), (2600, 16384, 512, True)])
 def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable(rows, cols, n, gated):
     """Valid calls, deep enough that the epilogue waits for many microseconds, whose waits are limited to a nanosecond: the
     kernel unwinds and sets `err`; the next call, with the default limit, gives the bits of a call before it."""
