@@ -239,13 +239,13 @@ void launch_linear(const MxLinearArgs& a, int dev, cudaStream_t st) {
   launch_pair<256, kGated>(a, dev, st);
 }
 
-// Blocks for `pieces` pieces, `per_block` of them per block and pass and `unroll` passes at once: all
-// that are of use, at most 8 per SM.
-int pieces_grid(int64_t pieces, int per_block, int unroll, int sms) {
-  const int64_t per = (int64_t)per_block * unroll;
-  return (int)std::min<int64_t>((pieces + per - 1) / per, 8LL * sms);
+// Blocks of a conversion: one pass each up to 32 per SM, several beyond.  Blocks that follow one another through the
+// matrix read and write HBM in order; 8 per SM that stride over it took 35.0 us where these take 32.0 (16384 x
+// 4096 to bf16; to fp32 61.9 and 51.9, 9216 x 4096 fp32 to MX8 30.3 and 28.3), and two pieces in flight per thread
+// made no difference then.
+int pieces_grid(int64_t pieces, int per_block, int sms) {
+  return (int)std::min<int64_t>((pieces + per_block - 1) / per_block, 32LL * sms);
 }
-constexpr int kConvertUnroll = 2;
 
 template <typename T, typename R, int CH, bool kVec, bool kShort>
 void launch_norm_rows(RmsNormArgs a, int sms, cudaStream_t st) {
@@ -311,14 +311,13 @@ int laya_op_mx8_quantize(const laya_mx8_convert* p, void* stream) {
   with_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const T* x = static_cast<const T*>(p->data);
-    auto go = [&](auto kern, int unroll) {
-      launch_k(kern, dim3(pieces_grid(groups, kMxThreads / 8, unroll, sms)), dim3(kMxThreads), 0, st, x, p->ld, rows, cols,
+    auto go = [&](auto kern) {
+      launch_k(kern, dim3(pieces_grid(groups, kMxThreads / 8, sms)), dim3(kMxThreads), 0, st, x, p->ld, rows, cols,
                FastDiv((uint32_t)mx_col_tiles(cols)),
                static_cast<uint8_t*>(p->values), p->ldv, static_cast<uint8_t*>(p->scales));
     };
-    if (!rows_vectored(x, p->ld, cols)) go(mx8_quantize_kernel<T, false, 1>, 1);
-    else if (groups < 8LL * 32 * sms) go(mx8_quantize_kernel<T, true, 1>, 1);
-    else go(mx8_quantize_kernel<T, true, kConvertUnroll>, kConvertUnroll);
+    if (rows_vectored(x, p->ld, cols)) go(mx8_quantize_kernel<T, true>);
+    else go(mx8_quantize_kernel<T, false>);
   });
   MX_API_END
 }
@@ -340,14 +339,13 @@ int laya_op_mx8_dequantize(const laya_mx8_convert* p, void* stream) {
   with_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     T* out = static_cast<T*>(p->data);
-    auto go = [&](auto kern, int unroll) {
-      launch_k(kern, dim3(pieces_grid(pieces, kMxThreads, unroll, sms)), dim3(kMxThreads), 0, st,
+    auto go = [&](auto kern) {
+      launch_k(kern, dim3(pieces_grid(pieces, kMxThreads, sms)), dim3(kMxThreads), 0, st,
                static_cast<const uint8_t*>(p->values), p->ldv, static_cast<const uint8_t*>(p->scales), rows, cols, FastDiv(per_row), out,
                p->ld);
     };
-    if (!rows_vectored(out, p->ld, cols)) go(mx8_dequantize_kernel<T, false, 1>, 1);
-    else if (pieces < 8LL * kMxThreads * sms) go(mx8_dequantize_kernel<T, true, 1>, 1);
-    else go(mx8_dequantize_kernel<T, true, kConvertUnroll>, kConvertUnroll);
+    if (rows_vectored(out, p->ld, cols)) go(mx8_dequantize_kernel<T, true>);
+    else go(mx8_dequantize_kernel<T, false>);
   });
   MX_API_END
 }

@@ -88,8 +88,8 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 // for 16384 x 4096 bf16 to MX8); sixteen share the addresses and shuffles.
 //
 // kVec: rows of whole 32-byte vectors (`rows_vectored`), read and written as such; a thread's bf16
-// piece is one of them.  (Two 16-byte stores per thread instead fill half sectors: 48 us against
-// 35 us for 16384 x 4096 back to bf16.)  Otherwise rows of any length and alignment: a piece is read
+// piece is one of them.  (Two 16-byte stores per thread instead fill half sectors: 48 us where this
+// took 35 for 16384 x 4096 back to bf16.)  Otherwise rows of any length and alignment: a piece is read
 // as the aligned 16-byte granules that hold it, shifted into place, and written element by element,
 // through shared memory so that neighbouring lanes write neighbouring elements.
 // ---------------------------------------------------------------------------------------------
@@ -249,44 +249,35 @@ __device__ __forceinline__ void mx_store_piece(const float (&v)[kMxPiece], int r
 }
 
 // ---------------------------------------------------------------------------------------------
-// x [rows][cols] -> MX8.  Eight threads take 128 columns of a row (a group), and each U of them at
-// once.  HBM-bound: x is read and the values and scales written once, 16384 x 4096 bf16 in 32.8 us and 9216 x
-// 4096 fp32 in 30.3 (6.2 TB/s, 95% of a copy's rate); a small call is its launch (768 values: 1.2 us).
+// x [rows][cols] -> MX8.  Eight threads take 128 columns of a row (a group).  HBM-bound: x is read and the
+// values and scales written once, 16384 x 4096 bf16 in 32.5 us (6.3 TB/s) and 9216 x 4096 fp32 in 28.3 (6.7; a
+// copy's rate is 6.5); a small call is its launch (768 values: 1.2 us).
 // ---------------------------------------------------------------------------------------------
 constexpr int kMxThreads = 256;
 
-template <typename T, bool kVec, int U>
+template <typename T, bool kVec>
 __global__ void __launch_bounds__(kMxThreads) mx8_quantize_kernel(const T* x, int64_t ldx, int rows, int cols, FastDiv col_tiles,
                                                                   uint8_t* q, int64_t ldq, uint8_t* scales) {
   pdl_wait();
   const uint32_t groups = (uint32_t)rows * col_tiles.d;  // below 2^31
   const uint32_t step = gridDim.x * (kMxThreads / 8);
   // The loop bound is the warp's first group, so that its 32 threads stay together.
-  for (uint32_t g0 = blockIdx.x * (kMxThreads / 8) + (threadIdx.x >> 5) * 4; g0 < groups; g0 += step * U) {
-    int row[U], col[U];
-    bool live[U];
-    Raw<T> raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t g = g0 + u * step + ((threadIdx.x >> 3) & 3);
-      live[u] = g < groups;
-      row[u] = live[u] ? (int)col_tiles.div(g) : 0;
-      col[u] = live[u] ? (int)(g - (uint32_t)row[u] * col_tiles.d) * kMxTileCols + (threadIdx.x & 7) * kMxPiece : 0;
-      if (kVec) raw[u] = load_raw(x + (size_t)row[u] * ldx + col[u], live[u] && col[u] < cols);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float v[kMxPiece];
-      if (kVec) unpack(raw[u], v);
-      else load_any(x + (size_t)row[u] * ldx + col[u], live[u] ? cols - col[u] : 0, v);
-      mx_store_piece(v, row[u], col[u], cols, (int)col_tiles.d, live[u], q, ldq, scales);
-    }
+  for (uint32_t g0 = blockIdx.x * (kMxThreads / 8) + (threadIdx.x >> 5) * 4; g0 < groups; g0 += step) {
+    const uint32_t g = g0 + ((threadIdx.x >> 3) & 3);
+    const bool live = g < groups;
+    const int row = live ? (int)col_tiles.div(g) : 0;
+    const int col = live ? (int)(g - (uint32_t)row * col_tiles.d) * kMxTileCols + (threadIdx.x & 7) * kMxPiece : 0;
+    const T* p = x + (size_t)row * ldx + col;
+    float v[kMxPiece];
+    if constexpr (kVec) unpack(load_raw(p, live && col < cols), v);
+    else load_any(p, live ? cols - col : 0, v);
+    mx_store_piece(v, row, col, cols, (int)col_tiles.d, live, q, ldq, scales);
   }
 }
 
-// MX8 -> out [rows][cols], U pieces per thread at once.  HBM-bound, two thirds of it writes: 16384 x 4096 to
-// bf16 in 34.9 us (5.8 TB/s), to fp32 in 61.8 (5.5).
-template <typename T, bool kVec, int U>
+// MX8 -> out [rows][cols], a piece per thread.  HBM-bound, two thirds of it writes: 16384 x 4096 to bf16 in
+// 32.0 us (6.4 TB/s), to fp32 in 51.9 (6.5).
+template <typename T, bool kVec>
 __global__ void __launch_bounds__(kMxThreads) mx8_dequantize_kernel(const uint8_t* q, int64_t ldq, const uint8_t* scales,
                                                                     int rows, int cols, FastDiv per_row, T* out, int64_t ldo) {
   pdl_wait();
@@ -295,39 +286,26 @@ __global__ void __launch_bounds__(kMxThreads) mx8_dequantize_kernel(const uint8_
   const uint32_t step = gridDim.x * kMxThreads;
   __shared__ __align__(16) T stage[kVec ? 1 : kMxThreads / 32][kVec ? 8 : 32 * kMxPiece];
   // The loop bound is the warp's first piece, so that its 32 threads stay together.
-  for (uint32_t w0 = blockIdx.x * kMxThreads + (threadIdx.x & ~31u); w0 < pieces; w0 += step * U) {
-    const uint32_t i0 = w0 + (threadIdx.x & 31);
-    int row[U], col[U];
-    uint4 w[U];
-    uint32_t byte[U];
+  for (uint32_t w0 = blockIdx.x * kMxThreads + (threadIdx.x & ~31u); w0 < pieces; w0 += step) {
+    const bool live = w0 + (threadIdx.x & 31) < pieces;
+    const uint32_t i = min(w0 + (threadIdx.x & 31), pieces - 1);  // past the end: the last piece again, not stored
+    const int row = (int)per_row.div(i), col = (int)(i - (uint32_t)row * per_row.d) * kMxPiece;
+    const uint4 w = *reinterpret_cast<const uint4*>(q + (size_t)row * ldq + col);
+    const float s = mx_scale(scales[mx_scale_tile(row, col / kMxTileCols, col_tiles) + mx_scale_row(row) + ((col / kMxBlock) & 3)]);
+    float v[kMxPiece];
+    mx_unpack4(w.x, v);
+    mx_unpack4(w.y, v + 4);
+    mx_unpack4(w.z, v + 8);
+    mx_unpack4(w.w, v + 12);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t i = min(i0 + u * step, pieces - 1);  // past the end: the last piece again, not stored
-      row[u] = (int)per_row.div(i);
-      col[u] = (int)(i - (uint32_t)row[u] * per_row.d) * kMxPiece;
-      w[u] = *reinterpret_cast<const uint4*>(q + (size_t)row[u] * ldq + col[u]);
-      byte[u] = scales[mx_scale_tile(row[u], col[u] / kMxTileCols, col_tiles) + mx_scale_row(row[u]) + ((col[u] / kMxBlock) & 3)];
+    for (int k = 0; k < kMxPiece; k += 2) {
+      const float2 t = mul2(make_float2(v[k], v[k + 1]), make_float2(s, s));
+      v[k] = t.x;
+      v[k + 1] = t.y;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float s = mx_scale(byte[u]);
-      const float2 s2 = make_float2(s, s);
-      float v[kMxPiece];
-      mx_unpack4(w[u].x, v);
-      mx_unpack4(w[u].y, v + 4);
-      mx_unpack4(w[u].z, v + 8);
-      mx_unpack4(w[u].w, v + 12);
-#pragma unroll
-      for (int k = 0; k < kMxPiece; k += 2) {
-        const float2 t = mul2(make_float2(v[k], v[k + 1]), s2);
-        v[k] = t.x;
-        v[k + 1] = t.y;
-      }
-      const bool live = i0 + u * step < pieces;
-      T* p = out + (size_t)row[u] * ldo + col[u];
-      if constexpr (kVec) store_vec(p, live, v);
-      else store_any(stage[threadIdx.x >> 5], p, live ? cols - col[u] : 0, v);
-    }
+    T* p = out + (size_t)row * ldo + col;
+    if constexpr (kVec) store_vec(p, live, v);
+    else store_any(stage[threadIdx.x >> 5], p, live ? cols - col : 0, v);
   }
 }
 
