@@ -90,8 +90,9 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 // kVec: rows of whole 32-byte vectors (`rows_vectored`), read and written as such; a thread's bf16
 // piece is one of them.  (Two 16-byte stores per thread instead fill half sectors: 48 us where this
 // took 35 for 16384 x 4096 back to bf16.)  Otherwise rows of any length and alignment: a piece is read
-// as the aligned 16-byte granules that hold it, shifted into place, and written element by element,
-// through shared memory so that neighbouring lanes write neighbouring elements.
+// as the aligned 16-byte granules that hold it, shifted into place, and written through shared memory:
+// element by element so that neighbouring lanes write neighbouring elements (`store_any`), or in
+// sectors put together from two lanes' pieces (`store_run`).
 // ---------------------------------------------------------------------------------------------
 constexpr int kMxPiece = 16;
 
@@ -146,17 +147,37 @@ __device__ __forceinline__ Raw<T> pack(const float (&v)[kMxPiece]) {
   return r;
 }
 
+// Sixteen elements to 32-byte aligned p.
 template <typename T>
-__device__ __forceinline__ void store_vec(T* p, bool live, const float (&v)[kMxPiece]) {
-  const Raw<T> r = pack<T>(v);
-  if (!live) return;
+__device__ __forceinline__ void store_raw(void* p, const Raw<T>& r) {
 #pragma unroll
   for (int i = 0; i < (int)sizeof(r.w) / 32; ++i) {
     const uint32_t* w = r.w + 8 * i;
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<char*>(p) + 32 * i),
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<char*>(p) + 32 * i),
                  "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, bool live, const float (&v)[kMxPiece]) {
+  const Raw<T> r = pack<T>(v);
+  if (live) store_raw(p, r);
+}
+
+// Sixteen elements out of the 16-byte granules that hold them, the first at byte `shift` of 16.
+template <typename T>
+__device__ __forceinline__ Raw<T> shift_granules(uint32_t (&w)[4 * (sizeof(T) + 1)], uint32_t shift) {
+  constexpr int kWords = 4 * (sizeof(T) + 1);
+#pragma unroll
+  for (int i = 0; i + 2 < kWords; ++i) w[i] = shift & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i + 1 < kWords - 2; ++i) w[i] = shift & 4 ? w[i + 1] : w[i];
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)(4 * sizeof(T)); ++i)
+    r.w[i] = sizeof(T) == 2 && (shift & 2) ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+  return r;
 }
 
 // The first n of sixteen elements at p, zeros for the others.  Only granules that hold an element
@@ -175,36 +196,79 @@ __device__ __forceinline__ void load_any(const T* p, int n, float (&v)[kMxPiece]
     if (16 * i < end) g = base[i];
     w[4 * i] = g.x; w[4 * i + 1] = g.y; w[4 * i + 2] = g.z; w[4 * i + 3] = g.w;
   }
-#pragma unroll
-  for (int i = 0; i + 2 < 4 * kGranules; ++i) w[i] = shift & 8 ? w[i + 2] : w[i];
-#pragma unroll
-  for (int i = 0; i + 1 < 4 * kGranules - 2; ++i) w[i] = shift & 4 ? w[i + 1] : w[i];
-  Raw<T> r;
-#pragma unroll
-  for (int i = 0; i < (int)(4 * sizeof(T)); ++i)
-    r.w[i] = sizeof(T) == 2 && (shift & 2) ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
-  unpack(r, v);
+  unpack(shift_granules<T>(w, shift), v);
 #pragma unroll
   for (int i = 0; i < kMxPiece; ++i) v[i] = i < n ? v[i] : 0.f;
 }
 
-// The first n of each lane's sixteen elements to its p; the warp calls this together.  `stage`: 512
-// elements of shared memory of the warp's own, 16-byte aligned.
+// The lanes' sixteen elements to `stage`, 512 elements of shared memory of the warp's own, 16-byte aligned.
 template <typename T>
-__device__ __forceinline__ void store_any(T* stage, T* p, int n, const float (&v)[kMxPiece]) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void stage_pieces(T* stage, const float (&v)[kMxPiece]) {
   const Raw<T> r = pack<T>(v);
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < (int)sizeof(T); ++i)
-    reinterpret_cast<uint4*>(stage + lane * kMxPiece)[i] = make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
+    reinterpret_cast<uint4*>(stage + (threadIdx.x & 31) * kMxPiece)[i] =
+        make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
   __syncwarp();
+}
+
+// The first n of each lane's sixteen elements to its p; the warp calls this together.
+template <typename T>
+__device__ __forceinline__ void store_any(T* stage, T* p, int n, const float (&v)[kMxPiece]) {
+  const int lane = threadIdx.x & 31;
+  stage_pieces(stage, v);
 #pragma unroll
   for (int j = 0; j < kMxPiece; ++j) {
     const int from = 2 * j + (lane >> 4), at = lane & 15;
     T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), from));
     const int many = __shfl_sync(0xffffffffu, n, from);
     if (at < many) to[at] = stage[32 * j + lane];
+  }
+}
+
+// The same for 16-bit types where most lanes' pieces follow one another: a lane whose p follows the piece of the
+// lane before writes the whole 32-byte sector that holds its first element, the end of that piece and the start of
+// its own.  What is in no lane's sector (the ends of rows and of the warp's run) goes an element at a time, two
+// lanes' pieces per instruction.
+template <typename T>
+__device__ __forceinline__ void store_run(T* stage, T* p, int n, const float (&v)[kMxPiece]) {
+  static_assert(sizeof(T) == 2, "a piece is a sector");
+  const int lane = threadIdx.x & 31;
+  stage_pieces(stage, v);
+  n = max(0, min(n, kMxPiece));
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const int over = (int)(at & 31);   // bytes of the sector before p
+  const int head = (32 - over) / 2;  // elements of this piece in the sector
+  const uintptr_t before = __shfl_up_sync(0xffffffffu, (unsigned long long)(n == kMxPiece ? at : 0), 1);
+  const bool follows = lane > 0 && before != 0 && before + 32 == at && n >= head;
+  const bool whole = follows || (over == 0 && n == kMxPiece);
+  const bool followed = __shfl_down_sync(0xffffffffu, (int)follows, 1) && lane < 31;
+  if (whole) {
+    const int from = lane * 32 - over;  // of the warp's bytes in `stage`
+    const uint32_t shift = (uint32_t)from & 15;
+    const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(stage) + (from - (int)shift));
+    uint32_t w[12];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      uint4 g = make_uint4(0, 0, 0, 0);
+      if (i < 2 || shift) g = base[i];
+      w[4 * i] = g.x; w[4 * i + 1] = g.y; w[4 * i + 2] = g.z; w[4 * i + 3] = g.w;
+    }
+    store_raw(reinterpret_cast<char*>(p) - over, shift_granules<T>(w, shift));
+  }
+  // Bit i: element i is in no lane's sector.
+  const uint32_t rest = ((1u << n) - 1) & ((whole ? 0 : (1u << head) - 1) | (followed ? 0 : ~0u << head));
+  uint32_t lanes = __ballot_sync(0xffffffffu, rest != 0);
+  while (lanes) {
+    const int first = __ffs(lanes) - 1;
+    lanes &= lanes - 1;
+    const int second = lanes ? __ffs(lanes) - 1 : first;
+    lanes &= lanes - 1;
+    const int of = lane < kMxPiece ? first : second, i = lane & (kMxPiece - 1);
+    const uint32_t bits = __shfl_sync(0xffffffffu, rest, of);
+    T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, (unsigned long long)at, of));
+    if (bits >> i & 1) to[i] = stage[of * kMxPiece + i];
   }
 }
 
@@ -277,14 +341,17 @@ __global__ void __launch_bounds__(kMxThreads) mx8_quantize_kernel(const T* x, in
 
 // MX8 -> out [rows][cols], a piece per thread.  HBM-bound, two thirds of it writes: 16384 x 4096 to bf16 in
 // 32.0 us (6.4 TB/s), to fp32 in 51.9 (6.5).
-template <typename T, bool kVec>
+enum class MxStore { kVectors, kElements, kRuns };
+
+template <typename T, MxStore kStore>
 __global__ void __launch_bounds__(kMxThreads) mx8_dequantize_kernel(const uint8_t* q, int64_t ldq, const uint8_t* scales,
                                                                     int rows, int cols, FastDiv per_row, T* out, int64_t ldo) {
   pdl_wait();
   const int col_tiles = mx_col_tiles(cols);
   const uint32_t pieces = (uint32_t)rows * per_row.d;  // below 2^31
   const uint32_t step = gridDim.x * kMxThreads;
-  __shared__ __align__(16) T stage[kVec ? 1 : kMxThreads / 32][kVec ? 8 : 32 * kMxPiece];
+  constexpr bool kStaged = kStore != MxStore::kVectors;
+  __shared__ __align__(16) T stage[kStaged ? kMxThreads / 32 : 1][kStaged ? 32 * kMxPiece : 8];
   // The loop bound is the warp's first piece, so that its 32 threads stay together.
   for (uint32_t w0 = blockIdx.x * kMxThreads + (threadIdx.x & ~31u); w0 < pieces; w0 += step) {
     const bool live = w0 + (threadIdx.x & 31) < pieces;
@@ -304,7 +371,8 @@ __global__ void __launch_bounds__(kMxThreads) mx8_dequantize_kernel(const uint8_
       v[k + 1] = t.y;
     }
     T* p = out + (size_t)row * ldo + col;
-    if constexpr (kVec) store_vec(p, live, v);
+    if constexpr (kStore == MxStore::kVectors) store_vec(p, live, v);
+    else if constexpr (kStore == MxStore::kRuns) store_run(stage[threadIdx.x >> 5], p, live ? cols - col : 0, v);
     else store_any(stage[threadIdx.x >> 5], p, live ? cols - col : 0, v);
   }
 }
@@ -477,7 +545,10 @@ __global__ void __launch_bounds__(kMxThreads) rms_norm_mx8_long_kernel(const Rms
       const int col = col0 + (threadIdx.x & 31) * kMxPiece, n = a.cols - col;
       float h[kMxPiece];
       load(col, h);
-      if (s) store_any(stage[threadIdx.x >> 5], s + col, n, h);
+      if (s) {
+        if constexpr (sizeof(R) == 2) store_run(stage[threadIdx.x >> 5], s + col, n, h);
+        else store_any(stage[threadIdx.x >> 5], s + col, n, h);
+      }
 #pragma unroll
       for (int i = 0; i < kMxPiece; ++i) h[i] = i < n ? h[i] * inv * a.weight[col + i] : 0.f;
       mx_store_piece(h, row, col, a.cols, col_tiles, true, a.q, a.ldq, a.scales);

@@ -192,6 +192,21 @@ def test_dequantize_is_exact(dtype, rows, cols, pad, offset):
     assert untouched(out, store, pad, offset)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,cols,pad", [(67, 199, 0), (67, 200, 0), (67, 201, 2), (40, 217, 0), (40, 233, 7), (9, 511, 0), (9, 512, 1), (9, 513, 0),
+                                           (5, 1025, 3), (3, 4095, 0)])
+def test_dequantize_into_every_alignment(dtype, rows, cols, pad):
+    """Each place in a 32-byte sector at which a row can start; what lies around the rows stays."""
+    rng = np.random.default_rng(rows * 1000 + cols + 2)
+    m, v = matrix(activations(rng, rows, cols))
+    want = torch.from_numpy(v).to(TYPES[dtype])
+    for offset in range(16):
+        out, store = strided(rows, cols, TYPES[dtype], pad, offset)
+        mx8.dequantize(m, out)
+        assert torch.equal(out.cpu(), want), offset
+        assert untouched(out, store, pad, offset), offset
+
+
 def test_dequantize_every_code_and_scale():
     """Each E4M3 code under each scale byte (fp32 output; overflow to infinity as the rounding gives)."""
     q = torch.arange(256, dtype=torch.uint8).repeat(256, 1)
@@ -254,6 +269,27 @@ def test_rms_norm(dtype, rdtype, rows, cols, pad, offset):
     assert untouched(total, store, pad, offset)
     # h itself is rounded to fp32 once before it is squared and scaled.
     check_mx8(out, y, norm_slack(cols) * np.abs(y))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("cols", [16385, 16400, 20001])
+def test_rms_norm_sum_of_long_rows_at_every_alignment(dtype, cols):
+    """The sum is one fp32 addition and one rounding, whatever the place in a sector at which a row starts; here
+    also over the residual itself."""
+    rng = np.random.default_rng(cols)
+    x = torch.from_numpy(activations(rng, 3, cols)).to(TYPES[dtype]).cuda()
+    r = rng.normal(0, 1, (3, cols)).astype(np.float32)
+    want = (x.float() + torch.from_numpy(r).to(TYPES[dtype]).cuda().float()).to(TYPES[dtype])
+    w = torch.ones(cols, device="cuda")
+    first = None
+    for offset in range(16):
+        stream, store = strided(3, cols, TYPES[dtype], 1, offset, r)
+        out = fresh(3, cols)
+        mx8.rms_norm(x, w, out, residual=stream, sum_out=stream, eps=1e-5)
+        assert torch.equal(stream, want), offset
+        assert untouched(stream, store, 1, offset), offset
+        first = out if first is None else first
+        assert torch.equal(out.values, first.values) and torch.equal(out.scales, first.scales), offset
 
 
 def test_rms_norm_without_residual_and_in_place():
