@@ -181,6 +181,10 @@ const char* laya_last_error(laya_engine* e);
  * CUDA graphs keep the options in effect when they were captured. */
 int laya_set_launch_options(int programmatic_launch, uint64_t wait_limit_ns);
 
+/* The calling thread's current CUDA device, the one that kernel-level entry points launch on
+ * (LAYA_ERR_NO_DEVICE where there is none). */
+int laya_current_device(int* device);
+
 /* ------------------------------------------------------------------------------------------
  * Kernel-level entry points (device pointers, enqueued on `stream`), used by the parity tests
  * the way the reference's tests drive Ops directly (tests/test_gpu.py, tests/test_attention.py).

@@ -1925,6 +1925,17 @@ int laya_set_launch_options(int programmatic_launch, uint64_t wait_limit_ns) {
   return LAYA_OK;
 }
 
+int laya_current_device(int* device) {
+  API_BEGIN
+  if (!device) fail(LAYA_ERR_INVALID, "null argument");
+  *device = -1;
+  if (cudaGetDevice(device) != cudaSuccess) {
+    cudaGetLastError();
+    fail(LAYA_ERR_NO_DEVICE, "no CUDA device");
+  }
+  API_END(nullptr)
+}
+
 // ---------------------------------------------------------------------------------------------
 // Kernel-level entry points
 // ---------------------------------------------------------------------------------------------

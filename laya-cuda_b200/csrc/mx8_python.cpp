@@ -23,12 +23,14 @@ using ConvertFn = int (*)(const laya_mx8_convert*, void*);
 using NormFn = int (*)(const laya_rms_norm_mx8*, void*);
 using LinearFn = int (*)(const laya_mx8_linear*, int*, void*);
 using ErrorFn = const char* (*)(laya_engine*);
+using DeviceFn = int (*)(int*);
 
 struct Library {
   ConvertFn quantize, dequantize;
   NormFn rms_norm;
   LinearFn linear;
   ErrorFn last_error;
+  DeviceFn current_device;
 } g_lib = {};
 PyObject* g_loader = nullptr;  // called before the first operator: it calls bind()
 
@@ -471,6 +473,18 @@ bool ready() {
   return r && g_lib.linear;
 }
 
+// Binds the library, and refuses buffers on another device than the one that the call would launch on.  (Without a
+// current device the library's call says what is wrong; without rows it needs none.)
+bool ready_on(int device, int rows) {
+  if (!ready()) return false;
+  int current;
+  if (rows && g_lib.current_device(&current) == LAYA_OK && current != device) {
+    PyErr_Format(PyExc_ValueError, "the matrix is on CUDA device %d, the current device is %d", device, current);
+    return false;
+  }
+  return true;
+}
+
 // ValueError for refused arguments, RuntimeError for the rest, with the library's message.
 PyObject* finish(int status) {
   if (status == LAYA_OK) Py_RETURN_NONE;
@@ -485,7 +499,7 @@ PyObject* finish(int status) {
 PyObject* convert(const char* tensor, Matrix* m, PyObject* t, PyObject* stream, ConvertFn Library::*call) {
   Rows data;
   void* st;
-  if (!take_rows(tensor, t, m->rows, m->cols, m->device, &data) || !to_stream(stream, &st) || !ready()) return nullptr;
+  if (!take_rows(tensor, t, m->rows, m->cols, m->device, &data) || !to_stream(stream, &st) || !ready_on(m->device, m->rows)) return nullptr;
   laya_mx8_convert a{};
   a.rows = m->rows; a.cols = m->cols; a.dtype = data.dtype;
   a.values = reinterpret_cast<void*>(m->values_ptr); a.scales = reinterpret_cast<void*>(m->scales_ptr); a.ldv = m->ld;
@@ -549,7 +563,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject*
     if (eps == -1.0 && PyErr_Occurred()) return nullptr;
     a.eps = (float)eps;
   }
-  if (!to_stream(g[6], &st) || !ready()) return nullptr;
+  if (!to_stream(g[6], &st) || !ready_on(m->device, m->rows)) return nullptr;
   a.rows = m->rows; a.cols = m->cols; a.dtype = x.dtype;
   a.x = x.ptr; a.ldx = x.ld; a.residual = r.ptr; a.ldr = r.ld; a.sum_out = s.ptr; a.lds = s.ld;
   a.values = reinterpret_cast<void*>(m->values_ptr); a.scales = reinterpret_cast<void*>(m->scales_ptr); a.ldv = m->ld;
@@ -627,7 +641,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* k
     err = static_cast<int*>(v.data);
   }
   void* st;
-  if (!to_stream(g[9], &st) || !ready()) return nullptr;
+  if (!to_stream(g[9], &st) || !ready_on(device, rows)) return nullptr;
   int status;
   Py_BEGIN_ALLOW_THREADS
   status = g_lib.linear(&a, err, st);
@@ -652,10 +666,10 @@ PyObject* set_loader(PyObject*, PyObject* loader) {
 }
 
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long q, d, n, l, e;
-  if (!PyArg_ParseTuple(args, "KKKKK", &q, &d, &n, &l, &e)) return nullptr;
+  unsigned long long q, d, n, l, e, c;
+  if (!PyArg_ParseTuple(args, "KKKKKK", &q, &d, &n, &l, &e, &c)) return nullptr;
   g_lib = {reinterpret_cast<ConvertFn>(q), reinterpret_cast<ConvertFn>(d), reinterpret_cast<NormFn>(n),
-           reinterpret_cast<LinearFn>(l), reinterpret_cast<ErrorFn>(e)};
+           reinterpret_cast<LinearFn>(l), reinterpret_cast<ErrorFn>(e), reinterpret_cast<DeviceFn>(c)};
   Py_RETURN_NONE;
 }
 
@@ -678,7 +692,7 @@ PyMethodDef methods[] = {
     {"scale_bytes", py_scale_bytes, METH_VARARGS,
      "scale_bytes(rows, cols)\n--\n\nBytes of the scales of an MX8 matrix (tiles of 128 rows x 128 columns, 512 bytes each)."},
     {"set_loader", set_loader, METH_O, "set_loader(f)\n--\n\nf() is called before the first operator and calls bind()."},
-    {"bind", bind, METH_VARARGS, "bind(quantize, dequantize, rms_norm, linear, last_error)\n--\n\nAddresses of the library's functions."},
+    {"bind", bind, METH_VARARGS, "bind(quantize, dequantize, rms_norm, linear, last_error, current_device)\n--\n\nAddresses of the library's functions."},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mx8", nullptr, -1, methods};

@@ -20,7 +20,7 @@ EXPORTS = (
     "laya_shape_class",
     "laya_forward_device", "laya_packed_ints", "laya_pack", "laya_reserve", "laya_stream", "laya_set_profiling",
     "laya_profile_read", "laya_read_tensor", "laya_cached_shapes", "laya_pool_bytes", "laya_destroy",
-    "laya_last_error", "laya_set_launch_options", "laya_op_gemm", "laya_op_gemm_ln", "laya_interleave_geglu", "laya_op_attention", "laya_op_attention_gathered",
+    "laya_last_error", "laya_set_launch_options", "laya_current_device", "laya_op_gemm", "laya_op_gemm_ln", "laya_interleave_geglu", "laya_op_attention", "laya_op_attention_gathered",
     "laya_attention_tiles", "laya_op_embed_norm", "laya_op_head_tail", "laya_op_norm", "laya_op_gemm_residual_static",
     "laya_mx8_scale_bytes", "laya_op_mx8_quantize", "laya_op_mx8_dequantize", "laya_op_rms_norm_mx8", "laya_op_mx8_linear",
 )
@@ -101,6 +101,7 @@ def load():
         "laya_destroy": (i, [p]),
         "laya_last_error": (ct.c_char_p, [p]),
         "laya_set_launch_options": (i, [i, ct.c_uint64]),
+        "laya_current_device": (i, [ct.POINTER(i)]),
         "laya_op_gemm": (i, [i, i, p, p, i, i, i, p, i, p, i, p, i, p, i, p, i, i, p, p]),
         "laya_op_gemm_ln": (i, [i, p, p, i, i, i, p, i, p, p, p, ct.c_float, p, i, p, p]),
         "laya_interleave_geglu": (i, [p, p, i, i]),

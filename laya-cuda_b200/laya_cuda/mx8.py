@@ -6,8 +6,9 @@ An MX8 matrix holds E4M3 values and one power-of-two scale per 32 consecutive va
 csrc/mx8_python.cpp reads (torch itself is not imported); rows must be contiguous, with any row
 stride.
 The caller owns every buffer.  The calls are enqueued on `stream` (a cudaStream_t as an integer;
-0, the default, is the legacy default stream) of the current device, allocate nothing and return
-at once: a tensor used on another stream than the one that wrote it is the caller's to order.
+0, the default, is the legacy default stream) of the current device, where the buffers must be,
+allocate nothing and return at once: a tensor used on another stream than the one that wrote it is
+the caller's to order.
 
     x8 = mx8.Matrix.empty(x, *x.shape)                  # buffers beside x
     mx8.rms_norm(h, weight, x8, residual=r, sum_out=r)  # r += h; x8 = norm(r) in 8 bits
@@ -29,7 +30,8 @@ __all__ = ["Matrix", "dequantize", "linear", "quantize", "rms_norm", "scale_byte
 def _bind():
     lib = _lib.load()
     _mx8.bind(*(ct.cast(getattr(lib, name), ct.c_void_p).value for name in (
-        "laya_op_mx8_quantize", "laya_op_mx8_dequantize", "laya_op_rms_norm_mx8", "laya_op_mx8_linear", "laya_last_error")))
+        "laya_op_mx8_quantize", "laya_op_mx8_dequantize", "laya_op_rms_norm_mx8", "laya_op_mx8_linear", "laya_last_error",
+        "laya_current_device")))
 
 
 _mx8.set_loader(_bind)

@@ -219,3 +219,54 @@ def test_tensors_on_the_host_are_refused():
     torch = pytest.importorskip("torch")
     with pytest.raises(ValueError, match="CUDA"):
         mx8.Matrix.empty(torch.zeros(1), 4, 32)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The extension over functions of the test's own in place of the library's: what would have been launched, as
+    (name, argument structure, stream), with device 0 the current one."""
+    from laya_cuda import _mx8
+    made = []
+
+    def entry(name, structure, *more):
+        def function(args, *rest):
+            kept = structure()
+            ct.memmove(ct.byref(kept), args, ct.sizeof(structure))
+            made.append((name, kept, rest[-1]))
+            return 0
+        return ct.CFUNCTYPE(ct.c_int, ct.c_void_p, *more, ct.c_void_p)(function)
+
+    @ct.CFUNCTYPE(ct.c_int, ct.POINTER(ct.c_int))
+    def current_device(out):
+        out[0] = 0
+        return 0
+
+    functions = (entry("quantize", _lib.Mx8Convert), entry("dequantize", _lib.Mx8Convert), entry("rms_norm", _lib.RmsNormMx8),
+                 entry("linear", _lib.Mx8Linear, ct.c_void_p), ct.CFUNCTYPE(ct.c_char_p, ct.c_void_p)(lambda e: b""), current_device)
+    _mx8.bind(*(ct.cast(f, ct.c_void_p).value for f in functions))
+    yield made
+    mx8._bind()
+
+
+def on(device):
+    """One call of each operator with everything on `device`."""
+    x, m, w = Fake((4, 32), device=device), matrix(4, 32, device), matrix(8, 32, device)
+    return (lambda: mx8.quantize(x, m), lambda: mx8.dequantize(m, x), lambda: mx8.rms_norm(x, Fake((32,), device=device), m),
+            lambda: mx8.linear(m, w, Fake((4, 8), device=device)))
+
+
+def test_buffers_on_another_device_than_the_current_one_are_refused(calls):
+    for call in on(1):
+        with pytest.raises(ValueError, match="on CUDA device 1, the current device is 0"):
+            call()
+    assert not calls
+    for call in on(0):
+        call()
+    assert [name for name, _, _ in calls] == ["quantize", "dequantize", "rms_norm", "linear"]
+
+
+def test_current_device(lib):
+    device = ct.c_int(7)
+    code = lib.laya_current_device(ct.byref(device))
+    assert (code == 0 and device.value >= 0) or (code == _lib.ERR_NO_DEVICE and device.value == -1)
+    assert lib.laya_current_device(None) == _lib.ERR_INVALID
