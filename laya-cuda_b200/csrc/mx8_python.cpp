@@ -285,15 +285,20 @@ struct Matrix {
   PyObject_HEAD
   PyObject* values;
   PyObject* scales;
-  int rows, cols, device;
-  long long ld;
-  unsigned long long values_ptr, scales_ptr;
+  int rows, cols;
+};
+
+// Where a matrix's buffers are.  Looked at anew by each call (0.1 us): a tensor's storage can be moved or resized
+// after a Matrix of it was made.
+struct Operand {
+  void *values, *scales;
+  long long ld;  // bytes from one row of values to the next
+  int device;
 };
 
 PyTypeObject MatrixType = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
-// Fills `m` (without references) from its arguments.
-bool matrix_check(Matrix* m, PyObject* values, PyObject* scales, int rows, int cols) {
+bool look(PyObject* values, PyObject* scales, int rows, int cols, Operand* m) {
   if (rows < 0 || cols < 1) {
     PyErr_Format(PyExc_ValueError, "bad shape %d x %d: rows may be 0, columns may not", rows, cols);
     return false;
@@ -318,27 +323,26 @@ bool matrix_check(Matrix* m, PyObject* values, PyObject* scales, int rows, int c
     PyErr_SetString(PyExc_ValueError, "values and scales must be on the same CUDA device");
     return false;
   }
-  m->rows = rows;
-  m->cols = cols;
   m->device = v.device;
-  m->values_ptr = reinterpret_cast<unsigned long long>(v.data);
-  m->scales_ptr = reinterpret_cast<unsigned long long>(s.data);
+  m->values = v.data;
+  m->scales = s.data;
   return true;
 }
+bool look(const Matrix* m, Operand* out) { return look(m->values, m->scales, m->rows, m->cols, out); }
 
 PyObject* matrix_make(PyTypeObject* type, PyObject* (&given)[4]) {
   int rows, cols;
   if (!to_int(given[2], "rows", &rows) || !to_int(given[3], "cols", &cols)) return nullptr;
-  Matrix filled;
-  if (!matrix_check(&filled, given[0], given[1], rows, cols)) return nullptr;
+  Operand checked;
+  if (!look(given[0], given[1], rows, cols, &checked)) return nullptr;
   Matrix* m = reinterpret_cast<Matrix*>(type->tp_alloc(type, 0));
   if (!m) return nullptr;
   Py_INCREF(given[0]);
   Py_INCREF(given[1]);
   m->values = given[0];
   m->scales = given[1];
-  m->rows = filled.rows; m->cols = filled.cols; m->device = filled.device; m->ld = filled.ld;
-  m->values_ptr = filled.values_ptr; m->scales_ptr = filled.scales_ptr;
+  m->rows = rows;
+  m->cols = cols;
   return reinterpret_cast<PyObject*>(m);
 }
 
@@ -395,9 +399,19 @@ PyMemberDef matrix_members[] = {
     {"scales", T_OBJECT_EX, offsetof(Matrix, scales), READONLY, nullptr},
     {"rows", T_INT, offsetof(Matrix, rows), READONLY, nullptr},
     {"cols", T_INT, offsetof(Matrix, cols), READONLY, nullptr},
-    {"ld", T_LONGLONG, offsetof(Matrix, ld), READONLY, "bytes from one row of values to the next"},
-    {"device", T_INT, offsetof(Matrix, device), READONLY, "index of the CUDA device"},
     {nullptr, 0, 0, 0, nullptr}};
+
+PyObject* matrix_ld(PyObject* self, void*) {
+  Operand m;
+  return look(reinterpret_cast<Matrix*>(self), &m) ? PyLong_FromLongLong(m.ld) : nullptr;
+}
+PyObject* matrix_device(PyObject* self, void*) {
+  Operand m;
+  return look(reinterpret_cast<Matrix*>(self), &m) ? PyLong_FromLong(m.device) : nullptr;
+}
+PyGetSetDef matrix_getset[] = {{"ld", matrix_ld, nullptr, "bytes from one row of values to the next", nullptr},
+                               {"device", matrix_device, nullptr, "index of the CUDA device", nullptr},
+                               {nullptr, nullptr, nullptr, nullptr, nullptr}};
 
 PyMethodDef matrix_methods[] = {
     {"empty", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(matrix_empty)), METH_FASTCALL | METH_KEYWORDS | METH_CLASS,
@@ -453,12 +467,14 @@ bool take_vector(const char* name, PyObject* t, int n, int device, const float**
   return true;
 }
 
-Matrix* take_matrix(const char* name, PyObject* o) {
+// A Matrix and where its buffers are now; null with an exception set where it is none or they no longer hold it.
+const Matrix* take_matrix(const char* name, PyObject* o, Operand* at) {
   if (Py_TYPE(o) != &MatrixType) {
     PyErr_Format(PyExc_TypeError, "%s must be a Matrix, not %s", name, Py_TYPE(o)->tp_name);
     return nullptr;
   }
-  return reinterpret_cast<Matrix*>(o);
+  const Matrix* m = reinterpret_cast<const Matrix*>(o);
+  return look(m, at) ? m : nullptr;
 }
 
 bool ready() {
@@ -496,13 +512,16 @@ PyObject* finish(int status) {
 // ---------------------------------------------------------------------------------------------
 // Operators
 // ---------------------------------------------------------------------------------------------
-PyObject* convert(const char* tensor, Matrix* m, PyObject* t, PyObject* stream, ConvertFn Library::*call) {
+PyObject* convert(const char* tensor, const char* matrix, PyObject* o, PyObject* t, PyObject* stream, ConvertFn Library::*call) {
+  Operand at;
+  const Matrix* m = take_matrix(matrix, o, &at);
+  if (!m) return nullptr;
   Rows data;
   void* st;
-  if (!take_rows(tensor, t, m->rows, m->cols, m->device, &data) || !to_stream(stream, &st) || !ready_on(m->device, m->rows)) return nullptr;
+  if (!take_rows(tensor, t, m->rows, m->cols, at.device, &data) || !to_stream(stream, &st) || !ready_on(at.device, m->rows)) return nullptr;
   laya_mx8_convert a{};
   a.rows = m->rows; a.cols = m->cols; a.dtype = data.dtype;
-  a.values = reinterpret_cast<void*>(m->values_ptr); a.scales = reinterpret_cast<void*>(m->scales_ptr); a.ldv = m->ld;
+  a.values = at.values; a.scales = at.scales; a.ldv = at.ld;
   a.data = data.ptr; a.ld = data.ld;
   int status;
   Py_BEGIN_ALLOW_THREADS
@@ -517,35 +536,34 @@ Signature<3> g_dequantize_args = {"dequantize", {"x", "out", "stream"}, {}};
 PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
   PyObject* g[3] = {};
   if (!parse(g_quantize_args, 2, args, nargs, kwnames, g)) return nullptr;
-  Matrix* m = take_matrix("out", g[1]);
-  return m ? convert("x", m, g[0], g[2], &Library::quantize) : nullptr;
+  return convert("x", "out", g[1], g[0], g[2], &Library::quantize);
 }
 
 PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
   PyObject* g[3] = {};
   if (!parse(g_dequantize_args, 2, args, nargs, kwnames, g)) return nullptr;
-  Matrix* m = take_matrix("x", g[0]);
-  return m ? convert("out", m, g[1], g[2], &Library::dequantize) : nullptr;
+  return convert("out", "x", g[0], g[1], g[2], &Library::dequantize);
 }
 
 PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
   static Signature<7> sig = {"rms_norm", {"x", "weight", "out", "residual", "sum_out", "eps", "stream"}, {}};
   PyObject* g[7] = {};
   if (!parse(sig, 3, args, nargs, kwnames, g)) return nullptr;
-  Matrix* m = take_matrix("out", g[2]);
+  Operand at;
+  const Matrix* m = take_matrix("out", g[2], &at);
   if (!m) return nullptr;
   laya_rms_norm_mx8 a{};
   Rows x, r = {}, s = {};
   void* st;
-  if (!take_rows("x", g[0], m->rows, m->cols, m->device, &x)) return nullptr;
+  if (!take_rows("x", g[0], m->rows, m->cols, at.device, &x)) return nullptr;
   a.residual_dtype = x.dtype;
   const bool residual = g[3] && g[3] != Py_None, sum = g[4] && g[4] != Py_None;
   if (residual) {
-    if (!take_rows("residual", g[3], m->rows, m->cols, m->device, &r)) return nullptr;
+    if (!take_rows("residual", g[3], m->rows, m->cols, at.device, &r)) return nullptr;
     a.residual_dtype = r.dtype;
   }
   if (sum) {
-    if (!take_rows("sum_out", g[4], m->rows, m->cols, m->device, &s)) return nullptr;
+    if (!take_rows("sum_out", g[4], m->rows, m->cols, at.device, &s)) return nullptr;
     if (residual && s.dtype != r.dtype) {
       PyErr_SetString(PyExc_ValueError, "sum_out must have the residual's type");
       return nullptr;
@@ -556,17 +574,17 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject*
     PyErr_SetString(PyExc_ValueError, "weight must be a tensor");
     return nullptr;
   }
-  if (!take_vector("weight", g[1], m->cols, m->device, &a.weight)) return nullptr;
+  if (!take_vector("weight", g[1], m->cols, at.device, &a.weight)) return nullptr;
   a.eps = 1e-6f;
   if (g[5]) {
     const double eps = PyFloat_AsDouble(g[5]);
     if (eps == -1.0 && PyErr_Occurred()) return nullptr;
     a.eps = (float)eps;
   }
-  if (!to_stream(g[6], &st) || !ready_on(m->device, m->rows)) return nullptr;
+  if (!to_stream(g[6], &st) || !ready_on(at.device, m->rows)) return nullptr;
   a.rows = m->rows; a.cols = m->cols; a.dtype = x.dtype;
   a.x = x.ptr; a.ldx = x.ld; a.residual = r.ptr; a.ldr = r.ld; a.sum_out = s.ptr; a.lds = s.ld;
-  a.values = reinterpret_cast<void*>(m->values_ptr); a.scales = reinterpret_cast<void*>(m->scales_ptr); a.ldv = m->ld;
+  a.values = at.values; a.scales = at.scales; a.ldv = at.ld;
   int status;
   Py_BEGIN_ALLOW_THREADS
   status = g_lib.rms_norm(&a, st);
@@ -590,27 +608,29 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* k
   static Signature<10> sig = {"linear", {"x", "w", "out", "bias", "gate", "gate_bias", "activation", "residual", "err", "stream"}, {}};
   PyObject* g[10] = {};
   if (!parse(sig, 3, args, nargs, kwnames, g)) return nullptr;
-  Matrix *x = take_matrix("x", g[0]), *w = x ? take_matrix("w", g[1]) : nullptr;
+  Operand x_at, w_at;
+  const Matrix *x = take_matrix("x", g[0], &x_at), *w = x ? take_matrix("w", g[1], &w_at) : nullptr;
   if (!w) return nullptr;
-  const int rows = x->rows, cols = x->cols, n = w->rows, device = x->device;
-  if (w->cols != cols || w->device != device) {
-    PyErr_Format(PyExc_ValueError, "w is %d x %d on device %d, x has %d columns on device %d", n, w->cols, w->device, cols, device);
+  const int rows = x->rows, cols = x->cols, n = w->rows, device = x_at.device;
+  if (w->cols != cols || w_at.device != device) {
+    PyErr_Format(PyExc_ValueError, "w is %d x %d on device %d, x has %d columns on device %d", n, w->cols, w_at.device, cols, device);
     return nullptr;
   }
   laya_mx8_linear a{};
   a.rows = rows; a.features = n; a.cols = cols;
   a.activation = activation(g[6]);
   if (a.activation < 0) return nullptr;
-  a.x = reinterpret_cast<void*>(x->values_ptr); a.x_scales = reinterpret_cast<void*>(x->scales_ptr); a.ldx = x->ld;
-  a.w = reinterpret_cast<void*>(w->values_ptr); a.w_scales = reinterpret_cast<void*>(w->scales_ptr); a.ldw = w->ld;
+  a.x = x_at.values; a.x_scales = x_at.scales; a.ldx = x_at.ld;
+  a.w = w_at.values; a.w_scales = w_at.scales; a.ldw = w_at.ld;
   if (g[4] && g[4] != Py_None) {
-    Matrix* gate = take_matrix("gate", g[4]);
+    Operand at;
+    const Matrix* gate = take_matrix("gate", g[4], &at);
     if (!gate) return nullptr;
-    if (gate->rows != n || gate->cols != cols || gate->device != device) {
+    if (gate->rows != n || gate->cols != cols || at.device != device) {
       PyErr_Format(PyExc_ValueError, "gate is %d x %d, w %d x %d", gate->rows, gate->cols, n, cols);
       return nullptr;
     }
-    a.gate = reinterpret_cast<void*>(gate->values_ptr); a.gate_scales = reinterpret_cast<void*>(gate->scales_ptr); a.ldg = gate->ld;
+    a.gate = at.values; a.gate_scales = at.scales; a.ldg = at.ld;
   }
   if (!take_vector("bias", g[3], n, device, &a.bias) || !take_vector("gate_bias", g[5], n, device, &a.gate_bias)) return nullptr;
   Rows t;
@@ -619,12 +639,14 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* k
     a.residual = t.ptr; a.ldr = t.ld; a.residual_dtype = t.dtype;
   }
   if (Py_TYPE(g[2]) == &MatrixType) {
-    Matrix* out = reinterpret_cast<Matrix*>(g[2]);
-    if (out->rows != rows || out->cols != n || out->device != device) {
+    Operand at;
+    const Matrix* out = take_matrix("out", g[2], &at);
+    if (!out) return nullptr;
+    if (out->rows != rows || out->cols != n || at.device != device) {
       PyErr_Format(PyExc_ValueError, "out is %d x %d, the result %d x %d", out->rows, out->cols, rows, n);
       return nullptr;
     }
-    a.out = reinterpret_cast<void*>(out->values_ptr); a.out_scales = reinterpret_cast<void*>(out->scales_ptr); a.ldo = out->ld;
+    a.out = at.values; a.out_scales = at.scales; a.ldo = at.ld;
     a.out_dtype = LAYA_DTYPE_MX8;
   } else {
     if (!take_rows("out", g[2], rows, n, device, &t)) return nullptr;
@@ -710,10 +732,11 @@ PyMODINIT_FUNC PyInit__mx8() {
       "An MX8 matrix [rows][cols]: `values`, bytes in `rows` rows of cols rounded up to a multiple of\n"
       "16, and `scales`, `scale_bytes(rows, cols)` bytes.  Both are contiguous, of any type of that many\n"
       "bytes; two-dimensional values of one-byte elements may have a larger row stride.  Holds\n"
-      "references to both buffers.";
+      "references to both tensors; each call looks anew at where their storage is.";
   MatrixType.tp_dealloc = matrix_dealloc;
   MatrixType.tp_vectorcall = matrix_call;
   MatrixType.tp_members = matrix_members;
+  MatrixType.tp_getset = matrix_getset;
   MatrixType.tp_methods = matrix_methods;
   if (PyType_Ready(&MatrixType) < 0) return nullptr;
   PyObject* m = PyModule_Create(&module);

@@ -270,3 +270,37 @@ def test_current_device(lib):
     code = lib.laya_current_device(ct.byref(device))
     assert (code == 0 and device.value >= 0) or (code == _lib.ERR_NO_DEVICE and device.value == -1)
     assert lib.laya_current_device(None) == _lib.ERR_INVALID
+
+
+def test_a_matrix_is_where_its_buffers_are_now(calls):
+    """Storage that moved, went to the host or shrank after a Matrix of it was made."""
+    m, w = matrix(4, 32), matrix(8, 32)
+    m.values.ptr, m.scales.ptr, w.values.ptr, w.scales.ptr = 0x21000, 0x22000, 0x23000, 0x24000
+    x, y = Fake((4, 32)), Fake((4, 8))
+    mx8.quantize(x, m), mx8.dequantize(m, x), mx8.rms_norm(x, Fake((32,)), m), mx8.linear(m, w, y, gate=w)
+    for _, a, _ in calls[:3]:
+        assert (a.values, a.scales, a.ldv) == (0x21000, 0x22000, 32)
+    a = calls[3][1]
+    assert (a.x, a.x_scales, a.w, a.w_scales, a.gate, a.gate_scales) == (0x21000, 0x22000, 0x23000, 0x24000, 0x23000, 0x24000)
+    del calls[:]
+    m.values.strides = (80, 1)
+    assert m.ld == 80
+    mx8.quantize(x, m)
+    assert calls[0][1].ldv == 80
+    del calls[:]
+    for change, word in ((dict(device=-1), "CUDA device"), (dict(device=1), "device"), (dict(shape=(3, 32)), "bytes"),
+                         (dict(strides=(32, 2)), "bytes")):
+        broken = matrix(4, 32)
+        for name, value in change.items():
+            setattr(broken.values, name, value)
+        for call in (lambda: mx8.quantize(x, broken), lambda: mx8.dequantize(broken, x), lambda: mx8.rms_norm(x, Fake((32,)), broken),
+                     lambda: mx8.linear(broken, w, y), lambda: mx8.linear(m, broken, Fake((4, 4))),
+                     lambda: mx8.linear(m, w, y, gate=broken), lambda: mx8.linear(m, matrix(32, 32), broken), lambda: broken.ld):
+            with pytest.raises(ValueError, match=word):
+                call()
+    small = matrix(4, 32)
+    small.scales.shape = (511,)
+    small.scales.strides = (1,)
+    with pytest.raises(ValueError, match="scales"):
+        mx8.quantize(x, small)
+    assert not calls

@@ -710,3 +710,20 @@ def test_the_feed_forward_example(capsys):
     mx8.linear(n8, block.up, a8, gate=block.gate, activation="silu")
     mx8.linear(a8, block.down, want, residual=total)
     assert torch.equal(got, want)
+
+
+def test_a_matrix_follows_its_buffers_storage():
+    """Weights whose storage is replaced after the Matrix was made: the product is with what the tensors hold now."""
+    rng = np.random.default_rng(16)
+    x, _ = matrix(activations(rng, 40, 160))
+    w, _ = matrix(rng.normal(0, 0.1, (96, 160)).astype(np.float32))
+    want, got = torch.empty(40, 96, device="cuda"), torch.empty(40, 96, device="cuda")
+    mx8.linear(x, w, want)
+    kept = w.values.data, w.scales.data
+    w.values.data, w.scales.data = w.values.data.clone(), w.scales.data.clone()
+    kept[0].zero_(), kept[1].zero_()
+    mx8.linear(x, w, got)
+    assert torch.equal(got, want) and bool(want.any())
+    w.values.data = w.values.data.cpu()
+    with pytest.raises(ValueError, match="CUDA"):
+        mx8.linear(x, w, got)
