@@ -26,7 +26,8 @@ constexpr int kMxTileRows = 128;
 constexpr int kMxTileCols = 128;
 constexpr int kMxTileBytes = 512;
 
-__host__ __device__ inline int mx_col_tiles(int cols) { return (cols + kMxTileCols - 1) / kMxTileCols; }
+// cols at least 1 and up to 2^31 - 1 (the sum of cols and a tile would wrap).
+__host__ __device__ inline int mx_col_tiles(int cols) { return (cols - 1) / kMxTileCols + 1; }
 
 __host__ __device__ inline size_t mx_scale_tile(int row, int col_tile, int col_tiles) {
   return ((size_t)(row / kMxTileRows) * col_tiles + col_tile) * kMxTileBytes;
@@ -289,8 +290,9 @@ struct FastDiv {
 };
 
 // Writes a piece as MX8.  Two neighbouring threads hold a block and eight a scale tile's 128 columns;
-// all 32 threads of the warp call this together, with zeros in columns past the last.
-__device__ __forceinline__ void mx_store_piece(const float (&v)[kMxPiece], int row, int col, int cols, int col_tiles, bool live,
+// all 32 threads of the warp call this together, with zeros in columns past the last.  `col` may be past the last
+// column, and past 2^31 with it.
+__device__ __forceinline__ void mx_store_piece(const float (&v)[kMxPiece], int row, uint32_t col, int cols, int col_tiles, bool live,
                                                uint8_t* q, int64_t ldq, uint8_t* scales) {
   float most = 0.f;
 #pragma unroll
@@ -302,14 +304,15 @@ __device__ __forceinline__ void mx_store_piece(const float (&v)[kMxPiece], int r
   uint32_t word = byte << (4 * (lane & 6));
   word |= __shfl_xor_sync(0xffffffffu, word, 2);
   word |= __shfl_xor_sync(0xffffffffu, word, 4);
-  if (!live || col >= col_tiles * kMxTileCols) return;
-  if (col < cols) {
+  const uint32_t col_tile = col / kMxTileCols;
+  if (!live || col_tile >= (uint32_t)col_tiles) return;
+  if (col < (uint32_t)cols) {
     const float inverse = mx_inverse(byte);
     *reinterpret_cast<uint4*>(q + (size_t)row * ldq + col) =
         make_uint4(mx_pack4(v, inverse), mx_pack4(v + 4, inverse), mx_pack4(v + 8, inverse), mx_pack4(v + 12, inverse));
   }
   if ((lane & 7) == 0)
-    *reinterpret_cast<uint32_t*>(scales + mx_scale_tile(row, col / kMxTileCols, col_tiles) + mx_scale_row(row)) = word;
+    *reinterpret_cast<uint32_t*>(scales + mx_scale_tile(row, (int)col_tile, col_tiles) + mx_scale_row(row)) = word;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -517,8 +520,9 @@ __global__ void __launch_bounds__(kMxThreads) rms_norm_mx8_long_kernel(const Rms
     const T* x = static_cast<const T*>(a.x) + (size_t)row * a.ldx;
     const R* r = a.residual ? static_cast<const R*>(a.residual) + (size_t)row * a.ldr : nullptr;
     R* s = a.sum_out ? static_cast<R*>(a.sum_out) + (size_t)row * a.lds : nullptr;
-    auto load = [&](int col, float (&h)[kMxPiece]) {
-      const int n = a.cols - col;
+    const uint32_t cols = (uint32_t)a.cols;  // columns step past 2^31
+    auto load = [&](uint32_t col, float (&h)[kMxPiece]) {
+      const int n = (int)(cols - col);
       load_any(x + col, n, h);
       if (r) {
         float t[kMxPiece];
@@ -528,7 +532,7 @@ __global__ void __launch_bounds__(kMxThreads) rms_norm_mx8_long_kernel(const Rms
       }
     };
     float sq = 0.f;
-    for (int col = threadIdx.x * kMxPiece; col < a.cols; col += kMxThreads * kMxPiece) {
+    for (uint32_t col = threadIdx.x * kMxPiece; col < cols; col += kMxThreads * kMxPiece) {
       float h[kMxPiece];
       load(col, h);
 #pragma unroll
@@ -541,8 +545,9 @@ __global__ void __launch_bounds__(kMxThreads) rms_norm_mx8_long_kernel(const Rms
 #pragma unroll
     for (int w = 0; w < kMxThreads / 32; ++w) sq += part[w];
     const float inv = rsqrtf(sq / (float)a.cols + a.eps);
-    for (int col0 = (threadIdx.x & ~31) * kMxPiece; col0 < a.cols; col0 += kMxThreads * kMxPiece) {  // whole warps
-      const int col = col0 + (threadIdx.x & 31) * kMxPiece, n = a.cols - col;
+    for (uint32_t col0 = (threadIdx.x & ~31) * kMxPiece; col0 < cols; col0 += kMxThreads * kMxPiece) {  // whole warps
+      const uint32_t col = col0 + (threadIdx.x & 31) * kMxPiece;
+      const int n = (int)(cols - col);
       float h[kMxPiece];
       load(col, h);
       if (s) {

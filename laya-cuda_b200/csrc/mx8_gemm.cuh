@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kMxThreadsPair, 1)
 
   const int m_blocks = (args.M + 255) / 256;
   const int n_blocks = (args.N + kOutCols - 1) / kOutCols;
-  const int k_blocks = (args.K + kMxBK - 1) / kMxBK;
+  const int k_blocks = mx_col_tiles(args.K);
   const int tiles = m_blocks * n_blocks;
 
   if (threadIdx.x == 0) {
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kMxThreadsFew, kGated ? 1 : 2)
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int split = (int)gridDim.z, rank = (int)cluster_rank();
   const int f0 = blockIdx.x * 128, t0 = blockIdx.y * BN;
-  const int k_tiles = (args.K + kMxBK - 1) / kMxBK;
+  const int k_tiles = mx_col_tiles(args.K);
   const int kb0 = (int)((int64_t)k_tiles * rank / split), kb1 = (int)((int64_t)k_tiles * (rank + 1) / split);
   const int k_blocks = kb1 - kb0;  // at least 1: split <= k_tiles
   const int issuers = kGated || k_blocks > 1 ? 2 : 1;

@@ -304,3 +304,10 @@ def test_a_matrix_is_where_its_buffers_are_now(calls):
     with pytest.raises(ValueError, match="scales"):
         mx8.quantize(x, small)
     assert not calls
+
+
+@pytest.mark.parametrize("name", ["laya_op_mx8_quantize", "laya_op_mx8_dequantize"])
+@pytest.mark.parametrize("cols", [2 ** 31 - 128, 2 ** 31 - 127, 2 ** 31 - 1])
+def test_conversions_refuse_too_many_values_in_the_widest_rows(lib, name, cols):
+    with pytest.raises(ValueError, match="too many"):
+        _lib.check(getattr(lib, name)(ct.byref(convert(rows=200, cols=cols, ld=cols, ldv=2 ** 31)), None))

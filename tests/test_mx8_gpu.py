@@ -727,3 +727,33 @@ def test_a_matrix_follows_its_buffers_storage():
     w.values.data = w.values.data.cpu()
     with pytest.raises(ValueError, match="CUDA"):
         mx8.linear(x, w, got)
+
+
+def test_the_widest_row():
+    """2^31 - 1 columns: the last tiles' index arithmetic.  The row repeats, so each block of it is compared with a short row's."""
+    cols, part = 2 ** 31 - 1, 2 ** 16
+    g = torch.Generator(device="cuda").manual_seed(17)
+    base = torch.randint(0, 2, (part,), generator=g, device="cuda").mul_(2).sub_(1).bfloat16()
+    x = base.repeat(2 ** 31 // part)[:cols].view(1, cols)
+    q = torch.full((1, 2 ** 31), 0xA5, dtype=torch.uint8, device="cuda")
+    s = torch.full((mx8.scale_bytes(1, cols),), 0xA5, dtype=torch.uint8, device="cuda")
+    wide, short = mx8.Matrix(q, s, 1, cols), fresh(1, part)
+    mx8.quantize(base.view(1, part), short)
+
+    def check():
+        rows = q.view(-1, part)
+        assert bool((rows[:-1] == short.values).all())
+        assert torch.equal(rows[-1, :-1], short.values[0, :-1]) and int(rows[-1, -1]) == 0
+        tiles = s.view(-1, 512)
+        assert bool((tiles[:, :4] == short.scales.view(-1, 512)[0, :4]).all()) and bool((tiles[:, 4:] == 0xA5).all())
+
+    mx8.quantize(x, wide)
+    check()
+    back = torch.full((1, cols), 7.0, dtype=torch.bfloat16, device="cuda")
+    mx8.dequantize(wide, back)
+    assert torch.equal(back, x)
+    q.fill_(0xA5), s.fill_(0xA5)
+    # The mean of 2^31 - 1 ones is 1 in fp32, sums of up to 2^23 of them are exact, and so is y = x.
+    mx8.rms_norm(x, torch.ones(cols, device="cuda"), wide, sum_out=back.zero_(), eps=0.0)
+    check()
+    assert torch.equal(back, x)
