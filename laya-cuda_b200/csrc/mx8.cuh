@@ -439,22 +439,23 @@ __global__ void __launch_bounds__(512) rms_norm_mx8_kernel(const RmsNormArgs a) 
   }
   Raw<T> rx[kVec ? CH : 1];
   Raw<R> rr[kVec ? CH : 1];
-  auto fetch = [&](int row) {
+  const uint32_t rows = (uint32_t)a.rows;  // rows step past 2^31
+  auto fetch = [&](uint32_t row) {
     if constexpr (kVec) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        const bool in = row < a.rows && col[c] < a.cols;
+        const bool in = row < rows && col[c] < a.cols;
         rx[c] = load_raw(x + (size_t)row * a.ldx + col[c], in);
         rr[c] = load_raw(r + (size_t)row * a.ldr + col[c], in && r);
       }
     }
   };
-  const int step = gridDim.x * per_block;
+  const uint32_t step = gridDim.x * per_block;
   int turn = 0;
-  int row = blockIdx.x * per_block + sub;
+  uint32_t row = blockIdx.x * per_block + sub;
   fetch(row);
-  for (int row0 = blockIdx.x * per_block; row0 < a.rows; row0 += step, row += step, turn ^= 1) {
-    const bool live = row < a.rows;
+  for (uint32_t row0 = blockIdx.x * per_block; row0 < rows; row0 += step, row += step, turn ^= 1) {
+    const bool live = row < rows;
     float h[CH][kMxPiece];
     float2 sq2 = make_float2(0.f, 0.f);
 #pragma unroll
@@ -503,7 +504,7 @@ __global__ void __launch_bounds__(512) rms_norm_mx8_kernel(const RmsNormArgs a) 
         h[c][i] = col[c] + (kVec ? 0 : i) < a.cols ? f.x : 0.f;
         h[c][i + 1] = col[c] + (kVec ? 0 : i + 1) < a.cols ? f.y : 0.f;
       }
-      mx_store_piece(h[c], row, col[c], a.cols, col_tiles, live, a.q, a.ldq, a.scales);
+      mx_store_piece(h[c], (int)row, col[c], a.cols, col_tiles, live, a.q, a.ldq, a.scales);
     }
   }
 }
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(kMxThreads) rms_norm_mx8_long_kernel(const Rms
   __shared__ float part[kMxThreads / 32];
   __shared__ __align__(16) R stage[kMxThreads / 32][32 * kMxPiece];
   const int col_tiles = mx_col_tiles(a.cols);
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  for (uint32_t row = blockIdx.x; row < (uint32_t)a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + (size_t)row * a.ldx;
     const R* r = a.residual ? static_cast<const R*>(a.residual) + (size_t)row * a.ldr : nullptr;
     R* s = a.sum_out ? static_cast<R*>(a.sum_out) + (size_t)row * a.lds : nullptr;
@@ -556,7 +557,7 @@ __global__ void __launch_bounds__(kMxThreads) rms_norm_mx8_long_kernel(const Rms
       }
 #pragma unroll
       for (int i = 0; i < kMxPiece; ++i) h[i] = i < n ? h[i] * inv * a.weight[col + i] : 0.f;
-      mx_store_piece(h, row, col, a.cols, col_tiles, true, a.q, a.ldq, a.scales);
+      mx_store_piece(h, (int)row, col, a.cols, col_tiles, true, a.q, a.ldq, a.scales);
     }
     __syncthreads();
   }

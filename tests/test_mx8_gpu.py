@@ -729,7 +729,14 @@ def test_a_matrix_follows_its_buffers_storage():
         mx8.linear(x, w, got)
 
 
-def test_the_widest_row():
+@pytest.fixture
+def large():
+    """For tests of tens of GB: what they held goes back to the device, for tests that allocate without torch."""
+    yield
+    torch.cuda.empty_cache()
+
+
+def test_the_widest_row(large):
     """2^31 - 1 columns: the last tiles' index arithmetic.  The row repeats, so each block of it is compared with a short row's."""
     cols, part = 2 ** 31 - 1, 2 ** 16
     g = torch.Generator(device="cuda").manual_seed(17)
@@ -757,3 +764,24 @@ def test_the_widest_row():
     mx8.rms_norm(x, torch.ones(cols, device="cuda"), wide, sum_out=back.zero_(), eps=0.0)
     check()
     assert torch.equal(back, x)
+
+
+@pytest.mark.parametrize("rows,cols", [(2 ** 31 - 1, 1), (2 ** 31 - 2 ** 15, 2)])
+def test_rms_norm_of_the_most_rows(large, rows, cols):
+    """Rows whose loop steps past 2^31: the kernels' row indices wrap there if they are signed."""
+    room = 16
+    sign = torch.randint(0, 2, (2 ** 16 * cols,), generator=torch.Generator(device="cuda").manual_seed(18), device="cuda").mul_(2).sub_(1)
+    x = sign.half().view(-1, cols).repeat(2 ** 15, 1)[:rows]
+    total = torch.zeros(rows, cols, dtype=torch.float16, device="cuda")
+    q = torch.full((rows, room), 0xA5, dtype=torch.uint8, device="cuda")
+    s = torch.full((mx8.scale_bytes(rows, cols),), 0xA5, dtype=torch.uint8, device="cuda")
+    mx8.rms_norm(x, torch.ones(cols, device="cuda"), mx8.Matrix(q, s, rows, cols), sum_out=total, eps=0.0)
+    assert torch.equal(total, x)
+    # Signs over a mean square of 1: 256 in E4M3 under the scale 2^-8.
+    for c in range(cols):
+        assert bool((q[:, c] == torch.where(x[:, c] > 0, 0x78, 0xF8)).all())
+    assert not bool(q[:, cols:].any())
+    words = s.view(torch.int32)
+    words = words.view(-1, 32, 4).transpose(1, 2).reshape(-1)  # by row
+    assert bool((words[:rows] == 119).all())
+    assert bool((words[rows:] == -0x5A5A5A5B).all())
