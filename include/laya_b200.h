@@ -365,9 +365,9 @@ typedef struct laya_mx8_linear {
 } laya_mx8_linear;
 
 /* out = act(x w^T + bias) + residual, or, gated, act(x gate^T + gate_bias) * (x w^T + bias) +
- * residual.  Sums in fp32, rounded once to out_dtype.  The result is the same each time.  err (zero
- * on entry, or NULL) receives a device error: a pipeline wait that ran out, after which out is
- * undefined. */
+ * residual.  rows and features: at most 2^31 - 256.  Sums in fp32, rounded once to out_dtype.  The
+ * result is the same each time.  err (zero on entry, or NULL) receives a device error: a pipeline
+ * wait that ran out, after which out is undefined. */
 int laya_op_mx8_linear(const laya_mx8_linear* args, int* err, void* stream);
 
 #ifdef __cplusplus

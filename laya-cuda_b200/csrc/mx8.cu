@@ -391,6 +391,9 @@ int laya_op_mx8_linear(const laya_mx8_linear* p, int* err, void* stream) {
   const int M = p->rows, N = p->features, K = p->cols;
   check_shape(M, N);
   if (K < 1) fail(LAYA_ERR_INVALID, "bad depth %d", K);
+  // A tile's rows and columns are counted in 32 bits past the result's last ones.
+  constexpr int kMost = INT32_MAX - 255;
+  if (M > kMost || N > kMost) fail(LAYA_ERR_INVALID, "result of %d x %d: rows and features may be at most %d", M, N, kMost);
   if (p->activation < LAYA_ACT_NONE || p->activation > LAYA_ACT_SILU) fail(LAYA_ERR_INVALID, "unknown activation %d", p->activation);
   if (p->out_dtype != LAYA_DTYPE_MX8) dtype_size(p->out_dtype);
   if (p->residual) dtype_size(p->residual_dtype);

@@ -311,3 +311,9 @@ def test_a_matrix_is_where_its_buffers_are_now(calls):
 def test_conversions_refuse_too_many_values_in_the_widest_rows(lib, name, cols):
     with pytest.raises(ValueError, match="too many"):
         _lib.check(getattr(lib, name)(ct.byref(convert(rows=200, cols=cols, ld=cols, ldv=2 ** 31)), None))
+
+
+@pytest.mark.parametrize("rows,features", [(2 ** 31 - 255, 1), (2 ** 31 - 1, 1), (1, 2 ** 31 - 255), (300, 2 ** 31 - 1)])
+def test_linear_refuses_results_whose_tiles_pass_32_bits(lib, rows, features):
+    with pytest.raises(ValueError, match="at most 2147483392"):
+        _lib.check(lib.laya_op_mx8_linear(ct.byref(linear(rows=rows, features=features, ldo=2 ** 31)), None, None))
