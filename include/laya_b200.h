@@ -312,8 +312,8 @@ int laya_op_gemm_residual_static(int precision, const void* x, const void* w, in
  * ------------------------------------------------------------------------------------------ */
 #define LAYA_ACT_NONE 0
 #define LAYA_ACT_RELU 1
-#define LAYA_ACT_GELU 2  /* exact (erf) */
-#define LAYA_ACT_SILU 3
+#define LAYA_ACT_GELU 2  /* x Phi(x) (erf); fp32, relative error below (25 + 1.5 x^2) 2^-24, 0 below x = -13.2 */
+#define LAYA_ACT_SILU 3  /* x / (1 + exp(-x)); fp32, relative error below (8 + 2 |x|) 2^-24, 0 below x = -87 */
 
 /* Bytes of the scales of an MX8 matrix; -1 for a bad shape (rows >= 0, cols >= 1). */
 int64_t laya_mx8_scale_bytes(int rows, int cols);

@@ -39,6 +39,28 @@ struct MxLinearArgs {
 
 // v / (1 + exp(-v)): the exponential overflows to infinity for v far below zero, the quotient to -0.
 __device__ __forceinline__ float mx_silu(float v) { return v * rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * v)); }
+// x Phi(x) with a small relative error on both sides of zero, as the fp32 results need it (the encoder's gelu_erf2 keeps an
+// absolute one for 16-bit results: it takes 1 - (1 - q) for negative x, which cancels).  With a = |x|,
+//   q = Phi(-a) = exp(-a^2 / 2) t P(t),  t = 1 / (1 + p a),  and  x Phi(x) = x q for x <= 0, x (1 - q) for x > 0.
+// P: the degree-7 polynomial of least relative error (1.0e-7) for 0 <= a <= 14.5, fitted for this function.  With the roundings
+// and the special functions' errors the result is within (25 + 1.5 x^2) 2^-24 of itself, the second term from the
+// exponent's rounding; below x = -13.2 the exponential is 0.
+__device__ __forceinline__ float2 mx_gelu2(float2 x) {
+  auto twice = [](float c) { return make_float2(c, c); };
+  const float2 d = fma2(make_float2(fabsf(x.x), fabsf(x.y)), twice(0.305f), twice(1.0f));
+  const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+  float2 h = fma2(twice(0.03663905f), t, twice(-0.15274677f));
+  h = fma2(h, t, twice(0.18531595f));
+  h = fma2(h, t, twice(-0.037621517f));
+  h = fma2(h, t, twice(0.12084079f));
+  h = fma2(h, t, twice(0.10347359f));
+  h = fma2(h, t, twice(0.1224587f));
+  h = fma2(h, t, twice(0.12164024f));
+  const float2 w = mul2(mul2(x, twice(-0.72134752044448170f)), x);  // -x^2 / 2 in powers of two
+  const float2 q = mul2(mul2(h, t), make_float2(ex2_approx(w.x), ex2_approx(w.y)));
+  const float2 r = fma2(q, twice(-1.0f), twice(1.0f));
+  return mul2(x, make_float2(x.x > 0.f ? r.x : q.x, x.y > 0.f ? r.y : q.y));
+}
 // max(v, 0) that keeps a NaN.
 __device__ __forceinline__ float mx_relu(float v) { return v < 0.f ? 0.f : v; }
 
@@ -153,7 +175,7 @@ __device__ __forceinline__ void mx_finish(const MxLinearArgs& a, int row0, int s
         on[k][i + 1] = y.y;
       }
   };
-  if (a.act == MX_ACT_GELU) apply([](float2 v) { return gelu_erf2(v); });
+  if (a.act == MX_ACT_GELU) apply([](float2 v) { return mx_gelu2(v); });
   else if (a.act == MX_ACT_SILU) apply([](float2 v) { return make_float2(mx_silu(v.x), mx_silu(v.y)); });
   else if (a.act == MX_ACT_RELU) apply([](float2 v) { return make_float2(mx_relu(v.x), mx_relu(v.y)); });
   if (kGated) {
@@ -335,7 +357,7 @@ __device__ __forceinline__ uint32_t mx_finish_row(const MxLinearArgs& a, int row
       on[i + 1] = y.y;
     }
   };
-  if (a.act == MX_ACT_GELU) apply([](float2 x) { return gelu_erf2(x); });
+  if (a.act == MX_ACT_GELU) apply([](float2 x) { return mx_gelu2(x); });
   else if (a.act == MX_ACT_SILU) apply([](float2 x) { return make_float2(mx_silu(x.x), mx_silu(x.y)); });
   else if (a.act == MX_ACT_RELU) apply([](float2 x) { return make_float2(mx_relu(x.x), mx_relu(x.y)); });
   if (kGated) {

@@ -785,3 +785,37 @@ def test_rms_norm_of_the_most_rows(large, rows, cols):
     words = words.view(-1, 32, 4).transpose(1, 2).reshape(-1)  # by row
     assert bool((words[:rows] == 119).all())
     assert bool((words[rows:] == -0x5A5A5A5B).all())
+
+
+# Bounds on an activation's relative error in fp32, in units of 2^-24: what its polynomial's fit, roundings and special
+# functions add up to (the fit 2, ex2 and rcp 4 each, at most 15 for sums and products), and the rounding of the
+# exponential's argument, up to three halves of a unit of it and one e-fold per unit.
+ACTIVATIONS = {
+    "gelu": (13.0, lambda x: 0.5 * x * torch.erfc(-x / math.sqrt(2)), lambda x: 25 + 1.5 * x * x),
+    "silu": (80.0, lambda x: x * torch.sigmoid(x), lambda x: 8 + 2 * x.abs())}
+
+
+@pytest.mark.parametrize("act", list(ACTIVATIONS))
+@pytest.mark.parametrize("rows,gated", [(1, False), (300, False), (2600, False), (3, True), (1200, True)])
+@pytest.mark.parametrize("out_type", ["f32", "f16", "bf16"])
+def test_activations_are_relatively_exact(act, rows, gated, out_type):
+    """Prescribed pre-activations (weights of zeros and a bias): the whole range of x, small results included."""
+    reach, define64, bound = ACTIVATIONS[act]
+    n = 1024
+    at = torch.linspace(-reach, reach, n, device="cuda")
+    at[:6] = torch.tensor([0.0, 1e-30, -1e-30, -1e-4, math.inf, math.nan])
+    zeros = fresh(n, 64)
+    mx8.quantize(torch.zeros(n, 64, device="cuda"), zeros)
+    x, out = fresh(rows, 64), torch.empty(rows, n, dtype=TYPES[out_type], device="cuda")
+    mx8.quantize(torch.ones(rows, 64, device="cuda"), x)
+    if gated:
+        mx8.linear(x, zeros, out, bias=torch.full((n,), 1.5, device="cuda"), gate=zeros, gate_bias=at, activation=act)
+    else:
+        mx8.linear(x, zeros, out, bias=at, activation=act)
+    want = define64(at.double()) * (1.5 if gated else 1)
+    assert bool((out[:, 4] == math.inf).all()) and bool(out[:, 5].isnan().all())
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[4:6] = False
+    off, want, x64 = (out.double() - want).abs()[:, keep], want[keep], at.double()[keep]
+    tol = want.abs() * ((bound(x64) + 1) * 2.0 ** -24 + HALF_ULP[out_type]) + TINY[out_type]
+    assert bool((off <= tol).all()), float((off / tol).max())
