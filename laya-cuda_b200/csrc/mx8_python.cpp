@@ -55,7 +55,7 @@ struct DLExchange {
   void* previous;
   void *allocate, *managed_from_object, *managed_to_object;
   int (*tensor_from_object)(void* object, DLTensor* out);  // no reference is kept, nothing is synchronised; may be null
-  void* current_stream;
+  int (*current_stream)(int32_t device_type, int32_t device_id, void** out);  // may be null
 };
 enum { kDLCuda = 2, kDLCudaManaged = 13, kDLInt = 0, kDLFloat = 2, kDLBfloat = 4 };
 
@@ -121,28 +121,29 @@ void settle(View* v) {
   if (!v->numel) v->contiguous = true;
 }
 
-// The exchange function of a tensor's type; null where it has none.  Types are looked at once (and kept).
-decltype(DLExchange::tensor_from_object) exchange_of(PyTypeObject* type) {
+// The exchange table of a tensor's type (kept as long as its framework is loaded); null where it has none.  Types are
+// looked at once (and kept).
+const DLExchange* exchange_of(PyTypeObject* type) {
   static struct {
     PyTypeObject* type;
-    decltype(DLExchange::tensor_from_object) function;
+    const DLExchange* table;
   } known[16];
   static int count = 0;
   for (int i = 0; i < count; ++i)
-    if (known[i].type == type) return known[i].function;
-  decltype(DLExchange::tensor_from_object) function = nullptr;
+    if (known[i].type == type) return known[i].table;
+  const DLExchange* table = nullptr;
   PyObject* capsule = PyObject_GetAttr(reinterpret_cast<PyObject*>(type), g_names[EXCHANGE]);
   if (capsule && PyCapsule_IsValid(capsule, "dlpack_exchange_api")) {
     const DLExchange* api = static_cast<const DLExchange*>(PyCapsule_GetPointer(capsule, "dlpack_exchange_api"));
-    if (api->major == 1) function = api->tensor_from_object;
+    if (api->major == 1) table = api;
   }
   Py_XDECREF(capsule);
   PyErr_Clear();
   if (count < 16) {
     Py_INCREF(type);
-    known[count++] = {type, function};
+    known[count++] = {type, table};
   }
-  return function;
+  return table;
 }
 
 // A tensor's attributes; false with an exception set where one is missing or fails.
@@ -177,11 +178,11 @@ bool view_attributes(PyObject* o, View* v) {
 }
 
 bool view(PyObject* o, View* v) {
-  const auto exchange = exchange_of(Py_TYPE(o));
+  const DLExchange* table = exchange_of(Py_TYPE(o));
   DLTensor t;
-  if (!exchange) return view_attributes(o, v);
+  if (!table || !table->tensor_from_object) return view_attributes(o, v);
   // Refused by the type (a tensor that requires a gradient, say): its attributes tell the same.
-  if (exchange(o, &t) != 0 || t.ndim > kMostDims || t.lanes != 1 || t.bits % 8) {
+  if (table->tensor_from_object(o, &t) != 0 || t.ndim > kMostDims || t.lanes != 1 || t.bits % 8) {
     PyErr_Clear();
     return view_attributes(o, v);
   }
@@ -269,9 +270,16 @@ bool to_int(PyObject* o, const char* what, int* out) {
   return true;
 }
 
-bool to_stream(PyObject* o, void** out) {
+// A stream given as an integer; without one, the stream on which the framework of `tensor` works on `device` now, or, where
+// its type does not tell, the legacy default stream.
+bool to_stream(PyObject* o, PyObject* tensor, int device, void** out) {
   *out = nullptr;
-  if (!o) return true;
+  if (!o || o == Py_None) {
+    const DLExchange* table = exchange_of(Py_TYPE(tensor));
+    if (!table || !table->current_stream || table->current_stream(kDLCuda, device, out) == 0) return true;
+    if (!PyErr_Occurred()) PyErr_Format(PyExc_RuntimeError, "no current stream on CUDA device %d", device);
+    return false;
+  }
   const unsigned long long n = PyLong_AsUnsignedLongLong(o);
   if (n == (unsigned long long)-1 && PyErr_Occurred()) return false;
   *out = reinterpret_cast<void*>(n);
@@ -518,7 +526,7 @@ PyObject* convert(const char* tensor, const char* matrix, PyObject* o, PyObject*
   if (!m) return nullptr;
   Rows data;
   void* st;
-  if (!take_rows(tensor, t, m->rows, m->cols, at.device, &data) || !to_stream(stream, &st) || !ready_on(at.device, m->rows)) return nullptr;
+  if (!take_rows(tensor, t, m->rows, m->cols, at.device, &data) || !to_stream(stream, m->values, at.device, &st) || !ready_on(at.device, m->rows)) return nullptr;
   laya_mx8_convert a{};
   a.rows = m->rows; a.cols = m->cols; a.dtype = data.dtype;
   a.values = at.values; a.scales = at.scales; a.ldv = at.ld;
@@ -581,7 +589,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject*
     if (eps == -1.0 && PyErr_Occurred()) return nullptr;
     a.eps = (float)eps;
   }
-  if (!to_stream(g[6], &st) || !ready_on(at.device, m->rows)) return nullptr;
+  if (!to_stream(g[6], m->values, at.device, &st) || !ready_on(at.device, m->rows)) return nullptr;
   a.rows = m->rows; a.cols = m->cols; a.dtype = x.dtype;
   a.x = x.ptr; a.ldx = x.ld; a.residual = r.ptr; a.ldr = r.ld; a.sum_out = s.ptr; a.lds = s.ld;
   a.values = at.values; a.scales = at.scales; a.ldv = at.ld;
@@ -663,7 +671,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* k
     err = static_cast<int*>(v.data);
   }
   void* st;
-  if (!to_stream(g[9], &st) || !ready_on(device, rows)) return nullptr;
+  if (!to_stream(g[9], x->values, device, &st) || !ready_on(device, rows)) return nullptr;
   int status;
   Py_BEGIN_ALLOW_THREADS
   status = g_lib.linear(&a, err, st);
@@ -697,14 +705,14 @@ PyObject* bind(PyObject*, PyObject* args) {
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL | METH_KEYWORDS
 PyMethodDef methods[] = {
-    {"quantize", FAST(quantize), "quantize(x, out, stream=0)\n--\n\nx [rows][cols] in 16 or 32 bits -> the Matrix `out`."},
-    {"dequantize", FAST(dequantize), "dequantize(x, out, stream=0)\n--\n\nThe Matrix `x` -> out [rows][cols] in 16 or 32 bits."},
+    {"quantize", FAST(quantize), "quantize(x, out, stream=None)\n--\n\nx [rows][cols] in 16 or 32 bits -> the Matrix `out`."},
+    {"dequantize", FAST(dequantize), "dequantize(x, out, stream=None)\n--\n\nThe Matrix `x` -> out [rows][cols] in 16 or 32 bits."},
     {"rms_norm", FAST(rms_norm),
-     "rms_norm(x, weight, out, residual=None, sum_out=None, eps=1e-6, stream=0)\n--\n\n"
+     "rms_norm(x, weight, out, residual=None, sum_out=None, eps=1e-6, stream=None)\n--\n\n"
      "h = x + residual; sum_out = h; out = h / sqrt(mean(h^2) + eps) * weight, in MX8.\n\n"
      "`residual` and `sum_out` are optional, of one type, and may be the same tensor."},
     {"linear", FAST(linear),
-     "linear(x, w, out, bias=None, gate=None, gate_bias=None, activation='none', residual=None, err=None, stream=0)\n--\n\n"
+     "linear(x, w, out, bias=None, gate=None, gate_bias=None, activation='none', residual=None, err=None, stream=None)\n--\n\n"
      "out = act(x w^T + bias) + residual, or, with a `gate` matrix,\n"
      "out = act(x gate^T + gate_bias) * (x w^T + bias) + residual.\n\n"
      "x: Matrix [rows][cols]; w, gate: Matrix [features][cols]; out: a Matrix or a tensor\n"

@@ -5,10 +5,11 @@ An MX8 matrix holds E4M3 values and one power-of-two scale per 32 consecutive va
 `Matrix` names its two buffers.  Tensors are torch's, or anything with the attributes of theirs that
 csrc/mx8_python.cpp reads (torch itself is not imported); rows must be contiguous, with any row
 stride.
-The caller owns every buffer.  The calls are enqueued on `stream` (a cudaStream_t as an integer;
-0, the default, is the legacy default stream) of the current device, where the buffers must be,
-allocate nothing and return at once: a tensor used on another stream than the one that wrote it is
-the caller's to order.
+The caller owns every buffer.  The calls are enqueued on `stream` (a cudaStream_t as an integer,
+0 being the legacy default stream; without it, torch's current stream, or that of whatever framework
+the tensors belong to, and the legacy default stream if its tensors do not tell) of the current
+device, where the buffers must be.  They allocate nothing and return at once: a tensor used on
+another stream than the one that wrote it is the caller's to order.
 
     x8 = mx8.Matrix.empty(x, *x.shape)                  # buffers beside x
     mx8.rms_norm(h, weight, x8, residual=r, sum_out=r)  # r += h; x8 = norm(r) in 8 bits

@@ -317,3 +317,73 @@ def test_conversions_refuse_too_many_values_in_the_widest_rows(lib, name, cols):
 def test_linear_refuses_results_whose_tiles_pass_32_bits(lib, rows, features):
     with pytest.raises(ValueError, match="at most 2147483392"):
         _lib.check(lib.laya_op_mx8_linear(ct.byref(linear(rows=rows, features=features, ldo=2 ** 31)), None, None))
+
+
+class DLTensor(ct.Structure):
+    _fields_ = [("data", ct.c_void_p), ("device_type", ct.c_int32), ("device_id", ct.c_int32), ("ndim", ct.c_int32),
+                ("code", ct.c_uint8), ("bits", ct.c_uint8), ("lanes", ct.c_uint16), ("shape", ct.POINTER(ct.c_int64)),
+                ("strides", ct.POINTER(ct.c_int64)), ("byte_offset", ct.c_uint64)]
+
+
+class DLExchange(ct.Structure):
+    _fields_ = [("major", ct.c_uint32), ("minor", ct.c_uint32), ("previous", ct.c_void_p), ("managed", ct.c_void_p * 3),
+                ("tensor_from_object", ct.c_void_p), ("current_stream", ct.c_void_p)]
+
+
+def exchanging(streams=None):
+    """A Fake whose type offers the DLPack exchange table; `streams`: device -> its current stream."""
+
+    @ct.PYFUNCTYPE(ct.c_int, ct.py_object, ct.POINTER(DLTensor))
+    def tensor_from_object(o, out):
+        n = len(o.shape)
+        o.kept = (ct.c_int64 * n)(*o.shape), (ct.c_int64 * n)(*o.strides)
+        code, bits = {"torch.float32": (2, 32), "torch.uint8": (1, 8)}[str(o.dtype)]
+        out[0] = DLTensor(o.ptr, 2, o.device, n, code, bits, 1, *(ct.cast(k, ct.POINTER(ct.c_int64)) for k in o.kept), 0)
+        return 0
+
+    @ct.PYFUNCTYPE(ct.c_int, ct.c_int32, ct.c_int32, ct.POINTER(ct.c_void_p))
+    def current_stream(kind, device, out):
+        if kind != 2 or device not in streams:
+            return -1
+        out[0] = streams[device]
+        return 0
+
+    address = lambda f: ct.cast(f, ct.c_void_p).value  # noqa: E731
+    table = DLExchange(1, 0, None, (ct.c_void_p * 3)(), address(tensor_from_object), address(current_stream) if streams is not None else None)
+    new = ct.pythonapi.PyCapsule_New
+    new.restype, new.argtypes = ct.py_object, [ct.c_void_p, ct.c_void_p, ct.c_void_p]
+    name = ct.create_string_buffer(b"dlpack_exchange_api")
+    members = {"__dlpack_c_exchange_api__": new(ct.addressof(table), ct.addressof(name), None),
+               "alive": (table, name, tensor_from_object, current_stream)}
+    return type("Exchanging", (Fake,), members)
+
+
+def test_calls_without_a_stream_take_the_frameworks_current_one(calls):
+    streams = {0: 0x770}
+    cls = exchanging(streams)
+    u = lambda *shape: cls(shape, "torch.uint8", 1)  # noqa: E731
+    m, w = mx8.Matrix(u(4, 32), u(512), 4, 32), mx8.Matrix(u(8, 32), u(512), 8, 32)
+    x = cls((4, 32))
+
+    def each(**how):
+        del calls[:]
+        mx8.quantize(x, m, **how), mx8.dequantize(m, x, **how)
+        mx8.rms_norm(x, cls((32,)), m, **how), mx8.linear(m, w, cls((4, 8)), **how)
+        return [stream for _, _, stream in calls]
+
+    assert each() == [0x770] * 4
+    assert each(stream=None) == [0x770] * 4
+    assert each(stream=0) == [None] * 4  # the legacy default stream
+    assert each(stream=0x99) == [0x99] * 4
+    streams[0] = 0x880
+    assert each() == [0x880] * 4
+    streams.clear()
+    with pytest.raises(RuntimeError, match="current stream"):
+        mx8.quantize(x, m)
+    # Types that do not tell.
+    cls = exchanging()
+    m, w, x = mx8.Matrix(u(4, 32), u(512), 4, 32), mx8.Matrix(u(8, 32), u(512), 8, 32), cls((4, 32))
+    assert each() == [None] * 4
+    cls = Fake
+    m, w, x = matrix(4, 32), matrix(8, 32), Fake((4, 32))
+    assert each() == [None] * 4

@@ -819,3 +819,30 @@ def test_activations_are_relatively_exact(act, rows, gated, out_type):
     off, want, x64 = (out.double() - want).abs()[:, keep], want[keep], at.double()[keep]
     tol = want.abs() * ((bound(x64) + 1) * 2.0 ** -24 + HALF_ULP[out_type]) + TINY[out_type]
     assert bool((off <= tol).all()), float((off / tol).max())
+
+
+def test_calls_without_a_stream_are_ordered_with_torchs_current_one():
+    rng = np.random.default_rng(19)
+    x = torch.from_numpy(activations(rng, 60, 256)).cuda()
+    w, _ = matrix(rng.normal(0, 0.1, (96, 256)).astype(np.float32))
+    want8, want = fresh(60, 256), torch.empty(60, 96, device="cuda")
+    x.mul_(-2.0), mx8.rms_norm(x, torch.ones(256, device="cuda"), want8), mx8.linear(want8, w, want)
+    x.div_(-2.0)
+    got8, got, ones = fresh(60, 256), torch.empty(60, 96, device="cuda"), torch.ones(256, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # some 10 ms, in which calls on another stream would be done
+        x.mul_(-2.0)
+        mx8.rms_norm(x, ones, got8)
+        mx8.linear(got8, w, got)
+        kept = got.clone()
+    side.synchronize()
+    assert torch.equal(kept, want) and torch.equal(got8.values, want8.values)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mx8.rms_norm(x, ones, got8)
+        mx8.linear(got8, w, got)
+    got.zero_()
+    graph.replay()
+    assert torch.equal(got, want)
