@@ -379,13 +379,20 @@ PyObject* matrix_empty(PyObject* type, PyObject* const* args, Py_ssize_t nargs, 
     PyErr_Format(PyExc_ValueError, "bad shape %d x %d: rows may be 0, columns may not", rows, cols);
     return nullptr;
   }
-  // like.new_zeros(n).byte(): a uint8 tensor of n elements beside `like`.
+  // like.new_zeros(n, dtype=torch.uint8).  `like` is torch's, so torch has been imported.
+  PyObject* torch = PyImport_ImportModule("torch");
+  PyObject* uint8 = torch ? PyObject_GetAttrString(torch, "uint8") : nullptr;
+  PyObject* dtype = uint8 ? Py_BuildValue("{s:O}", "dtype", uint8) : nullptr;
+  Py_XDECREF(torch);
+  Py_XDECREF(uint8);
+  if (!dtype) return nullptr;
   auto bytes = [&](long long n) -> PyObject* {
-    PyObject* wide = PyObject_CallMethod(given[0], "new_zeros", "L", n);
-    if (!wide) return nullptr;
-    PyObject* narrow = PyObject_CallMethod(wide, "byte", nullptr);
-    Py_DECREF(wide);
-    return narrow;
+    PyObject* method = PyObject_GetAttrString(given[0], "new_zeros");
+    PyObject* args = method ? Py_BuildValue("(L)", n) : nullptr;
+    PyObject* made = args ? PyObject_Call(method, args, dtype) : nullptr;
+    Py_XDECREF(method);
+    Py_XDECREF(args);
+    return made;
   };
   const long long room = ((long long)cols + 15) / 16 * 16;
   PyObject* flat = bytes(rows * room);
@@ -396,6 +403,7 @@ PyObject* matrix_empty(PyObject* type, PyObject* const* args, Py_ssize_t nargs, 
     PyObject* parts[4] = {values, scales, given[1], given[2]};
     made = matrix_make(reinterpret_cast<PyTypeObject*>(type), parts);
   }
+  Py_DECREF(dtype);
   Py_XDECREF(flat);
   Py_XDECREF(values);
   Py_XDECREF(scales);

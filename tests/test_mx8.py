@@ -387,3 +387,23 @@ def test_calls_without_a_stream_take_the_frameworks_current_one(calls):
     cls = Fake
     m, w, x = matrix(4, 32), matrix(8, 32), Fake((4, 32))
     assert each() == [None] * 4
+
+
+def test_empty_makes_no_more_bytes_than_the_matrix_has():
+    torch = pytest.importorskip("torch")
+    asked = []
+
+    class Like(Fake):
+        def new_zeros(self, n, dtype=None):
+            asked.append((n, dtype))
+            made = u8(n)
+            made.view = lambda rows, room: u8(rows, room)
+            made.byte = lambda: made
+            return made
+
+    m = mx8.Matrix.empty(Like((4,)), 300, 50)
+    assert (m.rows, m.cols, m.ld, m.values.shape, m.scales.shape) == (300, 50, 64, (300, 64), (3 * 512,))
+    assert asked == [(300 * 64, torch.uint8), (3 * 512, torch.uint8)]
+    for bad in (object(), Fake((4,))):
+        with pytest.raises(AttributeError):
+            mx8.Matrix.empty(bad, 4, 32)
