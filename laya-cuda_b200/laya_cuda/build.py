@@ -44,12 +44,23 @@ def run(target, cmd, verbose):
     os.replace(tmp, target)
 
 
+def build_extension(verbose=False):
+    """_mx8.so, which laya_cuda.mx8 alone needs: without this Python's headers it is left out, and one built from older
+    sources is taken away, so that importing laya_cuda.mx8 says so."""
+    include = Path(sysconfig.get_paths()["include"])
+    if not (include / "Python.h").exists():
+        EXTENSION.unlink(missing_ok=True)
+        print(f"{EXTENSION.name} is not built, and laya_cuda.mx8 not available: no {include / 'Python.h'}", file=sys.stderr)
+        return
+    run(EXTENSION, [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+                    "-I", str(include), str(EXTENSION_SOURCE)], verbose)
+
+
 def build(force=False, verbose=False):
     if force or not up_to_date(TARGET, DEPENDS):
         run(TARGET, [nvcc(), *FLAGS, "-I", str(INCLUDE), *map(str, SOURCES)], verbose)
     if force or not up_to_date(EXTENSION, [EXTENSION_SOURCE, INCLUDE / "laya_b200.h"]):
-        run(EXTENSION, [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
-                        "-I", sysconfig.get_paths()["include"], str(EXTENSION_SOURCE)], verbose)
+        build_extension(verbose)
     return TARGET
 
 
