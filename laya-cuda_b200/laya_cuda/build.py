@@ -1,4 +1,4 @@
-"""Builds liblaya_b200.so in-tree with nvcc for sm_100a (B200), and the Python extension _mx8.so.
+"""Builds liblaya_b200.so in-tree with nvcc for sm_100a (B200), and the Python extension _mx8.
 
     python -m laya_cuda.build            # from laya-cuda_b200/
 """
@@ -15,7 +15,8 @@ INCLUDE = PACKAGE.parents[1] / "include"
 TARGET = PACKAGE / "liblaya_b200.so"
 SOURCES = [CSRC / "laya_b200.cu", CSRC / "mx8.cu"]
 DEPENDS = SOURCES + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "laya_b200.h"]
-EXTENSION = PACKAGE / "_mx8.so"
+# Named for this Python's ABI, so that another one does not load it.
+EXTENSION = PACKAGE / ("_mx8" + sysconfig.get_config_var("EXT_SUFFIX"))
 EXTENSION_SOURCE = CSRC / "mx8_python.cpp"
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
          "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "--threads", "2"]
@@ -45,8 +46,9 @@ def run(target, cmd, verbose):
 
 
 def build_extension(verbose=False):
-    """_mx8.so, which laya_cuda.mx8 alone needs: without this Python's headers it is left out, and one built from older
+    """_mx8, which laya_cuda.mx8 alone needs: without this Python's headers it is left out, and one built from older
     sources is taken away, so that importing laya_cuda.mx8 says so."""
+    EXTENSION.with_name("_mx8.so").unlink(missing_ok=True)  # an earlier build's, which every Python would load
     include = Path(sysconfig.get_paths()["include"])
     if not (include / "Python.h").exists():
         EXTENSION.unlink(missing_ok=True)

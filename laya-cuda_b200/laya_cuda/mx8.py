@@ -23,7 +23,7 @@ from . import _lib
 try:
     from . import _mx8
 except ImportError as e:
-    raise RuntimeError("laya_cuda/_mx8.so is missing: build it with `python -m laya_cuda.build`") from e
+    raise RuntimeError("laya_cuda/_mx8 for this Python is missing: build it with `python -m laya_cuda.build`") from e
 
 __all__ = ["Matrix", "dequantize", "linear", "quantize", "rms_norm", "scale_bytes"]
 

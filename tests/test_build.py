@@ -32,3 +32,13 @@ def test_without_pythons_headers_the_library_is_built_and_the_extension_left_out
     assert [cmd[0] for cmd in compiled] == ["nvcc"]
     assert builder.TARGET.exists() and not builder.EXTENSION.exists()
     assert "laya_cuda.mx8 not available" in capsys.readouterr().err
+
+
+def test_the_extension_is_named_for_this_pythons_abi(compiled):
+    import importlib.machinery
+    suffix = importlib.machinery.EXTENSION_SUFFIXES[0]
+    assert builder.EXTENSION.name == "_mx8" + suffix and "cpython" in suffix
+    plain = builder.EXTENSION.with_name("_mx8.so")
+    plain.touch()
+    builder.build()
+    assert builder.EXTENSION.exists() and not plain.exists()
