@@ -36,9 +36,14 @@ class FeedForward:
         """What a batch of up to this many tokens needs beside the residual stream; reuse it."""
         return (mx8.Matrix.empty(like, tokens, self.up.cols), mx8.Matrix.empty(like, tokens, self.up.rows))
 
+    @staticmethod
+    def first(m, rows):
+        """The first rows of a matrix (tiles of scales follow one another by rows, so they start at the same byte)."""
+        return m if m.rows == rows else mx8.Matrix(m.values[:rows], m.scales, rows, m.cols)
+
     def __call__(self, x, residual, buffers):
         """Adds x and then the block's output to `residual`, in place."""
-        normed, hidden = buffers
+        normed, hidden = (self.first(m, x.shape[0]) for m in buffers)
         stream = torch.cuda.current_stream().cuda_stream
         mx8.rms_norm(x, self.weight, normed, residual=residual, sum_out=residual, eps=self.eps, stream=stream)
         mx8.linear(normed, self.up, hidden, gate=self.gate, activation="silu", stream=stream)

@@ -846,3 +846,19 @@ def test_calls_without_a_stream_are_ordered_with_torchs_current_one():
     got.zero_()
     graph.replay()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tokens", [1, 33, 128, 200])
+def test_the_examples_buffers_serve_smaller_batches(tokens):
+    import importlib.util
+    from pathlib import Path
+    spec = importlib.util.spec_from_file_location("mx8_feed_forward", Path(__file__).resolve().parents[1] / "examples" / "mx8_feed_forward.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    rng = np.random.default_rng(20)
+    d, f = 160, 224
+    block = example.FeedForward(*(torch.from_numpy(rng.normal(0, 0.1, s).astype(np.float32)).cuda() for s in ((d,), (f, d), (f, d), (d, f))))
+    x, r = (torch.from_numpy(activations(rng, tokens, d)).cuda() for _ in range(2))
+    buffers = block.buffers(200, x)
+    block(*(torch.from_numpy(activations(rng, 200, d)).cuda() for _ in range(2)), buffers)  # leaves other rows in them
+    assert torch.equal(block(x, r.clone(), buffers), block(x, r.clone(), block.buffers(tokens, x)))
