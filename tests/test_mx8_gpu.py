@@ -862,3 +862,115 @@ def test_the_examples_buffers_serve_smaller_batches(tokens):
     buffers = block.buffers(200, x)
     block(*(torch.from_numpy(activations(rng, 200, d)).cuda() for _ in range(2)), buffers)  # leaves other rows in them
     assert torch.equal(block(x, r.clone(), buffers), block(x, r.clone(), block.buffers(tokens, x)))
+
+
+# -------------------------------------------------------------------------------- several turns of the row kernels' loops
+#
+# More rows than the blocks that are launched take at once, so that each block comes round again: with the next row's loads,
+# the exchange of sums and the staging buffers of the turn before.  Neighbouring rows differ in size by powers of two, so that a
+# sum or a scale of another row shows.
+
+def scale_byte64(a):
+    """Scale bytes of blocks whose largest magnitudes are `a` (float64, finite)."""
+    mantissa, power = torch.frexp(a)
+    e = (power - 9 + (mantissa > 0.875).int()).clamp(min=-127)
+    return torch.where(a > 0, e + 127, torch.zeros_like(e))
+
+
+def blocks_gpu(v):
+    out = torch.zeros(v.shape[0], -(-v.shape[1] // 32) * 32, dtype=torch.float64, device="cuda")
+    out[:, : v.shape[1]] = v
+    return out.view(v.shape[0], -1, 32)
+
+
+def bytes_gpu(m):
+    return m.scales[torch.from_numpy(scale_index(m.rows, m.cols)).cuda()].int()
+
+
+def expand(byte, cols):
+    return torch.exp2(byte.double() - 127).repeat_interleave(32, dim=1)[:, :cols]
+
+
+def spread_rows(g, rows, cols, dtype, pad=0):
+    """Activations, each row times its own power of two, in a view `pad` wider than the row."""
+    v = torch.randn(rows, cols, generator=g, device="cuda") * torch.exp(0.8 * torch.randn(cols, generator=g, device="cuda"))
+    v *= torch.exp2(torch.randint(-5, 6, (rows, 1), generator=g, device="cuda").float())
+    store = torch.full((rows, cols + pad), 7.0, dtype=dtype, device="cuda")
+    store[:, :cols] = v
+    return store[:, :cols]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,cols", [(9000, 4096), (9000, 4095), (170000, 100), (90000, 200)])
+def test_quantize_many_rows(dtype, rows, cols):
+    g = torch.Generator(device="cuda").manual_seed(rows + cols)
+    x = spread_rows(g, rows, cols, TYPES[dtype])
+    out = fresh(rows, cols)
+    mx8.quantize(x, out)
+    v = x.double()
+    byte = scale_byte64(blocks_gpu(v).abs().amax(-1))
+    assert torch.equal(bytes_gpu(out), byte.int())
+    scale = expand(byte, cols)
+    # Nearest multiple of the step of the value's binade (of the subnormals' below 2^-6), ties to even.
+    step = torch.exp2((torch.frexp(v / scale)[1] - 1).clamp(min=-6).double() - 3)
+    assert torch.equal(decode_gpu(out), torch.round(v / scale / step) * step * scale)
+    assert not bool(out.values[:, cols:].any())
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,cols,pad", [(9000, 4096, 0), (9000, 4095, 0), (9000, 4090, 3), (200000, 133, 1)])
+def test_dequantize_many_rows(dtype, rows, cols, pad):
+    g = torch.Generator(device="cuda").manual_seed(rows + cols + 1)
+    m = fresh(rows, cols)
+    m.values.copy_(torch.randint(0, 127, m.values.shape, generator=g, device="cuda"))
+    m.values.bitwise_or_(torch.randint(0, 2, m.values.shape, generator=g, device="cuda").to(torch.uint8) << 7)
+    m.scales.copy_(torch.randint(105, 130, m.scales.shape, generator=g, device="cuda"))
+    store = torch.full((rows, cols + pad), 7.0, dtype=TYPES[dtype], device="cuda")
+    mx8.dequantize(m, store[:, :cols])
+    assert torch.equal(store[:, :cols], decode_gpu(m).float().to(TYPES[dtype]))  # exact in fp32
+    assert bool((store[:, cols:] == 7.0).all())
+
+
+MANY_ROWS = [(60000, 100), (60000, 200), (60000, 256), (20000, 768), (9000, 4096), (9000, 4095), (5000, 12001), (4000, 16384), (1500, 16401)]
+
+
+@pytest.mark.parametrize("dtype,rdtype", [("bf16", "f32"), ("f16", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("rows,cols", MANY_ROWS)
+@pytest.mark.parametrize("pad,in_place", [(0, False), (3, True)])
+def test_rms_norm_many_rows(dtype, rdtype, rows, cols, pad, in_place):
+    g = torch.Generator(device="cuda").manual_seed(rows + cols + 2)
+    x, r = spread_rows(g, rows, cols, TYPES[dtype], pad), spread_rows(g, rows, cols, TYPES[rdtype], pad)
+    w = 1 + 0.2 * torch.randn(cols, generator=g, device="cuda")
+    want = (x.float() + r.float()).to(TYPES[rdtype])
+    h = x.double() + r.double()
+    y = h * torch.rsqrt((h * h).mean(1, keepdim=True) + 1e-5) * w.double()
+    total = r if in_place else torch.empty_like(r)
+    out = fresh(rows, cols)
+    mx8.rms_norm(x, w, out, residual=r, sum_out=total, eps=1e-5)
+    assert torch.equal(total, want)
+    if pad and in_place:
+        assert bool((r.as_strided((rows, pad), (cols + pad, 1), cols) == 7.0).all())
+    # `check_mx8` on the GPU; h is rounded to fp32 once before it is squared and scaled.
+    slack = norm_slack(cols) * y.abs()
+    a, da, byte = blocks_gpu(y).abs().amax(-1), blocks_gpu(slack).amax(-1), bytes_gpu(out)
+    assert bool(((byte >= scale_byte64(a - da)) & (byte <= scale_byte64(a + da))).all())
+    scale = expand(byte, cols)
+    power = torch.frexp((y.abs() / scale).clamp(min=2.0 ** -6))[1] - 1
+    tol = scale * torch.exp2(power.double() - 4) * (1 + 1e-12) + 2 * slack
+    off = (decode_gpu(out) - y).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
+    assert not bool(out.values[:, cols:].any())
+
+
+def test_the_example_is_as_near_to_fp32_as_its_format():
+    """The block's update in MX8 against fp32.  A rounding to E4M3 is off by 0.026 of the value, root mean square: half a step,
+    at most 2^-4 of its binade's lower end, evenly spread (over the root of 3) and averaged over the binade (1.44).  n, G, U, a
+    and D are five such roundings; n's reaches the update through both factors of the gated product, and SiLU's slope makes
+    the gate's share up to 1.5 times as large: sqrt(1.5 0.037^2 + 0.037^2 + 2 0.026^2) = 0.069.  Half as much again is allowed."""
+    import importlib.util
+    from pathlib import Path
+    spec = importlib.util.spec_from_file_location("mx8_feed_forward", Path(__file__).resolve().parents[1] / "examples" / "mx8_feed_forward.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    for tokens, off in example.main(512, 1500):
+        assert off < 0.104, (tokens, off)
