@@ -303,12 +303,15 @@ int laya_op_gemm_residual_static(int precision, const void* x, const void* w, in
  * where a / 2^floor(log2 a) > 1.75, a the block's largest magnitude (e at least -127): the
  * smallest power of two under which no value passes 448.  Values are rounded to nearest even.  A
  * block that holds an infinity or a NaN reads back as NaN.  Scales of blocks past the last column
- * are written as 0 up to the tile's end; those of rows past the last are not written.
+ * are written as 0 up to the tile's end (255 there, in a matrix made elsewhere, would make a product
+ * NaN); those of rows past the last are not written.
  *
  * dtype: LAYA_DTYPE_F32, _F16 or _BF16.  Row strides (ld*) count elements; rows are contiguous and
- * may have any alignment their type allows (16-byte aligned rows run faster).  rows may be 0
- * (nothing is done).  Buffers belong to the current device, and so must `stream`
- * (LAYA_ERR_INVALID otherwise).  The calls allocate nothing and wait for nothing.
+ * may have any alignment their type allows.  Rows of whole 32-byte vectors run faster: base and
+ * stride multiples of 32 bytes, and a width that is a multiple of 16 (of 32 for a product's residual).
+ * rows may be 0 (nothing is done).  Buffers must be on the current device (laya_current_device; not
+ * checked here), and so must `stream` (LAYA_ERR_INVALID otherwise).  The calls allocate nothing and
+ * wait for nothing.
  * ------------------------------------------------------------------------------------------ */
 #define LAYA_ACT_NONE 0
 #define LAYA_ACT_RELU 1

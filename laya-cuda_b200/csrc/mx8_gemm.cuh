@@ -459,10 +459,9 @@ struct MxFewCfg {
   static constexpr int kStageB = BN * kMxBK;
   static constexpr int kStageScales = (kWeights + 1) * kMxTileBytes;
   static constexpr int kStageBytes = kWeights * kMxOperandBytes + kStageB + kStageScales;
-  // Not gated: shared memory for two CTAs per SM, so that the next kernel's CTAs set up while this one's
-  // finish (64 x 4096 x 4096: 6.8 us, with twice the stages 8.2), and an even number of stages, so that a
-  // stage always belongs to the same producer and issuer.  Gated stages are larger, and two of them too few
-  // (64 x 4096 x 2 x 4096: 12.9 us, with four 11.4).
+  // Not gated: as many stages as leave room for two CTAs per SM (64 x 4096 x 4096: 6.8 us, with twice the
+  // stages and one CTA 8.2), an even number of them, so that a stage always belongs to the same producer and
+  // issuer.  Gated stages are larger, and two of them too few (64 x 4096 x 2 x 4096: 12.9 us, with four 11.4).
   static constexpr int kStages = kGated ? 200 * 1024 / kStageBytes : 111 * 1024 / kStageBytes & ~1;
   static constexpr int kPartialBytes = kWeights * BN * 128 * 4;
   static constexpr int kSmemBytes = kStages * kStageBytes + 1024 /*align*/ + 256 /*barriers*/;

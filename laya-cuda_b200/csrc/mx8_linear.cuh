@@ -44,7 +44,8 @@ __device__ __forceinline__ float mx_silu(float v) { return v * rcp_approx(1.0f +
 //   q = Phi(-a) = exp(-a^2 / 2) t P(t),  t = 1 / (1 + p a),  and  x Phi(x) = x q for x <= 0, x (1 - q) for x > 0.
 // P: the degree-7 polynomial of least relative error (1.0e-7) for 0 <= a <= 14.5, fitted for this function.  With the roundings
 // and the special functions' errors the result is within (25 + 1.5 x^2) 2^-24 of itself, the second term from the
-// exponent's rounding; below x = -13.2 the exponential is 0.
+// exponent's rounding; below x = -13.2 the exponential is 0.  16384 x 64 x 4096 in bf16, all epilogue, takes 69 us
+// (gelu_erf2 64.5), 4096 x 768 x 3072 in f16 20.0 (19.6), 511 x 776 x 2304 7.0 with either.
 __device__ __forceinline__ float2 mx_gelu2(float2 x) {
   auto twice = [](float c) { return make_float2(c, c); };
   const float2 d = fma2(make_float2(fabsf(x.x), fabsf(x.y)), twice(0.305f), twice(1.0f));
@@ -248,9 +249,10 @@ __device__ __forceinline__ void mx_finish(const MxLinearArgs& a, int row0, int s
 // Epilogue of 32 columns of one row per thread (many rows): the lane's accumulator row as tensor memory
 // gives it, columns c0 .. c0 + 31, c0 a multiple of 32.  An MX8 block is one thread's, and 32-byte accesses
 // fill whole sectors without a transpose.  With K = 64, where the epilogue is all there is, 16384 x 4096 results
-// take 34 us in bf16 (of which 20 to write them), 26 in MX8 (11), 56 in bf16 with a GELU (its two special-
-// function operations per result are 2.2 us of a tile's 3.9) and 71 in bf16 with a bf16 residual (41 for the
-// bytes); four columns of eight rows per thread, through shared memory, took 39, 112, 79 and 75.
+// take 36 us in bf16 (of which 21 to write them), 33 in MX8 (11), 69 in bf16 with a GELU (its two special-
+// function operations per result are 2.2 us of a tile's 4.9) and 72 in bf16 with a bf16 residual (41 for the
+// bytes): launches in a row over three sets of buffers.  On one set, where the choice was made, 34, 26, 56 (with the
+// encoder's shorter GELU) and 71; four columns of eight rows per thread, through shared memory, 39, 112, 79 and 75.
 // ---------------------------------------------------------------------------------------------
 
 // How a kernel reads the residual.  The common forms are kernels of their own: a load behind a test (of
@@ -443,7 +445,7 @@ __device__ __forceinline__ uint32_t mx_finish_row(const MxLinearArgs& a, int row
     }
     return 0;
   }
-  // fp32 rows (a thread's 128 bytes in four stores, 16384 x 64 x 4096 + fp32: 131 us, this way 117) and rows
+  // fp32 rows (a thread's 128 bytes in four stores, 16384 x 64 x 4096 + fp32: 131 us, this way 117; over three sets of buffers 105) and rows
   // that are not made of aligned 32-byte vectors: through shared memory, so that eight lanes write 32
   // neighbouring columns of a row, or, where four columns are no vector, the warp writes one row after the other.
   const int lane = threadIdx.x & 31, row0 = row - lane;
