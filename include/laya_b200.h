@@ -373,6 +373,85 @@ typedef struct laya_mx8_linear {
  * wait that ran out, after which out is undefined. */
 int laya_op_mx8_linear(const laya_mx8_linear* args, int* err, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Rotary positions and attention for packed sequences (no counterpart in the reference, whose rotation
+ * is fused into a product and whose attention has 64-value heads and a symmetric window only): what stands
+ * between the two projections of a layer.
+ *
+ * Tensors are [tokens][heads][head_dim] with any token and head stride (in elements); the values of a
+ * head are contiguous.  Buffers must be on the current device (not checked here), and so must `stream`
+ * (LAYA_ERR_INVALID otherwise).  The calls allocate nothing and wait for nothing.
+ * ------------------------------------------------------------------------------------------ */
+#define LAYA_ROTARY_NONE 0    /* f_k = theta^(-2k / dims) */
+#define LAYA_ROTARY_LINEAR 1  /* f_k / factor */
+#define LAYA_ROTARY_NTK 2     /* theta * factor^(dims / (dims - 2)) in theta's place (dims > 2) */
+#define LAYA_ROTARY_PARTS 3   /* f_k (g + (1 - g) / factor), g = clamp((length f_k / 2 pi - low) / (high - low), 0, 1) */
+#define LAYA_ROTARY_MOST_DIMS 512
+
+/* One tensor of a rotation; `out` may be x itself (with x's strides). */
+typedef struct laya_heads {
+  const void* x; int64_t x_token, x_head;
+  void* out; int64_t out_token, out_head;
+  int32_t heads;                 /* 0: none */
+  int32_t reserved;
+} laya_heads;
+
+/* Arguments of laya_op_rotary. */
+typedef struct laya_rotary {
+  int32_t tokens, head_dim;
+  int32_t dims;                  /* leading values of a head that are turned: even, 2 .. min(head_dim, LAYA_ROTARY_MOST_DIMS) */
+  int32_t dtype;                 /* LAYA_DTYPE_F32, _F16 or _BF16 */
+  laya_heads part[2];            /* queries and keys, say */
+  const void* positions;         /* [tokens], int32 or int64 */
+  int32_t positions_64;
+  int32_t interleaved;           /* 1: pairs (2k, 2k + 1); 0: pairs (k, k + dims / 2) */
+  int32_t backward;              /* 1: the transposed map, from a gradient of the result to one of x */
+  int32_t scaling;               /* LAYA_ROTARY_* */
+  double theta, factor, length, low, high;
+  float magnitude;               /* multiplies the turned values */
+} laya_rotary;
+
+/* (a, b) -> magnitude (a cos w - b sin w, a sin w + b cos w) for the pairs k = 0 .. dims / 2 - 1 of each head,
+ * w = position f_k; the other values of a head are copied.  The angle is computed in 64 bits, its
+ * sine and cosine and the turn in 32, with one rounding to dtype. */
+int laya_op_rotary(const laya_rotary* args, void* stream);
+
+/* Arguments of laya_op_attend. */
+typedef struct laya_attend {
+  int32_t sequences, heads, kv_heads;  /* heads a multiple of kv_heads, of at most 128 times: head h reads kv head h / (heads / kv_heads) */
+  int32_t head_dim;              /* a multiple of 8, 8 .. 128 */
+  int32_t dtype;                 /* LAYA_DTYPE_F16 or _BF16 */
+  int32_t q_tokens, k_tokens;    /* rows of q and out, and of k and v */
+  int32_t max_queries, max_keys; /* bounds on the lengths; queries past max_queries of a sequence are not computed */
+  const void* q; int64_t q_token, q_head;    /* [q_tokens][heads][head_dim]; q, k, v: 16-byte aligned, */
+  const void* k; int64_t k_token, k_head;    /* [k_tokens][kv_heads][head_dim]; strides multiples of 8 */
+  const void* v; int64_t v_token, v_head;
+  void* out; int64_t out_token, out_head;    /* [q_tokens][heads][head_dim] */
+  float* lse;                    /* [q_tokens][heads], or NULL: log of the sum of exp(s), -infinity where nothing is visible */
+  const int32_t *starts, *lengths;      /* [sequences]: first row and number of queries */
+  const int32_t *k_starts, *k_lengths;  /* [sequences]: of keys; both NULL: as the queries */
+  float scale, cap;              /* cap 0: none */
+  int32_t causal;
+  int32_t window_left, window_right;    /* -1: no bound */
+  const int32_t* prefix;         /* [sequences] or NULL */
+  const int32_t *documents, *k_documents;  /* [q_tokens], [k_tokens], or both NULL */
+  const float* slopes;           /* [heads] or NULL */
+  const float* distance_bias;    /* [heads][2 reach + 1] or NULL; not with slopes */
+  int32_t reach;
+  int32_t reserved;
+} laya_attend;
+
+/* Query i of a sequence of n queries and m keys is at p = i + m - n, among the keys' positions 0 .. m - 1.
+ *   s = scale q . k;  s = cap tanh(s / cap);  s -= slopes[h] |p - j|;  s += distance_bias[h][clamp(j - p, -reach, reach) + reach]
+ *   out = sum softmax(s)_j v_j over the visible keys j, zeros where there are none (or all have s = -infinity)
+ * Key j is visible where j < prefix, or where documents[query] == k_documents[key], causal implies j <= p, and
+ * p - window_left <= j <= p + window_right.  Keys that are not visible may hold anything, rows outside the sequences
+ * too; rows of out that belong to no sequence are left as they were.  Scores and sums are held in 32 bits, softmax's
+ * numerators are rounded to dtype before they meet v.  The result is the same each time.
+ * err (zero on entry, or NULL) receives a device error: 4 for a sequence outside the tensors' rows, which is
+ * skipped, or a pipeline wait that ran out, after which out is undefined. */
+int laya_op_attend(const laya_attend* args, int* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

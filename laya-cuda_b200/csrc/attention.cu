@@ -1,0 +1,148 @@
+// Entry points of the rotary positions and of attention over packed sequences (see include/laya_b200.h): checks of
+// arguments and launches.
+#include <algorithm>
+#include <cmath>
+
+#include "attend.cuh"
+#include "host.cuh"
+#include "rotary.cuh"
+
+using namespace laya;
+
+namespace {
+
+// A tensor [tokens][heads][dim], strides in elements.
+void check_heads(const char* what, const void* p, int64_t token, int64_t head, int dtype) {
+  if (!p) fail(LAYA_ERR_INVALID, "%s is null", what);
+  if (token < 0 || head < 0) fail(LAYA_ERR_INVALID, "%s: a stride is negative; it must be at least 0", what);
+  if (reinterpret_cast<uintptr_t>(p) % dtype_size(dtype)) fail(LAYA_ERR_INVALID, "%s is not aligned to its elements", what);
+}
+
+// Tokens and heads apart from one another, as what is written must be.
+void check_apart(const char* what, int tokens, int heads, int dim, int64_t token, int64_t head) {
+  if ((tokens > 1 && token < dim) || (heads > 1 && head < dim))
+    fail(LAYA_ERR_INVALID, "%s: strides %lld and %lld must be at least a head's %d values", what, (long long)token, (long long)head, dim);
+}
+
+// 16-byte vectors, which the tensor maps and the stores of attention take.  The stride of a dimension of one says nothing and is
+// made one that they take.
+void check_vectors(const char* what, const void* p, int tokens, int heads, int dim, int64_t* token, int64_t* head, int dtype) {
+  if (heads == 1) *head = dim;
+  if (tokens == 1) *token = heads * *head;
+  check_heads(what, p, *token, *head, dtype);
+  check_apart(what, tokens, heads, dim, *token, *head);
+  if (reinterpret_cast<uintptr_t>(p) & 15) fail(LAYA_ERR_INVALID, "%s must be 16-byte aligned", what);
+  if (*token % 8 || *head % 8) fail(LAYA_ERR_INVALID, "%s: strides %lld and %lld must each be a multiple of 8", what, (long long)*token, (long long)*head);
+  if (*token >= (1ll << 38) || *head >= (1ll << 38)) fail(LAYA_ERR_INVALID, "%s: a stride is too large", what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int laya_op_rotary(const laya_rotary* p, void* stream) {
+  OP_API_BEGIN
+  if (!p) fail(LAYA_ERR_INVALID, "null argument");
+  if (p->tokens < 0 || p->head_dim < 1) fail(LAYA_ERR_INVALID, "bad shape: %d tokens, heads of %d", p->tokens, p->head_dim);
+  if (p->dims < 2 || p->dims % 2 || p->dims > std::min(p->head_dim, LAYA_ROTARY_MOST_DIMS))
+    fail(LAYA_ERR_INVALID, "dims %d is not even and between 2 and %d", p->dims, std::min(p->head_dim, LAYA_ROTARY_MOST_DIMS));
+  dtype_size(p->dtype);
+  if (p->scaling < LAYA_ROTARY_NONE || p->scaling > LAYA_ROTARY_PARTS) fail(LAYA_ERR_INVALID, "unknown scaling %d", p->scaling);
+  if (!(p->theta > 0) || !std::isfinite(p->theta)) fail(LAYA_ERR_INVALID, "theta must be positive");
+  if (p->scaling != LAYA_ROTARY_NONE && (!(p->factor > 0) || !std::isfinite(p->factor))) fail(LAYA_ERR_INVALID, "factor must be positive");
+  if (p->scaling == LAYA_ROTARY_NTK && p->dims <= 2) fail(LAYA_ERR_INVALID, "ntk scaling needs dims above 2");
+  if (p->scaling == LAYA_ROTARY_PARTS && (!(p->length > 0) || !(p->low < p->high)))
+    fail(LAYA_ERR_INVALID, "scaling by parts needs a length and low < high");
+  RotaryArgs a{};
+  for (int i = 0; i < 2; ++i) {
+    const laya_heads& h = p->part[i];
+    if (h.heads < 0) fail(LAYA_ERR_INVALID, "bad shape: %d heads", h.heads);
+    if (!h.heads || !p->tokens) continue;
+    check_heads("x", h.x, h.x_token, h.x_head, p->dtype);
+    check_heads("out", h.out, h.out_token, h.out_head, p->dtype);
+    check_apart("out", p->tokens, h.heads, p->head_dim, h.out_token, h.out_head);
+    const bool in_place = h.x == h.out;
+    if (in_place && (h.x_token != h.out_token || h.x_head != h.out_head))
+      fail(LAYA_ERR_INVALID, "out is x, but with other strides");
+    a.part[i] = {h.x, h.out, h.x_token, h.x_head, h.out_token, h.out_head, h.heads, !in_place};
+  }
+  if (!p->tokens || (!a.part[0].heads && !a.part[1].heads)) return LAYA_OK;
+  if (!p->positions) fail(LAYA_ERR_INVALID, "positions is null");
+  if (reinterpret_cast<uintptr_t>(p->positions) % (p->positions_64 ? 8 : 4)) fail(LAYA_ERR_INVALID, "positions is not aligned to its elements");
+  a.positions = p->positions;
+  a.positions_64 = p->positions_64;
+  a.tokens = p->tokens;
+  a.dim = p->head_dim;
+  a.pairs = p->dims / 2;
+  a.sine_sign = p->backward ? -1.f : 1.f;
+  a.magnitude = p->magnitude;
+  constexpr double kTurn = 6.283185307179586;
+  double theta = p->theta;
+  if (p->scaling == LAYA_ROTARY_NTK) theta *= std::pow(p->factor, p->dims / (p->dims - 2.0));
+  for (int k = 0; k < a.pairs; ++k) {
+    double f = std::pow(theta, -2.0 * k / p->dims);
+    if (p->scaling == LAYA_ROTARY_LINEAR) f /= p->factor;
+    if (p->scaling == LAYA_ROTARY_PARTS) {
+      const double keep = std::min(1.0, std::max(0.0, (p->length * f / kTurn - p->low) / (p->high - p->low)));
+      f *= keep + (1 - keep) / p->factor;
+    }
+    a.turns[k] = f / kTurn;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count(current_device(st));
+  with_type(p->dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    auto kern = p->interleaved ? rotary_kernel<T, true> : rotary_kernel<T, false>;
+    launch_k(kern, dim3(std::min(p->tokens, 64 * sms)), dim3(kRotaryThreads), 0, st, a);
+  });
+  OP_API_END
+}
+
+int laya_op_attend(const laya_attend* p, int* err, void* stream) {
+  OP_API_BEGIN
+  if (!p) fail(LAYA_ERR_INVALID, "null argument");
+  if (p->sequences < 0 || p->sequences > 65535 || p->q_tokens < 0 || p->k_tokens < 0 || p->max_queries < 0 || p->max_keys < 0)
+    fail(LAYA_ERR_INVALID, "bad shape: %d sequences (65535 at most), %d and %d tokens, at most %d and %d of a sequence", p->sequences,
+         p->q_tokens, p->k_tokens, p->max_queries, p->max_keys);
+  if (p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->heads / p->kv_heads > 128 || p->heads > 65535)
+    fail(LAYA_ERR_INVALID, "%d heads over %d kv heads: a multiple of at most 128 times", p->heads, p->kv_heads);
+  if (p->head_dim < 8 || p->head_dim > kAttendMostDim || p->head_dim % 8)
+    fail(LAYA_ERR_INVALID, "heads of %d values: a multiple of 8 up to %d", p->head_dim, kAttendMostDim);
+  if (p->dtype != LAYA_DTYPE_F16 && p->dtype != LAYA_DTYPE_BF16) fail(LAYA_ERR_INVALID, "dtype %d is not F16 or BF16", p->dtype);
+  if (!std::isfinite(p->scale)) fail(LAYA_ERR_INVALID, "scale must be finite");
+  if (!(p->cap >= 0.f) || !std::isfinite(p->cap)) fail(LAYA_ERR_INVALID, "cap must be at least 0");
+  if (p->window_left < -1 || p->window_right < -1) fail(LAYA_ERR_INVALID, "window bounds must be at least 0, or -1 for none");
+  if (p->slopes && p->distance_bias) fail(LAYA_ERR_INVALID, "slopes and distance_bias cannot both be given");
+  if (p->distance_bias && p->reach < 0) fail(LAYA_ERR_INVALID, "reach must be at least 0");
+  if (!p->documents != !p->k_documents) fail(LAYA_ERR_INVALID, "documents and k_documents go together");
+  if (!p->k_starts != !p->k_lengths) fail(LAYA_ERR_INVALID, "k_starts and k_lengths go together");
+  if (!p->sequences || !p->q_tokens || !p->max_queries) return LAYA_OK;
+  if (!p->starts || !p->lengths) fail(LAYA_ERR_INVALID, "starts or lengths is null");
+  AttendArgs a{};
+  a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.lse = p->lse;
+  a.q_token = p->q_token; a.q_head = p->q_head; a.k_token = p->k_token; a.k_head = p->k_head;
+  a.v_token = p->v_token; a.v_head = p->v_head; a.out_token = p->out_token; a.out_head = p->out_head;
+  check_vectors("q", p->q, p->q_tokens, p->heads, p->head_dim, &a.q_token, &a.q_head, p->dtype);
+  check_vectors("out", p->out, p->q_tokens, p->heads, p->head_dim, &a.out_token, &a.out_head, p->dtype);
+  if (p->k_tokens) {
+    check_vectors("k", p->k, p->k_tokens, p->kv_heads, p->head_dim, &a.k_token, &a.k_head, p->dtype);
+    check_vectors("v", p->v, p->k_tokens, p->kv_heads, p->head_dim, &a.v_token, &a.v_head, p->dtype);
+  }
+  a.starts = p->starts; a.lengths = p->lengths;
+  a.k_starts = p->k_starts ? p->k_starts : p->starts;
+  a.k_lengths = p->k_lengths ? p->k_lengths : p->lengths;
+  a.sequences = p->sequences; a.heads = p->heads; a.kv_heads = p->kv_heads; a.group = p->heads / p->kv_heads; a.dim = p->head_dim;
+  a.q_tokens = p->q_tokens; a.k_tokens = p->k_tokens; a.max_queries = std::min(p->max_queries, p->q_tokens);
+  a.scale = p->scale; a.cap = p->cap; a.causal = p->causal; a.left = p->window_left; a.right = p->window_right;
+  a.prefix = p->prefix; a.documents = p->documents; a.k_documents = p->k_documents;
+  a.slopes = p->slopes; a.table = p->distance_bias; a.reach = p->reach;
+  a.err = err;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  current_device(st);
+  const dim3 grid((a.max_queries + 3) / 4, a.heads, a.sequences);
+  if (p->dtype == LAYA_DTYPE_F16) launch_k(attend_rows_kernel<__half>, grid, dim3(128), 0, st, a);
+  else launch_k(attend_rows_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, a);
+  OP_API_END
+}
+
+}  // extern "C"

@@ -2,11 +2,14 @@
 // properties, process-wide launch options and the kernel launcher.
 #pragma once
 #include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <exception>
 #include <string>
 #include <utility>
 
@@ -93,6 +96,65 @@ void launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cuda
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
   CK(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
+// ---------------------------------------------------------------------------------------------
+// Entry points of operators: exceptions end in status codes, with the message in laya_last_error(NULL).
+// ---------------------------------------------------------------------------------------------
+#define OP_API_BEGIN try {
+#define OP_API_END                                     \
+  }                                                    \
+  catch (const Failure& f) {                           \
+    g_create_error = f.msg;                            \
+    return f.code;                                     \
+  }                                                    \
+  catch (const std::exception& x) {                    \
+    g_create_error = x.what();                         \
+    return LAYA_ERR_CUDA;                              \
+  }                                                    \
+  return LAYA_OK;
+
+inline size_t dtype_size(int dtype) {
+  switch (dtype) {
+    case LAYA_DTYPE_F32: return 4;
+    case LAYA_DTYPE_F16:
+    case LAYA_DTYPE_BF16: return 2;
+    default: fail(LAYA_ERR_INVALID, "dtype %d is not F32, F16 or BF16", dtype);
+  }
+}
+
+// Calls f with a null pointer of the element type that `dtype` names.
+template <typename F>
+void with_type(int dtype, F f) {
+  switch (dtype) {
+    case LAYA_DTYPE_F32: return f((float*)nullptr);
+    case LAYA_DTYPE_F16: return f((__half*)nullptr);
+    case LAYA_DTYPE_BF16: return f((__nv_bfloat16*)nullptr);
+    default: fail(LAYA_ERR_INVALID, "dtype %d is not F32, F16 or BF16", dtype);
+  }
+}
+
+// The current device, checked to be `stream`'s.  A stream under capture cannot be asked.
+inline int current_device(cudaStream_t stream) {
+  int dev = 0;
+  CK(cudaGetDevice(&dev));
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (stream) CK(cudaStreamIsCapturing(stream, &capture));
+  if (stream && capture == cudaStreamCaptureStatusNone) {
+    int of = -1;
+    CK(cudaStreamGetDevice(stream, &of));
+    if (of != dev) fail(LAYA_ERR_INVALID, "stream belongs to device %d, the current device is %d", of, dev);
+  }
+  return dev;
+}
+
+// Raises the kernel's dynamic shared memory limit once per device (`done`: one bit per device).
+template <typename K>
+void allow_smem(K kern, int bytes, int dev, std::atomic<uint64_t>& done) {
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 }  // namespace laya

@@ -11,39 +11,6 @@ using namespace laya;
 
 namespace {
 
-#define MX_API_BEGIN try {
-#define MX_API_END                                     \
-  }                                                    \
-  catch (const Failure& f) {                           \
-    g_create_error = f.msg;                            \
-    return f.code;                                     \
-  }                                                    \
-  catch (const std::exception& x) {                    \
-    g_create_error = x.what();                         \
-    return LAYA_ERR_CUDA;                              \
-  }                                                    \
-  return LAYA_OK;
-
-size_t dtype_size(int dtype) {
-  switch (dtype) {
-    case LAYA_DTYPE_F32: return 4;
-    case LAYA_DTYPE_F16:
-    case LAYA_DTYPE_BF16: return 2;
-    default: fail(LAYA_ERR_INVALID, "dtype %d is not F32, F16 or BF16", dtype);
-  }
-}
-
-// Calls f with a null pointer of the element type that `dtype` names.
-template <typename F>
-void with_type(int dtype, F f) {
-  switch (dtype) {
-    case LAYA_DTYPE_F32: return f((float*)nullptr);
-    case LAYA_DTYPE_F16: return f((__half*)nullptr);
-    case LAYA_DTYPE_BF16: return f((__nv_bfloat16*)nullptr);
-    default: fail(LAYA_ERR_INVALID, "dtype %d is not F32, F16 or BF16", dtype);
-  }
-}
-
 void check_shape(int rows, int cols) {
   if (rows < 0 || cols < 1) fail(LAYA_ERR_INVALID, "bad shape %d x %d: rows may be 0, columns may not", rows, cols);
 }
@@ -63,20 +30,6 @@ void check_mx8(const char* what, const void* q, int64_t ld, const void* scales, 
 
 void check_vector(const char* what, const float* p) {
   if (p && (reinterpret_cast<uintptr_t>(p) & 15)) fail(LAYA_ERR_INVALID, "%s must be 16-byte aligned", what);
-}
-
-// The current device, checked to be `stream`'s.  A stream under capture cannot be asked.
-int current_device(cudaStream_t stream) {
-  int dev = 0;
-  CK(cudaGetDevice(&dev));
-  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  if (stream) CK(cudaStreamIsCapturing(stream, &capture));
-  if (stream && capture == cudaStreamCaptureStatusNone) {
-    int of = -1;
-    CK(cudaStreamGetDevice(stream, &of));
-    if (of != dev) fail(LAYA_ERR_INVALID, "stream belongs to device %d, the current device is %d", of, dev);
-  }
-  return dev;
 }
 
 // E4M3 values [rows][cols], row stride ld bytes; box {128 columns, box_rows}, 128-byte swizzle.
@@ -120,15 +73,6 @@ MxMaps linear_maps(const MxLinearArgs& a, int x_box, int w_box, int w_tiles) {
     m.gs = scale_map(a.gate, a.N, a.K, w_tiles);
   }
   return m;
-}
-
-// Raises the kernel's dynamic shared memory limit once per device (`done`: one bit per device).
-template <typename K>
-void allow_smem(K kern, int bytes, int dev, std::atomic<uint64_t>& done) {
-  const uint64_t bit = 1ull << (dev & 63);
-  if (done.load(std::memory_order_relaxed) & bit) return;
-  CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 template <typename K>
@@ -296,7 +240,7 @@ int64_t laya_mx8_scale_bytes(int rows, int cols) {
 }
 
 int laya_op_mx8_quantize(const laya_mx8_convert* p, void* stream) {
-  MX_API_BEGIN
+  OP_API_BEGIN
   if (!p) fail(LAYA_ERR_INVALID, "null argument");
   const int rows = p->rows, cols = p->cols;
   check_shape(rows, cols);
@@ -319,11 +263,11 @@ int laya_op_mx8_quantize(const laya_mx8_convert* p, void* stream) {
     if (rows_vectored(x, p->ld, cols)) go(mx8_quantize_kernel<T, true>);
     else go(mx8_quantize_kernel<T, false>);
   });
-  MX_API_END
+  OP_API_END
 }
 
 int laya_op_mx8_dequantize(const laya_mx8_convert* p, void* stream) {
-  MX_API_BEGIN
+  OP_API_BEGIN
   if (!p) fail(LAYA_ERR_INVALID, "null argument");
   const int rows = p->rows, cols = p->cols;
   check_shape(rows, cols);
@@ -353,11 +297,11 @@ int laya_op_mx8_dequantize(const laya_mx8_convert* p, void* stream) {
       else go(mx8_dequantize_kernel<T, MxStore::kElements>);
     } else go(mx8_dequantize_kernel<T, MxStore::kElements>);
   });
-  MX_API_END
+  OP_API_END
 }
 
 int laya_op_rms_norm_mx8(const laya_rms_norm_mx8* p, void* stream) {
-  MX_API_BEGIN
+  OP_API_BEGIN
   if (!p) fail(LAYA_ERR_INVALID, "null argument");
   const int rows = p->rows, cols = p->cols;
   check_shape(rows, cols);
@@ -382,11 +326,11 @@ int laya_op_rms_norm_mx8(const laya_rms_norm_mx8* p, void* stream) {
       launch_norm<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(r)>>(a, sms, st);
     });
   });
-  MX_API_END
+  OP_API_END
 }
 
 int laya_op_mx8_linear(const laya_mx8_linear* p, int* err, void* stream) {
-  MX_API_BEGIN
+  OP_API_BEGIN
   if (!p) fail(LAYA_ERR_INVALID, "null argument");
   const int M = p->rows, N = p->features, K = p->cols;
   check_shape(M, N);
@@ -434,7 +378,7 @@ int laya_op_mx8_linear(const laya_mx8_linear* p, int* err, void* stream) {
   a.wait_ns = wait_ns();
   if (gated) launch_linear<true>(a, dev, st);
   else launch_linear<false>(a, dev, st);
-  MX_API_END
+  OP_API_END
 }
 
 }  // extern "C"

@@ -11,6 +11,7 @@ LIB_PATH = Path(__file__).with_name(LIB_NAME)
 
 OK, ERR_INVALID, ERR_CUDA, ERR_DEVICE, ERR_STATE, ERR_NO_DEVICE = range(6)
 DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_MX8 = 0, 1, 2, 3
+ROTARY_NONE, ROTARY_LINEAR, ROTARY_NTK, ROTARY_PARTS = 0, 1, 2, 3
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 PRECISION_BF16, PRECISION_F16 = 0, 1
 
@@ -23,6 +24,7 @@ EXPORTS = (
     "laya_last_error", "laya_set_launch_options", "laya_current_device", "laya_op_gemm", "laya_op_gemm_ln", "laya_interleave_geglu", "laya_op_attention", "laya_op_attention_gathered",
     "laya_attention_tiles", "laya_op_embed_norm", "laya_op_head_tail", "laya_op_norm", "laya_op_gemm_residual_static",
     "laya_mx8_scale_bytes", "laya_op_mx8_quantize", "laya_op_mx8_dequantize", "laya_op_rms_norm_mx8", "laya_op_mx8_linear",
+    "laya_op_rotary", "laya_op_attend",
 )
 STATIC_SCRATCH_FLOATS = 4 * 1024 * 1024
 
@@ -63,6 +65,32 @@ class Mx8Linear(ct.Structure):
                 ("residual", ct.c_void_p), ("ldr", ct.c_int64),
                 ("out", ct.c_void_p), ("out_scales", ct.c_void_p), ("ldo", ct.c_int64),
                 ("residual_dtype", ct.c_int32), ("out_dtype", ct.c_int32)]
+
+
+class Heads(ct.Structure):
+    _fields_ = [("x", ct.c_void_p), ("x_token", ct.c_int64), ("x_head", ct.c_int64),
+                ("out", ct.c_void_p), ("out_token", ct.c_int64), ("out_head", ct.c_int64),
+                ("heads", ct.c_int32), ("reserved", ct.c_int32)]
+
+
+class Rotary(ct.Structure):
+    _fields_ = [("tokens", ct.c_int32), ("head_dim", ct.c_int32), ("dims", ct.c_int32), ("dtype", ct.c_int32),
+                ("part", Heads * 2), ("positions", ct.c_void_p), ("positions_64", ct.c_int32), ("interleaved", ct.c_int32),
+                ("backward", ct.c_int32), ("scaling", ct.c_int32),
+                ("theta", ct.c_double), ("factor", ct.c_double), ("length", ct.c_double), ("low", ct.c_double), ("high", ct.c_double),
+                ("magnitude", ct.c_float)]
+
+
+class Attend(ct.Structure):
+    _fields_ = [(name, ct.c_int32) for name in ("sequences", "heads", "kv_heads", "head_dim", "dtype", "q_tokens", "k_tokens",
+                                                "max_queries", "max_keys")]
+    for _name in ("q", "k", "v", "out"):
+        _fields_ += [(_name, ct.c_void_p), (_name + "_token", ct.c_int64), (_name + "_head", ct.c_int64)]
+    _fields_ += [(_name, ct.c_void_p) for _name in ("lse", "starts", "lengths", "k_starts", "k_lengths")]
+    _fields_ += [("scale", ct.c_float), ("cap", ct.c_float), ("causal", ct.c_int32), ("window_left", ct.c_int32),
+                 ("window_right", ct.c_int32)]
+    _fields_ += [(_name, ct.c_void_p) for _name in ("prefix", "documents", "k_documents", "slopes", "distance_bias")]
+    _fields_ += [("reach", ct.c_int32), ("reserved", ct.c_int32)]
 
 
 _lib = None
@@ -119,6 +147,8 @@ def load():
         "laya_op_mx8_dequantize": (i, [p, p]),
         "laya_op_rms_norm_mx8": (i, [p, p]),
         "laya_op_mx8_linear": (i, [p, p, p]),
+        "laya_op_rotary": (i, [p, p]),
+        "laya_op_attend": (i, [p, p, p]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

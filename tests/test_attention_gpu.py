@@ -1,0 +1,594 @@
+"""Rotary positions and attention on the GPU against their definitions in 64 bits.
+
+Tolerances are bounds on the kernels' arithmetic, element by element: fp32 sums and products, the documented
+error of the exponentials, the rounding of softmax's numerators and the one of the output (`attend_slack`,
+`rotary_slack`).
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from laya_cuda import attention  # noqa: E402
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+HALF = {name: torch.finfo(t).eps / 2 for name, t in TYPES.items()}
+TINY = {"f32": 2.0 ** -149, "f16": 2.0 ** -25, "bf16": 2.0 ** -134}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("CUDA device required")
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda", dtype=torch.float64)
+
+
+# -------------------------------------------------------------------------------- rotary
+
+def frequencies(dims, theta, scaling, factor, length, low, high):
+    k = torch.arange(dims // 2, dtype=torch.float64)
+    if scaling == "ntk":
+        theta = theta * factor ** (dims / (dims - 2))
+    f = theta ** (-2 * k / dims)
+    if scaling == "linear":
+        f = f / factor
+    if scaling == "parts":
+        keep = ((length * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = f * (keep + (1 - keep) / factor)
+    return f.cuda()
+
+
+def rotate(x, positions, dims, interleaved, f, magnitude, backward):
+    """The definition, and the sum of the magnitudes of each result's two products."""
+    w = positions.double()[:, None, None] * f
+    cos, sin = magnitude * torch.cos(w), magnitude * torch.sin(w) * (-1 if backward else 1)
+    k = torch.arange(dims // 2, device="cuda")
+    first, second = (2 * k, 2 * k + 1) if interleaved else (k, k + dims // 2)
+    out, size = x.double().clone(), x.double().abs()
+    a, b = x[..., first].double(), x[..., second].double()
+    out[..., first], out[..., second] = a * cos - b * sin, a * sin + b * cos
+    size[..., first] = size[..., second] = abs(magnitude) * (a.abs() + b.abs())
+    return out, size
+
+
+def rotary_slack(want, size, dtype):
+    # Cosine and sine: the reduced angle (at most pi) rounded to fp32, the angle itself 2^-24 turns off for far positions, two
+    # units of sincospif: below 2^-20 in all, of |a| + |b|.  Three roundings in fp32, one to the type.
+    return 1.01 * HALF[dtype] * want.abs() + (2.0 ** -20 + 4 * 2.0 ** -24) * size + TINY[dtype]
+
+
+def check_rotary(x, got, positions, dtype, dims, interleaved=False, theta=10000.0, scaling="none", factor=1.0, length=0.0,
+                 low=1.0, high=32.0, magnitude=1.0, backward=False):
+    f = frequencies(dims, theta, scaling, factor, length, low, high)
+    want, size = rotate(x, positions, dims, interleaved, f, magnitude, backward)
+    error = (got.double() - want).abs() - rotary_slack(want, size, dtype)
+    assert error.max().item() <= 0 if error.numel() else True
+    assert torch.equal(got[..., dims:], x[..., dims:])
+
+
+def heads(g, tokens, n, dim, dtype, pad=0, offset=0):
+    """A [tokens][n][dim] view of a wider buffer of sevens."""
+    store = torch.full((tokens * (n * dim + pad) + offset + 16,), 7.0, dtype=TYPES[dtype], device="cuda")
+    view = store[offset: offset + tokens * (n * dim + pad)].view(tokens, n * dim + pad)[:, : n * dim].unflatten(1, (n, dim))
+    view.copy_(randn(g, tokens, n, dim))
+    return view, store
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens,n,n_k,dim,dims", [(1, 12, 12, 64, 64), (3, 1, 1, 2, 2), (77, 16, 4, 80, 32), (33, 5, 1, 40, 20), (130, 3, 2, 128, 128),
+                                                  (9, 2, 2, 96, 50), (300, 32, 8, 128, 64), (2, 2, 1, 600, 512), (1, 1, 1, 7, 6)])
+@pytest.mark.parametrize("pad,offset", [(0, 0), (1, 1), (24, 8)])
+def test_rotary_is_the_definition(dtype, interleaved, tokens, n, n_k, dim, dims, pad, offset):
+    g = generator(tokens * 1000 + dims)
+    (q, q_store), (k, _) = heads(g, tokens, n, dim, dtype, pad, offset), heads(g, tokens, n_k, dim, dtype, pad, offset)
+    positions = torch.randint(0, 5000, (tokens,), generator=g, device="cuda")
+    q_out, k_out = (heads(g, tokens, h, dim, dtype, pad, offset) for h in (n, n_k))
+    kept = q_store.clone()
+    attention.rotary(q, positions, q_out[0], k=k, k_out=k_out[0], dims=dims, interleaved=interleaved)
+    check_rotary(q, q_out[0], positions, dtype, dims, interleaved)
+    check_rotary(k, k_out[0], positions, dtype, dims, interleaved)
+    assert torch.equal(kept, q_store)
+    for view, store in (q_out, k_out):  # what lies between the rows is left as it was
+        view.fill_(7.0)
+        assert bool((store == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dims", [64, 24])
+def test_rotary_in_place_and_one_tensor(dtype, interleaved, dims):
+    g = generator(1)
+    x, _ = heads(g, 50, 6, 64, dtype, 8, 0)
+    before, positions = x.clone(), torch.arange(50, device="cuda", dtype=torch.int32)
+    attention.rotary(x, positions, x, dims=dims, interleaved=interleaved)
+    check_rotary(before, x, positions, dtype, dims, interleaved)
+
+
+@pytest.mark.parametrize("scaling,factor,length,low,high", [("none", 1.0, 0, 1, 32), ("linear", 8.0, 0, 1, 32), ("ntk", 4.0, 0, 1, 32),
+                                                            ("parts", 32.0, 8192, 1.0, 4.0), ("parts", 4.0, 4096, 1.0, 32.0)])
+@pytest.mark.parametrize("integers", [torch.int32, torch.int64])
+def test_rotary_scaled_and_far(scaling, factor, length, low, high, integers):
+    g = generator(2)
+    positions = torch.tensor([0, 1, 4095, 131071, 10 ** 6 + 1, 2 ** 24 + 1, 2 ** 30 + 7, 2 ** 31 - 1], device="cuda", dtype=integers)
+    x, _ = heads(g, len(positions), 3, 128, "f32")
+    out = torch.empty_like(x)
+    how = dict(theta=500000.0, scaling=scaling, factor=factor, length=length, low=low, high=high, magnitude=1.2)
+    attention.rotary(x, positions, out, **how)
+    check_rotary(x, out, positions, "f32", 128, **how)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_backward_is_the_gradient(interleaved):
+    g = generator(3)
+    x, grad = (heads(g, 40, 4, 48, "f32")[0] for _ in range(2))
+    positions = torch.arange(40, device="cuda") * 37
+    how = dict(dims=32, interleaved=interleaved, scaling="linear", factor=3.0, magnitude=1.3)
+    out = torch.empty_like(grad)
+    attention.rotary(grad, positions, out, backward=True, **how)
+    check_rotary(grad, out, positions, "f32", backward=True, **how)
+    leaf = x.double().requires_grad_()
+    f = frequencies(32, 10000.0, "linear", 3.0, 0, 1, 32)
+    w = positions.double()[:, None, None] * f
+    k = torch.arange(16, device="cuda")
+    first, second = (2 * k, 2 * k + 1) if interleaved else (k, k + 16)
+    a, b = leaf[..., first], leaf[..., second]
+    turned = torch.cat([1.3 * (a * w.cos() - b * w.sin()), 1.3 * (a * w.sin() + b * w.cos()), leaf[..., 32:]], -1)
+    order = torch.cat([first, second, torch.arange(32, 48, device="cuda")])
+    turned.backward(grad.double()[..., order])
+    # against the formula's gradient, and against a difference of the operator's own results (it is linear)
+    bound = rotary_slack(leaf.grad, 1.3 * 2 * grad.double().abs().amax(-1, keepdim=True), "f32")
+    assert ((out.double() - leaf.grad).abs() <= bound).all()
+    d = randn(g, *x.shape)
+    moved, still, shifted = torch.empty_like(x), torch.empty_like(x), (x.double() + d).float()
+    attention.rotary(shifted, positions, moved, **how)
+    attention.rotary(x, positions, still, **how)
+    left = ((moved.double() - still.double()) * grad.double()).sum()
+    right = (out.double() * (shifted.double() - x.double())).sum()
+    scale = ((moved.double().abs() + still.double().abs() + shifted.double().abs()) * grad.double().abs()).sum() * 1.3 * 4
+    assert abs(left - right) <= scale * 2.0 ** -19
+
+
+def test_rotary_of_many_tokens():
+    g = generator(4)
+    x, _ = heads(g, 70001, 2, 32, "bf16")
+    out, positions = torch.empty_like(x), torch.arange(70001, device="cuda")
+    attention.rotary(x, positions, out)
+    check_rotary(x, out, positions, "bf16", 32)
+
+
+def test_rotary_keeps_infinities_and_nan_to_their_pairs():
+    g = generator(5)
+    x, _ = heads(g, 4, 2, 64, "bf16")
+    x[1, 0, 3], x[2, 1, 40] = math.nan, math.inf
+    out, positions = torch.empty_like(x), torch.arange(4, device="cuda") + 1
+    attention.rotary(x, positions, out)
+    bad = ~out.isfinite()
+    want = torch.zeros_like(bad)
+    want[1, 0, [3, 35]] = want[2, 1, [8, 40]] = True
+    assert torch.equal(bad, want)
+
+
+# -------------------------------------------------------------------------------- attention: the definition
+
+def see(n, m, causal, left, right, prefix, doc_q, doc_k):
+    p, j = torch.arange(m - n, m, device="cuda")[:, None], torch.arange(m, device="cuda")
+    out = torch.ones(n, m, dtype=torch.bool, device="cuda")
+    if causal:
+        out &= j <= p
+    if left >= 0:
+        out &= j >= p - left
+    if right >= 0:
+        out &= j <= p + right
+    if doc_q is not None:
+        out &= doc_q[:, None] == doc_k[None]
+    return out | (j < prefix)
+
+
+def define(s):
+    """out and lse in 64 bits, and bounds on their errors."""
+    q, k, v, how = s["q"], s["k"], s["v"], s["how"]
+    dtype, h, group = s["dtype"], q.shape[1], q.shape[1] // k.shape[1]
+    dim, cap, scale = q.shape[2], how.get("cap", 0.0), how.get("scale", 1 / math.sqrt(q.shape[2]))
+    left, right = how.get("window") or (-1, -1)
+    out, lse = torch.full(q.shape, math.nan, dtype=torch.float64, device="cuda"), torch.full(q.shape[:2], math.nan, dtype=torch.float64, device="cuda")
+    out_slack, lse_slack = torch.zeros_like(out), torch.zeros_like(lse)
+    k_starts, k_lengths = (s["k_starts"], s["k_lengths"]) if s["k_starts"] is not None else (s["starts"], s["lengths"])
+    for b, (start, n, k_start, m) in enumerate(zip(s["starts"], s["lengths"], k_starts, k_lengths)):
+        if n == 0:
+            continue
+        rows, keys = slice(start, start + n), slice(k_start, k_start + m)
+        doc = how.get("documents")
+        doc_k = how.get("k_documents", doc)
+        visible = see(n, m, how.get("causal", False), left, right, s["prefix"][b] if s["prefix"] else 0,
+                      None if doc is None else doc[rows], None if doc is None else doc_k[keys])
+        p, j = torch.arange(m - n, m, device="cuda")[:, None], torch.arange(m, device="cuda")
+        for head in range(h):
+            qs, ks, vs = q[rows, head].double(), k[keys, head // group].double(), v[keys, head // group].double()
+            x = qs @ ks.T * scale
+            # fp32: the sum of dim exact products (an error of 2^-24 for each addition, of the products' magnitudes), then
+            # a few roundings; the cap is exact to 2^-21 of itself.
+            ds = (dim + 8) * 2.0 ** -24 * (qs.abs() @ ks.abs().T) * abs(scale)
+            if cap:
+                x = cap * torch.tanh(x / cap)
+                ds = ds + cap * 2.0 ** -21
+            if "slopes" in how:
+                bias = -how["slopes"][head].double() * (p - j).abs()
+                x = x + bias
+                ds = ds + 4 * 2.0 ** -24 * bias.abs()
+            if "distance_bias" in how:
+                t = how["distance_bias"][head].double()
+                reach = t.numel() // 2
+                bias = t[(j - p).clamp(-reach, reach) + reach]
+                x = x + bias
+                ds = ds + 4 * 2.0 ** -24 * torch.where(bias.isfinite(), bias.abs(), torch.zeros_like(bias))
+            ds = ds + 8 * 2.0 ** -24 * x.abs()
+            x = torch.where(visible, x, torch.full_like(x, -math.inf))
+            top = x.amax(1, keepdim=True) if m else torch.full((n, 1), -math.inf, dtype=torch.float64, device="cuda")
+            empty = top == -math.inf
+            e = torch.exp(x - torch.where(empty, torch.zeros_like(top), top))
+            total = e.sum(1, keepdim=True)
+            w = e / torch.where(empty, torch.ones_like(total), total)
+            vs = torch.where(visible.any(0)[:, None], vs, torch.zeros_like(vs)) if m else vs
+            # a hidden value that is not finite has no part in the sum
+            clean = torch.where(vs.isfinite(), vs, torch.zeros_like(vs))
+            y = w @ clean
+            poison = (visible & (w > 0)).double() @ (~vs.isfinite()).double() > 0
+            out[rows, head] = torch.where(poison, torch.full_like(y, math.nan), y)
+            lse[rows, head] = torch.where(empty, top, top + torch.log(torch.where(empty, torch.ones_like(total), total))).squeeze(1)
+            ds = torch.where(visible & x.isfinite(), ds, torch.zeros_like(ds))
+            # Each weight is off by its score's error, the exponential's 2^-13 and one rounding to the type, numerator only; below the
+            # smallest numbers of the type by 2^-32 of the largest (float16).  fp32 sums over m keys.
+            rel = HALF[dtype] + 2.0 ** -12 + (m / 16 + 64) * 2.0 ** -24
+            spread = (w * ds).sum(1, keepdim=True)
+            out_slack[rows, head] = ((w * ds) @ clean.abs() + (rel + spread) * (w @ clean.abs()) + 2.0 ** -31 * clean.abs().sum(0)
+                                     + 1.01 * HALF[dtype] * y.abs() + TINY[dtype])
+            lse_slack[rows, head] = (spread.squeeze(1) + 2.0 ** -12 + (m / 16 + 64) * 2.0 ** -24
+                                     + 4 * 2.0 ** -24 * torch.where(empty, torch.zeros_like(top), top.abs() + 1).squeeze(1))
+    return out, lse, out_slack, lse_slack
+
+
+def problem(seed, queries, keys=None, heads=4, kv_heads=2, dim=64, dtype="bf16", gap=0, room=0, prefix=None, **how):
+    """`keys` None: self-attention on slices of one buffer; else a cache, `room` rows more than keys apart."""
+    g = generator(seed)
+    s = {"dtype": dtype, "how": how, "prefix": prefix, "lengths": queries, "k_starts": None, "k_lengths": None}
+    s["starts"] = [gap + sum(queries[:b]) + gap * b for b in range(len(queries))]
+    rows = sum(queries) + gap * (len(queries) + 1)
+    if keys is None:
+        packed = randn(g, rows, heads + 2 * kv_heads, dim).to(TYPES[dtype])
+        s["q"], s["k"], s["v"] = packed[:, :heads], packed[:, heads: heads + kv_heads], packed[:, heads + kv_heads:]
+    else:
+        s["q"] = randn(g, rows, heads, dim).to(TYPES[dtype])
+        s["k_lengths"] = keys
+        s["k_starts"] = [sum(keys[:b]) + room * b for b in range(len(keys))]
+        s["k"], s["v"] = (randn(g, sum(keys) + room * len(keys), kv_heads, dim).to(TYPES[dtype]) for _ in range(2))
+    s["q"] *= 1.5
+    return s
+
+
+def run(s, out=None, lse=None, **other):
+    out = torch.full(s["q"].shape, 7.0, dtype=s["q"].dtype, device="cuda") if out is None else out
+    lse = torch.full(s["q"].shape[:2], 7.0, device="cuda") if lse is None else lse
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    k = {} if s["k_starts"] is None else {"k_starts": ints(s["k_starts"]), "k_lengths": ints(s["k_lengths"])}
+    if s["prefix"]:
+        k["prefix"] = ints(s["prefix"])
+    k.setdefault("max_queries", max(s["lengths"], default=0))
+    k.setdefault("max_keys", max(s["k_lengths"] if s["k_lengths"] is not None else s["lengths"], default=0))
+    attention.attend(s["q"], s["k"], s["v"], out, ints(s["starts"]), ints(s["lengths"]), lse=lse, err=err, **{**k, **s["how"], **other})
+    assert err.item() == 0
+    return out, lse
+
+
+def check(s, got=None):
+    out, lse = got or run(s)
+    want, want_lse, slack, lse_slack = define(s)
+    mine = ~want_lse.isnan()  # rows of a sequence
+    assert bool((out[~mine] == 7.0).all()) and bool((lse[~mine] == 7.0).all()), "rows outside the sequences were written"
+    want, got = want[mine], out[mine].double()
+    assert torch.equal(want.isnan(), ~got.isfinite() | want.isnan() & got.isnan())
+    error = torch.where(want.isnan(), torch.zeros_like(want), (got - want).abs() - slack[mine])
+    assert error.numel() == 0 or error.max().item() <= 0, (error.max().item(), int((error > 0).sum()), error.numel())
+    nothing = want_lse[mine] == -math.inf
+    assert torch.equal(lse[mine] == -math.inf, nothing)
+    assert not got[nothing].any()
+    error = torch.where(nothing, torch.zeros_like(want_lse[mine]), (lse[mine].double() - want_lse[mine]).abs() - lse_slack[mine])
+    error = error[~error.isnan()]
+    assert error.numel() == 0 or error.max().item() <= 0, error.max().item()
+    return out, lse
+
+
+# -------------------------------------------------------------------------------- attention: sizes, layouts, types
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(12, 12, 64), (4, 2, 128), (6, 2, 96), (7, 1, 72), (8, 1, 8), (3, 3, 40), (16, 1, 128), (128, 1, 16), (5, 5, 120)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_self_attention(dtype, heads, kv_heads, dim, causal):
+    check(problem(dim, [1, 300, 7, 128, 129, 64], heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype, causal=causal))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(12, 12, 64), (32, 8, 128), (7, 1, 80), (16, 1, 96), (1, 1, 128), (130, 65, 64)])
+@pytest.mark.parametrize("queries,keys", [([1], [1]), ([1], [77]), ([1, 1, 1], [1, 128, 1000]), ([5, 1, 3], [5, 129, 2049]), ([24, 200], [4099, 700]),
+                                          ([1], [20000]), ([1] * 40, [300 + 7 * b for b in range(40)])])
+def test_a_cache(dtype, heads, kv_heads, dim, queries, keys):
+    check(problem(len(queries), queries, keys, heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype, room=5, causal=True))
+
+
+@pytest.mark.parametrize("queries,keys", [([0], [5]), ([3], [0]), ([0, 4, 0], [0, 9, 3]), ([9], [4]), ([300], [20]), ([200, 3], [100, 0]), ([], [])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_empty_and_short_key_sequences(queries, keys, causal):
+    check(problem(3, queries, keys, causal=causal, room=2, gap=1))
+
+
+def test_no_keys_at_all():
+    s = problem(3, [3, 200], [0, 0])
+    assert s["k"].shape[0] == 0
+    check(s)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_between_and_behind_the_sequences_are_left(dim):
+    check(problem(4, [130, 5, 260], gap=3, dim=dim, causal=True))
+
+
+@pytest.mark.parametrize("dim", [64, 96])
+def test_layouts(dim):
+    """Heads outermost, rows of a wider buffer, and an `out` inside one."""
+    s = problem(5, [200, 31], heads=4, kv_heads=4, dim=dim, causal=True)
+    for name in ("q", "k", "v"):
+        t = s[name]
+        wide = torch.full((t.shape[1] + 1, t.shape[0], dim + 8), 3.0, dtype=t.dtype, device="cuda")
+        wide[:-1, :, :dim] = t.transpose(0, 1)
+        s[name] = wide[:-1, :, :dim].transpose(0, 1)
+    store = torch.full((s["q"].shape[0], 6, dim + 16), 7.0, dtype=s["q"].dtype, device="cuda")
+    out = store[:, 1:5, 8: dim + 8]
+    check(s, run(s, out=out))
+    out.fill_(7.0)
+    assert bool((store == 7.0).all())
+
+
+def test_bounds_above_and_below_the_lengths():
+    s = problem(6, [40, 300], causal=True)
+    want = run(s)
+    for bounds in (dict(max_queries=340, max_keys=340), dict(max_queries=10 ** 6, max_keys=10 ** 6), dict(max_queries=None, max_keys=None)):
+        got = run(s, **bounds)
+        check(s, got)
+    # Queries past max_queries are not computed.
+    out, lse = run(s, max_queries=100)
+    assert torch.equal(out[:140], want[0][:140]) and bool((out[140:] == 7.0).all()) and bool((lse[140:] == 7.0).all())
+    # max_keys only shapes the launch.
+    check(s, run(s, max_keys=3))
+
+
+def test_offsets_past_32_bits():
+    """Keys and values of a cache whose later sequences start more than 2^32 bytes in, and 2^31 values."""
+    rows, dim, kv = 2 ** 31 // (128 * 4) + 5000, 128, 4
+    k, v = (torch.zeros(rows, kv, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    s = problem(7, [1, 1, 6], [4000, 77, 900], heads=8, kv_heads=kv, dim=dim, causal=True)
+    at = [rows - 4000, 10, rows - 4900]
+    for b, (start, m) in enumerate(zip(s["k_starts"], s["k_lengths"])):
+        k[at[b]: at[b] + m], v[at[b]: at[b] + m] = s["k"][start: start + m], s["v"][start: start + m]
+    s["k"], s["v"], s["k_starts"] = k, v, at
+    check(s)
+
+
+# -------------------------------------------------------------------------------- attention: masks, caps, biases
+
+def documents(lengths, mean, seed, order=False):
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for n in lengths:
+        ids = torch.cumsum((torch.rand(n, generator=g) < 1 / mean).long(), 0)
+        out.append(ids if not order else torch.randint(0, 3, (n,), generator=g))
+    return torch.cat(out).to(torch.int32).cuda()
+
+
+MASKS = [dict(), dict(causal=True), dict(window=(0, 0)), dict(window=(17, 100)), dict(window=(-1, 3)), dict(window=(64, -1)), dict(causal=True, window=(200, -1)),
+         dict(causal=True, window=(-1, 5))]
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("prefix", [None, [1, 100, 5, 400]])
+@pytest.mark.parametrize("doc", ["none", "runs", "mixed"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_masks(mask, prefix, doc, dim):
+    lengths = [260, 515, 1, 390]
+    if doc != "none":
+        mask = {**mask, "documents": documents(lengths, 60, 1, doc == "mixed")}
+    check(problem(8, lengths, heads=3, kv_heads=1, dim=dim, prefix=prefix, **mask))
+
+
+@pytest.mark.parametrize("doc", [None, 40])
+@pytest.mark.parametrize("mask", [dict(causal=True), dict(window=(100, 20)), dict()])
+@pytest.mark.parametrize("queries", [[2, 1, 7], [150, 1, 64]])
+def test_masks_over_a_cache(mask, doc, queries):
+    keys = [300, 4000, 1290]
+    if doc:
+        k_documents = documents(keys, doc, 2)
+        starts = [0, 300, 4300]
+        mask = {**mask, "k_documents": k_documents, "documents": torch.cat([k_documents[a + m - n: a + m] for a, m, n in zip(starts, keys, queries)])}
+    check(problem(9, queries, keys, heads=8, kv_heads=2, dim=128, prefix=[20, 1000, 0], **mask))
+
+
+BIASES = [dict(cap=30.0), dict(cap=0.5), dict(slopes=True), dict(distance_bias=128), dict(distance_bias=0), dict(distance_bias=1000), dict(cap=20.0, slopes=True),
+          dict(cap=50.0, distance_bias=16)]
+
+
+def with_bias(how, heads, seed=0):
+    how = dict(how)
+    if "slopes" in how:
+        how["slopes"] = torch.exp2(-8 * torch.arange(1, heads + 1, device="cuda") / heads)
+    if "distance_bias" in how:
+        how["distance_bias"] = randn(generator(seed), heads, 2 * how["distance_bias"] + 1).float()
+    return how
+
+
+@pytest.mark.parametrize("how", BIASES)
+@pytest.mark.parametrize("mask", [dict(), dict(causal=True), dict(window=(90, 40))])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 64), (6, 2, 128)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_caps_and_biases(how, mask, heads, kv_heads, dim, dtype):
+    check(problem(10, [300, 17, 1], heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype, **with_bias(how, heads), **mask))
+
+
+@pytest.mark.parametrize("how", BIASES)
+@pytest.mark.parametrize("queries", [[1, 3], [20, 130]])
+def test_caps_and_biases_over_a_cache(how, queries):
+    check(problem(11, queries, [900, 2500], heads=14, kv_heads=2, dim=64, **with_bias(how, 14), causal=True))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+@pytest.mark.parametrize("cap", [0.0, 25.0])
+def test_scales(dtype, scale, cap):
+    """A scale of zero, a negative one, and one that makes single keys take all the weight."""
+    check(problem(12, [200, 50], dim=64, dtype=dtype, scale=scale, cap=cap, causal=True))
+
+
+@pytest.mark.parametrize("value", [-math.inf, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("queries,keys", [([300], None), ([1, 3], [700, 200])])
+def test_biases_that_mask(value, queries, keys):
+    """Distances ruled out by the bias; with the type's lowest value everywhere the weights are equal."""
+    table = torch.zeros(4, 101, device="cuda")
+    table[0, :] = value
+    table[1, 40:60] = value
+    table[2, 0] = table[2, -1] = value
+    check(problem(13, queries, keys, heads=4, kv_heads=2, distance_bias=table))
+
+
+def test_scores_rising_and_falling_along_the_keys():
+    """The running maximum is passed again and again, by much and by little."""
+    for sign in (1, -1):
+        s = problem(14, [150, 1], [3000, 2500], heads=4, kv_heads=2, dim=64, dtype="f16")
+        ramp = torch.linspace(-1, 1, 5500, device="cuda", dtype=torch.float64)
+        s["q"] = (s["q"].double() * 0.1 + 1).half()
+        s["k"] = (s["k"].double() * 0.1 + sign * 4 * ramp[:, None, None]).half()
+        check(s)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_hidden_keys_may_hold_anything(bad, dim):
+    """Rows outside the sequences, a cache's unused rows, and keys that a mask hides from some queries."""
+    s = problem(15, [3, 200], [150, 420], heads=4, kv_heads=2, dim=dim, room=64, gap=2, causal=True)
+    for name in ("k", "v"):
+        t = s[name]
+        for start, m in zip(s["k_starts"], s["k_lengths"]):
+            t[start + m: start + m + 64] = bad
+    check(s)
+    out, lse = run(s)
+    assert bool(out[s["starts"][1]: s["starts"][1] + 200].isfinite().all())
+    s["v"][s["k_starts"][1] + 300, 1, 5] = bad  # seen by queries 80 and on of the second sequence
+    check(s)
+    lengths = [260, 300]
+    s = problem(16, lengths, heads=4, kv_heads=4, dim=dim, documents=documents(lengths, 50, 3))
+    hit = s["how"]["documents"][:260] == s["how"]["documents"][100]
+    s["v"][:260][hit] = bad
+    s["k"][:260][hit] = bad
+    s["how"]["documents"] = s["how"]["documents"].clone()
+    out, lse = run(s)
+    clean = torch.ones(sum(lengths), dtype=torch.bool, device="cuda")
+    clean[:260] = ~hit
+    assert bool(out[clean].isfinite().all()) and bool(lse[clean].isfinite().all())
+    want = problem(16, lengths, heads=4, kv_heads=4, dim=dim, documents=s["how"]["documents"])
+    exact, _, slack, _ = define(want)
+    assert ((out[clean].double() - exact[clean]).abs() <= slack[clean]).all()
+
+
+# -------------------------------------------------------------------------------- attention: calls
+
+@pytest.mark.parametrize("queries,keys", [([300, 200], None), ([1, 1], [9000, 300])])
+def test_the_same_each_time(queries, keys):
+    s = problem(17, queries, keys, heads=16, kv_heads=4, dim=128, causal=True, cap=40.0)
+    first = run(s)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, run(s)))
+
+
+def test_sequences_outside_the_tensors_are_reported_and_skipped():
+    s = problem(18, [40, 50, 60], [100, 200, 300], causal=True, dim=64)
+    want, _ = run(s)
+    for name, at, value in (("starts", 1, -1), ("lengths", 1, 2 ** 30), ("k_starts", 1, 550), ("k_lengths", 1, -4), ("k_lengths", 1, 2 ** 31 - 1)):
+        fields = {n: list(s[n]) for n in ("starts", "lengths", "k_starts", "k_lengths")}
+        fields[name][at] = value
+        out, err = torch.full_like(want, 7.0), torch.zeros(1, dtype=torch.int32, device="cuda")
+        attention.attend(s["q"], s["k"], s["v"], out, ints(fields["starts"]), ints(fields["lengths"]), ints(fields["k_starts"]),
+                         ints(fields["k_lengths"]), causal=True, err=err)
+        assert err.item() == 4
+        assert torch.equal(out[:40], want[:40]) and torch.equal(out[90:], want[90:]) and bool((out[40:90] == 7.0).all())
+
+
+def test_streams_and_a_captured_graph_with_new_lengths():
+    s = problem(19, [1, 1], [5000, 3000], heads=8, kv_heads=2, dim=128, causal=True)
+    starts, lengths, k_starts, k_lengths = (ints(s[n]) for n in ("starts", "lengths", "k_starts", "k_lengths"))
+    positions = torch.tensor([4999, 2999], device="cuda")
+    q, out = torch.empty_like(s["q"]), torch.empty_like(s["q"])
+
+    def step():
+        attention.rotary(s["q"], positions, q)
+        attention.attend(q, s["k"], s["v"], out, starts, lengths, k_starts, k_lengths, max_queries=1, max_keys=5000, causal=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    eager = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    out.zero_()
+    graph.replay()
+    assert torch.equal(out, eager)
+    k_lengths.copy_(ints([1200, 2]))
+    positions.copy_(torch.tensor([1199, 1], device="cuda"))
+    graph.replay()
+    replayed = out.clone()
+    step()
+    assert torch.equal(out, replayed)
+    turned = {**s, "q": q, "k_lengths": [1200, 2]}
+    want, _, slack, _ = define(turned)
+    assert ((replayed.double() - want).abs() <= slack).all()
+
+
+def test_two_calls_at_once():
+    problems = [problem(20 + i, [700, 300], heads=8, kv_heads=4, dim=64, causal=True) for i in range(2)]
+    want = [run(s) for s in problems]
+    streams = [torch.cuda.Stream() for _ in problems]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for s, stream in zip(problems, streams):
+            with torch.cuda.stream(stream):
+                got.append(run(s))
+    torch.cuda.synchronize()
+    for i, (out, lse) in enumerate(got):
+        assert torch.equal(out, want[i % 2][0]) and torch.equal(lse, want[i % 2][1])
+
+
+def test_pieces_join_by_their_logarithms():
+    """A shared prefix and the rest of the keys, attended apart, give the whole."""
+    s = problem(22, [30], [1000], heads=4, kv_heads=2, dim=64)
+    want, _, slack, _ = define(s)
+    parts = []
+    for first, last in ((0, 333), (333, 1000)):
+        parts.append(run({**s, "k_starts": [first], "k_lengths": [last - first]}))
+    lse = torch.stack([p[1].double() for p in parts])
+    w = torch.softmax(lse, 0)[..., None]
+    joined = sum(wi * p[0].double() for wi, p in zip(w, parts))
+    # Each part within its own bound, which the weights mix; the weights are off by the logarithms' errors.
+    assert ((joined - want).abs() <= 3 * slack + 2.0 ** -10 * want.abs() + 2.0 ** -11).all()
