@@ -36,6 +36,74 @@ void check_vectors(const char* what, const void* p, int tokens, int heads, int d
   if (*token >= (1ll << 38) || *head >= (1ll << 38)) fail(LAYA_ERR_INVALID, "%s: a stride is too large", what);
 }
 
+template <typename F>
+void with_half(int dtype, F f) {
+  if (dtype == LAYA_DTYPE_F16) f((__half*)nullptr);
+  else f((__nv_bfloat16*)nullptr);
+}
+
+// A tensor [tokens][heads][dim] of 16-bit values in boxes of 64 values x box_heads x box_tokens, 128-byte swizzle.  Values past
+// dim and rows past the last read as zeros.
+CUtensorMap heads_map(bool bf16, const void* p, int dim, int heads, int tokens, int64_t head, int64_t token, int box_heads, int box_tokens) {
+  CUtensorMap map;
+  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)token * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = encode_fn()(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(p), dims, strides,
+                           box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) fail(LAYA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return map;
+}
+
+template <typename T, int DP, bool kGeneral>
+void launch_attend_kernel(const AttendArgs& a, const AttendMaps& maps, int64_t ctas, int dev, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  auto kern = attend_kernel<T, DP, kGeneral>;
+  allow_smem(kern, AttendCfg<DP>::kBytes, dev, done);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kAtThreads);
+  cfg.dynamicSmemBytes = AttendCfg<DP>::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (a.splits > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = a.splits;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  CK(cudaLaunchKernelEx(&cfg, kern, maps, a));
+}
+
+template <typename T, int DP>
+void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  const int per_tile = kAtRows / a.group;
+  a.pairs = (a.max_queries + 2 * per_tile - 1) / (2 * per_tile);
+  const int64_t items = (int64_t)a.pairs * a.sequences * a.kv_heads;
+  const int blocks = (max_keys + kAtKeys - 1) / kAtKeys, sms = sm_count(dev);
+  a.splits = 1;
+  while (a.splits < 8 && items * a.splits * 2 <= sms && a.splits * 4 <= blocks) a.splits *= 2;
+  if (items * a.splits > INT32_MAX) fail(LAYA_ERR_INVALID, "%d queries of %d sequences and %d heads are too many for one call", a.max_queries, a.sequences, a.heads);
+  AttendMaps maps;
+  maps.q = heads_map(kBf16, a.q, a.dim, a.heads, a.q_tokens, a.q_head, a.q_token, a.group, per_tile);
+  // Without a key there is nothing to load: any map will do.
+  maps.k = a.k_tokens ? heads_map(kBf16, a.k, a.dim, a.kv_heads, a.k_tokens, a.k_head, a.k_token, 1, kAtKeys) : maps.q;
+  maps.v = a.k_tokens ? heads_map(kBf16, a.v, a.dim, a.kv_heads, a.k_tokens, a.v_head, a.v_token, 1, kAtKeys) : maps.q;
+  if (a.cap > 0.f || a.slopes || a.table || !(a.scale > 0.f)) launch_attend_kernel<T, DP, true>(a, maps, items * a.splits, dev, st);
+  else launch_attend_kernel<T, DP, false>(a, maps, items * a.splits, dev, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -139,9 +207,12 @@ int laya_op_attend(const laya_attend* p, int* err, void* stream) {
   a.err = err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   current_device(st);
-  const dim3 grid((a.max_queries + 3) / 4, a.heads, a.sequences);
-  if (p->dtype == LAYA_DTYPE_F16) launch_k(attend_rows_kernel<__half>, grid, dim3(128), 0, st, a);
-  else launch_k(attend_rows_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, a);
+  a.wait_ns = wait_ns();
+  with_half(p->dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (a.dim > 64) launch_attend<T, 128>(a, std::min(p->max_keys, p->k_tokens), current_device(st), st);
+    else launch_attend<T, 64>(a, std::min(p->max_keys, p->k_tokens), current_device(st), st);
+  });
   OP_API_END
 }
 

@@ -43,6 +43,17 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 
 __device__ __forceinline__ bool elect_one_lane() { return (threadIdx.x & 31) == 0; }
 
+// One thread of a converged warp.  Instructions that take uniform registers (tcgen05.*, TMA) are
+// issued under this predicate, which the compiler knows to leave one thread: under a test of the
+// lane's number it serialises each of them over the active lanes (measured in the pair kernel: 575
+// cycles to issue a k-block's 3 scale copies, 4 MMAs and 2 commits, and 1,000 cycles a k-block
+// in all against 512 of MMA time).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t leader;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+  return leader != 0;
+}
+
 // ---------------------------------------------------------------------------------------------
 // mbarrier
 // ---------------------------------------------------------------------------------------------

@@ -13,17 +13,6 @@ namespace laya {
 constexpr int kMxBK = 128;                 // columns of K per stage, one scale tile
 constexpr int kMxOperandBytes = 128 * kMxBK;
 
-// One thread of a converged warp.  Instructions that take uniform registers (tcgen05.*, TMA) are
-// issued under this predicate, which the compiler knows to leave one thread: under a test of the
-// lane's number it serialises each of them over the active lanes (measured in the pair kernel: 575
-// cycles to issue a k-block's 3 scale copies, 4 MMAs and 2 commits, and 1,000 cycles a k-block
-// in all against 512 of MMA time).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t leader;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(leader));
-  return leader != 0;
-}
-
 // mbar_wait for a converged warp, with the same answer in every lane.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code, volatile int* abort,
                                           unsigned long long limit_ns) {

@@ -363,13 +363,14 @@ def test_layouts(dim):
 
 def test_bounds_above_and_below_the_lengths():
     s = problem(6, [40, 300], causal=True)
-    want = run(s)
     for bounds in (dict(max_queries=340, max_keys=340), dict(max_queries=10 ** 6, max_keys=10 ** 6), dict(max_queries=None, max_keys=None)):
         got = run(s, **bounds)
         check(s, got)
     # Queries past max_queries are not computed.
     out, lse = run(s, max_queries=100)
-    assert torch.equal(out[:140], want[0][:140]) and bool((out[140:] == 7.0).all()) and bool((lse[140:] == 7.0).all())
+    want, want_lse, slack, lse_slack = define(s)
+    assert ((out[:140].double() - want[:140]).abs() <= slack[:140]).all() and ((lse[:140].double() - want_lse[:140]).abs() <= lse_slack[:140]).all()
+    assert bool((out[140:] == 7.0).all()) and bool((lse[140:] == 7.0).all())
     # max_keys only shapes the launch.
     check(s, run(s, max_keys=3))
 
@@ -521,7 +522,7 @@ def test_the_same_each_time(queries, keys):
 
 def test_sequences_outside_the_tensors_are_reported_and_skipped():
     s = problem(18, [40, 50, 60], [100, 200, 300], causal=True, dim=64)
-    want, _ = run(s)
+    want, _ = run(s, max_queries=None, max_keys=None)  # the bounds decide how the keys are split, and so the last bits
     for name, at, value in (("starts", 1, -1), ("lengths", 1, 2 ** 30), ("k_starts", 1, 550), ("k_lengths", 1, -4), ("k_lengths", 1, 2 ** 31 - 1)):
         fields = {n: list(s[n]) for n in ("starts", "lengths", "k_starts", "k_lengths")}
         fields[name][at] = value
