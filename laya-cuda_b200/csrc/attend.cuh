@@ -108,36 +108,44 @@ __device__ void attend_row(const AttendArgs& a, const AttendSequence& s, int ful
 
 // ---------------------------------------------------------------------------------------------
 // The kernel: a CTA takes two tiles of 128 rows, a row being one query of one head of a kv head's group, and walks the keys in
-// blocks of 128.
+// steps of 128.
 //
-// Warps 0-3 are the softmax of tile 0, warps 4-7 of tile 1 (a thread per row, warp w owning TMEM lanes 32 (w % 4) on), warp 8
-// issues the tensor products, warp 9 finds the blocks that the masks leave and loads them.  TMEM: S of each tile (128 columns
-// each; P, 16-bit, over its first 64), O of each.  The tensor core runs the products in issue order, so O_t += P_t V of a block
-// and then S_t = Q_t K^T of the next are issued together as soon as P_t is there, and while tile 0's softmax works on its S
-// the tensor core has tile 1's products to do.
+// Warps 0-3 are the softmax of tile 0, warps 4-7 of tile 1 (a thread per row, warp w owning TMEM lanes 32 (w % 4) on); of the others one
+// issues the tensor products, and one finds the steps that the masks leave and loads them.  TMEM: S of each tile (128 columns),
+// O of each; P goes over S as 16-bit pairs.  The tensor core runs the products in issue order, so O += P V of a step and then S = Q K^T
+// of the next are issued together as soon as P is there, and the other tile's softmax hides them.
+//
+// Where one tile holds all rows (single tokens over a cache), both tiles take them, and each every other step; the two parts
+// are joined at the end as the parts of a split are.
 // ---------------------------------------------------------------------------------------------
 constexpr int kAtRows = 128;       // rows of a tile
-constexpr int kAtKeys = 128;       // keys of a block
-constexpr int kAtThreads = 320;
-constexpr int kAtInfo = 4;         // blocks announced ahead
+constexpr int kAtKeys = 128;       // keys of a step
+constexpr int kAtSoftmax = 8;       // softmax warps
+constexpr int kAtThreads = 32 * (kAtSoftmax + 4);
+constexpr int kAtMmaWarp = kAtSoftmax, kAtLoadWarp = kAtSoftmax + 1;
+constexpr int kAtInfo = 4;         // steps announced ahead
 constexpr float kAtRescale = 8.f;  // O is rescaled when a row's maximum has grown by more than 2^8
 enum AtClass : int { kAtEnd = -1, kAtSkip = 0, kAtMasked = 1, kAtFull = 2 };
+// What is done to the scores: nothing, a cap, slopes (of these three in log2 units, a scale above zero), or all else, in natural units (log2e
+// times the lowest number of a type would be -infinity).
+enum AtMode { kAtPlain, kAtCap, kAtSlopes, kAtGeneral };
 
 template <int DP>
 struct AttendCfg {
   static_assert(DP == 64 || DP == 128, "padded head size");
-  static constexpr int kSlots = DP == 128 ? 4 : 8;       // K and V blocks in flight
-  static constexpr int kTile = kAtKeys * DP * 2;         // a K or V block, and a tile of Q
-  static constexpr int kHalf = kAtKeys * 128;            // [128 rows][64 values]
-  static constexpr int kOffQ = 0, kOffRing = 2 * kTile;
-  static constexpr int kOffDocs = kOffRing + kSlots * kTile;
+  static constexpr int kTmemO = 256;                     // column of O of tile 0
+  static constexpr int kSlots = DP == 128 ? 2 : 4;       // K tiles in flight, and V tiles
+  static constexpr int kQTile = kAtRows * DP * 2, kQHalf = kAtRows * 128;  // halves: [rows][64 values]
+  static constexpr int kTile = kAtKeys * DP * 2, kHalf = kAtKeys * 128;
+  static constexpr int kOffQ = 0, kOffK = 2 * kQTile, kOffV = kOffK + kSlots * kTile;
+  static constexpr int kOffDocs = kOffV + kSlots * kTile;
   static constexpr int kOffBar = kOffDocs + kAtInfo * kAtKeys * 4;
-  static constexpr int kBars = 2 + 2 * kSlots + 2 * kAtInfo + 2 + 2 + 2 + 1;
+  static constexpr int kBars = 2 + 4 * kSlots + 2 * kAtInfo + 6;
   static constexpr int kOffInfo = kOffBar + kBars * 8;
   static constexpr int kOffSums = kOffInfo + kAtInfo * 4 + 16;  // (maximum, sum) of each row, for a split
   static constexpr int kBytes = kOffSums + 2 * kAtRows * 8 + 1024;
   static_assert(kOffSums % 8 == 0, "alignment");
-  static_assert(2 * kAtRows * DP * 4 <= kSlots * kTile, "a split's O fits the ring");
+  static_assert(2 * kAtRows * DP * 4 <= 2 * kSlots * kTile, "a split's O fits the K and V tiles");
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
@@ -185,19 +193,46 @@ __device__ __forceinline__ AttendSpan attend_span(const AttendArgs& a, int p, in
   return s;
 }
 
-// T, the padded head size, and whether scores get a cap or a bias (kGeneral: natural units, any scale).
-template <typename T, int DP, bool kGeneral>
+// out tanh(in s) for a raw product s, with out in some unit.
+//   near  for |in s| <= 0.75: s times a polynomial in s^2 by the Remez exchange algorithm, on the FMA pipe; off by 2.5e-7 out
+//   any   out - 2 out / (exp(2 in s) + 1) on the special-function unit; off by 2^-21 out
+struct CapTerms {
+  float in, out, c[5], most;  // most: the largest |s| for `near`
+  __device__ __forceinline__ CapTerms(float in_, float out_) : in(in_), out(out_) {
+    constexpr float kC[5] = {0.999997258f, -0.333231002f, 0.132262245f, -0.0492833108f, 0.0123209562f};
+    float power = out * in;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) { c[i] = kC[i] * power; power *= in * in; }
+    // Powers of `in` up to the ninth, and of s, stay in range.
+    most = fabsf(in) > 1e-3f && fabsf(in) < 1e3f ? 0.75f / fabsf(in) : -1.f;
+  }
+  __device__ __forceinline__ float2 slope(float2 s) const {  // out tanh(in s) / s
+    const float2 z = mul2(s, s);
+    float2 p = fma2(make_float2(c[4], c[4]), z, make_float2(c[3], c[3]));
+#pragma unroll
+    for (int i = 2; i >= 0; --i) p = fma2(p, z, make_float2(c[i], c[i]));
+    return p;
+  }
+  __device__ __forceinline__ float any(float s) const {
+    return fmaf(-2.f * out, rcp_approx(ex2_approx(s * (in * 2.8853900817779268f)) + 1.f), out);
+  }
+};
+
+// T, the padded head size, and what is done to the scores.
+template <typename T, int DP, int kMode>
 __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_constant__ AttendMaps maps, const __grid_constant__ AttendArgs a) {
   using Cfg = AttendCfg<DP>;
-  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kSlots = Cfg::kSlots;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value, kGeneral = kMode == kAtGeneral;
+  constexpr float kUnit = kGeneral ? 1.f : 1.4426950408889634f;  // of the scores: natural, or log2
   constexpr float kLog2e = 1.4426950408889634f;
   // float16 numerators end at 2^-24: they are kept 2^7 larger, so that weights down to 2^-31 of the largest count.
   constexpr float kShift = kBf16 ? 0.f : 7.f;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
-  uint64_t *q_full = bar, *full = bar + 2, *empty = full + Cfg::kSlots, *info_full = empty + Cfg::kSlots, *info_empty = info_full + kAtInfo,
-           *s_full = info_empty + kAtInfo, *p_full = s_full + 2, *o_full = p_full + 2, *drain = o_full + 2;
+  uint64_t *q_full = bar, *k_full = bar + 2, *k_empty = k_full + kSlots, *v_full = k_empty + kSlots, *v_empty = v_full + kSlots,
+           *info_full = v_empty + kSlots, *info_empty = info_full + kAtInfo, *s_full = info_empty + kAtInfo, *p_full = s_full + 2, *drain = p_full + 2;
   volatile int* info = reinterpret_cast<volatile int*>(smem + Cfg::kOffInfo);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffInfo + kAtInfo * 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -207,15 +242,19 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
   const unsigned long long wait_ns = wait_limit(a.wait_ns);
 
   if (threadIdx.x == 0) {
-    for (int t = 0; t < 2; ++t) { mbar_init(q_full + t, 1); mbar_init(s_full + t, 1); mbar_init(p_full + t, 4); mbar_init(o_full + t, 1); }
-    for (int i = 0; i < Cfg::kSlots; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-    for (int i = 0; i < kAtInfo; ++i) { mbar_init(info_full + i, 1); mbar_init(info_empty + i, 9); }
-    mbar_init(drain, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(q_full + t, 1);
+      mbar_init(s_full + t, 1);
+      mbar_init(p_full + t, 4);
+      mbar_init(drain + t, 1);
+    }
+    for (int i = 0; i < kSlots; ++i) { mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1); }
+    for (int i = 0; i < kAtInfo; ++i) { mbar_init(info_full + i, 1); mbar_init(info_empty + i, kAtSoftmax + 1); }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
-  if (warp == 9 && lane == 0) { tma_prefetch_desc(&maps.q); tma_prefetch_desc(&maps.k); tma_prefetch_desc(&maps.v); }
+  if (warp == kAtMmaWarp) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (warp == kAtLoadWarp && lane == 0) { tma_prefetch_desc(&maps.q); tma_prefetch_desc(&maps.k); tma_prefetch_desc(&maps.v); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -234,360 +273,274 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
   const int offset = s.keys - all_queries;  // a query's position less its number
   const int per_tile = kAtRows / a.group, first = 2 * pair * per_tile;
   const int tokens[2] = {max(0, min(per_tile, s.queries - first)), max(0, min(per_tile, s.queries - first - per_tile))};
-  const bool idle = tokens[0] == 0;  // of all CTAs of the cluster alike
-  const int nk = (a.dim + 15) / 16;  // steps of 16 values
+  const bool idle = tokens[0] == 0, few = tokens[1] == 0;  // of all CTAs of the cluster alike
+  const int nk = (a.dim + 15) / 16;  // depth steps of 16 values
   const int halves = a.dim > 64 ? 2 : 1;
 
-  if (!idle && warp == 9) {
-    // ---- blocks and loads
-    int doc_lo[2] = {INT_MAX, INT_MAX}, doc_hi[2] = {INT_MIN, INT_MIN};
-    if (a.documents)
-      for (int t = 0; t < 2; ++t) {
-        for (int i = lane; i < tokens[t]; i += 32) {
-          const int d = a.documents[s.q_start + first + t * per_tile + i];
-          doc_lo[t] = min(doc_lo[t], d);
-          doc_hi[t] = max(doc_hi[t], d);
-        }
-        doc_lo[t] = __reduce_min_sync(0xffffffffu, doc_lo[t]);
-        doc_hi[t] = __reduce_max_sync(0xffffffffu, doc_hi[t]);
-      }
-    if (elect_one())
-      for (int t = 0; t < 2; ++t)
-        if (tokens[t]) {
-          mbar_arrive_expect_tx(q_full + t, halves * 128 * a.group * per_tile);
-          for (int h = 0; h < halves; ++h)
-            tma_load_3d(smem + Cfg::kOffQ + t * Cfg::kTile + h * Cfg::kHalf, &maps.q, q_full + t, 64 * h, kv * a.group, s.q_start + first + t * per_tile);
-        }
-    __syncwarp();
-    // Spans of the tiles' first and last queries: [lo0, hi1] is what some query sees, [lo1, hi0] what all do.
-    AttendSpan outer[2], inner[2];
-    int from = INT_MAX, to = -1;
-    for (int t = 0; t < 2; ++t) {
-      if (!tokens[t]) { outer[t] = inner[t] = {1, 0}; continue; }
-      const int p0 = first + t * per_tile + offset;
-      const AttendSpan x = attend_span(a, p0, s.keys), y = attend_span(a, p0 + tokens[t] - 1, s.keys);
-      outer[t] = {x.lo, y.hi};
-      inner[t] = {y.lo, x.hi};
-      if (outer[t].lo <= outer[t].hi) { from = min(from, outer[t].lo); to = max(to, outer[t].hi); }
-    }
-    const int prefix = min(s.prefix, s.keys);
-    if (prefix > 0) { from = 0; to = max(to, prefix - 1); }
-    // This CTA's share of the blocks.
-    int at = from <= to ? from / kAtKeys : 0, end = from <= to ? to / kAtKeys + 1 : 0;
-    if (a.splits > 1) {
-      const int share = (end - at + a.splits - 1) / a.splits;
-      at += split * share;
-      end = min(end, at + share);
-    }
-    int n = 0, issued = 0;
-    bool ok = true;
-    for (; at < end && ok; ++at) {
-      const int kb = at * kAtKeys, last = min(kb + kAtKeys, s.keys) - 1;
-      int d[4], lo = INT_MAX, hi = INT_MIN;
-      if (a.documents) {
+  // Spans of the tiles' first and last queries: [outer.lo, outer.hi] is what some query sees, [inner.lo, inner.hi] what all do.  The CTA
+  // takes its share of the steps [at, end) from the first to the last key that some query sees.
+  AttendSpan outer[2], inner[2];
+  int from = INT_MAX, to = -1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = kb + lane + 32 * i;
-          d[i] = j <= last ? a.k_documents[s.k_start + j] : 0;
-          if (j <= last) { lo = min(lo, d[i]); hi = max(hi, d[i]); }
-        }
-        lo = __reduce_min_sync(0xffffffffu, lo);
-        hi = __reduce_max_sync(0xffffffffu, hi);
-      }
-      int cls[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const bool in_prefix = kb < prefix, whole_prefix = kb + kAtKeys <= prefix;
-        const bool meets = tokens[t] && kb <= outer[t].hi && last >= outer[t].lo && (!a.documents || (lo <= doc_hi[t] && hi >= doc_lo[t]));
-        const bool whole = kb >= inner[t].lo && kb + kAtKeys - 1 <= inner[t].hi &&
-                           (!a.documents || (lo == hi && doc_lo[t] == doc_hi[t] && lo == doc_lo[t]));
-        cls[t] = !tokens[t] ? kAtSkip : whole_prefix || whole ? kAtFull : in_prefix || meets ? kAtMasked : kAtSkip;
-      }
-      if (cls[0] == kAtSkip && cls[1] == kAtSkip) continue;
-      const int e = n % kAtInfo;
-      ok = mbar_wait(info_empty + e, ((n / kAtInfo) & 1) ^ 1, a.err, kErrAttnWait, abort_flag, wait_ns);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      if (a.documents)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) docs[e * kAtKeys + lane + 32 * i] = d[i];
-      if (lane == 0) info[e] = at << 4 | cls[1] << 2 | cls[0];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(info_full + e);
-#pragma unroll
-      for (int kv_part = 0; kv_part < 2 && ok; ++kv_part) {
-        const int load = 2 * n + kv_part, slot = load % Cfg::kSlots;
-        ok = mbar_wait(empty + slot, ((load / Cfg::kSlots) & 1) ^ 1, a.err, kErrAttnWait, abort_flag, wait_ns);
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok && elect_one()) {
-          mbar_arrive_expect_tx(full + slot, halves * Cfg::kHalf);
-          for (int h = 0; h < halves; ++h)
-            tma_load_3d(smem + Cfg::kOffRing + slot * Cfg::kTile + h * Cfg::kHalf, kv_part ? &maps.v : &maps.k, full + slot, 64 * h, kv, s.k_start + kb);
-        }
-        __syncwarp();
-        if (ok) ++issued;
-      }
-      if (ok) ++n;
-    }
-    if (ok) {
-      const int e = n % kAtInfo;
-      ok = mbar_wait(info_empty + e, ((n / kAtInfo) & 1) ^ 1, a.err, kErrAttnWait, abort_flag, wait_ns);
-      if (lane == 0 && ok) { info[e] = kAtEnd; mbar_arrive(info_full + e); }
-    }
-    __syncwarp();
-    if (*abort_flag) {
-      // Copies that nothing waits for any more land before the CTA ends.
-      for (int t = 0; t < 2; ++t)
-        if (tokens[t]) mbar_drain(q_full + t, 0);
-      for (int load = max(0, issued - Cfg::kSlots); load < issued; ++load) mbar_drain(full + load % Cfg::kSlots, (load / Cfg::kSlots) & 1);
-    }
-  } else if (!idle && warp == 8) {
-    // ---- tensor products
-    constexpr uint32_t idesc_s = mma_idesc<kBf16>(kAtRows, kAtKeys);
-    const uint32_t idesc_o = mma_idesc<kBf16>(kAtRows, 16) - (2u << 17) + ((uint32_t)(2 * nk) << 17) | 1u << 16;  // N = 16 nk; B by values
-    const uint32_t q_addr = smem_u32(smem + Cfg::kOffQ), ring = smem_u32(smem + Cfg::kOffRing);
-    bool ok = true, started[2] = {false, false};
-    int p_phase[2] = {0, 0};
-    auto wait = [&](uint64_t* which, int parity) {
-      ok = ok && mbar_wait(which, parity, a.err, kErrAttnWait, abort_flag, wait_ns);
-      ok = __all_sync(0xffffffffu, ok);
-    };
-    auto read = [&](int n) {
-      const int e = n % kAtInfo;
-      wait(info_full + e, (n / kAtInfo) & 1);
-      int x = kAtEnd;
-      if (ok) x = info[e];
-      __syncwarp();
-      if (ok && lane == 0) mbar_arrive(info_empty + e);
-      return x;
-    };
-    auto scores = [&](int t, int n) {
-      if (elect_one()) {
-        const uint32_t k_addr = ring + (2 * n % Cfg::kSlots) * Cfg::kTile;
-        for (int k = 0; k < nk; ++k) {
-          const uint32_t o = (k >> 2) * Cfg::kHalf + (k & 3) * 32;
-          tc_mma_f16(tmem + t * 128, smem_desc_sw128(q_addr + t * Cfg::kTile + o), smem_desc_sw128(k_addr + o), idesc_s, k > 0);
-        }
-        tc_commit(s_full + t);
-      }
-      __syncwarp();
-    };
-    int cur = read(0);
-    if (cur != kAtEnd && ok) {
-      for (int t = 0; t < 2; ++t)
-        if (tokens[t]) wait(q_full + t, 0);
-      wait(full, 0);
-      tc_fence_after();
-      if (ok)
-        for (int t = 0; t < 2; ++t)
-          if ((cur >> 2 * t) & 3) scores(t, 0);
-      if (ok && elect_one()) tc_commit(empty);
-      __syncwarp();
-      for (int n = 0; ok; ++n) {
-        const int next = read(n + 1);
-        const int v_slot = (2 * n + 1) % Cfg::kSlots, k_next = (2 * n + 2) % Cfg::kSlots;
-        bool v_here = false, k_here = false;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if ((cur >> 2 * t) & 3) {
-            if (!v_here) {
-              wait(full + v_slot, ((2 * n + 1) / Cfg::kSlots) & 1);
-              v_here = true;
-              // Rows past the last key may hold anything: a NaN there, times a weight of zero, would be a NaN.
-              const int rows = s.keys - (cur >> 4) * kAtKeys;
-              if (ok && rows < kAtKeys) {
-                for (int h = 0; h < halves; ++h) {
-                  uint4* tail = reinterpret_cast<uint4*>(smem + Cfg::kOffRing + v_slot * Cfg::kTile + h * Cfg::kHalf + rows * 128);
-                  for (int i = lane; i < (kAtKeys - rows) * 8; i += 32) tail[i] = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-              }
-            }
-            wait(p_full + t, p_phase[t]);
-            p_phase[t] ^= 1;
-            tc_fence_after();
-            if (ok && elect_one()) {
-              const uint32_t v_addr = ring + v_slot * Cfg::kTile;
-#pragma unroll
-              for (int k = 0; k < kAtKeys / 16; ++k)
-                tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * k, smem_desc_values(v_addr + k * 2048, Cfg::kHalf), idesc_o,
-                              started[t] || k > 0);
-            }
-            __syncwarp();
-            started[t] = true;
-          }
-          if (ok && next != kAtEnd && ((next >> 2 * t) & 3)) {
-            if (!k_here) { wait(full + k_next, ((2 * n + 2) / Cfg::kSlots) & 1); k_here = true; tc_fence_after(); }
-            if (ok) scores(t, n + 1);
-          }
-        }
-        if (ok && elect_one()) {
-          tc_commit(empty + v_slot);
-          if (next != kAtEnd) tc_commit(empty + k_next);
-        }
-        __syncwarp();
-        if (next == kAtEnd) break;
-        cur = next;
-      }
-    }
-    if (elect_one()) {
-      if (ok) { tc_commit(o_full); tc_commit(o_full + 1); }
-      tc_commit(drain);
-    }
-    __syncwarp();
-    mbar_drain(drain, 0);
+  for (int t = 0; t < 2; ++t) {
+    outer[t] = inner[t] = {1, 0};
+    if (!tokens[t]) continue;
+    const int p0 = first + t * per_tile + offset;
+    const AttendSpan x = attend_span(a, p0, s.keys), y = attend_span(a, p0 + tokens[t] - 1, s.keys);
+    outer[t] = {x.lo, y.hi};
+    inner[t] = {y.lo, x.hi};
+    if (outer[t].lo <= outer[t].hi) { from = min(from, outer[t].lo); to = max(to, outer[t].hi); }
   }
+  const int prefix = min(s.prefix, s.keys);
+  if (prefix > 0) { from = 0; to = max(to, prefix - 1); }
+  int at = from <= to ? from / kAtKeys : 0, end = from <= to ? to / kAtKeys + 1 : 0;
+  if (a.splits > 1) {
+    const int share = (end - at + a.splits - 1) / a.splits;
+    at += split * share;
+    end = min(end, at + share);
+  }
+  const bool dual = few && end - at > 1;            // both tiles take the rows of the first, each every other step
+  const bool joined = !idle && (a.splits > 1 || dual);  // the rows' results are in parts
+  float* part = reinterpret_cast<float*>(smem + Cfg::kOffK);  // unnormalised rows of O, once all products are done
 
-  // ---- softmax
-  const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // warps 0 .. 7
-  const bool worker = !idle && warp < 8;
-  const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
-  const uint32_t s_tmem = tmem + lane_addr + (t & 1) * 128, o_tmem = s_tmem + 256;
-  const int tile_token = row / a.group, head = kv * a.group + row - tile_token * a.group;
-  const int query = first + t * per_tile + tile_token;
-  const bool live = worker && tile_token < tokens[t & 1] ;
-  float m = -INFINITY, l = 0.f;  // the maximum that P is relative to (log2 units, natural ones with kGeneral), and the sum
-  bool ok = true;
-  if (worker) {
+  if (!idle && warp < kAtSoftmax) {
+    // ---- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane, tile = few ? 0 : t;
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + lane_addr + t * 128, o_tmem = tmem + lane_addr + Cfg::kTmemO + t * DP;
+    const uint32_t p_tmem = s_tmem;
+    const int tile_token = row / a.group, head = kv * a.group + row - tile_token * a.group;
+    const int query = first + tile * per_tile + tile_token;
+    const bool live = tile_token < tokens[tile];
+    const bool warp_live = __any_sync(0xffffffffu, live);
+    float m = -INFINITY, l = 0.f;  // the maximum that P is relative to (log2 units, natural ones with kGeneral), and the sum
     const int p = query + offset;
     AttendSpan span = attend_span(a, p, s.keys);
-    const int prefix = live ? min(s.prefix, s.keys) : 0;
     if (!live) span = {0, -1};
+    const int below = live ? prefix : 0;
     const int doc = live && a.documents ? a.documents[s.q_start + query] : 0;
-    const float scale_log2 = a.scale * kLog2e;
-    const float slope = kGeneral && live && a.slopes ? a.slopes[head] : 0.f;
+    const float scale = a.scale * kUnit;
+    const float slope = (kMode == kAtSlopes || kGeneral) && live && a.slopes ? a.slopes[head] * kUnit : 0.f;
     const float* table = kGeneral && a.table ? a.table + (int64_t)(live ? head : 0) * (2 * a.reach + 1) + a.reach : nullptr;
-    const float cap_in = kGeneral && a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : 0.f;
-    int s_phase = 0;
+    const bool capped = kMode == kAtCap || (kGeneral && a.cap > 0.f);
+    const CapTerms cap(capped ? a.scale / a.cap : 0.f, a.cap * kUnit);
+    bool ok = true;
+    int count = 0;  // steps of this tile
     for (int n = 0;; ++n) {
       const int e = n % kAtInfo;
       ok = mbar_wait(info_full + e, (n / kAtInfo) & 1, a.err, kErrAttnWait, abort_flag, wait_ns);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       const int x = info[e];
       if (x == kAtEnd) break;
-      const int cls = (x >> 2 * t) & 3, kb = (x >> 4) * kAtKeys;
+      const int cls = (x >> 2 * t) & 3, kb = (x >> 8) * kAtKeys;
       if (cls == kAtSkip) {
         __syncwarp();
         if (lane == 0) mbar_arrive(info_empty + e);
         continue;
       }
-      ok = mbar_wait(s_full + t, s_phase, a.err, kErrAttnWait, abort_flag, wait_ns);
+      // `whole` has a bit for each chunk of 32 keys that all rows see whole.
+      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u}, whole = 15;
+      if (cls == kAtMasked && warp_live) {
+        whole = 0;
+        const int mixed = x >> 4 & 15;  // chunks with keys of several documents
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int kc = kb + 32 * c;
+          bits[c] = low_bits(span.hi + 1 - kc) & ~low_bits(span.lo - kc);
+          if (a.documents) {
+            const int* dc = docs + e * kAtKeys + 32 * c;
+            uint32_t same = dc[0] == doc ? ~0u : 0u;
+            if ((mixed >> c) & 1) {
+              same = 0;
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const int4 d = *reinterpret_cast<const int4*>(dc + i);
+                same |= (d.x == doc) << i | (d.y == doc) << (i + 1) | (d.z == doc) << (i + 2) | (d.w == doc) << (i + 3);
+              }
+            }
+            bits[c] &= same;
+          }
+          bits[c] |= low_bits(below - kc);
+          if (__all_sync(0xffffffffu, bits[c] == ~0u || !live)) whole |= 1u << c;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(info_empty + e);
+      ok = mbar_wait(s_full + t, count & 1, a.err, kErrAttnWait, abort_flag, wait_ns);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      s_phase ^= 1;
       tc_fence_after();
+      ++count;
+      if (!warp_live) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + t);
+        continue;
+      }
       uint32_t sx[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32_async(s_tmem + 32 * c, sx[c]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_wait_ld(sx[c]);
-      if (kGeneral) {
+      const int d = kb - p;  // the step's first key less the query
+      float sum = 0.f;
+      // P from the exponents that f gives of the scores, to TMEM; the largest exponent.  kMasked: of the keys that `bits` shows.
+      auto numerators = [&](auto masked, auto f) {
+        float2 part[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (a.cap > 0.f) {
-            // cap tanh(y) = cap - 2 cap / (exp(2 y) + 1): off by 2^-21 cap at most.
+          uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              sx[c][i] = __float_as_uint(fmaf(-2.f * a.cap, rcp_approx(ex2_approx(__uint_as_float(sx[c][i]) * cap_in) + 1.f), a.cap));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) sx[c][i] = __float_as_uint(__uint_as_float(sx[c][i]) * a.scale);
-          }
-          const int d = kb + 32 * c - p;  // key less query
-          if (a.slopes) {
-            const float fd = (float)d;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) sx[c][i] = __float_as_uint(fmaf(-slope, fabsf(fd + (float)i), __uint_as_float(sx[c][i])));
-          }
-          if (table) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              sx[c][i] = __float_as_uint(__uint_as_float(sx[c][i]) + __ldg(table + min(max(d + i, -a.reach), a.reach)));
-          }
-        }
-      }
-      if (cls == kAtMasked) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int kc = kb + 32 * c;
-          uint32_t bits = low_bits(span.hi + 1 - kc) & ~low_bits(span.lo - kc);
-          if (a.documents) {
-            uint32_t same = 0;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const int4 d = *reinterpret_cast<const int4*>(docs + e * kAtKeys + 32 * c + i);
-              same |= (d.x == doc) << i | (d.y == doc) << (i + 1) | (d.z == doc) << (i + 2) | (d.w == doc) << (i + 3);
+          for (int i = 0; i < 32; i += 2) {
+            float2 v = f(make_float2(__uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1])), 32 * c + i);
+            if (decltype(masked)::value) {
+              if (!((bits[c] >> i) & 1)) v.x = -INFINITY;
+              if (!((bits[c] >> (i + 1)) & 1)) v.y = -INFINITY;
             }
-            bits &= same;
+            mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], v.x, v.y);
+            const float2 w = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+            part[(i >> 1) & 3] = add2(part[(i >> 1) & 3], w);
+            pk[i >> 1] = pack2<T>(w.x, w.y);
           }
-          bits |= low_bits(prefix - kc);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((bits >> i) & 1)) sx[c][i] = __float_as_uint(-INFINITY);
+          tmem_st16(p_tmem + 16 * c, pk);
         }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(info_empty + e);
-      float mx[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mx[i] = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 7] = max3(mx[(i >> 1) & 7], __uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1]));
-#pragma unroll
-      for (int w = 4; w >= 1; w >>= 1)
-#pragma unroll
-        for (int i = 0; i < w; ++i) mx[i] = fmaxf(mx[i], mx[i + w]);
-      const float top = kGeneral ? mx[0] : mx[0] * scale_log2;
-      float alpha = 1.f;
-      bool dirty = false;
-      if (top > m + (kGeneral ? kAtRescale / kLog2e : kAtRescale)) {
-        if (m != -INFINITY) { alpha = ex2_approx(kGeneral ? (m - top) * kLog2e : m - top); dirty = true; }
-        m = top;
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      float2 sum[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float2 y = make_float2(__uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1]));
-          // Differences before the factor: scores of the type's lowest value stay equal to one another.
-          if (kGeneral) y = fma2(sub2(y, make_float2(base, base)), make_float2(kLog2e, kLog2e), make_float2(kShift, kShift));
-          else y = fma2(y, make_float2(scale_log2, scale_log2), make_float2(kShift - base, kShift - base));
-          const float2 w = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-          sum[(i >> 1) & 3] = add2(sum[(i >> 1) & 3], w);
-          pk[i >> 1] = pack2<T>(w.x, w.y);
+        const float2 both = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+        sum = both.x + both.y;
+        return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      };
+      // A step relative to the maximum of the steps before, from the products at once: the exponents' maximum, found beside them,
+      // tells whether it will do (few steps raise it by more than kAtRescale).
+      auto at_once = [&](auto masked) {
+        const float2 by = make_float2(scale, scale), less = make_float2(kShift - m, kShift - m);
+        float most = INFINITY;
+        if (kMode == kAtPlain) {
+          most = numerators(masked, [&](float2 y, int) { return fma2(y, by, less); });
+        } else if (kMode == kAtCap) {
+          float big = 0.f;
+          most = numerators(masked, [&](float2 y, int) { big = max3(big, fabsf(y.x), fabsf(y.y)); return fma2(y, cap.slope(y), less); });
+          if (!(big <= cap.most)) most = INFINITY;
+        } else if (kMode == kAtSlopes) {
+          // All keys on one side of the query.
+          const bool left = d + kAtKeys - 1 <= 0;
+          if (__all_sync(0xffffffffu, left || d >= 0)) {
+            const float g = left ? slope : -slope, at_d = fmaf(g, (float)d, kShift - m);
+            const float2 from = make_float2(at_d, at_d), each = make_float2(g, g);
+            most = numerators(masked, [&](float2 y, int i) { return fma2(y, by, fma2(each, make_float2((float)i, (float)(i + 1)), from)); });
+          } else {
+            const float fd = (float)d;
+            most = numerators(masked, [&](float2 y, int i) {
+              return fma2(y, by, fma2(make_float2(-slope, -slope), make_float2(fabsf(fd + (float)i), fabsf(fd + (float)(i + 1))), less));
+            });
+          }
+        } else if (!capped && !a.slopes) {
+          const float2 unit = make_float2(kLog2e, kLog2e), shift = make_float2(kShift, kShift), at_m = make_float2(m, m);
+          // Past the reach on one side for all rows: one bias.
+          const bool left = table && d + kAtKeys - 1 <= -a.reach;
+          if (!table || __all_sync(0xffffffffu, left || d >= a.reach)) {
+            const float edge = !table ? 0.f : __ldg(table + (left ? -a.reach : a.reach));
+            const float2 bias = make_float2(edge, edge);
+            most = numerators(masked, [&](float2 y, int) { return fma2(sub2(fma2(y, by, bias), at_m), unit, shift); });
+          } else {
+            most = numerators(masked, [&](float2 y, int i) {
+              const float2 bias = make_float2(__ldg(table + min(max(d + i, -a.reach), a.reach)), __ldg(table + min(max(d + i + 1, -a.reach), a.reach)));
+              return fma2(sub2(fma2(y, by, bias), at_m), unit, shift);
+            });
+          }
         }
-        tmem_st16(s_tmem + 16 * c, pk);
-      }
-      const float2 total = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-      l = l * alpha + (total.x + total.y);
-      // O is settled: S of this block, which s_full announced, came after every product into O that was issued.
-      if (__any_sync(0xffffffffu, dirty)) {
+        return __all_sync(0xffffffffu, most <= kShift + kAtRescale || !live);
+      };
+      bool done = false;
+      if (__all_sync(0xffffffffu, m > -INFINITY || !live)) done = whole == 15 ? at_once(std::false_type{}) : at_once(std::true_type{});
+      if (!done) {
+        tmem_wait_st();  // before P is written again
+        auto each = [&](auto f) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 y = f(make_float2(__uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1])), 32 * c + i);
+              sx[c][i] = __float_as_uint(y.x);
+              sx[c][i + 1] = __float_as_uint(y.y);
+            }
+        };
+        if (capped) {
+          float big = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) big = max3(big, fabsf(__uint_as_float(sx[c][i])), fabsf(__uint_as_float(sx[c][i + 1])));
+          if (__all_sync(0xffffffffu, big <= cap.most)) each([&](float2 y, int) { return mul2(y, cap.slope(y)); });
+          else each([&](float2 y, int) { return make_float2(cap.any(y.x), cap.any(y.y)); });
+        }
+        const float2 by = capped ? make_float2(1.f, 1.f) : make_float2(scale, scale);
+        if ((kMode == kAtSlopes || kGeneral) && a.slopes) {
+          const float fd = (float)d;
+          each([&](float2 y, int i) { return fma2(y, by, make_float2(-slope * fabsf(fd + (float)i), -slope * fabsf(fd + (float)(i + 1)))); });
+        } else if (kGeneral && table) {
+          each([&](float2 y, int i) {
+            return fma2(y, by, make_float2(__ldg(table + min(max(d + i, -a.reach), a.reach)), __ldg(table + min(max(d + i + 1, -a.reach), a.reach))));
+          });
+        } else if (kMode == kAtPlain || (kGeneral && !capped)) {
+          each([&](float2 y, int) { return mul2(y, by); });
+        }
+        if (whole != 15) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (!((whole >> c) & 1))
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((bits[c] >> i) & 1)) sx[c][i] = __float_as_uint(-INFINITY);
+        }
+        float mx[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx[i] = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 7] = max3(mx[(i >> 1) & 7], __uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1]));
+#pragma unroll
+        for (int w = 4; w >= 1; w >>= 1)
+#pragma unroll
+          for (int i = 0; i < w; ++i) mx[i] = fmaxf(mx[i], mx[i + w]);
+        const float top = mx[0];
+        float alpha = 1.f;
+        bool dirty = false;
+        if (top > m + (kGeneral ? kAtRescale / kLog2e : kAtRescale)) {
+          if (m != -INFINITY) { alpha = ex2_approx(kGeneral ? (m - top) * kLog2e : m - top); dirty = true; }
+          m = top;
+        }
+        l *= alpha;
+        if (__any_sync(0xffffffffu, dirty)) {
+          // O is settled: s_full followed the products before.
 #pragma unroll 1
-        for (int c = 0; c < (a.dim + 31) / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32_async(o_tmem + 32 * c, o);
-          tmem_wait_ld(o);
+          for (int c = 0; c < (a.dim + 31) / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32_async(o_tmem + 32 * c, o);
+            tmem_wait_ld(o);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st32(o_tmem + 32 * c, o);
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(o_tmem + 32 * c, o);
+          }
         }
+        const float base = m == -INFINITY ? 0.f : m;
+        const float2 at_m = make_float2(base, base), unit = make_float2(kLog2e, kLog2e), shift = make_float2(kShift, kShift), less = make_float2(kShift - base, kShift - base);
+        // Differences before the factor in natural units: scores of the type's lowest value stay equal to one another.
+        numerators(std::false_type{}, [&](float2 y, int) { return kGeneral ? fma2(sub2(y, at_m), unit, shift) : add2(y, less); });
       }
+      l += sum;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + t);
     }
-    ok = ok && mbar_wait(o_full + t, 0, a.err, kErrAttnWait, abort_flag, wait_ns);
+    ok = ok && mbar_wait(drain + t, 0, a.err, kErrAttnWait, abort_flag, wait_ns);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
-  }
-  const int64_t token = s.q_start + query;
-  if (a.splits == 1) {
-    if (worker && ok) {
-      // Rows without a visible key, and rows that no block was made for, hold nothing in O.
+    if (joined) {
+      sums[t * kAtRows + row] = make_float2(m, ok ? l : NAN);
+    } else if (ok && warp_live && !(few && t)) {
+      // Rows without a visible key, and rows that no step was made for, hold nothing in O.
+      const int64_t token = s.q_start + query;
       const bool any = l > 0.f || l != l;
       const float inv = any ? 1.f / l : 0.f;
       bool fine = l - l == 0.f;
@@ -618,44 +571,244 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
         attend_row<T>(a, s, all_queries, __shfl_sync(0xffffffffu, query, src), __shfl_sync(0xffffffffu, head, src));
       }
     }
-  } else {
-    // Every CTA's rows into its own shared memory (all products are done, so the ring is free), then each warp of the cluster joins the
-    // parts of its share of the rows.
-    float* part = reinterpret_cast<float*>(smem + Cfg::kOffRing);
-    if (worker) {
-      const int slot = t * kAtRows + row;
-      sums[slot] = make_float2(m, ok ? l : NAN);
-#pragma unroll 1
-      for (int c = 0; c < a.dim; c += 32) {
-        uint32_t o[32];
-        tmem_ld32_async(o_tmem + c, o);
-        tmem_wait_ld(o);
-        if (live)
+  } else if (!idle) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == kAtLoadWarp) {
+      // ---- steps and loads
+      int doc_lo[2] = {INT_MAX, INT_MAX}, doc_hi[2] = {INT_MIN, INT_MIN};
+      if (elect_one())
+        for (int t = 0; t < 2; ++t)
+          if (tokens[t]) {
+            mbar_arrive_expect_tx(q_full + t, halves * 128 * a.group * per_tile);
+            for (int h = 0; h < halves; ++h)
+              tma_load_3d(smem + Cfg::kOffQ + t * Cfg::kQTile + h * Cfg::kQHalf, &maps.q, q_full + t, 64 * h, kv * a.group,
+                          s.q_start + first + t * per_tile);
+          }
+      __syncwarp();
+      if (a.documents)
+        for (int t = 0; t < 2; ++t) {
+          for (int i = lane; i < tokens[t]; i += 32) {
+            const int d = a.documents[s.q_start + first + t * per_tile + i];
+            doc_lo[t] = min(doc_lo[t], d);
+            doc_hi[t] = max(doc_hi[t], d);
+          }
+          doc_lo[t] = __reduce_min_sync(0xffffffffu, doc_lo[t]);
+          doc_hi[t] = __reduce_max_sync(0xffffffffu, doc_hi[t]);
+        }
+      int n = 0, k_issued = 0, v_issued = 0;
+      bool ok = true;
+      auto load = [&](const CUtensorMap* map, uint64_t* full, uint64_t* empty, int off, int kb, int& issued) {
+        const int slot = n % kSlots;
+        ok = ok && mbar_wait(empty + slot, ((n / kSlots) & 1) ^ 1, a.err, kErrAttnWait, abort_flag, wait_ns);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(full + slot, halves * Cfg::kHalf);
+          for (int h = 0; h < halves; ++h) tma_load_3d(smem + off + slot * Cfg::kTile + h * Cfg::kHalf, map, full + slot, 64 * h, kv, s.k_start + kb);
+        }
+        __syncwarp();
+        ++issued;
+      };
+      // With slopes the nearest keys first, whose scores the later ones then seldom exceed.
+      for (int i = at; i < end && ok; ++i) {
+        const int step = a.slopes ? at + end - 1 - i : i;
+        const int kb = step * kAtKeys, last = min(kb + kAtKeys, s.keys) - 1;
+        int d[4] = {0, 0, 0, 0}, lo = INT_MAX, hi = INT_MIN;
+        if (a.documents) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(part + slot * DP + (((c + i) / 4) ^ (row & 7)) * 4) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 4; ++i) {
+            const int j = kb + lane + 32 * i;
+            if (j <= last) {
+              d[i] = a.k_documents[s.k_start + j];
+              lo = min(lo, d[i]);
+              hi = max(hi, d[i]);
+            }
+          }
+          lo = __reduce_min_sync(0xffffffffu, lo);
+          hi = __reduce_max_sync(0xffffffffu, hi);
+        }
+        int mixed = 0;
+        if (a.documents)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!__all_sync(0xffffffffu, d[i] == __shfl_sync(0xffffffffu, d[i], 0))) mixed |= 1 << i;
+        int cls[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const bool in_prefix = kb < prefix, whole_prefix = kb + kAtKeys <= prefix;
+          const bool meets = kb <= outer[t].hi && last >= outer[t].lo && (!a.documents || (lo <= doc_hi[t] && hi >= doc_lo[t]));
+          const bool whole = kb >= inner[t].lo && kb + kAtKeys - 1 <= inner[t].hi &&
+                             (!a.documents || (lo == hi && doc_lo[t] == doc_hi[t] && lo == doc_lo[t]));
+          cls[t] = !tokens[t] ? kAtSkip : whole_prefix || whole ? kAtFull : in_prefix || meets ? kAtMasked : kAtSkip;
+        }
+        if (cls[0] == kAtSkip && cls[1] == kAtSkip) continue;
+        if (dual && (n & 1)) { cls[1] = cls[0]; cls[0] = kAtSkip; }
+        const int e = n % kAtInfo;
+        ok = mbar_wait(info_empty + e, ((n / kAtInfo) & 1) ^ 1, a.err, kErrAttnWait, abort_flag, wait_ns);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        if (a.documents) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) docs[e * kAtKeys + lane + 32 * i] = d[i];
+        }
+        if (lane == 0) info[e] = step << 8 | mixed << 4 | cls[1] << 2 | cls[0];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(info_full + e);
+        load(&maps.k, k_full, k_empty, Cfg::kOffK, kb, k_issued);
+        load(&maps.v, v_full, v_empty, Cfg::kOffV, kb, v_issued);
+        ++n;
+      }
+      if (ok) {
+        const int e = n % kAtInfo;
+        ok = mbar_wait(info_empty + e, ((n / kAtInfo) & 1) ^ 1, a.err, kErrAttnWait, abort_flag, wait_ns);
+        if (lane == 0 && ok) { info[e] = kAtEnd; mbar_arrive(info_full + e); }
+      }
+      __syncwarp();
+      if (*abort_flag) {
+        // Copies that nothing waits for any more land before the CTA ends.
+        for (int t = 0; t < 2; ++t)
+          if (tokens[t]) mbar_drain(q_full + t, 0);
+        for (int i = max(0, k_issued - kSlots); i < k_issued; ++i) mbar_drain(k_full + i % kSlots, (i / kSlots) & 1);
+        for (int i = max(0, v_issued - kSlots); i < v_issued; ++i) mbar_drain(v_full + i % kSlots, (i / kSlots) & 1);
+      }
+    } else if (warp == kAtMmaWarp) {
+      // ---- tensor products
+      constexpr uint32_t idesc_s = mma_idesc<kBf16>(kAtRows, kAtKeys);
+      const uint32_t idesc_o = mma_idesc<kBf16>(kAtRows, 0) | (uint32_t)(2 * nk) << 17 | 1u << 16;  // N = 16 nk; B by values
+      const uint32_t q_addr = smem_u32(smem + Cfg::kOffQ), k_addr = smem_u32(smem + Cfg::kOffK), v_addr = smem_u32(smem + Cfg::kOffV);
+      bool ok = true;
+      int used[2] = {0, 0};  // products P V of each tile
+      auto wait = [&](uint64_t* which, int parity) {
+        ok = ok && mbar_wait(which, parity, a.err, kErrAttnWait, abort_flag, wait_ns);
+        ok = __all_sync(0xffffffffu, ok);
+      };
+      auto read = [&](int n) {
+        const int e = n % kAtInfo;
+        wait(info_full + e, (n / kAtInfo) & 1);
+        int x = kAtEnd;
+        if (ok) x = info[e];
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(info_empty + e);
+        return x;
+      };
+      auto takes = [](int x, int t) { return x != kAtEnd && ((x >> 2 * t) & 3); };
+      // S of step n for tile t, over the P whose product has been issued.
+      auto scores = [&](int n, int t) {
+        tc_fence_after();
+        if (ok && elect_one()) {
+          const uint32_t qt = q_addr + (dual ? 0 : t * Cfg::kQTile), kt = k_addr + n % kSlots * Cfg::kTile;
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)  // (not to nk: rolled, the issue of a product took 80 cycles, more than the product)
+            if (k < nk)
+              tc_mma_f16(tmem + t * 128, smem_desc_sw128(qt + (k >> 2) * Cfg::kQHalf + (k & 3) * 32),
+                         smem_desc_sw128(kt + (k >> 2) * Cfg::kHalf + (k & 3) * 32), idesc_s, k > 0);
+          tc_commit(s_full + t);
+        }
+        __syncwarp();
+      };
+      auto values = [&](int n, int t) {
+        wait(p_full + t, used[t] & 1);
+        tc_fence_after();
+        if (ok && elect_one()) {
+          const uint32_t pt = tmem + t * 128;
+#pragma unroll
+          for (int k = 0; k < kAtKeys / 16; ++k)
+            tc_mma_f16_ts(tmem + Cfg::kTmemO + t * DP, pt + 8 * k, smem_desc_values(v_addr + n % kSlots * Cfg::kTile + k * 2048, Cfg::kHalf), idesc_o,
+                          used[t] > 0 || k > 0);
+        }
+        __syncwarp();
+        ++used[t];
+      };
+      auto release = [&](uint64_t* empty) {
+        if (ok && elect_one()) tc_commit(empty);
+        __syncwarp();
+      };
+      int cur = read(0);
+      if (cur != kAtEnd && ok) {
+        for (int t = 0; t < 2; ++t)
+          if (tokens[t]) wait(q_full + t, 0);
+        wait(k_full, 0);
+        for (int t = 0; t < 2; ++t)
+          if (takes(cur, t)) scores(0, t);
+        release(k_empty);
+        for (int n = 0; ok && cur != kAtEnd; ++n) {
+          const int next = read(n + 1), k_next = (n + 1) % kSlots;
+          if (next != kAtEnd) wait(k_full + k_next, ((n + 1) / kSlots) & 1);
+          wait(v_full + n % kSlots, (n / kSlots) & 1);
+          // Rows past the last key may hold anything: a NaN there, times a weight of zero, would be a NaN.
+          const int rows = s.keys - (cur >> 8) * kAtKeys;
+          if (ok && rows < kAtKeys) {
+            for (int h = 0; h < halves; ++h) {
+              uint4* tail = reinterpret_cast<uint4*>(smem + Cfg::kOffV + n % kSlots * Cfg::kTile + h * Cfg::kHalf + rows * 128);
+              for (int i = lane; i < (kAtKeys - rows) * 8; i += 32) tail[i] = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          for (int t = 0; t < 2; ++t) {
+            if (takes(cur, t)) values(n, t);
+            if (takes(next, t)) scores(n + 1, t);
+          }
+          release(v_empty + n % kSlots);
+          if (next != kAtEnd) release(k_empty + k_next);
+          cur = next;
+        }
+      }
+      if (elect_one()) { tc_commit(drain); tc_commit(drain + 1); }
+      __syncwarp();
+      mbar_drain(drain, 0);
+      mbar_drain(drain + 1, 0);
+    }
+  }
+  if (joined) {
+    __syncthreads();  // the products of both tiles are done: the tiles of K and V are free
+    tc_fence_after();
+    if (warp < kAtSoftmax && !*abort_flag) {
+      const int t = warp >> 2, row = (warp & 3) * 32 + lane, slot = t * kAtRows + row;
+      const bool live = row / a.group < tokens[few ? 0 : t];
+      if (__any_sync(0xffffffffu, live)) {
+#pragma unroll 1
+        for (int c = 0; c < a.dim; c += 32) {
+          uint32_t o[32];
+          tmem_ld32_async(tmem + ((uint32_t)((warp & 3) * 32) << 16) + Cfg::kTmemO + t * DP + c, o);
+          tmem_wait_ld(o);
+          if (live)
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4*>(part + slot * DP + (((c + i) / 4) ^ (row & 7)) * 4) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
       }
     }
     tc_fence_before();
-    cluster_sync();
-    if (worker && !*abort_flag) {
+    if (a.splits > 1) cluster_sync();
+    else __syncthreads();
+    // Each warp of the cluster joins the parts of its share of the rows.
+    if (warp < kAtSoftmax && !*abort_flag) {
       const uint32_t part_addr = smem_u32(part), sums_addr = smem_u32(sums);
-      const int rows0 = tokens[0] * a.group, rows = rows0 + tokens[1] * a.group;
-      for (int r = split * 8 + warp; r < rows; r += 8 * a.splits) {
-        const int tile = r >= rows0, at = tile ? r - rows0 : r, slot = tile * kAtRows + at;
-        float top = -INFINITY;
-        for (int c = 0; c < a.splits; ++c) top = fmaxf(top, ld_cluster_v2(cluster_addr(sums_addr + slot * 8, c)).x);
+      const int rows0 = tokens[0] * a.group, rows = rows0 + tokens[1] * a.group, parts = few ? 2 * a.splits : a.splits;
+      for (int r = split * kAtSoftmax + warp; r < rows; r += kAtSoftmax * a.splits) {
+        const int tile = r >= rows0, at_row = tile ? r - rows0 : r;
+        auto slot_of = [&](int c) { return (few ? c & 1 : tile) * kAtRows + at_row; };
+        auto rank_of = [&](int c) { return few ? c >> 1 : c; };
+        // A lane per part for the maximum and the sum (16 parts at most).
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < parts) ml = ld_cluster_v2(cluster_addr(sums_addr + slot_of(lane) * 8, rank_of(lane)));
+        float top = ml.x;
+#pragma unroll
+        for (int w = 8; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        top = __shfl_sync(0xffffffffu, top, 0);
+        const bool none = ml.x == -INFINITY && ml.y == 0.f;  // saw nothing: its O is not defined
+        const float weight = none ? 0.f : ex2_approx(kGeneral ? (ml.x - top) * kLog2e : ml.x - top);
+        const uint32_t some = __ballot_sync(0xffffffffu, !none);
         float sum = 0.f, o[DP / 32] = {};
-        for (int c = 0; c < a.splits; ++c) {
-          const float2 ml = ld_cluster_v2(cluster_addr(sums_addr + slot * 8, c));
-          if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing: its O is not defined
-          const float w = ex2_approx(kGeneral ? (ml.x - top) * kLog2e : ml.x - top);
-          sum = fmaf(ml.y, w, sum);
+        for (uint32_t left = some; left; left &= left - 1) {
+          const int c = __ffs(left) - 1;
+          const float w = __shfl_sync(0xffffffffu, weight, c);
+          sum = fmaf(__shfl_sync(0xffffffffu, ml.y, c), w, sum);
 #pragma unroll
           for (int i = 0; i < DP / 64; ++i) {
             const int d = 2 * lane + 64 * i;
             if (d < a.dim) {
-              const float2 x = ld_cluster_v2(cluster_addr(part_addr + (slot * DP + ((d / 4) ^ (at & 7)) * 4 + d % 4) * 4, c));
+              const float2 x = ld_cluster_v2(cluster_addr(part_addr + (slot_of(c) * DP + ((d / 4) ^ (at_row & 7)) * 4 + d % 4) * 4, rank_of(c)));
               o[2 * i] = fmaf(x.x, w, o[2 * i]);
               o[2 * i + 1] = fmaf(x.y, w, o[2 * i + 1]);
             }
@@ -664,7 +817,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
         const bool any = sum > 0.f || sum != sum;
         const float inv = any ? 1.f / sum : 0.f;
         bool fine = sum - sum == 0.f;
-        const int tok = at / a.group, h = kv * a.group + at - tok * a.group, qi = first + tile * per_tile + tok;
+        const int tok = at_row / a.group, h = kv * a.group + at_row - tok * a.group, qi = first + tile * per_tile + tok;
         T* out = static_cast<T*>(a.out) + (int64_t)(s.q_start + qi) * a.out_token + h * a.out_head;
 #pragma unroll
         for (int i = 0; i < DP / 64; ++i) {
@@ -678,12 +831,15 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
         if (__any_sync(0xffffffffu, !fine)) attend_row<T>(a, s, all_queries, qi, h);
       }
     }
-    cluster_sync();
+  }
+  if (a.splits > 1) {
+    if (idle) cluster_sync();
+    cluster_sync();  // no CTA ends while another reads its parts
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == kAtMmaWarp) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace laya

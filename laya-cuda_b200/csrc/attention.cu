@@ -57,10 +57,10 @@ CUtensorMap heads_map(bool bf16, const void* p, int dim, int heads, int tokens, 
   return map;
 }
 
-template <typename T, int DP, bool kGeneral>
+template <typename T, int DP, int kMode>
 void launch_attend_kernel(const AttendArgs& a, const AttendMaps& maps, int64_t ctas, int dev, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  auto kern = attend_kernel<T, DP, kGeneral>;
+  auto kern = attend_kernel<T, DP, kMode>;
   allow_smem(kern, AttendCfg<DP>::kBytes, dev, done);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
@@ -100,8 +100,11 @@ void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   // Without a key there is nothing to load: any map will do.
   maps.k = a.k_tokens ? heads_map(kBf16, a.k, a.dim, a.kv_heads, a.k_tokens, a.k_head, a.k_token, 1, kAtKeys) : maps.q;
   maps.v = a.k_tokens ? heads_map(kBf16, a.v, a.dim, a.kv_heads, a.k_tokens, a.v_head, a.v_token, 1, kAtKeys) : maps.q;
-  if (a.cap > 0.f || a.slopes || a.table || !(a.scale > 0.f)) launch_attend_kernel<T, DP, true>(a, maps, items * a.splits, dev, st);
-  else launch_attend_kernel<T, DP, false>(a, maps, items * a.splits, dev, st);
+  const int64_t ctas = items * a.splits;
+  if (a.table || !(a.scale > 0.f) || (a.slopes && a.cap > 0.f)) launch_attend_kernel<T, DP, kAtGeneral>(a, maps, ctas, dev, st);
+  else if (a.slopes) launch_attend_kernel<T, DP, kAtSlopes>(a, maps, ctas, dev, st);
+  else if (a.cap > 0.f) launch_attend_kernel<T, DP, kAtCap>(a, maps, ctas, dev, st);
+  else launch_attend_kernel<T, DP, kAtPlain>(a, maps, ctas, dev, st);
 }
 
 }  // namespace
