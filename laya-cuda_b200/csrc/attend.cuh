@@ -26,15 +26,17 @@ struct AttendArgs {
   int reach;
   int* err;
   unsigned long long wait_ns;
-  int pairs, splits;  // pairs of tiles for max_queries; CTAs (a cluster) that share a pair's keys
+  int per_tile;       // queries of a tile, which holds all heads of a group for each
+  int pairs, splits;  // CTAs for max_queries of a kv head; CTAs (a cluster) that share a tile's keys
+  FastDiv by_group, by_splits, by_kv, by_sequences;
 };
 
 struct AttendSequence {
   int q_start, queries, k_start, keys, prefix;
 };
 
-// The lengths of sequence b; none of it (and an error) where it does not lie in the tensors.
-__device__ __forceinline__ AttendSequence attend_sequence(const AttendArgs& a, int b) {
+// The lengths of sequence b; none of it (and an error) where it does not lie in the tensors.  *all: its queries before the bound on them.
+__device__ __forceinline__ AttendSequence attend_sequence(const AttendArgs& a, int b, int* all) {
   AttendSequence s{a.starts[b], a.lengths[b], a.k_starts[b], a.k_lengths[b], a.prefix ? a.prefix[b] : 0};
   const bool bad = s.q_start < 0 || s.queries < 0 || s.k_start < 0 || s.keys < 0 ||
                    (int64_t)s.q_start + s.queries > a.q_tokens || (int64_t)s.k_start + s.keys > a.k_tokens;
@@ -42,6 +44,7 @@ __device__ __forceinline__ AttendSequence attend_sequence(const AttendArgs& a, i
     if (a.err && threadIdx.x == 0) atomicCAS(a.err, 0, kErrBadIndex);
     s.queries = s.keys = 0;
   }
+  *all = s.queries;
   s.queries = min(s.queries, a.max_queries);
   return s;
 }
@@ -120,9 +123,6 @@ __device__ void attend_row(const AttendArgs& a, const AttendSequence& s, int ful
 // ---------------------------------------------------------------------------------------------
 constexpr int kAtRows = 128;       // rows of a tile
 constexpr int kAtKeys = 128;       // keys of a step
-constexpr int kAtSoftmax = 8;       // softmax warps
-constexpr int kAtThreads = 32 * (kAtSoftmax + 4);
-constexpr int kAtMmaWarp = kAtSoftmax, kAtLoadWarp = kAtSoftmax + 1;
 constexpr int kAtInfo = 4;         // steps announced ahead
 constexpr float kAtRescale = 8.f;  // O is rescaled when a row's maximum has grown by more than 2^8
 enum AtClass : int { kAtEnd = -1, kAtSkip = 0, kAtMasked = 1, kAtFull = 2 };
@@ -130,23 +130,34 @@ enum AtClass : int { kAtEnd = -1, kAtSkip = 0, kAtMasked = 1, kAtFull = 2 };
 // times the lowest number of a type would be -infinity).
 enum AtMode { kAtPlain, kAtCap, kAtSlopes, kAtGeneral };
 
-template <int DP>
+constexpr int kAtMostSplits = 8;
+
+// NT tiles per CTA, heads padded to DP values.
+template <int DP, int NT>
 struct AttendCfg {
-  static_assert(DP == 64 || DP == 128, "padded head size");
-  static constexpr int kTmemO = 256;                     // column of O of tile 0
-  static constexpr int kSlots = DP == 128 ? 2 : 4;       // K tiles in flight, and V tiles
+  static_assert((DP == 64 || DP == 128) && (NT == 1 || NT == 2), "padded head size, tiles");
+  static constexpr int kSoftmax = 4 * NT;                // softmax warps
+  static constexpr int kMmaWarp = kSoftmax, kLoadWarp = kSoftmax + 1, kThreads = 32 * (kSoftmax + 4), kCtas = NT == 1 ? 2 : 1;
+  // Registers: what the launch gives all threads (128 with one tile, 168 with two), moved to the softmax.
+  static constexpr int kSoftmaxRegs = NT == 1 ? 200 : 224, kOtherRegs = 56;
+  static_assert(32 * (kSoftmax * kSoftmaxRegs + 4 * kOtherRegs) <= kThreads * (NT == 1 ? 128 : 168), "registers of the launch");
+  static constexpr int kTmemO = 128 * NT, kTmemCols = NT == 1 ? 256 : 512;  // columns: O of tile 0, all
+  static_assert(kTmemO + NT * DP <= kTmemCols, "tensor memory");
+  static constexpr int kSlots = (DP == 128 ? 1 : 2) * NT;  // K tiles in flight, and V tiles
   static constexpr int kQTile = kAtRows * DP * 2, kQHalf = kAtRows * 128;  // halves: [rows][64 values]
   static constexpr int kTile = kAtKeys * DP * 2, kHalf = kAtKeys * 128;
-  static constexpr int kOffQ = 0, kOffK = 2 * kQTile, kOffV = kOffK + kSlots * kTile;
+  static constexpr int kOffQ = 0, kOffK = NT * kQTile, kOffV = kOffK + kSlots * kTile;
   static constexpr int kOffDocs = kOffV + kSlots * kTile;
   static constexpr int kOffBar = kOffDocs + kAtInfo * kAtKeys * 4;
   static constexpr int kBars = 2 + 4 * kSlots + 2 * kAtInfo + 6;
   static constexpr int kOffInfo = kOffBar + kBars * 8;
-  static constexpr int kOffSums = kOffInfo + kAtInfo * 4 + 16;  // (maximum, sum) of each row, for a split
-  static constexpr int kBytes = kOffSums + 2 * kAtRows * 8 + 1024;
+  static constexpr int kOffSums = kOffInfo + kAtInfo * 4 + 16;  // (maximum, sum) of each row, where results are joined
+  static constexpr int kWeights = 2 * NT * kAtRows + 2 * kAtMostSplits;  // of the parts of the rows that a CTA joins
+  static constexpr int kOffWeights = kOffSums + NT * kAtRows * 8;
+  static constexpr int kBytes = kOffWeights + kWeights * 4 + 1024;
   static_assert(kOffSums % 8 == 0, "alignment");
-  static_assert(2 * kAtRows * DP * 4 <= 2 * kSlots * kTile, "a split's O fits the K and V tiles");
-  static_assert(kBytes <= 227 * 1024, "shared memory");
+  static_assert(NT * kAtRows * DP * 4 <= 2 * kSlots * kTile, "a part's O fits the K and V tiles");
+  static_assert(kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
@@ -168,6 +179,11 @@ __device__ __forceinline__ uint64_t smem_desc_values(uint32_t saddr, int half) {
   return d;
 }
 
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
 __device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
@@ -219,9 +235,10 @@ struct CapTerms {
 };
 
 // T, the padded head size, and what is done to the scores.
-template <typename T, int DP, int kMode>
-__global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_constant__ AttendMaps maps, const __grid_constant__ AttendArgs a) {
-  using Cfg = AttendCfg<DP>;
+template <typename T, int DP, int NT, int kMode>
+__global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>::kCtas)
+    attend_kernel(const __grid_constant__ AttendMaps maps, const __grid_constant__ AttendArgs a) {
+  using Cfg = AttendCfg<DP, NT>;
   constexpr int kSlots = Cfg::kSlots;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value, kGeneral = kMode == kAtGeneral;
   constexpr float kUnit = kGeneral ? 1.f : 1.4426950408889634f;  // of the scores: natural, or log2
@@ -242,38 +259,39 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
   const unsigned long long wait_ns = wait_limit(a.wait_ns);
 
   if (threadIdx.x == 0) {
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < NT; ++t) {
       mbar_init(q_full + t, 1);
       mbar_init(s_full + t, 1);
       mbar_init(p_full + t, 4);
       mbar_init(drain + t, 1);
     }
     for (int i = 0; i < kSlots; ++i) { mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1); }
-    for (int i = 0; i < kAtInfo; ++i) { mbar_init(info_full + i, 1); mbar_init(info_empty + i, kAtSoftmax + 1); }
+    for (int i = 0; i < kAtInfo; ++i) { mbar_init(info_full + i, 1); mbar_init(info_empty + i, Cfg::kSoftmax + 1); }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == kAtMmaWarp) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
-  if (warp == kAtLoadWarp && lane == 0) { tma_prefetch_desc(&maps.q); tma_prefetch_desc(&maps.k); tma_prefetch_desc(&maps.v); }
+  if (warp == Cfg::kMmaWarp) { tmem_alloc(tmem_slot, Cfg::kTmemCols); tmem_relinquish(); }
+  if (warp == Cfg::kLoadWarp && lane == 0) { tma_prefetch_desc(&maps.q); tma_prefetch_desc(&maps.k); tma_prefetch_desc(&maps.v); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
 
-  // The work item: split x kv head x sequence x pair of tiles, the last queries first (they see the most keys under a causal mask).
-  const int split = blockIdx.x % a.splits;
-  uint32_t item = blockIdx.x / a.splits;
-  const int kv = item % a.kv_heads;
-  item /= a.kv_heads;
-  const int b = item % a.sequences;
-  const int pair = a.pairs - 1 - (int)(item / a.sequences);
-  const AttendSequence s = attend_sequence(a, b);
-  const int all_queries = s.queries ? a.lengths[b] : 0;
+  // The work item: split x kv head x sequence x group of tiles, the last queries first (they see the most keys under a causal mask).
+  uint32_t item = a.by_splits.div(blockIdx.x);
+  const int split = blockIdx.x - item * a.splits;
+  const uint32_t of_kv = a.by_kv.div(item);
+  const int kv = item - of_kv * a.kv_heads;
+  const uint32_t of_sequence = a.by_sequences.div(of_kv);
+  const int b = of_kv - of_sequence * a.sequences;
+  const int pair = a.pairs - 1 - (int)of_sequence;
+  int all_queries;
+  const AttendSequence s = attend_sequence(a, b, &all_queries);
   const int offset = s.keys - all_queries;  // a query's position less its number
-  const int per_tile = kAtRows / a.group, first = 2 * pair * per_tile;
-  const int tokens[2] = {max(0, min(per_tile, s.queries - first)), max(0, min(per_tile, s.queries - first - per_tile))};
-  const bool idle = tokens[0] == 0, few = tokens[1] == 0;  // of all CTAs of the cluster alike
+  const int per_tile = a.per_tile, first = NT * pair * per_tile;
+  const int tokens[2] = {max(0, min(per_tile, s.queries - first)), NT == 1 ? 0 : max(0, min(per_tile, s.queries - first - per_tile))};
+  const bool idle = tokens[0] == 0, few = NT == 2 && tokens[1] == 0;  // of all CTAs of the cluster alike
   const int nk = (a.dim + 15) / 16;  // depth steps of 16 values
   const int halves = a.dim > 64 ? 2 : 1;
 
@@ -282,7 +300,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
   AttendSpan outer[2], inner[2];
   int from = INT_MAX, to = -1;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < NT; ++t) {
     outer[t] = inner[t] = {1, 0};
     if (!tokens[t]) continue;
     const int p0 = first + t * per_tile + offset;
@@ -303,14 +321,14 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
   const bool joined = !idle && (a.splits > 1 || dual);  // the rows' results are in parts
   float* part = reinterpret_cast<float*>(smem + Cfg::kOffK);  // unnormalised rows of O, once all products are done
 
-  if (!idle && warp < kAtSoftmax) {
+  if (!idle && warp < Cfg::kSoftmax) {
     // ---- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    const int t = warp >> 2, row = (warp & 3) * 32 + lane, tile = few ? 0 : t;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kSoftmaxRegs));
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane, tile = few ? 0 : t;  // (t is 0 with one tile)
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + lane_addr + t * 128, o_tmem = tmem + lane_addr + Cfg::kTmemO + t * DP;
     const uint32_t p_tmem = s_tmem;
-    const int tile_token = row / a.group, head = kv * a.group + row - tile_token * a.group;
+    const int tile_token = a.by_group.div(row), head = kv * a.group + row - tile_token * a.group;
     const int query = first + tile * per_tile + tile_token;
     const bool live = tile_token < tokens[tile];
     const bool warp_live = __any_sync(0xffffffffu, live);
@@ -544,7 +562,8 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
       const bool any = l > 0.f || l != l;
       const float inv = any ? 1.f / l : 0.f;
       bool fine = l - l == 0.f;
-      T* out = static_cast<T*>(a.out) + token * a.out_token + head * a.out_head;
+      // Through the tile's Q in shared memory, which no product reads any more: 8 lanes then write 128 bytes of a row.
+      uint8_t* stage = smem + Cfg::kOffQ + t * Cfg::kQTile;
 #pragma unroll 1
       for (int c = 0; c < a.dim; c += 32) {
         uint32_t o[32];
@@ -559,9 +578,23 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
             if (c + i < a.dim) fine = fine && x - x == 0.f && y - y == 0.f;
             w[k] = pack2<T>(x, y);
           }
-          if (live && c + i < a.dim) *reinterpret_cast<uint4*>(out + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+          const int at_c = c + i;  // 16 bytes: value at_c of the row
+          *reinterpret_cast<uint4*>(stage + (at_c >> 6) * Cfg::kQHalf + row * 128 + (((at_c & 63) * 2) ^ ((row & 7) << 4))) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
+      __syncwarp();
+      for (int h = 0; h < halves; ++h) {
+        const int at_c = 64 * h + (lane & 7) * 8;
+#pragma unroll 4
+        for (int i = 0; i < 32; i += 4) {
+          const int r = (warp & 3) * 32 + i + (lane >> 3);
+          const int tok = a.by_group.div(r), hd = kv * a.group + r - tok * a.group;
+          if (tok < tokens[tile] && at_c < a.dim)
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (int64_t)(s.q_start + first + tile * per_tile + tok) * a.out_token + hd * a.out_head + at_c) =
+                *reinterpret_cast<const uint4*>(stage + h * Cfg::kQHalf + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+        }
+      }
+      __syncwarp();
       if (live && a.lse)
         a.lse[token * a.heads + head] = any ? (kGeneral ? m : m / kLog2e) + (log2f(l) - kShift) / kLog2e : -INFINITY;
       // A value that is not finite may come from a key that this row's mask hides (its weight of zero times that value): such rows
@@ -572,12 +605,12 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
       }
     }
   } else if (!idle) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == kAtLoadWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kOtherRegs));
+    if (warp == Cfg::kLoadWarp) {
       // ---- steps and loads
       int doc_lo[2] = {INT_MAX, INT_MAX}, doc_hi[2] = {INT_MIN, INT_MIN};
       if (elect_one())
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
           if (tokens[t]) {
             mbar_arrive_expect_tx(q_full + t, halves * 128 * a.group * per_tile);
             for (int h = 0; h < halves; ++h)
@@ -586,7 +619,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
           }
       __syncwarp();
       if (a.documents)
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < NT; ++t) {
           for (int i = lane; i < tokens[t]; i += 32) {
             const int d = a.documents[s.q_start + first + t * per_tile + i];
             doc_lo[t] = min(doc_lo[t], d);
@@ -632,9 +665,9 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (!__all_sync(0xffffffffu, d[i] == __shfl_sync(0xffffffffu, d[i], 0))) mixed |= 1 << i;
-        int cls[2];
+        int cls[2] = {kAtSkip, kAtSkip};
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < NT; ++t) {
           const bool in_prefix = kb < prefix, whole_prefix = kb + kAtKeys <= prefix;
           const bool meets = kb <= outer[t].hi && last >= outer[t].lo && (!a.documents || (lo <= doc_hi[t] && hi >= doc_lo[t]));
           const bool whole = kb >= inner[t].lo && kb + kAtKeys - 1 <= inner[t].hi &&
@@ -665,12 +698,12 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
       __syncwarp();
       if (*abort_flag) {
         // Copies that nothing waits for any more land before the CTA ends.
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
           if (tokens[t]) mbar_drain(q_full + t, 0);
         for (int i = max(0, k_issued - kSlots); i < k_issued; ++i) mbar_drain(k_full + i % kSlots, (i / kSlots) & 1);
         for (int i = max(0, v_issued - kSlots); i < v_issued; ++i) mbar_drain(v_full + i % kSlots, (i / kSlots) & 1);
       }
-    } else if (warp == kAtMmaWarp) {
+    } else if (warp == Cfg::kMmaWarp) {
       // ---- tensor products
       constexpr uint32_t idesc_s = mma_idesc<kBf16>(kAtRows, kAtKeys);
       const uint32_t idesc_o = mma_idesc<kBf16>(kAtRows, 0) | (uint32_t)(2 * nk) << 17 | 1u << 16;  // N = 16 nk; B by values
@@ -724,10 +757,10 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
       };
       int cur = read(0);
       if (cur != kAtEnd && ok) {
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
           if (tokens[t]) wait(q_full + t, 0);
         wait(k_full, 0);
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
           if (takes(cur, t)) scores(0, t);
         release(k_empty);
         for (int n = 0; ok && cur != kAtEnd; ++n) {
@@ -744,7 +777,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
             fence_proxy_async_smem();
             __syncwarp();
           }
-          for (int t = 0; t < 2; ++t) {
+          for (int t = 0; t < NT; ++t) {
             if (takes(cur, t)) values(n, t);
             if (takes(next, t)) scores(n + 1, t);
           }
@@ -753,18 +786,19 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
           cur = next;
         }
       }
-      if (elect_one()) { tc_commit(drain); tc_commit(drain + 1); }
+      if (elect_one())
+        for (int t = 0; t < NT; ++t) tc_commit(drain + t);
       __syncwarp();
-      mbar_drain(drain, 0);
-      mbar_drain(drain + 1, 0);
+      for (int t = 0; t < NT; ++t) mbar_drain(drain + t, 0);
     }
   }
   if (joined) {
-    __syncthreads();  // the products of both tiles are done: the tiles of K and V are free
+    // Every part of the rows into its CTA's shared memory: all products are done, so the tiles of K and V are free.
+    __syncthreads();
     tc_fence_after();
-    if (warp < kAtSoftmax && !*abort_flag) {
+    if (warp < Cfg::kSoftmax) {
       const int t = warp >> 2, row = (warp & 3) * 32 + lane, slot = t * kAtRows + row;
-      const bool live = row / a.group < tokens[few ? 0 : t];
+      const bool live = (int)a.by_group.div(row) < tokens[few ? 0 : t];
       if (__any_sync(0xffffffffu, live)) {
 #pragma unroll 1
         for (int c = 0; c < a.dim; c += 32) {
@@ -781,56 +815,69 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
     tc_fence_before();
     if (a.splits > 1) cluster_sync();
     else __syncthreads();
-    // Each warp of the cluster joins the parts of its share of the rows.
-    if (warp < kAtSoftmax && !*abort_flag) {
-      const uint32_t part_addr = smem_u32(part), sums_addr = smem_u32(sums);
-      const int rows0 = tokens[0] * a.group, rows = rows0 + tokens[1] * a.group, parts = few ? 2 * a.splits : a.splits;
-      for (int r = split * kAtSoftmax + warp; r < rows; r += kAtSoftmax * a.splits) {
-        const int tile = r >= rows0, at_row = tile ? r - rows0 : r;
-        auto slot_of = [&](int c) { return (few ? c & 1 : tile) * kAtRows + at_row; };
-        auto rank_of = [&](int c) { return few ? c >> 1 : c; };
-        // A lane per part for the maximum and the sum (16 parts at most).
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < parts) ml = ld_cluster_v2(cluster_addr(sums_addr + slot_of(lane) * 8, rank_of(lane)));
-        float top = ml.x;
-#pragma unroll
-        for (int w = 8; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-        top = __shfl_sync(0xffffffffu, top, 0);
-        const bool none = ml.x == -INFINITY && ml.y == 0.f;  // saw nothing: its O is not defined
-        const float weight = none ? 0.f : ex2_approx(kGeneral ? (ml.x - top) * kLog2e : ml.x - top);
-        const uint32_t some = __ballot_sync(0xffffffffu, !none);
-        float sum = 0.f, o[DP / 32] = {};
-        for (uint32_t left = some; left; left &= left - 1) {
-          const int c = __ffs(left) - 1;
-          const float w = __shfl_sync(0xffffffffu, weight, c);
-          sum = fmaf(__shfl_sync(0xffffffffu, ml.y, c), w, sum);
-#pragma unroll
-          for (int i = 0; i < DP / 64; ++i) {
-            const int d = 2 * lane + 64 * i;
-            if (d < a.dim) {
-              const float2 x = ld_cluster_v2(cluster_addr(part_addr + (slot_of(c) * DP + ((d / 4) ^ (at_row & 7)) * 4 + d % 4) * 4, rank_of(c)));
-              o[2 * i] = fmaf(x.x, w, o[2 * i]);
-              o[2 * i + 1] = fmaf(x.y, w, o[2 * i + 1]);
-            }
-          }
+    // Each CTA joins its share of the rows: their parts' weights, then the rows.  `fine` has a word for each row, 0 where a value is not finite.
+    const int rows0 = tokens[0] * a.group, rows = rows0 + tokens[1] * a.group, parts = few ? 2 * a.splits : a.splits;
+    const int share = (rows + a.splits - 1) / a.splits, row0 = split * share, mine = max(0, min(share, rows - row0));
+    float* weights = reinterpret_cast<float*>(smem + Cfg::kOffWeights);  // [parts][share]
+    volatile int* fine = docs;
+    static_assert(kAtInfo * kAtKeys >= 2 * kAtRows, "a word per row");
+    const uint32_t part_addr = smem_u32(part), sums_addr = smem_u32(sums);
+    auto slot_of = [&](int r, int c) { return few ? (c & 1) * kAtRows + r : r >= rows0 ? kAtRows + r - rows0 : r; };
+    auto rank_of = [&](int c) { return few ? c >> 1 : c; };
+    auto place = [&](int r, int* query, int* head) {
+      const int at_row = r >= rows0 ? r - rows0 : r, tok = a.by_group.div(at_row);
+      *query = first + (r >= rows0 ? per_tile : 0) + tok;
+      *head = kv * a.group + at_row - tok * a.group;
+    };
+    if (!*abort_flag)
+      for (int i = threadIdx.x; i < mine; i += Cfg::kThreads) {
+        const int r = row0 + i;
+        float top = -INFINITY, sum = 0.f;
+        for (int c = 0; c < parts; ++c) top = fmaxf(top, ld_cluster_v2(cluster_addr(sums_addr + slot_of(r, c) * 8, rank_of(c))).x);
+        for (int c = 0; c < parts; ++c) {
+          const float2 ml = ld_cluster_v2(cluster_addr(sums_addr + slot_of(r, c) * 8, rank_of(c)));
+          // A part that saw nothing has no weight, and its O holds anything.
+          const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2_approx(kGeneral ? (ml.x - top) * kLog2e : ml.x - top);
+          weights[c * share + i] = w;
+          sum = fmaf(ml.y, w, sum);
         }
         const bool any = sum > 0.f || sum != sum;
         const float inv = any ? 1.f / sum : 0.f;
-        bool fine = sum - sum == 0.f;
-        const int tok = at_row / a.group, h = kv * a.group + at_row - tok * a.group, qi = first + tile * per_tile + tok;
-        T* out = static_cast<T*>(a.out) + (int64_t)(s.q_start + qi) * a.out_token + h * a.out_head;
-#pragma unroll
-        for (int i = 0; i < DP / 64; ++i) {
-          const int d = 2 * lane + 64 * i;
-          const float x = o[2 * i] * inv, y = o[2 * i + 1] * inv;
-          fine = fine && x - x == 0.f && y - y == 0.f;
-          if (d < a.dim) *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(x, y);
-        }
-        if (a.lse && lane == 0)
+        for (int c = 0; c < parts; ++c) weights[c * share + i] *= inv;
+        fine[i] = sum - sum == 0.f;
+        if (a.lse) {
+          int qi, h;
+          place(r, &qi, &h);
           a.lse[(int64_t)(s.q_start + qi) * a.heads + h] = any ? (kGeneral ? top : top / kLog2e) + (log2f(sum) - kShift) / kLog2e : -INFINITY;
-        if (__any_sync(0xffffffffu, !fine)) attend_row<T>(a, s, all_queries, qi, h);
+        }
       }
-    }
+    __syncthreads();
+    if (!*abort_flag)
+      for (int i = threadIdx.x; i < mine * (DP / 4); i += Cfg::kThreads) {
+        const int at_row = i / (DP / 4), dv = i % (DP / 4), r = row0 + at_row;
+        if (4 * dv >= a.dim) continue;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < parts; ++c) {
+          const float w = weights[c * share + at_row];
+          const int slot = slot_of(r, c);
+          if (w == 0.f) continue;
+          const float4 x = ld_cluster_v4(cluster_addr(part_addr + (slot * DP + (dv ^ (slot & 7)) * 4) * 4, rank_of(c)));
+          o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
+        }
+        if (!(o.x - o.x == 0.f && o.y - o.y == 0.f && o.z - o.z == 0.f && o.w - o.w == 0.f)) fine[at_row] = 0;
+        int qi, h;
+        place(r, &qi, &h);
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(s.q_start + qi) * a.out_token + h * a.out_head + 4 * dv) =
+            make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
+      }
+    __syncthreads();
+    if (warp < Cfg::kSoftmax && !*abort_flag)
+      for (int i = warp; i < mine; i += Cfg::kSoftmax)
+        if (!fine[i]) {
+          int qi, h;
+          place(row0 + i, &qi, &h);
+          attend_row<T>(a, s, all_queries, qi, h);
+        }
   }
   if (a.splits > 1) {
     if (idle) cluster_sync();
@@ -839,7 +886,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) attend_kernel(const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kAtMmaWarp) tmem_dealloc(tmem, 512);
+  if (warp == Cfg::kMmaWarp) tmem_dealloc(tmem, Cfg::kTmemCols);
 }
 
 }  // namespace laya

@@ -9,6 +9,12 @@
 
 using namespace laya;
 
+#ifndef AT_NT64
+#define AT_NT64 1
+#endif
+#ifndef AT_NT128
+#define AT_NT128 2
+#endif
 namespace {
 
 // A tensor [tokens][heads][dim], strides in elements.
@@ -57,15 +63,16 @@ CUtensorMap heads_map(bool bf16, const void* p, int dim, int heads, int tokens, 
   return map;
 }
 
-template <typename T, int DP, int kMode>
+template <typename T, int DP, int NT, int kMode>
 void launch_attend_kernel(const AttendArgs& a, const AttendMaps& maps, int64_t ctas, int dev, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  auto kern = attend_kernel<T, DP, kMode>;
-  allow_smem(kern, AttendCfg<DP>::kBytes, dev, done);
+  using Cfg = AttendCfg<DP, NT>;
+  auto kern = attend_kernel<T, DP, NT, kMode>;
+  allow_smem(kern, Cfg::kBytes, dev, done);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kAtThreads);
-  cfg.dynamicSmemBytes = AttendCfg<DP>::kBytes;
+  cfg.blockDim = dim3(Cfg::kThreads);
+  cfg.dynamicSmemBytes = Cfg::kBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -85,26 +92,30 @@ void launch_attend_kernel(const AttendArgs& a, const AttendMaps& maps, int64_t c
   CK(cudaLaunchKernelEx(&cfg, kern, maps, a));
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int NT>
 void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  const int per_tile = kAtRows / a.group;
-  a.pairs = (a.max_queries + 2 * per_tile - 1) / (2 * per_tile);
+  a.per_tile = kAtRows / a.group;
+  a.pairs = (a.max_queries + NT * a.per_tile - 1) / (NT * a.per_tile);
   const int64_t items = (int64_t)a.pairs * a.sequences * a.kv_heads;
   const int blocks = (max_keys + kAtKeys - 1) / kAtKeys, sms = sm_count(dev);
   a.splits = 1;
-  while (a.splits < 8 && items * a.splits * 2 <= sms && a.splits * 4 <= blocks) a.splits *= 2;
-  if (items * a.splits > INT32_MAX) fail(LAYA_ERR_INVALID, "%d queries of %d sequences and %d heads are too many for one call", a.max_queries, a.sequences, a.heads);
+  while (a.splits < kAtMostSplits && items * a.splits * 2 <= sms && a.splits * 4 <= blocks) a.splits *= 2;
+  const int64_t ctas = items * a.splits;
+  if (ctas > INT32_MAX) fail(LAYA_ERR_INVALID, "%d queries of %d sequences and %d heads are too many for one call", a.max_queries, a.sequences, a.heads);
+  a.by_group = FastDiv(a.group);
+  a.by_splits = FastDiv(a.splits);
+  a.by_kv = FastDiv(a.kv_heads);
+  a.by_sequences = FastDiv(a.sequences);
   AttendMaps maps;
-  maps.q = heads_map(kBf16, a.q, a.dim, a.heads, a.q_tokens, a.q_head, a.q_token, a.group, per_tile);
+  maps.q = heads_map(kBf16, a.q, a.dim, a.heads, a.q_tokens, a.q_head, a.q_token, a.group, a.per_tile);
   // Without a key there is nothing to load: any map will do.
   maps.k = a.k_tokens ? heads_map(kBf16, a.k, a.dim, a.kv_heads, a.k_tokens, a.k_head, a.k_token, 1, kAtKeys) : maps.q;
   maps.v = a.k_tokens ? heads_map(kBf16, a.v, a.dim, a.kv_heads, a.k_tokens, a.v_head, a.v_token, 1, kAtKeys) : maps.q;
-  const int64_t ctas = items * a.splits;
-  if (a.table || !(a.scale > 0.f) || (a.slopes && a.cap > 0.f)) launch_attend_kernel<T, DP, kAtGeneral>(a, maps, ctas, dev, st);
-  else if (a.slopes) launch_attend_kernel<T, DP, kAtSlopes>(a, maps, ctas, dev, st);
-  else if (a.cap > 0.f) launch_attend_kernel<T, DP, kAtCap>(a, maps, ctas, dev, st);
-  else launch_attend_kernel<T, DP, kAtPlain>(a, maps, ctas, dev, st);
+  if (a.table || !(a.scale > 0.f) || (a.slopes && a.cap > 0.f)) launch_attend_kernel<T, DP, NT, kAtGeneral>(a, maps, ctas, dev, st);
+  else if (a.slopes) launch_attend_kernel<T, DP, NT, kAtSlopes>(a, maps, ctas, dev, st);
+  else if (a.cap > 0.f) launch_attend_kernel<T, DP, NT, kAtCap>(a, maps, ctas, dev, st);
+  else launch_attend_kernel<T, DP, NT, kAtPlain>(a, maps, ctas, dev, st);
 }
 
 }  // namespace
@@ -189,7 +200,7 @@ int laya_op_attend(const laya_attend* p, int* err, void* stream) {
   if (!p->k_starts != !p->k_lengths) fail(LAYA_ERR_INVALID, "k_starts and k_lengths go together");
   if (!p->sequences || !p->q_tokens || !p->max_queries) return LAYA_OK;
   if (!p->starts || !p->lengths) fail(LAYA_ERR_INVALID, "starts or lengths is null");
-  AttendArgs a{};
+  AttendArgs a = {};
   a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.lse = p->lse;
   a.q_token = p->q_token; a.q_head = p->q_head; a.k_token = p->k_token; a.k_head = p->k_head;
   a.v_token = p->v_token; a.v_head = p->v_head; a.out_token = p->out_token; a.out_head = p->out_head;
@@ -213,8 +224,9 @@ int laya_op_attend(const laya_attend* p, int* err, void* stream) {
   a.wait_ns = wait_ns();
   with_half(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (a.dim > 64) launch_attend<T, 128>(a, std::min(p->max_keys, p->k_tokens), current_device(st), st);
-    else launch_attend<T, 64>(a, std::min(p->max_keys, p->k_tokens), current_device(st), st);
+    const int dev = current_device(st), max_keys = std::min(p->max_keys, p->k_tokens);
+    if (a.dim > 64) launch_attend<T, 128, AT_NT128>(a, max_keys, dev, st);
+    else launch_attend<T, 64, AT_NT64>(a, max_keys, dev, st);
   });
   OP_API_END
 }

@@ -37,6 +37,18 @@ __device__ __forceinline__ unsigned long long global_ns() {
   return t;
 }
 
+// Division by a number that the kernel gets: n / d for n below 2^31 as a high product, a sum and a shift
+// (Granlund and Montgomery, "Division by invariant integers using multiplication").
+struct FastDiv {
+  uint32_t d, m, s;
+  FastDiv() : FastDiv(1) {}
+  explicit FastDiv(uint32_t divisor) : d(divisor), m(0), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

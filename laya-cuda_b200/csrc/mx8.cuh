@@ -276,17 +276,6 @@ inline bool rows_vectored(const T* p, int64_t ld, int cols) {
   return reinterpret_cast<uintptr_t>(p) % 32 == 0 && ld * (int64_t)sizeof(T) % 32 == 0 && cols % kMxPiece == 0;
 }
 
-// Division by a number that the kernel gets: n / d for n below 2^31 as a high product, a sum and a shift
-// (Granlund and Montgomery, "Division by invariant integers using multiplication").
-struct FastDiv {
-  uint32_t d, m, s;
-  explicit FastDiv(uint32_t divisor) : d(divisor), m(0), s(0) {
-    while ((1ull << s) < d) ++s;
-    m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
-};
-
 // Writes a piece as MX8.  Two neighbouring threads hold a block and eight a scale tile's 128 columns;
 // all 32 threads of the warp call this together, with zeros in columns past the last.  `col` may be past the last
 // column, and past 2^31 with it.
