@@ -27,6 +27,7 @@ struct AttendArgs {
   int* err;
   unsigned long long wait_ns;
   int per_tile;       // queries of a tile, which holds all heads of a group for each
+  int table_here, table_pad;  // the distance bias fits shared memory; values between its heads there
   int pairs, splits;  // CTAs for max_queries of a kv head; CTAs (a cluster) that share a tile's keys
   FastDiv by_group, by_splits, by_kv, by_sequences;
 };
@@ -118,8 +119,9 @@ __device__ void attend_row(const AttendArgs& a, const AttendSequence& s, int ful
 // O of each; P goes over S as 16-bit pairs.  The tensor core runs the products in issue order, so O += P V of a step and then S = Q K^T
 // of the next are issued together as soon as P is there, and the other tile's softmax hides them.
 //
-// Where one tile holds all rows (single tokens over a cache), both tiles take them, and each every other step; the two parts
-// are joined at the end as the parts of a split are.
+// Where one tile holds all rows, both take them, and each every other step; the parts are joined at the end as those of a split
+// are.  Where a quarter of a tile holds them (single tokens over a cache), each quarter has a copy of them and takes a quarter of
+// a step's keys: a softmax thread then has 32 scores of a step to do and not 128.
 // ---------------------------------------------------------------------------------------------
 constexpr int kAtRows = 128;       // rows of a tile
 constexpr int kAtKeys = 128;       // keys of a step
@@ -131,8 +133,9 @@ enum AtClass : int { kAtEnd = -1, kAtSkip = 0, kAtMasked = 1, kAtFull = 2 };
 enum AtMode { kAtPlain, kAtCap, kAtSlopes, kAtGeneral };
 
 constexpr int kAtMostSplits = 8;
+constexpr int kAtMostTable = 4096;  // values of the distance bias that are kept in shared memory, clamped past the reach
 
-// NT tiles per CTA, heads padded to DP values.
+// NT tiles per CTA, heads padded to DP values; kQuarters: all rows in a quarter of a tile.
 template <int DP, int NT>
 struct AttendCfg {
   static_assert((DP == 64 || DP == 128) && (NT == 1 || NT == 2), "padded head size, tiles");
@@ -149,12 +152,13 @@ struct AttendCfg {
   static constexpr int kOffQ = 0, kOffK = NT * kQTile, kOffV = kOffK + kSlots * kTile;
   static constexpr int kOffDocs = kOffV + kSlots * kTile;
   static constexpr int kOffBar = kOffDocs + kAtInfo * kAtKeys * 4;
-  static constexpr int kBars = 2 + 4 * kSlots + 2 * kAtInfo + 6;
+  static constexpr int kBars = 2 + 4 * kSlots + 2 * kAtInfo + 7;
   static constexpr int kOffInfo = kOffBar + kBars * 8;
   static constexpr int kOffSums = kOffInfo + kAtInfo * 4 + 16;  // (maximum, sum) of each row, where results are joined
   static constexpr int kWeights = 2 * NT * kAtRows + 2 * kAtMostSplits;  // of the parts of the rows that a CTA joins
   static constexpr int kOffWeights = kOffSums + NT * kAtRows * 8;
-  static constexpr int kBytes = kOffWeights + kWeights * 4 + 1024;
+  static constexpr int kOffTable = kOffWeights + kWeights * 4;
+  static constexpr int kBytes = kOffTable + kAtMostTable * 4 + 1024;
   static_assert(kOffSums % 8 == 0, "alignment");
   static_assert(NT * kAtRows * DP * 4 <= 2 * kSlots * kTile, "a part's O fits the K and V tiles");
   static_assert(kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory");
@@ -235,7 +239,7 @@ struct CapTerms {
 };
 
 // T, the padded head size, and what is done to the scores.
-template <typename T, int DP, int NT, int kMode>
+template <typename T, int DP, int NT, int kMode, bool kQuarters>
 __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>::kCtas)
     attend_kernel(const __grid_constant__ AttendMaps maps, const __grid_constant__ AttendArgs a) {
   using Cfg = AttendCfg<DP, NT>;
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
   uint64_t *q_full = bar, *k_full = bar + 2, *k_empty = k_full + kSlots, *v_full = k_empty + kSlots, *v_empty = v_full + kSlots,
-           *info_full = v_empty + kSlots, *info_empty = info_full + kAtInfo, *s_full = info_empty + kAtInfo, *p_full = s_full + 2, *drain = p_full + 2;
+           *info_full = v_empty + kSlots, *info_empty = info_full + kAtInfo, *s_full = info_empty + kAtInfo, *p_full = s_full + 2, *drain = p_full + 2, *table_full = drain + 2;
   volatile int* info = reinterpret_cast<volatile int*>(smem + Cfg::kOffInfo);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffInfo + kAtInfo * 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -266,6 +270,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       mbar_init(drain + t, 1);
     }
     for (int i = 0; i < kSlots; ++i) { mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1); }
+    mbar_init(table_full, Cfg::kSoftmax);
     for (int i = 0; i < kAtInfo; ++i) { mbar_init(info_full + i, 1); mbar_init(info_empty + i, Cfg::kSoftmax + 1); }
     *abort_flag = 0;
     fence_mbar_init();
@@ -318,17 +323,20 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     end = min(end, at + share);
   }
   const bool dual = few && end - at > 1;            // both tiles take the rows of the first, each every other step
-  const bool joined = !idle && (a.splits > 1 || dual);  // the rows' results are in parts
+  const bool joined = !idle && (a.splits > 1 || dual || kQuarters);  // the rows' results are in parts
   float* part = reinterpret_cast<float*>(smem + Cfg::kOffK);  // unnormalised rows of O, once all products are done
 
   if (!idle && warp < Cfg::kSoftmax) {
     // ---- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kSoftmaxRegs));
-    const int t = warp >> 2, row = (warp & 3) * 32 + lane, tile = few ? 0 : t;  // (t is 0 with one tile)
-    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+    const int t = warp >> 2, quarter = warp & 3, tile = few ? 0 : t;
+    const int row = quarter * 32 + lane, row_of_tile = kQuarters ? lane : row;
+    constexpr int NC = kQuarters ? 1 : 4;     // chunks of 32 keys of a step that this thread takes,
+    const int chunk0 = kQuarters ? quarter : 0;  // from this one on
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tmem = tmem + lane_addr + t * 128, o_tmem = tmem + lane_addr + Cfg::kTmemO + t * DP;
     const uint32_t p_tmem = s_tmem;
-    const int tile_token = a.by_group.div(row), head = kv * a.group + row - tile_token * a.group;
+    const int tile_token = a.by_group.div(row_of_tile), head = kv * a.group + row_of_tile - tile_token * a.group;
     const int query = first + tile * per_tile + tile_token;
     const bool live = tile_token < tokens[tile];
     const bool warp_live = __any_sync(0xffffffffu, live);
@@ -341,13 +349,26 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     const float scale = a.scale * kUnit;
     const float slope = (kMode == kAtSlopes || kGeneral) && live && a.slopes ? a.slopes[head] * kUnit : 0.f;
     const float* table = kGeneral && a.table ? a.table + (int64_t)(live ? head : 0) * (2 * a.reach + 1) + a.reach : nullptr;
+    // The distance bias of the group's heads in shared memory, with the edges' values as far past the reach as a tile and a step make.
+    const int wide = 2 * (a.reach + kAtKeys + kAtRows) + a.table_pad;
+    const bool table_here = kGeneral && a.table_here;
+    const float* near = reinterpret_cast<const float*>(smem + Cfg::kOffTable) + (head - kv * a.group) * wide + a.reach + kAtKeys + kAtRows;
+    if (table_here) {
+      float* to = reinterpret_cast<float*>(smem + Cfg::kOffTable);
+      for (int i = threadIdx.x; i < a.group * wide; i += 32 * Cfg::kSoftmax) {
+        const int g = i / wide, at_d = i - g * wide - (a.reach + kAtKeys + kAtRows);
+        to[i] = __ldg(a.table + (int64_t)(kv * a.group + g) * (2 * a.reach + 1) + a.reach + min(max(at_d, -a.reach), a.reach));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(table_full);
+    }
     const bool capped = kMode == kAtCap || (kGeneral && a.cap > 0.f);
     const CapTerms cap(capped ? a.scale / a.cap : 0.f, a.cap * kUnit);
-    bool ok = true;
+    bool ok = !table_here || mbar_wait(table_full, 0, a.err, kErrAttnWait, abort_flag, wait_ns);
     int count = 0;  // steps of this tile
     for (int n = 0;; ++n) {
       const int e = n % kAtInfo;
-      ok = mbar_wait(info_full + e, (n / kAtInfo) & 1, a.err, kErrAttnWait, abort_flag, wait_ns);
+      ok = ok && mbar_wait(info_full + e, (n / kAtInfo) & 1, a.err, kErrAttnWait, abort_flag, wait_ns);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       const int x = info[e];
       if (x == kAtEnd) break;
@@ -357,19 +378,19 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         if (lane == 0) mbar_arrive(info_empty + e);
         continue;
       }
-      // `whole` has a bit for each chunk of 32 keys that all rows see whole.
-      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u}, whole = 15;
+      // `whole`: all rows of the warp see all of its keys; otherwise `bits` says for each chunk of 32 what this row sees.
+      uint32_t bits[NC];
+      bool whole = true;
       if (cls == kAtMasked && warp_live) {
-        whole = 0;
         const int mixed = x >> 4 & 15;  // chunks with keys of several documents
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int kc = kb + 32 * c;
+        for (int c = 0; c < NC; ++c) {
+          const int kc = kb + 32 * (chunk0 + c);
           bits[c] = low_bits(span.hi + 1 - kc) & ~low_bits(span.lo - kc);
           if (a.documents) {
-            const int* dc = docs + e * kAtKeys + 32 * c;
+            const int* dc = docs + e * kAtKeys + 32 * (chunk0 + c);
             uint32_t same = dc[0] == doc ? ~0u : 0u;
-            if ((mixed >> c) & 1) {
+            if ((mixed >> (chunk0 + c)) & 1) {
               same = 0;
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
@@ -380,8 +401,9 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
             bits[c] &= same;
           }
           bits[c] |= low_bits(below - kc);
-          if (__all_sync(0xffffffffu, bits[c] == ~0u || !live)) whole |= 1u << c;
+          whole = whole && bits[c] == ~0u;
         }
+        whole = __all_sync(0xffffffffu, whole || !live);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(info_empty + e);
@@ -394,19 +416,28 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         if (lane == 0) mbar_arrive(p_full + t);
         continue;
       }
-      uint32_t sx[4][32];
+      uint32_t sx[NC][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32_async(s_tmem + 32 * c, sx[c]);
+      for (int c = 0; c < NC; ++c) tmem_ld32_async(s_tmem + 32 * (chunk0 + c), sx[c]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_wait_ld(sx[c]);
-      const int d = kb - p;  // the step's first key less the query
+      for (int c = 0; c < NC; ++c) tmem_wait_ld(sx[c]);
+      if (kQuarters) {
+        // No P for the keys of the other quarters.
+        uint32_t none[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) none[i] = 0u;
+#pragma unroll
+        for (int c = 1; c < 4; ++c) tmem_st16(p_tmem + 16 * ((chunk0 + c) & 3), none);
+      }
+      constexpr int kMine = 32 * NC;              // keys of this thread
+      const int d = kb + 32 * chunk0 - p;  // the first less the query
       float sum = 0.f;
       // P from the exponents that f gives of the scores, to TMEM; the largest exponent.  kMasked: of the keys that `bits` shows.
       auto numerators = [&](auto masked, auto f) {
         float2 part[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < NC; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
@@ -420,7 +451,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
             part[(i >> 1) & 3] = add2(part[(i >> 1) & 3], w);
             pk[i >> 1] = pack2<T>(w.x, w.y);
           }
-          tmem_st16(p_tmem + 16 * c, pk);
+          tmem_st16(p_tmem + 16 * (chunk0 + c), pk);
         }
         const float2 both = add2(add2(part[0], part[1]), add2(part[2], part[3]));
         sum = both.x + both.y;
@@ -429,7 +460,8 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       // A step relative to the maximum of the steps before, from the products at once: the exponents' maximum, found beside them,
       // tells whether it will do (few steps raise it by more than kAtRescale).
       auto at_once = [&](auto masked) {
-        const float2 by = make_float2(scale, scale), less = make_float2(kShift - m, kShift - m);
+        const float base = m == -INFINITY ? 0.f : m;  // (rows that have seen nothing yet, and see nothing of this step)
+        const float2 by = make_float2(scale, scale), less = make_float2(kShift - base, kShift - base);
         float most = INFINITY;
         if (kMode == kAtPlain) {
           most = numerators(masked, [&](float2 y, int) { return fma2(y, by, less); });
@@ -439,9 +471,9 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           if (!(big <= cap.most)) most = INFINITY;
         } else if (kMode == kAtSlopes) {
           // All keys on one side of the query.
-          const bool left = d + kAtKeys - 1 <= 0;
+          const bool left = d + kMine - 1 <= 0;
           if (__all_sync(0xffffffffu, left || d >= 0)) {
-            const float g = left ? slope : -slope, at_d = fmaf(g, (float)d, kShift - m);
+            const float g = left ? slope : -slope, at_d = fmaf(g, (float)d, kShift - base);
             const float2 from = make_float2(at_d, at_d), each = make_float2(g, g);
             most = numerators(masked, [&](float2 y, int i) { return fma2(y, by, fma2(each, make_float2((float)i, (float)(i + 1)), from)); });
           } else {
@@ -451,13 +483,16 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
             });
           }
         } else if (!capped && !a.slopes) {
-          const float2 unit = make_float2(kLog2e, kLog2e), shift = make_float2(kShift, kShift), at_m = make_float2(m, m);
+          const float2 unit = make_float2(kLog2e, kLog2e), shift = make_float2(kShift, kShift), at_m = make_float2(base, base);
           // Past the reach on one side for all rows: one bias.
-          const bool left = table && d + kAtKeys - 1 <= -a.reach;
+          const bool left = table && d + kMine - 1 <= -a.reach;
           if (!table || __all_sync(0xffffffffu, left || d >= a.reach)) {
             const float edge = !table ? 0.f : __ldg(table + (left ? -a.reach : a.reach));
             const float2 bias = make_float2(edge, edge);
             most = numerators(masked, [&](float2 y, int) { return fma2(sub2(fma2(y, by, bias), at_m), unit, shift); });
+          } else if (table_here) {
+            // Some row is within the reach of some key, so all are within the reach and a step's and a warp's length of all.
+            most = numerators(masked, [&](float2 y, int i) { return fma2(sub2(fma2(y, by, make_float2(near[d + i], near[d + i + 1])), at_m), unit, shift); });
           } else {
             most = numerators(masked, [&](float2 y, int i) {
               const float2 bias = make_float2(__ldg(table + min(max(d + i, -a.reach), a.reach)), __ldg(table + min(max(d + i + 1, -a.reach), a.reach)));
@@ -468,12 +503,25 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         return __all_sync(0xffffffffu, most <= kShift + kAtRescale || !live);
       };
       bool done = false;
-      if (__all_sync(0xffffffffu, m > -INFINITY || !live)) done = whole == 15 ? at_once(std::false_type{}) : at_once(std::true_type{});
+      const bool fresh = __any_sync(0xffffffffu, m == -INFINITY && live);
+      if ((kMode == kAtPlain || kMode == kAtCap) && fresh && whole) {
+        // A row's first scores: their maximum first.
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (m == -INFINITY && top != -INFINITY) m = kMode == kAtCap ? cap.any(top) : top * scale;
+        done = at_once(std::false_type{});
+      } else if (!fresh) {
+        done = whole ? at_once(std::false_type{}) : at_once(std::true_type{});
+      }
       if (!done) {
         tmem_wait_st();  // before P is written again
         auto each = [&](auto f) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               const float2 y = f(make_float2(__uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1])), 32 * c + i);
@@ -484,7 +532,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         if (capped) {
           float big = 0.f;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int i = 0; i < 32; i += 2) big = max3(big, fabsf(__uint_as_float(sx[c][i])), fabsf(__uint_as_float(sx[c][i + 1])));
           if (__all_sync(0xffffffffu, big <= cap.most)) each([&](float2 y, int) { return mul2(y, cap.slope(y)); });
@@ -501,10 +549,9 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         } else if (kMode == kAtPlain || (kGeneral && !capped)) {
           each([&](float2 y, int) { return mul2(y, by); });
         }
-        if (whole != 15) {
+        if (!whole) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (!((whole >> c) & 1))
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
               for (int i = 0; i < 32; ++i)
                 if (!((bits[c] >> i) & 1)) sx[c][i] = __float_as_uint(-INFINITY);
@@ -513,7 +560,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
 #pragma unroll
         for (int i = 0; i < 8; ++i) mx[i] = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 7] = max3(mx[(i >> 1) & 7], __uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1]));
 #pragma unroll
@@ -561,7 +608,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       const int64_t token = s.q_start + query;
       const bool any = l > 0.f || l != l;
       const float inv = any ? 1.f / l : 0.f;
-      bool fine = l - l == 0.f;
+      float poison = l - l;  // becomes a NaN with a value that is not finite
       // Through the tile's Q in shared memory, which no product reads any more: 8 lanes then write 128 bytes of a row.
       uint8_t* stage = smem + Cfg::kOffQ + t * Cfg::kQTile;
 #pragma unroll 1
@@ -575,7 +622,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const float x = any ? __uint_as_float(o[i + 2 * k]) * inv : 0.f, y = any ? __uint_as_float(o[i + 2 * k + 1]) * inv : 0.f;
-            if (c + i < a.dim) fine = fine && x - x == 0.f && y - y == 0.f;
+            if (c + i < a.dim) poison = fmaf(x, 0.f, fmaf(y, 0.f, poison));
             w[k] = pack2<T>(x, y);
           }
           const int at_c = c + i;  // 16 bytes: value at_c of the row
@@ -599,7 +646,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         a.lse[token * a.heads + head] = any ? (kGeneral ? m : m / kLog2e) + (log2f(l) - kShift) / kLog2e : -INFINITY;
       // A value that is not finite may come from a key that this row's mask hides (its weight of zero times that value): such rows
       // are computed once more, from the visible keys alone.
-      for (uint32_t again = __ballot_sync(0xffffffffu, live && !fine); again; again &= again - 1) {
+      for (uint32_t again = __ballot_sync(0xffffffffu, live && poison != 0.f); again; again &= again - 1) {
         const int src = __ffs(again) - 1;
         attend_row<T>(a, s, all_queries, __shfl_sync(0xffffffffu, query, src), __shfl_sync(0xffffffffu, head, src));
       }
@@ -612,10 +659,12 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       if (elect_one())
         for (int t = 0; t < NT; ++t)
           if (tokens[t]) {
-            mbar_arrive_expect_tx(q_full + t, halves * 128 * a.group * per_tile);
+            constexpr int kCopies = kQuarters ? 4 : 1;
+            mbar_arrive_expect_tx(q_full + t, kCopies * halves * 128 * a.group * per_tile);
             for (int h = 0; h < halves; ++h)
-              tma_load_3d(smem + Cfg::kOffQ + t * Cfg::kQTile + h * Cfg::kQHalf, &maps.q, q_full + t, 64 * h, kv * a.group,
-                          s.q_start + first + t * per_tile);
+              for (int c = 0; c < kCopies; ++c)
+                tma_load_3d(smem + Cfg::kOffQ + t * Cfg::kQTile + h * Cfg::kQHalf + c * 32 * 128, &maps.q, q_full + t, 64 * h, kv * a.group,
+                            s.q_start + first + t * per_tile);
           }
       __syncwarp();
       if (a.documents)
@@ -798,7 +847,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     tc_fence_after();
     if (warp < Cfg::kSoftmax) {
       const int t = warp >> 2, row = (warp & 3) * 32 + lane, slot = t * kAtRows + row;
-      const bool live = (int)a.by_group.div(row) < tokens[few ? 0 : t];
+      const bool live = (int)a.by_group.div(kQuarters ? lane : row) < tokens[few ? 0 : t];
       if (__any_sync(0xffffffffu, live)) {
 #pragma unroll 1
         for (int c = 0; c < a.dim; c += 32) {
@@ -816,39 +865,50 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     if (a.splits > 1) cluster_sync();
     else __syncthreads();
     // Each CTA joins its share of the rows: their parts' weights, then the rows.  `fine` has a word for each row, 0 where a value is not finite.
-    const int rows0 = tokens[0] * a.group, rows = rows0 + tokens[1] * a.group, parts = few ? 2 * a.splits : a.splits;
+    const int rows0 = tokens[0] * a.group, rows = rows0 + tokens[1] * a.group, parts = (kQuarters ? 8 : few ? 2 : 1) * a.splits;
     const int share = (rows + a.splits - 1) / a.splits, row0 = split * share, mine = max(0, min(share, rows - row0));
     float* weights = reinterpret_cast<float*>(smem + Cfg::kOffWeights);  // [parts][share]
     volatile int* fine = docs;
     static_assert(kAtInfo * kAtKeys >= 2 * kAtRows, "a word per row");
     const uint32_t part_addr = smem_u32(part), sums_addr = smem_u32(sums);
-    auto slot_of = [&](int r, int c) { return few ? (c & 1) * kAtRows + r : r >= rows0 ? kAtRows + r - rows0 : r; };
-    auto rank_of = [&](int c) { return few ? c >> 1 : c; };
+    auto slot_of = [&](int r, int c) { return kQuarters ? (c & 7) * 32 + r : few ? (c & 1) * kAtRows + r : r >= rows0 ? kAtRows + r - rows0 : r; };
+    auto rank_of = [&](int c) { return kQuarters ? c >> 3 : few ? c >> 1 : c; };
     auto place = [&](int r, int* query, int* head) {
       const int at_row = r >= rows0 ? r - rows0 : r, tok = a.by_group.div(at_row);
       *query = first + (r >= rows0 ? per_tile : 0) + tok;
       *head = kv * a.group + at_row - tok * a.group;
     };
     if (!*abort_flag)
-      for (int i = threadIdx.x; i < mine; i += Cfg::kThreads) {
+      for (int i = warp; i < mine; i += Cfg::kThreads / 32) {
+        // A lane per part, two where there are more than 32.
         const int r = row0 + i;
-        float top = -INFINITY, sum = 0.f;
-        for (int c = 0; c < parts; ++c) top = fmaxf(top, ld_cluster_v2(cluster_addr(sums_addr + slot_of(r, c) * 8, rank_of(c))).x);
-        for (int c = 0; c < parts; ++c) {
-          const float2 ml = ld_cluster_v2(cluster_addr(sums_addr + slot_of(r, c) * 8, rank_of(c)));
+        float2 ml[2] = {{-INFINITY, 0.f}, {-INFINITY, 0.f}};
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (lane + 32 * k < parts) ml[k] = ld_cluster_v2(cluster_addr(sums_addr + slot_of(r, lane + 32 * k) * 8, rank_of(lane + 32 * k)));
+        float top = fmaxf(ml[0].x, ml[1].x), sum = 0.f, w[2];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
           // A part that saw nothing has no weight, and its O holds anything.
-          const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2_approx(kGeneral ? (ml.x - top) * kLog2e : ml.x - top);
-          weights[c * share + i] = w;
-          sum = fmaf(ml.y, w, sum);
+          w[k] = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : ex2_approx(kGeneral ? (ml[k].x - top) * kLog2e : ml[k].x - top);
+          sum = fmaf(ml[k].y, w[k], sum);
         }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const bool any = sum > 0.f || sum != sum;
         const float inv = any ? 1.f / sum : 0.f;
-        for (int c = 0; c < parts; ++c) weights[c * share + i] *= inv;
-        fine[i] = sum - sum == 0.f;
-        if (a.lse) {
-          int qi, h;
-          place(r, &qi, &h);
-          a.lse[(int64_t)(s.q_start + qi) * a.heads + h] = any ? (kGeneral ? top : top / kLog2e) + (log2f(sum) - kShift) / kLog2e : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (lane + 32 * k < parts) weights[(lane + 32 * k) * share + i] = w[k] * inv;
+        if (lane == 0) {
+          fine[i] = sum - sum == 0.f;
+          if (a.lse) {
+            int qi, h;
+            place(r, &qi, &h);
+            a.lse[(int64_t)(s.q_start + qi) * a.heads + h] = any ? (kGeneral ? top : top / kLog2e) + (log2f(sum) - kShift) / kLog2e : -INFINITY;
+          }
         }
       }
     __syncthreads();
@@ -857,12 +917,12 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         const int at_row = i / (DP / 4), dv = i % (DP / 4), r = row0 + at_row;
         if (4 * dv >= a.dim) continue;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
         for (int c = 0; c < parts; ++c) {
           const float w = weights[c * share + at_row];
           const int slot = slot_of(r, c);
-          if (w == 0.f) continue;
           const float4 x = ld_cluster_v4(cluster_addr(part_addr + (slot * DP + (dv ^ (slot & 7)) * 4) * 4, rank_of(c)));
-          o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
+          if (w != 0.f) { o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w); }
         }
         if (!(o.x - o.x == 0.f && o.y - o.y == 0.f && o.z - o.z == 0.f && o.w - o.w == 0.f)) fine[at_row] = 0;
         int qi, h;

@@ -63,11 +63,11 @@ CUtensorMap heads_map(bool bf16, const void* p, int dim, int heads, int tokens, 
   return map;
 }
 
-template <typename T, int DP, int NT, int kMode>
+template <typename T, int DP, int NT, int kMode, bool kQuarters>
 void launch_attend_kernel(const AttendArgs& a, const AttendMaps& maps, int64_t ctas, int dev, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   using Cfg = AttendCfg<DP, NT>;
-  auto kern = attend_kernel<T, DP, NT, kMode>;
+  auto kern = attend_kernel<T, DP, NT, kMode, kQuarters>;
   allow_smem(kern, Cfg::kBytes, dev, done);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
@@ -92,10 +92,10 @@ void launch_attend_kernel(const AttendArgs& a, const AttendMaps& maps, int64_t c
   CK(cudaLaunchKernelEx(&cfg, kern, maps, a));
 }
 
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, bool kQuarters>
 void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  a.per_tile = kAtRows / a.group;
+  a.per_tile = (kQuarters ? kAtRows / 4 : kAtRows) / a.group;
   a.pairs = (a.max_queries + NT * a.per_tile - 1) / (NT * a.per_tile);
   const int64_t items = (int64_t)a.pairs * a.sequences * a.kv_heads;
   const int blocks = (max_keys + kAtKeys - 1) / kAtKeys, sms = sm_count(dev);
@@ -103,6 +103,9 @@ void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   while (a.splits < kAtMostSplits && items * a.splits * 2 <= sms && a.splits * 4 <= blocks) a.splits *= 2;
   const int64_t ctas = items * a.splits;
   if (ctas > INT32_MAX) fail(LAYA_ERR_INVALID, "%d queries of %d sequences and %d heads are too many for one call", a.max_queries, a.sequences, a.heads);
+  // The heads of a group on different banks for the rows of a warp.
+  a.table_pad = a.group > 1 ? (32 - 2 * a.reach % 32 + 32 / std::min(a.group, 32)) % 32 : 0;
+  a.table_here = a.table && (int64_t)a.group * (2ll * (a.reach + kAtKeys + kAtRows) + a.table_pad) <= kAtMostTable;
   a.by_group = FastDiv(a.group);
   a.by_splits = FastDiv(a.splits);
   a.by_kv = FastDiv(a.kv_heads);
@@ -112,10 +115,10 @@ void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   // Without a key there is nothing to load: any map will do.
   maps.k = a.k_tokens ? heads_map(kBf16, a.k, a.dim, a.kv_heads, a.k_tokens, a.k_head, a.k_token, 1, kAtKeys) : maps.q;
   maps.v = a.k_tokens ? heads_map(kBf16, a.v, a.dim, a.kv_heads, a.k_tokens, a.v_head, a.v_token, 1, kAtKeys) : maps.q;
-  if (a.table || !(a.scale > 0.f) || (a.slopes && a.cap > 0.f)) launch_attend_kernel<T, DP, NT, kAtGeneral>(a, maps, ctas, dev, st);
-  else if (a.slopes) launch_attend_kernel<T, DP, NT, kAtSlopes>(a, maps, ctas, dev, st);
-  else if (a.cap > 0.f) launch_attend_kernel<T, DP, NT, kAtCap>(a, maps, ctas, dev, st);
-  else launch_attend_kernel<T, DP, NT, kAtPlain>(a, maps, ctas, dev, st);
+  if (a.table || !(a.scale > 0.f) || (a.slopes && a.cap > 0.f)) launch_attend_kernel<T, DP, NT, kAtGeneral, kQuarters>(a, maps, ctas, dev, st);
+  else if (a.slopes) launch_attend_kernel<T, DP, NT, kAtSlopes, kQuarters>(a, maps, ctas, dev, st);
+  else if (a.cap > 0.f) launch_attend_kernel<T, DP, NT, kAtCap, kQuarters>(a, maps, ctas, dev, st);
+  else launch_attend_kernel<T, DP, NT, kAtPlain, kQuarters>(a, maps, ctas, dev, st);
 }
 
 }  // namespace
@@ -225,8 +228,12 @@ int laya_op_attend(const laya_attend* p, int* err, void* stream) {
   with_half(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const int dev = current_device(st), max_keys = std::min(p->max_keys, p->k_tokens);
-    if (a.dim > 64) launch_attend<T, 128, AT_NT128>(a, max_keys, dev, st);
-    else launch_attend<T, 64, AT_NT64>(a, max_keys, dev, st);
+    // All rows of a sequence's kv head in a quarter of a tile: single tokens, and a few where the group is small.
+    const bool quarters = (int64_t)a.max_queries * a.group <= kAtRows / 4;
+    if (a.dim > 64 && quarters) launch_attend<T, 128, 2, true>(a, max_keys, dev, st);
+    else if (a.dim > 64) launch_attend<T, 128, AT_NT128, false>(a, max_keys, dev, st);
+    else if (quarters) launch_attend<T, 64, 2, true>(a, max_keys, dev, st);
+    else launch_attend<T, 64, AT_NT64, false>(a, max_keys, dev, st);
   });
   OP_API_END
 }
