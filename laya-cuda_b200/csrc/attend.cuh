@@ -132,7 +132,7 @@ enum AtClass : int { kAtEnd = -1, kAtSkip = 0, kAtMasked = 1, kAtFull = 2 };
 // times the lowest number of a type would be -infinity).
 enum AtMode { kAtPlain, kAtCap, kAtSlopes, kAtGeneral };
 
-constexpr int kAtMostSplits = 8;
+constexpr int kAtMostSplits = 16;
 constexpr int kAtMostTable = 4096;  // values of the distance bias that are kept in shared memory, clamped past the reach
 
 // NT tiles per CTA, heads padded to DP values; kQuarters: all rows in a quarter of a tile.
@@ -142,7 +142,7 @@ struct AttendCfg {
   static constexpr int kSoftmax = 4 * NT;                // softmax warps
   static constexpr int kMmaWarp = kSoftmax, kLoadWarp = kSoftmax + 1, kThreads = 32 * (kSoftmax + 4), kCtas = NT == 1 ? 2 : 1;
   // Registers: what the launch gives all threads (128 with one tile, 168 with two), moved to the softmax.
-  static constexpr int kSoftmaxRegs = NT == 1 ? 200 : 224, kOtherRegs = 56;
+  static constexpr int kSoftmaxRegs = NT == 1 ? 200 : 216, kOtherRegs = NT == 1 ? 56 : 72;
   static_assert(32 * (kSoftmax * kSoftmaxRegs + 4 * kOtherRegs) <= kThreads * (NT == 1 ? 128 : 168), "registers of the launch");
   static constexpr int kTmemO = 128 * NT, kTmemCols = NT == 1 ? 256 : 512;  // columns: O of tile 0, all
   static_assert(kTmemO + NT * DP <= kTmemCols, "tensor memory");
@@ -155,11 +155,12 @@ struct AttendCfg {
   static constexpr int kBars = 2 + 4 * kSlots + 2 * kAtInfo + 7;
   static constexpr int kOffInfo = kOffBar + kBars * 8;
   static constexpr int kOffSums = kOffInfo + kAtInfo * 4 + 16;  // (maximum, sum) of each row, where results are joined
-  static constexpr int kWeights = 2 * NT * kAtRows + 2 * kAtMostSplits;  // of the parts of the rows that a CTA joins
+  static constexpr int kWeights = 2 * NT * kAtRows + 8 * kAtMostSplits;  // of the parts of the rows that a CTA joins
   static constexpr int kOffWeights = kOffSums + NT * kAtRows * 8;
   static constexpr int kOffTable = kOffWeights + kWeights * 4;
   static constexpr int kBytes = kOffTable + kAtMostTable * 4 + 1024;
   static_assert(kOffSums % 8 == 0, "alignment");
+  static_assert(2 * kAtMostSplits <= 32, "a lane per part");
   static_assert(NT * kAtRows * DP * 4 <= 2 * kSlots * kTile, "a part's O fits the K and V tiles");
   static_assert(kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory");
 };
@@ -411,6 +412,18 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_fence_after();
       ++count;
+      // Rows of V past the last key may hold anything: a NaN there, times a weight of zero, would be a NaN.  (Both tiles write the same.)
+      const int rows = s.keys - kb;
+      if (rows < kAtKeys) {
+        const int slot = n % kSlots;
+        ok = mbar_wait(v_full + slot, (n / kSlots) & 1, a.err, kErrAttnWait, abort_flag, wait_ns);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        for (int h = 0; h < halves; ++h) {
+          uint4* tail = reinterpret_cast<uint4*>(smem + Cfg::kOffV + slot * Cfg::kTile + h * Cfg::kHalf + rows * 128);
+          for (int i = row; i < (kAtKeys - rows) * 8; i += kAtRows) tail[i] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
       if (!warp_live) {
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + t);
@@ -753,30 +766,29 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         for (int i = max(0, v_issued - kSlots); i < v_issued; ++i) mbar_drain(v_full + i % kSlots, (i / kSlots) & 1);
       }
     } else if (warp == Cfg::kMmaWarp) {
-      // ---- tensor products
-      constexpr uint32_t idesc_s = mma_idesc<kBf16>(kAtRows, kAtKeys);
-      const uint32_t idesc_o = mma_idesc<kBf16>(kAtRows, 0) | (uint32_t)(2 * nk) << 17 | 1u << 16;  // N = 16 nk; B by values
-      const uint32_t q_addr = smem_u32(smem + Cfg::kOffQ), k_addr = smem_u32(smem + Cfg::kOffK), v_addr = smem_u32(smem + Cfg::kOffV);
-      bool ok = true;
-      int used[2] = {0, 0};  // products P V of each tile
-      auto wait = [&](uint64_t* which, int parity) {
-        ok = ok && mbar_wait(which, parity, a.err, kErrAttnWait, abort_flag, wait_ns);
-        ok = __all_sync(0xffffffffu, ok);
-      };
-      auto read = [&](int n) {
-        const int e = n % kAtInfo;
-        wait(info_full + e, (n / kAtInfo) & 1);
-        int x = kAtEnd;
-        if (ok) x = info[e];
-        __syncwarp();
-        if (ok && lane == 0) mbar_arrive(info_empty + e);
-        return x;
-      };
-      auto takes = [](int x, int t) { return x != kAtEnd && ((x >> 2 * t) & 3); };
-      // S of step n for tile t, over the P whose product has been issued.
-      auto scores = [&](int n, int t) {
-        tc_fence_after();
-        if (ok && elect_one()) {
+      // ---- tensor products, by one thread
+      if (elect_one()) {
+        constexpr uint32_t idesc_s = mma_idesc<kBf16>(kAtRows, kAtKeys);
+        const uint32_t idesc_o = mma_idesc<kBf16>(kAtRows, 0) | (uint32_t)(2 * nk) << 17 | 1u << 16;  // N = 16 nk; B by values
+        const uint32_t q_addr = smem_u32(smem + Cfg::kOffQ), k_addr = smem_u32(smem + Cfg::kOffK), v_addr = smem_u32(smem + Cfg::kOffV);
+        bool ok = true;
+        int used[2] = {0, 0};  // products P V of each tile
+        auto wait = [&](uint64_t* which, int parity) { ok = ok && mbar_wait(which, parity, a.err, kErrAttnWait, abort_flag, wait_ns); };
+        auto read = [&](int n) {
+          const int e = n % kAtInfo;
+          wait(info_full + e, (n / kAtInfo) & 1);
+          int x = kAtEnd;
+          if (ok) {
+            x = info[e];
+            mbar_arrive(info_empty + e);
+          }
+          return x;
+        };
+        auto takes = [](int x, int t) { return x != kAtEnd && ((x >> 2 * t) & 3); };
+        // S of step n for tile t, over the P whose product has been issued.
+        auto scores = [&](int n, int t) {
+          if (!ok) return;
+          tc_fence_after();
           const uint32_t qt = q_addr + (dual ? 0 : t * Cfg::kQTile), kt = k_addr + n % kSlots * Cfg::kTile;
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k)  // (not to nk: rolled, the issue of a product took 80 cycles, more than the product)
@@ -784,61 +796,49 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
               tc_mma_f16(tmem + t * 128, smem_desc_sw128(qt + (k >> 2) * Cfg::kQHalf + (k & 3) * 32),
                          smem_desc_sw128(kt + (k >> 2) * Cfg::kHalf + (k & 3) * 32), idesc_s, k > 0);
           tc_commit(s_full + t);
-        }
-        __syncwarp();
-      };
-      auto values = [&](int n, int t) {
-        wait(p_full + t, used[t] & 1);
-        tc_fence_after();
-        if (ok && elect_one()) {
+        };
+        auto values = [&](int n, int t) {
+          wait(p_full + t, used[t] & 1);
+          if (!ok) return;
+          tc_fence_after();
           const uint32_t pt = tmem + t * 128;
 #pragma unroll
           for (int k = 0; k < kAtKeys / 16; ++k)
             tc_mma_f16_ts(tmem + Cfg::kTmemO + t * DP, pt + 8 * k, smem_desc_values(v_addr + n % kSlots * Cfg::kTile + k * 2048, Cfg::kHalf), idesc_o,
                           used[t] > 0 || k > 0);
+          ++used[t];
+        };
+        int cur = read(0);
+        if (cur != kAtEnd) {
+          for (int t = 0; t < NT; ++t)
+            if (tokens[t]) wait(q_full + t, 0);
+          wait(k_full, 0);
+          for (int t = 0; t < NT; ++t)
+            if (takes(cur, t)) scores(0, t);
+          if (ok) tc_commit(k_empty);
         }
-        __syncwarp();
-        ++used[t];
-      };
-      auto release = [&](uint64_t* empty) {
-        if (ok && elect_one()) tc_commit(empty);
-        __syncwarp();
-      };
-      int cur = read(0);
-      if (cur != kAtEnd && ok) {
-        for (int t = 0; t < NT; ++t)
-          if (tokens[t]) wait(q_full + t, 0);
-        wait(k_full, 0);
-        for (int t = 0; t < NT; ++t)
-          if (takes(cur, t)) scores(0, t);
-        release(k_empty);
         for (int n = 0; ok && cur != kAtEnd; ++n) {
           const int next = read(n + 1), k_next = (n + 1) % kSlots;
           if (next != kAtEnd) wait(k_full + k_next, ((n + 1) / kSlots) & 1);
+          // A tile that has no part in this step need not wait for it.
+          for (int t = 0; t < NT; ++t)
+            if (!takes(cur, t) && takes(next, t)) scores(n + 1, t);
           wait(v_full + n % kSlots, (n / kSlots) & 1);
-          // Rows past the last key may hold anything: a NaN there, times a weight of zero, would be a NaN.
-          const int rows = s.keys - (cur >> 8) * kAtKeys;
-          if (ok && rows < kAtKeys) {
-            for (int h = 0; h < halves; ++h) {
-              uint4* tail = reinterpret_cast<uint4*>(smem + Cfg::kOffV + n % kSlots * Cfg::kTile + h * Cfg::kHalf + rows * 128);
-              for (int i = lane; i < (kAtKeys - rows) * 8; i += 32) tail[i] = make_uint4(0, 0, 0, 0);
+          for (int t = 0; t < NT; ++t)
+            if (takes(cur, t)) {
+              values(n, t);
+              if (takes(next, t)) scores(n + 1, t);
             }
-            fence_proxy_async_smem();
-            __syncwarp();
+          if (ok) {
+            tc_commit(v_empty + n % kSlots);
+            if (next != kAtEnd) tc_commit(k_empty + k_next);
           }
-          for (int t = 0; t < NT; ++t) {
-            if (takes(cur, t)) values(n, t);
-            if (takes(next, t)) scores(n + 1, t);
-          }
-          release(v_empty + n % kSlots);
-          if (next != kAtEnd) release(k_empty + k_next);
           cur = next;
         }
-      }
-      if (elect_one())
         for (int t = 0; t < NT; ++t) tc_commit(drain + t);
+        for (int t = 0; t < NT; ++t) mbar_drain(drain + t, 0);
+      }
       __syncwarp();
-      for (int t = 0; t < NT; ++t) mbar_drain(drain + t, 0);
     }
   }
   if (joined) {
@@ -880,17 +880,21 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     };
     if (!*abort_flag)
       for (int i = warp; i < mine; i += Cfg::kThreads / 32) {
-        // A lane per part, two where there are more than 32.
+        // A lane per part, several where there are more than 32.
+        constexpr int kEach = kQuarters ? 8 * kAtMostSplits / 32 : 1;
         const int r = row0 + i;
-        float2 ml[2] = {{-INFINITY, 0.f}, {-INFINITY, 0.f}};
+        float2 ml[kEach];
+        float top = -INFINITY, sum = 0.f, w[kEach];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < kEach; ++k) {
+          ml[k] = make_float2(-INFINITY, 0.f);
           if (lane + 32 * k < parts) ml[k] = ld_cluster_v2(cluster_addr(sums_addr + slot_of(r, lane + 32 * k) * 8, rank_of(lane + 32 * k)));
-        float top = fmaxf(ml[0].x, ml[1].x), sum = 0.f, w[2];
+          top = fmaxf(top, ml[k].x);
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < kEach; ++k) {
           // A part that saw nothing has no weight, and its O holds anything.
           w[k] = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : ex2_approx(kGeneral ? (ml[k].x - top) * kLog2e : ml[k].x - top);
           sum = fmaf(ml[k].y, w[k], sum);
@@ -900,7 +904,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         const bool any = sum > 0.f || sum != sum;
         const float inv = any ? 1.f / sum : 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < kEach; ++k)
           if (lane + 32 * k < parts) weights[(lane + 32 * k) * share + i] = w[k] * inv;
         if (lane == 0) {
           fine[i] = sum - sum == 0.f;

@@ -63,12 +63,22 @@ CUtensorMap heads_map(bool bf16, const void* p, int dim, int heads, int tokens, 
   return map;
 }
 
+// Clusters of more than 8 CTAs, once per device.
+template <typename K>
+void allow_wide_clusters(K kern, int dev, std::atomic<uint64_t>& done) {
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  CK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
 template <typename T, int DP, int NT, int kMode, bool kQuarters>
 void launch_attend_kernel(const AttendArgs& a, const AttendMaps& maps, int64_t ctas, int dev, cudaStream_t st) {
-  static std::atomic<uint64_t> done{0};
+  static std::atomic<uint64_t> done{0}, wide{0};
   using Cfg = AttendCfg<DP, NT>;
   auto kern = attend_kernel<T, DP, NT, kMode, kQuarters>;
   allow_smem(kern, Cfg::kBytes, dev, done);
+  if (a.splits > 8) allow_wide_clusters(kern, dev, wide);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(Cfg::kThreads);
@@ -100,7 +110,7 @@ void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   const int64_t items = (int64_t)a.pairs * a.sequences * a.kv_heads;
   const int blocks = (max_keys + kAtKeys - 1) / kAtKeys, sms = sm_count(dev);
   a.splits = 1;
-  while (a.splits < kAtMostSplits && items * a.splits * 2 <= sms && a.splits * 4 <= blocks) a.splits *= 2;
+  while (a.splits < kAtMostSplits && items * a.splits * 2 <= sms && a.splits * 4 <= blocks && (a.splits < 8 || items <= 4)) a.splits *= 2;
   const int64_t ctas = items * a.splits;
   if (ctas > INT32_MAX) fail(LAYA_ERR_INVALID, "%d queries of %d sequences and %d heads are too many for one call", a.max_queries, a.sequences, a.heads);
   // The heads of a group on different banks for the rows of a warp.
@@ -138,7 +148,9 @@ int laya_op_rotary(const laya_rotary* p, void* stream) {
   if (p->scaling == LAYA_ROTARY_NTK && p->dims <= 2) fail(LAYA_ERR_INVALID, "ntk scaling needs dims above 2");
   if (p->scaling == LAYA_ROTARY_PARTS && (!(p->length > 0) || !(p->low < p->high)))
     fail(LAYA_ERR_INVALID, "scaling by parts needs a length and low < high");
-  RotaryArgs a{};
+  RotaryArgs a = {};
+  const int size = (int)dtype_size(p->dtype), wide = 16 / size;
+  bool vectors = true, any = false;
   for (int i = 0; i < 2; ++i) {
     const laya_heads& h = p->part[i];
     if (h.heads < 0) fail(LAYA_ERR_INVALID, "bad shape: %d heads", h.heads);
@@ -150,35 +162,54 @@ int laya_op_rotary(const laya_rotary* p, void* stream) {
     if (in_place && (h.x_token != h.out_token || h.x_head != h.out_head))
       fail(LAYA_ERR_INVALID, "out is x, but with other strides");
     a.part[i] = {h.x, h.out, h.x_token, h.x_head, h.out_token, h.out_head, h.heads, !in_place};
+    vectors = vectors && ((reinterpret_cast<uintptr_t>(h.x) | reinterpret_cast<uintptr_t>(h.out)) & 15) == 0 &&
+              (h.x_token | h.x_head | h.out_token | h.out_head) % wide == 0;
+    any = true;
   }
-  if (!p->tokens || (!a.part[0].heads && !a.part[1].heads)) return LAYA_OK;
+  if (!any) return LAYA_OK;
   if (!p->positions) fail(LAYA_ERR_INVALID, "positions is null");
   if (reinterpret_cast<uintptr_t>(p->positions) % (p->positions_64 ? 8 : 4)) fail(LAYA_ERR_INVALID, "positions is not aligned to its elements");
   a.positions = p->positions;
   a.positions_64 = p->positions_64;
   a.tokens = p->tokens;
-  a.dim = p->head_dim;
   a.pairs = p->dims / 2;
+  // Vectors of 16 bytes where all of a head's parts are whole ones.
+  vectors = vectors && (p->interleaved ? p->dims : a.pairs) % wide == 0 && (p->head_dim - p->dims) % wide == 0;
+  const int v = vectors ? wide : 1;
+  a.places = p->interleaved && vectors ? p->dims / v : a.pairs / v;
+  a.rest = (p->head_dim - p->dims) / v;
+  if (((int64_t)a.part[0].heads + a.part[1].heads) * std::max(1, a.rest) > INT32_MAX / 2)
+    fail(LAYA_ERR_INVALID, "%d and %d heads of %d are too many for one call", a.part[0].heads, a.part[1].heads, p->head_dim);
+  a.abreast = std::max(1, 32 / a.places);
+  a.by_places = FastDiv(a.places);
+  a.by_rest = FastDiv(std::max(1, a.rest));
   a.sine_sign = p->backward ? -1.f : 1.f;
   a.magnitude = p->magnitude;
   constexpr double kTurn = 6.283185307179586;
-  double theta = p->theta;
-  if (p->scaling == LAYA_ROTARY_NTK) theta *= std::pow(p->factor, p->dims / (p->dims - 2.0));
-  for (int k = 0; k < a.pairs; ++k) {
-    double f = std::pow(theta, -2.0 * k / p->dims);
-    if (p->scaling == LAYA_ROTARY_LINEAR) f /= p->factor;
-    if (p->scaling == LAYA_ROTARY_PARTS) {
-      const double keep = std::min(1.0, std::max(0.0, (p->length * f / kTurn - p->low) / (p->high - p->low)));
-      f *= keep + (1 - keep) / p->factor;
-    }
-    a.turns[k] = f / kTurn;
+  const double theta = p->theta * (p->scaling == LAYA_ROTARY_NTK ? std::pow(p->factor, p->dims / (p->dims - 2.0)) : 1.0);
+  a.step = -2.0 / p->dims * std::log2(theta);
+  a.power = -std::log2(p->scaling == LAYA_ROTARY_LINEAR ? kTurn * p->factor : kTurn);
+  a.by_parts = p->scaling == LAYA_ROTARY_PARTS;
+  if (a.by_parts) {
+    a.above = p->length / (p->high - p->low);
+    a.below = p->low / (p->high - p->low);
+    a.shrink = 1.0 / p->factor;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sms = sm_count(current_device(st));
+  // A warp per token, more while the warps do not fill the SMs and a token has heads for them.
+  const int rounds = (int)(((int64_t)a.part[0].heads + a.part[1].heads + a.abreast - 1) / a.abreast);
+  a.shares = 1;
+  while (a.shares < rounds && (int64_t)a.tokens * a.shares * 2 <= 16ll * sms) a.shares *= 2;
+  a.by_shares = FastDiv(a.shares);
+  const int64_t warps = (int64_t)a.tokens * a.shares;  // at most 2^31 - 1: several to a token only where tokens are few
+  const dim3 grid((unsigned)((warps + kRotaryThreads / 32 - 1) / (kRotaryThreads / 32)));
   with_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    auto kern = p->interleaved ? rotary_kernel<T, true> : rotary_kernel<T, false>;
-    launch_k(kern, dim3(std::min(p->tokens, 64 * sms)), dim3(kRotaryThreads), 0, st, a);
+    constexpr int V = 16 / sizeof(T);
+    auto kern = vectors ? (p->interleaved ? rotary_kernel<T, V, true> : rotary_kernel<T, V, false>)
+                        : (p->interleaved ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
+    launch_k(kern, grid, dim3(kRotaryThreads), 0, st, a);
   });
   OP_API_END
 }
