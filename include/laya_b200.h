@@ -421,8 +421,9 @@ typedef struct laya_attend {
   int32_t sequences, heads, kv_heads;  /* heads a multiple of kv_heads, of at most 128 times: head h reads kv head h / (heads / kv_heads) */
   int32_t head_dim;              /* a multiple of 8, 8 .. 128 */
   int32_t dtype;                 /* LAYA_DTYPE_F16 or _BF16 */
-  int32_t q_tokens, k_tokens;    /* rows of q and out, and of k and v */
-  int32_t max_queries, max_keys; /* bounds on the lengths; queries past max_queries of a sequence are not computed */
+  int32_t q_tokens, k_tokens;    /* rows of q and out, and of k and v: at most 2^31 - 256 */
+  int32_t max_queries, max_keys; /* bounds on the lengths: queries past max_queries of a sequence are not computed, max_keys (which may
+                                    be too small) decides how far the keys are split, and so the last bits */
   const void* q; int64_t q_token, q_head;    /* [q_tokens][heads][head_dim]; q, k, v: 16-byte aligned, */
   const void* k; int64_t k_token, k_head;    /* [k_tokens][kv_heads][head_dim]; strides multiples of 8 */
   const void* v; int64_t v_token, v_head;
@@ -446,8 +447,8 @@ typedef struct laya_attend {
  *   out = sum softmax(s)_j v_j over the visible keys j, zeros where there are none (or all have s = -infinity)
  * Key j is visible where j < prefix, or where documents[query] == k_documents[key], causal implies j <= p, and
  * p - window_left <= j <= p + window_right.  Keys that are not visible may hold anything, rows outside the sequences
- * too; rows of out that belong to no sequence are left as they were.  Scores and sums are held in 32 bits, softmax's
- * numerators are rounded to dtype before they meet v.  The result is the same each time.
+ * too; rows of out that belong to no sequence are left as they were.  out must not overlap q, k or v.  Scores and sums are held in 32 bits, softmax's
+ * numerators are rounded to dtype before they meet v.  The same call gives the same result each time.
  * err (zero on entry, or NULL) receives a device error: 4 for a sequence outside the tensors' rows, which is
  * skipped, or a pipeline wait that ran out, after which out is undefined. */
 int laya_op_attend(const laya_attend* args, int* err, void* stream);

@@ -133,6 +133,7 @@ enum AtClass : int { kAtEnd = -1, kAtSkip = 0, kAtMasked = 1, kAtFull = 2 };
 enum AtMode { kAtPlain, kAtCap, kAtSlopes, kAtGeneral };
 
 constexpr int kAtMostSplits = 16;
+constexpr int kAtMostSummary = 256;  // steps whose documents are looked over ahead
 constexpr int kAtMostTable = 4096;  // values of the distance bias that are kept in shared memory, clamped past the reach
 
 // NT tiles per CTA, heads padded to DP values; kQuarters: all rows in a quarter of a tile.
@@ -152,13 +153,14 @@ struct AttendCfg {
   static constexpr int kOffQ = 0, kOffK = NT * kQTile, kOffV = kOffK + kSlots * kTile;
   static constexpr int kOffDocs = kOffV + kSlots * kTile;
   static constexpr int kOffBar = kOffDocs + kAtInfo * kAtKeys * 4;
-  static constexpr int kBars = 2 + 4 * kSlots + 2 * kAtInfo + 7;
+  static constexpr int kBars = 2 + 4 * kSlots + 2 * kAtInfo + 8;
   static constexpr int kOffInfo = kOffBar + kBars * 8;
   static constexpr int kOffSums = kOffInfo + kAtInfo * 4 + 16;  // (maximum, sum) of each row, where results are joined
   static constexpr int kWeights = 2 * NT * kAtRows + 8 * kAtMostSplits;  // of the parts of the rows that a CTA joins
   static constexpr int kOffWeights = kOffSums + NT * kAtRows * 8;
   static constexpr int kOffTable = kOffWeights + kWeights * 4;
-  static constexpr int kBytes = kOffTable + kAtMostTable * 4 + 1024;
+  static constexpr int kOffSummary = kOffTable + kAtMostTable * 4;
+  static constexpr int kBytes = kOffSummary + kAtMostSummary * 8 + 1024;
   static_assert(kOffSums % 8 == 0, "alignment");
   static_assert(2 * kAtMostSplits <= 32, "a lane per part");
   static_assert(NT * kAtRows * DP * 4 <= 2 * kSlots * kTile, "a part's O fits the K and V tiles");
@@ -215,23 +217,24 @@ __device__ __forceinline__ AttendSpan attend_span(const AttendArgs& a, int p, in
 }
 
 // out tanh(in s) for a raw product s, with out in some unit.
-//   near  for |in s| <= 0.75: s times a polynomial in s^2 by the Remez exchange algorithm, on the FMA pipe; off by 2.5e-7 out
+//   near  for |in s| <= 0.8: s times a polynomial in s^2 by the Remez exchange algorithm, on the FMA pipe; off by 1.2e-7 of itself (a term
+//         less made the logarithms of the sums ten times less exact than the exponentials do)
 //   any   out - 2 out / (exp(2 in s) + 1) on the special-function unit; off by 2^-21 out
 struct CapTerms {
-  float in, out, c[5], most;  // most: the largest |s| for `near`
+  float in, out, c[6], most;  // most: the largest |s| for `near`
   __device__ __forceinline__ CapTerms(float in_, float out_) : in(in_), out(out_) {
-    constexpr float kC[5] = {0.999997258f, -0.333231002f, 0.132262245f, -0.0492833108f, 0.0123209562f};
+    constexpr float kC[6] = {0.99999994f, -0.333326757f, 0.13321048f, -0.0531143174f, 0.0190933011f, -0.00435529975f};
     float power = out * in;
 #pragma unroll
-    for (int i = 0; i < 5; ++i) { c[i] = kC[i] * power; power *= in * in; }
-    // Powers of `in` up to the ninth, and of s, stay in range.
-    most = fabsf(in) > 1e-3f && fabsf(in) < 1e3f ? 0.75f / fabsf(in) : -1.f;
+    for (int i = 0; i < 6; ++i) { c[i] = kC[i] * power; power *= in * in; }
+    // Where the eleventh power of `in` stays in range (0.09 / cap up to caps of 300).
+    most = fabsf(c[5]) > 1e-36f && fabsf(c[5]) < 1e30f ? 0.8f / fabsf(in) : -1.f;
   }
   __device__ __forceinline__ float2 slope(float2 s) const {  // out tanh(in s) / s
     const float2 z = mul2(s, s);
-    float2 p = fma2(make_float2(c[4], c[4]), z, make_float2(c[3], c[3]));
+    float2 p = fma2(make_float2(c[5], c[5]), z, make_float2(c[4], c[4]));
 #pragma unroll
-    for (int i = 2; i >= 0; --i) p = fma2(p, z, make_float2(c[i], c[i]));
+    for (int i = 3; i >= 0; --i) p = fma2(p, z, make_float2(c[i], c[i]));
     return p;
   }
   __device__ __forceinline__ float any(float s) const {
@@ -254,7 +257,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
   uint64_t *q_full = bar, *k_full = bar + 2, *k_empty = k_full + kSlots, *v_full = k_empty + kSlots, *v_empty = v_full + kSlots,
-           *info_full = v_empty + kSlots, *info_empty = info_full + kAtInfo, *s_full = info_empty + kAtInfo, *p_full = s_full + 2, *drain = p_full + 2, *table_full = drain + 2;
+           *info_full = v_empty + kSlots, *info_empty = info_full + kAtInfo, *s_full = info_empty + kAtInfo, *p_full = s_full + 2, *drain = p_full + 2, *table_full = drain + 2, *summary_full = table_full + 1;
   volatile int* info = reinterpret_cast<volatile int*>(smem + Cfg::kOffInfo);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffInfo + kAtInfo * 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -272,6 +275,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     }
     for (int i = 0; i < kSlots; ++i) { mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1); }
     mbar_init(table_full, Cfg::kSoftmax);
+    mbar_init(summary_full, Cfg::kSoftmax);
     for (int i = 0; i < kAtInfo; ++i) { mbar_init(info_full + i, 1); mbar_init(info_empty + i, Cfg::kSoftmax + 1); }
     *abort_flag = 0;
     fence_mbar_init();
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     inner[t] = {y.lo, x.hi};
     if (outer[t].lo <= outer[t].hi) { from = min(from, outer[t].lo); to = max(to, outer[t].hi); }
   }
-  const int prefix = min(s.prefix, s.keys);
+  const int prefix = max(0, min(s.prefix, s.keys));
   if (prefix > 0) { from = 0; to = max(to, prefix - 1); }
   int at = from <= to ? from / kAtKeys : 0, end = from <= to ? to / kAtKeys + 1 : 0;
   if (a.splits > 1) {
@@ -323,6 +327,10 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     at += split * share;
     end = min(end, at + share);
   }
+  // Lowest and highest document of each of the CTA's steps, found by the softmax warps before there are scores: with documents most steps may
+  // show nothing, and one at a time each takes a trip to memory.
+  const bool summed = a.documents && end - at <= kAtMostSummary;
+  int2* summary = reinterpret_cast<int2*>(smem + Cfg::kOffSummary);
   const bool dual = few && end - at > 1;            // both tiles take the rows of the first, each every other step
   const bool joined = !idle && (a.splits > 1 || dual || kQuarters);  // the rows' results are in parts
   float* part = reinterpret_cast<float*>(smem + Cfg::kOffK);  // unnormalised rows of O, once all products are done
@@ -356,15 +364,40 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     const float* near = reinterpret_cast<const float*>(smem + Cfg::kOffTable) + (head - kv * a.group) * wide + a.reach + kAtKeys + kAtRows;
     if (table_here) {
       float* to = reinterpret_cast<float*>(smem + Cfg::kOffTable);
-      for (int i = threadIdx.x; i < a.group * wide; i += 32 * Cfg::kSoftmax) {
-        const int g = i / wide, at_d = i - g * wide - (a.reach + kAtKeys + kAtRows);
-        to[i] = __ldg(a.table + (int64_t)(kv * a.group + g) * (2 * a.reach + 1) + a.reach + min(max(at_d, -a.reach), a.reach));
+      for (int g = 0; g < a.group; ++g) {
+        const float* of = a.table + (int64_t)(kv * a.group + g) * (2 * a.reach + 1) + a.reach;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < wide; i += 32 * Cfg::kSoftmax)
+          to[g * wide + i] = __ldg(of + min(max(i - (a.reach + kAtKeys + kAtRows), -a.reach), a.reach));
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(table_full);
     }
     const bool capped = kMode == kAtCap || (kGeneral && a.cap > 0.f);
     const CapTerms cap(capped ? a.scale / a.cap : 0.f, a.cap * kUnit);
+    if (summed) {
+      for (int i0 = warp; i0 < end - at; i0 += 4 * Cfg::kSoftmax) {
+        int d[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int i = i0 + u * Cfg::kSoftmax, j = (at + i) * kAtKeys + 32 * c + lane;
+            // Past the last key the step's first document, which is in the step.
+            if (i < end - at) d[u][c] = a.k_documents[s.k_start + (j < s.keys ? j : (at + i) * kAtKeys)];
+          }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = i0 + u * Cfg::kSoftmax;
+          if (i >= end - at) break;
+          const int lo = __reduce_min_sync(0xffffffffu, min(min(d[u][0], d[u][1]), min(d[u][2], d[u][3])));
+          const int hi = __reduce_max_sync(0xffffffffu, max(max(d[u][0], d[u][1]), max(d[u][2], d[u][3])));
+          if (lane == 0) summary[i] = make_int2(lo, hi);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(summary_full);
+    }
     bool ok = !table_here || mbar_wait(table_full, 0, a.err, kErrAttnWait, abort_flag, wait_ns);
     int count = 0;  // steps of this tile
     for (int n = 0;; ++n) {
@@ -373,7 +406,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       const int x = info[e];
       if (x == kAtEnd) break;
-      const int cls = (x >> 2 * t) & 3, kb = (x >> 8) * kAtKeys;
+      const int cls = (x >> 2 * t) & 3, kb = (int)((uint32_t)x >> 8) * kAtKeys;
       if (cls == kAtSkip) {
         __syncwarp();
         if (lane == 0) mbar_arrive(info_empty + e);
@@ -549,16 +582,27 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
 #pragma unroll
             for (int i = 0; i < 32; i += 2) big = max3(big, fabsf(__uint_as_float(sx[c][i])), fabsf(__uint_as_float(sx[c][i + 1])));
           if (__all_sync(0xffffffffu, big <= cap.most)) each([&](float2 y, int) { return mul2(y, cap.slope(y)); });
-          else each([&](float2 y, int) { return make_float2(cap.any(y.x), cap.any(y.y)); });
+          else each([&](float2 y, int) {
+            const float2 n = mul2(y, cap.slope(y));
+            return make_float2(fabsf(y.x) <= cap.most ? n.x : cap.any(y.x), fabsf(y.y) <= cap.most ? n.y : cap.any(y.y));
+          });
         }
         const float2 by = capped ? make_float2(1.f, 1.f) : make_float2(scale, scale);
         if ((kMode == kAtSlopes || kGeneral) && a.slopes) {
           const float fd = (float)d;
           each([&](float2 y, int i) { return fma2(y, by, make_float2(-slope * fabsf(fd + (float)i), -slope * fabsf(fd + (float)(i + 1)))); });
         } else if (kGeneral && table) {
-          each([&](float2 y, int i) {
-            return fma2(y, by, make_float2(__ldg(table + min(max(d + i, -a.reach), a.reach)), __ldg(table + min(max(d + i + 1, -a.reach), a.reach))));
-          });
+          const bool left = d + kMine - 1 <= -a.reach;
+          if (__all_sync(0xffffffffu, left || d >= a.reach)) {
+            const float edge = __ldg(table + (left ? -a.reach : a.reach));
+            each([&](float2 y, int) { return fma2(y, by, make_float2(edge, edge)); });
+          } else if (table_here) {
+            each([&](float2 y, int i) { return fma2(y, by, make_float2(near[d + i], near[d + i + 1])); });
+          } else {
+            each([&](float2 y, int i) {
+              return fma2(y, by, make_float2(__ldg(table + min(max(d + i, -a.reach), a.reach)), __ldg(table + min(max(d + i + 1, -a.reach), a.reach))));
+            });
+          }
         } else if (kMode == kAtPlain || (kGeneral && !capped)) {
           each([&](float2 y, int) { return mul2(y, by); });
         }
@@ -691,7 +735,8 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           doc_hi[t] = __reduce_max_sync(0xffffffffu, doc_hi[t]);
         }
       int n = 0, k_issued = 0, v_issued = 0;
-      bool ok = true;
+      bool ok = !summed || mbar_wait(summary_full, 0, a.err, kErrAttnWait, abort_flag, wait_ns);
+      ok = __all_sync(0xffffffffu, ok);
       auto load = [&](const CUtensorMap* map, uint64_t* full, uint64_t* empty, int off, int kb, int& issued) {
         const int slot = n % kSlots;
         ok = ok && mbar_wait(empty + slot, ((n / kSlots) & 1) ^ 1, a.err, kErrAttnWait, abort_flag, wait_ns);
@@ -704,39 +749,63 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         __syncwarp();
         ++issued;
       };
-      // With slopes the nearest keys first, whose scores the later ones then seldom exceed.
-      for (int i = at; i < end && ok; ++i) {
-        const int step = a.slopes ? at + end - 1 - i : i;
+      // What a step with documents lo .. hi is to each tile: kAtClass of tile 0, and of tile 1 two bits up.
+      auto classify = [&](int step, int lo, int hi) {
         const int kb = step * kAtKeys, last = min(kb + kAtKeys, s.keys) - 1;
-        int d[4] = {0, 0, 0, 0}, lo = INT_MAX, hi = INT_MIN;
-        if (a.documents) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = kb + lane + 32 * i;
-            if (j <= last) {
-              d[i] = a.k_documents[s.k_start + j];
-              lo = min(lo, d[i]);
-              hi = max(hi, d[i]);
-            }
-          }
-          lo = __reduce_min_sync(0xffffffffu, lo);
-          hi = __reduce_max_sync(0xffffffffu, hi);
-        }
-        int mixed = 0;
-        if (a.documents)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!__all_sync(0xffffffffu, d[i] == __shfl_sync(0xffffffffu, d[i], 0))) mixed |= 1 << i;
-        int cls[2] = {kAtSkip, kAtSkip};
+        int both = 0;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const bool in_prefix = kb < prefix, whole_prefix = kb + kAtKeys <= prefix;
           const bool meets = kb <= outer[t].hi && last >= outer[t].lo && (!a.documents || (lo <= doc_hi[t] && hi >= doc_lo[t]));
           const bool whole = kb >= inner[t].lo && kb + kAtKeys - 1 <= inner[t].hi &&
                              (!a.documents || (lo == hi && doc_lo[t] == doc_hi[t] && lo == doc_lo[t]));
-          cls[t] = !tokens[t] ? kAtSkip : whole_prefix || whole ? kAtFull : in_prefix || meets ? kAtMasked : kAtSkip;
+          both |= (!tokens[t] ? kAtSkip : whole_prefix || whole ? kAtFull : in_prefix || meets ? kAtMasked : kAtSkip) << 2 * t;
         }
-        if (cls[0] == kAtSkip && cls[1] == kAtSkip) continue;
+        return both;
+      };
+      // With slopes the nearest keys first, whose scores the later ones then seldom exceed.
+      auto step_of = [&](int i) { return a.slopes ? at + end - 1 - i : i; };
+      // 32 steps at a time, each by a lane, then those that show something.  (Documents that are not known yet: all may be.)
+      uint32_t shown = 0;
+      int lane_lo = 0, lane_hi = 0, lane_class = 0;
+      for (int i = at; i < end && ok; ++i) {
+        const int in_group = (i - at) & 31;
+        if (in_group == 0) {
+          lane_lo = INT_MIN;
+          lane_hi = INT_MAX;
+          lane_class = 0;
+          if (i + lane < end) {
+            const int mine = step_of(i + lane);
+            if (summed) { lane_lo = summary[mine - at].x; lane_hi = summary[mine - at].y; }
+            lane_class = classify(mine, lane_lo, lane_hi);
+          }
+          shown = __ballot_sync(0xffffffffu, lane_class != 0);
+        }
+        const uint32_t left = shown >> in_group;
+        if (!left) { i += 31 - in_group; continue; }  // on to the next 32
+        const int next = __ffs(left) - 1 + in_group;
+        i += next - in_group;
+        const int step = step_of(i);
+        int both = __shfl_sync(0xffffffffu, lane_class, next), lo = __shfl_sync(0xffffffffu, lane_lo, next), hi = __shfl_sync(0xffffffffu, lane_hi, next);
+        const int kb = step * kAtKeys, last = min(kb + kAtKeys, s.keys) - 1;
+        int d[4] = {lo, lo, lo, lo}, mixed = 0;
+        if (a.documents && lo != hi) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int j = kb + lane + 32 * c;
+            d[c] = a.k_documents[s.k_start + (j <= last ? j : kb)];
+          }
+          if (!summed) {
+            lo = __reduce_min_sync(0xffffffffu, min(min(d[0], d[1]), min(d[2], d[3])));
+            hi = __reduce_max_sync(0xffffffffu, max(max(d[0], d[1]), max(d[2], d[3])));
+            both = classify(step, lo, hi);
+            if (!both) continue;
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (!__all_sync(0xffffffffu, d[c] == __shfl_sync(0xffffffffu, d[c], 0))) mixed |= 1 << c;
+        }
+        int cls[2] = {both & 3, both >> 2};
         if (dual && (n & 1)) { cls[1] = cls[0]; cls[0] = kAtSkip; }
         const int e = n % kAtInfo;
         ok = mbar_wait(info_empty + e, ((n / kAtInfo) & 1) ^ 1, a.err, kErrAttnWait, abort_flag, wait_ns);
@@ -745,7 +814,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
 #pragma unroll
           for (int i = 0; i < 4; ++i) docs[e * kAtKeys + lane + 32 * i] = d[i];
         }
-        if (lane == 0) info[e] = step << 8 | mixed << 4 | cls[1] << 2 | cls[0];
+        if (lane == 0) info[e] = (int)((uint32_t)step << 8 | mixed << 4 | cls[1] << 2 | cls[0]);
         __syncwarp();
         if (lane == 0) mbar_arrive(info_full + e);
         load(&maps.k, k_full, k_empty, Cfg::kOffK, kb, k_issued);

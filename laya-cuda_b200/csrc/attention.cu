@@ -9,12 +9,6 @@
 
 using namespace laya;
 
-#ifndef AT_NT64
-#define AT_NT64 1
-#endif
-#ifndef AT_NT128
-#define AT_NT128 2
-#endif
 namespace {
 
 // A tensor [tokens][heads][dim], strides in elements.
@@ -108,6 +102,8 @@ void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   a.per_tile = (kQuarters ? kAtRows / 4 : kAtRows) / a.group;
   a.pairs = (a.max_queries + NT * a.per_tile - 1) / (NT * a.per_tile);
   const int64_t items = (int64_t)a.pairs * a.sequences * a.kv_heads;
+  // Keys are split over the CTAs of a cluster while that finds idle SMs and leaves each four steps.  Clusters of 16 only for a few kv heads: four of them
+  // fit the GPU at once (1 x 131072 keys with 1 kv head 94 us, 177 with 8 CTAs; with 8 kv heads 208 us, 175 with 8).
   const int blocks = (max_keys + kAtKeys - 1) / kAtKeys, sms = sm_count(dev);
   a.splits = 1;
   while (a.splits < kAtMostSplits && items * a.splits * 2 <= sms && a.splits * 4 <= blocks && (a.splits < 8 || items <= 4)) a.splits *= 2;
@@ -220,6 +216,9 @@ int laya_op_attend(const laya_attend* p, int* err, void* stream) {
   if (p->sequences < 0 || p->sequences > 65535 || p->q_tokens < 0 || p->k_tokens < 0 || p->max_queries < 0 || p->max_keys < 0)
     fail(LAYA_ERR_INVALID, "bad shape: %d sequences (65535 at most), %d and %d tokens, at most %d and %d of a sequence", p->sequences,
          p->q_tokens, p->k_tokens, p->max_queries, p->max_keys);
+  // Positions and steps of keys past the last one are counted in 32 bits.
+  constexpr int kMost = INT32_MAX - 255;
+  if (p->q_tokens > kMost || p->k_tokens > kMost) fail(LAYA_ERR_INVALID, "%d and %d tokens: at most %d", p->q_tokens, p->k_tokens, kMost);
   if (p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->heads / p->kv_heads > 128 || p->heads > 65535)
     fail(LAYA_ERR_INVALID, "%d heads over %d kv heads: a multiple of at most 128 times", p->heads, p->kv_heads);
   if (p->head_dim < 8 || p->head_dim > kAttendMostDim || p->head_dim % 8)
@@ -262,9 +261,9 @@ int laya_op_attend(const laya_attend* p, int* err, void* stream) {
     // All rows of a sequence's kv head in a quarter of a tile: single tokens, and a few where the group is small.
     const bool quarters = (int64_t)a.max_queries * a.group <= kAtRows / 4;
     if (a.dim > 64 && quarters) launch_attend<T, 128, 2, true>(a, max_keys, dev, st);
-    else if (a.dim > 64) launch_attend<T, 128, AT_NT128, false>(a, max_keys, dev, st);
+    else if (a.dim > 64) launch_attend<T, 128, 2, false>(a, max_keys, dev, st);
     else if (quarters) launch_attend<T, 64, 2, true>(a, max_keys, dev, st);
-    else launch_attend<T, 64, AT_NT64, false>(a, max_keys, dev, st);
+    else launch_attend<T, 64, 1, false>(a, max_keys, dev, st);
   });
   OP_API_END
 }

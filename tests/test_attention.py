@@ -51,7 +51,7 @@ def attend(**other):
 
 @pytest.mark.parametrize("other,word", [
     (dict(sequences=-1), "shape"), (dict(sequences=65536), "shape"), (dict(q_tokens=-1), "shape"), (dict(k_tokens=-1), "shape"),
-    (dict(max_queries=-1), "shape"), (dict(max_keys=-1), "shape"), (dict(heads=0), "heads"), (dict(kv_heads=0), "heads"),
+    (dict(q_tokens=2 ** 31 - 255), "tokens"), (dict(k_tokens=2 ** 31 - 1), "tokens"), (dict(max_queries=-1), "shape"), (dict(max_keys=-1), "shape"), (dict(heads=0), "heads"), (dict(kv_heads=0), "heads"),
     (dict(kv_heads=3), "heads"), (dict(heads=258), "128"), (dict(head_dim=0), "head"), (dict(head_dim=60), "multiple of 8"),
     (dict(head_dim=136), "128"), (dict(dtype=0), "dtype"), (dict(dtype=3), "dtype"), (dict(scale=float("inf")), "scale"),
     (dict(cap=-1.0), "cap"), (dict(cap=float("nan")), "cap"), (dict(window_left=-2), "window"), (dict(window_right=-5), "window"),

@@ -593,3 +593,82 @@ def test_pieces_join_by_their_logarithms():
     joined = sum(wi * p[0].double() for wi, p in zip(w, parts))
     # Each part within its own bound, which the weights mix; the weights are off by the logarithms' errors.
     assert ((joined - want).abs() <= 3 * slack + 2.0 ** -10 * want.abs() + 2.0 ** -11).all()
+
+
+# -------------------------------------------------------------------------------- attention: what decides between its ways
+
+@pytest.mark.parametrize("heads,kv_heads,queries", [(32, 1, [1, 1]), (16, 1, [2, 1]), (33, 1, [1, 1]), (8, 8, [32, 7]), (8, 8, [33, 1]), (5, 1, [6, 2]), (128, 1, [1, 2]),
+                                                    (100, 1, [2, 1])])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("how", [dict(), dict(cap=30.0), dict(slopes=True), dict(distance_bias=100)])
+def test_rows_about_a_quarter_and_a_whole_tile(heads, kv_heads, queries, dim, how):
+    check(problem(30, queries, [700, 133], heads=heads, kv_heads=kv_heads, dim=dim, causal=True, prefix=[3, 0], **with_bias(how, heads)))
+
+
+@pytest.mark.parametrize("queries", [[1, 1], [5, 2], [200, 20]])
+@pytest.mark.parametrize("window", [None, (300, 10), (0, 0)])
+def test_masks_of_few_rows(queries, window):
+    keys = [1500, 260]
+    k_documents = documents(keys, 100, 4)
+    doc = torch.cat([k_documents[a + m - n: a + m] for a, m, n in zip([0, 1500], keys, queries)])
+    check(problem(31, queries, keys, heads=8, kv_heads=2, dim=64, window=window, documents=doc, k_documents=k_documents, prefix=[130, 0]))
+
+
+@pytest.mark.parametrize("queries", [[1], [40]])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_documents_of_many_steps(queries, mixed):
+    """More steps of keys than are looked over ahead, with documents that come back far apart."""
+    keys = [50000]
+    k_documents = documents(keys, 4000, 5)
+    if mixed:
+        k_documents = k_documents % 3
+    check(problem(32, queries, keys, heads=2, kv_heads=1, dim=64, documents=k_documents[-queries[0]:].clone(), k_documents=k_documents))
+
+
+@pytest.mark.parametrize("reach,heads,kv_heads", [(3000, 2, 2), (1000, 8, 1), (128, 64, 2), (1, 6, 2)])
+@pytest.mark.parametrize("queries,keys", [([300], None), ([1, 60], [3000, 200])])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_distance_biases_of_all_sizes(reach, heads, kv_heads, queries, keys, cap):
+    how = with_bias(dict(distance_bias=reach), heads, reach)
+    check(problem(33, queries, keys, heads=heads, kv_heads=kv_heads, dim=64, cap=cap, **how))
+
+
+@pytest.mark.parametrize("scale,cap", [(0.125, 0.01), (0.125, 1e-4), (0.125, 500.0), (0.125, 1e5), (3.0, 4.0), (1.0, 1e-3), (-0.3, 5.0), (1e-3, 50.0)])
+@pytest.mark.parametrize("queries,keys", [([300], None), ([1, 3], [900, 200])])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_caps_far_below_and_far_above_the_scores(scale, cap, queries, keys, dtype):
+    check(problem(34, queries, keys, heads=4, kv_heads=2, dim=64, dtype=dtype, scale=scale, cap=cap, causal=True))
+
+
+@pytest.mark.parametrize("slope", [0.0, 1e-6, 3.0, -0.25])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("queries,keys", [([500], None), ([1, 40], [3000, 700])])
+def test_slopes_of_all_sizes(slope, causal, queries, keys):
+    """Also ones that favour far keys, whose maximum the steps raise again and again."""
+    check(problem(35, queries, keys, heads=2, kv_heads=2, dim=64, causal=causal, slopes=torch.full((2,), slope, device="cuda")))
+
+
+def test_the_largest_documented_values():
+    """Documents and prefixes at the ends of 32 bits, windows as wide as numbers go."""
+    lengths = [300, 40]
+    doc = torch.randint(0, 2, (340,), generator=generator(6), device="cuda").mul(2 ** 32 - 1).sub(2 ** 31).to(torch.int32)
+    check(problem(36, lengths, heads=2, kv_heads=1, dim=64, documents=doc, window=(2 ** 31 - 1, 2 ** 31 - 1), prefix=[2 ** 31 - 1, -2 ** 31]))
+    check(problem(36, lengths, heads=2, kv_heads=1, dim=64, causal=True, window=(2 ** 31 - 1, 0), prefix=[-5, 0]))
+
+
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable():
+    """A valid call whose waits are limited to a nanosecond: it gives up, says so, and the next call is right."""
+    from laya_cuda import _lib
+    lib = _lib.load()
+    for queries, keys in (([1000], None), ([1], [9000]), ([20], [9000])):
+        s = problem(37, queries, keys, heads=4, kv_heads=1, dim=128, causal=True)
+        out, err = torch.zeros(s["q"].shape, dtype=s["q"].dtype, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+        k = {} if keys is None else {"k_starts": ints(s["k_starts"]), "k_lengths": ints(s["k_lengths"])}
+        _lib.check(lib.laya_set_launch_options(1, 1))
+        try:
+            attention.attend(s["q"], s["k"], s["v"], out, ints(s["starts"]), ints(s["lengths"]), err=err, causal=True, **k)
+            torch.cuda.synchronize()
+        finally:
+            _lib.check(lib.laya_set_launch_options(1, 0))
+        assert err.item() == 5
+        check(s)
