@@ -27,7 +27,7 @@ struct AttendArgs {
   int* err;
   unsigned long long wait_ns;
   int per_tile;       // queries of a tile, which holds all heads of a group for each
-  int table_here, table_pad;  // the distance bias fits shared memory; values between its heads there
+  int table_pad;      // values between the heads of a distance bias in shared memory
   int pairs, splits;  // CTAs for max_queries of a kv head; CTAs (a cluster) that share a tile's keys
   FastDiv by_group, by_splits, by_kv, by_sequences;
 };
@@ -128,9 +128,9 @@ constexpr int kAtKeys = 128;       // keys of a step
 constexpr int kAtInfo = 4;         // steps announced ahead
 constexpr float kAtRescale = 8.f;  // O is rescaled when a row's maximum has grown by more than 2^8
 enum AtClass : int { kAtEnd = -1, kAtSkip = 0, kAtMasked = 1, kAtFull = 2 };
-// What is done to the scores: nothing, a cap, slopes (of these three in log2 units, a scale above zero), or all else, in natural units (log2e
-// times the lowest number of a type would be -infinity).
-enum AtMode { kAtPlain, kAtCap, kAtSlopes, kAtGeneral };
+// What is done to the scores: nothing, a cap, slopes (these in log2 units, a scale above zero), a distance bias in shared memory, or all else
+// (these in natural units: log2e times the lowest number of a type would be -infinity; all else has a slower way only).
+enum AtMode { kAtPlain, kAtCap, kAtSlopes, kAtTable, kAtGeneral };
 
 constexpr int kAtMostSplits = 16;
 constexpr int kAtMostSummary = 256;  // steps whose documents are looked over ahead
@@ -248,8 +248,8 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     attend_kernel(const __grid_constant__ AttendMaps maps, const __grid_constant__ AttendArgs a) {
   using Cfg = AttendCfg<DP, NT>;
   constexpr int kSlots = Cfg::kSlots;
-  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value, kGeneral = kMode == kAtGeneral;
-  constexpr float kUnit = kGeneral ? 1.f : 1.4426950408889634f;  // of the scores: natural, or log2
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value, kGeneral = kMode == kAtGeneral, kNatural = kMode >= kAtTable;
+  constexpr float kUnit = kNatural ? 1.f : 1.4426950408889634f;  // of the scores: natural, or log2
   constexpr float kLog2e = 1.4426950408889634f;
   // float16 numerators end at 2^-24: they are kept 2^7 larger, so that weights down to 2^-31 of the largest count.
   constexpr float kShift = kBf16 ? 0.f : 7.f;
@@ -266,18 +266,12 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned long long wait_ns = wait_limit(a.wait_ns);
 
-  if (threadIdx.x == 0) {
-    for (int t = 0; t < NT; ++t) {
-      mbar_init(q_full + t, 1);
-      mbar_init(s_full + t, 1);
-      mbar_init(p_full + t, 4);
-      mbar_init(drain + t, 1);
+  if (warp == 0) {
+    for (int i = lane; i < Cfg::kBars; i += 32) {
+      const uint64_t* of = bar + i;
+      mbar_init(bar + i, of >= info_empty && of < s_full ? Cfg::kSoftmax + 1 : of >= p_full && of < drain ? 4 : of >= table_full ? Cfg::kSoftmax : 1);
     }
-    for (int i = 0; i < kSlots; ++i) { mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1); }
-    mbar_init(table_full, Cfg::kSoftmax);
-    mbar_init(summary_full, Cfg::kSoftmax);
-    for (int i = 0; i < kAtInfo; ++i) { mbar_init(info_full + i, 1); mbar_init(info_empty + i, Cfg::kSoftmax + 1); }
-    *abort_flag = 0;
+    if (lane == 0) *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == Cfg::kMmaWarp) { tmem_alloc(tmem_slot, Cfg::kTmemCols); tmem_relinquish(); }
@@ -349,7 +343,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     const int query = first + tile * per_tile + tile_token;
     const bool live = tile_token < tokens[tile];
     const bool warp_live = __any_sync(0xffffffffu, live);
-    float m = -INFINITY, l = 0.f;  // the maximum that P is relative to (log2 units, natural ones with kGeneral), and the sum
+    float m = -INFINITY, l = 0.f;  // the maximum that P is relative to (log2 units, natural ones with kNatural), and the sum
     const int p = query + offset;
     AttendSpan span = attend_span(a, p, s.keys);
     if (!live) span = {0, -1};
@@ -360,7 +354,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     const float* table = kGeneral && a.table ? a.table + (int64_t)(live ? head : 0) * (2 * a.reach + 1) + a.reach : nullptr;
     // The distance bias of the group's heads in shared memory, with the edges' values as far past the reach as a tile and a step make.
     const int wide = 2 * (a.reach + kAtKeys + kAtRows) + a.table_pad;
-    const bool table_here = kGeneral && a.table_here;
+    constexpr bool table_here = kMode == kAtTable;
     const float* near = reinterpret_cast<const float*>(smem + Cfg::kOffTable) + (head - kv * a.group) * wide + a.reach + kAtKeys + kAtRows;
     if (table_here) {
       float* to = reinterpret_cast<float*>(smem + Cfg::kOffTable);
@@ -505,9 +499,13 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       };
       // A step relative to the maximum of the steps before, from the products at once: the exponents' maximum, found beside them,
       // tells whether it will do (few steps raise it by more than kAtRescale).
+      const float fd = (float)d;
+      const float2 by = make_float2(scale, scale), unit = make_float2(kLog2e, kLog2e), shift = make_float2(kShift, kShift);
+      // The distance bias of the first key, in the part of the table that is there: past the reach all values are the edge's.
+      const float* bias = near + min(max(d, -(a.reach + kAtKeys + kAtRows)), a.reach + kAtRows);
       auto at_once = [&](auto masked) {
         const float base = m == -INFINITY ? 0.f : m;  // (rows that have seen nothing yet, and see nothing of this step)
-        const float2 by = make_float2(scale, scale), less = make_float2(kShift - base, kShift - base);
+        const float2 less = make_float2(kShift - base, kShift - base), at_m = make_float2(base, base);
         float most = INFINITY;
         if (kMode == kAtPlain) {
           most = numerators(masked, [&](float2 y, int) { return fma2(y, by, less); });
@@ -519,52 +517,54 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           // All keys on one side of the query.
           const bool left = d + kMine - 1 <= 0;
           if (__all_sync(0xffffffffu, left || d >= 0)) {
-            const float g = left ? slope : -slope, at_d = fmaf(g, (float)d, kShift - base);
+            const float g = left ? slope : -slope, at_d = fmaf(g, fd, kShift - base);
             const float2 from = make_float2(at_d, at_d), each = make_float2(g, g);
             most = numerators(masked, [&](float2 y, int i) { return fma2(y, by, fma2(each, make_float2((float)i, (float)(i + 1)), from)); });
           } else {
-            const float fd = (float)d;
             most = numerators(masked, [&](float2 y, int i) {
               return fma2(y, by, fma2(make_float2(-slope, -slope), make_float2(fabsf(fd + (float)i), fabsf(fd + (float)(i + 1))), less));
             });
           }
-        } else if (!capped && !a.slopes) {
-          const float2 unit = make_float2(kLog2e, kLog2e), shift = make_float2(kShift, kShift), at_m = make_float2(base, base);
-          // Past the reach on one side for all rows: one bias.
-          const bool left = table && d + kMine - 1 <= -a.reach;
-          if (!table || __all_sync(0xffffffffu, left || d >= a.reach)) {
-            const float edge = !table ? 0.f : __ldg(table + (left ? -a.reach : a.reach));
-            const float2 bias = make_float2(edge, edge);
-            most = numerators(masked, [&](float2 y, int) { return fma2(sub2(fma2(y, by, bias), at_m), unit, shift); });
-          } else if (table_here) {
-            // Some row is within the reach of some key, so all are within the reach and a step's and a warp's length of all.
-            most = numerators(masked, [&](float2 y, int i) { return fma2(sub2(fma2(y, by, make_float2(near[d + i], near[d + i + 1])), at_m), unit, shift); });
-          } else {
-            most = numerators(masked, [&](float2 y, int i) {
-              const float2 bias = make_float2(__ldg(table + min(max(d + i, -a.reach), a.reach)), __ldg(table + min(max(d + i + 1, -a.reach), a.reach)));
-              return fma2(sub2(fma2(y, by, bias), at_m), unit, shift);
-            });
-          }
+        } else if (kMode == kAtTable) {
+          most = numerators(masked, [&](float2 y, int i) { return fma2(sub2(fma2(y, by, make_float2(bias[i], bias[i + 1])), at_m), unit, shift); });
         }
         return __all_sync(0xffffffffu, most <= kShift + kAtRescale || !live);
       };
       bool done = false;
       const bool fresh = __any_sync(0xffffffffu, m == -INFINITY && live);
-      if ((kMode == kAtPlain || kMode == kAtCap) && fresh && whole) {
-        // A row's first scores: their maximum first.
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      // (With a cap and a mask the compiler finds no registers for both.)
+      if (!kGeneral && (kMode != kAtCap || whole || !fresh)) {
+        if (fresh) {
+          // A row's first scores: their maximum first.
+          uint32_t shown[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+          for (int c = 0; c < NC; ++c) {
+            shown[c] = kMode == kAtCap || whole ? ~0u : bits[c];
+            asm volatile("" : "+r"(shown[c]));  // (its selects are not to be kept in registers for those below)
+          }
+          auto highest = [&](auto score) {
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if (m == -INFINITY && top != -INFINITY) m = kMode == kAtCap ? cap.any(top) : top * scale;
-        done = at_once(std::false_type{});
-      } else if (!fresh) {
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float2 y = score(make_float2(__uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1])), 32 * c + i);
+                mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], kMode == kAtCap || ((shown[c] >> i) & 1) ? y.x : -INFINITY,
+                                        kMode == kAtCap || ((shown[c] >> (i + 1)) & 1) ? y.y : -INFINITY);
+              }
+            return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          };
+          float top;
+          if (kMode == kAtSlopes)
+            top = highest([&](float2 y, int i) { return fma2(y, by, make_float2(-slope * fabsf(fd + (float)i), -slope * fabsf(fd + (float)(i + 1)))); });
+          else if (kMode == kAtTable) top = highest([&](float2 y, int i) { return fma2(y, by, make_float2(bias[i], bias[i + 1])); });
+          else top = highest([&](float2 y, int) { return y; });
+          if (m == -INFINITY && top != -INFINITY) m = kMode == kAtCap ? cap.any(top) : kMode == kAtPlain ? top * scale : top;
+        }
         done = whole ? at_once(std::false_type{}) : at_once(std::true_type{});
       }
       if (!done) {
-        tmem_wait_st();  // before P is written again
+        if (!kGeneral) tmem_wait_st();  // before P is written again
         auto each = [&](auto f) {
 #pragma unroll
           for (int c = 0; c < NC; ++c)
@@ -587,31 +587,24 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
             return make_float2(fabsf(y.x) <= cap.most ? n.x : cap.any(y.x), fabsf(y.y) <= cap.most ? n.y : cap.any(y.y));
           });
         }
-        const float2 by = capped ? make_float2(1.f, 1.f) : make_float2(scale, scale);
+        const float2 factor = capped ? make_float2(1.f, 1.f) : by;
         if ((kMode == kAtSlopes || kGeneral) && a.slopes) {
-          const float fd = (float)d;
-          each([&](float2 y, int i) { return fma2(y, by, make_float2(-slope * fabsf(fd + (float)i), -slope * fabsf(fd + (float)(i + 1)))); });
+          each([&](float2 y, int i) { return fma2(y, factor, make_float2(-slope * fabsf(fd + (float)i), -slope * fabsf(fd + (float)(i + 1)))); });
+        } else if (kMode == kAtTable) {
+          each([&](float2 y, int i) { return fma2(y, factor, make_float2(bias[i], bias[i + 1])); });
         } else if (kGeneral && table) {
-          const bool left = d + kMine - 1 <= -a.reach;
-          if (__all_sync(0xffffffffu, left || d >= a.reach)) {
-            const float edge = __ldg(table + (left ? -a.reach : a.reach));
-            each([&](float2 y, int) { return fma2(y, by, make_float2(edge, edge)); });
-          } else if (table_here) {
-            each([&](float2 y, int i) { return fma2(y, by, make_float2(near[d + i], near[d + i + 1])); });
-          } else {
-            each([&](float2 y, int i) {
-              return fma2(y, by, make_float2(__ldg(table + min(max(d + i, -a.reach), a.reach)), __ldg(table + min(max(d + i + 1, -a.reach), a.reach))));
-            });
-          }
+          each([&](float2 y, int i) {
+            return fma2(y, factor, make_float2(__ldg(table + min(max(d + i, -a.reach), a.reach)), __ldg(table + min(max(d + i + 1, -a.reach), a.reach))));
+          });
         } else if (kMode == kAtPlain || (kGeneral && !capped)) {
-          each([&](float2 y, int) { return mul2(y, by); });
+          each([&](float2 y, int) { return mul2(y, factor); });
         }
         if (!whole) {
 #pragma unroll
           for (int c = 0; c < NC; ++c)
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!((bits[c] >> i) & 1)) sx[c][i] = __float_as_uint(-INFINITY);
+            for (int i = 0; i < 32; ++i)
+              if (!((bits[c] >> i) & 1)) sx[c][i] = __float_as_uint(-INFINITY);
         }
         float mx[8];
 #pragma unroll
@@ -627,8 +620,8 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         const float top = mx[0];
         float alpha = 1.f;
         bool dirty = false;
-        if (top > m + (kGeneral ? kAtRescale / kLog2e : kAtRescale)) {
-          if (m != -INFINITY) { alpha = ex2_approx(kGeneral ? (m - top) * kLog2e : m - top); dirty = true; }
+        if (top > m + (kNatural ? kAtRescale / kLog2e : kAtRescale)) {
+          if (m != -INFINITY) { alpha = ex2_approx(kNatural ? (m - top) * kLog2e : m - top); dirty = true; }
           m = top;
         }
         l *= alpha;
@@ -645,9 +638,9 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
-        const float2 at_m = make_float2(base, base), unit = make_float2(kLog2e, kLog2e), shift = make_float2(kShift, kShift), less = make_float2(kShift - base, kShift - base);
+        const float2 at_m = make_float2(base, base), less = make_float2(kShift - base, kShift - base);
         // Differences before the factor in natural units: scores of the type's lowest value stay equal to one another.
-        numerators(std::false_type{}, [&](float2 y, int) { return kGeneral ? fma2(sub2(y, at_m), unit, shift) : add2(y, less); });
+        numerators(std::false_type{}, [&](float2 y, int) { return kNatural ? fma2(sub2(y, at_m), unit, shift) : add2(y, less); });
       }
       l += sum;
       tmem_wait_st();
@@ -700,7 +693,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       }
       __syncwarp();
       if (live && a.lse)
-        a.lse[token * a.heads + head] = any ? (kGeneral ? m : m / kLog2e) + (log2f(l) - kShift) / kLog2e : -INFINITY;
+        a.lse[token * a.heads + head] = any ? (kNatural ? m : m / kLog2e) + (log2f(l) - kShift) / kLog2e : -INFINITY;
       // A value that is not finite may come from a key that this row's mask hides (its weight of zero times that value): such rows
       // are computed once more, from the visible keys alone.
       for (uint32_t again = __ballot_sync(0xffffffffu, live && poison != 0.f); again; again &= again - 1) {
@@ -965,7 +958,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
           // A part that saw nothing has no weight, and its O holds anything.
-          w[k] = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : ex2_approx(kGeneral ? (ml[k].x - top) * kLog2e : ml[k].x - top);
+          w[k] = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : ex2_approx(kNatural ? (ml[k].x - top) * kLog2e : ml[k].x - top);
           sum = fmaf(ml[k].y, w[k], sum);
         }
 #pragma unroll
@@ -980,7 +973,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           if (a.lse) {
             int qi, h;
             place(r, &qi, &h);
-            a.lse[(int64_t)(s.q_start + qi) * a.heads + h] = any ? (kGeneral ? top : top / kLog2e) + (log2f(sum) - kShift) / kLog2e : -INFINITY;
+            a.lse[(int64_t)(s.q_start + qi) * a.heads + h] = any ? (kNatural ? top : top / kLog2e) + (log2f(sum) - kShift) / kLog2e : -INFINITY;
           }
         }
       }

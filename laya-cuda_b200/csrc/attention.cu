@@ -111,7 +111,7 @@ void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   if (ctas > INT32_MAX) fail(LAYA_ERR_INVALID, "%d queries of %d sequences and %d heads are too many for one call", a.max_queries, a.sequences, a.heads);
   // The heads of a group on different banks for the rows of a warp.
   a.table_pad = a.group > 1 ? (32 - 2 * a.reach % 32 + 32 / std::min(a.group, 32)) % 32 : 0;
-  a.table_here = a.table && (int64_t)a.group * (2ll * (a.reach + kAtKeys + kAtRows) + a.table_pad) <= kAtMostTable;
+  const bool table_fits = a.table && (int64_t)a.group * (2ll * (a.reach + kAtKeys + kAtRows) + a.table_pad) <= kAtMostTable;
   a.by_group = FastDiv(a.group);
   a.by_splits = FastDiv(a.splits);
   a.by_kv = FastDiv(a.kv_heads);
@@ -121,9 +121,11 @@ void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   // Without a key there is nothing to load: any map will do.
   maps.k = a.k_tokens ? heads_map(kBf16, a.k, a.dim, a.kv_heads, a.k_tokens, a.k_head, a.k_token, 1, kAtKeys) : maps.q;
   maps.v = a.k_tokens ? heads_map(kBf16, a.v, a.dim, a.kv_heads, a.k_tokens, a.v_head, a.v_token, 1, kAtKeys) : maps.q;
-  if (a.table || !(a.scale > 0.f) || (a.slopes && a.cap > 0.f)) launch_attend_kernel<T, DP, NT, kAtGeneral, kQuarters>(a, maps, ctas, dev, st);
+  const bool positive = a.scale > 0.f, capped = a.cap > 0.f;
+  if (table_fits && !capped) launch_attend_kernel<T, DP, NT, kAtTable, kQuarters>(a, maps, ctas, dev, st);
+  else if (a.table || !positive || (a.slopes && capped)) launch_attend_kernel<T, DP, NT, kAtGeneral, kQuarters>(a, maps, ctas, dev, st);
   else if (a.slopes) launch_attend_kernel<T, DP, NT, kAtSlopes, kQuarters>(a, maps, ctas, dev, st);
-  else if (a.cap > 0.f) launch_attend_kernel<T, DP, NT, kAtCap, kQuarters>(a, maps, ctas, dev, st);
+  else if (capped) launch_attend_kernel<T, DP, NT, kAtCap, kQuarters>(a, maps, ctas, dev, st);
   else launch_attend_kernel<T, DP, NT, kAtPlain, kQuarters>(a, maps, ctas, dev, st);
 }
 

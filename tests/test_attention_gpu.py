@@ -672,3 +672,51 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable():
             _lib.check(lib.laya_set_launch_options(1, 0))
         assert err.item() == 5
         check(s)
+
+
+# -------------------------------------------------------------------------------- a layer
+
+def layer_example():
+    import importlib.util
+    from pathlib import Path
+    spec = importlib.util.spec_from_file_location("attention_layer", Path(__file__).resolve().parents[1] / "examples" / "attention_layer.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    return example
+
+
+def test_the_layer_example_runs(capsys):
+    seen = list(layer_example().main(6, 2, 64))
+    assert [s[:2] for s in seen] == [("prompt", 500), ("token", 1), ("prompt", 1720), ("token", 4)]
+    assert all(math.isfinite(s[2]) for s in seen) and capsys.readouterr().out.count("tokens") == 4
+
+
+def test_the_layer_is_its_operators_one_after_the_other():
+    """Prompts through the layer, bit for bit the operators' results, and tokens after them that see what the prompts left."""
+    from laya_cuda import mx8
+    example, g = layer_example(), generator(50)
+    heads, kv, dim, prompts = 4, 2, 32, [40, 9]
+    width, tokens = heads * dim, sum(prompts)
+    weight, qkv, out = randn(g, width).float(), randn(g, (heads + 2 * kv) * dim, width).float() * 0.1, randn(g, width, width).float() * 0.1
+    layer = example.AttentionLayer(weight, qkv, out, heads, kv)
+    cache = example.Cache(2, 64, kv, dim, torch.bfloat16)
+    x, r = randn(g, tokens, width).bfloat16(), randn(g, tokens, width).float()
+    positions = torch.cat([torch.arange(n, device="cuda") for n in prompts])
+    got = layer(x, r.clone(), ints([0, 40]), ints(prompts), positions, cache, 40)
+    n8, total, projected = mx8.Matrix.empty(x, tokens, width), r.clone(), torch.empty(tokens, (heads + 2 * kv) * dim, dtype=torch.bfloat16, device="cuda")
+    mx8.rms_norm(x, weight, n8, residual=total, sum_out=total)
+    mx8.linear(n8, layer.qkv, projected)
+    h = projected.view(tokens, heads + 2 * kv, dim)
+    q, k = torch.empty_like(h[:, :heads]).contiguous(), torch.empty(tokens, kv, dim, dtype=torch.bfloat16, device="cuda")
+    attention.rotary(h[:, :heads], positions, q, k=h[:, heads:-kv], k_out=k)
+    rows = torch.cat([b * 64 + torch.arange(n, device="cuda") for b, n in enumerate(prompts)])
+    assert torch.equal(cache.k[rows], k) and torch.equal(cache.v[rows], h[:, -kv:])
+    attended = torch.empty_like(q)
+    attention.attend(q, cache.k, cache.v, attended, ints([0, 40]), ints(prompts), cache.starts, ints(prompts), max_queries=40, max_keys=64, causal=True)
+    a8 = mx8.Matrix.empty(x, tokens, width)
+    mx8.quantize(attended.view(tokens, -1), a8)
+    mx8.linear(a8, layer.out, total, residual=total)
+    assert torch.equal(got, total)
+    kept = cache.k[rows].clone()
+    after = layer(x[:2], r[:2].clone(), ints([0, 1]), ints([1, 1]), torch.tensor(prompts, device="cuda"), cache, 1)
+    assert torch.equal(cache.k[rows], kept) and cache.lengths.tolist() == [41, 10] and bool(after.isfinite().all())
