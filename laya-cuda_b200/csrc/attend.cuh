@@ -472,8 +472,8 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       constexpr int kMine = 32 * NC;              // keys of this thread
       const int d = kb + 32 * chunk0 - p;  // the first less the query
       float sum = 0.f;
-      // P from the exponents that f gives of the scores, to TMEM; the largest exponent.  kMasked: of the keys that `bits` shows.
-      auto numerators = [&](auto masked, auto f) {
+      // P from the exponents that f gives of the scores, to TMEM; the largest exponent.
+      auto numerators = [&](auto f) {
         float2 part[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -481,11 +481,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            float2 v = f(make_float2(__uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1])), 32 * c + i);
-            if (decltype(masked)::value) {
-              if (!((bits[c] >> i) & 1)) v.x = -INFINITY;
-              if (!((bits[c] >> (i + 1)) & 1)) v.y = -INFINITY;
-            }
+            const float2 v = f(make_float2(__uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1])), 32 * c + i);
             mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], v.x, v.y);
             const float2 w = make_float2(ex2_approx(v.x), ex2_approx(v.y));
             part[(i >> 1) & 3] = add2(part[(i >> 1) & 3], w);
@@ -503,15 +499,15 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       const float2 by = make_float2(scale, scale), unit = make_float2(kLog2e, kLog2e), shift = make_float2(kShift, kShift);
       // The distance bias of the first key, in the part of the table that is there: past the reach all values are the edge's.
       const float* bias = near + min(max(d, -(a.reach + kAtKeys + kAtRows)), a.reach + kAtRows);
-      auto at_once = [&](auto masked) {
-        const float base = m == -INFINITY ? 0.f : m;  // (rows that have seen nothing yet, and see nothing of this step)
+      auto at_once = [&]() {
+        const float base = m == -INFINITY ? 0.f : m;  // (scores of -infinity)
         const float2 less = make_float2(kShift - base, kShift - base), at_m = make_float2(base, base);
         float most = INFINITY;
         if (kMode == kAtPlain) {
-          most = numerators(masked, [&](float2 y, int) { return fma2(y, by, less); });
+          most = numerators([&](float2 y, int) { return fma2(y, by, less); });
         } else if (kMode == kAtCap) {
           float big = 0.f;
-          most = numerators(masked, [&](float2 y, int) { big = max3(big, fabsf(y.x), fabsf(y.y)); return fma2(y, cap.slope(y), less); });
+          most = numerators([&](float2 y, int) { big = max3(big, fabsf(y.x), fabsf(y.y)); return fma2(y, cap.slope(y), less); });
           if (!(big <= cap.most)) most = INFINITY;
         } else if (kMode == kAtSlopes) {
           // All keys on one side of the query.
@@ -519,29 +515,22 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           if (__all_sync(0xffffffffu, left || d >= 0)) {
             const float g = left ? slope : -slope, at_d = fmaf(g, fd, kShift - base);
             const float2 from = make_float2(at_d, at_d), each = make_float2(g, g);
-            most = numerators(masked, [&](float2 y, int i) { return fma2(y, by, fma2(each, make_float2((float)i, (float)(i + 1)), from)); });
+            most = numerators([&](float2 y, int i) { return fma2(y, by, fma2(each, make_float2((float)i, (float)(i + 1)), from)); });
           } else {
-            most = numerators(masked, [&](float2 y, int i) {
+            most = numerators([&](float2 y, int i) {
               return fma2(y, by, fma2(make_float2(-slope, -slope), make_float2(fabsf(fd + (float)i), fabsf(fd + (float)(i + 1))), less));
             });
           }
         } else if (kMode == kAtTable) {
-          most = numerators(masked, [&](float2 y, int i) { return fma2(sub2(fma2(y, by, make_float2(bias[i], bias[i + 1])), at_m), unit, shift); });
+          most = numerators([&](float2 y, int i) { return fma2(sub2(fma2(y, by, make_float2(bias[i], bias[i + 1])), at_m), unit, shift); });
         }
         return __all_sync(0xffffffffu, most <= kShift + kAtRescale || !live);
       };
       bool done = false;
-      const bool fresh = __any_sync(0xffffffffu, m == -INFINITY && live);
-      // (With a cap and a mask the compiler finds no registers for both.)
-      if (!kGeneral && (kMode != kAtCap || whole || !fresh)) {
-        if (fresh) {
+      // (Masked steps take the other way: a second form of this one for them was no faster for them, and 3% slower for all, by its code's length.)
+      if (!kGeneral && whole) {
+        if (__any_sync(0xffffffffu, m == -INFINITY && live)) {
           // A row's first scores: their maximum first.
-          uint32_t shown[NC];
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            shown[c] = kMode == kAtCap || whole ? ~0u : bits[c];
-            asm volatile("" : "+r"(shown[c]));  // (its selects are not to be kept in registers for those below)
-          }
           auto highest = [&](auto score) {
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -549,8 +538,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
                 const float2 y = score(make_float2(__uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1])), 32 * c + i);
-                mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], kMode == kAtCap || ((shown[c] >> i) & 1) ? y.x : -INFINITY,
-                                        kMode == kAtCap || ((shown[c] >> (i + 1)) & 1) ? y.y : -INFINITY);
+                mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], y.x, y.y);
               }
             return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           };
@@ -561,7 +549,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           else top = highest([&](float2 y, int) { return y; });
           if (m == -INFINITY && top != -INFINITY) m = kMode == kAtCap ? cap.any(top) : kMode == kAtPlain ? top * scale : top;
         }
-        done = whole ? at_once(std::false_type{}) : at_once(std::true_type{});
+        done = at_once();
       }
       if (!done) {
         if (!kGeneral) tmem_wait_st();  // before P is written again
@@ -640,7 +628,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         const float base = m == -INFINITY ? 0.f : m;
         const float2 at_m = make_float2(base, base), less = make_float2(kShift - base, kShift - base);
         // Differences before the factor in natural units: scores of the type's lowest value stay equal to one another.
-        numerators(std::false_type{}, [&](float2 y, int) { return kNatural ? fma2(sub2(y, at_m), unit, shift) : add2(y, less); });
+        numerators([&](float2 y, int) { return kNatural ? fma2(sub2(y, at_m), unit, shift) : add2(y, less); });
       }
       l += sum;
       tmem_wait_st();
