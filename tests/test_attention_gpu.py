@@ -640,6 +640,20 @@ def test_caps_far_below_and_far_above_the_scores(scale, cap, queries, keys, dtyp
     check(problem(34, queries, keys, heads=4, kv_heads=2, dim=64, dtype=dtype, scale=scale, cap=cap, causal=True))
 
 
+@pytest.mark.parametrize("cap", [2e3, 1e4, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("queries,keys", [([300], None), ([1, 3], [900, 200])])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_a_cap_that_no_score_reaches_changes_little(cap, queries, keys, slopes):
+    # |x - cap tanh(x / cap)| <= |x|^3 / (3 cap^2), and |x| is below 10: scores of 64 products with a deviation of 1.
+    s = problem(36, queries, keys, heads=4, kv_heads=2, dim=64, dtype="bf16", cap=cap, causal=True, **(with_bias(dict(slopes=True), 4) if slopes else {}))
+    out, lse = run(s)
+    how = {k: v for k, v in s["how"].items() if k != "cap"}
+    want, want_lse, slack, lse_slack = define(dict(s, how=how))
+    less = 1000 / (3 * cap * cap)
+    assert ((lse.double() - want_lse).abs() <= lse_slack + less).all()
+    assert ((out.double() - want).abs() <= slack + 2 * less * s["v"].double().abs().max()).all()
+
+
 @pytest.mark.parametrize("slope", [0.0, 1e-6, 3.0, -0.25])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("queries,keys", [([500], None), ([1, 40], [3000, 700])])
