@@ -28,6 +28,7 @@ struct AttendArgs {
   unsigned long long wait_ns;
   int per_tile;       // queries of a tile, which holds all heads of a group for each
   int table_pad;      // values between the heads of a distance bias in shared memory
+  int longest_first;  // the sequences in the order of their keys' number (one pair; kAtMostOrdered of them at most)
   int pairs, splits;  // CTAs for max_queries of a kv head; CTAs (a cluster) that share a tile's keys
   FastDiv by_group, by_splits, by_kv, by_sequences;
 };
@@ -133,6 +134,7 @@ enum AtClass : int { kAtEnd = -1, kAtSkip = 0, kAtMasked = 1, kAtFull = 2 };
 enum AtMode { kAtPlain, kAtCap, kAtSlopes, kAtTable, kAtGeneral };
 
 constexpr int kAtMostSplits = 16;
+constexpr int kAtMostOrdered = 128;  // sequences that are put in order
 constexpr int kAtMostSummary = 256;  // steps whose documents are looked over ahead
 constexpr int kAtMostTable = 4096;  // values of the distance bias that are kept in shared memory, clamped past the reach
 
@@ -163,6 +165,7 @@ struct AttendCfg {
   static constexpr int kBytes = kOffSummary + kAtMostSummary * 8 + 1024;
   static_assert(kOffSums % 8 == 0, "alignment");
   static_assert(2 * kAtMostSplits <= 32, "a lane per part");
+  static_assert(kAtMostOrdered < kWeights && kAtMostOrdered <= kThreads, "lengths in the place of the weights, a thread each");
   static_assert(NT * kAtRows * DP * 4 <= 2 * kSlots * kTile, "a part's O fits the K and V tiles");
   static_assert(kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory");
 };
@@ -217,7 +220,7 @@ __device__ __forceinline__ AttendSpan attend_span(const AttendArgs& a, int p, in
 }
 
 // out tanh(in s) for a raw product s, with out in some unit.
-//   near  for |in s| <= 0.8: s times a polynomial in s^2 by the Remez exchange algorithm, on the FMA pipe; off by 1.2e-7 of itself (a term
+//   near  for |in s| <= 0.8 (less with large caps): s times a polynomial in s^2 by the Remez exchange algorithm, on the FMA pipe; off by 1.2e-7 of itself (a term
 //         less made the logarithms of the sums ten times less exact than the exponentials do)
 //   any   out - 2 out / (exp(2 in s) + 1) on the special-function unit; off by 2^-21 out
 struct CapTerms {
@@ -227,8 +230,13 @@ struct CapTerms {
     float power = out * in;
 #pragma unroll
     for (int i = 0; i < 6; ++i) { c[i] = kC[i] * power; power *= in * in; }
-    // Where the eleventh power of `in` stays in range (0.09 / cap up to caps of 300).
-    most = fabsf(c[5]) > 1e-36f && fabsf(c[5]) < 1e30f ? 0.8f / fabsf(in) : -1.f;
+    // Caps far above the scale (300 and more for 0.09) take the last factors below fp32's range: as far as the terms that are left reach.
+    constexpr float kReach[6] = {5e-4f, 0.03f, 0.1f, 0.2f, 0.3f, 0.8f}, kLeast = 1e-36f;
+    most = kReach[0];
+#pragma unroll
+    for (int i = 1; i < 6; ++i)
+      if (fabsf(c[i]) > kLeast) most = kReach[i];
+    most = fabsf(c[5]) < 1e30f ? most / fabsf(in) : -1.f;
   }
   __device__ __forceinline__ float2 slope(float2 s) const {  // out tanh(in s) / s
     const float2 z = mul2(s, s);
@@ -240,6 +248,7 @@ struct CapTerms {
   __device__ __forceinline__ float any(float s) const {
     return fmaf(-2.f * out, rcp_approx(ex2_approx(s * (in * 2.8853900817779268f)) + 1.f), out);
   }
+  __device__ __forceinline__ float one(float s) const { return fabsf(s) <= most ? s * slope(make_float2(s, s)).x : any(s); }
 };
 
 // T, the padded head size, and what is done to the scores.
@@ -288,7 +297,21 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
   const uint32_t of_kv = a.by_kv.div(item);
   const int kv = item - of_kv * a.kv_heads;
   const uint32_t of_sequence = a.by_sequences.div(of_kv);
-  const int b = of_kv - of_sequence * a.sequences;
+  int b = of_kv - of_sequence * a.sequences;
+  if (kQuarters && a.longest_first) {
+    // The sequence with b others before it.
+    int *lengths = reinterpret_cast<int*>(smem + Cfg::kOffWeights), *found = lengths + kAtMostOrdered, me = threadIdx.x;
+    if (me < a.sequences) lengths[me] = a.k_lengths[me];
+    __syncthreads();
+    if (me < a.sequences) {
+      int before = 0;
+#pragma unroll 8
+      for (int i = 0; i < a.sequences; ++i) before += lengths[i] > lengths[me] || (lengths[i] == lengths[me] && i < me);
+      if (before == b) *found = me;
+    }
+    __syncthreads();
+    b = *found;
+  }
   const int pair = a.pairs - 1 - (int)of_sequence;
   int all_queries;
   const AttendSequence s = attend_sequence(a, b, &all_queries);
@@ -547,7 +570,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
             top = highest([&](float2 y, int i) { return fma2(y, by, make_float2(-slope * fabsf(fd + (float)i), -slope * fabsf(fd + (float)(i + 1)))); });
           else if (kMode == kAtTable) top = highest([&](float2 y, int i) { return fma2(y, by, make_float2(bias[i], bias[i + 1])); });
           else top = highest([&](float2 y, int) { return y; });
-          if (m == -INFINITY && top != -INFINITY) m = kMode == kAtCap ? cap.any(top) : kMode == kAtPlain ? top * scale : top;
+          if (m == -INFINITY && top != -INFINITY) m = kMode == kAtCap ? cap.one(top) : kMode == kAtPlain ? top * scale : top;
         }
         done = at_once();
       }

@@ -107,7 +107,15 @@ void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   const int blocks = (max_keys + kAtKeys - 1) / kAtKeys, sms = sm_count(dev);
   a.splits = 1;
   while (a.splits < kAtMostSplits && items * a.splits * 2 <= sms && a.splits * 4 <= blocks && (a.splits < 8 || items <= 4)) a.splits *= 2;
+  // Single tokens over long caches, whose lengths differ: also past one CTA per SM, while parts keep 16 steps, so that the longest cache is not what all
+  // wait for (8 kv heads; 16 caches, one of 32768 keys and the others 4096 on: 330 -> 260 us, all of 32768 356 -> 373; 6 up to 16384 92 -> 63, all 100 -> 113;
+  // 24 up to 16384 186 -> 168, all 350 -> 295).  Clusters of 8 for few more than the SMs: 3 up to 65536 167 -> 111, all 177 -> 194; 4 of 32768 110 -> 165.
+  if (kQuarters)
+    while (a.splits < 8 && 3 * items * a.splits * 2 <= (a.splits < 4 ? 9 : 4) * sms && a.splits * 32 <= blocks) a.splits *= 2;
   const int64_t ctas = items * a.splits;
+  // The longest caches first where not all CTAs run at once: 64 caches up to 16384 442 -> 365 us, 32 283 -> 195; short ones lose more by it than they
+  // gain (64 up to 1000 61 -> 64).
+  a.longest_first = kQuarters && ctas > sms && a.sequences <= kAtMostOrdered && blocks >= 32;
   if (ctas > INT32_MAX) fail(LAYA_ERR_INVALID, "%d queries of %d sequences and %d heads are too many for one call", a.max_queries, a.sequences, a.heads);
   // The heads of a group on different banks for the rows of a warp.
   a.table_pad = a.group > 1 ? (32 - 2 * a.reach % 32 + 32 / std::min(a.group, 32)) % 32 : 0;

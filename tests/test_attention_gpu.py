@@ -640,6 +640,17 @@ def test_caps_far_below_and_far_above_the_scores(scale, cap, queries, keys, dtyp
     check(problem(34, queries, keys, heads=4, kv_heads=2, dim=64, dtype=dtype, scale=scale, cap=cap, causal=True))
 
 
+@pytest.mark.parametrize("sequences,kv_heads,dim", [(3, 8, 128), (6, 8, 64), (13, 8, 128), (24, 8, 64), (128, 2, 64), (129, 2, 64)])
+@pytest.mark.parametrize("queries", [1, 2])
+def test_single_tokens_over_caches_of_all_lengths(sequences, kv_heads, dim, queries):
+    keys = [[4700, 0, 1, 4700, 129, 8200, 3000, 0, 128, 6000][b % 10] // (1 if sequences < 100 else 4) for b in range(sequences)]
+    s = problem(37, [queries] * sequences, keys, heads=2 * kv_heads, kv_heads=kv_heads, dim=dim, causal=True)
+    check(s)
+    first = run(s, max_keys=40000)
+    check(s, first)
+    assert all(torch.equal(a, b) for a, b in zip(first, run(s, max_keys=40000)))
+
+
 @pytest.mark.parametrize("cap", [2e3, 1e4, 1e6, 1e9, 1e30])
 @pytest.mark.parametrize("queries,keys", [([300], None), ([1, 3], [900, 200])])
 @pytest.mark.parametrize("slopes", [False, True])
