@@ -438,7 +438,7 @@ typedef struct laya_attend {
   const int32_t *documents, *k_documents;  /* [q_tokens], [k_tokens], or both NULL */
   const float* slopes;           /* [heads] or NULL */
   const float* distance_bias;    /* [heads][2 reach + 1] or NULL; not with slopes */
-  int32_t reach;
+  int32_t reach;                 /* up to 2^30 - 1024 */
   int32_t reserved;
 } laya_attend;
 

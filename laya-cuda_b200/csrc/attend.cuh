@@ -112,13 +112,24 @@ __device__ void attend_row(const AttendArgs& a, const AttendSequence& s, int ful
 }
 
 // ---------------------------------------------------------------------------------------------
-// The kernel: a CTA takes two tiles of 128 rows, a row being one query of one head of a kv head's group, and walks the keys in
-// steps of 128.
+// The kernel.  out = sum_j softmax(s)_j v_j in one pass over the keys: with m a running bound of a row's scores, the numerators P = exp(s - m) of a step
+// and their sum l are relative to m; where a row's scores have grown by more than 2^8 beyond it, m follows and O and l are scaled by exp(m_old - m).
 //
-// Warps 0-3 are the softmax of tile 0, warps 4-7 of tile 1 (a thread per row, warp w owning TMEM lanes 32 (w % 4) on); of the others one
-// issues the tensor products, and one finds the steps that the masks leave and loads them.  TMEM: S of each tile (128 columns),
+// A CTA takes tiles of 128 rows, a row being one query of one head of a kv head's group (so that the group reads its keys once), and walks the
+// keys in steps of 128.  Warps 0-3 are the softmax of tile 0, warps 4-7 of tile 1 (a thread per row, warp w owning TMEM lanes 32 (w % 4) on); of the
+// others one issues the tensor products, and one finds the steps that the masks leave and loads them by TMA.  TMEM: S of each tile (128 columns),
 // O of each; P goes over S as 16-bit pairs.  The tensor core runs the products in issue order, so O += P V of a step and then S = Q K^T
 // of the next are issued together as soon as P is there, and the other tile's softmax hides them.
+//
+// What bounds it: with prompts the softmax.  A step of a tile with heads of 128 is 2 x 128^3 multiply-adds, some 512 cycles of the tensor core, and 128 x 128
+// exponentials, 1024 cycles of the special-function units that the two tiles share out: 16384 causal tokens, 16 heads of 128 over 4, bf16, 977 us (1.13 PFLOP/s
+// of 1.66), not causal 8192 565 us (0.97); heads of 64, which have as many exponentials for half the products, 853 us (0.64); a cap doubles the work on the FMA
+// pipe (1425 us); slopes cost 11%.  Single tokens: the caches' bytes, 6.0 TB/s (16 x 32768 keys, 8 kv heads of 128, 2.1 GB).  A few queries over one cache: the chain of
+// launch, first loads, products and the join (1 x 4000 keys 20 us, 1 x 96 7 us).
+//
+// Tiles: with heads past 64 two to a CTA and one CTA per SM (one tile, two CTAs: 16384 causal 977 -> 1040 us, documents 199 -> 229, a long prompt with a cap
+// and slopes 1475 -> 1604: K and V are loaded twice, and shared memory leaves them one buffer).  Heads up to 64: one to a CTA and two CTAs per SM, whose
+// starts and ends overlap (64 ragged sequences up to 1024 tokens 392 us; two tiles to a CTA 475).
 //
 // Where one tile holds all rows, both take them, and each every other step; the parts are joined at the end as those of a split
 // are.  Where a quarter of a tile holds them (single tokens over a cache), each quarter has a copy of them and takes a quarter of
@@ -144,7 +155,8 @@ struct AttendCfg {
   static_assert((DP == 64 || DP == 128) && (NT == 1 || NT == 2), "padded head size, tiles");
   static constexpr int kSoftmax = 4 * NT;                // softmax warps
   static constexpr int kMmaWarp = kSoftmax, kLoadWarp = kSoftmax + 1, kThreads = 32 * (kSoftmax + 4), kCtas = NT == 1 ? 2 : 1;
-  // Registers: what the launch gives all threads (128 with one tile, 168 with two), moved to the softmax.
+  // Registers: what the launch gives all threads (128 with one tile, 168 with two), moved to the softmax, whose threads hold a step's 128 scores.
+  // (224 and 56 with two tiles: a cap 3% faster, slopes and windows slower.)
   static constexpr int kSoftmaxRegs = NT == 1 ? 200 : 216, kOtherRegs = NT == 1 ? 56 : 72;
   static_assert(32 * (kSoftmax * kSoftmaxRegs + 4 * kOtherRegs) <= kThreads * (NT == 1 ? 128 : 168), "registers of the launch");
   static constexpr int kTmemO = 128 * NT, kTmemCols = NT == 1 ? 256 : 512;  // columns: O of tile 0, all

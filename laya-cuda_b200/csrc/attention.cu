@@ -193,6 +193,7 @@ int laya_op_rotary(const laya_rotary* p, void* stream) {
   a.magnitude = p->magnitude;
   constexpr double kTurn = 6.283185307179586;
   const double theta = p->theta * (p->scaling == LAYA_ROTARY_NTK ? std::pow(p->factor, p->dims / (p->dims - 2.0)) : 1.0);
+  if (!(theta > 0) || !std::isfinite(theta)) fail(LAYA_ERR_INVALID, "factor %g takes theta %g out of range", p->factor, p->theta);
   a.step = -2.0 / p->dims * std::log2(theta);
   a.power = -std::log2(p->scaling == LAYA_ROTARY_LINEAR ? kTurn * p->factor : kTurn);
   a.by_parts = p->scaling == LAYA_ROTARY_PARTS;
@@ -238,7 +239,9 @@ int laya_op_attend(const laya_attend* p, int* err, void* stream) {
   if (!(p->cap >= 0.f) || !std::isfinite(p->cap)) fail(LAYA_ERR_INVALID, "cap must be at least 0");
   if (p->window_left < -1 || p->window_right < -1) fail(LAYA_ERR_INVALID, "window bounds must be at least 0, or -1 for none");
   if (p->slopes && p->distance_bias) fail(LAYA_ERR_INVALID, "slopes and distance_bias cannot both be given");
-  if (p->distance_bias && p->reach < 0) fail(LAYA_ERR_INVALID, "reach must be at least 0");
+  // (Twice the reach and a step to either side of it are counted in 32 bits.)
+  constexpr int kMostReach = (1 << 30) - 1024;
+  if (p->distance_bias && (p->reach < 0 || p->reach > kMostReach)) fail(LAYA_ERR_INVALID, "reach %d must be at least 0 and at most %d", p->reach, kMostReach);
   if (!p->documents != !p->k_documents) fail(LAYA_ERR_INVALID, "documents and k_documents go together");
   if (!p->k_starts != !p->k_lengths) fail(LAYA_ERR_INVALID, "k_starts and k_lengths go together");
   if (!p->sequences || !p->q_tokens || !p->max_queries) return LAYA_OK;

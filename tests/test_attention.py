@@ -28,7 +28,7 @@ def rotary(part=None, **other):
     (dict(dims=66), None, "dims"), (dict(head_dim=2000, dims=514), None, "dims"), (dict(dtype=3), None, "dtype"),
     (dict(scaling=4), None, "scaling"), (dict(scaling=-1), None, "scaling"), (dict(theta=0.0), None, "theta"),
     (dict(theta=float("nan")), None, "theta"), (dict(scaling=1, factor=0.0), None, "factor"),
-    (dict(scaling=2, factor=2.0, dims=2), None, "ntk"), (dict(scaling=3, factor=2.0, length=0.0), None, "length"),
+    (dict(scaling=2, factor=2.0, dims=2), None, "ntk"), (dict(scaling=2, factor=1e300, theta=1e300), None, "out of range"), (dict(scaling=3, factor=2.0, length=0.0), None, "length"),
     (dict(scaling=3, factor=2.0, low=4.0, high=4.0), None, "low"), (dict(positions=None), None, "positions"),
     (dict(positions=P + 2), None, "positions"), (dict(positions=P + 4, positions_64=1), None, "positions"),
     ({}, dict(heads=-1), "heads"), ({}, dict(x=None), "null"), ({}, dict(out=None), "null"), ({}, dict(x=P + 1), "aligned"),
@@ -55,7 +55,7 @@ def attend(**other):
     (dict(kv_heads=3), "heads"), (dict(heads=258), "128"), (dict(head_dim=0), "head"), (dict(head_dim=60), "multiple of 8"),
     (dict(head_dim=136), "128"), (dict(dtype=0), "dtype"), (dict(dtype=3), "dtype"), (dict(scale=float("inf")), "scale"),
     (dict(cap=-1.0), "cap"), (dict(cap=float("nan")), "cap"), (dict(window_left=-2), "window"), (dict(window_right=-5), "window"),
-    (dict(slopes=P, distance_bias=P), "both"), (dict(distance_bias=P, reach=-1), "reach"), (dict(documents=P), "documents"),
+    (dict(slopes=P, distance_bias=P), "both"), (dict(distance_bias=P, reach=-1), "reach"), (dict(distance_bias=P, reach=2 ** 30), "reach"), (dict(documents=P), "documents"),
     (dict(k_documents=P), "documents"), (dict(k_starts=None), "k_lengths"), (dict(k_lengths=None), "k_starts"),
     (dict(starts=None), "null"), (dict(lengths=None), "null"), (dict(q=None), "null"), (dict(k=None), "null"), (dict(v=None), "null"),
     (dict(out=None), "null"), (dict(q=P + 8), "16-byte"), (dict(k=P + 2), "16-byte"), (dict(v=P + 4), "16-byte"),
