@@ -127,8 +127,8 @@ __device__ void attend_row(const AttendArgs& a, const AttendSequence& s, int ful
 // pipe (1425 us); slopes cost 11%.  Single tokens: the caches' bytes, 6.0 TB/s (16 x 32768 keys, 8 kv heads of 128, 2.1 GB).  A few queries over one cache: the chain of
 // launch, first loads, products and the join (1 x 4000 keys 20 us, 1 x 96 7 us).
 //
-// Tiles: with heads past 64 two to a CTA and one CTA per SM (one tile, two CTAs: 16384 causal 976 -> 999 us, documents 207 -> 229, a long prompt with slopes
-// 1494 -> 1604: K and V are loaded twice, into one buffer each).  Heads up to 64: one to a CTA and two CTAs per SM, whose starts and ends overlap
+// Tiles: with heads past 64 two to a CTA and one CTA per SM (one tile, two CTAs: 16384 causal 976 -> 999 us, with a cap 1441 -> 1482, 8192 tokens
+// in documents 207 -> 229: K and V are loaded twice, into one buffer each).  Heads up to 64: one to a CTA and two CTAs per SM, whose starts and ends overlap
 // (two tiles: 16384 causal 854 -> 915 us, 64 x 1024 444 -> 461, 1 x 1000 27 -> 32; with a distance bias 64 ragged sequences up to 1024 402 -> 369, but
 // 64 x 250 74 -> 82 and 40 causal ones up to 500 63 -> 73).
 //
