@@ -122,9 +122,9 @@ __device__ void attend_row(const AttendArgs& a, const AttendSequence& s, int ful
 // of the next are issued together as soon as P is there, and the other tile's softmax hides them.
 //
 // What bounds it: with prompts the softmax.  A step of a tile with heads of 128 is 2 x 128^3 multiply-adds, some 512 cycles of the tensor core, and 128 x 128
-// exponentials, 1024 cycles of the special-function units that the two tiles share out: 16384 causal tokens, 16 heads of 128 over 4, bf16, 977 us (1.13 PFLOP/s
-// of 1.66), not causal 8192 565 us (0.97); heads of 64, which have as many exponentials for half the products, 853 us (0.64); a cap doubles the work on the FMA
-// pipe (1425 us); slopes cost 11%.  Single tokens: the caches' bytes, 6.0 TB/s (16 x 32768 keys, 8 kv heads of 128, 2.1 GB).  A few queries over one cache: the chain of
+// exponentials, 1024 cycles of the special-function units that the two tiles share out: 16384 causal tokens, 16 heads of 128 over 4, bf16, 973 us (1.13 PFLOP/s
+// of 1.66), not causal 8192 559 us (0.98); heads of 64, which have as many exponentials for half the products, 849 us (0.64); a cap doubles the work on the FMA
+// pipe (1389 us); slopes cost 10%.  Single tokens: the caches' bytes, 6.0 TB/s (16 x 32768 keys, 8 kv heads of 128, 2.1 GB).  A few queries over one cache: the chain of
 // launch, first loads, products and the join (1 x 4000 keys 20 us, 1 x 96 7 us).
 //
 // Tiles: with heads past 64 two to a CTA and one CTA per SM (one tile, two CTAs: 16384 causal 976 -> 999 us, with a cap 1441 -> 1482, 8192 tokens
@@ -261,7 +261,6 @@ struct CapTerms {
   __device__ __forceinline__ float any(float s) const {
     return fmaf(-2.f * out, rcp_approx(ex2_approx(s * (in * 2.8853900817779268f)) + 1.f), out);
   }
-  __device__ __forceinline__ float one(float s) const { return fabsf(s) <= most ? s * slope(make_float2(s, s)).x : any(s); }
 };
 
 // T, the padded head size, and what is done to the scores.
@@ -536,7 +535,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       // The distance bias of the first key, in the part of the table that is there: past the reach all values are the edge's.
       const float* bias = near + min(max(d, -(a.reach + kAtKeys + kAtRows)), a.reach + kAtRows);
       auto at_once = [&]() {
-        const float base = m == -INFINITY ? 0.f : m;  // (scores of -infinity)
+        const float base = m == -INFINITY ? 0.f : m;  // (rows of no query)
         const float2 less = make_float2(kShift - base, kShift - base), at_m = make_float2(base, base);
         float most = INFINITY;
         if (kMode == kAtPlain) {
@@ -563,30 +562,10 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         return __all_sync(0xffffffffu, most <= kShift + kAtRescale || !live);
       };
       bool done = false;
-      // (Masked steps take the other way: a second form of this one for them was no faster for them, and 3% slower for all, by its code's length.)
-      if (!kGeneral && whole) {
-        if (__any_sync(0xffffffffu, m == -INFINITY && live)) {
-          // A row's first scores: their maximum first.
-          auto highest = [&](auto score) {
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                const float2 y = score(make_float2(__uint_as_float(sx[c][i]), __uint_as_float(sx[c][i + 1])), 32 * c + i);
-                mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], y.x, y.y);
-              }
-            return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          };
-          float top;
-          if (kMode == kAtSlopes)
-            top = highest([&](float2 y, int i) { return fma2(y, by, make_float2(-slope * fabsf(fd + (float)i), -slope * fabsf(fd + (float)(i + 1)))); });
-          else if (kMode == kAtTable) top = highest([&](float2 y, int i) { return fma2(y, by, make_float2(bias[i], bias[i + 1])); });
-          else top = highest([&](float2 y, int) { return y; });
-          if (m == -INFINITY && top != -INFINITY) m = kMode == kAtCap ? cap.one(top) : kMode == kAtPlain ? top * scale : top;
-        }
-        done = at_once();
-      }
+      // Masked steps and a row's first one take the other way: a second form of this one for masked steps made all 3% slower by its code's length, and
+      // a first maximum from the raw products, so that first steps too come here, took longer than it saved (a learned bias 189 -> 180 us at 64 x 512, a
+      // cap at 16384 causal 1436 -> 1389; plain ragged sequences of 64 306 -> 310).
+      if (!kGeneral && whole && !__any_sync(0xffffffffu, m == -INFINITY && live)) done = at_once();
       if (!done) {
         if (!kGeneral) tmem_wait_st();  // before P is written again
         auto each = [&](auto f) {
