@@ -28,9 +28,10 @@ struct AttendArgs {
   unsigned long long wait_ns;
   int per_tile;       // queries of a tile, which holds all heads of a group for each
   int table_pad;      // values between the heads of a distance bias in shared memory
+  int pairs_inside;   // a sequence's pairs one after the other, not all sequences' last ones first
   int longest_first;  // the sequences in the order of their keys' number (one pair; kAtMostOrdered of them at most)
   int pairs, splits;  // CTAs for max_queries of a kv head; CTAs (a cluster) that share a tile's keys
-  FastDiv by_group, by_splits, by_kv, by_sequences;
+  FastDiv by_group, by_splits, by_kv, by_inner;  // by_inner: by pairs, or by sequences
 };
 
 struct AttendSequence {
@@ -303,13 +304,14 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
 
-  // The work item: split x kv head x sequence x group of tiles, the last queries first (they see the most keys under a causal mask).
+  // The work item: split x kv head x sequence x group of tiles, the last queries first (they see the most keys under a causal mask); or with the
+  // tiles inside the sequences.
   uint32_t item = a.by_splits.div(blockIdx.x);
   const int split = blockIdx.x - item * a.splits;
   const uint32_t of_kv = a.by_kv.div(item);
   const int kv = item - of_kv * a.kv_heads;
-  const uint32_t of_sequence = a.by_sequences.div(of_kv);
-  int b = of_kv - of_sequence * a.sequences;
+  const int outer_index = a.by_inner.div(of_kv), inner_index = of_kv - outer_index * (a.pairs_inside ? a.pairs : a.sequences);
+  int b = a.pairs_inside ? outer_index : inner_index;
   if (kQuarters && a.longest_first) {
     // The sequence with b others before it.
     int *lengths = reinterpret_cast<int*>(smem + Cfg::kOffWeights), *found = lengths + kAtMostOrdered, me = threadIdx.x;
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     __syncthreads();
     b = *found;
   }
-  const int pair = a.pairs - 1 - (int)of_sequence;
+  const int pair = a.pairs - 1 - (a.pairs_inside ? inner_index : outer_index);
   int all_queries;
   const AttendSequence s = attend_sequence(a, b, &all_queries);
   const int offset = s.keys - all_queries;  // a query's position less its number

@@ -651,6 +651,13 @@ def test_single_tokens_over_caches_of_all_lengths(sequences, kv_heads, dim, quer
     assert all(torch.equal(a, b) for a, b in zip(first, run(s, max_keys=40000)))
 
 
+@pytest.mark.parametrize("how", [dict(), dict(causal=True), dict(distance_bias=20), dict(slopes=True), dict(window=(-1, 60))])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_sequences_of_several_tiles(how, dim):
+    lengths = [[300, 0, 1, 129, 260, 64, 128, 5][b % 8] for b in range(80)]
+    check(problem(38, lengths, heads=4, kv_heads=2, dim=dim, **with_bias(how, 4)))
+
+
 @pytest.mark.parametrize("cap", [2e3, 1e4, 1e6, 1e9, 1e30])
 @pytest.mark.parametrize("queries,keys", [([300], None), ([1, 3], [900, 200])])
 @pytest.mark.parametrize("slopes", [False, True])
