@@ -130,7 +130,7 @@ __device__ void attend_row(const AttendArgs& a, const AttendSequence& s, int ful
 //
 // Tiles: with heads past 64 two to a CTA and one CTA per SM (one tile, two CTAs: 16384 causal 976 -> 999 us, with a cap 1441 -> 1482, 8192 tokens
 // in documents 207 -> 229: K and V are loaded twice, into one buffer each).  Heads up to 64: one to a CTA and two CTAs per SM, whose starts and ends overlap
-// (two tiles: 16384 causal 854 -> 915 us, 64 x 1024 444 -> 461, 1 x 1000 27 -> 32; with a distance bias 64 ragged sequences up to 1024 402 -> 369, but
+// (two tiles, before a sequence's tiles ran one after the other: 16384 causal 854 -> 915 us, 64 x 1024 444 -> 461, 1 x 1000 27 -> 32; with a distance bias 64 ragged sequences up to 1024 402 -> 369, but
 // 64 x 250 74 -> 82 and 40 causal ones up to 500 63 -> 73).
 //
 // Where one tile holds all rows, both take them, and each every other step; the parts are joined at the end as those of a split
