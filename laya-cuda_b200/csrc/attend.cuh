@@ -876,9 +876,10 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           ++used[t];
         };
         int cur = read(0);
+        // Also where no step follows: the softmax warps, which wait for `drain` alone, then write their rows over Q.
+        for (int t = 0; t < NT; ++t)
+          if (tokens[t]) wait(q_full + t, 0);
         if (cur != kAtEnd) {
-          for (int t = 0; t < NT; ++t)
-            if (tokens[t]) wait(q_full + t, 0);
           wait(k_full, 0);
           for (int t = 0; t < NT; ++t)
             if (takes(cur, t)) scores(0, t);

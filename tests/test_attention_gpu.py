@@ -706,6 +706,50 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable():
         check(s)
 
 
+# -------------------------------------------------------------------------------- attention: tiles that no key is visible to
+
+def some_sequences(s, which):
+    return {**s, **{n: [s[n][b] for b in which] for n in ("starts", "lengths", "k_starts", "k_lengths")}}
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", ["no keys", "before the first key", "a document without keys", "single tokens", "shares without keys"])
+def test_thousands_of_tiles_without_a_visible_key(form, dim):
+    """Their queries come from memory, not from the L2 cache, and are of no use to any product."""
+    heads, how = 4, {}
+    if form == "no keys":
+        queries, keys = [130] * 1200, [200 if b % 50 == 7 else 0 for b in range(1200)]
+    elif form == "before the first key":
+        queries, keys, how = [400] * 400, [20] * 400, {"causal": True}
+    elif form == "a document without keys":
+        queries, keys = [130] * 1200, [64] * 1200
+        other = torch.tensor([b % 50 != 7 for b in range(1200)], device="cuda").int()
+        how = {"documents": other.repeat_interleave(130), "k_documents": torch.zeros(1200 * 64, dtype=torch.int32, device="cuda")}
+    elif form == "single tokens":
+        queries, keys, heads = [1] * 6000, [200 if b % 500 == 7 else 0 for b in range(6000)], 32
+    else:  # a cluster's CTAs past the last key of a short cache
+        queries, keys, heads = [1] * 4, [130, 0, 5000, 1], 16
+    s = problem(60, queries, keys, heads=heads, kv_heads=2, dim=dim, **how)
+    some = [b for b, m in enumerate(keys) if m and (len(keys) < 10 or b % 50 == 7)]
+    part = some_sequences(s, some)
+    want, want_lse, slack, lse_slack = define(part)
+    mine = ~want_lse.isnan()
+    nothing = torch.ones(len(s["q"]), dtype=torch.bool, device="cuda")
+    for b, (start, n) in enumerate(zip(s["starts"], queries)):
+        if form == "before the first key":
+            nothing[start + n - 20: start + n] = False
+        elif keys[b] and (form != "a document without keys" or b % 50 == 7):
+            nothing[start: start + n] = False
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    for i in range(4):
+        flush.fill_(i)
+        out, lse = run(s, **({"max_keys": 40000} if form == "shares without keys" else {}))
+        assert not out[nothing].any() and bool((lse[nothing] == -math.inf).all())
+        assert ((out.double() - want).abs() <= slack)[mine].all()
+        empty = want_lse == -math.inf
+        assert ((lse.double() - want_lse).abs() <= lse_slack)[mine & ~empty].all()
+
+
 # -------------------------------------------------------------------------------- a layer
 
 def layer_example():
