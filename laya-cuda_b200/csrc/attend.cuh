@@ -825,13 +825,11 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         if (lane == 0 && ok) { info[e] = kAtEnd; mbar_arrive(info_full + e); }
       }
       __syncwarp();
-      if (*abort_flag) {
-        // Copies that nothing waits for any more land before the CTA ends.
-        for (int t = 0; t < NT; ++t)
-          if (tokens[t]) mbar_drain(q_full + t, 0);
-        for (int i = max(0, k_issued - kSlots); i < k_issued; ++i) mbar_drain(k_full + i % kSlots, (i / kSlots) & 1);
-        for (int i = max(0, v_issued - kSlots); i < v_issued; ++i) mbar_drain(v_full + i % kSlots, (i / kSlots) & 1);
-      }
+      // Every copy has landed before this warp ends, and the CTA with it: all have been used by then, unless a role gave up, be it after this point.
+      for (int t = 0; t < NT; ++t)
+        if (tokens[t]) mbar_drain(q_full + t, 0);
+      for (int i = max(0, k_issued - kSlots); i < k_issued; ++i) mbar_drain(k_full + i % kSlots, (i / kSlots) & 1);
+      for (int i = max(0, v_issued - kSlots); i < v_issued; ++i) mbar_drain(v_full + i % kSlots, (i / kSlots) & 1);
     } else if (warp == Cfg::kMmaWarp) {
       // ---- tensor products, by one thread
       if (elect_one()) {

@@ -706,6 +706,31 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable():
         check(s)
 
 
+@pytest.mark.parametrize("queries,keys,dim", [([700, 300], None, 64), ([700, 300], None, 128), ([1] * 40, [3000] * 40, 128), ([20, 1], [9000, 0], 64)])
+def test_waits_that_run_out_early_and_late(queries, keys, dim):
+    """Limits under which some waits run out and others do not: a call that reports nothing is right, and calls after it are."""
+    from laya_cuda import _lib
+    lib = _lib.load()
+    s = problem(61, queries, keys, heads=8, kv_heads=2, dim=dim, causal=True)
+    want, _ = check(s)
+    k = {} if keys is None else {"k_starts": ints(s["k_starts"]), "k_lengths": ints(s["k_lengths"])}
+    starts, lengths, out = ints(s["starts"]), ints(s["lengths"]), torch.empty_like(want)
+    reported = set()
+    for limit in (1, 200, 700, 2000, 5000, 15000):
+        _lib.check(lib.laya_set_launch_options(1, limit))
+        try:
+            for _ in range(5):
+                err = torch.zeros(1, dtype=torch.int32, device="cuda")
+                out.fill_(7.0)
+                attention.attend(s["q"], s["k"], s["v"], out, starts, lengths, max_queries=max(queries), max_keys=max(keys or queries), causal=True, err=err, **k)
+                reported.add(err.item())
+                assert err.item() == 5 or torch.equal(out, want)
+        finally:
+            _lib.check(lib.laya_set_launch_options(1, 0))
+        check(s)
+    assert 5 in reported and reported <= {0, 5}
+
+
 # -------------------------------------------------------------------------------- attention: tiles that no key is visible to
 
 def some_sequences(s, which):
