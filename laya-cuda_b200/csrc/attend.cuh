@@ -961,8 +961,8 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
-          // A part that saw nothing has no weight, and its O holds anything.
-          w[k] = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : ex2_approx(kNatural ? (ml[k].x - top) * kLog2e : ml[k].x - top);
+          // A part that saw nothing has no weight (-1 here), and its O holds anything.  A weight of 0 counts: its part may hold a NaN.
+          w[k] = ml[k].x == -INFINITY && ml[k].y == 0.f ? -1.f : ex2_approx(kNatural ? (ml[k].x - top) * kLog2e : ml[k].x - top);
           sum = fmaf(ml[k].y, w[k], sum);
         }
 #pragma unroll
@@ -971,7 +971,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         const float inv = any ? 1.f / sum : 0.f;
 #pragma unroll
         for (int k = 0; k < kEach; ++k)
-          if (lane + 32 * k < parts) weights[(lane + 32 * k) * share + i] = w[k] * inv;
+          if (lane + 32 * k < parts) weights[(lane + 32 * k) * share + i] = w[k] < 0.f ? -1.f : w[k] * inv;
         if (lane == 0) {
           fine[i] = sum - sum == 0.f;
           if (a.lse) {
@@ -992,7 +992,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           const float w = weights[c * share + at_row];
           const int slot = slot_of(r, c);
           const float4 x = ld_cluster_v4(cluster_addr(part_addr + (slot * DP + (dv ^ (slot & 7)) * 4) * 4, rank_of(c)));
-          if (w != 0.f) { o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w); }
+          if (!(w < 0.f)) { o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w); }
         }
         if (!(o.x - o.x == 0.f && o.y - o.y == 0.f && o.z - o.z == 0.f && o.w - o.w == 0.f)) fine[at_row] = 0;
         int qi, h;

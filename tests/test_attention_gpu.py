@@ -775,6 +775,29 @@ def test_thousands_of_tiles_without_a_visible_key(form, dim):
         assert ((lse.double() - want_lse).abs() <= lse_slack)[mine & ~empty].all()
 
 
+# -------------------------------------------------------------------------------- attention: values that are not finite
+
+def same_kinds(got, want):
+    """NaN for NaN, infinities for infinities of their sign."""
+    return torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isposinf(), want.isposinf()) and torch.equal(got.isneginf(), want.isneginf())
+
+
+@pytest.mark.parametrize("queries,keys,heads", [([1], [9000], 4), ([2, 1], [9000, 700], 8), ([24], [9000], 4), ([300], [3000], 4), ([300], [400], 4)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_visible_nan_counts_however_small_its_weight(queries, keys, heads, dim):
+    """Weights below the smallest number of 32 bits, in a part of the keys that has no other."""
+    s = problem(62, queries, keys, heads=heads, kv_heads=2, dim=dim)
+    s["q"].fill_(1.0)
+    s["k"].fill_(-120 / dim ** 0.5)
+    for start in s["k_starts"]:
+        s["k"][start: start + 100] = 120 / dim ** 0.5
+    assert math.exp(-240) > 0 and 2 ** -149 > math.exp(-240)
+    at = s["k_starts"][0] + keys[0] - 50
+    s["v"][at, 1, 3] = math.nan
+    out, _ = check(s)
+    assert bool(out[: queries[0], heads // 2:, 3].isnan().all())
+
+
 # -------------------------------------------------------------------------------- a layer
 
 def layer_example():
