@@ -447,7 +447,7 @@ typedef struct laya_attend {
  *   out = sum softmax(s)_j v_j over the visible keys j, zeros where there are none (or all have s = -infinity)
  * Key j is visible where j < prefix, or where documents[query] == k_documents[key], causal implies j <= p, and
  * p - window_left <= j <= p + window_right.  Keys that are not visible may hold anything, rows outside the sequences
- * too; rows of out that belong to no sequence are left as they were.  out must not overlap q, k or v.  Scores and sums are held in 32 bits, softmax's
+ * too; a NaN or infinity in a visible key's v is one in that channel of the rows that see it, however small its weight; rows of out that belong to no sequence are left as they were.  out must not overlap q, k or v.  Scores and sums are held in 32 bits, softmax's
  * numerators are rounded to dtype before they meet v.  The same call gives the same result each time.
  * err (zero on entry, or NULL) receives a device error: 4 for a sequence outside the tensors' rows, which is
  * skipped, or a pipeline wait that ran out, after which out is undefined. */

@@ -1,6 +1,7 @@
 // Attention over packed sequences with caps, biases by distance and masks (see laya_op_attend in
 // include/laya_b200.h for the definition).
 #pragma once
+#include <float.h>
 #include <limits.h>
 
 #include <type_traits>
@@ -10,6 +11,8 @@
 namespace laya {
 
 constexpr int kAttendMostDim = 128;
+constexpr int kAtRows = 128;       // rows of a tile
+constexpr int kAtKeys = 128;       // keys of a step
 
 struct AttendArgs {
   const void *q, *k, *v;
@@ -52,64 +55,128 @@ __device__ __forceinline__ AttendSequence attend_sequence(const AttendArgs& a, i
   return s;
 }
 
-// One query of one head by one warp, in fp32 from global memory: a lane per key for the scores, a lane per value for the sum.
+// The n lowest bits.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
+// What a row sees of the keys, besides the documents: [lo, hi] and all below prefix.
+struct AttendSpan {
+  int lo, hi;
+};
+__device__ __forceinline__ AttendSpan attend_span(const AttendArgs& a, int p, int keys) {
+  AttendSpan s{0, keys - 1};
+  if (a.left >= 0) s.lo = (int)min((int64_t)INT_MAX - 1, max((int64_t)0, (int64_t)p - a.left));
+  if (a.causal) s.hi = min(s.hi, p);
+  if (a.right >= 0) s.hi = (int)min((int64_t)s.hi, (int64_t)p + a.right);
+  return s;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Values that are not finite.
+//
+// A hidden key's score becomes -infinity whatever it was, but its weight of zero times an infinity or NaN of v would be a NaN.  So where a step holds hidden keys, two
+// warps look its V over while the softmax is at work, put zeros in the place of what is not finite, and note the step.  What that took from rows that see such a key is put into their
+// results at the end: attend_scan finds it, reading v of the noted steps once for all rows of a warp, attend_put writes it.  (Steps that all rows see are left as they are.)
+// 4096 causal tokens, 4 heads of 128 over 2: 59 us; with a NaN in every key's v 88, with 100 NaN here and there 78 (50 ms when each row with a NaN was computed again by a warp).
+// What it costs without any: windowed documents 161 -> 168 us, a packed batch 347 -> 357, single tokens and long prompts nothing.
+// ---------------------------------------------------------------------------------------------
+
+// Pairs of 16-bit values.
 template <typename T>
-__device__ void attend_row(const AttendArgs& a, const AttendSequence& s, int full_queries, int query, int head) {
-  const int lane = threadIdx.x & 31;
-  const int token = s.q_start + query, p = query + s.keys - full_queries;
-  const T* q = static_cast<const T*>(a.q) + token * a.q_token + head * a.q_head;
-  const T* k = static_cast<const T*>(a.k) + s.k_start * a.k_token + head / a.group * a.k_head;
-  const T* v = static_cast<const T*>(a.v) + s.k_start * a.v_token + head / a.group * a.v_head;
-  const int doc = a.documents ? a.documents[token] : 0;
-  float m = -INFINITY, l = 0.f, o[kAttendMostDim / 32] = {};
-  for (int base = 0; base < s.keys; base += 32) {
-    const int j = base + lane;
-    bool see = j < s.keys;
-    if (see && j >= s.prefix)
-      see = (!a.causal || j <= p) && (a.left < 0 || j >= (int64_t)p - a.left) && (a.right < 0 || j <= (int64_t)p + a.right) &&
-            (!a.documents || a.k_documents[s.k_start + j] == doc);
-    if (!__any_sync(0xffffffffu, see)) continue;
-    float x = -INFINITY;
-    if (see) {
-      float dot = 0.f;
-      for (int d = 0; d < a.dim; ++d) dot = fmaf(to_f32(q[d]), to_f32(k[j * a.k_token + d]), dot);
-      x = dot * a.scale;
-      if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
-      if (a.slopes) x -= a.slopes[head] * fabsf((float)(p - j));
-      if (a.table) x += a.table[(int64_t)head * (2 * a.reach + 1) + min(max(j - p, -a.reach), a.reach) + a.reach];
-    }
-    float top = x;
-    bool nan = x != x;
-#pragma unroll
-    for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    if (__any_sync(0xffffffffu, nan)) top = NAN;
-    const float next = top != top || m != m ? NAN : fmaxf(m, top);
-    if (next == -INFINITY) continue;
-    const float alpha = m == -INFINITY ? 0.f : __expf(m - next);
-    float e = see && x != -INFINITY ? expf(x - next) : 0.f;
-    m = next;
-    float sum = e;
-#pragma unroll
-    for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-    l = l * alpha + sum;
-#pragma unroll
-    for (int i = 0; i < kAttendMostDim / 32; ++i) o[i] *= alpha;
-    const uint32_t who = __ballot_sync(0xffffffffu, see && x != -INFINITY);
-    for (uint32_t left = who; left; left &= left - 1) {
-      const int src = __ffs(left) - 1;
-      const float w = __shfl_sync(0xffffffffu, e, src);
-      const T* row = v + (base + src) * a.v_token;
-#pragma unroll
-      for (int i = 0; i < kAttendMostDim / 32; ++i)
-        if (lane + 32 * i < a.dim) o[i] = fmaf(w, to_f32(row[lane + 32 * i]), o[i]);
+struct NotFinite {
+  static constexpr uint32_t kTop = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;  // an infinity; NaN are above it
+  static constexpr uint32_t kBits = kTop << 16 | kTop, kAdd = 0x80008000u - kBits;
+  // Bits 15 and 31: which of the two are not finite (an addition to the exponent's bits carries there when all are set).
+  static __device__ __forceinline__ uint32_t carries(uint32_t pair) { return (pair & kBits) + kAdd; }
+  // sum + 0 pair: not finite any more once a value was not.
+  static __device__ __forceinline__ uint32_t gather(uint32_t pair, uint32_t sum) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162 r = __hfma2(reinterpret_cast<const __nv_bfloat162&>(pair), __nv_bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0)), reinterpret_cast<const __nv_bfloat162&>(sum));
+      return reinterpret_cast<const uint32_t&>(r);
+    } else {
+      const __half2 r = __hfma2(reinterpret_cast<const __half2&>(pair), __half2(__ushort_as_half(0), __ushort_as_half(0)), reinterpret_cast<const __half2&>(sum));
+      return reinterpret_cast<const uint32_t&>(r);
     }
   }
-  T* out = static_cast<T*>(a.out) + token * a.out_token + head * a.out_head;
-  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+  static __device__ __forceinline__ uint32_t cleared(uint32_t pair) {
+    const uint32_t c = carries(pair);
+    return pair & ~((c >> 15 & 1) * 0xffffu | (c >> 31) * 0xffff0000u);
+  }
+};
+
+// Channels that are NaN, infinity and -infinity for a key that a row sees: bit i of word c is channel 8 (i % 16) + c + 4 (i / 16).
+struct AttendFound {
+  uint32_t nan[4] = {}, up[4] = {}, down[4] = {};
+  __device__ __forceinline__ bool any() const {
+    uint32_t all = 0;
 #pragma unroll
-  for (int i = 0; i < kAttendMostDim / 32; ++i)
-    if (lane + 32 * i < a.dim) out[lane + 32 * i] = from_f32<T>(o[i] * inv);
-  if (a.lse && lane == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : m + logf(l);
+    for (int c = 0; c < 4; ++c) all |= nan[c] | up[c] | down[c];
+    return all != 0;
+  }
+};
+
+// What the rows of a warp (a lane per row; those that ask) see that is not finite, among the keys 32 first .. 32 last + 31, every `stride`-th 32 of them.
+template <typename T>
+__device__ void attend_scan(const AttendArgs& a, AttendSequence s, int full_queries, int query, int kv, bool asks, int first, int last, int stride, AttendFound& found) {
+  using F = NotFinite<T>;
+  const int lane = threadIdx.x & 31;
+  const AttendSpan span = attend_span(a, query + s.keys - full_queries, s.keys);
+  const int below = max(0, min(s.prefix, s.keys)), doc = asks && a.documents ? a.documents[s.q_start + query] : 0;
+  // Half a warp reads a key's channels.
+  const int odd = lane >> 4, channel = 8 * (lane & 15);
+  const T* v = static_cast<const T*>(a.v) + s.k_start * a.v_token + kv * a.v_head + channel;
+  for (int block = first; block <= last; block += stride) {
+    const int kc = 32 * block;
+    uint32_t seen = low_bits(span.hi + 1 - kc) & ~low_bits(span.lo - kc);
+    if (a.documents) {
+      const int theirs = kc + lane < s.keys ? a.k_documents[s.k_start + kc + lane] : 0;
+      uint32_t same = 0;
+      for (int i = 0; i < 32; ++i) same |= (uint32_t)(__shfl_sync(0xffffffffu, theirs, i) == doc) << i;
+      seen &= same;
+    }
+    seen = asks ? (seen | low_bits(below - kc)) & low_bits(s.keys - kc) : 0;
+    const uint32_t some = __reduce_or_sync(0xffffffffu, seen);
+    for (int i = 0; i < 32; i += 8) {
+      if (!(some >> i & 0xff)) continue;
+      uint4 w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int key = i + 2 * u + odd;
+        w[u] = channel < a.dim && (some >> key & 1) ? *reinterpret_cast<const uint4*>(v + (kc + key) * a.v_token) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t words[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+        if (!__any_sync(0xffffffffu, ((F::carries(words[0]) | F::carries(words[1]) | F::carries(words[2]) | F::carries(words[3])) & 0x80008000u) != 0)) continue;
+        const uint32_t sees = seen >> (i + 2 * u) & 3;  // the two keys, for this lane's row
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          // Values c and c + 4 of the lanes' eight.
+          const uint32_t x = words[c >> 1] >> 16 * (c & 1) & 0xffff, y = words[2 + (c >> 1)] >> 16 * (c & 1) & 0xffff;
+          auto mark = [&](uint32_t& word, bool px, bool py) {
+            const uint32_t bx = __ballot_sync(0xffffffffu, px), by = __ballot_sync(0xffffffffu, py);
+            if (sees & 1) word |= (bx & 0xffff) | by << 16;
+            if (sees & 2) word |= bx >> 16 | (by & 0xffff0000);
+          };
+          mark(found.nan[c], (x & 0x7fff) > F::kTop, (y & 0x7fff) > F::kTop);
+          mark(found.up[c], x == F::kTop, y == F::kTop);
+          mark(found.down[c], x == (F::kTop | 0x8000), y == (F::kTop | 0x8000));
+        }
+      }
+    }
+  }
+}
+
+// Puts what a row sees that is not finite into its result, by a warp: added to it, or, where all that it sees is known, in its place.
+template <typename T>
+__device__ void attend_put(const AttendArgs& a, int token, int head, const AttendFound& found, bool all) {
+  const int lane = threadIdx.x & 31, bit = (lane >> 1) + 16 * (lane & 1);  // channels 4 lane .. 4 lane + 3
+  if (4 * lane >= a.dim) return;
+  T* out = static_cast<T*>(a.out) + token * a.out_token + head * a.out_head + 4 * lane;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const bool up = found.up[c] >> bit & 1, down = found.down[c] >> bit & 1, nan = (found.nan[c] >> bit & 1) || (up && down);
+    if (nan || up || down) out[c] = from_f32<T>((all ? 0.f : to_f32(out[c])) + (nan ? NAN : up ? INFINITY : -INFINITY));
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -118,7 +185,7 @@ __device__ void attend_row(const AttendArgs& a, const AttendSequence& s, int ful
 //
 // A CTA takes tiles of 128 rows, a row being one query of one head of a kv head's group (so that the group reads its keys once), and walks the
 // keys in steps of 128.  Warps 0-3 are the softmax of tile 0, warps 4-7 of tile 1 (a thread per row, warp w owning TMEM lanes 32 (w % 4) on); of the
-// others one issues the tensor products, and one finds the steps that the masks leave and loads them by TMA.  TMEM: S of each tile (128 columns),
+// others one issues the tensor products, one finds the steps that the masks leave and loads them by TMA, and two look over V where a mask cuts a step.  TMEM: S of each tile (128 columns),
 // O of each; P goes over S as 16-bit pairs.  The tensor core runs the products in issue order, so O += P V of a step and then S = Q K^T
 // of the next are issued together as soon as P is there, and the other tile's softmax hides them.
 //
@@ -137,13 +204,15 @@ __device__ void attend_row(const AttendArgs& a, const AttendSequence& s, int ful
 // are.  Where a quarter of a tile holds them (single tokens over a cache), each quarter has a copy of them and takes a quarter of
 // a step's keys: a softmax thread then has 32 scores of a step to do and not 128.
 // ---------------------------------------------------------------------------------------------
-constexpr int kAtRows = 128;       // rows of a tile
-constexpr int kAtKeys = 128;       // keys of a step
 constexpr int kAtInfo = 4;         // steps announced ahead
 constexpr float kAtRescale = 8.f;  // O is rescaled when a row's maximum has grown by more than 2^8
-enum AtClass : int { kAtEnd = -1, kAtSkip = 0, kAtMasked = 1, kAtFull = 2 };
+// kAtTail: all rows see all of its keys, which are fewer than a step's.
+enum AtClass : int { kAtEnd = -1, kAtSkip = 0, kAtMasked = 1, kAtFull = 2, kAtTail = 3 };
 // What is done to the scores: nothing, a cap, slopes (these in log2 units, a scale above zero), a distance bias in shared memory, or all else
 // (these in natural units: log2e times the lowest number of a type would be -infinity; all else has a slower way only).
+// Of a step as it is announced, with the classes of tile 0 and, two bits up, of tile 1: whether one is kAtMasked or kAtTail (the odd ones); whether one is kAtMasked.
+__device__ __forceinline__ bool attend_cut(int x) { return (x & 5) != 0; }
+__device__ __forceinline__ bool attend_hides(int x) { return (x & 3) == kAtMasked || (x >> 2 & 3) == kAtMasked; }
 enum AtMode { kAtPlain, kAtCap, kAtSlopes, kAtTable, kAtGeneral };
 
 constexpr int kAtMostSplits = 16;
@@ -156,7 +225,7 @@ template <int DP, int NT>
 struct AttendCfg {
   static_assert((DP == 64 || DP == 128) && (NT == 1 || NT == 2), "padded head size, tiles");
   static constexpr int kSoftmax = 4 * NT;                // softmax warps
-  static constexpr int kMmaWarp = kSoftmax, kLoadWarp = kSoftmax + 1, kThreads = 32 * (kSoftmax + 4), kCtas = NT == 1 ? 2 : 1;
+  static constexpr int kMmaWarp = kSoftmax, kLoadWarp = kSoftmax + 1, kCheckWarp = kSoftmax + 2, kThreads = 32 * (kSoftmax + 4), kCtas = NT == 1 ? 2 : 1;
   // Registers: what the launch gives all threads (128 with one tile, 168 with two), moved to the softmax, whose threads hold a step's 128 scores.
   // (224 and 56 with two tiles: a cap 3% faster, slopes and windows slower.)
   static constexpr int kSoftmaxRegs = NT == 1 ? 200 : 216, kOtherRegs = NT == 1 ? 56 : 72;
@@ -169,9 +238,9 @@ struct AttendCfg {
   static constexpr int kOffQ = 0, kOffK = NT * kQTile, kOffV = kOffK + kSlots * kTile;
   static constexpr int kOffDocs = kOffV + kSlots * kTile;
   static constexpr int kOffBar = kOffDocs + kAtInfo * kAtKeys * 4;
-  static constexpr int kBars = 2 + 4 * kSlots + 2 * kAtInfo + 8;
+  static constexpr int kBars = 2 + 4 * kSlots + 2 * kAtInfo + 10;
   static constexpr int kOffInfo = kOffBar + kBars * 8;
-  static constexpr int kOffSums = kOffInfo + kAtInfo * 4 + 16;  // (maximum, sum) of each row, where results are joined
+  static constexpr int kOffSums = kOffInfo + kAtInfo * 4 + 24;  // (maximum, sum) of each row, where results are joined
   static constexpr int kWeights = 2 * NT * kAtRows + 8 * kAtMostSplits;  // of the parts of the rows that a CTA joins
   static constexpr int kOffWeights = kOffSums + NT * kAtRows * 8;
   static constexpr int kOffTable = kOffWeights + kWeights * 4;
@@ -214,24 +283,9 @@ __device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
   return v;
 }
 
-// The n lowest bits.
-__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
-
 struct AttendMaps {
   CUtensorMap q, k, v;
 };
-
-// What a row sees of the keys, besides the documents: [lo, hi] and all below prefix.
-struct AttendSpan {
-  int lo, hi;
-};
-__device__ __forceinline__ AttendSpan attend_span(const AttendArgs& a, int p, int keys) {
-  AttendSpan s{0, keys - 1};
-  if (a.left >= 0) s.lo = (int)min((int64_t)INT_MAX - 1, max((int64_t)0, (int64_t)p - a.left));
-  if (a.causal) s.hi = min(s.hi, p);
-  if (a.right >= 0) s.hi = (int)min((int64_t)s.hi, (int64_t)p + a.right);
-  return s;
-}
 
 // out tanh(in s) for a raw product s, with out in some unit.
 //   near  for |in s| <= 0.8 (less with large caps): s times a polynomial in s^2 by the Remez exchange algorithm, on the FMA pipe; off by 1.2e-7 of itself (a term
@@ -239,9 +293,10 @@ __device__ __forceinline__ AttendSpan attend_span(const AttendArgs& a, int p, in
 //   any   out - 2 out / (exp(2 in s) + 1) on the special-function unit; off by 2^-21 out
 struct CapTerms {
   float in, out, c[6], most;  // most: the largest |s| for `near`
-  __device__ __forceinline__ CapTerms(float in_, float out_) : in(in_), out(out_) {
+  // scale: in out, which has all its bits where `in` is below fp32's normal numbers.
+  __device__ __forceinline__ CapTerms(float in_, float out_, float scale) : in(in_), out(out_) {
     constexpr float kC[6] = {0.99999994f, -0.333326757f, 0.13321048f, -0.0531143174f, 0.0190933011f, -0.00435529975f};
-    float power = out * in;
+    float power = scale;
 #pragma unroll
     for (int i = 0; i < 6; ++i) { c[i] = kC[i] * power; power *= in * in; }
     // Caps far above the scale (300 and more for 0.09) take the last factors below fp32's range: as far as the terms that are left reach.
@@ -279,10 +334,12 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
   uint64_t *q_full = bar, *k_full = bar + 2, *k_empty = k_full + kSlots, *v_full = k_empty + kSlots, *v_empty = v_full + kSlots,
-           *info_full = v_empty + kSlots, *info_empty = info_full + kAtInfo, *s_full = info_empty + kAtInfo, *p_full = s_full + 2, *drain = p_full + 2, *table_full = drain + 2, *summary_full = table_full + 1;
+           *info_full = v_empty + kSlots, *info_empty = info_full + kAtInfo, *s_full = info_empty + kAtInfo, *p_full = s_full + 2, *drain = p_full + 2, *table_full = drain + 2, *summary_full = table_full + 1, *v_ask = summary_full + 1, *v_clean = v_ask + 1;
   volatile int* info = reinterpret_cast<volatile int*>(smem + Cfg::kOffInfo);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffInfo + kAtInfo * 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* ask = reinterpret_cast<volatile int*>(tmem_slot + 4);  // a step whose V is to be looked over: its number among the CTA's, and of all (-1: no more)
+  int* noted = reinterpret_cast<int*>(tmem_slot + 2);  // first and last step whose V held what is not finite
   int* docs = reinterpret_cast<int*>(smem + Cfg::kOffDocs);
   float2* sums = reinterpret_cast<float2*>(smem + Cfg::kOffSums);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -291,9 +348,13 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
   if (warp == 0) {
     for (int i = lane; i < Cfg::kBars; i += 32) {
       const uint64_t* of = bar + i;
-      mbar_init(bar + i, of >= info_empty && of < s_full ? Cfg::kSoftmax + 1 : of >= p_full && of < drain ? 4 : of >= table_full ? Cfg::kSoftmax : 1);
+      mbar_init(bar + i, of == v_clean ? 2 : of == v_ask ? 1 : of >= table_full ? Cfg::kSoftmax : of >= drain ? 3 : of >= p_full ? 4 : of >= info_empty && of < s_full ? Cfg::kSoftmax + 1 : 1);
     }
-    if (lane == 0) *abort_flag = 0;
+    if (lane == 0) {
+      *abort_flag = 0;
+      noted[0] = INT_MAX;
+      noted[1] = -1;
+    }
     fence_mbar_init();
   }
   if (warp == Cfg::kMmaWarp) { tmem_alloc(tmem_slot, Cfg::kTmemCols); tmem_relinquish(); }
@@ -386,8 +447,11 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     if (!live) span = {0, -1};
     const int below = live ? prefix : 0;
     const int doc = live && a.documents ? a.documents[s.q_start + query] : 0;
-    const float scale = a.scale * kUnit;
-    const float slope = (kMode == kAtSlopes || kGeneral) && live && a.slopes ? a.slopes[head] * kUnit : 0.f;
+    // Finite factors stay finite in log2 units.
+    auto in_units = [&](float x) { return fabsf(x) <= FLT_MAX ? fminf(fmaxf(x * kUnit, -FLT_MAX), FLT_MAX) : x; };
+    const float scale = in_units(a.scale);
+    const float slope = (kMode == kAtSlopes || kGeneral) && live && a.slopes ? in_units(a.slopes[head]) : 0.f;
+    const bool tame = fabsf(slope) < 1e28f;  // its products with distances are finite
     const float* table = kGeneral && a.table ? a.table + (int64_t)(live ? head : 0) * (2 * a.reach + 1) + a.reach : nullptr;
     // The distance bias of the group's heads in shared memory, with the edges' values as far past the reach as a tile and a step make.
     const int wide = 2 * (a.reach + kAtKeys + kAtRows) + a.table_pad;
@@ -405,7 +469,9 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       if (lane == 0) mbar_arrive(table_full);
     }
     const bool capped = kMode == kAtCap || (kGeneral && a.cap > 0.f);
-    const CapTerms cap(capped ? a.scale / a.cap : 0.f, a.cap * kUnit);
+    // Caps near the ends of fp32's range stay finite: past 1e37 a cap's quotient is a step, and past 1e38 a cap is above all scores.
+    const float most_cap = fminf(a.cap, 1e38f);
+    const CapTerms cap(capped ? fminf(fmaxf(a.scale / most_cap, -1e37f), 1e37f) : 0.f, most_cap * kUnit, scale);
     if (summed) {
       for (int i0 = warp; i0 < end - at; i0 += 4 * Cfg::kSoftmax) {
         int d[4][4];
@@ -446,7 +512,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       // `whole`: all rows of the warp see all of its keys; otherwise `bits` says for each chunk of 32 what this row sees.
       uint32_t bits[NC];
       bool whole = true;
-      if (cls == kAtMasked && warp_live) {
+      if (cls != kAtFull && warp_live) {
         const int mixed = x >> 4 & 15;  // chunks with keys of several documents
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -476,18 +542,6 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_fence_after();
       ++count;
-      // Rows of V past the last key may hold anything: a NaN there, times a weight of zero, would be a NaN.  (Both tiles write the same.)
-      const int rows = s.keys - kb;
-      if (rows < kAtKeys) {
-        const int slot = n % kSlots;
-        ok = mbar_wait(v_full + slot, (n / kSlots) & 1, a.err, kErrAttnWait, abort_flag, wait_ns);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        for (int h = 0; h < halves; ++h) {
-          uint4* tail = reinterpret_cast<uint4*>(smem + Cfg::kOffV + slot * Cfg::kTile + h * Cfg::kHalf + rows * 128);
-          for (int i = row; i < (kAtKeys - rows) * 8; i += kAtRows) tail[i] = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-      }
       if (!warp_live) {
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + t);
@@ -549,7 +603,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         } else if (kMode == kAtSlopes) {
           // All keys on one side of the query.
           const bool left = d + kMine - 1 <= 0;
-          if (__all_sync(0xffffffffu, left || d >= 0)) {
+          if (__all_sync(0xffffffffu, tame && (left || d >= 0))) {
             const float g = left ? slope : -slope, at_d = fmaf(g, fd, kShift - base);
             const float2 from = make_float2(at_d, at_d), each = make_float2(g, g);
             most = numerators([&](float2 y, int i) { return fma2(y, by, fma2(each, make_float2((float)i, (float)(i + 1)), from)); });
@@ -663,7 +717,6 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       const int64_t token = s.q_start + query;
       const bool any = l > 0.f || l != l;
       const float inv = any ? 1.f / l : 0.f;
-      float poison = l - l;  // becomes a NaN with a value that is not finite
       // Through the tile's Q in shared memory, which no product reads any more: 8 lanes then write 128 bytes of a row.
       uint8_t* stage = smem + Cfg::kOffQ + t * Cfg::kQTile;
 #pragma unroll 1
@@ -677,7 +730,6 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const float x = any ? __uint_as_float(o[i + 2 * k]) * inv : 0.f, y = any ? __uint_as_float(o[i + 2 * k + 1]) * inv : 0.f;
-            if (c + i < a.dim) poison = fmaf(x, 0.f, fmaf(y, 0.f, poison));
             w[k] = pack2<T>(x, y);
           }
           const int at_c = c + i;  // 16 bytes: value at_c of the row
@@ -699,11 +751,20 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       __syncwarp();
       if (live && a.lse)
         a.lse[token * a.heads + head] = any ? (kNatural ? m : m / kLog2e) + (log2f(l) - kShift) / kLog2e : -INFINITY;
-      // A value that is not finite may come from a key that this row's mask hides (its weight of zero times that value): such rows
-      // are computed once more, from the visible keys alone.
-      for (uint32_t again = __ballot_sync(0xffffffffu, live && poison != 0.f); again; again &= again - 1) {
-        const int src = __ffs(again) - 1;
-        attend_row<T>(a, s, all_queries, __shfl_sync(0xffffffffu, query, src), __shfl_sync(0xffffffffu, head, src));
+      if (noted[1] >= 0) {
+        AttendFound found;
+        attend_scan<T>(a, s, all_queries, query, kv, live && l > 0.f, 4 * noted[0], min(4 * noted[1] + 3, (s.keys - 1) >> 5), 1, found);
+        for (uint32_t rest = __ballot_sync(0xffffffffu, found.any()); rest; rest &= rest - 1) {
+          const int src = __ffs(rest) - 1;
+          AttendFound theirs;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            theirs.nan[c] = __shfl_sync(0xffffffffu, found.nan[c], src);
+            theirs.up[c] = __shfl_sync(0xffffffffu, found.up[c], src);
+            theirs.down[c] = __shfl_sync(0xffffffffu, found.down[c], src);
+          }
+          attend_put<T>(a, s.q_start + __shfl_sync(0xffffffffu, query, src), __shfl_sync(0xffffffffu, head, src), theirs, false);
+        }
       }
     }
   } else if (!idle) {
@@ -755,9 +816,10 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         for (int t = 0; t < NT; ++t) {
           const bool in_prefix = kb < prefix, whole_prefix = kb + kAtKeys <= prefix;
           const bool meets = kb <= outer[t].hi && last >= outer[t].lo && (!a.documents || (lo <= doc_hi[t] && hi >= doc_lo[t]));
-          const bool whole = kb >= inner[t].lo && kb + kAtKeys - 1 <= inner[t].hi &&
-                             (!a.documents || (lo == hi && doc_lo[t] == doc_hi[t] && lo == doc_lo[t]));
-          both |= (!tokens[t] ? kAtSkip : whole_prefix || whole ? kAtFull : in_prefix || meets ? kAtMasked : kAtSkip) << 2 * t;
+          const bool to_last = last < prefix || (kb >= inner[t].lo && last <= inner[t].hi &&
+                                                 (!a.documents || (lo == hi && doc_lo[t] == doc_hi[t] && lo == doc_lo[t])));
+          both |= (!tokens[t] ? kAtSkip : whole_prefix || (to_last && last == kb + kAtKeys - 1) ? kAtFull : to_last ? kAtTail : in_prefix || meets ? kAtMasked : kAtSkip)
+                  << 2 * t;
         }
         return both;
       };
@@ -838,6 +900,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         const uint32_t q_addr = smem_u32(smem + Cfg::kOffQ), k_addr = smem_u32(smem + Cfg::kOffK), v_addr = smem_u32(smem + Cfg::kOffV);
         bool ok = true;
         int used[2] = {0, 0};  // products P V of each tile
+        int checked = 0;       // steps whose V was looked over
         auto wait = [&](uint64_t* which, int parity) { ok = ok && mbar_wait(which, parity, a.err, kErrAttnWait, abort_flag, wait_ns); };
         auto read = [&](int n) {
           const int e = n % kAtInfo;
@@ -884,12 +947,19 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           if (ok) tc_commit(k_empty);
         }
         for (int n = 0; ok && cur != kAtEnd; ++n) {
+          wait(v_full + n % kSlots, (n / kSlots) & 1);  // (V of a step is loaded before K of the next)
+          const bool asked = ok && attend_cut(cur);
+          if (asked) {
+            ask[0] = 2 * n + attend_hides(cur);
+            ask[1] = (int)((uint32_t)cur >> 8);
+            mbar_arrive(v_ask);
+          }
           const int next = read(n + 1), k_next = (n + 1) % kSlots;
           if (next != kAtEnd) wait(k_full + k_next, ((n + 1) / kSlots) & 1);
           // A tile that has no part in this step need not wait for it.
           for (int t = 0; t < NT; ++t)
             if (!takes(cur, t) && takes(next, t)) scores(n + 1, t);
-          wait(v_full + n % kSlots, (n / kSlots) & 1);
+          if (asked) wait(v_clean, checked++ & 1);
           for (int t = 0; t < NT; ++t)
             if (takes(cur, t)) {
               values(n, t);
@@ -901,10 +971,62 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           }
           cur = next;
         }
+        ask[1] = -1;
+        mbar_arrive(v_ask);
         for (int t = 0; t < NT; ++t) tc_commit(drain + t);
         for (int t = 0; t < NT; ++t) mbar_drain(drain + t, 0);
       }
       __syncwarp();
+    } else {
+      // ---- V of steps with hidden keys: no value that is not finite, and zeros past the last key, whose rows may hold anything.  A warp takes half of the keys.
+      using F = NotFinite<T>;
+      for (int checked = 0;; ++checked) {
+        // (Between two of them all steps that the CTA has may lie.)
+        const bool ok = mbar_wait(v_ask, checked & 1, a.err, kErrAttnWait, abort_flag, wait_ns * (unsigned long long)(max(0, end - at) + 2));
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const int n = ask[0] >> 1, step = ask[1], slot = n % kSlots, rows = s.keys - step * kAtKeys;
+        if (step < 0 || !__all_sync(0xffffffffu, mbar_wait(v_full + slot, (n / kSlots) & 1, a.err, kErrAttnWait, abort_flag, wait_ns))) break;
+        uint8_t* tile = smem + Cfg::kOffV + slot * Cfg::kTile;
+        for (int h = 0; rows < kAtKeys && h < halves; ++h)
+          for (int i = rows * 8 + threadIdx.x - 32 * Cfg::kCheckWarp; i < kAtKeys * 8; i += 64) reinterpret_cast<uint4*>(tile + h * Cfg::kHalf)[i] = make_uint4(0, 0, 0, 0);
+        bool found = false;
+        if (ask[0] & 1) {
+          const int key0 = (warp - Cfg::kCheckWarp) * 64;  // 4 keys at a time
+          uint32_t sum[4] = {};
+          for (int h = 0; h < halves; ++h) {
+            const uint4* v = reinterpret_cast<const uint4*>(tile + h * Cfg::kHalf + key0 * 128) + lane;
+#pragma unroll 8
+            for (int i = 0; i < 16; ++i) {
+              const uint4 w = key0 + 4 * i + (lane >> 3) < rows ? v[32 * i] : make_uint4(0, 0, 0, 0);
+              sum[0] = F::gather(w.x, sum[0]);
+              sum[1] = F::gather(w.y, sum[1]);
+              sum[2] = F::gather(w.z, sum[2]);
+              sum[3] = F::gather(w.w, sum[3]);
+            }
+          }
+          found = ((F::carries(sum[0]) | F::carries(sum[1]) | F::carries(sum[2]) | F::carries(sum[3])) & 0x80008000u) != 0;
+          if (found)
+            for (int h = 0; h < halves; ++h) {
+              uint4* v = reinterpret_cast<uint4*>(tile + h * Cfg::kHalf + key0 * 128) + lane;
+#pragma unroll 1
+              for (int i = 0; i < 16; ++i)
+                if (key0 + 4 * i + (lane >> 3) < rows) {
+                  const uint4 w = v[32 * i];
+                  v[32 * i] = make_uint4(F::cleared(w.x), F::cleared(w.y), F::cleared(w.z), F::cleared(w.w));
+                }
+            }
+        }
+        if (found) {
+          atomicMin(noted, step);
+          atomicMax(noted + 1, step);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_clean);
+      }
+      __syncwarp();
+      if (lane == 0)
+        for (int t = 0; t < NT; ++t) mbar_arrive(drain + t);
     }
   }
   if (joined) {
@@ -930,11 +1052,11 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
     tc_fence_before();
     if (a.splits > 1) cluster_sync();
     else __syncthreads();
-    // Each CTA joins its share of the rows: their parts' weights, then the rows.  `fine` has a word for each row, 0 where a value is not finite.
+    // Each CTA joins its share of the rows: their parts' weights, then the rows.  `sound` has a word for each row, whether its sum is finite and above zero.
     const int rows0 = tokens[0] * a.group, rows = rows0 + tokens[1] * a.group, parts = (kQuarters ? 8 : few ? 2 : 1) * a.splits;
     const int share = (rows + a.splits - 1) / a.splits, row0 = split * share, mine = max(0, min(share, rows - row0));
     float* weights = reinterpret_cast<float*>(smem + Cfg::kOffWeights);  // [parts][share]
-    volatile int* fine = docs;
+    volatile int* sound = docs;
     static_assert(kAtInfo * kAtKeys >= 2 * kAtRows, "a word per row");
     const uint32_t part_addr = smem_u32(part), sums_addr = smem_u32(sums);
     auto slot_of = [&](int r, int c) { return kQuarters ? (c & 7) * 32 + r : few ? (c & 1) * kAtRows + r : r >= rows0 ? kAtRows + r - rows0 : r; };
@@ -973,7 +1095,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         for (int k = 0; k < kEach; ++k)
           if (lane + 32 * k < parts) weights[(lane + 32 * k) * share + i] = w[k] < 0.f ? -1.f : w[k] * inv;
         if (lane == 0) {
-          fine[i] = sum - sum == 0.f;
+          sound[i] = sum > 0.f && sum - sum == 0.f;
           if (a.lse) {
             int qi, h;
             place(r, &qi, &h);
@@ -982,6 +1104,9 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         }
       }
     __syncthreads();
+    // The steps that the CTAs of the cluster have noted.
+    auto noted_by = [&](int rank) { return ld_cluster_v2(cluster_addr(smem_u32(noted), rank)); };
+    bool odd = a.splits == 1 ? noted[1] >= 0 : threadIdx.x < a.splits && __float_as_int(noted_by(threadIdx.x).y) >= 0;
     if (!*abort_flag)
       for (int i = threadIdx.x; i < mine * (DP / 4); i += Cfg::kThreads) {
         const int at_row = i / (DP / 4), dv = i % (DP / 4), r = row0 + at_row;
@@ -994,20 +1119,56 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           const float4 x = ld_cluster_v4(cluster_addr(part_addr + (slot * DP + (dv ^ (slot & 7)) * 4) * 4, rank_of(c)));
           if (!(w < 0.f)) { o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w); }
         }
-        if (!(o.x - o.x == 0.f && o.y - o.y == 0.f && o.z - o.z == 0.f && o.w - o.w == 0.f)) fine[at_row] = 0;
+        // Each quarter's copy of a row has weights of zero for the other quarters' keys, whose infinities make NaN.
+        if (kQuarters && (o.x != o.x || o.y != o.y || o.z != o.z || o.w != o.w) && sound[at_row]) odd = true;
         int qi, h;
         place(r, &qi, &h);
         *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(s.q_start + qi) * a.out_token + h * a.out_head + 4 * dv) =
             make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
       }
-    __syncthreads();
-    if (warp < Cfg::kSoftmax && !*abort_flag)
-      for (int i = warp; i < mine; i += Cfg::kSoftmax)
-        if (!fine[i]) {
-          int qi, h;
-          place(row0 + i, &qi, &h);
-          attend_row<T>(a, s, all_queries, qi, h);
+    if (__syncthreads_or(odd)) {
+      // All warps read v for 32 rows at a time, and put together what they find in the weights' place.
+      constexpr int kWarps = Cfg::kThreads / 32, kWords = 12;
+      uint32_t* marks = reinterpret_cast<uint32_t*>(weights);
+      static_assert(32 * kWords <= Cfg::kWeights, "three masks of 128 channels for each of 32 rows");
+      int lo = 0, hi = (s.keys - 1) >> 5;
+      if (!kQuarters) {
+        int first_noted = INT_MAX, last_noted = -1;
+        for (int c = 0; c < a.splits; ++c) {
+          const float2 of = noted_by(c);
+          first_noted = min(first_noted, __float_as_int(of.x));
+          last_noted = max(last_noted, __float_as_int(of.y));
         }
+        lo = 4 * first_noted;
+        hi = min(hi, 4 * last_noted + 3);
+      }
+      for (int g = 0; g < mine; g += 32) {
+        int qi, h;
+        place(row0 + min(g + lane, mine - 1), &qi, &h);
+        __syncthreads();  // (the marks of the 32 rows before have been read)
+        for (int i = threadIdx.x; i < 32 * kWords; i += Cfg::kThreads) marks[i] = 0;
+        __syncthreads();
+        AttendFound found;
+        attend_scan<T>(a, s, all_queries, qi, kv, g + lane < mine && sound[min(g + lane, mine - 1)], lo + warp, hi, kWarps, found);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (found.nan[c]) atomicOr(marks + kWords * lane + c, found.nan[c]);
+          if (found.up[c]) atomicOr(marks + kWords * lane + 4 + c, found.up[c]);
+          if (found.down[c]) atomicOr(marks + kWords * lane + 8 + c, found.down[c]);
+        }
+        __syncthreads();
+        for (int i = warp; i < min(32, mine - g); i += kWarps) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            found.nan[c] = marks[kWords * i + c];
+            found.up[c] = marks[kWords * i + 4 + c];
+            found.down[c] = marks[kWords * i + 8 + c];
+          }
+          place(row0 + g + i, &qi, &h);
+          attend_put<T>(a, s.q_start + qi, h, found, kQuarters);
+        }
+      }
+    }
   }
   if (a.splits > 1) {
     if (idle) cluster_sync();

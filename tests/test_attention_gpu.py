@@ -798,6 +798,133 @@ def test_a_visible_nan_counts_however_small_its_weight(queries, keys, heads, dim
     assert bool(out[: queries[0], heads // 2:, 3].isnan().all())
 
 
+def kinds(s):
+    """Which results are NaN, and which are infinities, for values that are not and weights that are all above zero."""
+    out = torch.zeros(s["q"].shape, dtype=torch.float64, device="cuda")
+    how, group = s["how"], s["q"].shape[1] // s["k"].shape[1]
+    left, right = how.get("window") or (-1, -1)
+    k_starts, k_lengths = (s["k_starts"], s["k_lengths"]) if s["k_starts"] is not None else (s["starts"], s["lengths"])
+    for b, (start, n, k_start, m) in enumerate(zip(s["starts"], s["lengths"], k_starts, k_lengths)):
+        rows, keys = slice(start, start + n), slice(k_start, k_start + m)
+        doc = how.get("documents")
+        doc_k = how.get("k_documents", doc)
+        sees = see(n, m, how.get("causal", False), left, right, s["prefix"][b] if s["prefix"] else 0,
+                   None if doc is None else doc[rows], None if doc is None else doc_k[keys]).double()
+        for head in range(s["q"].shape[1]):
+            v = s["v"][keys, head // group]
+            nan, up, down = (sees @ t.double() > 0 for t in (v.isnan(), v.isposinf(), v.isneginf()))
+            y = out[rows, head]
+            y[up], y[down] = math.inf, -math.inf
+            y[nan | (up & down)] = math.nan
+    return out
+
+
+@pytest.mark.parametrize("form", ["causal", "window", "documents", "prefix", "few rows", "single tokens"])
+@pytest.mark.parametrize("heads,dim", [(2, 64), (6, 128), (4, 40)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("often", [0.002, 0.05])
+def test_infinities_and_nan_are_those_of_the_visible_values(form, heads, dim, dtype, often):
+    """Whatever the hidden values of the same channels are, in a mask's steps and in those past them."""
+    lengths = [300, 129]
+    if form == "few rows":
+        s = problem(63, [40, 20], [700, 133], heads=heads, kv_heads=2, dim=dim, dtype=dtype, causal=True)
+    elif form == "single tokens":
+        keys = [3000, 200]
+        k_documents = documents(keys, 300, 7) % 3
+        s = problem(63, [2, 1], keys, heads=heads, kv_heads=2, dim=dim, dtype=dtype, documents=k_documents[torch.tensor([2998, 2999, 3199], device="cuda")].clone(),
+                    k_documents=k_documents)
+    else:
+        how = {"causal": dict(causal=True), "window": dict(window=(70, 9)), "documents": dict(documents=documents(lengths, 40, 6)), "prefix": dict(causal=True, window=(20, -1))}[form]
+        s = problem(63, lengths, heads=heads, kv_heads=2, dim=dim, dtype=dtype, prefix=[60, 7] if form == "prefix" else None, **how)
+    g = generator(64)
+    for value in (math.nan, math.inf, -math.inf):
+        s["v"][torch.rand(s["v"].shape, generator=g, device="cuda") < often / 12] = value
+    out, lse = run(s)
+    want = kinds(s)
+    mine = ~define(s)[1].isnan()
+    assert same_kinds(out[mine].double(), want[mine])
+    # Where all a row's values are finite, it is the definition's.
+    clean = {**s, "v": torch.where(s["v"].isfinite(), s["v"], torch.zeros_like(s["v"]))}
+    exact, exact_lse, slack, lse_slack = define(clean)
+    fine = (want == 0) & mine[..., None]
+    assert (out.double() - exact)[fine].abs().sub(slack[fine]).max() <= 0
+    seen = mine & (exact_lse != -math.inf)
+    assert (lse.double() - exact_lse)[seen].abs().sub(lse_slack[seen]).max() <= 0
+
+
+@pytest.mark.parametrize("bad", ["a query", "an early key", "an early value", "a channel", "values here and there"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_visible_nan_takes_no_longer(bad, dim):
+    """A long prompt that has met a NaN is wrong, and not slow: ten times a clean one's time at most."""
+    s = problem(65, [4096], heads=4, kv_heads=2, dim=dim, causal=True)
+    starts, lengths, out = ints(s["starts"]), ints(s["lengths"]), torch.empty_like(s["q"])
+
+    def best():
+        times = []
+        for _ in range(6):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            attention.attend(s["q"], s["k"], s["v"], out, starts, lengths, causal=True)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    clean = best()
+    if bad == "a query":
+        s["q"][50:60, 1] = math.nan
+    elif bad == "an early key":
+        s["k"][50, 0] = math.inf
+    elif bad == "an early value":
+        s["v"][50, :, 7] = math.inf
+    elif bad == "a channel":
+        s["v"][:, 1, 9] = math.nan
+    else:
+        s["v"][torch.rand(s["v"].shape, generator=generator(66), device="cuda") < 1e-4] = math.nan
+    spent = best()
+    want, _, slack, _ = define(s)
+    assert torch.equal(~out.isfinite(), want.isnan())
+    fine = ~want.isnan()
+    assert (out.double() - want)[fine].abs().sub(slack[fine]).max() <= 0
+    assert spent <= 10 * clean, (spent, clean)
+
+
+@pytest.mark.parametrize("queries,keys,dim", [([1] * 40, [3000] * 40, 128), ([1] * 40, [200] * 40, 64), ([700, 300], None, 128), ([20, 1], [9000, 130], 64)])
+def test_the_same_hundreds_of_times(queries, keys, dim):
+    """Roles of a CTA that meet in another order each time."""
+    s = problem(69, queries, keys, heads=8, kv_heads=2, dim=dim, causal=True)
+    want, want_lse = check(s)
+    k = {} if keys is None else {"k_starts": ints(s["k_starts"]), "k_lengths": ints(s["k_lengths"])}
+    starts, lengths, out, lse = ints(s["starts"]), ints(s["lengths"]), torch.empty_like(want), torch.empty_like(want_lse)
+    err, others = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(400):
+        out.fill_(7.0)
+        attention.attend(s["q"], s["k"], s["v"], out, starts, lengths, max_queries=max(queries), max_keys=max(keys or queries), causal=True, lse=lse, err=err, **k)
+        others += (out != want).sum() + (lse != want_lse).sum()
+    assert err.item() == 0 and others.item() == 0
+
+
+@pytest.mark.parametrize("how", [dict(slopes=1e30), dict(slopes=2e38), dict(slopes=3.4e38), dict(cap=1e-30), dict(cap=1e-40), dict(cap=1e-45), dict(cap=3e38),
+                                 dict(cap=1e30, scale=1e-10), dict(cap=1e-40, slopes=0.5), dict(cap=1e-40, distance_bias=3)])
+@pytest.mark.parametrize("queries,keys", [([300], None), ([1, 3], [900, 200])])
+def test_factors_at_the_ends_of_their_range(how, queries, keys):
+    how = dict(how)
+    if "slopes" in how:
+        how["slopes"] = torch.full((4,), how["slopes"], device="cuda")
+    if "distance_bias" in how:
+        how = with_bias(how, 4)
+    s = problem(67, queries, keys, heads=4, kv_heads=2, dim=64, causal=True, **how)
+    s["q"][::3] = 0
+    check(s)
+
+
+def test_a_scale_at_the_end_of_its_range():
+    for value in (3e38, -3e38):
+        s = problem(68, [300, 1], heads=4, kv_heads=2, dim=64, causal=True, scale=value)
+        s["q"].zero_()
+        check(s)
+
+
 # -------------------------------------------------------------------------------- a layer
 
 def layer_example():
