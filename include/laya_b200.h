@@ -378,7 +378,8 @@ int laya_op_mx8_linear(const laya_mx8_linear* args, int* err, void* stream);
  * is fused into a product and whose attention has 64-value heads and a symmetric window only): what stands
  * between the two projections of a layer.
  *
- * Tensors are [tokens][heads][head_dim] with any token and head stride (in elements); the values of a
+ * Tensors are [tokens][heads][head_dim] with token and head strides of their own (in elements): at least 0 for x, at least head_dim
+ * for q, k and v (a dimension that is broadcast has to be laid out), and such that no two heads overlap for what is written; the values of a
  * head are contiguous.  Buffers must be on the current device (not checked here), and so must `stream`
  * (LAYA_ERR_INVALID otherwise).  The calls allocate nothing and wait for nothing.
  * ------------------------------------------------------------------------------------------ */

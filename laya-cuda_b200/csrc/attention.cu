@@ -18,19 +18,36 @@ void check_heads(const char* what, const void* p, int64_t token, int64_t head, i
   if (reinterpret_cast<uintptr_t>(p) % dtype_size(dtype)) fail(LAYA_ERR_INVALID, "%s is not aligned to its elements", what);
 }
 
-// Tokens and heads apart from one another, as what is written must be.
-void check_apart(const char* what, int tokens, int heads, int dim, int64_t token, int64_t head) {
+void check_strides(const char* what, int tokens, int heads, int dim, int64_t token, int64_t head) {
   if ((tokens > 1 && token < dim) || (heads > 1 && head < dim))
     fail(LAYA_ERR_INVALID, "%s: strides %lld and %lld must be at least a head's %d values", what, (long long)token, (long long)head, dim);
 }
 
+// Tokens and heads apart from one another, as what is written must be.
+void check_apart(const char* what, int tokens, int heads, int dim, int64_t token, int64_t head) {
+  check_strides(what, tokens, heads, dim, token, head);
+  if (tokens <= 1 || heads <= 1) return;
+  using Wide = __int128;
+  if (token >= (Wide)(heads - 1) * head + dim || head >= (Wide)(tokens - 1) * token + dim) return;
+  // Neither lies within a step of the other: j steps of one meet i of the other where they are less than a head apart.
+  const int few = std::min(tokens, heads), many = std::max(tokens, heads);
+  const int64_t by = tokens < heads ? token : head, of = tokens < heads ? head : token;
+  for (int j = 1; j < few; ++j) {
+    const Wide at = (Wide)j * by;
+    for (Wide i = std::max<Wide>(1, at / of); i <= at / of + 1 && i < many; ++i)
+      if (at - i * of < dim && i * of - at < dim)
+        fail(LAYA_ERR_INVALID, "%s: with strides %lld and %lld heads of %d values overlap", what, (long long)token, (long long)head, dim);
+  }
+}
+
 // 16-byte vectors, which the tensor maps and the stores of attention take.  The stride of a dimension of one says nothing and is
 // made one that they take.
-void check_vectors(const char* what, const void* p, int tokens, int heads, int dim, int64_t* token, int64_t* head, int dtype) {
+void check_vectors(const char* what, const void* p, int tokens, int heads, int dim, int64_t* token, int64_t* head, int dtype, bool written) {
   if (heads == 1) *head = dim;
   if (tokens == 1) *token = heads * *head;
   check_heads(what, p, *token, *head, dtype);
-  check_apart(what, tokens, heads, dim, *token, *head);
+  if (written) check_apart(what, tokens, heads, dim, *token, *head);
+  else check_strides(what, tokens, heads, dim, *token, *head);
   if (reinterpret_cast<uintptr_t>(p) & 15) fail(LAYA_ERR_INVALID, "%s must be 16-byte aligned", what);
   if (*token % 8 || *head % 8) fail(LAYA_ERR_INVALID, "%s: strides %lld and %lld must each be a multiple of 8", what, (long long)*token, (long long)*head);
   if (*token >= (1ll << 38) || *head >= (1ll << 38)) fail(LAYA_ERR_INVALID, "%s: a stride is too large", what);
@@ -254,11 +271,11 @@ int laya_op_attend(const laya_attend* p, int* err, void* stream) {
   a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.lse = p->lse;
   a.q_token = p->q_token; a.q_head = p->q_head; a.k_token = p->k_token; a.k_head = p->k_head;
   a.v_token = p->v_token; a.v_head = p->v_head; a.out_token = p->out_token; a.out_head = p->out_head;
-  check_vectors("q", p->q, p->q_tokens, p->heads, p->head_dim, &a.q_token, &a.q_head, p->dtype);
-  check_vectors("out", p->out, p->q_tokens, p->heads, p->head_dim, &a.out_token, &a.out_head, p->dtype);
+  check_vectors("q", p->q, p->q_tokens, p->heads, p->head_dim, &a.q_token, &a.q_head, p->dtype, false);
+  check_vectors("out", p->out, p->q_tokens, p->heads, p->head_dim, &a.out_token, &a.out_head, p->dtype, true);
   if (p->k_tokens) {
-    check_vectors("k", p->k, p->k_tokens, p->kv_heads, p->head_dim, &a.k_token, &a.k_head, p->dtype);
-    check_vectors("v", p->v, p->k_tokens, p->kv_heads, p->head_dim, &a.v_token, &a.v_head, p->dtype);
+    check_vectors("k", p->k, p->k_tokens, p->kv_heads, p->head_dim, &a.k_token, &a.k_head, p->dtype, false);
+    check_vectors("v", p->v, p->k_tokens, p->kv_heads, p->head_dim, &a.v_token, &a.v_head, p->dtype, false);
   }
   a.starts = p->starts; a.lengths = p->lengths;
   a.k_starts = p->k_starts ? p->k_starts : p->starts;

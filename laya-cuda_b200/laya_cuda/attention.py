@@ -1,8 +1,8 @@
 """Between a layer's projections: rotary positions, and attention over packed sequences with caps, biases by distance
 and masks (laya_op_rotary and laya_op_attend of include/laya_b200.h).
 
-Tensors are [tokens][heads][head_dim] with any token and head stride, so slices of a projection's result
-serve as they are; they are torch's, or anything with the attributes of theirs that csrc/python_tensors.h
+Tensors are [tokens][heads][head_dim] with token and head strides of their own, so slices of a projection's result
+serve as they are (q, k and v may not be broadcast, and heads that are written may not overlap); they are torch's, or anything with the attributes of theirs that csrc/python_tensors.h
 reads (torch itself is not imported).  The caller owns every buffer.  The calls are enqueued on `stream` (a
 cudaStream_t as an integer, 0 being the legacy default stream; without it, torch's current stream, or that of
 whatever framework the tensors belong to, and the legacy default stream if its tensors do not tell) of the

@@ -69,6 +69,22 @@ def test_attend_refuses(lib, other, word):
         _lib.check(lib.laya_op_attend(None, None, None))
 
 
+@pytest.mark.parametrize("tokens,heads,token,head", [(4, 2, 64, 64), (10, 4, 128, 64), (10, 4, 64, 256), (2, 3, 128, 128), (3, 2, 128, 256), (5, 4, 256, 96), (5, 7, 200, 320),
+                                                     (10 ** 6, 3, 64, 64 * 999999)])
+def test_heads_that_overlap_are_not_written(lib, tokens, heads, token, head):
+    if tokens < 100:  # by enumeration
+        at = sorted(i * token + j * head for i in range(tokens) for j in range(heads))
+        assert min(b - a for a, b in zip(at, at[1:])) < 64
+    with pytest.raises(ValueError, match="overlap"):
+        _lib.check(lib.laya_op_rotary(ct.byref(rotary(dict(out_token=token, out_head=head, heads=heads), tokens=tokens)), None))
+    if token % 8 == 0 and head % 8 == 0:
+        with pytest.raises(ValueError, match="overlap"):
+            _lib.check(lib.laya_op_attend(ct.byref(attend(q_tokens=tokens, heads=heads, kv_heads=1, q_token=heads * 64, q_head=64, out_token=token, out_head=head)), None, None))
+    for name in ("q", "k", "v"):  # what is read may overlap, but not lie within a head
+        with pytest.raises(ValueError, match=f"{name}: strides .* at least"):
+            _lib.check(lib.laya_op_attend(ct.byref(attend(**{name + "_head": 0})), None, None))
+
+
 def test_nothing_to_do_needs_no_buffers_and_no_device(lib):
     assert lib.laya_op_rotary(ct.byref(rotary(dict(x=None, out=None), tokens=0, positions=None)), None) == 0
     assert lib.laya_op_rotary(ct.byref(rotary(dict(x=None, out=None, heads=0), positions=None)), None) == 0

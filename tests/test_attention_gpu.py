@@ -387,6 +387,21 @@ def test_offsets_past_32_bits():
     check(s)
 
 
+@pytest.mark.parametrize("token,head", [(3, 2), (2, 3), (5, 2), (2, 7)])
+def test_heads_between_one_another(token, head):
+    """Strides of `token` and `head` heads: neither dimension within a step of the other, and no two the same."""
+    s = problem(70, [2, 1] if head < token else [1, 1], heads=2 if token != 5 else 3, kv_heads=1, dim=64, causal=True)
+    rows, heads = s["q"].shape[:2]
+    assert len({i * token + j * head for i in range(rows) for j in range(heads)}) == rows * heads
+    store = torch.full(((rows - 1) * token + (heads - 1) * head + 1, 64), 7.0, dtype=s["q"].dtype, device="cuda").view(-1)
+    out = store.as_strided((rows, heads, 64), (token * 64, head * 64, 1))
+    check(s, run(s, out=out))
+    positions = torch.arange(rows, device="cuda")
+    before = s["q"].clone()
+    attention.rotary(s["q"], positions, out)
+    check_rotary(before, out, positions, "bf16", 64)
+
+
 # -------------------------------------------------------------------------------- attention: masks, caps, biases
 
 def documents(lengths, mean, seed, order=False):
