@@ -203,7 +203,7 @@ bool take_rows(const char* name, PyObject* t, int rows, int cols, int device, Ro
     PyErr_Format(PyExc_ValueError, "%s: the values of a row must be contiguous", name);
     return false;
   }
-  if (v.dtype < 0 || v.dtype == kInt32) {
+  if (v.dtype < 0 || v.dtype >= kInt32) {
     PyErr_Format(PyExc_ValueError, "%s is not float32, float16 or bfloat16", name);
     return false;
   }

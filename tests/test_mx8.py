@@ -407,3 +407,18 @@ def test_empty_makes_no_more_bytes_than_the_matrix_has():
     for bad in (object(), Fake((4,))):
         with pytest.raises(AttributeError):
             mx8.Matrix.empty(bad, 4, 32)
+
+
+@pytest.mark.parametrize("name", ["torch.int64", "torch.int32", "torch.bool"])
+def test_matrices_of_other_types_are_refused_by_name(name):
+    def other(shape, size=8):
+        made = Fake(shape, size=size)
+        made.dtype = Dtype(name)
+        return made
+
+    for call, what in ((lambda: mx8.quantize(other((4, 32)), matrix(4, 32)), "x"), (lambda: mx8.dequantize(matrix(4, 32), other((4, 32))), "out"),
+                       (lambda: mx8.rms_norm(other((4, 32)), Fake((32,)), matrix(4, 32)), "x"),
+                       (lambda: mx8.rms_norm(Fake((4, 32)), Fake((32,)), matrix(4, 32), residual=other((4, 32)), sum_out=Fake((4, 32))), "residual"),
+                       (lambda: mx8.linear(matrix(4, 32), matrix(8, 32), other((4, 8))), "out")):
+        with pytest.raises(ValueError, match=f"^{what} is not float32, float16 or bfloat16$"):
+            call()
