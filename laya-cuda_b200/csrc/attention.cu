@@ -267,6 +267,11 @@ int laya_op_attend(const laya_attend* p, int* err, void* stream) {
   if (!p->k_starts != !p->k_lengths) fail(LAYA_ERR_INVALID, "k_starts and k_lengths go together");
   if (!p->sequences || !p->q_tokens || !p->max_queries) return LAYA_OK;
   if (!p->starts || !p->lengths) fail(LAYA_ERR_INVALID, "starts or lengths is null");
+  const struct { const char* name; const void* p; } vectors[] = {
+      {"starts", p->starts}, {"lengths", p->lengths}, {"k_starts", p->k_starts}, {"k_lengths", p->k_lengths}, {"prefix", p->prefix}, {"documents", p->documents},
+      {"k_documents", p->k_documents}, {"slopes", p->slopes}, {"distance_bias", p->distance_bias}, {"lse", p->lse}, {"err", err}};
+  for (const auto& v : vectors)
+    if (reinterpret_cast<uintptr_t>(v.p) % 4) fail(LAYA_ERR_INVALID, "%s is not aligned to its elements", v.name);
   AttendArgs a = {};
   a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.lse = p->lse;
   a.q_token = p->q_token; a.q_head = p->q_head; a.k_token = p->k_token; a.k_head = p->k_head;

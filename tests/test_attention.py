@@ -85,6 +85,16 @@ def test_heads_that_overlap_are_not_written(lib, tokens, heads, token, head):
             _lib.check(lib.laya_op_attend(ct.byref(attend(**{name + "_head": 0})), None, None))
 
 
+@pytest.mark.parametrize("name", ["starts", "lengths", "k_starts", "k_lengths", "prefix", "documents", "k_documents", "slopes", "distance_bias", "lse", "err"])
+@pytest.mark.parametrize("off", [1, 2])
+def test_attend_refuses_unaligned_vectors(lib, name, off):
+    fields = dict(documents=P, k_documents=P) if "documents" in name else {}
+    if name != "err":
+        fields[name] = P + off
+    with pytest.raises(ValueError, match=f"^{name} is not aligned"):
+        _lib.check(lib.laya_op_attend(ct.byref(attend(**fields)), ct.c_void_p(P + off) if name == "err" else None, None))
+
+
 def test_nothing_to_do_needs_no_buffers_and_no_device(lib):
     assert lib.laya_op_rotary(ct.byref(rotary(dict(x=None, out=None), tokens=0, positions=None)), None) == 0
     assert lib.laya_op_rotary(ct.byref(rotary(dict(x=None, out=None, heads=0), positions=None)), None) == 0
