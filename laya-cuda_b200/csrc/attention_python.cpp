@@ -3,6 +3,7 @@
 #include "python_tensors.h"
 
 #include <cmath>
+#include <limits>
 
 namespace {
 
@@ -244,6 +245,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* k
     return nullptr;
   a.scale = (float)scale;
   a.cap = (float)cap;
+  if (cap > 0 && a.cap == 0) a.cap = std::numeric_limits<float>::denorm_min();  // 0 would be no cap
   if (!take_vector("slopes", g[SLOPES], q.heads, device, &a.slopes)) return nullptr;
   if (given(g[DISTANCE_BIAS])) {
     View t;

@@ -933,6 +933,11 @@ def test_factors_at_the_ends_of_their_range(how, queries, keys):
     check(s)
 
 
+@pytest.mark.parametrize("cap", [1e-46, 1e-60, 5e-324])
+def test_a_cap_below_32_bits_is_a_cap(cap):
+    check(problem(71, [300, 1], heads=4, kv_heads=2, dim=64, causal=True, cap=cap))
+
+
 def test_a_scale_at_the_end_of_its_range():
     for value in (3e38, -3e38):
         s = problem(68, [300, 1], heads=4, kv_heads=2, dim=64, causal=True, scale=value)
