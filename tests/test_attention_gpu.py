@@ -596,6 +596,47 @@ def test_two_calls_at_once():
         assert torch.equal(out, want[i % 2][0]) and torch.equal(lse, want[i % 2][1])
 
 
+@pytest.mark.parametrize("threads", [1, 2])
+def test_calls_in_flight_together(threads):
+    """Each on a stream of its own, held back until all are enqueued: tiles of both head sizes, single tokens in a quarter of a tile and over a cluster, joined
+    halves.  Few CTAs each, so that those of different calls share the GPU and its SMs."""
+    from concurrent.futures import ThreadPoolExecutor
+    forms = [problem(72, [260, 100], heads=4, kv_heads=2, dim=64, causal=True), problem(73, [300], heads=4, kv_heads=2, dim=128, causal=True, cap=30.0),
+             problem(74, [1, 1], [9000, 300], heads=8, kv_heads=2, dim=128), problem(75, [40], [700], heads=2, kv_heads=1, dim=128, causal=True),
+             problem(76, [1] * 9, [200] * 9, heads=4, kv_heads=2, dim=64, causal=True), problem(77, [200, 90], heads=4, kv_heads=2, dim=64, distance_bias=randn(generator(1), 4, 41).float())]
+    calls = []
+    for s in forms:
+        want, want_lse = check(s)
+        k = {} if s["k_starts"] is None else {"k_starts": ints(s["k_starts"]), "k_lengths": ints(s["k_lengths"])}
+        bounds = dict(max_queries=max(s["lengths"]), max_keys=max(s["k_lengths"] or s["lengths"]))
+        calls.append(dict(args=(s["q"], s["k"], s["v"]), out=torch.empty_like(want), starts=ints(s["starts"]), lengths=ints(s["lengths"]), how={**k, **bounds, **s["how"]},
+                          lse=torch.empty_like(want_lse), err=torch.zeros(1, dtype=torch.int32, device="cuda"), want=want, want_lse=want_lse,
+                          others=torch.zeros((), dtype=torch.int64, device="cuda"), stream=torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    gate = torch.cuda.Event()
+    torch.cuda._sleep(40_000_000)
+    gate.record()
+
+    def enqueue(some):
+        for c in some:
+            c["stream"].wait_event(gate)
+        for _ in range(25):
+            for c in some:
+                with torch.cuda.stream(c["stream"]):
+                    c["out"].fill_(7.0)
+                    attention.attend(*c["args"], c["out"], c["starts"], c["lengths"], lse=c["lse"], err=c["err"], **c["how"])
+                    c["others"] += (c["out"] != c["want"]).sum() + (c["lse"] != c["want_lse"]).sum()
+
+    if threads == 1:
+        enqueue(calls)
+    else:
+        with ThreadPoolExecutor(threads) as pool:
+            list(pool.map(enqueue, (calls[::2], calls[1::2])))
+    torch.cuda.synchronize()
+    assert [c["err"].item() for c in calls] == [0] * len(calls)
+    assert [c["others"].item() for c in calls] == [0] * len(calls)
+
+
 def test_pieces_join_by_their_logarithms():
     """A shared prefix and the rest of the keys, attended apart, give the whole."""
     s = problem(22, [30], [1000], heads=4, kv_heads=2, dim=64)
