@@ -525,6 +525,57 @@ def test_hidden_keys_may_hold_anything(bad, dim):
     assert ((out[clean].double() - exact[clean]).abs() <= slack[clean]).all()
 
 
+def narrow_bounds(s):
+    """out and lse in 64 bits, and bounds that count each rounding: exponentials to 2^-22 of themselves, a cap's polynomial up to 0.8 of the cap, with its
+    roundings, to 2^-21 of its result, beyond that to 2^-21 of the cap, the logarithm to a unit in its last place."""
+    u, how, (rows, heads, dim), kv = 2.0 ** -24, s["how"], s["q"].shape, s["k"].shape[1]
+    cap, k_starts, k_lengths = how.get("cap", 0.0), s["k_starts"] or s["starts"], s["k_lengths"] or s["lengths"]
+    out, lse = torch.zeros(rows, heads, dim, dtype=torch.float64, device="cuda"), torch.zeros(rows, heads, dtype=torch.float64, device="cuda")
+    out_slack, lse_slack = torch.zeros_like(out), torch.zeros_like(lse)
+    for start, n, k_start, m in zip(s["starts"], s["lengths"], k_starts, k_lengths):
+        at, keys = slice(start, start + n), slice(k_start, k_start + m)
+        p, j = torch.arange(m - n, m, device="cuda")[:, None], torch.arange(m, device="cuda")
+        for h in range(heads):
+            q, k, v = s["q"][at, h].double(), s["k"][keys, h * kv // heads].double(), s["v"][keys, h * kv // heads].double()
+            x, ds = q @ k.T / math.sqrt(dim), (dim + 8) * u * (q.abs() @ k.abs().T) / math.sqrt(dim)
+            if cap:
+                near = (x / cap).abs() <= 0.8
+                x = cap * torch.tanh(x / cap)
+                ds = ds + 2.0 ** -21 * torch.where(near, x.abs(), torch.full_like(x, cap))
+            bias = torch.zeros_like(x)
+            if "slopes" in how:
+                bias = -how["slopes"][h].double() * (p - j).abs()
+            if "distance_bias" in how:
+                table = how["distance_bias"][h].double()
+                bias = table[(j - p).clamp(-(len(table) // 2), len(table) // 2) + len(table) // 2]
+            x = x + bias
+            if how.get("causal"):
+                x = torch.where(j <= p, x, torch.full_like(x, -math.inf))
+            top, w, full = x.amax(1), torch.softmax(x, 1), torch.logsumexp(x, 1)
+            ds = torch.where(w > 0, ds + 4 * u * bias.abs() + 6 * u * (x.abs() + top[:, None].abs()), torch.zeros_like(ds))
+            spread, sums = (w * ds).sum(1), 2.0 ** -21 + (m / 16 + 64) * u
+            y, size = w @ v, w @ v.abs()
+            out[at, h], lse[at, h] = y, full
+            out_slack[at, h] = ((w * ds) @ v.abs() + (HALF[s["dtype"]] + sums + spread[:, None]) * size + 2.0 ** -31 * v.abs().sum(0)
+                                + 1.01 * HALF[s["dtype"]] * y.abs() + TINY[s["dtype"]])
+            lse_slack[at, h] = spread + sums + 2 * u * (math.log(m) + 10) + 6 * u * (full.abs() + top.abs() + 1)
+    return out, lse, out_slack, lse_slack
+
+
+@pytest.mark.parametrize("how", [dict(), dict(cap=30.0), dict(cap=2.0), dict(cap=500.0), dict(slopes=True), dict(distance_bias=50), dict(cap=20.0, slopes=True), dict(cap=50.0, distance_bias=16)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (3, 1, 128)])
+@pytest.mark.parametrize("queries,keys", [([300, 129], None), ([1, 3], [1500, 200])])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_logarithms_and_caps_to_their_roundings(how, heads, kv_heads, dim, queries, keys, dtype):
+    s = problem(80, queries, keys, heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype, causal=True, **with_bias(how, heads))
+    out, lse = run(s)
+    want, want_lse, slack, lse_slack = narrow_bounds(s)
+    off = (lse.double() - want_lse).abs()
+    assert bool((off <= lse_slack).all()), ((off / lse_slack).max().item(), off.max().item(), lse_slack.max().item())
+    off = (out.double() - want).abs()
+    assert bool((off <= slack).all()), (off / slack).max().item()
+
+
 # -------------------------------------------------------------------------------- attention: calls
 
 @pytest.mark.parametrize("queries,keys", [([300, 200], None), ([1, 1], [9000, 300])])
