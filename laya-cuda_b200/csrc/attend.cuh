@@ -77,7 +77,8 @@ __device__ __forceinline__ AttendSpan attend_span(const AttendArgs& a, int p, in
 // warps look its V over while the softmax is at work, put zeros in the place of what is not finite, and note the step.  What that took from rows that see such a key is put into their
 // results at the end: attend_scan finds it, reading v of the noted steps once for all rows of a warp, attend_put writes it.  (Steps that all rows see are left as they are.)
 // 4096 causal tokens, 4 heads of 128 over 2: 59 us; with a NaN in every key's v 88, with 100 NaN here and there 78 (50 ms when each row with a NaN was computed again by a warp).
-// What it costs without any: windowed documents 161 -> 168 us, a packed batch 347 -> 357, single tokens and long prompts nothing.
+// What it costs without any: windowed documents 160 -> 168 us, a packed batch 345 -> 356, ragged sequences up to 300 with heads of 64 69 -> 75 and with a window and a
+// learned bias 312 -> 348; single tokens and long prompts nothing.
 // ---------------------------------------------------------------------------------------------
 
 // Pairs of 16-bit values.
@@ -814,12 +815,10 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         int both = 0;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const bool in_prefix = kb < prefix, whole_prefix = kb + kAtKeys <= prefix;
-          const bool meets = kb <= outer[t].hi && last >= outer[t].lo && (!a.documents || (lo <= doc_hi[t] && hi >= doc_lo[t]));
-          const bool to_last = last < prefix || (kb >= inner[t].lo && last <= inner[t].hi &&
-                                                 (!a.documents || (lo == hi && doc_lo[t] == doc_hi[t] && lo == doc_lo[t])));
-          both |= (!tokens[t] ? kAtSkip : whole_prefix || (to_last && last == kb + kAtKeys - 1) ? kAtFull : to_last ? kAtTail : in_prefix || meets ? kAtMasked : kAtSkip)
-                  << 2 * t;
+          const bool one = !a.documents || (lo == hi && doc_lo[t] == doc_hi[t] && lo == doc_lo[t]);
+          const bool to_last = last < prefix || (kb >= inner[t].lo && last <= inner[t].hi && one);
+          const bool meets = kb < prefix || (kb <= outer[t].hi && last >= outer[t].lo && (!a.documents || (lo <= doc_hi[t] && hi >= doc_lo[t])));
+          both |= (!tokens[t] ? kAtSkip : to_last ? (last == kb + kAtKeys - 1 ? kAtFull : kAtTail) : meets ? kAtMasked : kAtSkip) << 2 * t;
         }
         return both;
       };
@@ -858,6 +857,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           if (!summed) {
             lo = __reduce_min_sync(0xffffffffu, min(min(d[0], d[1]), min(d[2], d[3])));
             hi = __reduce_max_sync(0xffffffffu, max(max(d[0], d[1]), max(d[2], d[3])));
+            if (kb >= prefix && (lo > doc_hi[0] || hi < doc_lo[0]) && (NT == 1 || lo > doc_hi[1] || hi < doc_lo[1])) continue;  // (most steps of many documents)
             both = classify(step, lo, hi);
             if (!both) continue;
           }
@@ -995,7 +995,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           uint32_t sum[4] = {};
           for (int h = 0; h < halves; ++h) {
             const uint4* v = reinterpret_cast<const uint4*>(tile + h * Cfg::kHalf + key0 * 128) + lane;
-#pragma unroll 8
+#pragma unroll 4  // (8 are no faster)
             for (int i = 0; i < 16; ++i) {
               const uint4 w = key0 + 4 * i + (lane >> 3) < rows ? v[32 * i] : make_uint4(0, 0, 0, 0);
               sum[0] = F::gather(w.x, sum[0]);
