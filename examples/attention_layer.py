@@ -2,7 +2,8 @@
 
     r += x;  n = rms_norm(r) * weight                       one kernel, n in MX8
     q, k, v = n W^T                                         one kernel, 16 bits
-    q, k turned by their positions, k into the cache        one kernel
+    q, k turned by their positions, in place                one kernel
+    k, v into the cache                                     torch's indexing
     a = attention of q over the cache                       one kernel (the prompt's tokens, or one token for each sequence)
     r += a O^T                                              two kernels, a put into MX8 first
 

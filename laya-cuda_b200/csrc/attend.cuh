@@ -191,10 +191,12 @@ __device__ void attend_put(const AttendArgs& a, int token, int head, const Atten
 // of the next are issued together as soon as P is there, and the other tile's softmax hides them.
 //
 // What bounds it: with prompts the softmax.  A step of a tile with heads of 128 is 2 x 128^3 multiply-adds, some 512 cycles of the tensor core, and 128 x 128
-// exponentials, 1024 cycles of the special-function units that the two tiles share out: 16384 causal tokens, 16 heads of 128 over 4, bf16, 973 us (1.13 PFLOP/s
-// of 1.66), not causal 8192 559 us (0.98); heads of 64, which have as many exponentials for half the products, 849 us (0.64); a cap doubles the work on the FMA
-// pipe (1389 us); slopes cost 10%.  Single tokens: the caches' bytes, 6.0 TB/s (16 x 32768 keys, 8 kv heads of 128, 2.1 GB).  A few queries over one cache: the chain of
-// launch, first loads, products and the join (1 x 4000 keys 20 us, 1 x 96 7 us).
+// exponentials, 1024 cycles of the special-function units that the two tiles share out: 16384 causal tokens, 16 heads of 128 over 4, bf16, inputs of unit variance, 980-1000 us
+// (1.11 PFLOP/s of 1.66), not causal 8192 570 us (0.97); heads of 64, which have as many exponentials for half the products, 888 us (0.62); a cap doubles the work on the FMA
+// pipe (1370 us); slopes cost 8%.  Single tokens: the caches' bytes, 5.8 TB/s (16 x 32768 keys, 8 kv heads of 128, 2.1 GB, 367 us); but one cache of 131072 keys is 64 CTAs' work,
+// 168 us (3.2 TB/s), with 1 kv head 16 CTAs', 92 us.  A few queries over one cache: the chain of launch, first loads, products and the join (1 x 4000 keys 22 us, cold, 1 x 96 7 us).
+// Documents are looked over ahead up to 256 steps of a CTA; past that each step costs a trip to memory (causal tokens in documents of 600, 8 heads of 128 over 2:
+// 32768 215 us, 65536 1460).
 //
 // Tiles: with heads past 64 two to a CTA and one CTA per SM (one tile, two CTAs: 16384 causal 976 -> 999 us, with a cap 1441 -> 1482, 8192 tokens
 // in documents 207 -> 229: K and V are loaded twice, into one buffer each).  Heads up to 64: one to a CTA and two CTAs per SM, whose starts and ends overlap
@@ -564,7 +566,9 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       constexpr int kMine = 32 * NC;              // keys of this thread
       const int d = kb + 32 * chunk0 - p;  // the first less the query
       float sum = 0.f;
-      // P from the exponents that f gives of the scores, to TMEM; the largest exponent.
+      // P from the exponents that f gives of the scores, to TMEM; the largest exponent.  P is rounded to the inputs' type, in which the tensor core takes it (bf16 results
+      // are then off by 0.0020 of their size where the rounding of the results alone gives 0.0016, f16 ones by 0.00028 and 0.00021); their sum is not.  ex2.approx is
+      // off by 2^-22.
       auto numerators = [&](auto f) {
         float2 part[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -620,8 +624,8 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
       };
       bool done = false;
       // Masked steps and a row's first one take the other way: a second form of this one for masked steps made all 3% slower by its code's length, and
-      // a first maximum from the raw products, so that first steps too come here, took longer than it saved (a learned bias 189 -> 180 us at 64 x 512, a
-      // cap at 16384 causal 1436 -> 1389; plain ragged sequences of 64 306 -> 310).
+      // a first maximum from the raw products, so that first steps too come here, took longer than it saved (without it a learned bias 189 -> 180 us at 64 x 512, a
+      // cap at 16384 causal, unit variance, 1436 -> 1389; plain ragged sequences of 64 306 -> 310).
       if (!kGeneral && whole && !__any_sync(0xffffffffu, m == -INFINITY && live)) done = at_once();
       if (!done) {
         if (!kGeneral) tmem_wait_st();  // before P is written again

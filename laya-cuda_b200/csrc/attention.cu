@@ -141,7 +141,7 @@ void launch_attend(AttendArgs a, int max_keys, int dev, cudaStream_t st) {
   a.by_splits = FastDiv(a.splits);
   a.by_kv = FastDiv(a.kv_heads);
   // Where all of a sequence's tiles see the same keys, they run one after the other and find them in the L2 cache: 64 ragged sequences up to 1024 (12 heads of
-  // 64) 315 -> 280 us, with a learned bias 394 -> 345, 24 up to 4096 (8 kv heads of 128) 3179 -> 2680.  A causal mask wants the longest tiles of all
+  // 64) 315 -> 280 us, with a learned bias 394 -> 345, 24 up to 4096 (8 kv heads of 128) 3179 -> 2680 when it was taken.  A causal mask wants the longest tiles of all
   // sequences first (64 x 512 128 us, 150 otherwise), a window gains nothing (314, 321).
   a.pairs_inside = !a.causal && a.left < 0 && a.right < 0 && (int64_t)a.sequences * a.kv_heads >= sms;
   a.by_inner = FastDiv(a.pairs_inside ? a.pairs : a.sequences);

@@ -323,7 +323,8 @@ PyMethodDef methods[] = {
      "s -= slopes[head] |p - j|, or s += distance_bias[head][clamp(j - p, -reach, reach) + reach].\n"
      "Key j is visible where j < prefix[b], or where documents[query] == k_documents[key], causal implies\n"
      "j <= p, and p - left <= j <= p + right (window; -1: no bound).  max_queries, max_keys: bounds on the lengths\n"
-     "(the tensors' rows, without them); tight ones launch less.  lse: float32 [q tokens][heads], receives the\n"
+     "(the tensors' rows, without them): each sequence is launched for max_queries, so give it where there are several\n"
+     "(64 x 1024 tokens, 12 heads of 64: 0.34 ms, 2.2 without).  lse: float32 [q tokens][heads], receives the\n"
      "logarithm of the sum of exp(s).  err: an int32 tensor, zero on entry, that receives a device error."},
     {"set_attention_loader", set_loader, METH_O, "set_attention_loader(f)\n--\n\nf() is called before the first operator and calls bind_attention()."},
     {"bind_attention", bind, METH_VARARGS, "bind_attention(rotary, attend, last_error, current_device)\n--\n\nAddresses of the library's functions."},

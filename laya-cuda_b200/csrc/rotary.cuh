@@ -49,8 +49,8 @@ struct alignas(V == 1 ? sizeof(T) : 16) RotaryVector {
 // A place is, in the half layout, two vectors of V values half of the turned values apart; interleaved, one vector, or two values where V is 1.
 //
 // Heads of a lane at a time, with as many on the way, and blocks of an SM, as measured: vectors of the half layout one and five (16384 x 40 x 128
-// bf16 70 us; two and four 84, four and two, without loads ahead, 121), interleaved 16-bit ones the same (78 us; two 88), of 32 bits two
-// and four (9001 x 32 x 96 49 us; one 65), single values four and four.
+// bf16 70 us; two and four 84, four and two, without loads ahead, 121), interleaved 16-bit ones the same (78-80 us; two 88), of 32 bits two
+// and four (9001 x 32 x 96 49 us; one 65), single values four and four (rows that are not whole vectors: 16384 x 40 x 128 bf16 125 us, 9001 x 32 x 96 of 32 bits 66).
 template <typename T, int V, bool kInterleaved>
 __global__ void __launch_bounds__(kRotaryThreads, V > 1 && (!kInterleaved || sizeof(T) == 2) ? 5 : 4) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int P = kInterleaved && V > 1 ? V / 2 : V;  // pairs of a place
@@ -98,6 +98,7 @@ __global__ void __launch_bounds__(kRotaryThreads, V > 1 && (!kInterleaved || siz
           f *= keep + (1.0 - keep) * a.shrink;
         }
         const double t = (double)position * f;
+        // The angle within a turn, its sine and cosine in 32 bits (32-bit results 5.1e-8 off, 4.2e-8 with these in 64).
         float s, c;
         sincospif((float)(2.0 * (t - rint(t))), &s, &c);
         mine[k] = make_float2(c * a.magnitude, s * a.magnitude * a.sine_sign);

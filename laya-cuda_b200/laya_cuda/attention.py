@@ -12,7 +12,7 @@ stream than the one that wrote it is the caller's to order.
     qkv = projected.view(tokens, heads + 2 * kv_heads, head_dim)
     q, k, v = qkv[:, :heads], qkv[:, heads:-kv_heads], qkv[:, -kv_heads:]
     attention.rotary(q, positions, q, k=k, k_out=k)                      # in place
-    attention.attend(q, k, v, out, starts, lengths, causal=True, cap=50.0)
+    attention.attend(q, k, v, out, starts, lengths, max_queries=longest, max_keys=longest, causal=True, cap=50.0)
 
 `examples/attention_layer.py` runs them between two products of laya_cuda.mx8.
 """
