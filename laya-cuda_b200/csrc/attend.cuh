@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
         a.lse[token * a.heads + head] = any ? (kNatural ? m : m / kLog2e) + (log2f(l) - kShift) / kLog2e : -INFINITY;
       if (noted[1] >= 0) {
         AttendFound found;
-        attend_scan<T>(a, s, all_queries, query, kv, live && l > 0.f, 4 * noted[0], min(4 * noted[1] + 3, (s.keys - 1) >> 5), 1, found);
+        attend_scan<T>(a, s, all_queries, query, kv, live && l > 0.f, 4 * min(noted[0], noted[1]), min(4 * noted[1] + 3, (s.keys - 1) >> 5), 1, found);
         for (uint32_t rest = __ballot_sync(0xffffffffu, found.any()); rest; rest &= rest - 1) {
           const int src = __ffs(rest) - 1;
           AttendFound theirs;
@@ -1143,7 +1143,7 @@ __global__ void __launch_bounds__(AttendCfg<DP, NT>::kThreads, AttendCfg<DP, NT>
           first_noted = min(first_noted, __float_as_int(of.x));
           last_noted = max(last_noted, __float_as_int(of.y));
         }
-        lo = 4 * first_noted;
+        lo = 4 * max(0, min(first_noted, last_noted));
         hi = min(hi, 4 * last_noted + 3);
       }
       for (int g = 0; g < mine; g += 32) {

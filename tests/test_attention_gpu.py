@@ -959,6 +959,30 @@ def test_infinities_and_nan_are_those_of_the_visible_values(form, heads, dim, dt
     assert (lse.double() - exact_lse)[seen].abs().sub(lse_slack[seen]).max() <= 0
 
 
+@pytest.mark.parametrize("queries,keys", [([24], [9000]), ([1], [9000]), ([5, 100], [7000, 3000]), ([40], [50000])])
+@pytest.mark.parametrize("heads,dim", [(2, 72), (8, 128), (4, 8)])
+@pytest.mark.parametrize("mask", ["documents", "window", "prefix"])
+def test_infinities_and_nan_over_split_keys(queries, keys, heads, dim, mask):
+    """Hidden and visible ones in the shares of several CTAs of a cluster, and past the steps whose documents are looked over ahead."""
+    how = {"window": (500, 3)} if mask == "window" else {}
+    if mask != "window":
+        k_documents = documents(keys, 700, 8) % (3 if mask == "documents" else 2)
+        at = torch.cat([sum(keys[:b]) + m - n + torch.arange(n, device="cuda") for b, (n, m) in enumerate(zip(queries, keys))])
+        how = dict(documents=k_documents[at].clone(), k_documents=k_documents)
+    s = problem(81, queries, keys, heads=heads, kv_heads=2, dim=dim, prefix=[1300] * len(queries) if mask == "prefix" else None, **how)
+    g = generator(82)
+    for value in (math.nan, math.inf, -math.inf):
+        s["v"][torch.rand(s["v"].shape, generator=g, device="cuda") < 0.25 / sum(keys)] = value
+    out, lse = run(s)
+    want = kinds(s)
+    assert same_kinds(out.double(), want)
+    clean = {**s, "v": torch.where(s["v"].isfinite(), s["v"], torch.zeros_like(s["v"]))}
+    exact, exact_lse, slack, lse_slack = define(clean)
+    fine = want == 0
+    assert (out.double() - exact)[fine].abs().sub(slack[fine]).max() <= 0
+    assert ((lse.double() - exact_lse).abs() <= lse_slack).all()
+
+
 @pytest.mark.parametrize("bad", ["a query", "an early key", "an early value", "a channel", "values here and there"])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_visible_nan_takes_no_longer(bad, dim):
