@@ -186,7 +186,7 @@ int laya_op_rotary(const laya_rotary* p, void* stream) {
     check_heads("out", h.out, h.out_token, h.out_head, p->dtype);
     check_apart("out", p->tokens, h.heads, p->head_dim, h.out_token, h.out_head);
     const bool in_place = h.x == h.out;
-    if (in_place && (h.x_token != h.out_token || h.x_head != h.out_head))
+    if (in_place && ((p->tokens > 1 && h.x_token != h.out_token) || (h.heads > 1 && h.x_head != h.out_head)))
       fail(LAYA_ERR_INVALID, "out is x, but with other strides");
     a.part[i] = {h.x, h.out, h.x_token, h.x_head, h.out_token, h.out_head, h.heads, !in_place};
     vectors = vectors && ((reinterpret_cast<uintptr_t>(h.x) | reinterpret_cast<uintptr_t>(h.out)) & 15) == 0 &&

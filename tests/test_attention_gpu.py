@@ -162,6 +162,20 @@ def test_rotary_backward_is_the_gradient(interleaved):
     assert abs(left - right) <= scale * 2.0 ** -19
 
 
+@pytest.mark.parametrize("tokens,heads,strides", [(1, 3, dict(x_token=64, out_token=4096)), (5, 1, dict(x_head=64, out_head=128)), (1, 1, dict(x_token=0, x_head=0, out_token=7, out_head=9))])
+def test_rotary_in_place_asks_nothing_of_a_single_dimensions_stride(tokens, heads, strides):
+    import ctypes as ct
+    from laya_cuda import _lib
+    x = randn(generator(6), tokens, heads, 64).float()
+    before, positions = x.clone(), torch.arange(3, 3 + tokens, device="cuda")
+    args = _lib.Rotary(tokens=tokens, head_dim=64, dims=64, dtype=0, positions=positions.data_ptr(), positions_64=1, theta=10000.0, factor=1.0, magnitude=1.0)
+    args.part[0] = _lib.Heads(**{**dict(x=x.data_ptr(), x_token=heads * 64, x_head=64, out=x.data_ptr(), out_token=heads * 64, out_head=64, heads=heads), **strides})
+    torch.cuda.synchronize()
+    _lib.check(_lib.load().laya_op_rotary(ct.byref(args), None))
+    torch.cuda.synchronize()
+    check_rotary(before, x, positions, "f32", 64)
+
+
 def test_rotary_of_many_tokens():
     g = generator(4)
     x, _ = heads(g, 70001, 2, 32, "bf16")
